@@ -279,6 +279,51 @@ int gdn_gated_rmsnorm_bwd(const void *y, const void *z, const float *w, const vo
                           float *dw, void *workspace, size_t workspace_bytes, int64_t rows, int D, float eps,
                           int dtype, int z_dtype, int dout_dtype, void *stream);
 
+/* ---------------------------------------------------------------------------------------------------------
+ * Operators of a language model around the mixer.  No counterpart in the reference's engine; error codes, streams and
+ * ownership as above, and nothing is allocated.
+ * --------------------------------------------------------------------------------------------------------- */
+
+/* Rotary positions on q [B][T][Hq][D] and k [B][T][Hk][D] (dtype; element strides given, channels contiguous): pair i of
+ * a head's first R channels turns by positions[b][t] * inv_freq[i] and is multiplied by factor, the rest is copied.
+ * Pairs are (i, i + R/2), or (2i, 2i + 1) when interleaved.  inv_freq [R/2] fp64; positions int64 or int32 (element
+ * strides given, 0 to share them over the batch); q_out, k_out contiguous, not overlapping the inputs.  backward turns by
+ * the negative angles: from the outputs' cotangents to the inputs' gradients.  Hq or Hk may be 0.  R even, at most 1024. */
+int gdn_rotary(const void *q, const void *k, void *q_out, void *k_out, const void *positions, const double *inv_freq,
+               int64_t q_stride_b, int64_t q_stride_t, int64_t q_stride_h, int64_t k_stride_b, int64_t k_stride_t,
+               int64_t k_stride_h, int64_t pos_stride_b, int64_t pos_stride_t, int B, int T, int Hq, int Hk, int D,
+               int R, int interleaved, int backward, int positions_64, float factor, int dtype, void *stream);
+
+/* Log probabilities of given tokens.  logits [outer][inner][V] (dtype; row strides in elements, a row contiguous),
+ * targets [outer * inner]:
+ *   logp [rows]      log softmax at the target; 0 where targets == ignore_index; NaN where the target is outside [0, V)
+ *   entropy [rows]   of the row's distribution (may be NULL)
+ *   stat [rows][2]   what gdn_logprobs_bwd needs (may be NULL)
+ *   top_ids, top_logp [rows][top]  the largest log probabilities, equal ones by index (NULL with top = 0; top <= 64)
+ * fp32 outputs.  Logits of -inf have probability 0; a row with nothing else has log probabilities -inf, entropy 0 and no
+ * gradient.  At most 2^24 pieces of 8192 logits over all rows, and top * ceil(V / 8192) <= 8192.
+ *
+ * gdn_logprobs_bwd: dlogits [rows][V] contiguous (dtype) from the cotangents dlogp and dentropy [rows] (either may be
+ * NULL; dentropy needs the forward's entropy). */
+size_t gdn_logprobs_workspace_bytes(int64_t rows, int64_t V, int top);
+int gdn_logprobs_fwd(const void *logits, const int64_t *targets, float *logp, float *entropy, float *stat,
+                     int64_t *top_ids, float *top_logp, void *workspace, size_t workspace_bytes, int64_t outer,
+                     int64_t inner, int64_t V, int64_t stride_outer, int64_t stride_inner, int64_t ignore_index,
+                     int top, int dtype, void *stream);
+int gdn_logprobs_bwd(const void *logits, const int64_t *targets, const float *stat, const float *entropy,
+                     const float *dlogp, const float *dentropy, void *dlogits, int64_t outer, int64_t inner, int64_t V,
+                     int64_t stride_outer, int64_t stride_inner, int64_t ignore_index, int dtype, void *stream);
+
+/* The norm over every element of `count` contiguous tensors x[i] (numel[i] elements of dtypes[i]) into norm [1] (device,
+ * fp32): the root of the sum of squares, summed in 64 bits, or with norm_inf the largest magnitude.  With y, also
+ * y[i] = x[i] * min(1, max_norm / (norm + eps)), y[i] of x[i]'s type and possibly x[i] itself; no other overlap is
+ * taken.  A NaN makes the norm NaN and every output with it.  The arrays x, y, numel and dtypes are host memory, read
+ * during the call.  Results are deterministic (no atomics). */
+size_t gdn_clip_grad_norm_workspace_bytes(const int64_t *numel, int count);
+int gdn_clip_grad_norm(const void *const *x, void *const *y, const int64_t *numel, const int *dtypes, int count,
+                       int norm_inf, double max_norm, double eps, float *norm, void *workspace, size_t workspace_bytes,
+                       void *stream);
+
 #ifdef __cplusplus
 }
 #endif

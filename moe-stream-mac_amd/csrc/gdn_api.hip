@@ -13,6 +13,7 @@
 #include <vector>
 
 #include "gdn_common.h"
+#include "gdn_host.h"
 #include "gdn_internal.h"
 #include "../../include/gdn_mi355x.h"
 
@@ -20,13 +21,15 @@ namespace gdn {
 
 static thread_local char g_err[512];
 
-static int fail(int code, const char *fmt, ...) {
+int fail(int code, const char *fmt, ...) {
     va_list ap;
     va_start(ap, fmt);
     vsnprintf(g_err, sizeof g_err, fmt, ap);
     va_end(ap);
     return code;
 }
+
+void clear_error() { g_err[0] = 0; }
 
 static bool debug_sync() {
     static const int on = [] {
@@ -37,7 +40,7 @@ static bool debug_sync() {
 }
 
 // After a launch: report launch errors, and in debug mode synchronise and report execution errors.
-static int check_launch(hipStream_t st, const char *what) {
+int check_launch(hipStream_t st, const char *what) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return fail(GDN_ERR_LAUNCH, "%s: launch failed: %s", what, hipGetErrorString(e));
     if (debug_sync()) {
@@ -57,25 +60,20 @@ static std::mutex g_prof_mu;
 static std::vector<ProfRec> g_prof;
 static std::atomic<bool> g_prof_on{false};  // read by every launch without the lock
 
-struct Timed {
-    const char *name;
-    hipStream_t st;
-    hipEvent_t start = nullptr, stop = nullptr;
-    Timed(const char *n, hipStream_t s) : name(n), st(s) {
-        if (!g_prof_on.load(std::memory_order_relaxed)) return;
-        if (hipEventCreate(&start) != hipSuccess || hipEventCreate(&stop) != hipSuccess) {
-            start = stop = nullptr;
-            return;
-        }
-        (void)hipEventRecord(start, st);
+Timed::Timed(const char *n, hipStream_t s) : name(n), st(s) {
+    if (!g_prof_on.load(std::memory_order_relaxed)) return;
+    if (hipEventCreate(&start) != hipSuccess || hipEventCreate(&stop) != hipSuccess) {
+        start = stop = nullptr;
+        return;
     }
-    ~Timed() {
-        if (!start) return;
-        (void)hipEventRecord(stop, st);
-        std::lock_guard<std::mutex> lk(g_prof_mu);
-        g_prof.push_back({name, start, stop});
-    }
-};
+    (void)hipEventRecord(start, st);
+}
+Timed::~Timed() {
+    if (!start) return;
+    (void)hipEventRecord(stop, st);
+    std::lock_guard<std::mutex> lk(g_prof_mu);
+    g_prof.push_back({name, start, stop});
+}
 
 __global__ void copy_or_zero_kernel(float *dst, const float *src, size_t n) {
     const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;

@@ -1,0 +1,31 @@
+// What the entry points of the C ABI share: the calling thread's error message, launch checks and launch timing.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace gdn {
+
+// Sets the message of gdn_last_error() and returns code; clear_error empties it.
+int fail(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3)));
+void clear_error();
+
+// After a launch: reports launch errors, and with GDN_DEBUG_SYNC=1 synchronises and reports execution errors.
+int check_launch(hipStream_t st, const char *what);
+
+// Brackets the launches of its scope with two events while gdn_profile_enable is on.
+struct Timed {
+    const char *name;
+    hipStream_t st;
+    hipEvent_t start = nullptr, stop = nullptr;
+    Timed(const char *n, hipStream_t s);
+    ~Timed();
+    Timed(const Timed &) = delete;
+    Timed &operator=(const Timed &) = delete;
+};
+
+inline size_t align_up256(size_t x) { return (x + 255) & ~(size_t)255; }
+inline bool aligned_to(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+}  // namespace gdn

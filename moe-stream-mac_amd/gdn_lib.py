@@ -7,6 +7,7 @@ There is no fallback: a missing library is an error.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import re
@@ -29,6 +30,7 @@ _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
 _f = ctypes.c_float
+_d = ctypes.c_double
 _sz = ctypes.c_size_t
 _SIGS = {
     "gdn_gates_fwd": ([_vp] * 6 + [_i64, _i, _i, _i, _i, _vp], _i),
@@ -46,6 +48,12 @@ _SIGS = {
     "gdn_gated_rmsnorm_bwd": ([_vp] * 8 + [_sz, _i64, _i, _f, _i, _i, _i, _vp], _i),
     "gdn_small_linears": ([_vp] * 4 + [_i] * 4 + [_vp], _i),
     "gdn_block_decode": ([_vp] * 13 + [_i] * 11 + [_f] * 3 + [_vp], _i),
+    "gdn_rotary": ([_vp] * 6 + [_i64] * 8 + [_i] * 9 + [_f, _i, _vp], _i),
+    "gdn_logprobs_workspace_bytes": ([_i64, _i64, _i], _sz),
+    "gdn_logprobs_fwd": ([_vp] * 8 + [_sz] + [_i64] * 6 + [_i, _i, _vp], _i),
+    "gdn_logprobs_bwd": ([_vp] * 7 + [_i64] * 6 + [_i, _vp], _i),
+    "gdn_clip_grad_norm_workspace_bytes": ([_vp, _i], _sz),
+    "gdn_clip_grad_norm": ([_vp] * 4 + [_i, _i, _d, _d, _vp, _vp, _sz, _vp], _i),
     "gdn_version": ([], _i),
     "gdn_last_error": ([], ctypes.c_char_p),
     "gdn_num_snapshots": ([_i, _i], ctypes.c_int64),
@@ -126,6 +134,11 @@ def profile_collect() -> dict[str, tuple[float, int]]:
         raw = names.raw[i * name_len:(i + 1) * name_len]
         out[raw.split(b"\0", 1)[0].decode()] = (ms[i], counts[i])
     return out
+
+
+def on_device(dev: torch.device):
+    """A context in which launches go to ``dev``: nothing where it is the current device already."""
+    return contextlib.nullcontext() if dev.index in (None, torch.cuda.current_device()) else torch.cuda.device(dev)
 
 
 def stream_handle(device: torch.device) -> int:

@@ -1,0 +1,103 @@
+"""The global norm of a model's gradients, and the gradients scaled by it: a few launches for any number of tensors, no
+synchronisation with the host.  Tensors must live on a ROCm device; there is no CPU path.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Iterable, Optional
+
+import torch
+
+import gdn_lib as L
+
+Array = torch.Tensor
+
+
+def _dense(t: Array) -> bool:
+    """Whether the tensor fills a block of memory in some order of its axes (a transposed weight does)."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for n, s in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda p: p[1]):
+        if s != want:
+            return False
+        want *= n
+    return True
+
+
+def _check(tensors, norm_type) -> None:
+    if norm_type not in (2.0, math.inf):
+        raise ValueError(f"norm_type must be 2 or inf; got {norm_type}")
+    dev = tensors[0].device
+    for t in tensors:
+        if t.dtype not in L.DTYPE_CODE or t.layout != torch.strided:
+            raise ValueError(f"unsupported tensor ({t.dtype}, {t.layout}); use dense float32, bfloat16 or float16")
+        if t.device != dev:
+            raise ValueError("all tensors must be on the same device")
+    if dev.type != "cuda":
+        raise RuntimeError("grad_clip runs on a ROCm GPU only; got tensors on " + str(dev))
+
+
+def _call(tensors, outs, max_norm, norm_type, eps) -> Array:
+    dev, code = tensors[0].device, L.DTYPE_CODE
+    n = len(tensors)
+    ptrs, sizes, ints = ctypes.c_void_p * n, ctypes.c_int64 * n, ctypes.c_int * n
+    numel = sizes(*[t.numel() for t in tensors])
+    lib = L.load()
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    nws = lib.gdn_clip_grad_norm_workspace_bytes(numel, n)
+    ws = torch.empty((nws,), dtype=torch.uint8, device=dev)
+    with L.on_device(dev):
+        L.check(lib.gdn_clip_grad_norm(ptrs(*[t.data_ptr() for t in tensors]),
+                                       None if outs is None else ptrs(*[t.data_ptr() for t in outs]), numel,
+                                       ints(*[code[t.dtype] for t in tensors]), n, int(norm_type == math.inf),
+                                       float(max_norm), float(eps), norm.data_ptr(), ws.data_ptr(), nws,
+                                       L.stream_handle(dev)))
+    return norm
+
+
+def grad_norm(tensors: Iterable[Array], norm_type: float = 2.0) -> Array:
+    """The norm over all elements of all tensors: 2 (squares summed in 64 bits) or inf; a float32 scalar on the device."""
+    ts = [t.detach() for t in tensors]
+    if not ts:
+        return torch.zeros(())
+    _check(ts, norm_type)
+    return _call([t if _dense(t) else t.contiguous() for t in ts], None, 0.0, float(norm_type), 0.0)
+
+
+def clip_grad_norm(grads: Iterable[Array], max_norm: float, norm_type: float = 2.0, *,
+                   out: Optional[Iterable[Array]] = None, eps: float = 1e-6) -> Array:
+    """Multiplies every tensor by min(1, max_norm / (norm + eps)) in place, or into the tensors of ``out`` (same shapes
+    and types), and returns the norm over all of them before that, as a float32 scalar on the device.  ``norm_type`` is 2
+    or inf.  A NaN in any tensor makes the norm and every result NaN; an infinite norm scales by 0.  Tensors may differ
+    in type and have any strides; none may share memory with another that is written.  Not differentiable."""
+    gs = [t.detach() for t in grads]
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm must be >= 0; got {max_norm}")
+    if not eps >= 0:
+        raise ValueError(f"eps must be >= 0; got {eps}")
+    if not gs:
+        return torch.zeros(())
+    _check(gs, norm_type)
+    os_ = gs if out is None else [t.detach() for t in out]
+    if out is not None:
+        if len(os_) != len(gs) or any(o.shape != g.shape or o.dtype != g.dtype or o.device != g.device
+                                      for o, g in zip(os_, gs)):
+            raise ValueError("out must hold one tensor of the same shape, type and device for each gradient")
+    # memory order does not matter to the kernels where input and output share it; others go through a copy
+    src, dst, back = [], [], []
+    for g, o in zip(gs, os_):
+        plain = g.is_contiguous() and (o is g or o.is_contiguous())
+        if plain or (_dense(g) and g.stride() == o.stride()):
+            src.append(g)
+            dst.append(o)
+        else:
+            src.append(g.contiguous())
+            dst.append(torch.empty_like(src[-1]))
+            back.append((o, dst[-1]))
+    norm = _call(src, dst, max_norm, float(norm_type), eps)
+    for o, tmp in back:
+        o.copy_(tmp)
+    return norm
