@@ -284,6 +284,35 @@ int gdn_gated_rmsnorm_bwd(const void *y, const void *z, const float *w, const vo
  * ownership as above, and nothing is allocated.
  * --------------------------------------------------------------------------------------------------------- */
 
+/* Linear attention with a log decay for each value head (value head h reads key head h / (Hv / Hk)):
+ *   S_t = e^{g_t} S_{t-1} + v_t k_t^T,   y_t = scale S_t q_t
+ * q, k [B][T][Hk][Dk] and v [B][T][Hv][Dv] of dtype, g [B][T][Hv] of g_dtype.  strides (host memory, read during the call)
+ * holds the element strides over batch, tokens and heads of q, k, v and g, 12 numbers; channels are contiguous.  One log
+ * decay per head: strides of 0 over batch and tokens.  A log decay of -inf keeps nothing of the state.  state0 [B][Hv][Dv][Dk]
+ * fp32, or NULL for zeros; y [B][T][Hv][Dv] contiguous, of dtype; state_T as state0 (may be NULL).  Dk, Dv <= 256,
+ * B * Hv <= 65535, T > 0.
+ *
+ * saved (gdn_linatt_saved_bytes, which may be 0) holds the states entering each segment of the sequence; gdn_linatt_bwd
+ * reads it.  From the cotangents dy (contiguous, of dtype) and dstate_T (fp32, or NULL for zeros; needs state_T) it writes dq,
+ * dk, dv (contiguous, of dtype), dg (of g_dtype: [B][T][Hv], or with g_per_head [Hv], summed over batch and tokens) and
+ * dstate0 (may be NULL).
+ *
+ * gdn_linatt_step: one token of B sequences; q, k [B][Hk][Dk], v, y [B][Hv][Dv] contiguous, g with element strides over
+ * batch and heads, state [B][Hv][Dv][Dk] fp32 updated in place. */
+size_t gdn_linatt_saved_bytes(int B, int T, int Hk, int Hv, int Dk, int Dv);
+size_t gdn_linatt_bwd_workspace_bytes(int B, int T, int Hk, int Hv, int Dk, int Dv);
+int gdn_linatt_fwd(const void *q, const void *k, const void *v, const void *g, const float *state0, void *y,
+                   float *state_T, void *saved, size_t saved_bytes, const int64_t *strides, int B, int T, int Hk, int Hv,
+                   int Dk, int Dv, float scale, int dtype, int g_dtype, void *stream);
+int gdn_linatt_bwd(const void *q, const void *k, const void *v, const void *g, const float *state0, const float *state_T,
+                   const void *saved, size_t saved_bytes, const void *dy, const float *dstate_T, void *dq, void *dk,
+                   void *dv, void *dg, float *dstate0, void *workspace, size_t workspace_bytes, const int64_t *strides,
+                   int B, int T, int Hk, int Hv, int Dk, int Dv, float scale, int g_per_head, int dtype, int g_dtype,
+                   void *stream);
+int gdn_linatt_step(const void *q, const void *k, const void *v, const void *g, float *state, void *y, int64_t g_stride_b,
+                    int64_t g_stride_h, int B, int Hk, int Hv, int Dk, int Dv, float scale, int dtype, int g_dtype,
+                    void *stream);
+
 /* Rotary positions on q [B][T][Hq][D] and k [B][T][Hk][D] (dtype; element strides given, channels contiguous): pair i of
  * a head's first R channels turns by positions[b][t] * inv_freq[i] and is multiplied by factor, the rest is copied.
  * Pairs are (i, i + R/2), or (2i, 2i + 1) when interleaved.  inv_freq [R/2] fp64; positions int64 or int32 (element

@@ -1,0 +1,404 @@
+// Linear attention: joining segments, heads and decays' gradients, the single token, and the C ABI.  The formulas and the
+// kernels that walk the chunks are in gdn_linatt.h.
+#include "gdn_linatt.h"
+
+#include "../../include/gdn_mi355x.h"
+
+namespace gdn {
+namespace la {
+
+constexpr int MAX_D = 256;
+
+// The segments' sums become the states entering them: from s0 (or nothing) on, in place.
+template <bool REV>
+__global__ __launch_bounds__(NT) void scan_kernel(float *s, const float *decay, const float *s0, int nseg, int64_t size) {
+    const int64_t head = blockIdx.y, i = (int64_t)blockIdx.x * NT + threadIdx.x;
+    if (i >= size) return;
+    float cur = s0 ? s0[head * size + i] : 0.f;
+    for (int j = 0; j < nseg; ++j) {
+        const int seg = REV ? nseg - 1 - j : j;
+        float *p = s + (head * nseg + seg) * size + i;
+        const float add = j < nseg - 1 ? *p : 0.f, f = j < nseg - 1 ? decay[head * nseg + seg] : 0.f;
+        *p = cur;
+        cur = fmaf(f, cur, add);
+    }
+}
+
+// The heads of a group added in order: part [rows][group][D] to o [rows][D].
+__global__ __launch_bounds__(NT) void group_kernel(const float *part, void *o, int64_t n, int group, int D, int dt) {
+    const int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x;
+    if (i >= n) return;
+    const int64_t row = i / D;
+    const float *p = part + row * group * D + i % D;
+    float s = p[0];
+    for (int j = 1; j < group; ++j) s += p[j * D];
+    store_from_f32(o, i, s, dt);
+}
+
+struct DecayGrad {
+    const float *a, *b, *cross;  // [slices][B][Hv][T]; cross: [cross_slices]
+    const float *decay;          // [B][Hv][nc]
+    const float *dlast, *last;   // [B][Hv][size], or dlast NULL
+    void *dg;                    // [B][T][Hv], or [Hv]
+    int B, T, Hv, slices, cross_slices, per_head, dt, nc;
+    int64_t size;
+};
+
+constexpr int DW = 16;  // waves
+
+__device__ __forceinline__ double block_sum(double x, double *red) {
+    x = readlane_f64(wave_prefix_sum(x), 63);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+    __syncthreads();
+    double r = 0.;
+    for (int i = 0; i < DW; ++i) r += red[i];
+    __syncthreads();
+    return r;
+}
+
+// dg of one value head, from the end of each sequence backwards, in 64 bits: a wave sums one chunk, the chunks chain.  grid
+// (Hv, B), or (Hv) per head.
+__global__ __launch_bounds__(64 * DW) void dg_kernel(const DecayGrad a) {
+    __shared__ double sumA[DW], sumB[DW], red[DW];
+    __shared__ int anew[DW];
+    const int h = blockIdx.x, l = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t heads = (int64_t)a.B * a.Hv;
+    double sum = 0.;
+    for (int b = a.per_head ? 0 : blockIdx.y; b < (a.per_head ? a.B : (int)blockIdx.y + 1); ++b) {
+        const int64_t head = (int64_t)b * a.Hv + h;
+        double D = 0.;
+        if (a.dlast) {
+            for (int64_t i = threadIdx.x; i < a.size; i += 64 * DW)
+                D = fma((double)a.dlast[head * a.size + i], (double)a.last[head * a.size + i], D);
+            D = block_sum(D, red);
+        }
+        for (int c1 = a.nc - 1; c1 >= 0; c1 -= DW) {
+            const int c = c1 - w;  // later chunks in lower waves, later tokens in lower lanes
+            const int64_t t = (int64_t)c * C + C - 1 - l;
+            const bool in = c >= 0 && t < a.T;
+            double xa = 0., xb = 0., x = 0.;
+            if (in) {
+                for (int s = 0; s < a.slices; ++s) {
+                    xa += (double)a.a[(s * heads + head) * a.T + t];
+                    xb += (double)a.b[(s * heads + head) * a.T + t];
+                }
+                for (int s = 0; s < a.cross_slices; ++s) x += (double)a.cross[(s * heads + head) * a.T + t];
+            }
+            xa = wave_prefix_sum(xa);
+            xb = wave_prefix_sum(xb);
+            const double B = readlane_f64(xb, 63);
+            if (l == 63) {
+                sumA[w] = xa;
+                sumB[w] = xb;
+                anew[w] = c >= 0 && a.decay[head * a.nc + c] < 0x1p-30f;
+            }
+            __syncthreads();
+            double mine = 0.;
+            for (int i = 0; i < DW; ++i) {
+                const double c0 = anew[i] ? 0. : D - sumB[i];
+                if (i == w) mine = c0;
+                D = c0 + sumA[i];
+            }
+            x += mine + xa + (B - xb);
+            if (in) {
+                if (a.per_head) sum += x;
+                else store_from_f32(a.dg, (b * (int64_t)a.T + t) * a.Hv + h, (float)x, a.dt);
+            }
+            __syncthreads();
+        }
+    }
+    if (a.per_head) {
+        sum = block_sum(sum, red);
+        if (threadIdx.x == 0) store_from_f32(a.dg, h, (float)sum, a.dt);
+    }
+}
+
+// One token: y = scale S' q, S' = e^g S + v k^T, in place.  L lanes share a row of the state, 4 channels each at a time.
+struct Step {
+    const void *q, *k, *v;
+    Gate g;
+    float *state;
+    void *y;
+    int Hk, Hv, Dk, Dv, dt, lanes;
+    float scale;
+};
+template <int V>
+__global__ __launch_bounds__(NT) void step_kernel(const Step a) {
+    const int lanes = a.lanes, lane = threadIdx.x & (lanes - 1), rows = NT / lanes;
+    const int row = blockIdx.x * rows + threadIdx.x / lanes, h = blockIdx.y, b = blockIdx.z;
+    const int64_t hv = (int64_t)b * a.Hv + h, hk = (int64_t)b * a.Hk + h / (a.Hv / a.Hk);
+    const float f = __builtin_amdgcn_exp2f(a.g.load(b, 0, h) * (float)LOG2E);
+    const bool in = row < a.Dv;
+    const float v = in ? load_as_f32(a.v, hv * a.Dv + row, a.dt) : 0.f;
+    float *s = a.state + (hv * a.Dv + (in ? row : 0)) * a.Dk;
+    float y = 0.f;
+    for (int c = lane * V; c < a.Dk; c += lanes * V) {
+        float x[V], q[V], k[V];
+        ops::loadv<V>(s, c, DT_F32, x);
+        ops::loadv<V>(a.q, hk * a.Dk + c, a.dt, q);
+        ops::loadv<V>(a.k, hk * a.Dk + c, a.dt, k);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            x[j] = fmaf(v, k[j], f * x[j]);
+            y = fmaf(x[j], q[j], y);
+        }
+        if (in) ops::storev<V>(s, c, DT_F32, x);
+    }
+    for (int m = 1; m < lanes; m <<= 1) y += __shfl_xor(y, m);
+    if (in && lane == 0) store_from_f32(a.y, hv * a.Dv + row, y * a.scale, a.dt);
+}
+
+// ---------------------------------------------------------------------------------------------------- host
+
+static int slices_of(int dk, int dv) { return (dv + cols_of(dk, dv) - 1) / cols_of(dk, dv); }
+
+struct Plan {
+    int nseg, cps, nc;  // segments, chunks of each, chunks of the sequence
+};
+// Segments: two workgroups for each compute unit, and at least four chunks of work for each.
+static Plan plan(int B, int T, int Hv, int Dk, int Dv) {
+    const int64_t wgs = (int64_t)B * Hv * slices_of(Dk, Dv), nc = ((int64_t)T + C - 1) / C;
+    int64_t want = (512 + wgs - 1) / wgs;
+    if (want > (nc + 3) / 4) want = (nc + 3) / 4;
+    if (want < 1) want = 1;
+    const int64_t cps = (nc + want - 1) / want;
+    return {(int)((nc + cps - 1) / cps), (int)cps, (int)nc};
+}
+
+static Ten ten(const void *p, const int64_t *st, int div, int D, int dt) {
+    const int e = dt == DT_F32 ? 4 : 2, m = 16 / e;  // 8 channels: one 16-byte load, or two
+    const bool v = D % 8 == 0 && aligned_to(p, 16) && st[0] % m == 0 && st[1] % m == 0 && st[2] % m == 0;
+    return {p, st[0], st[1], st[2], div, v};
+}
+
+static int run_pass(Pass a, Kind kind, hipStream_t st) {
+    static const char *const names[] = {"linatt_fwd", "linatt_dq", "linatt_dk", "linatt_dv"};
+    a.slices = slices_of(a.dk, a.dv);
+    a.o_vec = a.dv % 8 == 0 && aligned_to(a.o, 16);
+    {
+        Timed tm(names[kind], st);
+        (a.dk <= 64 ? pass_d64 : a.dk <= 128 ? pass_d128 : pass_d256)(a, kind, st);
+    }
+    return check_launch(st, names[kind]);
+}
+
+// The states entering each segment (nseg > 1), from s0 on (reverse: the cotangents, from the end).
+template <bool REV>
+static int run_segments(Seg a, const float *s0, hipStream_t st) {
+    a.slices = slices_of(a.dk, a.dv);
+    {
+        Timed tm(REV ? "linatt_segments_rev" : "linatt_segments", st);
+        (a.dk <= 64 ? seg_d64 : a.dk <= 128 ? seg_d128 : seg_d256)(a, REV, st);
+    }
+    const int rc = check_launch(st, "linear attention (segments)");
+    if (rc) return rc;
+    const int64_t size = (int64_t)a.dk * a.dv;
+    {
+        Timed tm("linatt_scan", st);
+        hipLaunchKernelGGL(scan_kernel<REV>, dim3((unsigned)((size + NT - 1) / NT), (unsigned)(a.B * a.Hv)), dim3(NT), 0, st,
+                           a.s, a.decay, s0, a.nseg, size);
+    }
+    return check_launch(st, "linear attention (scan)");
+}
+
+struct Sizes {
+    size_t state, decay, part, dot, cross, chunks, bwd;
+};
+static Sizes sizes(int B, int T, int Hk, int Hv, int Dk, int Dv) {
+    const Plan p = plan(B, T, Hv, Dk, Dv);
+    Sizes s{};
+    if (p.nseg > 1) {
+        s.state = align_up256((size_t)B * Hv * p.nseg * Dk * Dv * sizeof(float));
+        s.decay = align_up256((size_t)B * Hv * p.nseg * sizeof(float));
+    }
+    if (Hv > Hk) s.part = align_up256((size_t)B * T * Hv * Dk * sizeof(float));
+    const size_t rows = (size_t)B * Hv * T * sizeof(float);
+    s.dot = align_up256(rows * slices_of(Dv, Dk));
+    s.cross = align_up256(rows * slices_of(Dk, Dv));
+    s.chunks = align_up256((size_t)B * Hv * p.nc * sizeof(float));
+    s.bwd = s.state + s.decay + s.part + 2 * s.dot + s.cross + s.chunks;
+    return s;
+}
+
+static int check(int B, int T, int Hk, int Hv, int Dk, int Dv, int dtype, int g_dtype) {
+    if (B < 0 || T < 0) return fail(GDN_ERR_INVALID, "B and T must be >= 0");
+    if (Hk <= 0 || Hv <= 0 || Dk <= 0 || Dv <= 0) return fail(GDN_ERR_INVALID, "head counts and sizes must be positive");
+    if (Hv % Hk) return fail(GDN_ERR_INVALID, "the key heads (%d) must divide the value heads (%d)", Hk, Hv);
+    for (int d : {dtype, g_dtype})
+        if (d != GDN_F32 && d != GDN_BF16 && d != GDN_F16) return fail(GDN_ERR_INVALID, "unknown dtype code");
+    if (Dk > MAX_D || Dv > MAX_D) return fail(GDN_ERR_UNSUPPORTED, "heads of more than %d channels are not supported", MAX_D);
+    if ((int64_t)B * Hv > 65535 || Hv > 65535) return fail(GDN_ERR_UNSUPPORTED, "more than 65535 heads over the batch");
+    return 0;
+}
+
+}  // namespace la
+}  // namespace gdn
+
+using namespace gdn;
+
+extern "C" size_t gdn_linatt_saved_bytes(int B, int T, int Hk, int Hv, int Dk, int Dv) {
+    if (B <= 0 || T <= 0 || Hk <= 0 || Hv <= 0 || Dk <= 0 || Dv <= 0) return 0;
+    const la::Sizes s = la::sizes(B, T, Hk, Hv, Dk, Dv);
+    return s.state + s.decay;
+}
+extern "C" size_t gdn_linatt_bwd_workspace_bytes(int B, int T, int Hk, int Hv, int Dk, int Dv) {
+    if (B <= 0 || T <= 0 || Hk <= 0 || Hv <= 0 || Dk <= 0 || Dv <= 0) return 0;
+    return la::sizes(B, T, Hk, Hv, Dk, Dv).bwd;
+}
+
+extern "C" int gdn_linatt_fwd(const void *q, const void *k, const void *v, const void *g, const float *state0, void *y,
+                              float *state_T, void *saved, size_t saved_bytes, const int64_t *strides, int B, int T, int Hk,
+                              int Hv, int Dk, int Dv, float scale, int dtype, int g_dtype, void *stream) {
+    clear_error();
+    int rc = la::check(B, T, Hk, Hv, Dk, Dv, dtype, g_dtype);
+    if (rc) return rc;
+    if (B == 0) return GDN_OK;
+    if (T == 0) return fail(GDN_ERR_INVALID, "T must be positive");
+    if (!q || !k || !v || !g || !y || !strides) return fail(GDN_ERR_INVALID, "null pointer");
+    const la::Plan pl = la::plan(B, T, Hv, Dk, Dv);
+    const la::Sizes sz = la::sizes(B, T, Hk, Hv, Dk, Dv);
+    if (saved_bytes < sz.state + sz.decay || (sz.state && !saved))
+        return fail(GDN_ERR_WORKSPACE, "saved buffer of %zu bytes is smaller than the %zu bytes required", saved_bytes,
+                    sz.state + sz.decay);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int r = Hv / Hk;
+    const la::Gate gate{g, strides[9], strides[10], strides[11], g_dtype};
+    la::Pass p{};
+    p.Q = la::ten(q, strides, r, Dk, dtype);
+    p.K = la::ten(k, strides + 3, r, Dk, dtype);
+    p.V = la::ten(v, strides + 6, 1, Dv, dtype);
+    p.g = gate;
+    p.B = B; p.T = T; p.Hv = Hv; p.dk = Dk; p.dv = Dv; p.nseg = pl.nseg; p.cps = pl.cps; p.nc = pl.nc;
+    p.dt = p.o_dt = dtype;
+    p.scale = scale;
+    p.o = y;
+    p.s_in = state0;
+    p.s_head = (int64_t)Dk * Dv;
+    p.s_out = state_T;
+    if (pl.nseg > 1) {
+        float *s = static_cast<float *>(saved), *decay = reinterpret_cast<float *>(static_cast<char *>(saved) + sz.state);
+        const la::Seg a{p.K, p.V, gate, s, decay, B, T, Hv, Dk, Dv, 0, pl.nseg, pl.cps, pl.nc, dtype, scale};
+        rc = la::run_segments<false>(a, state0, st);
+        if (rc) return rc;
+        p.s_in = s;
+        p.s_seg = p.s_head;
+        p.s_head *= pl.nseg;
+    }
+    return la::run_pass(p, la::Y, st);
+}
+
+extern "C" int gdn_linatt_bwd(const void *q, const void *k, const void *v, const void *g, const float *state0,
+                              const float *state_T, const void *saved, size_t saved_bytes, const void *dy,
+                              const float *dstate_T, void *dq, void *dk, void *dv, void *dg, float *dstate0, void *workspace,
+                              size_t workspace_bytes, const int64_t *strides, int B, int T, int Hk, int Hv, int Dk, int Dv,
+                              float scale, int g_per_head, int dtype, int g_dtype, void *stream) {
+    clear_error();
+    int rc = la::check(B, T, Hk, Hv, Dk, Dv, dtype, g_dtype);
+    if (rc) return rc;
+    if (B == 0) return GDN_OK;
+    if (T == 0) return fail(GDN_ERR_INVALID, "T must be positive");
+    if (!q || !k || !v || !g || !dy || !dq || !dk || !dv || !dg || !strides || (dstate_T && !state_T))
+        return fail(GDN_ERR_INVALID, "null pointer");
+    const la::Plan pl = la::plan(B, T, Hv, Dk, Dv);
+    const la::Sizes sz = la::sizes(B, T, Hk, Hv, Dk, Dv);
+    if (sz.state && (!saved || saved_bytes < sz.state + sz.decay))
+        return fail(GDN_ERR_INVALID, "the saved buffer written by gdn_linatt_fwd (%zu bytes) is required", sz.state + sz.decay);
+    if (!workspace || workspace_bytes < sz.bwd)
+        return fail(GDN_ERR_WORKSPACE, "workspace of %zu bytes is smaller than the %zu bytes required", workspace_bytes, sz.bwd);
+    char *ws = static_cast<char *>(workspace);
+    const auto take = [&ws](size_t bytes) {
+        float *p = reinterpret_cast<float *>(ws);
+        ws += bytes;
+        return p;
+    };
+    float *ds = take(sz.state), *decay = take(sz.decay), *part = take(sz.part);
+    float *sa = take(sz.dot), *sb = take(sz.dot), *cross = take(sz.cross), *chunks = take(sz.chunks);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const int r = Hv / Hk;
+    const int64_t dys[3] = {(int64_t)T * Hv * Dv, (int64_t)Hv * Dv, Dv}, size = (int64_t)Dk * Dv;
+    const la::Ten tq = la::ten(q, strides, r, Dk, dtype), tk = la::ten(k, strides + 3, r, Dk, dtype);
+    const la::Ten tv = la::ten(v, strides + 6, 1, Dv, dtype), tdy = la::ten(dy, dys, 1, Dv, dtype);
+    const la::Gate gate{g, strides[9], strides[10], strides[11], g_dtype};
+    la::Pass p{};
+    p.g = gate;
+    p.B = B; p.T = T; p.Hv = Hv; p.nseg = pl.nseg; p.cps = pl.cps; p.nc = pl.nc;
+    p.dt = dtype;
+    p.scale = scale;
+    const int64_t n = (int64_t)B * T * Hk * Dk;
+    const auto grouped = [&](void *out, la::Kind kind) {
+        p.o = r > 1 ? part : out;
+        p.o_dt = r > 1 ? GDN_F32 : dtype;
+        const int e = la::run_pass(p, kind, st);
+        if (e || r == 1) return e;
+        {
+            Timed tm("linatt_group", st);
+            hipLaunchKernelGGL(la::group_kernel, dim3((unsigned)((n + la::NT - 1) / la::NT)), dim3(la::NT), 0, st, part, out, n,
+                               r, Dk, dtype);
+        }
+        return check_launch(st, "linear attention (groups)");
+    };
+    // dq = LA(dy, v, k): the forward's states, read as [k' = value channel][v' = key channel]
+    p.Q = tdy; p.K = tv; p.V = tk; p.X = tq;
+    p.dk = Dv; p.dv = Dk;
+    p.s_t = 1;
+    p.s_head = size * (pl.nseg > 1 ? pl.nseg : 1);
+    p.s_seg = size;
+    p.s_in = pl.nseg > 1 ? static_cast<const float *>(saved) : state0;
+    p.dot = sa;
+    rc = grouped(dq, la::DQ);
+    if (rc) return rc;
+    const float *s_in = dstate_T;
+    if (pl.nseg > 1) {
+        const la::Seg a{tq, tdy, gate, ds, decay, B, T, Hv, Dk, Dv, 0, pl.nseg, pl.cps, pl.nc, dtype, scale};
+        rc = la::run_segments<true>(a, dstate_T, st);
+        if (rc) return rc;
+        s_in = ds;
+    }
+    // dk = RLA(v, dy, q)
+    p.Q = tv; p.K = tdy; p.V = tq; p.X = tk;
+    p.s_in = s_in;
+    p.dot = sb;
+    p.decay = chunks;
+    rc = grouped(dk, la::DK);
+    if (rc) return rc;
+    // dv = RLA(k, q, dy)
+    p.Q = tk; p.K = tq; p.V = tdy; p.X = tv;
+    p.dk = Dk; p.dv = Dv;
+    p.s_t = 0;
+    p.dot = cross;
+    p.o = dv;
+    p.o_dt = dtype;
+    p.s_out = dstate0;
+    rc = la::run_pass(p, la::DV, st);
+    if (rc) return rc;
+    const la::DecayGrad d{sa, sb, cross, chunks, dstate_T, state_T, dg, B, T, Hv, la::slices_of(Dv, Dk), la::slices_of(Dk, Dv),
+                          g_per_head != 0, g_dtype, pl.nc, size};
+    {
+        Timed tm("linatt_dg", st);
+        hipLaunchKernelGGL(la::dg_kernel, dim3((unsigned)Hv, g_per_head ? 1u : (unsigned)B), dim3(64 * la::DW), 0,
+                           st, d);
+    }
+    return check_launch(st, "linear attention (dg)");
+}
+
+extern "C" int gdn_linatt_step(const void *q, const void *k, const void *v, const void *g, float *state, void *y, int64_t gs_b,
+                               int64_t gs_h, int B, int Hk, int Hv, int Dk, int Dv, float scale, int dtype, int g_dtype,
+                               void *stream) {
+    clear_error();
+    const int rc = la::check(B, 1, Hk, Hv, Dk, Dv, dtype, g_dtype);
+    if (rc) return rc;
+    if (B == 0) return GDN_OK;
+    if (!q || !k || !v || !g || !state || !y) return fail(GDN_ERR_INVALID, "null pointer");
+    const bool vec = Dk % 4 == 0 && aligned_to(q, 16) && aligned_to(k, 16) && aligned_to(state, 16);
+    la::Step a{q, k, v, {g, gs_b, 0, gs_h, g_dtype}, state, y, Hk, Hv, Dk, Dv, dtype, 1, scale};
+    while (a.lanes < 64 && a.lanes * (vec ? 4 : 1) < Dk) a.lanes *= 2;
+    const int rows = la::NT / a.lanes;
+    const dim3 grid((unsigned)((Dv + rows - 1) / rows), (unsigned)Hv, (unsigned)B);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    {
+        Timed tm("linatt_step", st);
+        if (vec) hipLaunchKernelGGL(la::step_kernel<4>, grid, dim3(la::NT), 0, st, a);
+        else hipLaunchKernelGGL(la::step_kernel<1>, grid, dim3(la::NT), 0, st, a);
+    }
+    return check_launch(st, "gdn_linatt_step");
+}

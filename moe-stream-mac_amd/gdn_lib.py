@@ -54,6 +54,11 @@ _SIGS = {
     "gdn_logprobs_bwd": ([_vp] * 7 + [_i64] * 6 + [_i, _vp], _i),
     "gdn_clip_grad_norm_workspace_bytes": ([_vp, _i], _sz),
     "gdn_clip_grad_norm": ([_vp] * 4 + [_i, _i, _d, _d, _vp, _vp, _sz, _vp], _i),
+    "gdn_linatt_saved_bytes": ([_i] * 6, _sz),
+    "gdn_linatt_bwd_workspace_bytes": ([_i] * 6, _sz),
+    "gdn_linatt_fwd": ([_vp] * 8 + [_sz, _vp] + [_i] * 6 + [_f, _i, _i, _vp], _i),
+    "gdn_linatt_bwd": ([_vp] * 7 + [_sz] + [_vp] * 8 + [_sz, _vp] + [_i] * 6 + [_f, _i, _i, _i, _vp], _i),
+    "gdn_linatt_step": ([_vp] * 6 + [_i64, _i64] + [_i] * 5 + [_f, _i, _i, _vp], _i),
     "gdn_version": ([], _i),
     "gdn_last_error": ([], ctypes.c_char_p),
     "gdn_num_snapshots": ([_i, _i], ctypes.c_int64),

@@ -119,3 +119,48 @@ def test_rotary_frequencies():
                 lambda: rotary_frequencies(8, factor=0.5), lambda: rotary_frequencies(8, base=-1.0)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_linear_attention_abi_refusals():
+    lib = L.load()
+    fake = ctypes.c_void_p(4096)  # never dereferenced: every call fails its checks first
+    strides = (ctypes.c_int64 * 12)(*[1] * 12)
+
+    def fwd(B=1, T=100, Hk=1, Hv=2, Dk=64, Dv=64, dt=0, gdt=0, p=fake, saved=1 << 40, st=strides):
+        return lib.gdn_linatt_fwd(p, p, p, p, p, p, p, p, saved, st, B, T, Hk, Hv, Dk, Dv, 1.0, dt, gdt, None)
+
+    for kw in (dict(B=-1), dict(T=-1), dict(T=0), dict(Hk=0), dict(Hv=0), dict(Dk=0), dict(Dv=0), dict(Hk=2, Hv=3),
+               dict(dt=3), dict(gdt=-1), dict(p=None), dict(st=None)):
+        assert fwd(**kw) == L.GDN_ERR_INVALID, kw
+    for kw in (dict(Dk=257), dict(Dv=300), dict(B=40000, Hv=2), dict(Hk=1, Hv=70000)):
+        assert fwd(**kw) == L.GDN_ERR_UNSUPPORTED, kw
+    assert fwd(B=0, p=None) == 0
+    n = lib.gdn_linatt_saved_bytes(1, 5000, 1, 2, 64, 64)
+    assert n > 0 and fwd(T=5000, saved=n - 1) == L.GDN_ERR_WORKSPACE
+    assert lib.gdn_linatt_saved_bytes(64, 60, 1, 32, 64, 64) == 0  # one segment: nothing to keep
+    assert lib.gdn_linatt_saved_bytes(0, 60, 1, 32, 64, 64) == 0
+
+    def bwd(T=100, last=fake, saved=fake, ns=1 << 40, ws=1 << 40, dq=fake):
+        return lib.gdn_linatt_bwd(fake, fake, fake, fake, fake, last, saved, ns, fake, fake, dq, fake, fake, fake, fake, fake,
+                                  ws, strides, 1, T, 1, 2, 64, 64, 1.0, 0, 0, 0, None)
+
+    assert bwd(last=None) == L.GDN_ERR_INVALID and bwd(dq=None) == L.GDN_ERR_INVALID and bwd(T=0) == L.GDN_ERR_INVALID
+    assert bwd(T=5000, saved=None) == L.GDN_ERR_INVALID and bwd(T=5000, ns=n - 1) == L.GDN_ERR_INVALID
+    assert bwd(ws=lib.gdn_linatt_bwd_workspace_bytes(1, 100, 1, 2, 64, 64) - 1) == L.GDN_ERR_WORKSPACE
+    step = lambda p, Dk: lib.gdn_linatt_step(p, p, p, p, p, p, 1, 1, 1, 1, 2, Dk, 64, 1.0, 0, 0, None)  # noqa: E731
+    assert step(None, 64) == L.GDN_ERR_INVALID and step(fake, 0) == L.GDN_ERR_INVALID
+    assert step(fake, 300) == L.GDN_ERR_UNSUPPORTED
+
+
+def test_linear_attention_wrappers_refuse():
+    from linear_attention import linear_attention, linear_attention_step
+    q, v, g, s = torch.zeros(2, 5, 1, 8), torch.zeros(2, 5, 3, 4), torch.zeros(2, 5, 3), torch.zeros(2, 3, 4, 8)
+    for f, a in ((linear_attention, (q, q, v, g, s)), (linear_attention_step, (q[:, 0], q[:, 0], v[:, 0], g[:, 0], s))):
+        with pytest.raises(RuntimeError, match="ROCm GPU"):
+            f(*a)
+        for i, bad in ((0, a[0][..., :7]), (1, a[1][:1]), (2, a[2][:1]), (3, a[3][..., :2]), (4, s[:, :2]), (0, a[0].half()),
+                       (2, a[2].double()), (3, a[3].int()), (0, a[0][..., 0]), (3, g[0])):
+            with pytest.raises(ValueError):
+                f(*a[:i], bad, *a[i + 1:])
+    with pytest.raises(ValueError, match="divide"):
+        linear_attention(torch.zeros(2, 5, 2, 8), torch.zeros(2, 5, 2, 8), v, g, s)
