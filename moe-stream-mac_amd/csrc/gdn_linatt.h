@@ -44,6 +44,12 @@ typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef short s8 __attribute__((ext_vector_type(8)));
 
+// x, unknown to the compiler from here on.
+__device__ __forceinline__ int opaque(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 // A 16 x 32 operand: lane l holds row l % 16 at the 8 indices 8 (l / 16) + j of the summed axis.
 struct F32Frag {
     float v[8];
@@ -77,16 +83,16 @@ __device__ __forceinline__ F32Frag row_frag(const float *p) {
 // The operand whose summed axis runs down the rows k0 .. k0 + 31 of a tile: lane 4 c + i of 16 holds column c0 + c cs + i.
 // bf16: the LDS's transposing read, where the four lanes 4 j .. 4 j + 3 of 16 give the addresses of row j's four quads of
 // columns and lane 4 c + i receives column i of quad c, rows 0 to 3.
-__device__ __forceinline__ bf8 col_frag(const bf16 *t, int ld, int k0, int c0, int cs) {
+__device__ __forceinline__ bf8 col_frag(const bf16 *t, int ld, int k0, int c0, int cs, int l) {
     typedef __attribute__((address_space(3))) s4 lds_s4;
-    const int l = threadIdx.x & 63, li = l & 15, g = l >> 4;
+    const int li = l & 15, g = l >> 4;
     const bf16 *p = t + (k0 + 8 * g + (li >> 2)) * ld + c0 + (li & 3) * cs;
     const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)p);
     const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p + 4 * ld));
     return __builtin_bit_cast(bf8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
-__device__ __forceinline__ F32Frag col_frag(const float *t, int ld, int k0, int c0, int cs) {
-    const int l = threadIdx.x & 63, li = l & 15, g = l >> 4;
+__device__ __forceinline__ F32Frag col_frag(const float *t, int ld, int k0, int c0, int cs, int l) {
+    const int li = l & 15, g = l >> 4;
     const float *p = t + (k0 + 8 * g) * ld + c0 + (li >> 2) * cs + (li & 3);
     F32Frag f;
 #pragma unroll
@@ -129,55 +135,154 @@ constexpr int pad() { return std::is_same_v<ET, float> ? 4 : 8; }  // 16 bytes: 
 struct Ten {
     const void *p;
     int64_t sb, st, sh;
-    int div, vec;  // vec: every 8-channel piece is 16-byte aligned and D % 8 == 0
-    __host__ __device__ int64_t at(int b, int64_t t, int h) const { return b * sb + t * st + (h / div) * sh; }
+    int div;
+    __device__ __forceinline__ int64_t at(int b, int64_t t, int h) const { return b * sb + t * st + (h / div) * sh; }
+    __device__ __forceinline__ const char *from(int b, int64_t t, int h, int c, int dt) const {
+        return static_cast<const char *>(p) + (at(b, t, h) + c) * (dt == DT_F32 ? 4 : 2);
+    }
 };
 
-// A [ROWS][W] tile in registers on its way from memory to LDS; rows >= n and columns >= w are zero.
-template <typename ET, int ROWS, int W>
+// 16 bytes from an address that is a multiple of the element's size only
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+struct __attribute__((packed, aligned(2))) u4_any {
+    u4 v;
+};
+
+// A [C][W] tile in registers on its way from memory to LDS, 8 channels to a piece; rows >= n and columns >= w are zero.  VEC:
+// w is a multiple of 8 (or none is left), pieces are loaded whole.  No load stands under a branch, where it would be waited
+// for: rows and columns out of range load ones in range, and turn to zeros on the way to LDS.
+template <typename ET, int W, bool VEC>
 struct Tile {
-    static constexpr int PER = ROWS * W / 8 / NT;
-    static_assert(PER * NT * 8 == ROWS * W, "a tile splits evenly");
-    std::conditional_t<std::is_same_v<ET, float>, float, uint32_t> x[PER][std::is_same_v<ET, float> ? 8 : 4];
-    __device__ __forceinline__ void fetch(const Ten &t, int64_t at, int n, int w, int dt) {
+    static constexpr bool F32 = std::is_same_v<ET, float>;
+    static constexpr int PER = C * W / 8 / NT, STEP = NT / (W / 8);
+    static_assert(PER * NT * 8 == C * W, "a tile splits evenly");
+    u4 x[PER][F32 ? 2 : 1];
+    // t0: the tile's first row and channel; dt: its type; st: elements between rows
+    __device__ __forceinline__ void fetch(const char *t0, int64_t st, int n, int w, int dt) {
+        const int tid = opaque(threadIdx.x), r0 = tid / (W / 8), c0 = (tid % (W / 8)) * 8;
+        const unsigned size = dt == DT_F32 ? 4 : 2, row = (unsigned)st * size;
+        if constexpr (VEC) {
+            const unsigned c = (c0 < w ? c0 : 0) * size;
 #pragma unroll
-        for (int p = 0; p < PER; ++p) {
-            const int v = threadIdx.x + p * NT, r = v / (W / 8), c = (v % (W / 8)) * 8;
-            const int64_t i = at + r * t.st + c;
+            for (int p = 0; p < PER; ++p) {
+                const char *s = t0 + ((unsigned)min(r0 + p * STEP, n - 1) * row + c);
+                x[p][0] = reinterpret_cast<const u4_any *>(s)->v;
+                if constexpr (F32) x[p][1] = reinterpret_cast<const u4_any *>(s + (dt == DT_F32 ? 16 : 0))->v;
+            }
+        } else {
 #pragma unroll
-            for (int j = 0; j < (int)(sizeof(x[p]) / 4); ++j) x[p][j] = 0;
-            if (r >= n || c >= w) continue;
-            if (t.vec) {
-                if constexpr (std::is_same_v<ET, float>) {
-                    ops::loadv<8>(t.p, i, dt, x[p]);
-                } else {
-                    const uint4 u = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(t.p) + i);
-                    x[p][0] = u.x; x[p][1] = u.y; x[p][2] = u.z; x[p][3] = u.w;
+            for (int p = 0; p < PER; ++p) {
+                const unsigned at = (unsigned)min(r0 + p * STEP, n - 1) * (unsigned)st;
+                u4 y[2] = {};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const unsigned i = at + (c0 + j < w ? c0 + j : 0);
+                    if (F32 && dt == DT_F32) {
+                        const uint32_t v = reinterpret_cast<const uint32_t *>(t0)[i];
+                        y[j / 4][j % 4] = c0 + j < w ? v : 0;
+                    } else {
+                        const uint32_t v = reinterpret_cast<const uint16_t *>(t0)[i];
+                        y[0][j / 2] |= (c0 + j < w ? v : 0) << (16 * (j & 1));
+                    }
                 }
-            } else if constexpr (std::is_same_v<ET, float>) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (c + j < w) x[p][j] = load_as_f32(t.p, i + j, dt);
-            } else {
-                const uint16_t *s = static_cast<const uint16_t *>(t.p) + i;
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (c + j < w) x[p][j / 2] |= (uint32_t)s[j] << (16 * (j & 1));
+                x[p][0] = y[0];
+                if constexpr (F32) x[p][1] = y[1];
             }
         }
     }
-    __device__ __forceinline__ void store(ET *dst) const {
+    __device__ __forceinline__ void store(ET *dst, int n, int w, int dt) const {
+        const int tid = opaque(threadIdx.x), r0 = tid / (W / 8), c0 = (tid % (W / 8)) * 8;
 #pragma unroll
         for (int p = 0; p < PER; ++p) {
-            const int v = threadIdx.x + p * NT, r = v / (W / 8), c = (v % (W / 8)) * 8;
-            ET *d = dst + r * (W + pad<ET>()) + c;
-            if constexpr (std::is_same_v<ET, float>) {
-                *reinterpret_cast<float4 *>(d) = make_float4(x[p][0], x[p][1], x[p][2], x[p][3]);
-                *reinterpret_cast<float4 *>(d + 4) = make_float4(x[p][4], x[p][5], x[p][6], x[p][7]);
+            const int r = r0 + p * STEP;
+            ET *d = dst + r * (W + pad<ET>()) + c0;
+            const bool in = r < n && c0 < w;
+            u4 a = x[p][0];
+            if constexpr (F32) {
+                u4 b = x[p][1];
+                if (dt != DT_F32) {
+                    const u4 h = a;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        a[j] = __float_as_uint(ops::half_bits_to_f32(h[j / 2] >> (16 * (j & 1))));
+                        b[j] = __float_as_uint(ops::half_bits_to_f32(h[2 + j / 2] >> (16 * (j & 1))));
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) b[j] = in ? b[j] : 0;
+                *reinterpret_cast<u4 *>(d + 4) = b;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) a[j] = in ? a[j] : 0;
+            *reinterpret_cast<u4 *>(d) = a;
+        }
+    }
+};
+
+// 4 or 8 channels from element i on, at any alignment, in 16 bits or (two pieces a 4) fp32.
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+struct __attribute__((packed, aligned(2))) u2_any {
+    u2 v;
+};
+template <int N, typename ET>
+__device__ __forceinline__ void store_row(void *p, int64_t i, int dt, const float (&o)[N]) {
+    if (dt == DT_F32) {
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            const u4 a = {__float_as_uint(o[j]), __float_as_uint(o[j + 1]), __float_as_uint(o[j + 2]), __float_as_uint(o[j + 3])};
+            reinterpret_cast<u4_any *>(static_cast<float *>(p) + i + j)->v = a;
+        }
+    } else {
+        uint32_t u[N / 2];
+#pragma unroll
+        for (int j = 0; j < N / 2; ++j) {
+            if constexpr (std::is_same_v<ET, bf16>)
+                u[j] = (uint32_t)f32_to_bf16_cvt(o[2 * j]) | ((uint32_t)f32_to_bf16_cvt(o[2 * j + 1]) << 16);
+            else u[j] = ops::pack2(o[2 * j], o[2 * j + 1], DT_F16);
+        }
+        uint16_t *d = static_cast<uint16_t *>(p) + i;
+        if constexpr (N == 8) reinterpret_cast<u4_any *>(d)->v = u4{u[0], u[1], u[2], u[3]};
+        else reinterpret_cast<u2_any *>(d)->v = u2{u[0], u[1]};
+    }
+}
+
+// N channels of a row on their way to a sum: raw bits, turned to fp32 where they are used.
+template <int N, typename ET, bool VEC>
+struct Piece {
+    static constexpr bool F32 = std::is_same_v<ET, float>;
+    uint32_t u[F32 ? N : N / 2];
+    // p: the tensor's type dt; elements from i on, w of them left
+    __device__ __forceinline__ void fetch(const char *p, unsigned i, int w, int dt) {
+        if constexpr (VEC) {
+            const char *q = p + (w > 0 ? i : 0) * (F32 && dt == DT_F32 ? 4 : 2);
+            if (N == 4 && !(F32 && dt == DT_F32)) {
+                const u2 a = reinterpret_cast<const u2_any *>(q)->v;
+                u[0] = a[0];
+                u[1] = a[1];
             } else {
-                *reinterpret_cast<uint4 *>(d) = make_uint4(x[p][0], x[p][1], x[p][2], x[p][3]);
+#pragma unroll
+                for (int j = 0; j < (int)(sizeof(u) / 16); ++j) {
+                    const u4 a = reinterpret_cast<const u4_any *>(q + (F32 && dt != DT_F32 ? 0 : 16 * j))->v;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) u[4 * j + k] = a[k];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+                const unsigned e = j < w ? i + j : 0;
+                uint32_t v;
+                if (F32 && dt == DT_F32) v = reinterpret_cast<const uint32_t *>(p)[e];
+                else v = reinterpret_cast<const uint16_t *>(p)[e];
+                if constexpr (F32) u[j] = v;
+                else u[j / 2] = j & 1 ? u[j / 2] | (v << 16) : v;
             }
         }
+    }
+    __device__ __forceinline__ float get(int j, int dt) const {
+        if constexpr (!F32) return __uint_as_float(j & 1 ? u[j / 2] & 0xffff0000u : u[j / 2] << 16);
+        else if (dt == DT_F32) return __uint_as_float(u[j]);
+        else return ops::half_bits_to_f32(VEC ? u[j / 2] >> (16 * (j & 1)) : u[j]);
     }
 };
 
@@ -186,10 +291,15 @@ struct Gate {
     int64_t sb, st, sh;
     int dt;
     // log decays below -1e4 (-inf: nothing is kept) run as -1e4, whose exponential is 0 and whose differences are finite
-    __device__ __forceinline__ float load(int b, int64_t t, int h) const {
-        const float g = load_as_f32(p, b * sb + t * st + h * sh, dt);
+    __device__ __forceinline__ uint32_t fetch(int b, int64_t t, int h) const {
+        const int64_t i = b * sb + t * st + h * sh;
+        return dt == DT_F32 ? static_cast<const uint32_t *>(p)[i] : (uint32_t) static_cast<const uint16_t *>(p)[i];
+    }
+    __device__ __forceinline__ float value(uint32_t u) const {
+        const float g = dt == DT_F32 ? __uint_as_float(u) : dt == DT_BF16 ? __uint_as_float(u << 16) : ops::half_bits_to_f32(u);
         return g < -1e4f ? -1e4f : g;
     }
+    __device__ __forceinline__ float load(int b, int64_t t, int h) const { return value(fetch(b, t, h)); }
 };
 
 // Of one chunk: G (in powers of two), and the weights of its outputs and sources, e^{G_r} and e^{G_C - G_s} (reverse: the
@@ -225,7 +335,7 @@ struct Pass {
     float *dot;         // per token [slices][B][Hv][T]: DQ, DK X . (O from the state); DV the pairs that cross it, X = v
     float *decay;       // DK: of each chunk, [B][Hv][nc]
     int B, T, Hv, dk, dv, slices, nseg, cps, nc;  // cps: chunks of a segment, nc: of the sequence
-    int dt, o_dt, o_vec;
+    int dt, o_dt;
     float scale;
 };
 
@@ -240,8 +350,9 @@ struct Shared {
     ET Q[C * (D + pad<ET>())], K[C * (D + pad<ET>())], V[C * LV];
     ET own_p[TAKEN ? 8 : C * LP], own_x[KIND == DV && !TAKEN ? C * LV : 8];
     Decays d;
-    float dot[4][C];
-    double cross[KIND == DV ? 4 : 1][C];
+    float dot[KIND == DQ || KIND == DK ? 4 : 1][KIND == DQ || KIND == DK ? C : 1];
+    // where Q' was, once it is used: the waves' sums of M, [4][C]
+    __device__ __forceinline__ double *cross() { return reinterpret_cast<double *>(Q + (TAKEN ? C * LP + C * LV : 0)); }
     __device__ __forceinline__ ET *p() { return TAKEN ? Q : own_p; }
     __device__ __forceinline__ ET *x() { return TAKEN ? Q + C * LP : own_x; }
 };
@@ -256,35 +367,45 @@ struct State {
         const int l = threadIdx.x & 63, li = l & 15, w = threadIdx.x >> 6;
         return 16 * NV * w + 4 * NV * (li >> 2) + 4 * n + (li & 3);
     }
-    template <typename F>
-    __device__ __forceinline__ void each(int dk, int dv, int c0, F f) {
+    // p: [v'][k'], or with tr [k'][v']; out of range (and without p) zeros
+    __device__ __forceinline__ void load(const float *p, int dk, int dv, int c0, int tr) {
         const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
-        for (int t = 0; t < D / 16; ++t)
+        for (int T = 0; T < D / 32; ++T)
 #pragma unroll
-            for (int n = 0; n < NV; ++n)
+            for (int n = 0; n < NV; ++n) {
+                const int k = 32 * T + 8 * g, v = c0 + col(n), vv = min(v, dv - 1);
+                float x[8] = {};
+                if (p) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int k = 32 * (t >> 1) + 8 * g + 4 * (t & 1) + e, v = c0 + col(n);
-                    f(s[t][n], e, k, v, k < dk && v < dv);
+                    for (int e = 0; e < 8; ++e) {
+                        const int kk = min(k + e, dk - 1);
+                        x[e] = p[tr ? kk * dv + vv : vv * dk + kk];
+                    }
                 }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s[2 * T + e / 4][n][e % 4] = k + e < dk && v < dv ? x[e] : 0.f;
+            }
     }
-    __device__ __forceinline__ void load(const float *p, int dk, int dv, int c0, int tr) {
-        each(dk, dv, c0, [&](f4 &x, int e, int k, int v, bool in) {
-            x[e] = p && in ? p[tr ? (int64_t)k * dv + v : (int64_t)v * dk + k] : 0.f;
-        });
-    }
-    __device__ __forceinline__ void store(float *p, int dk, int dv, int c0, int tr) {
-        each(dk, dv, c0, [&](f4 &x, int e, int k, int v, bool in) {
-            if (in) p[tr ? (int64_t)k * dv + v : (int64_t)v * dk + k] = x[e];
-        });
+    __device__ __forceinline__ void store(float *p, int dk, int dv, int c0, int tr) const {
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int T = 0; T < D / 32; ++T)
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                const int k = 32 * T + 8 * g, v = c0 + col(n);
+                if (v >= dv) continue;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (k + e < dk) p[tr ? (k + e) * dv + v : v * dk + k + e] = s[2 * T + e / 4][n][e % 4];
+            }
     }
     // s = total s + sum over 32 rows of the tiles: K'^T diag(weights) V', the weighted V' in NS terms
     template <int NS, typename ET>
-    __device__ __forceinline__ void add(const ET *sK, int k0, const Frag<ET> (&vw)[NV][NS]) {
+    __device__ __forceinline__ void add(const ET *sK, int k0, const Frag<ET> (&vw)[NV][NS], int l) {
 #pragma unroll
         for (int t = 0; t < D / 16; ++t) {
-            const Frag<ET> a = col_frag(sK, D + pad<ET>(), k0, 32 * (t >> 1) + 4 * (t & 1), 8);
+            const Frag<ET> a = col_frag(sK, D + pad<ET>(), k0, 32 * (t >> 1) + 4 * (t & 1), 8, l);
 #pragma unroll
             for (int i = 0; i < NS; ++i)
 #pragma unroll
@@ -302,15 +423,30 @@ __device__ __forceinline__ void weigh(const Frag<ET> &v, const float *w, Frag<ET
     split(x, o);
 }
 
+// The e-th of the ten 16 x 16 blocks of P that hold pairs: its first output and source.
+struct Block {
+    int r0, s0;
+    bool in;
+};
+template <bool REV>
+__device__ __forceinline__ Block block(int e) {
+    const int i = (e >= 1) + (e >= 3) + (e >= 6), j = e - i * (i + 1) / 2;
+    return REV ? Block{16 * j, 16 * i, e < 10} : Block{16 * i, 16 * j, e < 10};
+}
+
+// Waves to a SIMD: two where a wave's state, tiles and sums fit 256 registers.
+template <typename ET, int D>
+constexpr int waves() { return std::is_same_v<ET, bf16> && D <= 128 ? 2 : 1; }
+
 // One segment of one value head, 64 NV columns of V'.
-template <typename ET, int D, int NV, int KIND>
-__global__ __launch_bounds__(NT) void pass_kernel(const Pass a) {
+template <typename ET, int D, int NV, int KIND, bool VEC>
+__global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a) {
     constexpr bool F32 = std::is_same_v<ET, float>, REV = KIND >= DK, DOT = KIND == DQ || KIND == DK;
     constexpr int NS = F32 ? 1 : 3, NH = F32 || !DOT ? 1 : 2;  // terms of the weighted V', of the state as an operand
     constexpr int LK = D + pad<ET>(), LV = 64 * NV + pad<ET>(), LP = C + pad<ET>(), RT = C / 16;
     constexpr bool TAKEN = Shared<ET, D, NV, KIND>::TAKEN;
     __shared__ __attribute__((aligned(16))) Shared<ET, D, NV, KIND> sh;
-    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, li = l & 15, g = l >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int id = blockIdx.x;
     const int slice = id % a.slices;
     id /= a.slices;
@@ -323,34 +459,50 @@ __global__ __launch_bounds__(NT) void pass_kernel(const Pass a) {
     State<D, NV> S;
     S.load(a.s_in ? a.s_in + head * a.s_head + seg * a.s_seg : nullptr, a.dk, a.dv, c0, a.s_t);
 
-    Tile<ET, C, D> tq, tk;
-    Tile<ET, C, 64 * NV> tv, tx;
-    float tg = 0.f;
+    Tile<ET, D, VEC> tq, tk;
+    Tile<ET, 64 * NV, VEC> tv, tx;
+    uint32_t tg = 0;
     const auto fetch = [&](int c) {
         const int64_t t0 = (int64_t)c * C;
+        const int l = threadIdx.x & 63;
         const int n = min((int64_t)C, a.T - t0);
-        tq.fetch(a.Q, a.Q.at(b, t0, h), n, a.dk, a.dt);
-        tk.fetch(a.K, a.K.at(b, t0, h), n, a.dk, a.dt);
-        tv.fetch(a.V, a.V.at(b, t0, h) + c0, n, a.dv - c0, a.dt);
-        if constexpr (KIND == DV && !TAKEN) tx.fetch(a.X, a.X.at(b, t0, h) + c0, n, a.dv - c0, a.dt);
-        if (w == 0) tg = l < n ? a.g.load(b, t0 + l, h) : 0.f;
+        tq.fetch(a.Q.from(b, t0, h, 0, a.dt), a.Q.st, n, a.dk, a.dt);
+        tk.fetch(a.K.from(b, t0, h, 0, a.dt), a.K.st, n, a.dk, a.dt);
+        tv.fetch(a.V.from(b, t0, h, c0, a.dt), a.V.st, n, a.dv - c0, a.dt);
+        if constexpr (KIND == DV && !TAKEN) tx.fetch(a.X.from(b, t0, h, c0, a.dt), a.X.st, n, a.dv - c0, a.dt);
+        tg = a.g.fetch(b, t0 + min(l, n - 1), h);
     };
+    Piece<4 * NV, ET, VEC> px[RT];
+    const auto fetch_x = [&](int c) {
+        const int64_t t0 = (int64_t)c * C;
+        const int n = min((int64_t)C, a.T - t0);
+        const char *x0 = a.X.from(b, t0, h, 0, a.dt);
+        const int l = opaque(threadIdx.x & 63), li = l & 15, col = c0 + 16 * NV * w + 4 * NV * (l >> 4);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+            px[rt].fetch(x0, (unsigned)min(16 * rt + li, n - 1) * (unsigned)a.X.st + col, a.dv - col, a.dt);
+    };
+    if constexpr (DOT) fetch_x(REV ? last : first);
     for (int i = first - 1; i <= last; ++i) {
+        const int c = REV ? first + last - i : i;
+        const int64_t t0 = (int64_t)c * C;
+        const int n = min((int64_t)C, a.T - t0);
+        // opaque: addresses in LDS are formed where they are used, not hoisted out of the loop and spilled
+        const int tid = opaque(threadIdx.x), l = tid & 63, li = l & 15, g = l >> 4;
+        const int col = c0 + 16 * NV * w + 4 * NV * g;  // the lane's first column of O
         if (i >= first) {
             __syncthreads();
-            tq.store(sh.Q);
-            tk.store(sh.K);
-            tv.store(sh.V);
-            if constexpr (KIND == DV && !TAKEN) tx.store(sh.x());
-            if (w == 0) sh.d.template set<REV>(tg, a.scale);
+            tq.store(sh.Q, n, a.dk, a.dt);
+            tk.store(sh.K, n, a.dk, a.dt);
+            tv.store(sh.V, n, a.dv - c0, a.dt);
+            if constexpr (KIND == DV && !TAKEN) tx.store(sh.x(), n, a.dv - c0, a.dt);
+            if (w == 0) sh.d.template set<REV>(l < n ? a.g.value(tg) : 0.f, a.scale);
             __syncthreads();
         }
         if (i < last) fetch(REV ? first + last - i - 1 : i + 1);
         if (i < first) continue;
-        const int c = REV ? first + last - i : i;
-        const int64_t t0 = (int64_t)c * C;
-        const int n = min((int64_t)C, a.T - t0);
 
+        __builtin_amdgcn_sched_barrier(0);
         // O = diag(wo) S Q'^T, later + P V', transposed: a lane holds one token, 4 NV consecutive columns
         f4 O[RT][NV];
 #pragma unroll
@@ -385,7 +537,6 @@ __global__ __launch_bounds__(NT) void pass_kernel(const Pass a) {
 #pragma unroll
             for (int x = 0; x < NV; ++x) O[rt][x] *= wo;
         }
-        const int col = c0 + 16 * NV * w + 4 * NV * g;  // the lane's first column of O
         const auto row_of = [&](int rt, float (&o)[4 * NV]) {
 #pragma unroll
             for (int x = 0; x < NV; ++x)
@@ -398,107 +549,93 @@ __global__ __launch_bounds__(NT) void pass_kernel(const Pass a) {
                 const int r = 16 * rt + li;
                 float o[4 * NV], s = 0.f;
                 row_of(rt, o);
-                if (r < n) {
-                    const int64_t at = a.X.at(b, t0 + r, h) + col;
-                    if (a.X.vec && col + 4 * NV <= a.dv) {
-                        float x[4 * NV];
-                        ops::loadv<4 * NV>(a.X.p, at, a.dt, x);
 #pragma unroll
-                        for (int j = 0; j < 4 * NV; ++j) s = fmaf(x[j], o[j], s);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4 * NV; ++j)
-                            if (col + j < a.dv) s = fmaf(load_as_f32(a.X.p, at + j, a.dt), o[j], s);
-                    }
-                }
+                for (int j = 0; j < 4 * NV; ++j) s = fmaf(col + j < a.dv ? px[rt].get(j, a.dt) : 0.f, o[j], s);
+                s = r < n ? s : 0.f;
                 s += lane_xor16(s);
                 s += lane_xor32(s);
                 if (g == 0) sh.dot[w][r] = s;
             }
+            if (i < last) fetch_x(REV ? c - 1 : c + 1);
         }
 
+        __builtin_amdgcn_sched_barrier(0);
         // P: blocks (rt, st) of 16 outputs by 16 sources with st <= rt (reverse: >=), one to a wave in turn; the blocks that
         // fill a product's 32 sources are zeros
-        {
-            ET *const sP = sh.p();
-            f4 acc[3];
-            int e = 0;
+        ET *const sP = sh.p();
+        f4 acc[3];
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
+        for (int e = 0; e < 3; ++e) {
+            const Block k = block<REV>(w + 4 * e);
+            if (!k.in) continue;
+            acc[e] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int st = REV ? rt : 0; st < (REV ? RT : rt + 1); ++st, ++e) {
-                    if ((e & 3) != w) continue;
-                    f4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int k = 0; k < D; k += 32)
-                        x = mma(row_frag(sh.K + (16 * st + li) * LK + k + 8 * g),
-                                row_frag(sh.Q + (16 * rt + li) * LK + k + 8 * g), x);
-                    acc[e >> 2] = x;
-                }
-            if constexpr (TAKEN) __syncthreads();
-            if constexpr (KIND == DV && TAKEN) {
-                tx.fetch(a.X, a.X.at(b, t0, h) + c0, n, a.dv - c0, a.dt);
-                tx.store(sh.x());
-            }
-            const auto put = [&](int rt, int st, const ET (&p)[4]) {
-                ET *o = sP + (16 * rt + li) * LP + 16 * st + 4 * g;
-                if constexpr (F32) *reinterpret_cast<float4 *>(o) = make_float4(p[0], p[1], p[2], p[3]);
-                else *reinterpret_cast<uint2 *>(o) = *reinterpret_cast<const uint2 *>(p);
-            };
-            e = 0;
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-                for (int st = REV ? rt : 0; st < (REV ? RT : rt + 1); ++st, ++e) {
-                    if ((e & 3) != w) continue;
-                    const int r = 16 * rt + li, s0 = 16 * st + 4 * g;
-                    const double gr = sh.d.G[r];
-                    ET p[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float d = (float)(REV ? sh.d.G[s0 + j] - gr : gr - sh.d.G[s0 + j]);
-                        const bool in = REV ? s0 + j >= r : s0 + j <= r;
-                        acc[e >> 2][j] = in ? acc[e >> 2][j] * (a.scale * __builtin_amdgcn_exp2f(d)) : 0.f;
-                        p[j] = (ET)acc[e >> 2][j];
-                    }
-                    put(rt, st, p);
-                }
-                const ET zero[4] = {(ET)0.f, (ET)0.f, (ET)0.f, (ET)0.f};
-                if (w == rt && (rt & 1) == (REV ? 1 : 0)) put(rt, rt ^ 1, zero);
-            }
+            for (int x = 0; x < D; x += 32)
+                acc[e] = mma(row_frag(sh.K + (k.s0 + li) * LK + x + 8 * g), row_frag(sh.Q + (k.r0 + li) * LK + x + 8 * g), acc[e]);
+        }
+        if constexpr (TAKEN) {
             __syncthreads();
-            // M of the same blocks, its sums over outputs and sources apart in 64 bits: their difference from a token on is
-            // the sum of the pairs that cross it
             if constexpr (KIND == DV) {
-                double *cross = sh.cross[w];
-                cross[l] = 0.;
-                e = 0;
+                tx.fetch(a.X.from(b, t0, h, c0, a.dt), a.X.st, n, a.dv - c0, a.dt);
+                tx.store(sh.x(), n, a.dv - c0, a.dt);
+            }
+        }
+        const auto put = [&](int r, int s, const ET (&p)[4]) {
+            ET *o = sP + r * LP + s;
+            if constexpr (F32) *reinterpret_cast<float4 *>(o) = make_float4(p[0], p[1], p[2], p[3]);
+            else *reinterpret_cast<uint2 *>(o) = *reinterpret_cast<const uint2 *>(p);
+        };
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
+        for (int e = 0; e < 3; ++e) {
+            const Block k = block<REV>(w + 4 * e);
+            if (!k.in) continue;
+            const int r = k.r0 + li, s0 = k.s0 + 4 * g;
+            const double gr = sh.d.G[r];
+            double gs[4];
 #pragma unroll
-                    for (int st = rt; st < RT; ++st, ++e) {
-                        if ((e & 3) != w) continue;
-                        f4 x = {0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < 4; ++j) gs[j] = sh.d.G[s0 + j];
+            ET p[4];
 #pragma unroll
-                        for (int k = 0; k < 64 * NV; k += 32)
-                            x = mma(row_frag(sh.V + (16 * st + li) * LV + k + 8 * g),
-                                    row_frag(sh.x() + (16 * rt + li) * LV + k + 8 * g), x);
-                        double out = 0.;
+            for (int j = 0; j < 4; ++j) {
+                const float x = acc[e][j] * (a.scale * __builtin_amdgcn_exp2f((float)(REV ? gs[j] - gr : gr - gs[j])));
+                acc[e][j] = (REV ? s0 + j >= r : s0 + j <= r) ? x : 0.f;
+                p[j] = (ET)acc[e][j];
+            }
+            put(r, s0, p);
+        }
+        if (w < 2) {
+            const ET zero[4] = {(ET)0.f, (ET)0.f, (ET)0.f, (ET)0.f};
+            put(32 * w + (REV ? 16 : 0) + li, 32 * w + (REV ? 0 : 16) + 4 * g, zero);
+        }
+        __syncthreads();
+        // M of the same blocks, its sums over outputs and sources apart in 64 bits: their difference from a token on is the sum
+        // of the pairs that cross it
+        if constexpr (KIND == DV) {
+            double *cross = sh.cross() + w * C;
+            cross[l] = 0.;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int s = 16 * st + 4 * g + j;
-                            double m = s > 16 * rt + li ? (double)x[j] * (double)acc[e >> 2][j] : 0.;
-                            out += m;
-                            m += dpp_mov_f64<DPP_QUAD_1032>(m);
-                            m += dpp_mov_f64<DPP_QUAD_2301>(m);
-                            m += dpp_mov_f64<DPP_ROW_HALF_MIRROR>(m);
-                            m += dpp_mov_f64<DPP_ROW_MIRROR>(m);
-                            if (li == 0) cross[s] += m;
-                        }
-                        out += __shfl_xor(out, 16);
-                        out += __shfl_xor(out, 32);
-                        if (g == 0) cross[16 * rt + li] -= out;
-                    }
+            for (int e = 0; e < 3; ++e) {
+                const Block k = block<REV>(w + 4 * e);
+                if (!k.in) continue;
+                f4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < 64 * NV; i += 32)
+                    x = mma(row_frag(sh.V + (k.s0 + li) * LV + i + 8 * g), row_frag(sh.x() + (k.r0 + li) * LV + i + 8 * g), x);
+                double out = 0.;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int s = k.s0 + 4 * g + j;
+                    double m = s > k.r0 + li ? (double)x[j] * (double)acc[e][j] : 0.;
+                    out += m;
+                    m += dpp_mov_f64<DPP_QUAD_1032>(m);
+                    m += dpp_mov_f64<DPP_QUAD_2301>(m);
+                    m += dpp_mov_f64<DPP_ROW_HALF_MIRROR>(m);
+                    m += dpp_mov_f64<DPP_ROW_MIRROR>(m);
+                    if (li == 0) cross[s] += m;
+                }
+                out += __shfl_xor(out, 16);
+                out += __shfl_xor(out, 32);
+                if (g == 0) cross[k.r0 + li] -= out;
             }
         }
         const float total = sh.d.total;
@@ -511,7 +648,7 @@ __global__ __launch_bounds__(NT) void pass_kernel(const Pass a) {
             Frag<ET> v[NV], vw[NV][NS];
 #pragma unroll
             for (int x = 0; x < NV; ++x) {
-                v[x] = col_frag(sh.V, LV, k0, 16 * NV * w + 4 * x, 4 * NV);
+                v[x] = col_frag(sh.V, LV, k0, 16 * NV * w + 4 * x, 4 * NV, l);
                 weigh<ET>(v[x], sh.d.ws + k0 + 8 * g, vw[x]);
             }
 #pragma unroll
@@ -521,7 +658,9 @@ __global__ __launch_bounds__(NT) void pass_kernel(const Pass a) {
 #pragma unroll
                 for (int x = 0; x < NV; ++x) O[rt][x] = mma(v[x], p, O[rt][x]);
             }
-            S.template add<NS, ET>(sh.K, k0, vw);
+            __builtin_amdgcn_sched_barrier(0);
+            S.template add<NS, ET>(sh.K, k0, vw, l);
+            __builtin_amdgcn_sched_barrier(0);
         }
 
 #pragma unroll
@@ -531,8 +670,8 @@ __global__ __launch_bounds__(NT) void pass_kernel(const Pass a) {
             row_of(rt, o);
             if (r < n) {
                 const int64_t at = ((b * (int64_t)a.T + t0 + r) * a.Hv + h) * a.dv + col;
-                if (a.o_vec && col + 4 * NV <= a.dv) {
-                    ops::storev<4 * NV>(a.o, at, a.o_dt, o);
+                if constexpr (VEC) {
+                    if (col < a.dv) store_row<4 * NV, ET>(a.o, at, a.o_dt, o);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4 * NV; ++j)
@@ -550,7 +689,8 @@ __global__ __launch_bounds__(NT) void pass_kernel(const Pass a) {
             __syncthreads();
             if (w == 0) {
                 const int t = C - 1 - l;
-                const double x = (sh.cross[0][t] + sh.cross[1][t]) + (sh.cross[2][t] + sh.cross[3][t]);
+                const double *const x0 = sh.cross() + t;
+                const double x = (x0[0] + x0[C]) + (x0[2 * C] + x0[3 * C]);
                 const double s = wave_prefix_sum(x);
                 if (t < n) a.dot[at + t] = (float)s;
             }
@@ -570,8 +710,8 @@ struct Seg {
 
 // What a segment adds to a state that starts from nothing, and its decay.  The segment that the chain ends with is left out
 // (the last; reverse: the first).
-template <typename ET, int D, int NV, bool REV>
-__global__ __launch_bounds__(NT) void seg_kernel(const Seg a) {
+template <typename ET, int D, int NV, bool REV, bool VEC>
+__global__ __launch_bounds__(NT, (waves<ET, D>())) void seg_kernel(const Seg a) {
     constexpr int NS = std::is_same_v<ET, float> ? 1 : 3, LV = 64 * NV + pad<ET>();
     __shared__ __attribute__((aligned(16))) ET sK[C * (D + pad<ET>())];
     __shared__ __attribute__((aligned(16))) ET sV[C * LV];
@@ -586,22 +726,24 @@ __global__ __launch_bounds__(NT) void seg_kernel(const Seg a) {
     const int first = seg * a.cps, last = min(a.nc, first + a.cps) - 1;
     State<D, NV> S;
     S.load(nullptr, a.dk, a.dv, c0, 0);
-    Tile<ET, C, D> tk;
-    Tile<ET, C, 64 * NV> tv;
-    float tg = 0.f, all = 1.f;
+    Tile<ET, D, VEC> tk;
+    Tile<ET, 64 * NV, VEC> tv;
+    uint32_t tg = 0;
+    float all = 1.f;
     const auto fetch = [&](int c) {
         const int64_t t0 = (int64_t)c * C;
         const int n = min((int64_t)C, a.T - t0);
-        tk.fetch(a.K, a.K.at(b, t0, h), n, a.dk, a.dt);
-        tv.fetch(a.V, a.V.at(b, t0, h) + c0, n, a.dv - c0, a.dt);
-        if (w == 0) tg = l < n ? a.g.load(b, t0 + l, h) : 0.f;
+        tk.fetch(a.K.from(b, t0, h, 0, a.dt), a.K.st, n, a.dk, a.dt);
+        tv.fetch(a.V.from(b, t0, h, c0, a.dt), a.V.st, n, a.dv - c0, a.dt);
+        tg = a.g.fetch(b, t0 + min(l, n - 1), h);
     };
     for (int i = first - 1; i <= last; ++i) {
+        const int n = min((int64_t)C, a.T - (int64_t)(REV ? first + last - i : i) * C);
         if (i >= first) {
             __syncthreads();
-            tk.store(sK);
-            tv.store(sV);
-            if (w == 0) d.template set<REV>(tg, a.scale);
+            tk.store(sK, n, a.dk, a.dt);
+            tv.store(sV, n, a.dv - c0, a.dt);
+            if (w == 0) d.template set<REV>(l < n ? a.g.value(tg) : 0.f, a.scale);
             __syncthreads();
         }
         if (i < last) fetch(REV ? first + last - i - 1 : i + 1);
@@ -617,8 +759,8 @@ __global__ __launch_bounds__(NT) void seg_kernel(const Seg a) {
             Frag<ET> vw[NV][NS];
 #pragma unroll
             for (int x = 0; x < NV; ++x)
-                weigh<ET>(col_frag(sV, LV, k0, 16 * NV * w + 4 * x, 4 * NV), d.ws + k0 + 8 * g, vw[x]);
-            S.template add<NS, ET>(sK, k0, vw);
+                weigh<ET>(col_frag(sV, LV, k0, 16 * NV * w + 4 * x, 4 * NV, l), d.ws + k0 + 8 * g, vw[x]);
+            S.template add<NS, ET>(sK, k0, vw, l);
         }
     }
     const int64_t at = ((int64_t)b * a.Hv + h) * a.nseg + seg;
@@ -629,28 +771,55 @@ __global__ __launch_bounds__(NT) void seg_kernel(const Seg a) {
 // Columns of V' to a workgroup: 64, or 128 where the state of 128 fits the registers beside the tiles.
 inline int cols_of(int dk, int dv) { return dv <= 64 || dk > 128 ? 64 : 128; }
 
-// Launches for K' heads of up to 64, 128 and 256 channels; a.slices is set.
-void pass_d64(const Pass &a, Kind kind, hipStream_t st);
-void pass_d128(const Pass &a, Kind kind, hipStream_t st);
-void pass_d256(const Pass &a, Kind kind, hipStream_t st);
-void seg_d64(const Seg &a, bool rev, hipStream_t st);
-void seg_d128(const Seg &a, bool rev, hipStream_t st);
-void seg_d256(const Seg &a, bool rev, hipStream_t st);
+// Launches for K' heads of up to 64, 128 and 256 channels, the second set for sizes that are no multiple of 8.
+#define GDN_LINATT_DECLARE(NAME)                                  \
+    void pass_##NAME(const Pass &a, Kind kind, hipStream_t st);   \
+    void seg_##NAME(const Seg &a, bool rev, hipStream_t st);
+GDN_LINATT_DECLARE(d64)
+GDN_LINATT_DECLARE(d128)
+GDN_LINATT_DECLARE(d256)
+GDN_LINATT_DECLARE(odd64)
+GDN_LINATT_DECLARE(odd128)
+GDN_LINATT_DECLARE(odd256)
 
-template <typename ET, int D, int NV>
+// VEC: all heads' channels are a multiple of 8.
+template <typename ET, int D, int NV, bool VEC>
 void launch_pass(const Pass &a, Kind kind, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)a.slices * a.Hv * a.B * a.nseg));
-    if (kind == Y) hipLaunchKernelGGL((pass_kernel<ET, D, NV, Y>), grid, dim3(NT), 0, st, a);
-    else if (kind == DQ) hipLaunchKernelGGL((pass_kernel<ET, D, NV, DQ>), grid, dim3(NT), 0, st, a);
-    else if (kind == DK) hipLaunchKernelGGL((pass_kernel<ET, D, NV, DK>), grid, dim3(NT), 0, st, a);
-    else hipLaunchKernelGGL((pass_kernel<ET, D, NV, DV>), grid, dim3(NT), 0, st, a);
+    if (kind == Y) hipLaunchKernelGGL((pass_kernel<ET, D, NV, Y, VEC>), grid, dim3(NT), 0, st, a);
+    else if (kind == DQ) hipLaunchKernelGGL((pass_kernel<ET, D, NV, DQ, VEC>), grid, dim3(NT), 0, st, a);
+    else if (kind == DK) hipLaunchKernelGGL((pass_kernel<ET, D, NV, DK, VEC>), grid, dim3(NT), 0, st, a);
+    else hipLaunchKernelGGL((pass_kernel<ET, D, NV, DV, VEC>), grid, dim3(NT), 0, st, a);
 }
-template <typename ET, int D, int NV>
+template <typename ET, int D, int NV, bool VEC>
 void launch_seg(const Seg &a, bool rev, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)a.slices * a.Hv * a.B * (a.nseg - 1)));
-    if (rev) hipLaunchKernelGGL((seg_kernel<ET, D, NV, true>), grid, dim3(NT), 0, st, a);
-    else hipLaunchKernelGGL((seg_kernel<ET, D, NV, false>), grid, dim3(NT), 0, st, a);
+    if (rev) hipLaunchKernelGGL((seg_kernel<ET, D, NV, true, VEC>), grid, dim3(NT), 0, st, a);
+    else hipLaunchKernelGGL((seg_kernel<ET, D, NV, false, VEC>), grid, dim3(NT), 0, st, a);
 }
+template <typename ET, int D, bool VEC>
+void launch_pass_cols(const Pass &a, Kind kind, hipStream_t st) {
+    if constexpr (D <= 128) {
+        if (cols_of(D, a.dv) == 128) return launch_pass<ET, D, 2, VEC>(a, kind, st);
+    }
+    launch_pass<ET, D, 1, VEC>(a, kind, st);
+}
+template <typename ET, int D, bool VEC>
+void launch_seg_cols(const Seg &a, bool rev, hipStream_t st) {
+    if constexpr (D <= 128) {
+        if (cols_of(D, a.dv) == 128) return launch_seg<ET, D, 2, VEC>(a, rev, st);
+    }
+    launch_seg<ET, D, 1, VEC>(a, rev, st);
+}
+#define GDN_LINATT(NAME, D, VEC)                                       \
+    void pass_##NAME(const Pass &a, Kind kind, hipStream_t st) {        \
+        if (a.dt == DT_BF16) launch_pass_cols<bf16, D, VEC>(a, kind, st); \
+        else launch_pass_cols<float, D, VEC>(a, kind, st);             \
+    }                                                                  \
+    void seg_##NAME(const Seg &a, bool rev, hipStream_t st) {           \
+        if (a.dt == DT_BF16) launch_seg_cols<bf16, D, VEC>(a, rev, st);  \
+        else launch_seg_cols<float, D, VEC>(a, rev, st);               \
+    }
 
 }  // namespace la
 }  // namespace gdn

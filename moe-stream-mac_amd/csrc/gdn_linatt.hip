@@ -165,19 +165,17 @@ static Plan plan(int B, int T, int Hv, int Dk, int Dv) {
     return {(int)((nc + cps - 1) / cps), (int)cps, (int)nc};
 }
 
-static Ten ten(const void *p, const int64_t *st, int div, int D, int dt) {
-    const int e = dt == DT_F32 ? 4 : 2, m = 16 / e;  // 8 channels: one 16-byte load, or two
-    const bool v = D % 8 == 0 && aligned_to(p, 16) && st[0] % m == 0 && st[1] % m == 0 && st[2] % m == 0;
-    return {p, st[0], st[1], st[2], div, v};
-}
+static Ten ten(const void *p, const int64_t *st, int div) { return {p, st[0], st[1], st[2], div}; }
+
+static int slot(int dk, int dv) { return (dk <= 64 ? 0 : dk <= 128 ? 1 : 2) + (dk % 8 || dv % 8 ? 3 : 0); }
 
 static int run_pass(Pass a, Kind kind, hipStream_t st) {
     static const char *const names[] = {"linatt_fwd", "linatt_dq", "linatt_dk", "linatt_dv"};
     a.slices = slices_of(a.dk, a.dv);
-    a.o_vec = a.dv % 8 == 0 && aligned_to(a.o, 16);
     {
         Timed tm(names[kind], st);
-        (a.dk <= 64 ? pass_d64 : a.dk <= 128 ? pass_d128 : pass_d256)(a, kind, st);
+        constexpr decltype(&pass_d64) run[] = {pass_d64, pass_d128, pass_d256, pass_odd64, pass_odd128, pass_odd256};
+        run[slot(a.dk, a.dv)](a, kind, st);
     }
     return check_launch(st, names[kind]);
 }
@@ -188,7 +186,8 @@ static int run_segments(Seg a, const float *s0, hipStream_t st) {
     a.slices = slices_of(a.dk, a.dv);
     {
         Timed tm(REV ? "linatt_segments_rev" : "linatt_segments", st);
-        (a.dk <= 64 ? seg_d64 : a.dk <= 128 ? seg_d128 : seg_d256)(a, REV, st);
+        constexpr decltype(&seg_d64) run[] = {seg_d64, seg_d128, seg_d256, seg_odd64, seg_odd128, seg_odd256};
+        run[slot(a.dk, a.dv)](a, REV, st);
     }
     const int rc = check_launch(st, "linear attention (segments)");
     if (rc) return rc;
@@ -220,14 +219,18 @@ static Sizes sizes(int B, int T, int Hk, int Hv, int Dk, int Dv) {
     return s;
 }
 
-static int check(int B, int T, int Hk, int Hv, int Dk, int Dv, int dtype, int g_dtype) {
+static int check(const int64_t *strides, int B, int T, int Hk, int Hv, int Dk, int Dv, int dtype, int g_dtype) {
     if (B < 0 || T < 0) return fail(GDN_ERR_INVALID, "B and T must be >= 0");
     if (Hk <= 0 || Hv <= 0 || Dk <= 0 || Dv <= 0) return fail(GDN_ERR_INVALID, "head counts and sizes must be positive");
     if (Hv % Hk) return fail(GDN_ERR_INVALID, "the key heads (%d) must divide the value heads (%d)", Hk, Hv);
     for (int d : {dtype, g_dtype})
         if (d != GDN_F32 && d != GDN_BF16 && d != GDN_F16) return fail(GDN_ERR_INVALID, "unknown dtype code");
     if (Dk > MAX_D || Dv > MAX_D) return fail(GDN_ERR_UNSUPPORTED, "heads of more than %d channels are not supported", MAX_D);
+    for (int i = 0; strides && i < 9; i += 3)
+        if (strides[i + 1] < 0 || strides[i + 1] >= 1 << 24)  // a chunk's rows are addressed in 32 bits
+            return fail(GDN_ERR_UNSUPPORTED, "tokens of q, k and v must be less than 2^24 elements apart");
     if ((int64_t)B * Hv > 65535 || Hv > 65535) return fail(GDN_ERR_UNSUPPORTED, "more than 65535 heads over the batch");
+    if ((int64_t)Hv * (Dk > Dv ? Dk : Dv) >= 1 << 24) return fail(GDN_ERR_UNSUPPORTED, "a token of more than 2^24 elements");
     return 0;
 }
 
@@ -250,7 +253,7 @@ extern "C" int gdn_linatt_fwd(const void *q, const void *k, const void *v, const
                               float *state_T, void *saved, size_t saved_bytes, const int64_t *strides, int B, int T, int Hk,
                               int Hv, int Dk, int Dv, float scale, int dtype, int g_dtype, void *stream) {
     clear_error();
-    int rc = la::check(B, T, Hk, Hv, Dk, Dv, dtype, g_dtype);
+    int rc = la::check(strides, B, T, Hk, Hv, Dk, Dv, dtype, g_dtype);
     if (rc) return rc;
     if (B == 0) return GDN_OK;
     if (T == 0) return fail(GDN_ERR_INVALID, "T must be positive");
@@ -264,9 +267,9 @@ extern "C" int gdn_linatt_fwd(const void *q, const void *k, const void *v, const
     const int r = Hv / Hk;
     const la::Gate gate{g, strides[9], strides[10], strides[11], g_dtype};
     la::Pass p{};
-    p.Q = la::ten(q, strides, r, Dk, dtype);
-    p.K = la::ten(k, strides + 3, r, Dk, dtype);
-    p.V = la::ten(v, strides + 6, 1, Dv, dtype);
+    p.Q = la::ten(q, strides, r);
+    p.K = la::ten(k, strides + 3, r);
+    p.V = la::ten(v, strides + 6, 1);
     p.g = gate;
     p.B = B; p.T = T; p.Hv = Hv; p.dk = Dk; p.dv = Dv; p.nseg = pl.nseg; p.cps = pl.cps; p.nc = pl.nc;
     p.dt = p.o_dt = dtype;
@@ -293,7 +296,7 @@ extern "C" int gdn_linatt_bwd(const void *q, const void *k, const void *v, const
                               size_t workspace_bytes, const int64_t *strides, int B, int T, int Hk, int Hv, int Dk, int Dv,
                               float scale, int g_per_head, int dtype, int g_dtype, void *stream) {
     clear_error();
-    int rc = la::check(B, T, Hk, Hv, Dk, Dv, dtype, g_dtype);
+    int rc = la::check(strides, B, T, Hk, Hv, Dk, Dv, dtype, g_dtype);
     if (rc) return rc;
     if (B == 0) return GDN_OK;
     if (T == 0) return fail(GDN_ERR_INVALID, "T must be positive");
@@ -316,8 +319,8 @@ extern "C" int gdn_linatt_bwd(const void *q, const void *k, const void *v, const
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int r = Hv / Hk;
     const int64_t dys[3] = {(int64_t)T * Hv * Dv, (int64_t)Hv * Dv, Dv}, size = (int64_t)Dk * Dv;
-    const la::Ten tq = la::ten(q, strides, r, Dk, dtype), tk = la::ten(k, strides + 3, r, Dk, dtype);
-    const la::Ten tv = la::ten(v, strides + 6, 1, Dv, dtype), tdy = la::ten(dy, dys, 1, Dv, dtype);
+    const la::Ten tq = la::ten(q, strides, r), tk = la::ten(k, strides + 3, r);
+    const la::Ten tv = la::ten(v, strides + 6, 1), tdy = la::ten(dy, dys, 1);
     const la::Gate gate{g, strides[9], strides[10], strides[11], g_dtype};
     la::Pass p{};
     p.g = gate;
@@ -385,7 +388,7 @@ extern "C" int gdn_linatt_step(const void *q, const void *k, const void *v, cons
                                int64_t gs_h, int B, int Hk, int Hv, int Dk, int Dv, float scale, int dtype, int g_dtype,
                                void *stream) {
     clear_error();
-    const int rc = la::check(B, 1, Hk, Hv, Dk, Dv, dtype, g_dtype);
+    const int rc = la::check(nullptr, B, 1, Hk, Hv, Dk, Dv, dtype, g_dtype);
     if (rc) return rc;
     if (B == 0) return GDN_OK;
     if (!q || !k || !v || !g || !state || !y) return fail(GDN_ERR_INVALID, "null pointer");

@@ -1,0 +1,10 @@
+// Linear attention: the kernels for K' heads of up to 64 channels, sizes that are no multiple of 8.
+#include "gdn_linatt.h"
+
+namespace gdn {
+namespace la {
+
+GDN_LINATT(odd64, 64, false)
+
+}  // namespace la
+}  // namespace gdn
