@@ -67,9 +67,41 @@ __device__ __forceinline__ f4 mma(const F32Frag &a, const F32Frag &b, f4 acc) {
     return acc;
 }
 
-// The operand whose summed axis is contiguous: p is the lane's first element.
-__device__ __forceinline__ bf8 row_frag(const bf16 *p) { return *reinterpret_cast<const bf8 *>(p); }
-__device__ __forceinline__ F32Frag row_frag(const float *p) {
+// A tile [rows][W] in LDS.  fp32 rows are padded by 16 bytes.  bf16 rows are not, their 16-byte chunks are permuted: chunk c of
+// row r lies at c ^ swz(r), so that the 16 lanes of one cycle of a 16-byte read (0-3, 12-15, 20-23 and 24-27, ...) and the 4
+// rows by 4 chunks of a transposing read lie in different banks.  swz depends on r mod 16 only and x, a multiple of 32 columns,
+// enters by exclusive or: an offset is (lane part ^ x) + rows.
+template <typename ET, int W>
+struct Lds {
+    static constexpr bool F32 = std::is_same_v<ET, float>;
+    static constexpr int LD = W + (F32 ? 4 : 0);
+    static __device__ __forceinline__ int swz(int r) {
+        const int q = (r >> 2) & 3, low = ((q ^ (q << 1)) & 2) | (q >> 1);  // 0, 2, 3, 1
+        return W == 64 ? ((r & 2) << 1) | low : ((r & 3) << 2) | low;
+    }
+    static __device__ __forceinline__ int add(int o, int x) { return F32 ? o + x : o ^ x; }
+    // 8 columns from c on, c a multiple of 8
+    static __device__ __forceinline__ int at8(int r, int c) { return F32 ? r * LD + c : r * W + (c ^ (swz(r) << 3)); }
+    // 4 columns from c on, c a multiple of 4
+    static __device__ __forceinline__ int at4(int r, int c) { return F32 ? r * LD + c : r * W + (c ^ (swz(r) << 3)); }
+    // the operand whose summed axis is contiguous: row li, 8 columns 8 g on of 32
+    static __device__ __forceinline__ int row_lane(int li, int g) { return at8(li, 8 * g); }
+    // the operand whose summed axis runs down the rows: what col_frag takes, for quads of columns CS apart
+    template <int CS>
+    static __device__ __forceinline__ int col_lane(int li, int g) {
+        if constexpr (F32) return 8 * g * LD + (li >> 2) * CS + (li & 3);
+        else return at4(8 * g + (li >> 2), (li & 3) * CS);
+    }
+};
+
+// Row r0 (a multiple of 16) + the lane's, columns x (of 32) on.
+template <typename L>
+__device__ __forceinline__ bf8 row_frag(const bf16 *t, int lane, int r0, int x) {
+    return *reinterpret_cast<const bf8 *>(t + L::add(lane, x) + r0 * L::LD);
+}
+template <typename L>
+__device__ __forceinline__ F32Frag row_frag(const float *t, int lane, int r0, int x) {
+    const float *p = t + L::add(lane, x) + r0 * L::LD;
     F32Frag f;
     const f4 a = *reinterpret_cast<const f4 *>(p), b = *reinterpret_cast<const f4 *>(p + 4);
 #pragma unroll
@@ -80,23 +112,23 @@ __device__ __forceinline__ F32Frag row_frag(const float *p) {
     return f;
 }
 
-// The operand whose summed axis runs down the rows k0 .. k0 + 31 of a tile: lane 4 c + i of 16 holds column c0 + c cs + i.
-// bf16: the LDS's transposing read, where the four lanes 4 j .. 4 j + 3 of 16 give the addresses of row j's four quads of
-// columns and lane 4 c + i receives column i of quad c, rows 0 to 3.
-__device__ __forceinline__ bf8 col_frag(const bf16 *t, int ld, int k0, int c0, int cs, int l) {
+// Rows k0 (of 32) on: lane 4 c + i of 16 holds column x + c CS + i (+ half, 0 or 4).  bf16: the LDS's transposing read, where
+// the four lanes 4 j .. 4 j + 3 of 16 give the addresses of row j's four quads of columns and lane 4 c + i receives column i of
+// quad c, rows 0 to 3; rows 4 on are a second read (their swz differs by 2).
+template <typename L>
+__device__ __forceinline__ bf8 col_frag(const bf16 *t, int lane, int k0, int x, int half) {
     typedef __attribute__((address_space(3))) s4 lds_s4;
-    const int li = l & 15, g = l >> 4;
-    const bf16 *p = t + (k0 + 8 * g + (li >> 2)) * ld + c0 + (li & 3) * cs;
-    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)p);
-    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p + 4 * ld));
+    const int o = L::add(lane, x);
+    const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(t + o + k0 * L::LD + half));
+    const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(t + (o ^ 16) + (k0 + 4) * L::LD + half));
     return __builtin_bit_cast(bf8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
-__device__ __forceinline__ F32Frag col_frag(const float *t, int ld, int k0, int c0, int cs, int l) {
-    const int li = l & 15, g = l >> 4;
-    const float *p = t + (k0 + 8 * g) * ld + c0 + (li >> 2) * cs + (li & 3);
+template <typename L>
+__device__ __forceinline__ F32Frag col_frag(const float *t, int lane, int k0, int x, int half) {
+    const float *p = t + lane + x + half + k0 * L::LD;
     F32Frag f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f.v[j] = p[j * ld];
+    for (int j = 0; j < 8; ++j) f.v[j] = p[j * L::LD];
     return f;
 }
 
@@ -127,9 +159,6 @@ __device__ __forceinline__ void to_f32(const F32Frag &a, float (&x)[8]) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = a.v[j];
 }
-
-template <typename ET>
-constexpr int pad() { return std::is_same_v<ET, float> ? 4 : 8; }  // 16 bytes: rows of a 16-byte read in other banks
 
 // A tensor [B][T][heads][D], channels contiguous; value head h reads head h / div.
 struct Ten {
@@ -165,14 +194,14 @@ struct Tile {
             const unsigned c = (c0 < w ? c0 : 0) * size;
 #pragma unroll
             for (int p = 0; p < PER; ++p) {
-                const char *s = t0 + ((unsigned)min(r0 + p * STEP, n - 1) * row + c);
+                const char *s = t0 + (__umul24(min(r0 + p * STEP, n - 1), row) + c);
                 x[p][0] = reinterpret_cast<const u4_any *>(s)->v;
                 if constexpr (F32) x[p][1] = reinterpret_cast<const u4_any *>(s + (dt == DT_F32 ? 16 : 0))->v;
             }
         } else {
 #pragma unroll
             for (int p = 0; p < PER; ++p) {
-                const unsigned at = (unsigned)min(r0 + p * STEP, n - 1) * (unsigned)st;
+                const unsigned at = __umul24(min(r0 + p * STEP, n - 1), (unsigned)st);
                 u4 y[2] = {};
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -191,12 +220,18 @@ struct Tile {
         }
     }
     __device__ __forceinline__ void store(ET *dst, int n, int w, int dt) const {
+        if (n == C && w >= W) store_as<true>(dst, n, w, dt);
+        else store_as<false>(dst, n, w, dt);
+    }
+    template <bool FULL>
+    __device__ __forceinline__ void store_as(ET *dst, int n, int w, int dt) const {
         const int tid = opaque(threadIdx.x), r0 = tid / (W / 8), c0 = (tid % (W / 8)) * 8;
 #pragma unroll
         for (int p = 0; p < PER; ++p) {
             const int r = r0 + p * STEP;
-            ET *d = dst + r * (W + pad<ET>()) + c0;
-            const bool in = r < n && c0 < w;
+            // STEP rows on the permutation is the same where STEP is a multiple of 16
+            ET *d = dst + (STEP % 16 == 0 ? Lds<ET, W>::at8(r0, c0) + p * STEP * Lds<ET, W>::LD : Lds<ET, W>::at8(r, c0));
+            const bool in = FULL || (r < n && c0 < w);
             u4 a = x[p][0];
             if constexpr (F32) {
                 u4 b = x[p][1];
@@ -233,11 +268,11 @@ __device__ __forceinline__ void store_row(void *p, int64_t i, int dt, const floa
             reinterpret_cast<u4_any *>(static_cast<float *>(p) + i + j)->v = a;
         }
     } else {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
         uint32_t u[N / 2];
 #pragma unroll
         for (int j = 0; j < N / 2; ++j) {
-            if constexpr (std::is_same_v<ET, bf16>)
-                u[j] = (uint32_t)f32_to_bf16_cvt(o[2 * j]) | ((uint32_t)f32_to_bf16_cvt(o[2 * j + 1]) << 16);
+            if constexpr (std::is_same_v<ET, bf16>) u[j] = __builtin_bit_cast(uint32_t, b2{(bf16)o[2 * j], (bf16)o[2 * j + 1]});
             else u[j] = ops::pack2(o[2 * j], o[2 * j + 1], DT_F16);
         }
         uint16_t *d = static_cast<uint16_t *>(p) + i;
@@ -302,10 +337,10 @@ struct Gate {
     __device__ __forceinline__ float load(int b, int64_t t, int h) const { return value(fetch(b, t, h)); }
 };
 
-// Of one chunk: G (in powers of two), and the weights of its outputs and sources, e^{G_r} and e^{G_C - G_s} (reverse: the
+// Of one chunk: G (as powers of two), and the weights of its outputs and sources, e^{G_r} and e^{G_C - G_s} (reverse: the
 // other way round), the scale in the outputs' (reverse: the sources').
 struct Decays {
-    double G[C];
+    float2 G[C];  // in two terms: differences hold where sums are large
     float wo[C], ws[C], total;
     // wave 0; g of token t in lane t, 0 past the end
     template <bool REV>
@@ -314,7 +349,8 @@ struct Decays {
         const double s = wave_prefix_sum((double)g * LOG2E), end = readlane_f64(s, C - 1);
         {
             const float in = __builtin_amdgcn_exp2f((float)s), out = __builtin_amdgcn_exp2f((float)(end - s));
-            G[l] = s;
+            const float hi = (float)s;
+            G[l] = make_float2(hi, (float)(s - (double)hi));
             wo[l] = REV ? out : in * scale;
             ws[l] = REV ? in * scale : out;
         }
@@ -345,16 +381,18 @@ constexpr bool p_over_q() { return std::is_same_v<ET, float> && D > 128; }
 
 template <typename ET, int D, int NV, int KIND>
 struct Shared {
-    static constexpr int LV = 64 * NV + pad<ET>(), LP = C + pad<ET>();
+    using LK = Lds<ET, D>;        // tiles Q' and K'
+    using LV = Lds<ET, 64 * NV>;  // V' and X
+    using LP = Lds<ET, C>;        // P
     static constexpr bool TAKEN = p_over_q<ET, D>();
-    ET Q[C * (D + pad<ET>())], K[C * (D + pad<ET>())], V[C * LV];
-    ET own_p[TAKEN ? 8 : C * LP], own_x[KIND == DV && !TAKEN ? C * LV : 8];
+    ET Q[C * LK::LD], K[C * LK::LD], V[C * LV::LD];
+    ET own_p[TAKEN ? 8 : C * LP::LD], own_x[KIND == DV && !TAKEN ? C * LV::LD : 8];
     Decays d;
     float dot[KIND == DQ || KIND == DK ? 4 : 1][KIND == DQ || KIND == DK ? C : 1];
     // where Q' was, once it is used: the waves' sums of M, [4][C]
-    __device__ __forceinline__ double *cross() { return reinterpret_cast<double *>(Q + (TAKEN ? C * LP + C * LV : 0)); }
+    __device__ __forceinline__ double *cross() { return reinterpret_cast<double *>(Q + (TAKEN ? C * LP::LD + C * LV::LD : 0)); }
     __device__ __forceinline__ ET *p() { return TAKEN ? Q : own_p; }
-    __device__ __forceinline__ ET *x() { return TAKEN ? Q + C * LP : own_x; }
+    __device__ __forceinline__ ET *x() { return TAKEN ? Q + C * LP::LD : own_x; }
 };
 
 // The state of a wave: K' rows 32 T + 8 (l / 16) + 4 (t & 1) + e of tile t = 2 T, 2 T + 1 by its columns 16 NV w + ...: what
@@ -402,10 +440,10 @@ struct State {
     }
     // s = total s + sum over 32 rows of the tiles: K'^T diag(weights) V', the weighted V' in NS terms
     template <int NS, typename ET>
-    __device__ __forceinline__ void add(const ET *sK, int k0, const Frag<ET> (&vw)[NV][NS], int l) {
+    __device__ __forceinline__ void add(const ET *sK, int lane, int k0, const Frag<ET> (&vw)[NV][NS]) {
 #pragma unroll
         for (int t = 0; t < D / 16; ++t) {
-            const Frag<ET> a = col_frag(sK, D + pad<ET>(), k0, 32 * (t >> 1) + 4 * (t & 1), 8, l);
+            const Frag<ET> a = col_frag<Lds<ET, D>>(sK, lane, k0, 32 * (t >> 1), 4 * (t & 1));
 #pragma unroll
             for (int i = 0; i < NS; ++i)
 #pragma unroll
@@ -434,6 +472,10 @@ __device__ __forceinline__ Block block(int e) {
     return REV ? Block{16 * j, 16 * i, e < 10} : Block{16 * i, 16 * j, e < 10};
 }
 
+// Workgroups go to the 8 XCDs in turn, each with its own L2: an order in which neighbours, the heads that share a key head,
+// stay on one.
+__device__ __forceinline__ int xcd_order(int i, int n) { return n % 8 == 0 ? (i % 8) * (n / 8) + i / 8 : i; }
+
 // Waves to a SIMD: two where a wave's state, tiles and sums fit 256 registers.
 template <typename ET, int D>
 constexpr int waves() { return std::is_same_v<ET, bf16> && D <= 128 ? 2 : 1; }
@@ -443,11 +485,14 @@ template <typename ET, int D, int NV, int KIND, bool VEC>
 __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a) {
     constexpr bool F32 = std::is_same_v<ET, float>, REV = KIND >= DK, DOT = KIND == DQ || KIND == DK;
     constexpr int NS = F32 ? 1 : 3, NH = F32 || !DOT ? 1 : 2;  // terms of the weighted V', of the state as an operand
-    constexpr int LK = D + pad<ET>(), LV = 64 * NV + pad<ET>(), LP = C + pad<ET>(), RT = C / 16;
+    constexpr int RT = C / 16;
+    using LK = Lds<ET, D>;
+    using LV = Lds<ET, 64 * NV>;
+    using LP = Lds<ET, C>;
     constexpr bool TAKEN = Shared<ET, D, NV, KIND>::TAKEN;
     __shared__ __attribute__((aligned(16))) Shared<ET, D, NV, KIND> sh;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int id = blockIdx.x;
+    int id = xcd_order(blockIdx.x, gridDim.x);
     const int slice = id % a.slices;
     id /= a.slices;
     const int h = id % a.Hv;
@@ -469,7 +514,6 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
         tq.fetch(a.Q.from(b, t0, h, 0, a.dt), a.Q.st, n, a.dk, a.dt);
         tk.fetch(a.K.from(b, t0, h, 0, a.dt), a.K.st, n, a.dk, a.dt);
         tv.fetch(a.V.from(b, t0, h, c0, a.dt), a.V.st, n, a.dv - c0, a.dt);
-        if constexpr (KIND == DV && !TAKEN) tx.fetch(a.X.from(b, t0, h, c0, a.dt), a.X.st, n, a.dv - c0, a.dt);
         tg = a.g.fetch(b, t0 + min(l, n - 1), h);
     };
     Piece<4 * NV, ET, VEC> px[RT];
@@ -480,30 +524,29 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
         const int l = opaque(threadIdx.x & 63), li = l & 15, col = c0 + 16 * NV * w + 4 * NV * (l >> 4);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
-            px[rt].fetch(x0, (unsigned)min(16 * rt + li, n - 1) * (unsigned)a.X.st + col, a.dv - col, a.dt);
+            px[rt].fetch(x0, __umul24(min(16 * rt + li, n - 1), (unsigned)a.X.st) + col, a.dv - col, a.dt);
     };
-    if constexpr (DOT) fetch_x(REV ? last : first);
-    for (int i = first - 1; i <= last; ++i) {
+    fetch(REV ? last : first);
+    for (int i = first; i <= last; ++i) {
         const int c = REV ? first + last - i : i;
         const int64_t t0 = (int64_t)c * C;
         const int n = min((int64_t)C, a.T - t0);
         // opaque: addresses in LDS are formed where they are used, not hoisted out of the loop and spilled
         const int tid = opaque(threadIdx.x), l = tid & 63, li = l & 15, g = l >> 4;
         const int col = c0 + 16 * NV * w + 4 * NV * g;  // the lane's first column of O
-        if (i >= first) {
-            __syncthreads();
-            tq.store(sh.Q, n, a.dk, a.dt);
-            tk.store(sh.K, n, a.dk, a.dt);
-            tv.store(sh.V, n, a.dv - c0, a.dt);
-            if constexpr (KIND == DV && !TAKEN) tx.store(sh.x(), n, a.dv - c0, a.dt);
-            if (w == 0) sh.d.template set<REV>(l < n ? a.g.value(tg) : 0.f, a.scale);
-            __syncthreads();
-        }
-        if (i < last) fetch(REV ? first + last - i - 1 : i + 1);
-        if (i < first) continue;
+        __syncthreads();
+        tq.store(sh.Q, n, a.dk, a.dt);
+        tk.store(sh.K, n, a.dk, a.dt);
+        tv.store(sh.V, n, a.dv - c0, a.dt);
+        if (w == 0) sh.d.template set<REV>(l < n ? a.g.value(tg) : 0.f, a.scale);
+        __syncthreads();
+        // X before the next tiles: loads are waited for in their order
+        if constexpr (DOT) fetch_x(c);
+        if constexpr (KIND == DV) tx.fetch(a.X.from(b, t0, h, c0, a.dt), a.X.st, n, a.dv - c0, a.dt);
+        if (i < last) fetch(REV ? c - 1 : c + 1);
 
-        __builtin_amdgcn_sched_barrier(0);
         // O = diag(wo) S Q'^T, later + P V', transposed: a lane holds one token, 4 NV consecutive columns
+        const int lk = LK::row_lane(li, g);
         f4 O[RT][NV];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -524,7 +567,7 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
             }
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                const Frag<ET> q = row_frag(sh.Q + (16 * rt + li) * LK + 32 * T + 8 * g);
+                const Frag<ET> q = row_frag<LK>(sh.Q, lk, 16 * rt, 32 * T);
 #pragma unroll
                 for (int j = 0; j < NH; ++j)
 #pragma unroll
@@ -556,10 +599,8 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
                 s += lane_xor32(s);
                 if (g == 0) sh.dot[w][r] = s;
             }
-            if (i < last) fetch_x(REV ? c - 1 : c + 1);
         }
 
-        __builtin_amdgcn_sched_barrier(0);
         // P: blocks (rt, st) of 16 outputs by 16 sources with st <= rt (reverse: >=), one to a wave in turn; the blocks that
         // fill a product's 32 sources are zeros
         ET *const sP = sh.p();
@@ -571,17 +612,14 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
             acc[e] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int x = 0; x < D; x += 32)
-                acc[e] = mma(row_frag(sh.K + (k.s0 + li) * LK + x + 8 * g), row_frag(sh.Q + (k.r0 + li) * LK + x + 8 * g), acc[e]);
+                acc[e] = mma(row_frag<LK>(sh.K, lk, k.s0, x), row_frag<LK>(sh.Q, lk, k.r0, x), acc[e]);
         }
         if constexpr (TAKEN) {
             __syncthreads();
-            if constexpr (KIND == DV) {
-                tx.fetch(a.X.from(b, t0, h, c0, a.dt), a.X.st, n, a.dv - c0, a.dt);
-                tx.store(sh.x(), n, a.dv - c0, a.dt);
-            }
         }
+        if constexpr (KIND == DV) tx.store(sh.x(), n, a.dv - c0, a.dt);
         const auto put = [&](int r, int s, const ET (&p)[4]) {
-            ET *o = sP + r * LP + s;
+            ET *o = sP + LP::at4(r, s);
             if constexpr (F32) *reinterpret_cast<float4 *>(o) = make_float4(p[0], p[1], p[2], p[3]);
             else *reinterpret_cast<uint2 *>(o) = *reinterpret_cast<const uint2 *>(p);
         };
@@ -590,14 +628,15 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
             const Block k = block<REV>(w + 4 * e);
             if (!k.in) continue;
             const int r = k.r0 + li, s0 = k.s0 + 4 * g;
-            const double gr = sh.d.G[r];
-            double gs[4];
+            const float2 gr = sh.d.G[r];
+            float2 gs[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) gs[j] = sh.d.G[s0 + j];
             ET p[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float x = acc[e][j] * (a.scale * __builtin_amdgcn_exp2f((float)(REV ? gs[j] - gr : gr - gs[j])));
+                const float d = (gr.x - gs[j].x) + (gr.y - gs[j].y);
+                const float x = acc[e][j] * (a.scale * __builtin_amdgcn_exp2f(REV ? -d : d));
                 acc[e][j] = (REV ? s0 + j >= r : s0 + j <= r) ? x : 0.f;
                 p[j] = (ET)acc[e][j];
             }
@@ -611,6 +650,7 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
         // M of the same blocks, its sums over outputs and sources apart in 64 bits: their difference from a token on is the sum
         // of the pairs that cross it
         if constexpr (KIND == DV) {
+            const int lv = LV::row_lane(li, g);
             double *cross = sh.cross() + w * C;
             cross[l] = 0.;
 #pragma unroll
@@ -620,7 +660,7 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
                 f4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < 64 * NV; i += 32)
-                    x = mma(row_frag(sh.V + (k.s0 + li) * LV + i + 8 * g), row_frag(sh.x() + (k.r0 + li) * LV + i + 8 * g), x);
+                    x = mma(row_frag<LV>(sh.V, lv, k.s0, i), row_frag<LV>(sh.x(), lv, k.r0, i), x);
                 double out = 0.;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -643,24 +683,23 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
         for (int t = 0; t < D / 16; ++t)
 #pragma unroll
             for (int x = 0; x < NV; ++x) S.s[t][x] *= total;
-#pragma unroll
+        const int lp = LP::row_lane(li, g), lvc = LV::template col_lane<4 * NV>(li, g), lkc = LK::template col_lane<8>(li, g);
+#pragma unroll 1
         for (int k0 = 0; k0 < C; k0 += 32) {
             Frag<ET> v[NV], vw[NV][NS];
 #pragma unroll
             for (int x = 0; x < NV; ++x) {
-                v[x] = col_frag(sh.V, LV, k0, 16 * NV * w + 4 * x, 4 * NV, l);
+                v[x] = col_frag<LV>(sh.V, lvc, k0, 16 * NV * w, 4 * x);
                 weigh<ET>(v[x], sh.d.ws + k0 + 8 * g, vw[x]);
             }
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 if (REV ? 16 * rt >= k0 + 32 : 16 * rt + 16 <= k0) continue;
-                const Frag<ET> p = row_frag(sh.p() + (16 * rt + li) * LP + k0 + 8 * g);
+                const Frag<ET> p = row_frag<LP>(sP, lp, 16 * rt, k0);
 #pragma unroll
                 for (int x = 0; x < NV; ++x) O[rt][x] = mma(v[x], p, O[rt][x]);
             }
-            __builtin_amdgcn_sched_barrier(0);
-            S.template add<NS, ET>(sh.K, k0, vw, l);
-            __builtin_amdgcn_sched_barrier(0);
+            S.template add<NS, ET>(sh.K, lkc, k0, vw);
         }
 
 #pragma unroll
@@ -712,12 +751,14 @@ struct Seg {
 // (the last; reverse: the first).
 template <typename ET, int D, int NV, bool REV, bool VEC>
 __global__ __launch_bounds__(NT, (waves<ET, D>())) void seg_kernel(const Seg a) {
-    constexpr int NS = std::is_same_v<ET, float> ? 1 : 3, LV = 64 * NV + pad<ET>();
-    __shared__ __attribute__((aligned(16))) ET sK[C * (D + pad<ET>())];
-    __shared__ __attribute__((aligned(16))) ET sV[C * LV];
+    constexpr int NS = std::is_same_v<ET, float> ? 1 : 3;
+    using LK = Lds<ET, D>;
+    using LV = Lds<ET, 64 * NV>;
+    __shared__ __attribute__((aligned(16))) ET sK[C * LK::LD];
+    __shared__ __attribute__((aligned(16))) ET sV[C * LV::LD];
     __shared__ Decays d;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4;
-    int id = blockIdx.x;
+    int id = xcd_order(blockIdx.x, gridDim.x);
     const int slice = id % a.slices;
     id /= a.slices;
     const int h = id % a.Hv;
@@ -737,30 +778,29 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void seg_kernel(const Seg a) 
         tv.fetch(a.V.from(b, t0, h, c0, a.dt), a.V.st, n, a.dv - c0, a.dt);
         tg = a.g.fetch(b, t0 + min(l, n - 1), h);
     };
-    for (int i = first - 1; i <= last; ++i) {
-        const int n = min((int64_t)C, a.T - (int64_t)(REV ? first + last - i : i) * C);
-        if (i >= first) {
-            __syncthreads();
-            tk.store(sK, n, a.dk, a.dt);
-            tv.store(sV, n, a.dv - c0, a.dt);
-            if (w == 0) d.template set<REV>(l < n ? a.g.value(tg) : 0.f, a.scale);
-            __syncthreads();
-        }
-        if (i < last) fetch(REV ? first + last - i - 1 : i + 1);
-        if (i < first) continue;
+    fetch(REV ? last : first);
+    for (int i = first; i <= last; ++i) {
+        const int c = REV ? first + last - i : i, n = min((int64_t)C, a.T - (int64_t)c * C);
+        __syncthreads();
+        tk.store(sK, n, a.dk, a.dt);
+        tv.store(sV, n, a.dv - c0, a.dt);
+        if (w == 0) d.template set<REV>(l < n ? a.g.value(tg) : 0.f, a.scale);
+        __syncthreads();
+        if (i < last) fetch(REV ? c - 1 : c + 1);
         const float total = d.total;
         all *= total;
 #pragma unroll
         for (int t = 0; t < D / 16; ++t)
 #pragma unroll
             for (int x = 0; x < NV; ++x) S.s[t][x] *= total;
+        const int li = l & 15, lvc = LV::template col_lane<4 * NV>(li, g), lkc = LK::template col_lane<8>(li, g);
 #pragma unroll
         for (int k0 = 0; k0 < C; k0 += 32) {
             Frag<ET> vw[NV][NS];
 #pragma unroll
             for (int x = 0; x < NV; ++x)
-                weigh<ET>(col_frag(sV, LV, k0, 16 * NV * w + 4 * x, 4 * NV, l), d.ws + k0 + 8 * g, vw[x]);
-            S.template add<NS, ET>(sK, k0, vw, l);
+                weigh<ET>(col_frag<LV>(sV, lvc, k0, 16 * NV * w, 4 * x), d.ws + k0 + 8 * g, vw[x]);
+            S.template add<NS, ET>(sK, lkc, k0, vw);
         }
     }
     const int64_t at = ((int64_t)b * a.Hv + h) * a.nseg + seg;

@@ -227,10 +227,10 @@ static int check(const int64_t *strides, int B, int T, int Hk, int Hv, int Dk, i
         if (d != GDN_F32 && d != GDN_BF16 && d != GDN_F16) return fail(GDN_ERR_INVALID, "unknown dtype code");
     if (Dk > MAX_D || Dv > MAX_D) return fail(GDN_ERR_UNSUPPORTED, "heads of more than %d channels are not supported", MAX_D);
     for (int i = 0; strides && i < 9; i += 3)
-        if (strides[i + 1] < 0 || strides[i + 1] >= 1 << 24)  // a chunk's rows are addressed in 32 bits
-            return fail(GDN_ERR_UNSUPPORTED, "tokens of q, k and v must be less than 2^24 elements apart");
+        if (strides[i + 1] < 0 || strides[i + 1] >= 1 << 22)  // a chunk's rows are addressed in 32 bits
+            return fail(GDN_ERR_UNSUPPORTED, "tokens of q, k and v must be less than 2^22 elements apart");
     if ((int64_t)B * Hv > 65535 || Hv > 65535) return fail(GDN_ERR_UNSUPPORTED, "more than 65535 heads over the batch");
-    if ((int64_t)Hv * (Dk > Dv ? Dk : Dv) >= 1 << 24) return fail(GDN_ERR_UNSUPPORTED, "a token of more than 2^24 elements");
+    if ((int64_t)Hv * (Dk > Dv ? Dk : Dv) >= 1 << 22) return fail(GDN_ERR_UNSUPPORTED, "a token of more than 2^22 elements");
     return 0;
 }
 
