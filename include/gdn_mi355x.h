@@ -292,7 +292,7 @@ int gdn_gated_rmsnorm_bwd(const void *y, const void *z, const float *w, const vo
  * fp32, or NULL for zeros; y [B][T][Hv][Dv] contiguous, of dtype; state_T as state0 (may be NULL).  Dk, Dv <= 256,
  * B * Hv <= 65535, T > 0.
  *
- * saved (gdn_linatt_saved_bytes, which may be 0) holds the states entering each segment of the sequence; gdn_linatt_bwd
+ * saved (gdn_linatt_saved_bytes) holds the decays' sums and the states entering each segment of the sequence; gdn_linatt_bwd
  * reads it.  From the cotangents dy (contiguous, of dtype) and dstate_T (fp32, or NULL for zeros; needs state_T) it writes dq,
  * dk, dv (contiguous, of dtype), dg (of g_dtype: [B][T][Hv], or with g_per_head [Hv], summed over batch and tokens) and
  * dstate0 (may be NULL).
@@ -300,7 +300,7 @@ int gdn_gated_rmsnorm_bwd(const void *y, const void *z, const float *w, const vo
  * gdn_linatt_step: one token of B sequences; q, k [B][Hk][Dk], v, y [B][Hv][Dv] contiguous, g with element strides over
  * batch and heads, state [B][Hv][Dv][Dk] fp32 updated in place. */
 size_t gdn_linatt_saved_bytes(int B, int T, int Hk, int Hv, int Dk, int Dv);
-size_t gdn_linatt_bwd_workspace_bytes(int B, int T, int Hk, int Hv, int Dk, int Dv);
+size_t gdn_linatt_bwd_workspace_bytes(int B, int T, int Hk, int Hv, int Dk, int Dv, int dtype);
 int gdn_linatt_fwd(const void *q, const void *k, const void *v, const void *g, const float *state0, void *y,
                    float *state_T, void *saved, size_t saved_bytes, const int64_t *strides, int B, int T, int Hk, int Hv,
                    int Dk, int Dv, float scale, int dtype, int g_dtype, void *stream);

@@ -177,18 +177,18 @@ struct __attribute__((packed, aligned(2))) u4_any {
     u4 v;
 };
 
-// A [C][W] tile in registers on its way from memory to LDS, 8 channels to a piece; rows >= n and columns >= w are zero.  VEC:
+// A [C][W] tile in registers on its way from memory to LDS, 8 channels to a piece, by N threads; rows >= n and columns >= w are zero.  VEC:
 // w is a multiple of 8 (or none is left), pieces are loaded whole.  No load stands under a branch, where it would be waited
 // for: rows and columns out of range load ones in range, and turn to zeros on the way to LDS.
-template <typename ET, int W, bool VEC>
+template <typename ET, int W, bool VEC, int N = NT>
 struct Tile {
     static constexpr bool F32 = std::is_same_v<ET, float>;
-    static constexpr int PER = C * W / 8 / NT, STEP = NT / (W / 8);
-    static_assert(PER * NT * 8 == C * W, "a tile splits evenly");
+    static constexpr int PER = C * W / 8 / N, STEP = N / (W / 8);
+    static_assert(PER * N * 8 == C * W, "a tile splits evenly");
     u4 x[PER][F32 ? 2 : 1];
     // t0: the tile's first row and channel; dt: its type; st: elements between rows
     __device__ __forceinline__ void fetch(const char *t0, int64_t st, int n, int w, int dt) {
-        const int tid = opaque(threadIdx.x), r0 = tid / (W / 8), c0 = (tid % (W / 8)) * 8;
+        const int tid = opaque(threadIdx.x) & (N - 1), r0 = tid / (W / 8), c0 = (tid % (W / 8)) * 8;
         const unsigned size = dt == DT_F32 ? 4 : 2, row = (unsigned)st * size;
         if constexpr (VEC) {
             const unsigned c = (c0 < w ? c0 : 0) * size;
@@ -225,7 +225,7 @@ struct Tile {
     }
     template <bool FULL>
     __device__ __forceinline__ void store_as(ET *dst, int n, int w, int dt) const {
-        const int tid = opaque(threadIdx.x), r0 = tid / (W / 8), c0 = (tid % (W / 8)) * 8;
+        const int tid = opaque(threadIdx.x) & (N - 1), r0 = tid / (W / 8), c0 = (tid % (W / 8)) * 8;
 #pragma unroll
         for (int p = 0; p < PER; ++p) {
             const int r = r0 + p * STEP;
@@ -337,41 +337,28 @@ struct Gate {
     __device__ __forceinline__ float load(int b, int64_t t, int h) const { return value(fetch(b, t, h)); }
 };
 
-// Of one chunk: G (as powers of two), and the weights of its outputs and sources, e^{G_r} and e^{G_C - G_s} (reverse: the
-// other way round), the scale in the outputs' (reverse: the sources').
+// Of one chunk, as decay_kernel writes them, 256 floats: G as powers of two, in two terms (differences hold where sums are
+// large), e^{G_r}, and e^{G_C - G_s}.
 struct Decays {
-    float2 G[C];  // in two terms: differences hold where sums are large
-    float wo[C], ws[C], total;
-    // wave 0; g of token t in lane t, 0 past the end
-    template <bool REV>
-    __device__ __forceinline__ void set(float g, float scale) {
-        const int l = threadIdx.x & 63;
-        const double s = wave_prefix_sum((double)g * LOG2E), end = readlane_f64(s, C - 1);
-        {
-            const float in = __builtin_amdgcn_exp2f((float)s), out = __builtin_amdgcn_exp2f((float)(end - s));
-            const float hi = (float)s;
-            G[l] = make_float2(hi, (float)(s - (double)hi));
-            wo[l] = REV ? out : in * scale;
-            ws[l] = REV ? in * scale : out;
-        }
-        if (l == 0) total = __builtin_amdgcn_exp2f((float)end);
-    }
+    float2 G[C];
+    float in[C], out[C];
 };
+constexpr int DECAYS = sizeof(Decays) / sizeof(float);
+static_assert(DECAYS == NT, "one float to a thread");
 
 enum Kind { Y, DQ, DK, DV };  // what a pass computes
 
 struct Pass {
     Ten Q, K, V, X;
-    Gate g;
+    const float *decays;  // [B][Hv][nc][DECAYS]
     const float *s_in;  // states entering the segments, head (b, h) at s_in + (b Hv + h) s_head, segment j at + j s_seg; or NULL
     float *s_out;       // the state leaving the last segment (reverse: the first), [B][Hv][..], or NULL
     int64_t s_head, s_seg;
     int s_t;            // states are [v'][k'] (0) or [k'][v'] (1)
     void *o;            // [B][T][heads][dv] contiguous
     float *dot;         // per token [slices][B][Hv][T]: DQ, DK X . (O from the state); DV the pairs that cross it, X = v
-    float *decay;       // DK: of each chunk, [B][Hv][nc]
     int B, T, Hv, dk, dv, slices, nseg, cps, nc;  // cps: chunks of a segment, nc: of the sequence
-    int dt, o_dt;
+    int dt, o_dt, pair;  // pair: two heads to a workgroup, whose outputs are added
     float scale;
 };
 
@@ -379,20 +366,25 @@ struct Pass {
 template <typename ET, int D>
 constexpr bool p_over_q() { return std::is_same_v<ET, float> && D > 128; }
 
-template <typename ET, int D, int NV, int KIND>
+// G: heads to a workgroup, four waves each, that share V'.
+template <typename ET, int D, int NV, int KIND, int G>
 struct Shared {
     using LK = Lds<ET, D>;        // tiles Q' and K'
     using LV = Lds<ET, 64 * NV>;  // V' and X
     using LP = Lds<ET, C>;        // P
-    static constexpr bool TAKEN = p_over_q<ET, D>();
-    ET Q[C * LK::LD], K[C * LK::LD], V[C * LV::LD];
-    ET own_p[TAKEN ? 8 : C * LP::LD], own_x[KIND == DV && !TAKEN ? C * LV::LD : 8];
-    Decays d;
-    float dot[KIND == DQ || KIND == DK ? 4 : 1][KIND == DQ || KIND == DK ? C : 1];
+    static constexpr bool TAKEN = p_over_q<ET, D>(), DOT = KIND == DQ || KIND == DK;
+    static constexpr int SUM = 4 * NV * NT;  // float4s of a head's outputs
+    ET Q[G][C * LK::LD], K[G][C * LK::LD], V[C * LV::LD];
+    ET own_p[G][TAKEN ? 8 : C * LP::LD], own_x[KIND == DV && !TAKEN ? C * LV::LD : 8];
+    Decays d[G];
+    float total[G], dot[DOT ? G : 1][DOT ? 4 : 1][DOT ? C : 1];
+    static constexpr bool SUM_OVER_Q = SUM * sizeof(float4) <= G * C * LK::LD * sizeof(ET);
+    float4 own_sum[G == 2 && !SUM_OVER_Q ? SUM : 1];
     // where Q' was, once it is used: the waves' sums of M, [4][C]
-    __device__ __forceinline__ double *cross() { return reinterpret_cast<double *>(Q + (TAKEN ? C * LP::LD + C * LV::LD : 0)); }
-    __device__ __forceinline__ ET *p() { return TAKEN ? Q : own_p; }
-    __device__ __forceinline__ ET *x() { return TAKEN ? Q + C * LP::LD : own_x; }
+    __device__ __forceinline__ double *cross() { return reinterpret_cast<double *>(Q[0] + (TAKEN ? C * LP::LD + C * LV::LD : 0)); }
+    __device__ __forceinline__ ET *p(int i) { return TAKEN ? Q[0] : own_p[i]; }
+    __device__ __forceinline__ ET *x() { return TAKEN ? Q[0] + C * LP::LD : own_x; }
+    __device__ __forceinline__ float4 *sum() { return SUM_OVER_Q ? reinterpret_cast<float4 *>(Q[0]) : own_sum; }
 };
 
 // The state of a wave: K' rows 32 T + 8 (l / 16) + 4 (t & 1) + e of tile t = 2 T, 2 T + 1 by its columns 16 NV w + ...: what
@@ -402,7 +394,7 @@ struct State {
     f4 s[D / 16][NV];
     // the lane's column of tile n
     static __device__ __forceinline__ int col(int n) {
-        const int l = threadIdx.x & 63, li = l & 15, w = threadIdx.x >> 6;
+        const int l = threadIdx.x & 63, li = l & 15, w = (threadIdx.x >> 6) & 3;
         return 16 * NV * w + 4 * NV * (li >> 2) + 4 * n + (li & 3);
     }
     // p: [v'][k'], or with tr [k'][v']; out of range (and without p) zeros
@@ -480,23 +472,23 @@ __device__ __forceinline__ int xcd_order(int i, int n) { return n % 8 == 0 ? (i 
 template <typename ET, int D>
 constexpr int waves() { return std::is_same_v<ET, bf16> && D <= 128 ? 2 : 1; }
 
-// One segment of one value head, 64 NV columns of V'.
-template <typename ET, int D, int NV, int KIND, bool VEC>
-__global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a) {
+// One segment of G value heads, 64 NV columns of V'.
+template <typename ET, int D, int NV, int KIND, int G, bool VEC>
+__global__ __launch_bounds__(NT * G, (waves<ET, D>())) void pass_kernel(const Pass a) {
     constexpr bool F32 = std::is_same_v<ET, float>, REV = KIND >= DK, DOT = KIND == DQ || KIND == DK;
     constexpr int NS = F32 ? 1 : 3, NH = F32 || !DOT ? 1 : 2;  // terms of the weighted V', of the state as an operand
     constexpr int RT = C / 16;
     using LK = Lds<ET, D>;
     using LV = Lds<ET, 64 * NV>;
     using LP = Lds<ET, C>;
-    constexpr bool TAKEN = Shared<ET, D, NV, KIND>::TAKEN;
-    __shared__ __attribute__((aligned(16))) Shared<ET, D, NV, KIND> sh;
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr bool TAKEN = Shared<ET, D, NV, KIND, G>::TAKEN;
+    __shared__ __attribute__((aligned(16))) Shared<ET, D, NV, KIND, G> sh;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3, grp = wave >> 2;
     int id = xcd_order(blockIdx.x, gridDim.x);
     const int slice = id % a.slices;
     id /= a.slices;
-    const int h = id % a.Hv;
-    id /= a.Hv;
+    const int hg = id % (a.Hv / G), h = hg * G + grp;
+    id /= a.Hv / G;
     const int b = id % a.B, seg = id / a.B, c0 = slice * 64 * NV;
     const int first = seg * a.cps, last = min(a.nc, first + a.cps) - 1;
     const int64_t head = (int64_t)b * a.Hv + h;
@@ -505,16 +497,16 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
     S.load(a.s_in ? a.s_in + head * a.s_head + seg * a.s_seg : nullptr, a.dk, a.dv, c0, a.s_t);
 
     Tile<ET, D, VEC> tq, tk;
-    Tile<ET, 64 * NV, VEC> tv, tx;
-    uint32_t tg = 0;
+    Tile<ET, 64 * NV, VEC, NT * G> tv;
+    Tile<ET, 64 * NV, VEC> tx;
+    float td = 0.f;
     const auto fetch = [&](int c) {
         const int64_t t0 = (int64_t)c * C;
-        const int l = threadIdx.x & 63;
         const int n = min((int64_t)C, a.T - t0);
         tq.fetch(a.Q.from(b, t0, h, 0, a.dt), a.Q.st, n, a.dk, a.dt);
         tk.fetch(a.K.from(b, t0, h, 0, a.dt), a.K.st, n, a.dk, a.dt);
         tv.fetch(a.V.from(b, t0, h, c0, a.dt), a.V.st, n, a.dv - c0, a.dt);
-        tg = a.g.fetch(b, t0 + min(l, n - 1), h);
+        td = a.decays[(head * a.nc + c) * DECAYS + (threadIdx.x & (NT - 1))];
     };
     Piece<4 * NV, ET, VEC> px[RT];
     const auto fetch_x = [&](int c) {
@@ -535,10 +527,12 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
         const int tid = opaque(threadIdx.x), l = tid & 63, li = l & 15, g = l >> 4;
         const int col = c0 + 16 * NV * w + 4 * NV * g;  // the lane's first column of O
         __syncthreads();
-        tq.store(sh.Q, n, a.dk, a.dt);
-        tk.store(sh.K, n, a.dk, a.dt);
+        tq.store(sh.Q[grp], n, a.dk, a.dt);
+        tk.store(sh.K[grp], n, a.dk, a.dt);
         tv.store(sh.V, n, a.dv - c0, a.dt);
-        if (w == 0) sh.d.template set<REV>(l < n ? a.g.value(tg) : 0.f, a.scale);
+        // the scale goes with e^{G_r}: into the outputs, reverse into the sources
+        reinterpret_cast<float *>(&sh.d[grp])[tid & (NT - 1)] = w == 2 ? td * a.scale : td;
+        if (w == 2 && l == C - 1) sh.total[grp] = td;
         __syncthreads();
         // X before the next tiles: loads are waited for in their order
         if constexpr (DOT) fetch_x(c);
@@ -567,7 +561,7 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
             }
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
-                const Frag<ET> q = row_frag<LK>(sh.Q, lk, 16 * rt, 32 * T);
+                const Frag<ET> q = row_frag<LK>(sh.Q[grp], lk, 16 * rt, 32 * T);
 #pragma unroll
                 for (int j = 0; j < NH; ++j)
 #pragma unroll
@@ -576,7 +570,7 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
         }
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            const float wo = sh.d.wo[16 * rt + li];
+            const float wo = (REV ? sh.d[grp].out : sh.d[grp].in)[16 * rt + li];
 #pragma unroll
             for (int x = 0; x < NV; ++x) O[rt][x] *= wo;
         }
@@ -597,13 +591,13 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
                 s = r < n ? s : 0.f;
                 s += lane_xor16(s);
                 s += lane_xor32(s);
-                if (g == 0) sh.dot[w][r] = s;
+                if (g == 0) sh.dot[grp][w][r] = s;
             }
         }
 
         // P: blocks (rt, st) of 16 outputs by 16 sources with st <= rt (reverse: >=), one to a wave in turn; the blocks that
         // fill a product's 32 sources are zeros
-        ET *const sP = sh.p();
+        ET *const sP = sh.p(grp);
         f4 acc[3];
 #pragma unroll
         for (int e = 0; e < 3; ++e) {
@@ -612,7 +606,7 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
             acc[e] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int x = 0; x < D; x += 32)
-                acc[e] = mma(row_frag<LK>(sh.K, lk, k.s0, x), row_frag<LK>(sh.Q, lk, k.r0, x), acc[e]);
+                acc[e] = mma(row_frag<LK>(sh.K[grp], lk, k.s0, x), row_frag<LK>(sh.Q[grp], lk, k.r0, x), acc[e]);
         }
         if constexpr (TAKEN) {
             __syncthreads();
@@ -628,10 +622,10 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
             const Block k = block<REV>(w + 4 * e);
             if (!k.in) continue;
             const int r = k.r0 + li, s0 = k.s0 + 4 * g;
-            const float2 gr = sh.d.G[r];
+            const float2 gr = sh.d[grp].G[r];
             float2 gs[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) gs[j] = sh.d.G[s0 + j];
+            for (int j = 0; j < 4; ++j) gs[j] = sh.d[grp].G[s0 + j];
             ET p[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -678,7 +672,7 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
                 if (g == 0) cross[k.r0 + li] -= out;
             }
         }
-        const float total = sh.d.total;
+        const float total = sh.total[grp];
 #pragma unroll
         for (int t = 0; t < D / 16; ++t)
 #pragma unroll
@@ -690,7 +684,7 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
 #pragma unroll
             for (int x = 0; x < NV; ++x) {
                 v[x] = col_frag<LV>(sh.V, lvc, k0, 16 * NV * w, 4 * x);
-                weigh<ET>(v[x], sh.d.ws + k0 + 8 * g, vw[x]);
+                weigh<ET>(v[x], (REV ? sh.d[grp].in : sh.d[grp].out) + k0 + 8 * g, vw[x]);
             }
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
@@ -699,16 +693,36 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
 #pragma unroll
                 for (int x = 0; x < NV; ++x) O[rt][x] = mma(v[x], p, O[rt][x]);
             }
-            S.template add<NS, ET>(sh.K, lkc, k0, vw);
+            S.template add<NS, ET>(sh.K[grp], lkc, k0, vw);
         }
 
+        if constexpr (G == 2) {
+            float4 *const sum = sh.sum() + w * 64 + l;
+            if (grp == 1) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int x = 0; x < NV; ++x)
+                        sum[(rt * NV + x) * NT] = make_float4(O[rt][x][0], O[rt][x][1], O[rt][x][2], O[rt][x][3]);
+            }
+            __syncthreads();
+            if (grp == 0) {
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int x = 0; x < NV; ++x) {
+                        const float4 y = sum[(rt * NV + x) * NT];
+                        O[rt][x] += f4{y.x, y.y, y.z, y.w};
+                    }
+            }
+        }
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const int r = 16 * rt + li;
             float o[4 * NV];
             row_of(rt, o);
-            if (r < n) {
-                const int64_t at = ((b * (int64_t)a.T + t0 + r) * a.Hv + h) * a.dv + col;
+            if (r < n && grp == 0) {
+                const int64_t at = ((b * (int64_t)a.T + t0 + r) * (a.Hv / G) + hg) * a.dv + col;
                 if constexpr (VEC) {
                     if (col < a.dv) store_row<4 * NV, ET>(a.o, at, a.o_dt, o);
                 } else {
@@ -721,8 +735,8 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
         const int64_t at = (((int64_t)slice * a.B + b) * a.Hv + h) * a.T + t0;
         if constexpr (DOT) {
             __syncthreads();
-            if (tid < n) a.dot[at + tid] = (sh.dot[0][tid] + sh.dot[1][tid]) + (sh.dot[2][tid] + sh.dot[3][tid]);
-            if (KIND == DK && tid == 0 && slice == 0) a.decay[head * a.nc + c] = total;
+            const float(&d)[4][C] = sh.dot[grp];
+            if (w == 0 && l < n) a.dot[at + l] = (d[0][l] + d[1][l]) + (d[2][l] + d[3][l]);
         }
         if constexpr (KIND == DV) {
             __syncthreads();
@@ -740,7 +754,7 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void pass_kernel(const Pass a
 
 struct Seg {
     Ten K, V;
-    Gate g;
+    const float *decays;
     float *s;      // [B][Hv][nseg][dv][dk]
     float *decay;  // [B][Hv][nseg]
     int B, T, Hv, dk, dv, slices, nseg, cps, nc, dt;
@@ -757,6 +771,7 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void seg_kernel(const Seg a) 
     __shared__ __attribute__((aligned(16))) ET sK[C * LK::LD];
     __shared__ __attribute__((aligned(16))) ET sV[C * LV::LD];
     __shared__ Decays d;
+    __shared__ float sum;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4;
     int id = xcd_order(blockIdx.x, gridDim.x);
     const int slice = id % a.slices;
@@ -769,14 +784,13 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void seg_kernel(const Seg a) 
     S.load(nullptr, a.dk, a.dv, c0, 0);
     Tile<ET, D, VEC> tk;
     Tile<ET, 64 * NV, VEC> tv;
-    uint32_t tg = 0;
-    float all = 1.f;
+    float td = 0.f, all = 1.f;
     const auto fetch = [&](int c) {
         const int64_t t0 = (int64_t)c * C;
         const int n = min((int64_t)C, a.T - t0);
         tk.fetch(a.K.from(b, t0, h, 0, a.dt), a.K.st, n, a.dk, a.dt);
         tv.fetch(a.V.from(b, t0, h, c0, a.dt), a.V.st, n, a.dv - c0, a.dt);
-        tg = a.g.fetch(b, t0 + min(l, n - 1), h);
+        td = a.decays[(((int64_t)b * a.Hv + h) * a.nc + c) * DECAYS + tid];
     };
     fetch(REV ? last : first);
     for (int i = first; i <= last; ++i) {
@@ -784,10 +798,11 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void seg_kernel(const Seg a) 
         __syncthreads();
         tk.store(sK, n, a.dk, a.dt);
         tv.store(sV, n, a.dv - c0, a.dt);
-        if (w == 0) d.template set<REV>(l < n ? a.g.value(tg) : 0.f, a.scale);
+        reinterpret_cast<float *>(&d)[tid] = REV && w == 2 ? td * a.scale : td;
+        if (w == 2 && l == C - 1) sum = td;
         __syncthreads();
         if (i < last) fetch(REV ? c - 1 : c + 1);
-        const float total = d.total;
+        const float total = sum;
         all *= total;
 #pragma unroll
         for (int t = 0; t < D / 16; ++t)
@@ -799,7 +814,7 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void seg_kernel(const Seg a) 
             Frag<ET> vw[NV][NS];
 #pragma unroll
             for (int x = 0; x < NV; ++x)
-                weigh<ET>(col_frag<LV>(sV, lvc, k0, 16 * NV * w, 4 * x), d.ws + k0 + 8 * g, vw[x]);
+                weigh<ET>(col_frag<LV>(sV, lvc, k0, 16 * NV * w, 4 * x), (REV ? d.in : d.out) + k0 + 8 * g, vw[x]);
             S.template add<NS, ET>(sK, lkc, k0, vw);
         }
     }
@@ -810,6 +825,10 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void seg_kernel(const Seg a) 
 
 // Columns of V' to a workgroup: 64, or 128 where the state of 128 fits the registers beside the tiles.
 inline int cols_of(int dk, int dv) { return dv <= 64 || dk > 128 ? 64 : 128; }
+
+// dq and dk of two value heads are added in one workgroup where its LDS holds both.
+template <typename ET, int D>
+constexpr bool pairs() { return std::is_same_v<ET, bf16> && D <= 128; }
 
 // Launches for K' heads of up to 64, 128 and 256 channels, the second set for sizes that are no multiple of 8.
 #define GDN_LINATT_DECLARE(NAME)                                  \
@@ -825,11 +844,19 @@ GDN_LINATT_DECLARE(odd256)
 // VEC: all heads' channels are a multiple of 8.
 template <typename ET, int D, int NV, bool VEC>
 void launch_pass(const Pass &a, Kind kind, hipStream_t st) {
-    const dim3 grid((unsigned)((int64_t)a.slices * a.Hv * a.B * a.nseg));
-    if (kind == Y) hipLaunchKernelGGL((pass_kernel<ET, D, NV, Y, VEC>), grid, dim3(NT), 0, st, a);
-    else if (kind == DQ) hipLaunchKernelGGL((pass_kernel<ET, D, NV, DQ, VEC>), grid, dim3(NT), 0, st, a);
-    else if (kind == DK) hipLaunchKernelGGL((pass_kernel<ET, D, NV, DK, VEC>), grid, dim3(NT), 0, st, a);
-    else hipLaunchKernelGGL((pass_kernel<ET, D, NV, DV, VEC>), grid, dim3(NT), 0, st, a);
+    const dim3 grid((unsigned)((int64_t)a.slices * a.Hv * a.B * a.nseg / (a.pair ? 2 : 1)));
+    if constexpr (pairs<ET, D>()) {
+        if (a.pair) {
+            const dim3 block(2 * NT);
+            if (kind == DQ) hipLaunchKernelGGL((pass_kernel<ET, D, NV, DQ, 2, VEC>), grid, block, 0, st, a);
+            else hipLaunchKernelGGL((pass_kernel<ET, D, NV, DK, 2, VEC>), grid, block, 0, st, a);
+            return;
+        }
+    }
+    if (kind == Y) hipLaunchKernelGGL((pass_kernel<ET, D, NV, Y, 1, VEC>), grid, dim3(NT), 0, st, a);
+    else if (kind == DQ) hipLaunchKernelGGL((pass_kernel<ET, D, NV, DQ, 1, VEC>), grid, dim3(NT), 0, st, a);
+    else if (kind == DK) hipLaunchKernelGGL((pass_kernel<ET, D, NV, DK, 1, VEC>), grid, dim3(NT), 0, st, a);
+    else hipLaunchKernelGGL((pass_kernel<ET, D, NV, DV, 1, VEC>), grid, dim3(NT), 0, st, a);
 }
 template <typename ET, int D, int NV, bool VEC>
 void launch_seg(const Seg &a, bool rev, hipStream_t st) {

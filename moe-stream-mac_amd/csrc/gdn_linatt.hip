@@ -9,6 +9,21 @@ namespace la {
 
 constexpr int MAX_D = 256;
 
+// The decays of every chunk; a wave to a chunk.  Their sums run in 64 bits.
+__global__ __launch_bounds__(NT) void decay_kernel(Gate g, float *o, int B, int T, int Hv, int nc) {
+    const int64_t id = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
+    const int l = threadIdx.x & 63;
+    if (id >= (int64_t)B * Hv * nc) return;
+    const int h = id % Hv, c = (id / Hv) % nc, b = id / Hv / nc;  // heads side by side: their decays are, in memory
+    const int64_t t = (int64_t)c * C + l;
+    const double s = wave_prefix_sum(t < T ? (double)g.load(b, t, h) * LOG2E : 0.), end = readlane_f64(s, C - 1);
+    const float hi = (float)s;
+    float *const p = o + (((int64_t)b * Hv + h) * nc + c) * DECAYS;
+    reinterpret_cast<float2 *>(p)[l] = make_float2(hi, (float)(s - (double)hi));
+    p[2 * C + l] = __builtin_amdgcn_exp2f(hi);
+    p[3 * C + l] = __builtin_amdgcn_exp2f((float)(end - s));
+}
+
 // The segments' sums become the states entering them: from s0 (or nothing) on, in place.
 template <bool REV>
 __global__ __launch_bounds__(NT) void scan_kernel(float *s, const float *decay, const float *s0, int nseg, int64_t size) {
@@ -37,7 +52,7 @@ __global__ __launch_bounds__(NT) void group_kernel(const float *part, void *o, i
 
 struct DecayGrad {
     const float *a, *b, *cross;  // [slices][B][Hv][T]; cross: [cross_slices]
-    const float *decay;          // [B][Hv][nc]
+    const float *decays;         // [B][Hv][nc][DECAYS]
     const float *dlast, *last;   // [B][Hv][size], or dlast NULL
     void *dg;                    // [B][T][Hv], or [Hv]
     int B, T, Hv, slices, cross_slices, per_head, dt, nc;
@@ -90,7 +105,7 @@ __global__ __launch_bounds__(64 * DW) void dg_kernel(const DecayGrad a) {
             if (l == 63) {
                 sumA[w] = xa;
                 sumB[w] = xb;
-                anew[w] = c >= 0 && a.decay[head * a.nc + c] < 0x1p-30f;
+                anew[w] = c >= 0 && a.decays[(head * a.nc + c) * DECAYS + 3 * C - 1] < 0x1p-30f;  // e^{G_C}
             }
             __syncthreads();
             double mine = 0.;
@@ -201,21 +216,26 @@ static int run_segments(Seg a, const float *s0, hipStream_t st) {
 }
 
 struct Sizes {
-    size_t state, decay, part, dot, cross, chunks, bwd;
+    size_t decays, state, decay, saved, part, dot, cross, bwd;
 };
-static Sizes sizes(int B, int T, int Hk, int Hv, int Dk, int Dv) {
+// value heads of a key head whose dq and dk are added after the passes: all, or the pairs of pair_heads()
+static bool pair_heads(int r, int Dv, int dtype) { return dtype == DT_BF16 && Dv <= 128 && r % 2 == 0; }
+
+static Sizes sizes(int B, int T, int Hk, int Hv, int Dk, int Dv, int dtype = DT_F32) {
     const Plan p = plan(B, T, Hv, Dk, Dv);
     Sizes s{};
+    s.decays = align_up256((size_t)B * Hv * p.nc * DECAYS * sizeof(float));
     if (p.nseg > 1) {
         s.state = align_up256((size_t)B * Hv * p.nseg * Dk * Dv * sizeof(float));
         s.decay = align_up256((size_t)B * Hv * p.nseg * sizeof(float));
     }
-    if (Hv > Hk) s.part = align_up256((size_t)B * T * Hv * Dk * sizeof(float));
+    s.saved = s.decays + s.state;
+    const int group = Hv / Hk / (pair_heads(Hv / Hk, Dv, dtype) ? 2 : 1);
+    if (group > 1) s.part = align_up256((size_t)B * T * Hk * group * Dk * sizeof(float));
     const size_t rows = (size_t)B * Hv * T * sizeof(float);
     s.dot = align_up256(rows * slices_of(Dv, Dk));
     s.cross = align_up256(rows * slices_of(Dk, Dv));
-    s.chunks = align_up256((size_t)B * Hv * p.nc * sizeof(float));
-    s.bwd = s.state + s.decay + s.part + 2 * s.dot + s.cross + s.chunks;
+    s.bwd = s.state + s.decay + s.part + 2 * s.dot + s.cross;
     return s;
 }
 
@@ -242,11 +262,11 @@ using namespace gdn;
 extern "C" size_t gdn_linatt_saved_bytes(int B, int T, int Hk, int Hv, int Dk, int Dv) {
     if (B <= 0 || T <= 0 || Hk <= 0 || Hv <= 0 || Dk <= 0 || Dv <= 0) return 0;
     const la::Sizes s = la::sizes(B, T, Hk, Hv, Dk, Dv);
-    return s.state + s.decay;
+    return s.saved + s.decay;
 }
-extern "C" size_t gdn_linatt_bwd_workspace_bytes(int B, int T, int Hk, int Hv, int Dk, int Dv) {
+extern "C" size_t gdn_linatt_bwd_workspace_bytes(int B, int T, int Hk, int Hv, int Dk, int Dv, int dtype) {
     if (B <= 0 || T <= 0 || Hk <= 0 || Hv <= 0 || Dk <= 0 || Dv <= 0) return 0;
-    return la::sizes(B, T, Hk, Hv, Dk, Dv).bwd;
+    return la::sizes(B, T, Hk, Hv, Dk, Dv, dtype).bwd;
 }
 
 extern "C" int gdn_linatt_fwd(const void *q, const void *k, const void *v, const void *g, const float *state0, void *y,
@@ -260,17 +280,27 @@ extern "C" int gdn_linatt_fwd(const void *q, const void *k, const void *v, const
     if (!q || !k || !v || !g || !y || !strides) return fail(GDN_ERR_INVALID, "null pointer");
     const la::Plan pl = la::plan(B, T, Hv, Dk, Dv);
     const la::Sizes sz = la::sizes(B, T, Hk, Hv, Dk, Dv);
-    if (saved_bytes < sz.state + sz.decay || (sz.state && !saved))
+    if (saved_bytes < sz.saved + sz.decay || !saved)
         return fail(GDN_ERR_WORKSPACE, "saved buffer of %zu bytes is smaller than the %zu bytes required", saved_bytes,
-                    sz.state + sz.decay);
+                    sz.saved + sz.decay);
+    float *decays = static_cast<float *>(saved), *states = reinterpret_cast<float *>(static_cast<char *>(saved) + sz.decays);
+    float *seg_decay = reinterpret_cast<float *>(static_cast<char *>(saved) + sz.saved);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int r = Hv / Hk;
     const la::Gate gate{g, strides[9], strides[10], strides[11], g_dtype};
+    {
+        Timed tm("linatt_decays", st);
+        const int64_t waves = (int64_t)B * Hv * pl.nc;
+        hipLaunchKernelGGL(la::decay_kernel, dim3((unsigned)((waves + 3) / 4)), dim3(la::NT), 0, st, gate, decays, B, T, Hv,
+                           pl.nc);
+    }
+    rc = check_launch(st, "linear attention (decays)");
+    if (rc) return rc;
     la::Pass p{};
     p.Q = la::ten(q, strides, r);
     p.K = la::ten(k, strides + 3, r);
     p.V = la::ten(v, strides + 6, 1);
-    p.g = gate;
+    p.decays = decays;
     p.B = B; p.T = T; p.Hv = Hv; p.dk = Dk; p.dv = Dv; p.nseg = pl.nseg; p.cps = pl.cps; p.nc = pl.nc;
     p.dt = p.o_dt = dtype;
     p.scale = scale;
@@ -279,11 +309,10 @@ extern "C" int gdn_linatt_fwd(const void *q, const void *k, const void *v, const
     p.s_head = (int64_t)Dk * Dv;
     p.s_out = state_T;
     if (pl.nseg > 1) {
-        float *s = static_cast<float *>(saved), *decay = reinterpret_cast<float *>(static_cast<char *>(saved) + sz.state);
-        const la::Seg a{p.K, p.V, gate, s, decay, B, T, Hv, Dk, Dv, 0, pl.nseg, pl.cps, pl.nc, dtype, scale};
+        const la::Seg a{p.K, p.V, decays, states, seg_decay, B, T, Hv, Dk, Dv, 0, pl.nseg, pl.cps, pl.nc, dtype, scale};
         rc = la::run_segments<false>(a, state0, st);
         if (rc) return rc;
-        p.s_in = s;
+        p.s_in = states;
         p.s_seg = p.s_head;
         p.s_head *= pl.nseg;
     }
@@ -303,9 +332,11 @@ extern "C" int gdn_linatt_bwd(const void *q, const void *k, const void *v, const
     if (!q || !k || !v || !g || !dy || !dq || !dk || !dv || !dg || !strides || (dstate_T && !state_T))
         return fail(GDN_ERR_INVALID, "null pointer");
     const la::Plan pl = la::plan(B, T, Hv, Dk, Dv);
-    const la::Sizes sz = la::sizes(B, T, Hk, Hv, Dk, Dv);
-    if (sz.state && (!saved || saved_bytes < sz.state + sz.decay))
-        return fail(GDN_ERR_INVALID, "the saved buffer written by gdn_linatt_fwd (%zu bytes) is required", sz.state + sz.decay);
+    const la::Sizes sz = la::sizes(B, T, Hk, Hv, Dk, Dv, dtype);
+    if (!saved || saved_bytes < sz.saved + sz.decay)
+        return fail(GDN_ERR_INVALID, "the saved buffer written by gdn_linatt_fwd (%zu bytes) is required", sz.saved + sz.decay);
+    const float *decays = static_cast<const float *>(saved);
+    const float *states = reinterpret_cast<const float *>(static_cast<const char *>(saved) + sz.decays);
     if (!workspace || workspace_bytes < sz.bwd)
         return fail(GDN_ERR_WORKSPACE, "workspace of %zu bytes is smaller than the %zu bytes required", workspace_bytes, sz.bwd);
     char *ws = static_cast<char *>(workspace);
@@ -315,28 +346,30 @@ extern "C" int gdn_linatt_bwd(const void *q, const void *k, const void *v, const
         return p;
     };
     float *ds = take(sz.state), *decay = take(sz.decay), *part = take(sz.part);
-    float *sa = take(sz.dot), *sb = take(sz.dot), *cross = take(sz.cross), *chunks = take(sz.chunks);
+    float *sa = take(sz.dot), *sb = take(sz.dot), *cross = take(sz.cross);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int r = Hv / Hk;
     const int64_t dys[3] = {(int64_t)T * Hv * Dv, (int64_t)Hv * Dv, Dv}, size = (int64_t)Dk * Dv;
     const la::Ten tq = la::ten(q, strides, r), tk = la::ten(k, strides + 3, r);
     const la::Ten tv = la::ten(v, strides + 6, 1), tdy = la::ten(dy, dys, 1);
-    const la::Gate gate{g, strides[9], strides[10], strides[11], g_dtype};
     la::Pass p{};
-    p.g = gate;
+    p.decays = decays;
     p.B = B; p.T = T; p.Hv = Hv; p.nseg = pl.nseg; p.cps = pl.cps; p.nc = pl.nc;
     p.dt = dtype;
     p.scale = scale;
     const int64_t n = (int64_t)B * T * Hk * Dk;
+    // value heads that share a key head: two to a workgroup, or each for itself, the rest added afterwards
+    const int pair = la::pair_heads(r, Dv, dtype), group = pair ? r / 2 : r;
     const auto grouped = [&](void *out, la::Kind kind) {
-        p.o = r > 1 ? part : out;
-        p.o_dt = r > 1 ? GDN_F32 : dtype;
+        p.pair = pair;
+        p.o = group > 1 ? part : out;
+        p.o_dt = group > 1 ? GDN_F32 : dtype;
         const int e = la::run_pass(p, kind, st);
-        if (e || r == 1) return e;
+        if (e || group == 1) return e;
         {
             Timed tm("linatt_group", st);
             hipLaunchKernelGGL(la::group_kernel, dim3((unsigned)((n + la::NT - 1) / la::NT)), dim3(la::NT), 0, st, part, out, n,
-                               r, Dk, dtype);
+                               group, Dk, dtype);
         }
         return check_launch(st, "linear attention (groups)");
     };
@@ -346,13 +379,13 @@ extern "C" int gdn_linatt_bwd(const void *q, const void *k, const void *v, const
     p.s_t = 1;
     p.s_head = size * (pl.nseg > 1 ? pl.nseg : 1);
     p.s_seg = size;
-    p.s_in = pl.nseg > 1 ? static_cast<const float *>(saved) : state0;
+    p.s_in = pl.nseg > 1 ? states : state0;
     p.dot = sa;
     rc = grouped(dq, la::DQ);
     if (rc) return rc;
     const float *s_in = dstate_T;
     if (pl.nseg > 1) {
-        const la::Seg a{tq, tdy, gate, ds, decay, B, T, Hv, Dk, Dv, 0, pl.nseg, pl.cps, pl.nc, dtype, scale};
+        const la::Seg a{tq, tdy, decays, ds, decay, B, T, Hv, Dk, Dv, 0, pl.nseg, pl.cps, pl.nc, dtype, scale};
         rc = la::run_segments<true>(a, dstate_T, st);
         if (rc) return rc;
         s_in = ds;
@@ -361,11 +394,11 @@ extern "C" int gdn_linatt_bwd(const void *q, const void *k, const void *v, const
     p.Q = tv; p.K = tdy; p.V = tq; p.X = tk;
     p.s_in = s_in;
     p.dot = sb;
-    p.decay = chunks;
     rc = grouped(dk, la::DK);
     if (rc) return rc;
     // dv = RLA(k, q, dy)
     p.Q = tk; p.K = tq; p.V = tdy; p.X = tv;
+    p.pair = 0;
     p.dk = Dk; p.dv = Dv;
     p.s_t = 0;
     p.dot = cross;
@@ -374,7 +407,7 @@ extern "C" int gdn_linatt_bwd(const void *q, const void *k, const void *v, const
     p.s_out = dstate0;
     rc = la::run_pass(p, la::DV, st);
     if (rc) return rc;
-    const la::DecayGrad d{sa, sb, cross, chunks, dstate_T, state_T, dg, B, T, Hv, la::slices_of(Dv, Dk), la::slices_of(Dk, Dv),
+    const la::DecayGrad d{sa, sb, cross, decays, dstate_T, state_T, dg, B, T, Hv, la::slices_of(Dv, Dk), la::slices_of(Dk, Dv),
                           g_per_head != 0, g_dtype, pl.nc, size};
     {
         Timed tm("linatt_dg", st);

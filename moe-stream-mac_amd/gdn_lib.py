@@ -55,7 +55,7 @@ _SIGS = {
     "gdn_clip_grad_norm_workspace_bytes": ([_vp, _i], _sz),
     "gdn_clip_grad_norm": ([_vp] * 4 + [_i, _i, _d, _d, _vp, _vp, _sz, _vp], _i),
     "gdn_linatt_saved_bytes": ([_i] * 6, _sz),
-    "gdn_linatt_bwd_workspace_bytes": ([_i] * 6, _sz),
+    "gdn_linatt_bwd_workspace_bytes": ([_i] * 7, _sz),
     "gdn_linatt_fwd": ([_vp] * 8 + [_sz, _vp] + [_i] * 6 + [_f, _i, _i, _vp], _i),
     "gdn_linatt_bwd": ([_vp] * 7 + [_sz] + [_vp] * 8 + [_sz, _vp] + [_i] * 6 + [_f, _i, _i, _i, _vp], _i),
     "gdn_linatt_step": ([_vp] * 6 + [_i64, _i64] + [_i] * 5 + [_f, _i, _i, _vp], _i),

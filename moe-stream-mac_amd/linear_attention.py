@@ -62,10 +62,10 @@ class _LinearAttention(torch.autograd.Function):
         last = torch.empty((B, Hv, Dv, Dk), dtype=torch.float32, device=dev)
         lib = L.load()
         n = lib.gdn_linatt_saved_bytes(B, T, Hk, Hv, Dk, Dv)
-        saved = torch.empty((n,), dtype=torch.uint8, device=dev) if n else None
+        saved = torch.empty((n,), dtype=torch.uint8, device=dev)
         with L.on_device(dev):
             L.check(lib.gdn_linatt_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), L.ptr(state), y.data_ptr(),
-                                       last.data_ptr(), L.ptr(saved), n, _strides(q, k, v, g), B, T, Hk, Hv, Dk, Dv, scale,
+                                       last.data_ptr(), saved.data_ptr(), n, _strides(q, k, v, g), B, T, Hk, Hv, Dk, Dv, scale,
                                        L.DTYPE_CODE[q.dtype], L.DTYPE_CODE[g.dtype], L.stream_handle(dev)))
         ctx.save_for_backward(q, k, v, g, state, last, saved)
         ctx.scale = scale
@@ -84,11 +84,11 @@ class _LinearAttention(torch.autograd.Function):
         dg = torch.empty(g.shape, dtype=g.dtype, device=dev)
         dstate = torch.empty_like(state) if ctx.needs_input_grad[4] else None
         lib = L.load()
-        n = lib.gdn_linatt_bwd_workspace_bytes(B, T, Hk, Hv, Dk, Dv)
+        n = lib.gdn_linatt_bwd_workspace_bytes(B, T, Hk, Hv, Dk, Dv, L.DTYPE_CODE[q.dtype])
         ws = torch.empty((n,), dtype=torch.uint8, device=dev)
         with L.on_device(dev):
             L.check(lib.gdn_linatt_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), L.ptr(state), last.data_ptr(),
-                                       L.ptr(saved), 0 if saved is None else saved.numel(), dy.data_ptr(), L.ptr(dlast),
+                                       saved.data_ptr(), saved.numel(), dy.data_ptr(), L.ptr(dlast),
                                        dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr(), L.ptr(dstate),
                                        ws.data_ptr(), n, _strides(q, k, v, g), B, T, Hk, Hv, Dk, Dv, ctx.scale,
                                        int(g.dim() == 1), L.DTYPE_CODE[q.dtype], L.DTYPE_CODE[g.dtype],

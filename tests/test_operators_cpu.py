@@ -137,7 +137,7 @@ def test_linear_attention_abi_refusals():
     assert fwd(B=0, p=None) == 0
     n = lib.gdn_linatt_saved_bytes(1, 5000, 1, 2, 64, 64)
     assert n > 0 and fwd(T=5000, saved=n - 1) == L.GDN_ERR_WORKSPACE
-    assert lib.gdn_linatt_saved_bytes(64, 60, 1, 32, 64, 64) == 0  # one segment: nothing to keep
+    assert lib.gdn_linatt_saved_bytes(64, 60, 1, 32, 64, 64) == 64 * 32 * 1024  # one segment: the decays of its chunk
     assert lib.gdn_linatt_saved_bytes(0, 60, 1, 32, 64, 64) == 0
 
     def bwd(T=100, last=fake, saved=fake, ns=1 << 40, ws=1 << 40, dq=fake):
@@ -146,7 +146,7 @@ def test_linear_attention_abi_refusals():
 
     assert bwd(last=None) == L.GDN_ERR_INVALID and bwd(dq=None) == L.GDN_ERR_INVALID and bwd(T=0) == L.GDN_ERR_INVALID
     assert bwd(T=5000, saved=None) == L.GDN_ERR_INVALID and bwd(T=5000, ns=n - 1) == L.GDN_ERR_INVALID
-    assert bwd(ws=lib.gdn_linatt_bwd_workspace_bytes(1, 100, 1, 2, 64, 64) - 1) == L.GDN_ERR_WORKSPACE
+    assert bwd(ws=lib.gdn_linatt_bwd_workspace_bytes(1, 100, 1, 2, 64, 64, 0) - 1) == L.GDN_ERR_WORKSPACE
     step = lambda p, Dk: lib.gdn_linatt_step(p, p, p, p, p, p, 1, 1, 1, 1, 2, Dk, 64, 1.0, 0, 0, None)  # noqa: E731
     assert step(None, 64) == L.GDN_ERR_INVALID and step(fake, 0) == L.GDN_ERR_INVALID
     assert step(fake, 300) == L.GDN_ERR_UNSUPPORTED
