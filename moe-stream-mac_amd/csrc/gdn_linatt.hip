@@ -128,7 +128,10 @@ __global__ __launch_bounds__(64 * DW) void dg_kernel(const DecayGrad a) {
     }
 }
 
-// One token: y = scale S' q, S' = e^g S + v k^T, in place.  L lanes share a row of the state, 4 channels each at a time.
+// One token: y = scale S' q, S' = e^g S + v k^T, in place.  `lanes` lanes share a row of the state, V channels each at a time,
+// and walk STEP_ROWS rows side by side, all of whose loads are under way before the first is used: the state, read and
+// written once, is the kernel's traffic.
+constexpr int STEP_ROWS = 4;
 struct Step {
     const void *q, *k, *v;
     Gate g;
@@ -140,27 +143,35 @@ struct Step {
 template <int V>
 __global__ __launch_bounds__(NT) void step_kernel(const Step a) {
     const int lanes = a.lanes, lane = threadIdx.x & (lanes - 1), rows = NT / lanes;
-    const int row = blockIdx.x * rows + threadIdx.x / lanes, h = blockIdx.y, b = blockIdx.z;
+    const int row0 = blockIdx.x * rows * STEP_ROWS + threadIdx.x / lanes, h = blockIdx.y, b = blockIdx.z;
     const int64_t hv = (int64_t)b * a.Hv + h, hk = (int64_t)b * a.Hk + h / (a.Hv / a.Hk);
     const float f = __builtin_amdgcn_exp2f(a.g.load(b, 0, h) * (float)LOG2E);
-    const bool in = row < a.Dv;
-    const float v = in ? load_as_f32(a.v, hv * a.Dv + row, a.dt) : 0.f;
-    float *s = a.state + (hv * a.Dv + (in ? row : 0)) * a.Dk;
-    float y = 0.f;
+    float *const s = a.state + hv * a.Dv * a.Dk;
+    float y[STEP_ROWS] = {}, v[STEP_ROWS];
+#pragma unroll
+    for (int i = 0; i < STEP_ROWS; ++i) v[i] = load_as_f32(a.v, hv * a.Dv + min(row0 + i * rows, a.Dv - 1), a.dt);
     for (int c = lane * V; c < a.Dk; c += lanes * V) {
-        float x[V], q[V], k[V];
-        ops::loadv<V>(s, c, DT_F32, x);
+        float x[STEP_ROWS][V], q[V], k[V];
+#pragma unroll
+        for (int i = 0; i < STEP_ROWS; ++i) ops::loadv<V>(s, (int64_t)min(row0 + i * rows, a.Dv - 1) * a.Dk + c, DT_F32, x[i]);
         ops::loadv<V>(a.q, hk * a.Dk + c, a.dt, q);
         ops::loadv<V>(a.k, hk * a.Dk + c, a.dt, k);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            x[j] = fmaf(v, k[j], f * x[j]);
-            y = fmaf(x[j], q[j], y);
+        for (int i = 0; i < STEP_ROWS; ++i) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                x[i][j] = fmaf(v[i], k[j], f * x[i][j]);
+                y[i] = fmaf(x[i][j], q[j], y[i]);
+            }
+            if (row0 + i * rows < a.Dv) ops::storev<V>(s, (int64_t)(row0 + i * rows) * a.Dk + c, DT_F32, x[i]);
         }
-        if (in) ops::storev<V>(s, c, DT_F32, x);
     }
-    for (int m = 1; m < lanes; m <<= 1) y += __shfl_xor(y, m);
-    if (in && lane == 0) store_from_f32(a.y, hv * a.Dv + row, y * a.scale, a.dt);
+#pragma unroll
+    for (int i = 0; i < STEP_ROWS; ++i) {
+        for (int m = 1; m < lanes; m <<= 1) y[i] += __shfl_xor(y[i], m);
+        const int row = row0 + i * rows;
+        if (lane == 0 && row < a.Dv) store_from_f32(a.y, hv * a.Dv + row, y[i] * a.scale, a.dt);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------- host
@@ -428,7 +439,7 @@ extern "C" int gdn_linatt_step(const void *q, const void *k, const void *v, cons
     const bool vec = Dk % 4 == 0 && aligned_to(q, 16) && aligned_to(k, 16) && aligned_to(state, 16);
     la::Step a{q, k, v, {g, gs_b, 0, gs_h, g_dtype}, state, y, Hk, Hv, Dk, Dv, dtype, 1, scale};
     while (a.lanes < 64 && a.lanes * (vec ? 4 : 1) < Dk) a.lanes *= 2;
-    const int rows = la::NT / a.lanes;
+    const int rows = la::NT / a.lanes * la::STEP_ROWS;
     const dim3 grid((unsigned)((Dv + rows - 1) / rows), (unsigned)Hv, (unsigned)B);
     hipStream_t st = static_cast<hipStream_t>(stream);
     {

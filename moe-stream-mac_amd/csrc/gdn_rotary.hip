@@ -18,6 +18,7 @@ namespace rope {
 
 constexpr int NT = 256;
 constexpr int MAX_R = 1024;  // channels that turn: 512 pairs per token in LDS
+constexpr int MAX_TOK = 4;   // tokens to a workgroup
 
 struct Args {
     const void *x[2];      // q, k
@@ -33,69 +34,101 @@ struct Args {
     int T, D, R, interleaved, dt, tok, units, lanes;
 };
 
-// V angles per unit: a unit is 2V channels that turn, or V that pass.  `lanes` (a power of two) lanes walk the units of
-// one head; a workgroup takes `tok` tokens.
+// A unit is 2 V channels: V pairs that turn, or as many that pass.  `lanes` (a power of two) lanes walk the units of one head;
+// a workgroup takes `tok` tokens, whose places in memory are worked out once, and its groups of lanes two heads at a time,
+// loads first: 16 bytes times four under way for each lane.
+template <int V>
+struct Unit {
+    float p[V], q[V];
+    int e0, e1;
+    bool turns, second;
+    __device__ __forceinline__ void load(const Args &a, const void *x, int64_t at, int u, int turning) {
+        turns = u < turning;
+        e0 = turns ? (a.interleaved ? 2 * V * u : V * u) : a.R + (u - turning) * 2 * V;
+        e1 = turns && !a.interleaved ? e0 + a.R / 2 : e0 + V;
+        second = e1 < a.D;
+        ops::loadv<V>(x, at + e0, a.dt, p);
+        ops::loadv<V>(x, at + (second ? e1 : e0), a.dt, q);
+    }
+    __device__ __forceinline__ void store(const Args &a, void *y, int64_t at, const float2 *c) {
+        if (turns) {
+            if (a.interleaved) {
+                float z[2 * V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) { z[i] = p[i]; z[V + i] = q[i]; }
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float r = z[2 * i], s = z[2 * i + 1];
+                    z[2 * i] = r * c[i].x - s * c[i].y;
+                    z[2 * i + 1] = s * c[i].x + r * c[i].y;
+                }
+#pragma unroll
+                for (int i = 0; i < V; ++i) { p[i] = z[i]; q[i] = z[V + i]; }
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const float r = p[i], s = q[i];
+                    p[i] = r * c[i].x - s * c[i].y;
+                    q[i] = s * c[i].x + r * c[i].y;
+                }
+            }
+        }
+        ops::storev<V>(y, at + e0, a.dt, p);
+        if (second) ops::storev<V>(y, at + e1, a.dt, q);
+    }
+};
+
 template <int V>
 __global__ __launch_bounds__(NT) void rotary_kernel(const Args a) {
     extern __shared__ float2 cs[];  // [tok][R / 2]
+    __shared__ int64_t from[MAX_TOK][2];
     const int tid = threadIdx.x, half = a.R / 2;
     const int64_t t0 = (int64_t)blockIdx.x * a.tok;
     const int ntok = (int)min((int64_t)a.tok, a.tokens - t0);
+    if (tid < ntok) {
+        const int64_t b = (t0 + tid) / a.T, t = (t0 + tid) % a.T;
+        for (int w = 0; w < 2; ++w) from[tid][w] = b * a.sb[w] + t * a.st[w];
+    }
     for (int i = tid; i < ntok * half; i += NT) {
-        const int64_t tok = t0 + i / half;
-        const int64_t at = (tok / a.T) * a.psb + (tok % a.T) * a.pst;
+        const int tk = i / half;
+        const int64_t b = (t0 + tk) / a.T, at = b * a.psb + (t0 + tk - b * a.T) * a.pst;
         const double p = a.pos64 ? (double)static_cast<const int64_t *>(a.pos)[at]
                                  : (double)static_cast<const int32_t *>(a.pos)[at];
-        const double turns = p * a.inv[i % half] * 0.15915494309189533577;  // 1 / 2 pi
+        const double turns = p * a.inv[i - tk * half] * 0.15915494309189533577;  // 1 / 2 pi
         const float f = 2.f * (float)(turns - rint(turns));
         cs[i] = make_float2(a.factor * cospif(f), a.sign * a.factor * sinpif(f));
     }
     __syncthreads();
-    const int lane = tid & (a.lanes - 1), slot = tid / a.lanes, slots = NT / a.lanes;
+    const int lane = tid & (a.lanes - 1), slots = NT / a.lanes;
     const int heads = a.H[0] + a.H[1], turning = a.R / (2 * V);
-    for (int item = slot; item < ntok * heads; item += slots) {
-        const int tk = item / heads, hh = item - tk * heads;
-        const int w = hh >= a.H[0], h = w ? hh - a.H[0] : hh;
-        const int64_t tok = t0 + tk;
-        const int64_t in = (tok / a.T) * a.sb[w] + (tok % a.T) * a.st[w] + h * a.sh[w];
-        const int64_t out = (tok * a.H[w] + h) * a.D;
-        const void *x = a.x[w];
-        void *y = a.y[w];
+    int tk = 0, hh = tid / a.lanes;  // this group's next head
+    const auto skip = [&] {
+        while (hh >= heads && tk < ntok) { hh -= heads; ++tk; }
+    };
+    skip();
+    while (tk < ntok) {
+        int64_t in[2], out[2];
+        int w[2], at[2], n = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            // a group without a second head loads the first again
+            const bool any = tk < ntok;
+            const int k = any ? tk : at[0], g = any ? hh : -1;
+            w[i] = any ? g >= a.H[0] : w[0];
+            const int h = w[i] ? g - a.H[0] : g;
+            in[i] = any ? from[k][w[i]] + h * a.sh[w[i]] : in[0];
+            out[i] = any ? ((t0 + k) * a.H[w[i]] + h) * a.D : out[0];
+            at[i] = k;
+            n += any;
+            hh += slots;
+            skip();
+        }
         for (int u = lane; u < a.units; u += a.lanes) {
-            if (u < turning) {
-                float p[V], q[V];
-                const int e0 = a.interleaved ? 2 * V * u : V * u, e1 = a.interleaved ? e0 + V : e0 + half;
-                ops::loadv<V>(x, in + e0, a.dt, p);
-                ops::loadv<V>(x, in + e1, a.dt, q);
-                const float2 *c = cs + tk * half + V * u;
-                if (a.interleaved) {
-                    float z[2 * V];
-#pragma unroll
-                    for (int i = 0; i < V; ++i) { z[i] = p[i]; z[V + i] = q[i]; }
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const float r = z[2 * i], s = z[2 * i + 1];
-                        z[2 * i] = r * c[i].x - s * c[i].y;
-                        z[2 * i + 1] = s * c[i].x + r * c[i].y;
-                    }
-#pragma unroll
-                    for (int i = 0; i < V; ++i) { p[i] = z[i]; q[i] = z[V + i]; }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const float r = p[i], s = q[i];
-                        p[i] = r * c[i].x - s * c[i].y;
-                        q[i] = s * c[i].x + r * c[i].y;
-                    }
-                }
-                ops::storev<V>(y, out + e0, a.dt, p);
-                ops::storev<V>(y, out + e1, a.dt, q);
-            } else {
-                float p[V];
-                const int e = a.R + (u - turning) * V;
-                ops::loadv<V>(x, in + e, a.dt, p);
-                ops::storev<V>(y, out + e, a.dt, p);
-            }
+            Unit<V> x, y;
+            x.load(a, a.x[w[0]], in[0], u, turning);
+            y.load(a, a.x[w[1]], in[1], u, turning);
+            x.store(a, a.y[w[0]], out[0], cs + at[0] * half + (u < turning ? V * u : 0));
+            if (n == 2) y.store(a, a.y[w[1]], out[1], cs + at[1] * half + (u < turning ? V * u : 0));
         }
     }
 }
@@ -138,10 +171,10 @@ extern "C" int gdn_rotary(const void *q, const void *k, void *q_out, void *k_out
                                     aligned_to(a.x[w], 16) && aligned_to(a.y[w], 16)));
         if (ok) break;
     }
-    a.units = R / (2 * V) + (D - R) / V;
+    a.units = R / (2 * V) + (D - R + 2 * V - 1) / (2 * V);
     a.lanes = 1;
     while (a.lanes < a.units && a.lanes < 64) a.lanes *= 2;
-    a.tok = tokens >= 2048 ? 4 : 1;  // few tokens: a workgroup each
+    a.tok = tokens >= 2048 ? rope::MAX_TOK : 1;  // few tokens: a workgroup each
     const int64_t blocks = (tokens + a.tok - 1) / a.tok;
     if (blocks > 0x7fffffff) return fail(GDN_ERR_UNSUPPORTED, "too many tokens");
     const size_t lds = (size_t)a.tok * (R / 2) * sizeof(float2);

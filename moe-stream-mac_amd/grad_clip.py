@@ -28,14 +28,16 @@ def _dense(t: Array) -> bool:
 
 
 def _check(tensors, norm_type) -> None:
+    """Attribute by attribute over all tensors: a model has hundreds, each of a few microseconds otherwise."""
     if norm_type not in (2.0, math.inf):
         raise ValueError(f"norm_type must be 2 or inf; got {norm_type}")
-    dev = tensors[0].device
-    for t in tensors:
-        if t.dtype not in L.DTYPE_CODE or t.layout != torch.strided:
-            raise ValueError(f"unsupported tensor ({t.dtype}, {t.layout}); use dense float32, bfloat16 or float16")
-        if t.device != dev:
-            raise ValueError("all tensors must be on the same device")
+    if {t.layout for t in tensors} != {torch.strided} or not {t.dtype for t in tensors} <= L.DTYPE_CODE.keys():
+        t = next(t for t in tensors if t.layout != torch.strided or t.dtype not in L.DTYPE_CODE)
+        raise ValueError(f"unsupported tensor ({t.dtype}, {t.layout}); use dense float32, bfloat16 or float16")
+    devices = {t.device for t in tensors}
+    if len(devices) > 1:
+        raise ValueError("all tensors must be on the same device")
+    (dev,) = devices
     if dev.type != "cuda":
         raise RuntimeError("grad_clip runs on a ROCm GPU only; got tensors on " + str(dev))
 
@@ -43,24 +45,24 @@ def _check(tensors, norm_type) -> None:
 def _call(tensors, outs, max_norm, norm_type, eps) -> Array:
     dev, code = tensors[0].device, L.DTYPE_CODE
     n = len(tensors)
-    ptrs, sizes, ints = ctypes.c_void_p * n, ctypes.c_int64 * n, ctypes.c_int * n
-    numel = sizes(*[t.numel() for t in tensors])
+    ptrs = ctypes.c_void_p * n
+    numel = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
     lib = L.load()
     norm = torch.empty((), dtype=torch.float32, device=dev)
     nws = lib.gdn_clip_grad_norm_workspace_bytes(numel, n)
     ws = torch.empty((nws,), dtype=torch.uint8, device=dev)
+    x = ptrs(*[t.data_ptr() for t in tensors])
+    y = None if outs is None else x if outs is tensors else ptrs(*[t.data_ptr() for t in outs])
     with L.on_device(dev):
-        L.check(lib.gdn_clip_grad_norm(ptrs(*[t.data_ptr() for t in tensors]),
-                                       None if outs is None else ptrs(*[t.data_ptr() for t in outs]), numel,
-                                       ints(*[code[t.dtype] for t in tensors]), n, int(norm_type == math.inf),
-                                       float(max_norm), float(eps), norm.data_ptr(), ws.data_ptr(), nws,
-                                       L.stream_handle(dev)))
+        L.check(lib.gdn_clip_grad_norm(x, y, numel, (ctypes.c_int * n)(*[code[t.dtype] for t in tensors]), n,
+                                       int(norm_type == math.inf), float(max_norm), float(eps), norm.data_ptr(),
+                                       ws.data_ptr(), nws, L.stream_handle(dev)))
     return norm
 
 
 def grad_norm(tensors: Iterable[Array], norm_type: float = 2.0) -> Array:
     """The norm over all elements of all tensors: 2 (squares summed in 64 bits) or inf; a float32 scalar on the device."""
-    ts = [t.detach() for t in tensors]
+    ts = list(tensors)
     if not ts:
         return torch.zeros(())
     _check(ts, norm_type)
@@ -73,7 +75,7 @@ def clip_grad_norm(grads: Iterable[Array], max_norm: float, norm_type: float = 2
     and types), and returns the norm over all of them before that, as a float32 scalar on the device.  ``norm_type`` is 2
     or inf.  A NaN in any tensor makes the norm and every result NaN; an infinite norm scales by 0.  Tensors may differ
     in type and have any strides; none may share memory with another that is written.  Not differentiable."""
-    gs = [t.detach() for t in grads]
+    gs = list(grads)
     if not max_norm >= 0:
         raise ValueError(f"max_norm must be >= 0; got {max_norm}")
     if not eps >= 0:
@@ -81,16 +83,18 @@ def clip_grad_norm(grads: Iterable[Array], max_norm: float, norm_type: float = 2
     if not gs:
         return torch.zeros(())
     _check(gs, norm_type)
-    os_ = gs if out is None else [t.detach() for t in out]
-    if out is not None:
-        if len(os_) != len(gs) or any(o.shape != g.shape or o.dtype != g.dtype or o.device != g.device
-                                      for o, g in zip(os_, gs)):
-            raise ValueError("out must hold one tensor of the same shape, type and device for each gradient")
+    os_ = gs if out is None else list(out)
+    if out is not None and ([o.shape for o in os_] != [g.shape for g in gs] or
+                            [o.dtype for o in os_] != [g.dtype for g in gs] or
+                            {o.device for o in os_} != {gs[0].device} or {o.layout for o in os_} != {torch.strided}):
+        raise ValueError("out must hold one tensor of the same shape, type and device for each gradient")
+    if all([g.is_contiguous() for g in gs]) and (os_ is gs or all([o.is_contiguous() for o in os_])):
+        return _call(gs, os_, max_norm, float(norm_type), eps)
     # memory order does not matter to the kernels where input and output share it; others go through a copy
     src, dst, back = [], [], []
     for g, o in zip(gs, os_):
-        plain = g.is_contiguous() and (o is g or o.is_contiguous())
-        if plain or (_dense(g) and g.stride() == o.stride()):
+        g, o = g.detach(), o.detach()
+        if (g.is_contiguous() and o.is_contiguous()) or (_dense(g) and g.stride() == o.stride()):
             src.append(g)
             dst.append(o)
         else:

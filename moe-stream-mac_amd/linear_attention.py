@@ -51,22 +51,28 @@ def _strides(q: Array, k: Array, v: Array, g: Array):
     return (ctypes.c_int64 * 12)(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *gs)
 
 
+def _forward(q, k, v, g, state, scale):
+    """(y, last), and what the backward needs: (q, k, v, state, saved)."""
+    q, k, v = _channels(q), _channels(k), _channels(v)
+    (B, T, Hk, Dk), (Hv, Dv), dev = q.shape, v.shape[2:], q.device
+    state = None if state is None else state.contiguous()
+    y = torch.empty((B, T, Hv, Dv), dtype=q.dtype, device=dev)
+    last = torch.empty((B, Hv, Dv, Dk), dtype=torch.float32, device=dev)
+    lib = L.load()
+    n = lib.gdn_linatt_saved_bytes(B, T, Hk, Hv, Dk, Dv)
+    saved = torch.empty((n,), dtype=torch.uint8, device=dev)
+    with L.on_device(dev):
+        L.check(lib.gdn_linatt_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), L.ptr(state), y.data_ptr(),
+                                   last.data_ptr(), saved.data_ptr(), n, _strides(q, k, v, g), B, T, Hk, Hv, Dk, Dv, scale,
+                                   L.DTYPE_CODE[q.dtype], L.DTYPE_CODE[g.dtype], L.stream_handle(dev)))
+    return (y, last), (q, k, v, state, saved)
+
+
 class _LinearAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, state, scale):
         ctx.set_materialize_grads(False)
-        q, k, v = _channels(q), _channels(k), _channels(v)
-        (B, T, Hk, Dk), (Hv, Dv), dev = q.shape, v.shape[2:], q.device
-        state = None if state is None else state.contiguous()
-        y = torch.empty((B, T, Hv, Dv), dtype=q.dtype, device=dev)
-        last = torch.empty((B, Hv, Dv, Dk), dtype=torch.float32, device=dev)
-        lib = L.load()
-        n = lib.gdn_linatt_saved_bytes(B, T, Hk, Hv, Dk, Dv)
-        saved = torch.empty((n,), dtype=torch.uint8, device=dev)
-        with L.on_device(dev):
-            L.check(lib.gdn_linatt_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), L.ptr(state), y.data_ptr(),
-                                       last.data_ptr(), saved.data_ptr(), n, _strides(q, k, v, g), B, T, Hk, Hv, Dk, Dv, scale,
-                                       L.DTYPE_CODE[q.dtype], L.DTYPE_CODE[g.dtype], L.stream_handle(dev)))
+        (y, last), (q, k, v, state, saved) = _forward(q, k, v, g, state, scale)
         ctx.save_for_backward(q, k, v, g, state, last, saved)
         ctx.scale = scale
         return y, last
@@ -110,7 +116,10 @@ def linear_attention(q: Array, k: Array, v: Array, g: Array, state: Optional[Arr
         B, (Hv, Dv) = q.shape[0], v.shape[2:]
         last = q.new_zeros((B, Hv, Dv, q.shape[-1]), dtype=torch.float32) if state is None else state.float().clone()
         return v.new_empty((*q.shape[:2], Hv, Dv)), last
-    return _LinearAttention.apply(q, k, v, g, None if state is None else state.float(), scale)
+    state = None if state is None else state.float()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, state)):
+        return _LinearAttention.apply(q, k, v, g, state, scale)
+    return _forward(q, k, v, g, state, scale)[0]
 
 
 def linear_attention_step(q: Array, k: Array, v: Array, g: Array, state: Array, *,

@@ -102,5 +102,7 @@ def rotary(q: Array, k: Array, positions: Array, inv_freq: Array, *, interleaved
         raise RuntimeError("rotary runs on a ROCm GPU only; got tensors on " + str(q.device))
     if any(t.device != q.device for t in (k, positions, inv_freq)):
         raise ValueError("all inputs must be on the same device")
-    return _Rotary.apply(q, k, positions, inv_freq.detach().to(torch.float64).contiguous(), bool(interleaved),
-                         float(factor))
+    inv = inv_freq.detach().to(torch.float64).contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+        return _Rotary.apply(q, k, positions, inv, bool(interleaved), float(factor))
+    return _launch(q, k, positions, inv, bool(interleaved), float(factor), False)
