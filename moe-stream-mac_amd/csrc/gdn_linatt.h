@@ -11,9 +11,9 @@
 // dg_t is what the loss draws from everything before t through everything from t on.  In t's chunk, with a_r = q_r . (dq_r
 // from the state entering it), b_s = k_s . (dk_s from the cotangent of the state leaving it) and M_rs = P_rs (dy_r . v_s):
 //   dg_t = c + sum_{r >= t} a_r + sum_{s < t} b_s + sum_{r >= t > s} M_rs,   c = e^{G_C} <dS', S>,
-// sums without cancellation, and c by the chain c = D - sum b, D of the chunk before = c + sum a, from D = <dS_T, S_T> on.  A
-// chunk whose decay is below 2^-30 starts the chain anew with c = 0, which is nearer than the difference of two fp32 sums:
-// rounding errors do not outlive what they belong to.
+// sums without cancellation, and c by the chain c = D - sum b, D of the chunk before = c + sum a, from D = <dS_T, S_T> on.  So
+// that rounding errors do not outlive what they belong to, every segment (below) starts from a D of its own, the product of the
+// states at its end, and a chunk whose decay is below 2^-30 from c = 0, which is nearer than the difference of two fp32 sums.
 // So one kernel, pass_kernel, computes all four.  Where there are few heads, the sequence is cut into segments: seg_kernel
 // sums each segment's state from nothing, scan_kernel joins them to the states entering each segment, and the passes run all
 // segments at once.
@@ -366,21 +366,21 @@ struct Pass {
 template <typename ET, int D>
 constexpr bool p_over_q() { return std::is_same_v<ET, float> && D > 128; }
 
-// G: heads to a workgroup, four waves each, that share V'.
-template <typename ET, int D, int NV, int KIND, int G>
+// G: heads to a workgroup, NW waves each, that share V'.
+template <typename ET, int D, int NV, int NW, int KIND, int G>
 struct Shared {
     using LK = Lds<ET, D>;        // tiles Q' and K'
-    using LV = Lds<ET, 64 * NV>;  // V' and X
+    using LV = Lds<ET, 16 * NV * NW>;  // V' and X
     using LP = Lds<ET, C>;        // P
     static constexpr bool TAKEN = p_over_q<ET, D>(), DOT = KIND == DQ || KIND == DK;
-    static constexpr int SUM = 4 * NV * NT;  // float4s of a head's outputs
+    static constexpr int SUM = 4 * NV * 64 * NW;  // float4s of a head's outputs
     ET Q[G][C * LK::LD], K[G][C * LK::LD], V[C * LV::LD];
     ET own_p[G][TAKEN ? 8 : C * LP::LD], own_x[KIND == DV && !TAKEN ? C * LV::LD : 8];
     Decays d[G];
-    float total[G], dot[DOT ? G : 1][DOT ? 4 : 1][DOT ? C : 1];
+    float total[G], dot[DOT ? G : 1][DOT ? NW : 1][DOT ? C : 1];
     static constexpr bool SUM_OVER_Q = SUM * sizeof(float4) <= G * C * LK::LD * sizeof(ET);
     float4 own_sum[G == 2 && !SUM_OVER_Q ? SUM : 1];
-    // where Q' was, once it is used: the waves' sums of M, [4][C]
+    // where Q' was, once it is used: the waves' sums of M, [NW][C]
     __device__ __forceinline__ double *cross() { return reinterpret_cast<double *>(Q[0] + (TAKEN ? C * LP::LD + C * LV::LD : 0)); }
     __device__ __forceinline__ ET *p(int i) { return TAKEN ? Q[0] : own_p[i]; }
     __device__ __forceinline__ ET *x() { return TAKEN ? Q[0] + C * LP::LD : own_x; }
@@ -389,12 +389,12 @@ struct Shared {
 
 // The state of a wave: K' rows 32 T + 8 (l / 16) + 4 (t & 1) + e of tile t = 2 T, 2 T + 1 by its columns 16 NV w + ...: what
 // lane l holds of two tiles is 8 consecutive K' rows of one column, an operand as it stands.
-template <int D, int NV>
+template <int D, int NV, int NW>
 struct State {
     f4 s[D / 16][NV];
     // the lane's column of tile n
     static __device__ __forceinline__ int col(int n) {
-        const int l = threadIdx.x & 63, li = l & 15, w = (threadIdx.x >> 6) & 3;
+        const int l = threadIdx.x & 63, li = l & 15, w = (threadIdx.x >> 6) & (NW - 1);
         return 16 * NV * w + 4 * NV * (li >> 2) + 4 * n + (li & 3);
     }
     // p: [v'][k'], or with tr [k'][v']; out of range (and without p) zeros
@@ -468,37 +468,37 @@ __device__ __forceinline__ Block block(int e) {
 // stay on one.
 __device__ __forceinline__ int xcd_order(int i, int n) { return n % 8 == 0 ? (i % 8) * (n / 8) + i / 8 : i; }
 
-// Waves to a SIMD: two where a wave's state, tiles and sums fit 256 registers.
+// Waves to a SIMD that the registers have to allow.
 template <typename ET, int D>
 constexpr int waves() { return std::is_same_v<ET, bf16> && D <= 128 ? 2 : 1; }
 
 // One segment of G value heads, 64 NV columns of V'.
-template <typename ET, int D, int NV, int KIND, int G, bool VEC>
-__global__ __launch_bounds__(NT * G, (waves<ET, D>())) void pass_kernel(const Pass a) {
+template <typename ET, int D, int NV, int NW, int KIND, int G, bool VEC>
+__global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(const Pass a) {
     constexpr bool F32 = std::is_same_v<ET, float>, REV = KIND >= DK, DOT = KIND == DQ || KIND == DK;
     constexpr int NS = F32 ? 1 : 3, NH = F32 || !DOT ? 1 : 2;  // terms of the weighted V', of the state as an operand
     constexpr int RT = C / 16;
     using LK = Lds<ET, D>;
-    using LV = Lds<ET, 64 * NV>;
+    using LV = Lds<ET, 16 * NV * NW>;
     using LP = Lds<ET, C>;
-    constexpr bool TAKEN = Shared<ET, D, NV, KIND, G>::TAKEN;
-    __shared__ __attribute__((aligned(16))) Shared<ET, D, NV, KIND, G> sh;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3, grp = wave >> 2;
+    constexpr bool TAKEN = Shared<ET, D, NV, NW, KIND, G>::TAKEN;
+    __shared__ __attribute__((aligned(16))) Shared<ET, D, NV, NW, KIND, G> sh;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & (NW - 1), grp = wave / NW;
     int id = xcd_order(blockIdx.x, gridDim.x);
     const int slice = id % a.slices;
     id /= a.slices;
     const int hg = id % (a.Hv / G), h = hg * G + grp;
     id /= a.Hv / G;
-    const int b = id % a.B, seg = id / a.B, c0 = slice * 64 * NV;
+    const int b = id % a.B, seg = id / a.B, c0 = slice * 16 * NV * NW;
     const int first = seg * a.cps, last = min(a.nc, first + a.cps) - 1;
     const int64_t head = (int64_t)b * a.Hv + h;
 
-    State<D, NV> S;
+    State<D, NV, NW> S;
     S.load(a.s_in ? a.s_in + head * a.s_head + seg * a.s_seg : nullptr, a.dk, a.dv, c0, a.s_t);
 
-    Tile<ET, D, VEC> tq, tk;
-    Tile<ET, 64 * NV, VEC, NT * G> tv;
-    Tile<ET, 64 * NV, VEC> tx;
+    Tile<ET, D, VEC, 64 * NW> tq, tk;
+    Tile<ET, 16 * NV * NW, VEC, 64 * NW * G> tv;
+    Tile<ET, 16 * NV * NW, VEC, 64 * NW> tx;
     float td = 0.f;
     const auto fetch = [&](int c) {
         const int64_t t0 = (int64_t)c * C;
@@ -531,7 +531,7 @@ __global__ __launch_bounds__(NT * G, (waves<ET, D>())) void pass_kernel(const Pa
         tk.store(sh.K[grp], n, a.dk, a.dt);
         tv.store(sh.V, n, a.dv - c0, a.dt);
         // the scale goes with e^{G_r}: into the outputs, reverse into the sources
-        reinterpret_cast<float *>(&sh.d[grp])[tid & (NT - 1)] = w == 2 ? td * a.scale : td;
+        reinterpret_cast<float *>(&sh.d[grp])[tid & (NT - 1)] = (w & 3) == 2 ? td * a.scale : td;
         if (w == 2 && l == C - 1) sh.total[grp] = td;
         __syncthreads();
         // X before the next tiles: loads are waited for in their order
@@ -598,15 +598,21 @@ __global__ __launch_bounds__(NT * G, (waves<ET, D>())) void pass_kernel(const Pa
         // P: blocks (rt, st) of 16 outputs by 16 sources with st <= rt (reverse: >=), one to a wave in turn; the blocks that
         // fill a product's 32 sources are zeros
         ET *const sP = sh.p(grp);
-        f4 acc[3];
+        constexpr int BLOCKS = (10 + NW - 1) / NW;
+        f4 acc[BLOCKS] = {};
 #pragma unroll
-        for (int e = 0; e < 3; ++e) {
-            const Block k = block<REV>(w + 4 * e);
-            if (!k.in) continue;
-            acc[e] = f4{0.f, 0.f, 0.f, 0.f};
+        for (int x = 0; x < D; x += 32)
+#pragma unroll
+            for (int e = 0; e < BLOCKS - 1; ++e) {
+                const Block k = block<REV>(w + NW * e);
+                acc[e] = mma(row_frag<LK>(sh.K[grp], lk, k.s0, x), row_frag<LK>(sh.Q[grp], lk, k.r0, x), acc[e]);
+            }
+        if (w < 2) {
+            constexpr int E = BLOCKS - 1;
+            const Block k = block<REV>(8 + w);
 #pragma unroll
             for (int x = 0; x < D; x += 32)
-                acc[e] = mma(row_frag<LK>(sh.K[grp], lk, k.s0, x), row_frag<LK>(sh.Q[grp], lk, k.r0, x), acc[e]);
+                acc[E] = mma(row_frag<LK>(sh.K[grp], lk, k.s0, x), row_frag<LK>(sh.Q[grp], lk, k.r0, x), acc[E]);
         }
         if constexpr (TAKEN) {
             __syncthreads();
@@ -618,8 +624,8 @@ __global__ __launch_bounds__(NT * G, (waves<ET, D>())) void pass_kernel(const Pa
             else *reinterpret_cast<uint2 *>(o) = *reinterpret_cast<const uint2 *>(p);
         };
 #pragma unroll
-        for (int e = 0; e < 3; ++e) {
-            const Block k = block<REV>(w + 4 * e);
+        for (int e = 0; e < BLOCKS; ++e) {
+            const Block k = block<REV>(w + NW * e);
             if (!k.in) continue;
             const int r = k.r0 + li, s0 = k.s0 + 4 * g;
             const float2 gr = sh.d[grp].G[r];
@@ -648,12 +654,12 @@ __global__ __launch_bounds__(NT * G, (waves<ET, D>())) void pass_kernel(const Pa
             double *cross = sh.cross() + w * C;
             cross[l] = 0.;
 #pragma unroll
-            for (int e = 0; e < 3; ++e) {
-                const Block k = block<REV>(w + 4 * e);
+            for (int e = 0; e < BLOCKS; ++e) {
+                const Block k = block<REV>(w + NW * e);
                 if (!k.in) continue;
                 f4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < 64 * NV; i += 32)
+                for (int i = 0; i < 16 * NV * NW; i += 32)
                     x = mma(row_frag<LV>(sh.V, lv, k.s0, i), row_frag<LV>(sh.x(), lv, k.r0, i), x);
                 double out = 0.;
 #pragma unroll
@@ -703,7 +709,7 @@ __global__ __launch_bounds__(NT * G, (waves<ET, D>())) void pass_kernel(const Pa
                 for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                     for (int x = 0; x < NV; ++x)
-                        sum[(rt * NV + x) * NT] = make_float4(O[rt][x][0], O[rt][x][1], O[rt][x][2], O[rt][x][3]);
+                        sum[(rt * NV + x) * 64 * NW] = make_float4(O[rt][x][0], O[rt][x][1], O[rt][x][2], O[rt][x][3]);
             }
             __syncthreads();
             if (grp == 0) {
@@ -711,7 +717,7 @@ __global__ __launch_bounds__(NT * G, (waves<ET, D>())) void pass_kernel(const Pa
                 for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
                     for (int x = 0; x < NV; ++x) {
-                        const float4 y = sum[(rt * NV + x) * NT];
+                        const float4 y = sum[(rt * NV + x) * 64 * NW];
                         O[rt][x] += f4{y.x, y.y, y.z, y.w};
                     }
             }
@@ -735,15 +741,21 @@ __global__ __launch_bounds__(NT * G, (waves<ET, D>())) void pass_kernel(const Pa
         const int64_t at = (((int64_t)slice * a.B + b) * a.Hv + h) * a.T + t0;
         if constexpr (DOT) {
             __syncthreads();
-            const float(&d)[4][C] = sh.dot[grp];
-            if (w == 0 && l < n) a.dot[at + l] = (d[0][l] + d[1][l]) + (d[2][l] + d[3][l]);
+            if (w == 0 && l < n) {
+                float d = 0.f;
+#pragma unroll
+                for (int i = 0; i < NW; ++i) d += sh.dot[grp][i][l];
+                a.dot[at + l] = d;
+            }
         }
         if constexpr (KIND == DV) {
             __syncthreads();
             if (w == 0) {
                 const int t = C - 1 - l;
                 const double *const x0 = sh.cross() + t;
-                const double x = (x0[0] + x0[C]) + (x0[2 * C] + x0[3 * C]);
+                double x = 0.;
+#pragma unroll
+                for (int i = 0; i < NW; ++i) x += x0[i * C];
                 const double s = wave_prefix_sum(x);
                 if (t < n) a.dot[at + t] = (float)s;
             }
@@ -763,11 +775,11 @@ struct Seg {
 
 // What a segment adds to a state that starts from nothing, and its decay.  The segment that the chain ends with is left out
 // (the last; reverse: the first).
-template <typename ET, int D, int NV, bool REV, bool VEC>
-__global__ __launch_bounds__(NT, (waves<ET, D>())) void seg_kernel(const Seg a) {
+template <typename ET, int D, int NV, int NW, bool REV, bool VEC>
+__global__ __launch_bounds__(64 * NW, (waves<ET, D>())) void seg_kernel(const Seg a) {
     constexpr int NS = std::is_same_v<ET, float> ? 1 : 3;
     using LK = Lds<ET, D>;
-    using LV = Lds<ET, 64 * NV>;
+    using LV = Lds<ET, 16 * NV * NW>;
     __shared__ __attribute__((aligned(16))) ET sK[C * LK::LD];
     __shared__ __attribute__((aligned(16))) ET sV[C * LV::LD];
     __shared__ Decays d;
@@ -778,19 +790,19 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void seg_kernel(const Seg a) 
     id /= a.slices;
     const int h = id % a.Hv;
     id /= a.Hv;
-    const int b = id % a.B, seg = id / a.B + (REV ? 1 : 0), c0 = slice * 64 * NV;
+    const int b = id % a.B, seg = id / a.B + (REV ? 1 : 0), c0 = slice * 16 * NV * NW;
     const int first = seg * a.cps, last = min(a.nc, first + a.cps) - 1;
-    State<D, NV> S;
+    State<D, NV, NW> S;
     S.load(nullptr, a.dk, a.dv, c0, 0);
-    Tile<ET, D, VEC> tk;
-    Tile<ET, 64 * NV, VEC> tv;
+    Tile<ET, D, VEC, 64 * NW> tk;
+    Tile<ET, 16 * NV * NW, VEC, 64 * NW> tv;
     float td = 0.f, all = 1.f;
     const auto fetch = [&](int c) {
         const int64_t t0 = (int64_t)c * C;
         const int n = min((int64_t)C, a.T - t0);
         tk.fetch(a.K.from(b, t0, h, 0, a.dt), a.K.st, n, a.dk, a.dt);
         tv.fetch(a.V.from(b, t0, h, c0, a.dt), a.V.st, n, a.dv - c0, a.dt);
-        td = a.decays[(((int64_t)b * a.Hv + h) * a.nc + c) * DECAYS + tid];
+        td = a.decays[(((int64_t)b * a.Hv + h) * a.nc + c) * DECAYS + (tid & (NT - 1))];
     };
     fetch(REV ? last : first);
     for (int i = first; i <= last; ++i) {
@@ -798,7 +810,7 @@ __global__ __launch_bounds__(NT, (waves<ET, D>())) void seg_kernel(const Seg a) 
         __syncthreads();
         tk.store(sK, n, a.dk, a.dt);
         tv.store(sV, n, a.dv - c0, a.dt);
-        reinterpret_cast<float *>(&d)[tid] = REV && w == 2 ? td * a.scale : td;
+        reinterpret_cast<float *>(&d)[tid & (NT - 1)] = REV && (w & 3) == 2 ? td * a.scale : td;
         if (w == 2 && l == C - 1) sum = td;
         __syncthreads();
         if (i < last) fetch(REV ? c - 1 : c + 1);
@@ -842,41 +854,48 @@ GDN_LINATT_DECLARE(odd128)
 GDN_LINATT_DECLARE(odd256)
 
 // VEC: all heads' channels are a multiple of 8.
-template <typename ET, int D, int NV, bool VEC>
+template <typename ET, int D, int NV, int NW, bool VEC>
 void launch_pass(const Pass &a, Kind kind, hipStream_t st) {
     const dim3 grid((unsigned)((int64_t)a.slices * a.Hv * a.B * a.nseg / (a.pair ? 2 : 1)));
     if constexpr (pairs<ET, D>()) {
         if (a.pair) {
-            const dim3 block(2 * NT);
-            if (kind == DQ) hipLaunchKernelGGL((pass_kernel<ET, D, NV, DQ, 2, VEC>), grid, block, 0, st, a);
-            else hipLaunchKernelGGL((pass_kernel<ET, D, NV, DK, 2, VEC>), grid, block, 0, st, a);
+            const dim3 block(128 * NW);
+            if (kind == DQ) hipLaunchKernelGGL((pass_kernel<ET, D, NV, NW, DQ, 2, VEC>), grid, block, 0, st, a);
+            else hipLaunchKernelGGL((pass_kernel<ET, D, NV, NW, DK, 2, VEC>), grid, block, 0, st, a);
             return;
         }
     }
-    if (kind == Y) hipLaunchKernelGGL((pass_kernel<ET, D, NV, Y, 1, VEC>), grid, dim3(NT), 0, st, a);
-    else if (kind == DQ) hipLaunchKernelGGL((pass_kernel<ET, D, NV, DQ, 1, VEC>), grid, dim3(NT), 0, st, a);
-    else if (kind == DK) hipLaunchKernelGGL((pass_kernel<ET, D, NV, DK, 1, VEC>), grid, dim3(NT), 0, st, a);
-    else hipLaunchKernelGGL((pass_kernel<ET, D, NV, DV, 1, VEC>), grid, dim3(NT), 0, st, a);
+    const dim3 block(64 * NW);
+    if (kind == Y) hipLaunchKernelGGL((pass_kernel<ET, D, NV, NW, Y, 1, VEC>), grid, block, 0, st, a);
+    else if (kind == DQ) hipLaunchKernelGGL((pass_kernel<ET, D, NV, NW, DQ, 1, VEC>), grid, block, 0, st, a);
+    else if (kind == DK) hipLaunchKernelGGL((pass_kernel<ET, D, NV, NW, DK, 1, VEC>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((pass_kernel<ET, D, NV, NW, DV, 1, VEC>), grid, block, 0, st, a);
 }
-template <typename ET, int D, int NV, bool VEC>
+template <typename ET, int D, int NV, int NW, bool VEC>
 void launch_seg(const Seg &a, bool rev, hipStream_t st) {
-    const dim3 grid((unsigned)((int64_t)a.slices * a.Hv * a.B * (a.nseg - 1)));
-    if (rev) hipLaunchKernelGGL((seg_kernel<ET, D, NV, true, VEC>), grid, dim3(NT), 0, st, a);
-    else hipLaunchKernelGGL((seg_kernel<ET, D, NV, false, VEC>), grid, dim3(NT), 0, st, a);
+    const dim3 grid((unsigned)((int64_t)a.slices * a.Hv * a.B * (a.nseg - 1))), block(64 * NW);
+    if (rev) hipLaunchKernelGGL((seg_kernel<ET, D, NV, NW, true, VEC>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((seg_kernel<ET, D, NV, NW, false, VEC>), grid, block, 0, st, a);
 }
+// 128 columns of V' go to four waves of 32 in bf16 (eight of 16 read the K' and Q' tiles twice as often: 171 us against 144
+// for two sequences of 8100 tokens, 32 heads), to eight of 16 in fp32 (two waves to a SIMD: 83 us against 87 for 2047 tokens).
+template <typename ET>
+constexpr int wide_columns() { return std::is_same_v<ET, bf16> ? 2 : 1; }
 template <typename ET, int D, bool VEC>
 void launch_pass_cols(const Pass &a, Kind kind, hipStream_t st) {
     if constexpr (D <= 128) {
-        if (cols_of(D, a.dv) == 128) return launch_pass<ET, D, 2, VEC>(a, kind, st);
+        constexpr int NV = wide_columns<ET>();
+        if (cols_of(D, a.dv) == 128) return launch_pass<ET, D, NV, 8 / NV, VEC>(a, kind, st);
     }
-    launch_pass<ET, D, 1, VEC>(a, kind, st);
+    launch_pass<ET, D, 1, 4, VEC>(a, kind, st);
 }
 template <typename ET, int D, bool VEC>
 void launch_seg_cols(const Seg &a, bool rev, hipStream_t st) {
     if constexpr (D <= 128) {
-        if (cols_of(D, a.dv) == 128) return launch_seg<ET, D, 2, VEC>(a, rev, st);
+        constexpr int NV = wide_columns<ET>();
+        if (cols_of(D, a.dv) == 128) return launch_seg<ET, D, NV, 8 / NV, VEC>(a, rev, st);
     }
-    launch_seg<ET, D, 1, VEC>(a, rev, st);
+    launch_seg<ET, D, 1, 4, VEC>(a, rev, st);
 }
 #define GDN_LINATT(NAME, D, VEC)                                       \
     void pass_##NAME(const Pass &a, Kind kind, hipStream_t st) {        \

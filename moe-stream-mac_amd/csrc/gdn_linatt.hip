@@ -20,22 +20,49 @@ __global__ __launch_bounds__(NT) void decay_kernel(Gate g, float *o, int B, int 
     const float hi = (float)s;
     float *const p = o + (((int64_t)b * Hv + h) * nc + c) * DECAYS;
     reinterpret_cast<float2 *>(p)[l] = make_float2(hi, (float)(s - (double)hi));
-    p[2 * C + l] = __builtin_amdgcn_exp2f(hi);
-    p[3 * C + l] = __builtin_amdgcn_exp2f((float)(end - s));
+    // rounded once: with one log decay for a whole head their errors repeat in every chunk
+    p[2 * C + l] = (float)exp2(s);
+    p[3 * C + l] = (float)exp2(end - s);
 }
 
-// The segments' sums become the states entering them: from s0 (or nothing) on, in place.
-template <bool REV>
-__global__ __launch_bounds__(NT) void scan_kernel(float *s, const float *decay, const float *s0, int nseg, int64_t size) {
-    const int64_t head = blockIdx.y, i = (int64_t)blockIdx.x * NT + threadIdx.x;
-    if (i >= size) return;
-    float cur = s0 ? s0[head * size + i] : 0.f;
+__device__ __forceinline__ double block_sum(double x, double *red, int waves) {
+    x = readlane_f64(wave_prefix_sum(x), 63);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+    __syncthreads();
+    double r = 0.;
+    for (int i = 0; i < waves; ++i) r += red[i];
+    __syncthreads();
+    return r;
+}
+
+// The segments' sums become the states entering them: from s0 (or nothing) on, in place.  With `at` (reverse), the states
+// entering the segments forwards, also the products of both at the segments' ends, <dS, S>: part [heads][nseg][blocks].
+template <bool REV, int V>
+__global__ __launch_bounds__(NT) void scan_kernel(float *s, const float *decay, const float *s0, const float *at, double *part,
+                                                  int nseg, int64_t size) {
+    __shared__ double red[NT / 64];
+    const int64_t head = blockIdx.y, i = ((int64_t)blockIdx.x * NT + threadIdx.x) * V;
+    const bool in = i < size;
+    float cur[V] = {};
+    if (s0 && in)
+        for (int e = 0; e < V; ++e) cur[e] = s0[head * size + i + e];  // at any alignment
     for (int j = 0; j < nseg; ++j) {
         const int seg = REV ? nseg - 1 - j : j;
-        float *p = s + (head * nseg + seg) * size + i;
-        const float add = j < nseg - 1 ? *p : 0.f, f = j < nseg - 1 ? decay[head * nseg + seg] : 0.f;
-        *p = cur;
-        cur = fmaf(f, cur, add);
+        const int64_t p = (head * nseg + seg) * size + i;
+        const float f = j < nseg - 1 ? decay[head * nseg + seg] : 0.f;
+        float add[V] = {}, S[V] = {};
+        if (j < nseg - 1 && in) ops::loadv<V>(s, p, DT_F32, add);
+        if (in) ops::storev<V>(s, p, DT_F32, cur);
+        if (REV && at && j > 0) {  // the last segment's end is the sequence's
+            if (in) ops::loadv<V>(at, p + size, DT_F32, S);
+            double x = 0.;
+#pragma unroll
+            for (int e = 0; e < V; ++e) x = fma((double)cur[e], (double)S[e], x);
+            x = block_sum(x, red, NT / 64);
+            if (threadIdx.x == 0) part[(head * nseg + seg) * gridDim.x + blockIdx.x] = x;
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) cur[e] = fmaf(f, cur[e], add[e]);
     }
 }
 
@@ -54,28 +81,19 @@ struct DecayGrad {
     const float *a, *b, *cross;  // [slices][B][Hv][T]; cross: [cross_slices]
     const float *decays;         // [B][Hv][nc][DECAYS]
     const float *dlast, *last;   // [B][Hv][size], or dlast NULL
+    const double *ends;          // <dS, S> at the segments' ends but the last, [B][Hv][nseg][blocks]
     void *dg;                    // [B][T][Hv], or [Hv]
-    int B, T, Hv, slices, cross_slices, per_head, dt, nc;
+    int B, T, Hv, slices, cross_slices, per_head, dt, nc, cps, nseg, blocks;
     int64_t size;
 };
 
 constexpr int DW = 16;  // waves
 
-__device__ __forceinline__ double block_sum(double x, double *red) {
-    x = readlane_f64(wave_prefix_sum(x), 63);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
-    __syncthreads();
-    double r = 0.;
-    for (int i = 0; i < DW; ++i) r += red[i];
-    __syncthreads();
-    return r;
-}
-
 // dg of one value head, from the end of each sequence backwards, in 64 bits: a wave sums one chunk, the chunks chain.  grid
 // (Hv, B), or (Hv) per head.
 __global__ __launch_bounds__(64 * DW) void dg_kernel(const DecayGrad a) {
-    __shared__ double sumA[DW], sumB[DW], red[DW];
-    __shared__ int anew[DW];
+    __shared__ double sumA[DW], sumB[DW], own[DW], red[DW];
+    __shared__ int anew[DW], ends[DW];
     const int h = blockIdx.x, l = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int64_t heads = (int64_t)a.B * a.Hv;
     double sum = 0.;
@@ -85,7 +103,7 @@ __global__ __launch_bounds__(64 * DW) void dg_kernel(const DecayGrad a) {
         if (a.dlast) {
             for (int64_t i = threadIdx.x; i < a.size; i += 64 * DW)
                 D = fma((double)a.dlast[head * a.size + i], (double)a.last[head * a.size + i], D);
-            D = block_sum(D, red);
+            D = block_sum(D, red, DW);
         }
         for (int c1 = a.nc - 1; c1 >= 0; c1 -= DW) {
             const int c = c1 - w;  // later chunks in lower waves, later tokens in lower lanes
@@ -102,7 +120,16 @@ __global__ __launch_bounds__(64 * DW) void dg_kernel(const DecayGrad a) {
             xa = wave_prefix_sum(xa);
             xb = wave_prefix_sum(xb);
             const double B = readlane_f64(xb, 63);
+            const int seg = c / a.cps;
+            const bool end = c >= 0 && seg < a.nseg - 1 && (c + 1) % a.cps == 0;
+            double e = 0.;
+            if (end) {
+                for (int i = l; i < a.blocks; i += 64) e += a.ends[(head * a.nseg + seg) * a.blocks + i];
+                e = wave_prefix_sum(e);
+            }
             if (l == 63) {
+                ends[w] = end;
+                own[w] = e;
                 sumA[w] = xa;
                 sumB[w] = xb;
                 anew[w] = c >= 0 && a.decays[(head * a.nc + c) * DECAYS + 3 * C - 1] < 0x1p-30f;  // e^{G_C}
@@ -110,6 +137,7 @@ __global__ __launch_bounds__(64 * DW) void dg_kernel(const DecayGrad a) {
             __syncthreads();
             double mine = 0.;
             for (int i = 0; i < DW; ++i) {
+                if (ends[i]) D = own[i];
                 const double c0 = anew[i] ? 0. : D - sumB[i];
                 if (i == w) mine = c0;
                 D = c0 + sumA[i];
@@ -123,7 +151,7 @@ __global__ __launch_bounds__(64 * DW) void dg_kernel(const DecayGrad a) {
         }
     }
     if (a.per_head) {
-        sum = block_sum(sum, red);
+        sum = block_sum(sum, red, DW);
         if (threadIdx.x == 0) store_from_f32(a.dg, h, (float)sum, a.dt);
     }
 }
@@ -207,8 +235,10 @@ static int run_pass(Pass a, Kind kind, hipStream_t st) {
 }
 
 // The states entering each segment (nseg > 1), from s0 on (reverse: the cotangents, from the end).
+static int scan_width(int64_t size) { return size % 4 ? 1 : 4; }
+static int scan_blocks(int64_t size) { return (int)((size + NT * scan_width(size) - 1) / (NT * scan_width(size))); }
 template <bool REV>
-static int run_segments(Seg a, const float *s0, hipStream_t st) {
+static int run_segments(Seg a, const float *s0, const float *at, double *part, hipStream_t st) {
     a.slices = slices_of(a.dk, a.dv);
     {
         Timed tm(REV ? "linatt_segments_rev" : "linatt_segments", st);
@@ -220,14 +250,17 @@ static int run_segments(Seg a, const float *s0, hipStream_t st) {
     const int64_t size = (int64_t)a.dk * a.dv;
     {
         Timed tm("linatt_scan", st);
-        hipLaunchKernelGGL(scan_kernel<REV>, dim3((unsigned)((size + NT - 1) / NT), (unsigned)(a.B * a.Hv)), dim3(NT), 0, st,
-                           a.s, a.decay, s0, a.nseg, size);
+        const dim3 grid((unsigned)scan_blocks(size), (unsigned)(a.B * a.Hv));
+        if (scan_width(size) == 4)
+            hipLaunchKernelGGL((scan_kernel<REV, 4>), grid, dim3(NT), 0, st, a.s, a.decay, s0, at, part, a.nseg, size);
+        else
+            hipLaunchKernelGGL((scan_kernel<REV, 1>), grid, dim3(NT), 0, st, a.s, a.decay, s0, at, part, a.nseg, size);
     }
     return check_launch(st, "linear attention (scan)");
 }
 
 struct Sizes {
-    size_t decays, state, decay, saved, part, dot, cross, bwd;
+    size_t decays, state, decay, saved, part, dot, cross, ends, bwd;
 };
 // value heads of a key head whose dq and dk are added after the passes: all, or the pairs of pair_heads()
 static bool pair_heads(int r, int Dv, int dtype) { return dtype == DT_BF16 && Dv <= 128 && r % 2 == 0; }
@@ -246,7 +279,8 @@ static Sizes sizes(int B, int T, int Hk, int Hv, int Dk, int Dv, int dtype = DT_
     const size_t rows = (size_t)B * Hv * T * sizeof(float);
     s.dot = align_up256(rows * slices_of(Dv, Dk));
     s.cross = align_up256(rows * slices_of(Dk, Dv));
-    s.bwd = s.state + s.decay + s.part + 2 * s.dot + s.cross;
+    if (p.nseg > 1) s.ends = align_up256((size_t)B * Hv * p.nseg * scan_blocks((int64_t)Dk * Dv) * sizeof(double));
+    s.bwd = s.state + s.decay + s.part + 2 * s.dot + s.cross + s.ends;
     return s;
 }
 
@@ -321,7 +355,7 @@ extern "C" int gdn_linatt_fwd(const void *q, const void *k, const void *v, const
     p.s_out = state_T;
     if (pl.nseg > 1) {
         const la::Seg a{p.K, p.V, decays, states, seg_decay, B, T, Hv, Dk, Dv, 0, pl.nseg, pl.cps, pl.nc, dtype, scale};
-        rc = la::run_segments<false>(a, state0, st);
+        rc = la::run_segments<false>(a, state0, nullptr, nullptr, st);
         if (rc) return rc;
         p.s_in = states;
         p.s_seg = p.s_head;
@@ -358,6 +392,7 @@ extern "C" int gdn_linatt_bwd(const void *q, const void *k, const void *v, const
     };
     float *ds = take(sz.state), *decay = take(sz.decay), *part = take(sz.part);
     float *sa = take(sz.dot), *sb = take(sz.dot), *cross = take(sz.cross);
+    double *ends = reinterpret_cast<double *>(take(sz.ends));
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int r = Hv / Hk;
     const int64_t dys[3] = {(int64_t)T * Hv * Dv, (int64_t)Hv * Dv, Dv}, size = (int64_t)Dk * Dv;
@@ -397,7 +432,7 @@ extern "C" int gdn_linatt_bwd(const void *q, const void *k, const void *v, const
     const float *s_in = dstate_T;
     if (pl.nseg > 1) {
         const la::Seg a{tq, tdy, decays, ds, decay, B, T, Hv, Dk, Dv, 0, pl.nseg, pl.cps, pl.nc, dtype, scale};
-        rc = la::run_segments<true>(a, dstate_T, st);
+        rc = la::run_segments<true>(a, dstate_T, states, ends, st);
         if (rc) return rc;
         s_in = ds;
     }
@@ -418,8 +453,8 @@ extern "C" int gdn_linatt_bwd(const void *q, const void *k, const void *v, const
     p.s_out = dstate0;
     rc = la::run_pass(p, la::DV, st);
     if (rc) return rc;
-    const la::DecayGrad d{sa, sb, cross, decays, dstate_T, state_T, dg, B, T, Hv, la::slices_of(Dv, Dk), la::slices_of(Dk, Dv),
-                          g_per_head != 0, g_dtype, pl.nc, size};
+    const la::DecayGrad d{sa, sb, cross, decays, dstate_T, state_T, ends, dg, B, T, Hv, la::slices_of(Dv, Dk),
+                          la::slices_of(Dk, Dv), g_per_head != 0, g_dtype, pl.nc, pl.cps, pl.nseg, la::scan_blocks(size), size};
     {
         Timed tm("linatt_dg", st);
         hipLaunchKernelGGL(la::dg_kernel, dim3((unsigned)Hv, g_per_head ? 1u : (unsigned)B), dim3(64 * la::DW), 0,
