@@ -31,13 +31,13 @@ struct Args {
     const double *inv;
     float factor, sign;
     int64_t tokens;        // B * T
-    int T, D, R, interleaved, dt, tok, units, lanes;
+    int T, D, R, interleaved, tok, units, lanes;
 };
 
 // A unit is 2 V channels: V pairs that turn, or as many that pass.  `lanes` (a power of two) lanes walk the units of one head;
 // a workgroup takes `tok` tokens, whose places in memory are worked out once, and its groups of lanes two heads at a time,
 // loads first: 16 bytes times four under way for each lane.
-template <int V>
+template <int V, int DT>
 struct Unit {
     float p[V], q[V];
     int e0, e1;
@@ -47,8 +47,8 @@ struct Unit {
         e0 = turns ? (a.interleaved ? 2 * V * u : V * u) : a.R + (u - turning) * 2 * V;
         e1 = turns && !a.interleaved ? e0 + a.R / 2 : e0 + V;
         second = e1 < a.D;
-        ops::loadv<V>(x, at + e0, a.dt, p);
-        ops::loadv<V>(x, at + (second ? e1 : e0), a.dt, q);
+        ops::loadv<V>(x, at + e0, DT, p);
+        ops::loadv<V>(x, at + (second ? e1 : e0), DT, q);
     }
     __device__ __forceinline__ void store(const Args &a, void *y, int64_t at, const float2 *c) {
         if (turns) {
@@ -73,12 +73,12 @@ struct Unit {
                 }
             }
         }
-        ops::storev<V>(y, at + e0, a.dt, p);
-        if (second) ops::storev<V>(y, at + e1, a.dt, q);
+        ops::storev<V>(y, at + e0, DT, p);
+        if (second) ops::storev<V>(y, at + e1, DT, q);
     }
 };
 
-template <int V>
+template <int V, int DT>
 __global__ __launch_bounds__(NT) void rotary_kernel(const Args a) {
     extern __shared__ float2 cs[];  // [tok][R / 2]
     __shared__ int64_t from[MAX_TOK][2];
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(NT) void rotary_kernel(const Args a) {
             skip();
         }
         for (int u = lane; u < a.units; u += a.lanes) {
-            Unit<V> x, y;
+            Unit<V, DT> x, y;
             x.load(a, a.x[w[0]], in[0], u, turning);
             y.load(a, a.x[w[1]], in[1], u, turning);
             x.store(a, a.y[w[0]], out[0], cs + at[0] * half + (u < turning ? V * u : 0));
@@ -161,7 +161,7 @@ extern "C" int gdn_rotary(const void *q, const void *k, void *q_out, void *k_out
     a.H[0] = Hq; a.H[1] = Hk;
     a.pos = positions; a.psb = pos_stride_b; a.pst = pos_stride_t; a.pos64 = positions_64 != 0;
     a.inv = inv_freq; a.factor = factor; a.sign = backward ? -1.f : 1.f;
-    a.tokens = tokens; a.T = T; a.D = D; a.R = R; a.interleaved = interleaved != 0; a.dt = dtype;
+    a.tokens = tokens; a.T = T; a.D = D; a.R = R; a.interleaved = interleaved != 0;
     // channels per load: 16 bytes of 16-bit data where sizes, strides and addresses allow, else 4 channels, else 1
     int V = 8;
     for (; V > 1; V = V == 8 ? 4 : 1) {
@@ -182,9 +182,14 @@ extern "C" int gdn_rotary(const void *q, const void *k, void *q_out, void *k_out
     {
         Timed tm("rotary", st);
         const dim3 grid((unsigned)blocks), block(rope::NT);
-        if (V == 8) hipLaunchKernelGGL(rope::rotary_kernel<8>, grid, block, lds, st, a);
-        else if (V == 4) hipLaunchKernelGGL(rope::rotary_kernel<4>, grid, block, lds, st, a);
-        else hipLaunchKernelGGL(rope::rotary_kernel<1>, grid, block, lds, st, a);
+#define GDN_ROTARY(DT)                                                                                      \
+    if (V == 8) hipLaunchKernelGGL((rope::rotary_kernel<8, DT>), grid, block, lds, st, a);                   \
+    else if (V == 4) hipLaunchKernelGGL((rope::rotary_kernel<4, DT>), grid, block, lds, st, a);              \
+    else hipLaunchKernelGGL((rope::rotary_kernel<1, DT>), grid, block, lds, st, a)
+        if (dtype == GDN_BF16) { GDN_ROTARY(DT_BF16); }
+        else if (dtype == GDN_F32) { GDN_ROTARY(DT_F32); }
+        else { GDN_ROTARY(DT_F16); }
+#undef GDN_ROTARY
     }
     return check_launch(st, "gdn_rotary");
 }
