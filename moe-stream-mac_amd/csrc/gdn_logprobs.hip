@@ -77,7 +77,7 @@ __device__ __forceinline__ void store8(void *p, int64_t i, const float (&o)[8]) 
     } else {
         u4 a;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) a[j] = ops::pack2(o[2 * j], o[2 * j + 1], DT);
+        for (int j = 0; j < 4; ++j) a[j] = ops::pack2_cvt(o[2 * j], o[2 * j + 1], DT);
         reinterpret_cast<u4_any *>(static_cast<uint16_t *>(p) + i)->v = a;
     }
 }
@@ -127,8 +127,21 @@ __device__ __forceinline__ uint64_t key_of(float x, uint32_t i) { return ((uint6
 struct TopShared {
     uint64_t best[NT];
     uint64_t list[MAX_TOP * E];  // at most `top` threads hand on at most E keys each
-    int n;
+    uint64_t border;
+    float group[NT / 4], least;
+    int n, odd;
 };
+
+// The keys of the list by rank, the r-th to out[r]; places without a key get 0.
+__device__ __forceinline__ void rank_list(const TopShared &sh, int n, int top, uint64_t *out) {
+    for (int i = threadIdx.x; i < n; i += NT) {
+        const uint64_t k = sh.list[i];
+        int r = 0;
+        for (int j = 0; j < n; ++j) r += sh.list[j] > k;
+        if (r < top) out[r] = k;
+    }
+    for (int i = n + threadIdx.x; i < top; i += NT) out[i] = 0;
+}
 
 // The `top` largest of the workgroup's keys (0: none), the r-th to out[r]; places without a key get 0.  Every thread
 // calls it.
@@ -147,12 +160,11 @@ __device__ __forceinline__ void select_top(TopShared &sh, KEY key, int top, uint
     int before = 0;
     for (int i = 0; i < NT; ++i) before += sh.best[i] > best;
     // the top-th largest of the threads' best is at most the top-th largest of all
-    __shared__ uint64_t border;
-    if (tid == 0) border = 0;
+    if (tid == 0) sh.border = 0;
     __syncthreads();
-    if (best && before == top - 1) border = best;
+    if (best && before == top - 1) sh.border = best;
     __syncthreads();
-    const uint64_t b = border;  // 0 where fewer than `top` threads hold a key: everything is handed on
+    const uint64_t b = sh.border;  // 0 where fewer than `top` threads hold a key: everything is handed on
     if (best && before < top) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -161,14 +173,51 @@ __device__ __forceinline__ void select_top(TopShared &sh, KEY key, int top, uint
         }
     }
     __syncthreads();
-    const int n = sh.n;
-    for (int i = tid; i < n; i += NT) {
-        const uint64_t k = sh.list[i];
-        int r = 0;
-        for (int j = 0; j < n; ++j) r += sh.list[j] > k;
-        if (r < top) out[r] = k;
+    rank_list(sh, sh.n, top, out);
+}
+
+// The same from the logits: those not below the top-th largest of 64 groups' maxima (at least `top` of them, seldom many
+// more) are handed on.  False, and nothing written, where that gives more than the list holds (equal logits, most of them
+// -inf) or a logit is NaN, whose order the maxima do not show.  mine: the thread's largest logit; index: a logit's place in
+// the row, or < 0 past its end.
+template <typename INDEX>
+__device__ __forceinline__ bool select_values(TopShared &sh, const float (&x)[E], float mine, INDEX index, int top,
+                                              uint64_t *out) {
+    const int tid = threadIdx.x;
+    float nan = 0.f, g = mine;
+#pragma unroll
+    for (int e = 0; e < E; ++e) nan += x[e] != x[e] ? 1.f : 0.f;
+    g = fmaxf(g, dpp_mov<DPP_QUAD_1032>(g));
+    g = fmaxf(g, dpp_mov<DPP_QUAD_2301>(g));
+    if ((tid & 3) == 0) sh.group[tid / 4] = g;
+    if (tid == 0) sh.n = sh.odd = 0;
+    __syncthreads();
+    if (nan != 0.f) sh.odd = 1;
+    int above = 0, equal = 0;
+#pragma unroll
+    for (int i = 0; i < NT / 4; i += 4) {
+        const float4 v = *reinterpret_cast<const float4 *>(sh.group + i);
+        above += (v.x > g) + (v.y > g) + (v.z > g) + (v.w > g);
+        equal += (v.x == g) + (v.y == g) + (v.z == g) + (v.w == g);
     }
-    for (int i = n + tid; i < top; i += NT) out[i] = 0;
+    if (above < top && above + equal >= top) sh.least = g;  // the same value from every group that has it
+    __syncthreads();
+    if (sh.odd) return false;
+    const float least = sh.least;
+    if (mine >= least) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int64_t j = index(e);
+            if (j >= 0 && x[e] >= least) {
+                const int at = atomicAdd(&sh.n, 1);
+                if (at < MAX_TOP * E) sh.list[at] = key_of(x[e], (uint32_t)j);
+            }
+        }
+    }
+    __syncthreads();
+    if (sh.n > MAX_TOP * E) return false;
+    rank_list(sh, sh.n, top, out);
+    return true;
 }
 
 // One piece of one row: part[row][piece] = (m, s, t, -), keys[row][piece][top].
@@ -179,10 +228,10 @@ __global__ __launch_bounds__(NT) void piece_kernel(Rows a, float4 *part, uint64_
     float x[E];
     load_piece<DT>(a, row, v0, x, -__builtin_inff());
     __shared__ float red[3][NT / 64];
-    float m = x[0];
+    float mine = x[0];
 #pragma unroll
-    for (int e = 1; e < E; ++e) m = fmaxf(m, x[e]);
-    m = wave_max(m);
+    for (int e = 1; e < E; ++e) mine = fmaxf(mine, x[e]);
+    float m = wave_max(mine);
     if ((tid & 63) == 0) red[0][tid >> 6] = m;
     __syncthreads();
     m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
@@ -209,13 +258,12 @@ __global__ __launch_bounds__(NT) void piece_kernel(Rows a, float4 *part, uint64_
     if constexpr (TOP) {
         __shared__ TopShared sh;
         const int64_t left = a.V - v0;
-        select_top(
-            sh,
-            [&](int e) {
-                const int64_t j = (int64_t)((e / 8) * NT + tid) * 8 + e % 8;
-                return j < left ? key_of(x[e], (uint32_t)(v0 + j)) : (uint64_t)0;
-            },
-            top, keys + (row * pieces + piece) * top);
+        const auto at = [&](int e) { return (int64_t)((e / 8) * NT + tid) * 8 + e % 8; };
+        uint64_t *const out = keys + (row * pieces + piece) * top;
+        if (!select_values(sh, x, mine, [&](int e) { return at(e) < left ? v0 + at(e) : (int64_t)-1; }, top, out)) {
+            __syncthreads();
+            select_top(sh, [&](int e) { return at(e) < left ? key_of(x[e], (uint32_t)(v0 + at(e))) : (uint64_t)0; }, top, out);
+        }
     }
 }
 
@@ -280,13 +328,25 @@ __global__ __launch_bounds__(NT) void join_top_kernel(Join j) {
     const int64_t row = blockIdx.x;
     const int n = j.pieces * j.top, tid = threadIdx.x;
     const uint64_t *k = j.keys + row * n;
-    uint64_t mine[E];
+    if (n <= MAX_TOP * E) {  // all of them ranked; some may be 0, below every key
+        for (int i = tid; i < n; i += NT) sh.list[i] = k[i];
+        if (tid < j.top) best[tid] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += NT) {
+            const uint64_t own = sh.list[i];
+            int r = 0;
+            for (int e = 0; e < n; ++e) r += sh.list[e] > own;
+            if (own && r < j.top) best[r] = own;
+        }
+    } else {
+        uint64_t mine[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int i = e * NT + tid;
-        mine[e] = i < n ? k[i] : 0;
+        for (int e = 0; e < E; ++e) {
+            const int i = e * NT + tid;
+            mine[e] = i < n ? k[i] : 0;
+        }
+        select_top(sh, [&](int e) { return mine[e]; }, j.top, best);
     }
-    select_top(sh, [&](int e) { return mine[e]; }, j.top, best);
     __syncthreads();
     float M, ls;
     if (tid < 64) {
@@ -318,7 +378,7 @@ __global__ __launch_bounds__(NT) void bwd_kernel(Bwd b) {
     if (live && (y < 0 || y >= b.a.V)) d = __builtin_nanf("");  // as its logp
     const float e = ENT ? b.dent[row] : 0.f;
     const int64_t out = row * b.a.V + v0;
-    float x[E];
+    float x[E] = {};
     const bool zero = !live && (!ENT || e == 0.f);  // an ignored row: nothing to read
     if (!zero) load_piece<DT>(b.a, row, v0, x, 0.f);
     const float M = b.stat[2 * row], ls = b.stat[2 * row + 1], h = ENT ? b.entropy[row] : 0.f;
@@ -329,15 +389,16 @@ __global__ __launch_bounds__(NT) void bwd_kernel(Bwd b) {
         float o[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            if (zero || none) {
-                o[i] = 0.f;
-                continue;
-            }
             const float l = x[c * 8 + i] - M - ls, p = exp_(l);
             float w = d;
             if constexpr (ENT) w = p > 0.f ? fmaf(e, l + h, d) : 0.f;
-            o[i] = -p * w;
-            if (v0 + j + i == y && live) o[i] += d;
+            o[i] = zero || none ? 0.f : -p * w;
+        }
+        const int64_t hit = y - v0 - j;
+        if (live && !none && hit >= 0 && hit < 8) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (hit == i) o[i] += d;
         }
         if (j + 8 <= left) {
             store8<DT>(b.dz, out + j, o);

@@ -76,6 +76,13 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, int dt) {
     return (uint32_t)__half_as_ushort(__float2half(a)) | ((uint32_t)__half_as_ushort(__float2half(b)) << 16);
 }
 
+// The same by gfx950's v_cvt_pk_bf16_f32: one instruction for the two.
+__device__ __forceinline__ uint32_t pack2_cvt(float a, float b, int dt) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    if (dt == DT_BF16) return __builtin_bit_cast(uint32_t, b2{(__bf16)a, (__bf16)b});
+    return pack2(a, b, dt);
+}
+
 template <int V>
 __device__ __forceinline__ void storev(void *p, size_t i, int dt, const float (&o)[V]) {
     if constexpr (V == 1) {
