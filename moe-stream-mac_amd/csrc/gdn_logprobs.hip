@@ -25,6 +25,7 @@ constexpr int NT = 256;
 constexpr int E = 32;             // logits per thread
 constexpr int PIECE = NT * E;
 constexpr int MAX_TOP = 64;
+constexpr int TURN = 32;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct Rows {  // row r of [outer][inner] rows of V logits
@@ -43,30 +44,21 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 struct __attribute__((packed, aligned(2))) u4_any {
     u4 v;
 };
+// Eight logits as they lie in memory.
 template <int DT>
-__device__ __forceinline__ void load8(const void *p, int64_t i, float (&o)[8]) {
-    if constexpr (DT == DT_F32) {
-        const u4 a = reinterpret_cast<const u4_any *>(static_cast<const float *>(p) + i)->v;
-        const u4 b = reinterpret_cast<const u4_any *>(static_cast<const float *>(p) + i + 4)->v;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            o[j] = __uint_as_float(a[j]);
-            o[4 + j] = __uint_as_float(b[j]);
-        }
-    } else {
-        const u4 a = reinterpret_cast<const u4_any *>(static_cast<const uint16_t *>(p) + i)->v;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if constexpr (DT == DT_BF16) {
-                o[2 * j] = __uint_as_float(a[j] << 16);
-                o[2 * j + 1] = __uint_as_float(a[j] & 0xffff0000u);
-            } else {
-                o[2 * j] = ops::half_bits_to_f32(a[j]);
-                o[2 * j + 1] = ops::half_bits_to_f32(a[j] >> 16);
-            }
-        }
+struct Raw8 {
+    u4 a[DT == DT_F32 ? 2 : 1];
+    __device__ __forceinline__ void load(const void *p, int64_t i) {
+        const char *s = static_cast<const char *>(p) + i * (DT == DT_F32 ? 4 : 2);
+        a[0] = reinterpret_cast<const u4_any *>(s)->v;
+        if constexpr (DT == DT_F32) a[1] = reinterpret_cast<const u4_any *>(s + 16)->v;
     }
-}
+    __device__ __forceinline__ float get(int j) const {
+        if constexpr (DT == DT_F32) return __uint_as_float(a[j / 4][j % 4]);
+        else if constexpr (DT == DT_BF16) return __uint_as_float(j & 1 ? a[0][j / 2] & 0xffff0000u : a[0][j / 2] << 16);
+        else return ops::half_bits_to_f32(a[0][j / 2] >> (16 * (j & 1)));
+    }
+};
 template <int DT>
 __device__ __forceinline__ void store8(void *p, int64_t i, const float (&o)[8]) {
     if constexpr (DT == DT_F32) {
@@ -82,23 +74,35 @@ __device__ __forceinline__ void store8(void *p, int64_t i, const float (&o)[8]) 
     }
 }
 
-// The E logits of thread tid of the piece that starts at v0: 8 at a time, NT * 8 apart; past the end `fill`.
+// The E logits of thread tid of the piece that starts at v0: 8 at a time, NT * 8 apart; past the end `fill`.  All loads are
+// issued before the first is used: none stands under a branch, those past the end read the piece's first logits.
 template <int DT>
 __device__ __forceinline__ void load_piece(const Rows &a, int64_t row, int64_t v0, float (&x)[E], float fill) {
     const int64_t base = a.at(row) + v0;
-    const int64_t left = a.V - v0;
+    const int left = (int)min((int64_t)PIECE, a.V - v0);
+    if (left < 8) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = fill;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (threadIdx.x == 0 && i < left) x[i] = load_as_f32(a.z, base + i, DT);
+        return;
+    }
+    Raw8<DT> raw[E / 8];
 #pragma unroll
     for (int c = 0; c < E / 8; ++c) {
-        const int64_t j = (int64_t)(c * NT + threadIdx.x) * 8;
-        float o[8];
-        if (j + 8 <= left) {
-            load8<DT>(a.z, base + j, o);
-        } else {
+        const int j = (c * NT + threadIdx.x) * 8;
+        raw[c].load(a.z, base + (j + 8 <= left ? j : 0));
+    }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = j + i < left ? load_as_f32(a.z, base + j + i, DT) : fill;
+    for (int c = 0; c < E / 8; ++c) {
+        const int j = (c * NT + threadIdx.x) * 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[c * 8 + i] = raw[c].get(i);
+        if (j + 8 > left) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[c * 8 + i] = j + i < left ? load_as_f32(a.z, base + j + i, DT) : fill;
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[c * 8 + i] = o[i];
     }
 }
 
@@ -126,21 +130,35 @@ __device__ __forceinline__ uint64_t key_of(float x, uint32_t i) { return ((uint6
 
 struct TopShared {
     uint64_t best[NT];
-    uint64_t list[MAX_TOP * E];  // at most `top` threads hand on at most E keys each
+    __attribute__((aligned(16))) uint64_t list[MAX_TOP * E + TURN];  // at most `top` threads hand on at most E keys each
     uint64_t border;
     float group[NT / 4], least;
     int n, odd;
 };
 
-// The keys of the list by rank, the r-th to out[r]; places without a key get 0.
-__device__ __forceinline__ void rank_list(const TopShared &sh, int n, int top, uint64_t *out) {
-    for (int i = threadIdx.x; i < n; i += NT) {
-        const uint64_t k = sh.list[i];
+// The keys of the list by rank, the r-th to out[r]; places without a key get 0, as keys of 0 are none.  Four lanes count the
+// larger ones for a key, 32 to a turn and all of a turn's reads under way at once (one by one their latency is the kernel's
+// time: 15 us for 20 alternatives of 16 pieces).  Every thread calls it; it begins with a barrier.
+__device__ __forceinline__ void rank_list(TopShared &sh, int n, int top, uint64_t *out) {
+    const int tid = threadIdx.x;
+    if (tid < TURN) sh.list[n + tid] = 0;
+    for (int i = n + tid; i < top; i += NT) out[i] = 0;
+    __syncthreads();
+    for (int i0 = 0; i0 < n; i0 += NT / 4) {
+        const int i = i0 + tid / 4;
+        const uint64_t k = i < n ? sh.list[i] : ~(uint64_t)0;
         int r = 0;
-        for (int j = 0; j < n; ++j) r += sh.list[j] > k;
-        if (r < top) out[r] = k;
+        for (int j = 2 * (tid & 3); j < n; j += TURN) {
+            ulonglong2 v[TURN / 8];
+#pragma unroll
+            for (int e = 0; e < TURN / 8; ++e) v[e] = *reinterpret_cast<const ulonglong2 *>(sh.list + j + 8 * e);
+#pragma unroll
+            for (int e = 0; e < TURN / 8; ++e) r += (v[e].x > k) + (v[e].y > k);
+        }
+        r += __shfl_xor(r, 1);
+        r += __shfl_xor(r, 2);
+        if (i < n && k && r < top && (tid & 3) == 0) out[r] = k;
     }
-    for (int i = n + threadIdx.x; i < top; i += NT) out[i] = 0;
 }
 
 // The `top` largest of the workgroup's keys (0: none), the r-th to out[r]; places without a key get 0.  Every thread
@@ -332,12 +350,7 @@ __global__ __launch_bounds__(NT) void join_top_kernel(Join j) {
         for (int i = tid; i < n; i += NT) sh.list[i] = k[i];
         if (tid < j.top) best[tid] = 0;
         __syncthreads();
-        for (int i = tid; i < n; i += NT) {
-            const uint64_t own = sh.list[i];
-            int r = 0;
-            for (int e = 0; e < n; ++e) r += sh.list[e] > own;
-            if (own && r < j.top) best[r] = own;
-        }
+        rank_list(sh, n, j.top, best);
     } else {
         uint64_t mine[E];
 #pragma unroll
