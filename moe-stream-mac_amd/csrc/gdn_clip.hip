@@ -198,19 +198,23 @@ extern "C" int gdn_clip_grad_norm(const void *const *x, void *const *y, const in
             int i, out;
         };
         try {
-            std::vector<Span> s;
-            s.reserve(2 * (size_t)count);
+            // most callers' lists run through memory in order: the two are merged then, not sorted
+            std::vector<Span> s[2];
+            const auto less = [](const Span &a, const Span &b) { return a.lo < b.lo; };
             for (int i = 0; i < count; ++i) {
                 if (!numel[i]) continue;
                 const uintptr_t o = reinterpret_cast<uintptr_t>(y[i]), in = reinterpret_cast<uintptr_t>(x[i]);
                 const uintptr_t len = (uintptr_t)(numel[i] * clip::bytes_of(dtypes[i]));
-                s.push_back({o, o + len, i, 1});
-                if (o != in) s.push_back({in, in + len, i, 0});
+                s[0].push_back({o, o + len, i, 1});
+                if (o != in) s[1].push_back({in, in + len, i, 0});
             }
-            std::sort(s.begin(), s.end(), [](const Span &a, const Span &b) { return a.lo < b.lo; });
+            for (auto &v : s)
+                if (!std::is_sorted(v.begin(), v.end(), less)) std::sort(v.begin(), v.end(), less);
+            std::vector<Span> all(s[0].size() + s[1].size());
+            std::merge(s[0].begin(), s[0].end(), s[1].begin(), s[1].end(), all.begin(), less);
             uintptr_t out_end = 0, any_end = 0;
             int out_i = 0, any_i = 0;
-            for (const Span &v : s) {
+            for (const Span &v : all) {
                 if (v.lo < out_end || (v.out && v.lo < any_end))
                     return fail(GDN_ERR_INVALID, "tensors %d and %d share memory that is written", v.i,
                                 v.lo < out_end ? out_i : any_i);

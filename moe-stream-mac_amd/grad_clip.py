@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+from operator import attrgetter
 from typing import Iterable, Optional
 
 import torch
@@ -13,6 +14,10 @@ import torch
 import gdn_lib as L
 
 Array = torch.Tensor
+
+# a model has hundreds of tensors: attributes are taken by maps, without a line of Python for each
+_layout, _dtype, _shape = attrgetter("layout"), attrgetter("dtype"), attrgetter("shape")
+_index, _numel, _ptr, _contiguous = Array.get_device, Array.numel, Array.data_ptr, Array.is_contiguous
 
 
 def _dense(t: Array) -> bool:
@@ -28,33 +33,30 @@ def _dense(t: Array) -> bool:
 
 
 def _check(tensors, norm_type) -> None:
-    """Attribute by attribute over all tensors: a model has hundreds, each of a few microseconds otherwise."""
     if norm_type not in (2.0, math.inf):
         raise ValueError(f"norm_type must be 2 or inf; got {norm_type}")
-    if {t.layout for t in tensors} != {torch.strided} or not {t.dtype for t in tensors} <= L.DTYPE_CODE.keys():
+    if set(map(_layout, tensors)) != {torch.strided} or not set(map(_dtype, tensors)) <= L.DTYPE_CODE.keys():
         t = next(t for t in tensors if t.layout != torch.strided or t.dtype not in L.DTYPE_CODE)
         raise ValueError(f"unsupported tensor ({t.dtype}, {t.layout}); use dense float32, bfloat16 or float16")
-    devices = {t.device for t in tensors}
-    if len(devices) > 1:
+    if len(set(map(_index, tensors))) > 1:
         raise ValueError("all tensors must be on the same device")
-    (dev,) = devices
-    if dev.type != "cuda":
-        raise RuntimeError("grad_clip runs on a ROCm GPU only; got tensors on " + str(dev))
+    if tensors[0].device.type != "cuda":
+        raise RuntimeError("grad_clip runs on a ROCm GPU only; got tensors on " + str(tensors[0].device))
 
 
 def _call(tensors, outs, max_norm, norm_type, eps) -> Array:
     dev, code = tensors[0].device, L.DTYPE_CODE
     n = len(tensors)
     ptrs = ctypes.c_void_p * n
-    numel = (ctypes.c_int64 * n)(*[t.numel() for t in tensors])
+    numel = (ctypes.c_int64 * n)(*map(_numel, tensors))
     lib = L.load()
     norm = torch.empty((), dtype=torch.float32, device=dev)
     nws = lib.gdn_clip_grad_norm_workspace_bytes(numel, n)
     ws = torch.empty((nws,), dtype=torch.uint8, device=dev)
-    x = ptrs(*[t.data_ptr() for t in tensors])
-    y = None if outs is None else x if outs is tensors else ptrs(*[t.data_ptr() for t in outs])
+    x = ptrs(*map(_ptr, tensors))
+    y = None if outs is None else x if outs is tensors else ptrs(*map(_ptr, outs))
     with L.on_device(dev):
-        L.check(lib.gdn_clip_grad_norm(x, y, numel, (ctypes.c_int * n)(*[code[t.dtype] for t in tensors]), n,
+        L.check(lib.gdn_clip_grad_norm(x, y, numel, (ctypes.c_int * n)(*map(code.__getitem__, map(_dtype, tensors))), n,
                                        int(norm_type == math.inf), float(max_norm), float(eps), norm.data_ptr(),
                                        ws.data_ptr(), nws, L.stream_handle(dev)))
     return norm
@@ -84,11 +86,11 @@ def clip_grad_norm(grads: Iterable[Array], max_norm: float, norm_type: float = 2
         return torch.zeros(())
     _check(gs, norm_type)
     os_ = gs if out is None else list(out)
-    if out is not None and ([o.shape for o in os_] != [g.shape for g in gs] or
-                            [o.dtype for o in os_] != [g.dtype for g in gs] or
-                            {o.device for o in os_} != {gs[0].device} or {o.layout for o in os_} != {torch.strided}):
+    if out is not None and (list(map(_shape, os_)) != list(map(_shape, gs)) or
+                            list(map(_dtype, os_)) != list(map(_dtype, gs)) or
+                            set(map(_index, os_)) != {gs[0].get_device()} or set(map(_layout, os_)) != {torch.strided}):
         raise ValueError("out must hold one tensor of the same shape, type and device for each gradient")
-    if all([g.is_contiguous() for g in gs]) and (os_ is gs or all([o.is_contiguous() for o in os_])):
+    if all(map(_contiguous, gs)) and (os_ is gs or all(map(_contiguous, os_))):
         return _call(gs, os_, max_norm, float(norm_type), eps)
     # memory order does not matter to the kernels where input and output share it; others go through a copy
     src, dst, back = [], [], []
