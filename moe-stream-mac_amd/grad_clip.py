@@ -4,8 +4,8 @@ synchronisation with the host.  Tensors must live on a ROCm device; there is no 
 
 from __future__ import annotations
 
-import ctypes
 import math
+from array import array
 from operator import attrgetter
 from typing import Iterable, Optional
 
@@ -44,19 +44,27 @@ def _check(tensors, norm_type) -> None:
         raise RuntimeError("grad_clip runs on a ROCm GPU only; got tensors on " + str(tensors[0].device))
 
 
+def _same_dtypes(a, b) -> bool:
+    one = set(map(_dtype, a))
+    return set(map(_dtype, b)) == one and (len(one) == 1 or list(map(_dtype, a)) == list(map(_dtype, b)))
+
+
 def _call(tensors, outs, max_norm, norm_type, eps) -> Array:
-    dev, code = tensors[0].device, L.DTYPE_CODE
-    n = len(tensors)
-    ptrs = ctypes.c_void_p * n
-    numel = (ctypes.c_int64 * n)(*map(_numel, tensors))
+    dev, n = tensors[0].device, len(tensors)
+    dtypes = set(map(_dtype, tensors))
+    if len(dtypes) == 1:
+        codes = array("i", [L.DTYPE_CODE[dtypes.pop()]]) * n
+    else:
+        codes = array("i", map(L.DTYPE_CODE.__getitem__, map(_dtype, tensors)))
+    numel, x = array("q", map(_numel, tensors)), array("Q", map(_ptr, tensors))
+    y = None if outs is None else x if outs is tensors else array("Q", map(_ptr, outs))
+    at = lambda a: a.buffer_info()[0]  # noqa: E731  (the arrays live until the call is over)
     lib = L.load()
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    nws = lib.gdn_clip_grad_norm_workspace_bytes(numel, n)
+    nws = lib.gdn_clip_grad_norm_workspace_bytes(at(numel), n)
     ws = torch.empty((nws,), dtype=torch.uint8, device=dev)
-    x = ptrs(*map(_ptr, tensors))
-    y = None if outs is None else x if outs is tensors else ptrs(*map(_ptr, outs))
     with L.on_device(dev):
-        L.check(lib.gdn_clip_grad_norm(x, y, numel, (ctypes.c_int * n)(*map(code.__getitem__, map(_dtype, tensors))), n,
+        L.check(lib.gdn_clip_grad_norm(at(x), None if y is None else at(y), at(numel), at(codes), n,
                                        int(norm_type == math.inf), float(max_norm), float(eps), norm.data_ptr(),
                                        ws.data_ptr(), nws, L.stream_handle(dev)))
     return norm
@@ -87,7 +95,7 @@ def clip_grad_norm(grads: Iterable[Array], max_norm: float, norm_type: float = 2
     _check(gs, norm_type)
     os_ = gs if out is None else list(out)
     if out is not None and (list(map(_shape, os_)) != list(map(_shape, gs)) or
-                            list(map(_dtype, os_)) != list(map(_dtype, gs)) or
+                            not _same_dtypes(gs, os_) or
                             set(map(_index, os_)) != {gs[0].get_device()} or set(map(_layout, os_)) != {torch.strided}):
         raise ValueError("out must hold one tensor of the same shape, type and device for each gradient")
     if all(map(_contiguous, gs)) and (os_ is gs or all(map(_contiguous, os_))):
