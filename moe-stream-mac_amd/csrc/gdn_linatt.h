@@ -39,6 +39,7 @@ constexpr int C = 64;  // tokens of a chunk
 constexpr double LOG2E = 1.4426950408889634074;
 
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16;
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
@@ -132,19 +133,33 @@ __device__ __forceinline__ F32Frag col_frag(const float *t, int lane, int k0, in
     return f;
 }
 
+// Two numbers rounded to bf16 by one instruction, and back.
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, b2));
+}
+__device__ __forceinline__ float low_bf16(uint32_t u) { return __uint_as_float(u << 16); }
+__device__ __forceinline__ float high_bf16(uint32_t u) { return __uint_as_float(u & 0xffff0000u); }
+
 // x as the sum of N operands (fp32: itself).
 template <int N>
 __device__ __forceinline__ void split(const float (&x)[8], bf8 (&o)[N]) {
+    u4 u[N];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        float r = x[j];
+    for (int j = 0; j < 4; ++j) {
+        float a = x[2 * j], b = x[2 * j + 1];
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const bf16 h = (bf16)r;
-            o[n][j] = h;
-            r -= (float)h;
+            u[n][j] = pack_bf16(a, b);
+            if (n + 1 < N) {
+                a -= low_bf16(u[n][j]);
+                b -= high_bf16(u[n][j]);
+            }
         }
     }
+#pragma unroll
+    for (int n = 0; n < N; ++n) o[n] = __builtin_bit_cast(bf8, u[n]);
 }
 template <int N>
 __device__ __forceinline__ void split(const float (&x)[8], F32Frag (&o)[N]) {
@@ -166,13 +181,13 @@ struct Ten {
     int64_t sb, st, sh;
     int div;
     __device__ __forceinline__ int64_t at(int b, int64_t t, int h) const { return b * sb + t * st + (h / div) * sh; }
+    template <typename ET>
     __device__ __forceinline__ const char *from(int b, int64_t t, int h, int c, int dt) const {
-        return static_cast<const char *>(p) + (at(b, t, h) + c) * (dt == DT_F32 ? 4 : 2);
+        return static_cast<const char *>(p) + (at(b, t, h) + c) * (std::is_same_v<ET, float> && dt == DT_F32 ? 4 : 2);
     }
 };
 
 // 16 bytes from an address that is a multiple of the element's size only
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 struct __attribute__((packed, aligned(2))) u4_any {
     u4 v;
 };
@@ -189,7 +204,7 @@ struct Tile {
     // t0: the tile's first row and channel; dt: its type; st: elements between rows
     __device__ __forceinline__ void fetch(const char *t0, int64_t st, int n, int w, int dt) {
         const int tid = opaque(threadIdx.x) & (N - 1), r0 = tid / (W / 8), c0 = (tid % (W / 8)) * 8;
-        const unsigned size = dt == DT_F32 ? 4 : 2, row = (unsigned)st * size;
+        const unsigned size = F32 && dt == DT_F32 ? 4 : 2, row = (unsigned)st * size;
         if constexpr (VEC) {
             const unsigned c = (c0 < w ? c0 : 0) * size;
 #pragma unroll
@@ -260,24 +275,22 @@ struct __attribute__((packed, aligned(2))) u2_any {
     u2 v;
 };
 template <int N, typename ET>
-__device__ __forceinline__ void store_row(void *p, int64_t i, int dt, const float (&o)[N]) {
+__device__ __forceinline__ void store_row(char *p, unsigned i, int dt, const float (&o)[N]) {
     if (dt == DT_F32) {
 #pragma unroll
         for (int j = 0; j < N; j += 4) {
             const u4 a = {__float_as_uint(o[j]), __float_as_uint(o[j + 1]), __float_as_uint(o[j + 2]), __float_as_uint(o[j + 3])};
-            reinterpret_cast<u4_any *>(static_cast<float *>(p) + i + j)->v = a;
+            reinterpret_cast<u4_any *>(p + 4 * (i + j))->v = a;
         }
     } else {
-        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
         uint32_t u[N / 2];
 #pragma unroll
         for (int j = 0; j < N / 2; ++j) {
-            if constexpr (std::is_same_v<ET, bf16>) u[j] = __builtin_bit_cast(uint32_t, b2{(bf16)o[2 * j], (bf16)o[2 * j + 1]});
+            if constexpr (std::is_same_v<ET, bf16>) u[j] = pack_bf16(o[2 * j], o[2 * j + 1]);
             else u[j] = ops::pack2(o[2 * j], o[2 * j + 1], DT_F16);
         }
-        uint16_t *d = static_cast<uint16_t *>(p) + i;
-        if constexpr (N == 8) reinterpret_cast<u4_any *>(d)->v = u4{u[0], u[1], u[2], u[3]};
-        else reinterpret_cast<u2_any *>(d)->v = u2{u[0], u[1]};
+        if constexpr (N == 8) reinterpret_cast<u4_any *>(p + 2 * i)->v = u4{u[0], u[1], u[2], u[3]};
+        else reinterpret_cast<u2_any *>(p + 2 * i)->v = u2{u[0], u[1]};
     }
 }
 
@@ -387,6 +400,50 @@ struct Shared {
     __device__ __forceinline__ float4 *sum() { return SUM_OVER_Q ? reinterpret_cast<float4 *>(Q[0]) : own_sum; }
 };
 
+// 32 rows of a wave's V', and the same times their weights in NS terms, worked out two elements of a lane at a time: PARTS
+// parts, to stand between matrix products, which leave the vector unit 12 of their 16 cycles.
+template <typename ET, int NV, int NS>
+struct Weighted {
+    static constexpr int PARTS = 4 * NV;
+    static constexpr bool F32 = std::is_same_v<ET, float>;
+    Frag<ET> v[NV];
+    std::conditional_t<F32, F32Frag, u4> t[NV][NS];
+    float w[8];
+    __device__ __forceinline__ Frag<ET> term(int x, int n) const { return __builtin_bit_cast(Frag<ET>, t[x][n]); }
+    template <typename L>
+    __device__ __forceinline__ void read(const ET *sV, int lane, int k0, int x0, const float *weights) {
+#pragma unroll
+        for (int x = 0; x < NV; ++x) v[x] = col_frag<L>(sV, lane, k0, x0, 4 * x);
+        const f4 a = *reinterpret_cast<const f4 *>(weights), b = *reinterpret_cast<const f4 *>(weights + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            w[j] = a[j];
+            w[4 + j] = b[j];
+        }
+    }
+    __device__ __forceinline__ void part(int i) {
+        const int x = i / 4, j = 2 * (i % 4);
+        if constexpr (F32) {
+            t[x][0].v[j] = v[x].v[j] * w[j];
+            t[x][0].v[j + 1] = v[x].v[j + 1] * w[j + 1];
+        } else {
+            const uint32_t u = __builtin_bit_cast(u4, v[x])[j / 2];
+            float a = low_bf16(u) * w[j], b = high_bf16(u) * w[j + 1];
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                const uint32_t h = pack_bf16(a, b);
+                t[x][n][j / 2] = h;
+                a -= low_bf16(h);
+                b -= high_bf16(h);
+            }
+        }
+    }
+    __device__ __forceinline__ void all() {
+#pragma unroll
+        for (int i = 0; i < PARTS; ++i) part(i);
+    }
+};
+
 // The state of a wave: K' rows 32 T + 8 (l / 16) + 4 (t & 1) + e of tile t = 2 T, 2 T + 1 by its columns 16 NV w + ...: what
 // lane l holds of two tiles is 8 consecutive K' rows of one column, an operand as it stands.
 template <int D, int NV, int NW>
@@ -430,38 +487,39 @@ struct State {
                     if (k + e < dk) p[tr ? (k + e) * dv + v : v * dk + k + e] = s[2 * T + e / 4][n][e % 4];
             }
     }
-    // s = total s + sum over 32 rows of the tiles: K'^T diag(weights) V', the weighted V' in NS terms
-    template <int NS, typename ET>
-    __device__ __forceinline__ void add(const ET *sK, int lane, int k0, const Frag<ET> (&vw)[NV][NS]) {
+    // s += K'^T diag(weights) V' over 32 rows, tile by tile, between(t) behind the products of each
+    template <int NS, typename ET, typename F>
+    __device__ __forceinline__ void add(const ET *sK, int lane, int k0, const Weighted<ET, NV, NS> &v, F between) {
+        Frag<ET> a = col_frag<Lds<ET, D>>(sK, lane, k0, 0, 0);
 #pragma unroll
         for (int t = 0; t < D / 16; ++t) {
-            const Frag<ET> a = col_frag<Lds<ET, D>>(sK, lane, k0, 32 * (t >> 1), 4 * (t & 1));
+            Frag<ET> next = a;
+            if (t + 1 < D / 16) next = col_frag<Lds<ET, D>>(sK, lane, k0, 32 * ((t + 1) >> 1), 4 * ((t + 1) & 1));
 #pragma unroll
             for (int i = 0; i < NS; ++i)
 #pragma unroll
-                for (int n = 0; n < NV; ++n) s[t][n] = mma(a, vw[n][i], s[t][n]);
+                for (int n = 0; n < NV; ++n) s[t][n] = mma(a, v.term(n, i), s[t][n]);
+            between(t);
+            if constexpr (NS == 3) __builtin_amdgcn_sched_barrier(0);
+            a = next;
         }
+    }
+    __device__ __forceinline__ void scale(int t, float f) {
+#pragma unroll
+        for (int n = 0; n < NV; ++n) s[t][n] *= f;
     }
 };
 
-template <typename ET, int N>
-__device__ __forceinline__ void weigh(const Frag<ET> &v, const float *w, Frag<ET> (&o)[N]) {
-    float x[8];
-    to_f32(v, x);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] *= w[j];
-    split(x, o);
-}
-
-// The e-th of the ten 16 x 16 blocks of P that hold pairs: its first output and source.
+// The e-th of twelve 16 x 16 blocks of P, its first output and source: the ten that hold pairs, and two that fill the products'
+// 32 sources with zeros.  Blocks 0-7 are the four of two outputs (for the last of them all sources count; reverse: the first),
+// so that a wave's blocks e and e + 4 share their sources.
 struct Block {
     int r0, s0;
-    bool in;
 };
 template <bool REV>
 __device__ __forceinline__ Block block(int e) {
-    const int i = (e >= 1) + (e >= 3) + (e >= 6), j = e - i * (i + 1) / 2;
-    return REV ? Block{16 * j, 16 * i, e < 10} : Block{16 * i, 16 * j, e < 10};
+    const int r = e < 8 ? 2 + (e >> 2) : (e >> 1) & 1, s = e < 8 ? e & 3 : e & 1;
+    return REV ? Block{48 - 16 * r, 48 - 16 * s} : Block{16 * r, 16 * s};
 }
 
 // Workgroups go to the 8 XCDs in turn, each with its own L2: an order in which neighbours, the heads that share a key head,
@@ -500,25 +558,30 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
     Tile<ET, 16 * NV * NW, VEC, 64 * NW * G> tv;
     Tile<ET, 16 * NV * NW, VEC, 64 * NW> tx;
     float td = 0.f;
-    const auto fetch = [&](int c) {
+    // the next chunk's tiles, one by one between the phases of this one
+    const auto fetch = [&](int c, int part) {
         const int64_t t0 = (int64_t)c * C;
         const int n = min((int64_t)C, a.T - t0);
-        tq.fetch(a.Q.from(b, t0, h, 0, a.dt), a.Q.st, n, a.dk, a.dt);
-        tk.fetch(a.K.from(b, t0, h, 0, a.dt), a.K.st, n, a.dk, a.dt);
-        tv.fetch(a.V.from(b, t0, h, c0, a.dt), a.V.st, n, a.dv - c0, a.dt);
-        td = a.decays[(head * a.nc + c) * DECAYS + (threadIdx.x & (NT - 1))];
+        if (part == 0) {
+            tq.fetch(a.Q.template from<ET>(b, t0, h, 0, a.dt), a.Q.st, n, a.dk, a.dt);
+            td = a.decays[(head * a.nc + c) * DECAYS + (threadIdx.x & (NT - 1))];
+        } else if (part == 1) {
+            tk.fetch(a.K.template from<ET>(b, t0, h, 0, a.dt), a.K.st, n, a.dk, a.dt);
+        } else {
+            tv.fetch(a.V.template from<ET>(b, t0, h, c0, a.dt), a.V.st, n, a.dv - c0, a.dt);
+        }
     };
     Piece<4 * NV, ET, VEC> px[RT];
     const auto fetch_x = [&](int c) {
         const int64_t t0 = (int64_t)c * C;
         const int n = min((int64_t)C, a.T - t0);
-        const char *x0 = a.X.from(b, t0, h, 0, a.dt);
+        const char *x0 = a.X.template from<ET>(b, t0, h, 0, a.dt);
         const int l = opaque(threadIdx.x & 63), li = l & 15, col = c0 + 16 * NV * w + 4 * NV * (l >> 4);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
             px[rt].fetch(x0, __umul24(min(16 * rt + li, n - 1), (unsigned)a.X.st) + col, a.dv - col, a.dt);
     };
-    fetch(REV ? last : first);
+    for (int part = 0; part < 3; ++part) fetch(REV ? last : first, part);
     for (int i = first; i <= last; ++i) {
         const int c = REV ? first + last - i : i;
         const int64_t t0 = (int64_t)c * C;
@@ -536,8 +599,9 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
         __syncthreads();
         // X before the next tiles: loads are waited for in their order
         if constexpr (DOT) fetch_x(c);
-        if constexpr (KIND == DV) tx.fetch(a.X.from(b, t0, h, c0, a.dt), a.X.st, n, a.dv - c0, a.dt);
-        if (i < last) fetch(REV ? c - 1 : c + 1);
+        if constexpr (KIND == DV) tx.fetch(a.X.template from<ET>(b, t0, h, c0, a.dt), a.X.st, n, a.dv - c0, a.dt);
+        const int after = REV ? c - 1 : c + 1;
+        if (i < last) fetch(after, 0);
 
         // O = diag(wo) S Q'^T, later + P V', transposed: a lane holds one token, 4 NV consecutive columns
         const int lk = LK::row_lane(li, g);
@@ -546,6 +610,10 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int x = 0; x < NV; ++x) O[rt][x] = f4{0.f, 0.f, 0.f, 0.f};
+        const int lvc = LV::template col_lane<4 * NV>(li, g);
+        const float *const weights = (REV ? sh.d[grp].in : sh.d[grp].out) + 8 * g;
+        Weighted<ET, NV, NS> v;
+        v.template read<LV>(sh.V, lvc, 0, 16 * NV * w, weights);
 #pragma unroll
         for (int T = 0; T < D / 32; ++T) {
             Frag<ET> f[NV][NH];
@@ -567,6 +635,8 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
 #pragma unroll
                     for (int x = 0; x < NV; ++x) O[rt][x] = mma(f[x][j], q, O[rt][x]);
             }
+#pragma unroll
+            for (int i = T * v.PARTS * 32 / D; i < (T + 1) * v.PARTS * 32 / D; ++i) v.part(i);
         }
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -595,58 +665,56 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
             }
         }
 
-        // P: blocks (rt, st) of 16 outputs by 16 sources with st <= rt (reverse: >=), one to a wave in turn; the blocks that
-        // fill a product's 32 sources are zeros
+        if (i < last) fetch(after, 1);
+        // P: its blocks to the waves in turn
         ET *const sP = sh.p(grp);
-        constexpr int BLOCKS = (10 + NW - 1) / NW;
+        constexpr int BLOCKS = (12 + NW - 1) / NW;
+        const bool last_block = 12 % NW == 0 || w < 12 % NW;
         f4 acc[BLOCKS] = {};
+        float2 gr[BLOCKS], gs[BLOCKS][4];
+        const auto read_decays = [&] {
+#pragma unroll
+                for (int e = 0; e < BLOCKS; ++e) {
+                const Block k = block<REV>(w + NW * e);
+                gr[e] = sh.d[grp].G[(k.r0 + li) & (C - 1)];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) gs[e][j] = sh.d[grp].G[(k.s0 + 4 * g + j) & (C - 1)];
+            }
+        };
+        if constexpr (KIND != DV) read_decays();  // ahead of the products; DV has no registers left for it
 #pragma unroll
         for (int x = 0; x < D; x += 32)
 #pragma unroll
-            for (int e = 0; e < BLOCKS - 1; ++e) {
+            for (int e = 0; e < BLOCKS; ++e) {
+                if (e == BLOCKS - 1 && !last_block) continue;
                 const Block k = block<REV>(w + NW * e);
                 acc[e] = mma(row_frag<LK>(sh.K[grp], lk, k.s0, x), row_frag<LK>(sh.Q[grp], lk, k.r0, x), acc[e]);
             }
-        if (w < 2) {
-            constexpr int E = BLOCKS - 1;
-            const Block k = block<REV>(8 + w);
-#pragma unroll
-            for (int x = 0; x < D; x += 32)
-                acc[E] = mma(row_frag<LK>(sh.K[grp], lk, k.s0, x), row_frag<LK>(sh.Q[grp], lk, k.r0, x), acc[E]);
-        }
         if constexpr (TAKEN) {
             __syncthreads();
         }
         if constexpr (KIND == DV) tx.store(sh.x(), n, a.dv - c0, a.dt);
-        const auto put = [&](int r, int s, const ET (&p)[4]) {
+        if constexpr (KIND == DV) read_decays();
+        const auto put = [&](int r, int s, const f4 &p) {
             ET *o = sP + LP::at4(r, s);
-            if constexpr (F32) *reinterpret_cast<float4 *>(o) = make_float4(p[0], p[1], p[2], p[3]);
-            else *reinterpret_cast<uint2 *>(o) = *reinterpret_cast<const uint2 *>(p);
+            if constexpr (F32) *reinterpret_cast<f4 *>(o) = p;
+            else *reinterpret_cast<uint2 *>(o) = make_uint2(pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]));
         };
 #pragma unroll
         for (int e = 0; e < BLOCKS; ++e) {
+            if (e == BLOCKS - 1 && !last_block) continue;
             const Block k = block<REV>(w + NW * e);
-            if (!k.in) continue;
             const int r = k.r0 + li, s0 = k.s0 + 4 * g;
-            const float2 gr = sh.d[grp].G[r];
-            float2 gs[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) gs[j] = sh.d[grp].G[s0 + j];
-            ET p[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float d = (gr.x - gs[j].x) + (gr.y - gs[j].y);
+                const float d = (gr[e].x - gs[e][j].x) + (gr[e].y - gs[e][j].y);
                 const float x = acc[e][j] * (a.scale * __builtin_amdgcn_exp2f(REV ? -d : d));
                 acc[e][j] = (REV ? s0 + j >= r : s0 + j <= r) ? x : 0.f;
-                p[j] = (ET)acc[e][j];
             }
-            put(r, s0, p);
-        }
-        if (w < 2) {
-            const ET zero[4] = {(ET)0.f, (ET)0.f, (ET)0.f, (ET)0.f};
-            put(32 * w + (REV ? 16 : 0) + li, 32 * w + (REV ? 0 : 16) + 4 * g, zero);
+            put(r, s0, acc[e]);
         }
         __syncthreads();
+        if (i < last) fetch(after, 2);
         // M of the same blocks, its sums over outputs and sources apart in 64 bits: their difference from a token on is the sum
         // of the pairs that cross it
         if constexpr (KIND == DV) {
@@ -655,8 +723,8 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
             cross[l] = 0.;
 #pragma unroll
             for (int e = 0; e < BLOCKS; ++e) {
+                if (e == BLOCKS - 1 && !last_block) continue;
                 const Block k = block<REV>(w + NW * e);
-                if (!k.in) continue;
                 f4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < 16 * NV * NW; i += 32)
@@ -679,19 +747,8 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
             }
         }
         const float total = sh.total[grp];
-#pragma unroll
-        for (int t = 0; t < D / 16; ++t)
-#pragma unroll
-            for (int x = 0; x < NV; ++x) S.s[t][x] *= total;
-        const int lp = LP::row_lane(li, g), lvc = LV::template col_lane<4 * NV>(li, g), lkc = LK::template col_lane<8>(li, g);
-#pragma unroll 1
-        for (int k0 = 0; k0 < C; k0 += 32) {
-            Frag<ET> v[NV], vw[NV][NS];
-#pragma unroll
-            for (int x = 0; x < NV; ++x) {
-                v[x] = col_frag<LV>(sh.V, lvc, k0, 16 * NV * w, 4 * x);
-                weigh<ET>(v[x], (REV ? sh.d[grp].in : sh.d[grp].out) + k0 + 8 * g, vw[x]);
-            }
+        const int lp = LP::row_lane(li, g), lkc = LK::template col_lane<8>(li, g);
+        const auto pairs_of = [&](int k0, const Frag<ET> (&v)[NV]) {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 if (REV ? 16 * rt >= k0 + 32 : 16 * rt + 16 <= k0) continue;
@@ -699,8 +756,20 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
 #pragma unroll
                 for (int x = 0; x < NV; ++x) O[rt][x] = mma(v[x], p, O[rt][x]);
             }
-            S.template add<NS, ET>(sh.K[grp], lkc, k0, vw);
-        }
+        };
+        Weighted<ET, NV, NS> next;
+        next.template read<LV>(sh.V, lvc, 32, 16 * NV * w, weights + 32);
+        S.scale(0, total);
+        pairs_of(0, v.v);
+        S.template add<NS, ET>(
+            sh.K[grp], lkc, 0, v,
+            [&](int t) {
+                if (t + 1 < D / 16) S.scale(t + 1, total);
+#pragma unroll
+                for (int i = t * next.PARTS * 16 / D; i < (t + 1) * next.PARTS * 16 / D; ++i) next.part(i);
+            });
+        pairs_of(32, next.v);
+        S.template add<NS, ET>(sh.K[grp], lkc, 32, next, [](int) {});
 
         if constexpr (G == 2) {
             float4 *const sum = sh.sum() + w * 64 + l;
@@ -722,19 +791,21 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
                     }
             }
         }
+        const unsigned o_row = (a.Hv / G) * a.dv;
+        char *const o0 = static_cast<char *>(a.o) + (((b * (int64_t)a.T + t0) * (a.Hv / G) + hg) * a.dv << (a.o_dt == DT_F32 ? 2 : 1));
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const int r = 16 * rt + li;
             float o[4 * NV];
             row_of(rt, o);
             if (r < n && grp == 0) {
-                const int64_t at = ((b * (int64_t)a.T + t0 + r) * (a.Hv / G) + hg) * a.dv + col;
+                const unsigned at = __umul24(r, o_row) + col;
                 if constexpr (VEC) {
-                    if (col < a.dv) store_row<4 * NV, ET>(a.o, at, a.o_dt, o);
+                    if (col < a.dv) store_row<4 * NV, ET>(o0, at, a.o_dt, o);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 4 * NV; ++j)
-                        if (col + j < a.dv) store_from_f32(a.o, at + j, o[j], a.o_dt);
+                        if (col + j < a.dv) store_from_f32(o0, at + j, o[j], a.o_dt);
                 }
             }
         }
@@ -800,8 +871,8 @@ __global__ __launch_bounds__(64 * NW, (waves<ET, D>())) void seg_kernel(const Se
     const auto fetch = [&](int c) {
         const int64_t t0 = (int64_t)c * C;
         const int n = min((int64_t)C, a.T - t0);
-        tk.fetch(a.K.from(b, t0, h, 0, a.dt), a.K.st, n, a.dk, a.dt);
-        tv.fetch(a.V.from(b, t0, h, c0, a.dt), a.V.st, n, a.dv - c0, a.dt);
+        tk.fetch(a.K.template from<ET>(b, t0, h, 0, a.dt), a.K.st, n, a.dk, a.dt);
+        tv.fetch(a.V.template from<ET>(b, t0, h, c0, a.dt), a.V.st, n, a.dv - c0, a.dt);
         td = a.decays[(((int64_t)b * a.Hv + h) * a.nc + c) * DECAYS + (tid & (NT - 1))];
     };
     fetch(REV ? last : first);
@@ -816,19 +887,21 @@ __global__ __launch_bounds__(64 * NW, (waves<ET, D>())) void seg_kernel(const Se
         if (i < last) fetch(REV ? c - 1 : c + 1);
         const float total = sum;
         all *= total;
-#pragma unroll
-        for (int t = 0; t < D / 16; ++t)
-#pragma unroll
-            for (int x = 0; x < NV; ++x) S.s[t][x] *= total;
         const int li = l & 15, lvc = LV::template col_lane<4 * NV>(li, g), lkc = LK::template col_lane<8>(li, g);
+        const float *const weights = (REV ? d.in : d.out) + 8 * g;
+        Weighted<ET, NV, NS> v, next;
+        v.template read<LV>(sV, lvc, 0, 16 * NV * w, weights);
+        v.all();
+        next.template read<LV>(sV, lvc, 32, 16 * NV * w, weights + 32);
+        S.scale(0, total);
+        S.template add<NS, ET>(
+            sK, lkc, 0, v,
+            [&](int t) {
+                if (t + 1 < D / 16) S.scale(t + 1, total);
 #pragma unroll
-        for (int k0 = 0; k0 < C; k0 += 32) {
-            Frag<ET> vw[NV][NS];
-#pragma unroll
-            for (int x = 0; x < NV; ++x)
-                weigh<ET>(col_frag<LV>(sV, lvc, k0, 16 * NV * w, 4 * x), (REV ? d.in : d.out) + k0 + 8 * g, vw[x]);
-            S.template add<NS, ET>(sK, lkc, k0, vw);
-        }
+                for (int i = t * next.PARTS * 16 / D; i < (t + 1) * next.PARTS * 16 / D; ++i) next.part(i);
+            });
+        S.template add<NS, ET>(sK, lkc, 32, next, [](int) {});
     }
     const int64_t at = ((int64_t)b * a.Hv + h) * a.nseg + seg;
     S.store(a.s + at * a.dk * a.dv, a.dk, a.dv, c0, 0);
