@@ -394,7 +394,8 @@ struct Shared {
     static constexpr bool SUM_OVER_Q = SUM * sizeof(float4) <= G * C * LK::LD * sizeof(ET);
     float4 own_sum[G == 2 && !SUM_OVER_Q ? SUM : 1];
     // where Q' was, once it is used: the waves' sums of M, [NW][C]
-    __device__ __forceinline__ double *cross() { return reinterpret_cast<double *>(Q[0] + (TAKEN ? C * LP::LD + C * LV::LD : 0)); }
+    using Cross = std::conditional_t<std::is_same_v<ET, float>, double, float>;
+    __device__ __forceinline__ Cross *cross() { return reinterpret_cast<Cross *>(Q[0] + (TAKEN ? C * LP::LD + C * LV::LD : 0)); }
     __device__ __forceinline__ ET *p(int i) { return TAKEN ? Q[0] : own_p[i]; }
     __device__ __forceinline__ ET *x() { return TAKEN ? Q[0] + C * LP::LD : own_x; }
     __device__ __forceinline__ float4 *sum() { return SUM_OVER_Q ? reinterpret_cast<float4 *>(Q[0]) : own_sum; }
@@ -525,6 +526,15 @@ __device__ __forceinline__ Block block(int e) {
 // Workgroups go to the 8 XCDs in turn, each with its own L2: an order in which neighbours, the heads that share a key head,
 // stay on one.
 __device__ __forceinline__ int xcd_order(int i, int n) { return n % 8 == 0 ? (i % 8) * (n / 8) + i / 8 : i; }
+
+// The sum over 16 lanes.
+__device__ __forceinline__ float sum16(float x) { return row16_allreduce(x); }
+__device__ __forceinline__ double sum16(double x) {
+    x += dpp_mov_f64<DPP_QUAD_1032>(x);
+    x += dpp_mov_f64<DPP_QUAD_2301>(x);
+    x += dpp_mov_f64<DPP_ROW_HALF_MIRROR>(x);
+    return x + dpp_mov_f64<DPP_ROW_MIRROR>(x);
+}
 
 // Waves to a SIMD that the registers have to allow.
 template <typename ET, int D>
@@ -674,7 +684,7 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
         float2 gr[BLOCKS], gs[BLOCKS][4];
         const auto read_decays = [&] {
 #pragma unroll
-                for (int e = 0; e < BLOCKS; ++e) {
+            for (int e = 0; e < BLOCKS; ++e) {
                 const Block k = block<REV>(w + NW * e);
                 gr[e] = sh.d[grp].G[(k.r0 + li) & (C - 1)];
 #pragma unroll
@@ -715,12 +725,13 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
         }
         __syncthreads();
         if (i < last) fetch(after, 2);
-        // M of the same blocks, its sums over outputs and sources apart in 64 bits: their difference from a token on is the sum
-        // of the pairs that cross it
+        // M of the same blocks, its sums over outputs and sources apart (fp32 inputs: in 64 bits): their difference from a token
+        // on is the sum of the pairs that cross it
         if constexpr (KIND == DV) {
+            using Cross = typename Shared<ET, D, NV, NW, KIND, G>::Cross;
             const int lv = LV::row_lane(li, g);
-            double *cross = sh.cross() + w * C;
-            cross[l] = 0.;
+            Cross *cross = sh.cross() + w * C;
+            cross[l] = 0;
 #pragma unroll
             for (int e = 0; e < BLOCKS; ++e) {
                 if (e == BLOCKS - 1 && !last_block) continue;
@@ -729,17 +740,14 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
 #pragma unroll
                 for (int i = 0; i < 16 * NV * NW; i += 32)
                     x = mma(row_frag<LV>(sh.V, lv, k.s0, i), row_frag<LV>(sh.x(), lv, k.r0, i), x);
-                double out = 0.;
+                Cross out = 0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int s = k.s0 + 4 * g + j;
-                    double m = s > k.r0 + li ? (double)x[j] * (double)acc[e][j] : 0.;
+                    const Cross p = (Cross)x[j] * (Cross)acc[e][j], m = s > k.r0 + li ? p : 0;
                     out += m;
-                    m += dpp_mov_f64<DPP_QUAD_1032>(m);
-                    m += dpp_mov_f64<DPP_QUAD_2301>(m);
-                    m += dpp_mov_f64<DPP_ROW_HALF_MIRROR>(m);
-                    m += dpp_mov_f64<DPP_ROW_MIRROR>(m);
-                    if (li == 0) cross[s] += m;
+                    const Cross sum = sum16(m);
+                    if (li == 0) cross[s] += sum;
                 }
                 out += __shfl_xor(out, 16);
                 out += __shfl_xor(out, 32);
@@ -823,10 +831,10 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
             __syncthreads();
             if (w == 0) {
                 const int t = C - 1 - l;
-                const double *const x0 = sh.cross() + t;
+                const auto *const x0 = sh.cross() + t;
                 double x = 0.;
 #pragma unroll
-                for (int i = 0; i < NW; ++i) x += x0[i * C];
+                for (int i = 0; i < NW; ++i) x += (double)x0[i * C];
                 const double s = wave_prefix_sum(x);
                 if (t < n) a.dot[at + t] = (float)s;
             }
