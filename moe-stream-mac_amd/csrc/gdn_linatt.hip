@@ -101,21 +101,32 @@ __global__ __launch_bounds__(64 * DW) void dg_kernel(const DecayGrad a) {
         const int64_t head = (int64_t)b * a.Hv + h;
         double D = 0.;
         if (a.dlast) {
-            for (int64_t i = threadIdx.x; i < a.size; i += 64 * DW)
-                D = fma((double)a.dlast[head * a.size + i], (double)a.last[head * a.size + i], D);
+            const float *x = a.dlast + head * a.size, *y = a.last + head * a.size;
+#pragma unroll 8
+            for (int i = threadIdx.x; i < (int)a.size; i += 64 * DW) D = fma((double)x[i], (double)y[i], D);
             D = block_sum(D, red, DW);
         }
+        // the first slices' numbers of a turn are loaded during the turn before
+        float na, nb, nx;
+        const auto fetch = [&](int c) {
+            const int64_t t = (int64_t)c * C + C - 1 - l, at = head * a.T + (c >= 0 && t < a.T ? t : 0);
+            na = a.a[at];
+            nb = a.b[at];
+            nx = a.cross[at];
+        };
+        fetch(a.nc - 1 - w);
         for (int c1 = a.nc - 1; c1 >= 0; c1 -= DW) {
             const int c = c1 - w;  // later chunks in lower waves, later tokens in lower lanes
             const int64_t t = (int64_t)c * C + C - 1 - l;
             const bool in = c >= 0 && t < a.T;
-            double xa = 0., xb = 0., x = 0.;
+            double xa = in ? na : 0., xb = in ? nb : 0., x = in ? nx : 0.;
+            if (c1 >= DW) fetch(c - DW);
             if (in) {
-                for (int s = 0; s < a.slices; ++s) {
+                for (int s = 1; s < a.slices; ++s) {
                     xa += (double)a.a[(s * heads + head) * a.T + t];
                     xb += (double)a.b[(s * heads + head) * a.T + t];
                 }
-                for (int s = 0; s < a.cross_slices; ++s) x += (double)a.cross[(s * heads + head) * a.T + t];
+                for (int s = 1; s < a.cross_slices; ++s) x += (double)a.cross[(s * heads + head) * a.T + t];
             }
             xa = wave_prefix_sum(xa);
             xb = wave_prefix_sum(xb);
