@@ -121,6 +121,27 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def written(tensors) -> None:
+    """Tensors that a kernel changed in place: autograd refuses to go back through what had saved their old values."""
+    torch.autograd.graph.increment_version(tensors)
+
+
+class _Once(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, n, *inputs_and_grads):
+        return inputs_and_grads[n:]
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise RuntimeError("gradients of this operator cannot be differentiated twice")
+
+
+def once(inputs, *grads):
+    """A backward pass's results: with create_graph, ones that raise when they are differentiated in what they depend on,
+    its ``inputs``, instead of constants."""
+    return _Once.apply(len(inputs), *inputs, *grads) if torch.is_grad_enabled() else grads
+
+
 def profile_enable(on: bool) -> None:
     load().gdn_profile_enable(1 if on else 0)
 

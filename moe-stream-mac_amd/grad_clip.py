@@ -99,7 +99,9 @@ def clip_grad_norm(grads: Iterable[Array], max_norm: float, norm_type: float = 2
                             set(map(_index, os_)) != {gs[0].get_device()} or set(map(_layout, os_)) != {torch.strided}):
         raise ValueError("out must hold one tensor of the same shape, type and device for each gradient")
     if all(map(_contiguous, gs)) and (os_ is gs or all(map(_contiguous, os_))):
-        return _call(gs, os_, max_norm, float(norm_type), eps)
+        norm = _call(gs, os_, max_norm, float(norm_type), eps)
+        L.written(os_)
+        return norm
     # memory order does not matter to the kernels where input and output share it; others go through a copy
     src, dst, back = [], [], []
     for g, o in zip(gs, os_):
@@ -114,4 +116,5 @@ def clip_grad_norm(grads: Iterable[Array], max_norm: float, norm_type: float = 2
     norm = _call(src, dst, max_norm, float(norm_type), eps)
     for o, tmp in back:
         o.copy_(tmp)
+    L.written(os_)
     return norm

@@ -42,8 +42,9 @@ def _check(q: Array, k: Array, v: Array, g: Array, state: Optional[Array], lead:
         raise ValueError("all inputs must be on the same device")
 
 
-def _channels(t: Array) -> Array:
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+def _rows(t: Array) -> Array:
+    """t with channels side by side and tokens less than 2^22 elements apart, what the kernels take."""
+    return t if (t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(1) < 1 << 22 else t.contiguous()
 
 
 def _strides(q: Array, k: Array, v: Array, g: Array):
@@ -52,10 +53,8 @@ def _strides(q: Array, k: Array, v: Array, g: Array):
 
 
 def _forward(q, k, v, g, state, scale):
-    """(y, last), and what the backward needs: (q, k, v, state, saved)."""
-    q, k, v = _channels(q), _channels(k), _channels(v)
+    """y, the final state and what the backward needs of the states between."""
     (B, T, Hk, Dk), (Hv, Dv), dev = q.shape, v.shape[2:], q.device
-    state = None if state is None else state.contiguous()
     y = torch.empty((B, T, Hv, Dv), dtype=q.dtype, device=dev)
     last = torch.empty((B, Hv, Dv, Dk), dtype=torch.float32, device=dev)
     lib = L.load()
@@ -65,14 +64,14 @@ def _forward(q, k, v, g, state, scale):
         L.check(lib.gdn_linatt_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), L.ptr(state), y.data_ptr(),
                                    last.data_ptr(), saved.data_ptr(), n, _strides(q, k, v, g), B, T, Hk, Hv, Dk, Dv, scale,
                                    L.DTYPE_CODE[q.dtype], L.DTYPE_CODE[g.dtype], L.stream_handle(dev)))
-    return (y, last), (q, k, v, state, saved)
+    return y, last, saved
 
 
 class _LinearAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, state, scale):
         ctx.set_materialize_grads(False)
-        (y, last), (q, k, v, state, saved) = _forward(q, k, v, g, state, scale)
+        y, last, saved = _forward(q, k, v, g, state, scale)
         ctx.save_for_backward(q, k, v, g, state, last, saved)
         ctx.scale = scale
         return y, last
@@ -99,7 +98,7 @@ class _LinearAttention(torch.autograd.Function):
                                        ws.data_ptr(), n, _strides(q, k, v, g), B, T, Hk, Hv, Dk, Dv, ctx.scale,
                                        int(g.dim() == 1), L.DTYPE_CODE[q.dtype], L.DTYPE_CODE[g.dtype],
                                        L.stream_handle(dev)))
-        return dq, dk, dv, dg, dstate, None
+        return (*L.once((q, k, v, g, state, dy, dlast), dq, dk, dv, dg, dstate), None)
 
 
 def linear_attention(q: Array, k: Array, v: Array, g: Array, state: Optional[Array] = None, *,
@@ -116,10 +115,11 @@ def linear_attention(q: Array, k: Array, v: Array, g: Array, state: Optional[Arr
         B, (Hv, Dv) = q.shape[0], v.shape[2:]
         last = q.new_zeros((B, Hv, Dv, q.shape[-1]), dtype=torch.float32) if state is None else state.float().clone()
         return v.new_empty((*q.shape[:2], Hv, Dv)), last
-    state = None if state is None else state.float()
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    state = None if state is None else state.float().contiguous()
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, g, state)):
         return _LinearAttention.apply(q, k, v, g, state, scale)
-    return _forward(q, k, v, g, state, scale)[0]
+    return _forward(q, k, v, g, state, scale)[:2]
 
 
 def linear_attention_step(q: Array, k: Array, v: Array, g: Array, state: Array, *,
@@ -139,4 +139,5 @@ def linear_attention_step(q: Array, k: Array, v: Array, g: Array, state: Array, 
                                          y.data_ptr(), *gs, B, Hk, Hv, Dk, Dv,
                                          Dk ** -0.5 if scale is None else float(scale), L.DTYPE_CODE[q.dtype],
                                          L.DTYPE_CODE[g.dtype], L.stream_handle(dev)))
+    L.written((state,))
     return y

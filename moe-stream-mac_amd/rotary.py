@@ -77,7 +77,7 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dq, dk):
         pos, inv = ctx.saved_tensors
-        return (*_launch(dq, dk, pos, inv, *ctx.meta, True), None, None, None, None)
+        return (*L.once((dq, dk), *_launch(dq, dk, pos, inv, *ctx.meta, True)), None, None, None, None)
 
 
 def rotary(q: Array, k: Array, positions: Array, inv_freq: Array, *, interleaved: bool = False,

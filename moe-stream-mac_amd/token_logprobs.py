@@ -45,10 +45,9 @@ def _rows(z: Array) -> tuple[Array, tuple[int, int, int, int]]:
     return z, (o, i, so, si)
 
 
-def _forward(z, targets, entropy, top, ignore_index, need_grad):
-    """(logp, entropy, ids, top_logp), and what the backward needs: (z, row layout, statistics)."""
+def _forward(z, layout, targets, entropy, top, ignore_index, need_grad):
+    """(logp, entropy, ids, top_logp), and the rows' statistics for the backward."""
     dev, lead, V = z.device, z.shape[:-1], z.shape[-1]
-    z, layout = _rows(z)
     rows = targets.numel()
     f32 = dict(dtype=torch.float32, device=dev)
     logp = torch.empty(lead, **f32)
@@ -64,14 +63,14 @@ def _forward(z, targets, entropy, top, ignore_index, need_grad):
         L.check(lib.gdn_logprobs_fwd(z.data_ptr(), targets.data_ptr(), logp.data_ptr(), L.ptr(ent), L.ptr(stat),
                                      L.ptr(ids), L.ptr(tlp), ws.data_ptr(), nws, outer, inner, V, so, si,
                                      ignore_index, top, L.DTYPE_CODE[z.dtype], L.stream_handle(dev)))
-    return (logp, ent, ids, tlp), (z, layout, stat)
+    return (logp, ent, ids, tlp), stat
 
 
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, z, targets, entropy, top, ignore_index):
+    def forward(ctx, z, layout, targets, entropy, top, ignore_index):
         ctx.set_materialize_grads(False)
-        out, (z, layout, stat) = _forward(z, targets, entropy, top, ignore_index, True)
+        out, stat = _forward(z, layout, targets, entropy, top, ignore_index, True)
         ctx.save_for_backward(z, targets, stat, out[1])
         ctx.meta = (*layout, ignore_index, z.shape)
         ctx.mark_non_differentiable(*[t for t in out[2:] if t is not None])
@@ -83,7 +82,7 @@ class _TokenLogprobs(torch.autograd.Function):
         outer, inner, so, si, ignore_index, shape = ctx.meta
         dev = z.device
         if dlogp is None and dent is None:
-            return (None,) * 5
+            return (None,) * 6
         dlogp = None if dlogp is None else dlogp.float().contiguous()
         dent = None if dent is None else dent.float().contiguous()
         dz = torch.empty(shape, dtype=z.dtype, device=dev)
@@ -91,7 +90,7 @@ class _TokenLogprobs(torch.autograd.Function):
             L.check(L.load().gdn_logprobs_bwd(z.data_ptr(), targets.data_ptr(), stat.data_ptr(), L.ptr(ent),
                                               L.ptr(dlogp), L.ptr(dent), dz.data_ptr(), outer, inner, shape[-1], so, si,
                                               ignore_index, L.DTYPE_CODE[z.dtype], L.stream_handle(dev)))
-        return dz, None, None, None, None
+        return (*L.once((z, dlogp, dent), dz), None, None, None, None, None)
 
 
 def token_logprobs(logits: Array, targets: Array, *, entropy: bool = False, top: int = 0,
@@ -116,7 +115,7 @@ def token_logprobs(logits: Array, targets: Array, *, entropy: bool = False, top:
         raise RuntimeError("token_logprobs runs on a ROCm GPU only; got tensors on " + str(logits.device))
     if targets.device != logits.device:
         raise ValueError("all inputs must be on the same device")
-    args = (logits, targets.to(torch.int64).contiguous(), bool(entropy), int(top), int(ignore_index))
+    args = (*_rows(logits), targets.to(torch.int64).contiguous(), bool(entropy), int(top), int(ignore_index))
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*_TokenLogprobs.apply(*args))
     return TokenLogprobs(*_forward(*args, False)[0])

@@ -269,3 +269,62 @@ def test_graph_and_other_stream(dev):
         got = [t.clone() for t in held]
         for a, b in zip(got, work()):
             assert torch.equal(a, b), i
+
+
+# four and six value heads on a key head (dq and dk of two heads added in one workgroup, the pairs afterwards), odd ratios
+# (each head for itself), values too wide for two heads at a time; several segments
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [(1, 200, 1, 4, 128, 128), (2, 70, 2, 12, 64, 40), (1, 530, 1, 6, 64, 136), (1, 410, 1, 3, 256, 96),
+                                  (1, 330, 1, 4, 255, 128)])
+def test_heads_that_share_a_key_head(dev, size, dtype):
+    print("linear attention", size, dtype, flush=True)
+    check(dev, *size, dtype, per_head=size[3] == 12, seed=size[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_broadcast_inputs_and_far_apart_tokens(dev, dtype):
+    """One key head expanded over three, one sequence's decays over the batch, a cotangent of one number; tokens 2^22 elements
+    apart are copied.  The same bits twice: nothing depends on an order of arrival."""
+    from linear_attention import linear_attention
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(11)
+    n = lambda *s: torch.randn(*s, device=dev, generator=gen)  # noqa: E731
+    q, k, v = n(2, 150, 1, 64).to(dtype), n(2, 150, 1, 64).to(dtype), n(2, 150, 3, 32).to(dtype)
+    g = -torch.rand(1, 150, 3, device=dev, generator=gen)
+    leaves = [x.requires_grad_(True) for x in (q, k, v, g)]
+
+    def run():
+        y, last = linear_attention(q.expand(-1, -1, 3, -1), k.expand(-1, -1, 3, -1), v, g.expand(2, -1, -1))
+        return y, last, torch.autograd.grad(y.float().sum(), leaves)
+
+    y, last, grads = run()
+    want = recurrence64(q, k, v, g, None, 0.125, torch.ones_like(y), torch.zeros_like(last))
+    out, st = bounds(dtype)
+    near(y, want[0], out, "y")
+    near(last, want[1], st, "last")
+    for got, w, name in zip(grads, (*want[2:5], want[5].sum(0, keepdim=True)), ("dq", "dk", "dv", "dg")):
+        # torch adds the three heads' gradients in dtype: two more roundings
+        near(got, w, out + 2 * torch.finfo(dtype).eps / 2, name)
+    y2, last2, grads2 = run()
+    assert torch.equal(y, y2) and torch.equal(last, last2) and all(map(torch.equal, grads, grads2))
+    far = torch.zeros(3, 1 << 22, device=dev, dtype=dtype)
+    far[:, :64] = q.detach()[0, :3, 0]
+    x = far.as_strided((1, 3, 1, 64), (3 << 22, 1 << 22, 64, 1))
+    with torch.no_grad():
+        assert torch.equal(linear_attention(x, k[:1, :3], v[:1, :3], g[:, :3])[0],
+                           linear_attention(q[:1, :3], k[:1, :3], v[:1, :3], g[:, :3])[0])
+
+
+def test_stale_and_second_gradients_are_refused(dev):
+    """A final state that a step has overwritten is not read by the backward pass, and gradients have none of their own."""
+    from linear_attention import linear_attention, linear_attention_step
+    q, k, v, g, state, dy, _ = inputs(dev, 1, 20, 1, 2, 64, 64, torch.float32, False, True, 12)
+    q.requires_grad_(True)
+    y, last = linear_attention(q, k, v, g, state)
+    linear_attention_step(q[:, 0], k[:, 0], v[:, 0], g[:, 0], last)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad((y * dy).sum(), q)
+    y, _ = linear_attention(q, k, v, g, state)
+    (dq,) = torch.autograd.grad((y * dy).sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(dq.sum(), q)
