@@ -23,6 +23,15 @@
 //   P and the state as operands of Y, once (2^-8 of an element at most, as the output's own rounding);
 //   the state in the passes that a and b are formed from, in two terms (2^-17): the chain subtracts them;
 //   e^{G_C - G_s} v_s in three terms (2^-26): the final state is an fp32 output.
+//
+// What bounds the passes is the issue of instructions, not memory: 4 sequences of 4096 tokens, 16 key and 32 value heads of 128
+// channels, bf16: Y 149 us, DQ and DK 179 each, DV 183, a segment sum 80, for 0.3 to 0.4 GB of traffic each (60 to 80 us at
+// the card's copy rate).  A wave's matrix instructions (Y: 152 of 16 cycles in a chunk) and its vector instructions (decays,
+// the state and V' split into bf16 terms, tiles to LDS) take the SIMD's time one after the other, and two waves to a SIMD
+// leave little of it idle.  Measured along the way: loads under branches, each waited for where it stands, and one workgroup
+// to a CU: Y 295 us, DQ 367.  LDS rows padded instead of permuted (three times the conflicts) and X loaded behind the next
+// tiles: DQ 269, DV 245.  P in sixteen blocks instead of the twelve that count, weights formed ahead of all products instead
+// of between them, and a chunk's loads all at one place: Y 161, DQ 208, DV 203.
 #pragma once
 
 #include <type_traits>
@@ -166,15 +175,6 @@ __device__ __forceinline__ void split(const float (&x)[8], F32Frag (&o)[N]) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) o[0].v[j] = x[j];
 }
-__device__ __forceinline__ void to_f32(const bf8 &a, float (&x)[8]) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = (float)a[j];
-}
-__device__ __forceinline__ void to_f32(const F32Frag &a, float (&x)[8]) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = a.v[j];
-}
-
 // A tensor [B][T][heads][D], channels contiguous; value head h reads head h / div.
 struct Ten {
     const void *p;
@@ -192,8 +192,8 @@ struct __attribute__((packed, aligned(2))) u4_any {
     u4 v;
 };
 
-// A [C][W] tile in registers on its way from memory to LDS, 8 channels to a piece, by N threads; rows >= n and columns >= w are zero.  VEC:
-// w is a multiple of 8 (or none is left), pieces are loaded whole.  No load stands under a branch, where it would be waited
+// A [C][W] tile in registers on its way from memory to LDS, 8 channels to a piece, by N threads; rows >= n and columns >= w are
+// zero.  VEC: w is a multiple of 8 (or none is left), pieces are loaded whole.  No load stands under a branch, where it would be waited
 // for: rows and columns out of range load ones in range, and turn to zeros on the way to LDS.
 template <typename ET, int W, bool VEC, int N = NT>
 struct Tile {
@@ -540,7 +540,10 @@ __device__ __forceinline__ double sum16(double x) {
 template <typename ET, int D>
 constexpr int waves() { return std::is_same_v<ET, bf16> && D <= 128 ? 2 : 1; }
 
-// One segment of G value heads, 64 NV columns of V'.
+// One segment of G value heads, 16 NV NW columns of V'.  The state stays in the accumulators of the products that sum it, laid
+// out so that it is an operand of the next chunk's O as it stands; tiles pass once from memory through registers, a chunk
+// ahead, to LDS.  32 columns to a wave: every operand read from LDS serves two products (state, V') or is shared by all waves
+// (P).  O is formed transposed, so that a lane stores consecutive channels.
 template <typename ET, int D, int NV, int NW, int KIND, int G, bool VEC>
 __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(const Pass a) {
     constexpr bool F32 = std::is_same_v<ET, float>, REV = KIND >= DK, DOT = KIND == DQ || KIND == DK;
@@ -853,7 +856,8 @@ struct Seg {
 };
 
 // What a segment adds to a state that starts from nothing, and its decay.  The segment that the chain ends with is left out
-// (the last; reverse: the first).
+// (the last; reverse: the first).  Three quarters of the sequence's state products once more (80 us at B=4, T=4096, Hv=32), for
+// four times as many workgroups in every pass: unsplit, 128 heads leave half of 256 CUs without work.
 template <typename ET, int D, int NV, int NW, bool REV, bool VEC>
 __global__ __launch_bounds__(64 * NW, (waves<ET, D>())) void seg_kernel(const Seg a) {
     constexpr int NS = std::is_same_v<ET, float> ? 1 : 3;
@@ -959,7 +963,8 @@ void launch_seg(const Seg &a, bool rev, hipStream_t st) {
     else hipLaunchKernelGGL((seg_kernel<ET, D, NV, NW, false, VEC>), grid, block, 0, st, a);
 }
 // 128 columns of V' go to four waves of 32 in bf16 (eight of 16 read the K' and Q' tiles twice as often: 171 us against 144
-// for two sequences of 8100 tokens, 32 heads), to eight of 16 in fp32 (two waves to a SIMD: 83 us against 87 for 2047 tokens).
+// for two sequences of 8100 tokens, 32 heads, when both were tried; now 137), to eight of 16 in fp32 (two waves to a SIMD: 83 us
+// against 87 for 2047 tokens; now 80).
 template <typename ET>
 constexpr int wide_columns() { return std::is_same_v<ET, bf16> ? 2 : 1; }
 template <typename ET, int D, bool VEC>
