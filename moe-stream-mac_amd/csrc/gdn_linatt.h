@@ -25,7 +25,7 @@
 //   e^{G_C - G_s} v_s in three terms (2^-26): the final state is an fp32 output.
 //
 // What bounds the passes is the issue of instructions, not memory: 4 sequences of 4096 tokens, 16 key and 32 value heads of 128
-// channels, bf16: Y 149 us, DQ and DK 179 each, DV 183, a segment sum 80, for 0.3 to 0.4 GB of traffic each (60 to 80 us at
+// channels, bf16: Y 148 us, DQ and DK 178 each, DV 183, a segment sum 67, for 0.3 to 0.4 GB of traffic each (60 to 80 us at
 // the card's copy rate).  A wave's matrix instructions (Y: 152 of 16 cycles in a chunk) and its vector instructions (decays,
 // the state and V' split into bf16 terms, tiles to LDS) take the SIMD's time one after the other, and two waves to a SIMD
 // leave little of it idle.  Measured along the way: loads under branches, each waited for where it stands, and one workgroup
@@ -856,7 +856,7 @@ struct Seg {
 };
 
 // What a segment adds to a state that starts from nothing, and its decay.  The segment that the chain ends with is left out
-// (the last; reverse: the first).  Three quarters of the sequence's state products once more (80 us at B=4, T=4096, Hv=32), for
+// (the last; reverse: the first).  Three quarters of the sequence's state products once more (67 us at B=4, T=4096, Hv=32), for
 // four times as many workgroups in every pass: unsplit, 128 heads leave half of 256 CUs without work.
 template <typename ET, int D, int NV, int NW, bool REV, bool VEC>
 __global__ __launch_bounds__(64 * NW, (waves<ET, D>())) void seg_kernel(const Seg a) {
@@ -922,6 +922,9 @@ __global__ __launch_bounds__(64 * NW, (waves<ET, D>())) void seg_kernel(const Se
 
 // Columns of V' to a workgroup: 64, or 128 where the state of 128 fits the registers beside the tiles.
 inline int cols_of(int dk, int dv) { return dv <= 64 || dk > 128 ? 64 : 128; }
+// For segment sums in bf16 always 64: three quarters of two workgroups for each compute unit become three halves, which share
+// out evenly, three waves to a SIMD (B=4, T=4096, Hv=32: 67 us against 79; two LDS buffers at 128 columns gained nothing).
+inline int seg_cols(int dk, int dv, int dt) { return dt == DT_BF16 ? 64 : cols_of(dk, dv); }
 
 // dq and dk of two value heads are added in one workgroup where its LDS holds both.
 template <typename ET, int D>
@@ -977,9 +980,8 @@ void launch_pass_cols(const Pass &a, Kind kind, hipStream_t st) {
 }
 template <typename ET, int D, bool VEC>
 void launch_seg_cols(const Seg &a, bool rev, hipStream_t st) {
-    if constexpr (D <= 128) {
-        constexpr int NV = wide_columns<ET>();
-        if (cols_of(D, a.dv) == 128) return launch_seg<ET, D, NV, 8 / NV, VEC>(a, rev, st);
+    if constexpr (D <= 128 && std::is_same_v<ET, float>) {
+        if (seg_cols(D, a.dv, a.dt) == 128) return launch_seg<ET, D, 1, 8, VEC>(a, rev, st);
     }
     launch_seg<ET, D, 1, 4, VEC>(a, rev, st);
 }

@@ -258,7 +258,8 @@ static int scan_width(int64_t size) { return size % 4 ? 1 : 4; }
 static int scan_blocks(int64_t size) { return (int)((size + NT * scan_width(size) - 1) / (NT * scan_width(size))); }
 template <bool REV>
 static int run_segments(Seg a, const float *s0, const float *at, double *part, hipStream_t st) {
-    a.slices = slices_of(a.dk, a.dv);
+    const int cols = seg_cols(a.dk, a.dv, a.dt);
+    a.slices = (a.dv + cols - 1) / cols;
     {
         Timed tm(REV ? "linatt_segments_rev" : "linatt_segments", st);
         constexpr decltype(&seg_d64) run[] = {seg_d64, seg_d128, seg_d256, seg_odd64, seg_odd128, seg_odd256};
