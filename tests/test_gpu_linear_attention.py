@@ -328,3 +328,28 @@ def test_stale_and_second_gradients_are_refused(dev):
     (dq,) = torch.autograd.grad((y * dy).sum(), q, create_graph=True)
     with pytest.raises(RuntimeError, match="twice"):
         torch.autograd.grad(dq.sum(), q)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes", [(2, 2, 4, 128, 128), (1, 1, 2, 64, 40), (1, 1, 1, 256, 33)])
+def test_later_tokens_do_not_reach_earlier_outputs(dev, sizes, dtype):
+    """Infinite and NaN values, keys, queries and decays of a token: outputs before it are those of the clean call, in its chunk
+    too; sums may take another order (bounds)."""
+    from linear_attention import linear_attention
+    B, Hk, Hv, Dk, Dv = sizes
+    for seed, t in enumerate((5, 37, 70, 199)):
+        q, k, v, g, state, _, _ = inputs(dev, B, 200, Hk, Hv, Dk, Dv, dtype, False, True, 20 + seed)
+        clean, _ = linear_attention(q, k, v, g, state)
+        for what, bad in (("v", math.inf), ("v", math.nan), ("k", math.nan), ("q", math.inf), ("g", math.nan)):
+            x = dict(q=q.clone(), k=k.clone(), v=v.clone(), g=g.clone())
+            x[what][:, t, 0, ...] = bad
+            y, last = linear_attention(x["q"], x["k"], x["v"], x["g"], state)
+            near(y[:, :t], clean[:, :t], bounds(dtype)[0], (what, bad, t))
+            assert not bool(torch.isfinite(y[:, t, 0]).any()), (what, bad, t)
+            assert bool(torch.isfinite(last[:, 0]).all()) == (what == "q"), (what, bad, t)
+    x = v.clone()
+    x[:, 199, 0, 0] = math.nan  # one channel: the others are clean
+    y, _ = linear_attention(q, k, x, g, state)
+    near(y[..., 1:], clean[..., 1:], bounds(dtype)[0], "other channels")
+    near(y[:, :199], clean[:, :199], bounds(dtype)[0], "earlier tokens")
+    assert bool(y[:, 199, 0, 0].isnan().all())
