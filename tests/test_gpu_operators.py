@@ -327,3 +327,24 @@ def test_operators_in_a_graph_and_on_another_stream(dev):
         got = [t.clone() for t in held]
         for a, b in zip(got, work()):
             assert torch.equal(a, b), i
+
+
+def test_second_gradients_and_overwritten_tensors_are_refused(dev):
+    from grad_clip import clip_grad_norm
+    from rotary import rotary, rotary_frequencies
+    from token_logprobs import token_logprobs
+    z = torch.randn(3, 50, device=dev, requires_grad=True)
+    (dz,) = torch.autograd.grad(token_logprobs(z, torch.arange(3, device=dev)).logp.sum(), z, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(dz.sum(), z)
+    q, w = (torch.randn(1, 4, 2, 8, device=dev, requires_grad=True) for _ in range(2))
+    inv, _ = rotary_frequencies(8)
+    a, _ = rotary(q, q.detach(), torch.arange(4, device=dev), inv.to(dev))
+    (dq,) = torch.autograd.grad((a * w).sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(dq.sum(), w)
+    x = torch.randn(10, device=dev, requires_grad=True)
+    p = x.exp()  # its gradient reads p
+    clip_grad_norm([p.detach()], 1e-3)
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(p.sum(), x)
