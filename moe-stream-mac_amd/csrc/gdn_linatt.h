@@ -24,11 +24,12 @@
 //   the state in the passes that a and b are formed from, in two terms (2^-17): the chain subtracts them;
 //   e^{G_C - G_s} v_s in three terms (2^-26): the final state is an fp32 output.
 //
-// What bounds the passes is the issue of instructions, not memory: 4 sequences of 4096 tokens, 16 key and 32 value heads of 128
-// channels, bf16: Y 148 us, DQ and DK 178 each, DV 183, a segment sum 67, for 0.3 to 0.4 GB of traffic each (60 to 80 us at
-// the card's copy rate).  A wave's matrix instructions (Y: 152 of 16 cycles in a chunk) and its vector instructions (decays,
-// the state and V' split into bf16 terms, tiles to LDS) take the SIMD's time one after the other, and two waves to a SIMD
-// leave little of it idle.  Measured along the way: loads under branches, each waited for where it stands, and one workgroup
+// What bounds the passes is the issue of instructions and the waits between them, not memory: 4 sequences of 4096 tokens, 16
+// key and 32 value heads of 128 channels, bf16: Y 155 us, DQ and DK 186 each, DV 190, a segment sum 68 (up to 5% less on
+// other cards), for 0.3 to 0.5 GB of traffic each (60 to 100 us at the card's copy rate).  A wave's matrix instructions (Y:
+// 156 of 16 cycles in a chunk) and its vector instructions (some 770: decays, the state and V' split into bf16 terms, tiles
+// to LDS) take the SIMD's time one after the other, and each of its two waves spends a third of its time on a dependency and
+// a quarter at barriers.  Measured along the way: loads under branches, each waited for where it stands, and one workgroup
 // to a CU: Y 295 us, DQ 367.  LDS rows padded instead of permuted (three times the conflicts) and X loaded behind the next
 // tiles: DQ 269, DV 245.  P in sixteen blocks instead of the twelve that count, weights formed ahead of all products instead
 // of between them, and a chunk's loads all at one place: Y 161, DQ 208, DV 203.
@@ -760,26 +761,24 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
         const float total = sh.total[grp];
         const int lp = LP::row_lane(li, g), lkc = LK::template col_lane<8>(li, g);
         const auto pairs_of = [&](int k0, const Frag<ET> (&v)[NV]) {
-            // an infinite or NaN value of a later token must not reach an output through its weight of 0: where a product with
-            // zeros shows one, the sum takes the pairs that count one by one (2% of Y's time for the look).  Not in the
-            // gradients: a NaN or infinite input may make those of the whole chunk NaN.
-            if constexpr (KIND == Y) {
-                f4 z = {0.f, 0.f, 0.f, 0.f};
+            // an infinite or NaN source of a later token (reverse: an earlier one) must not reach an output through its weight
+            // of 0: where a product with zeros shows one, the sum takes the pairs that count one by one (looking costs a pass
+            // 1 to 2% of its time)
+            f4 z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int x = 0; x < NV; ++x) z = mma(v[x], Frag<ET>{}, z);
-                if (__any((z[0] + z[1]) + (z[2] + z[3]) != 0.f)) {
+            for (int x = 0; x < NV; ++x) z = mma(v[x], Frag<ET>{}, z);
+            if (__any((z[0] + z[1]) + (z[2] + z[3]) != 0.f)) {
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
+                for (int rt = 0; rt < RT; ++rt)
 #pragma unroll 1
-                        for (int s = k0; s < k0 + 32; ++s) {
-                            if (s > 16 * rt + li) continue;
-                            const float p = (float)sP[LP::at4(16 * rt + li, s & ~3) + (s & 3)];
-                            const ET *const vs = sh.V + LV::at4(s, col - c0);
+                    for (int s = k0; s < k0 + 32; ++s) {
+                        if (REV ? s < 16 * rt + li : s > 16 * rt + li) continue;
+                        const float p = (float)sP[LP::at4(16 * rt + li, s & ~3) + (s & 3)];
+                        const ET *const vs = sh.V + LV::at4(s, col - c0);
 #pragma unroll
-                            for (int j = 0; j < 4 * NV; ++j) O[rt][j / 4][j % 4] = fmaf(p, (float)vs[j], O[rt][j / 4][j % 4]);
-                        }
-                    return;
-                }
+                        for (int j = 0; j < 4 * NV; ++j) O[rt][j / 4][j % 4] = fmaf(p, (float)vs[j], O[rt][j / 4][j % 4]);
+                    }
+                return;
             }
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {

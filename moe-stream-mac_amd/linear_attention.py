@@ -107,8 +107,7 @@ def linear_attention(q: Array, k: Array, v: Array, g: Array, state: Optional[Arr
     and the log decays ``g`` [B, T, Hv], or [Hv] for one of each head; value head h reads key head h / (Hv / Hk).
 
     ``state`` is the state before the first token (None: zeros), ``scale`` defaults to Dk^-1/2.  A log decay of -inf keeps
-    nothing of the state.  A token's infinite or NaN values do not reach earlier outputs; gradients may be NaN over its
-    chunk of 64 tokens.  q, k, v and g may be strided views; heads have at most 256 channels.  Differentiable in q, k, v,
+    nothing of the state.  A token's infinite or NaN values do not reach earlier outputs.  q, k, v and g may be strided views; heads have at most 256 channels.  Differentiable in q, k, v,
     g and state (once: no second derivatives); gradients have their inputs' types."""
     _check(q, k, v, g, state, 2)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)

@@ -353,3 +353,28 @@ def test_later_tokens_do_not_reach_earlier_outputs(dev, sizes, dtype):
     near(y[..., 1:], clean[..., 1:], bounds(dtype)[0], "other channels")
     near(y[:, :199], clean[:, :199], bounds(dtype)[0], "earlier tokens")
     assert bool(y[:, 199, 0, 0].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes", [(2, 2, 4, 128, 128), (1, 1, 3, 64, 40), (1, 1, 1, 256, 33)])
+def test_nan_tokens_do_not_reach_gradients_they_have_no_part_in(dev, sizes, dtype):
+    """A NaN key from which on nothing is in the loss: dq before it is the clean one.  A NaN query whose output is not in the
+    loss: dk and dv after it are.  The same rounded operands, summed in another order: within the bounds."""
+    from linear_attention import linear_attention
+    B, Hk, Hv, Dk, Dv = sizes
+    for seed, t in enumerate((5, 37, 70, 190)):
+        q, k, v, g, state, dy, _ = inputs(dev, B, 200, Hk, Hv, Dk, Dv, dtype, False, True, 40 + seed)
+
+        def grads(q, k, dy):
+            leaves = [x.clone().requires_grad_(True) for x in (q, k, v)]
+            return torch.autograd.grad(linear_attention(*leaves, g, state)[0], leaves, dy)
+
+        bad, cut = k.clone(), dy.clone()
+        bad[:, t, 0] = math.nan
+        cut[:, t:] = 0
+        near(grads(q, bad, cut)[0][:, :t], grads(q, k, cut)[0][:, :t], bounds(dtype)[0], ("dq", t))
+        bad, cut = q.clone(), dy.clone()
+        bad[:, t, 0] = math.nan
+        cut[:, t] = 0
+        for got, want, name in list(zip(grads(bad, k, cut), grads(q, k, cut), ("dq", "dk", "dv")))[1:]:
+            near(got[:, t + 1:], want[:, t + 1:], bounds(dtype)[0], (name, t))
