@@ -301,6 +301,10 @@ struct Join {
     int pieces, top;
 };
 
+// A row of -inf alone, from its statistics: no logit above -inf and the sum 0, for which join_row leaves log s = 0.  Maxima
+// skip NaN, so that a row of NaN has M = -inf too, but its log s is NaN.
+__device__ __forceinline__ bool nothing_left(float M, float ls) { return M == -__builtin_inff() && ls == 0.f; }
+
 // Joins the pieces of a row in one wave; the lanes' sums are combined in a fixed order.
 __device__ __forceinline__ void join_row(const Join &j, int64_t row, int lane, float &M, float &ls) {
     const float4 *p = j.part + row * j.pieces;
@@ -330,7 +334,7 @@ __device__ __forceinline__ void join_row(const Join &j, int64_t row, int lane, f
             if (y != j.ignore) {
                 // a target outside the vocabulary has no probability
                 o = y < 0 || y >= j.a.V ? __builtin_nanf("") : load_as_f32(j.a.z, j.a.at(row) + y, j.a.dt);
-                if (o != -__builtin_inff()) o = o - M - ls;
+                if (!nothing_left(M, ls)) o = o - M - ls;
             }
             j.logp[row] = o;
         }
@@ -372,7 +376,7 @@ __global__ __launch_bounds__(NT) void join_top_kernel(Join j) {
             const uint64_t b = best[tid];
             const float v = unordered((uint32_t)(b >> 32));
             j.top_ids[row * j.top + tid] = (int64_t)(uint32_t)~(uint32_t)b;
-            j.top_logp[row * j.top + tid] = v == -__builtin_inff() ? v : v - M - ls;
+            j.top_logp[row * j.top + tid] = nothing_left(M, ls) ? v : v - M - ls;
         }
     }
 }
@@ -399,7 +403,7 @@ __global__ __launch_bounds__(NT) void bwd_kernel(Bwd b) {
     const bool zero = !live && (!ENT || e == 0.f);  // an ignored row: nothing to read
     if (!zero) load_piece<DT>(b.a, row, v0, x, 0.f);
     const float M = b.stat[2 * row], ls = b.stat[2 * row + 1], h = ENT ? b.entropy[row] : 0.f;
-    const bool none = M == -__builtin_inff();  // no logit left: no gradient
+    const bool none = nothing_left(M, ls);  // no gradient
 #pragma unroll
     for (int c = 0; c < E / 8; ++c) {
         const int64_t j = (int64_t)(c * NT + threadIdx.x) * 8;

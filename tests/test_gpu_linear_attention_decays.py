@@ -1,0 +1,106 @@
+"""GPU checks of the decays' gradients of linear attention: every head for itself, against the recurrence in 64 bits.
+
+dg_t = a_t <dS_t, S_{t-1}> is the sum of what crosses t: the pairs of its chunk, a_r = q_r . dq_r and b_s = k_s . dk_s of the
+parts that come through the state, and c, which a chain of a's and b's carries from chunk to chunk between products of the
+states themselves.
+
+Tolerances, of one head's gradients as a whole (2-norms), so that no head hides behind another.  e is the error of an a or a b
+relative to the norms that enter it: for bf16 inputs the state goes into them in two terms of 8 bits (2^-16 at most), for fp32
+and fp16 inputs they are fp32 sums of up to 128 terms (2^-24 each, independent: 2^-20 is far above).  The products of the states
+are at most 8 chunks apart and the chain runs from the nearer end, so c carries the errors of at most 4 * 64 a's and as many b's,
+independent ones: with memories of tau tokens, e sqrt(512 / tau) of a c, below 8 e for memories from 8 tokens on (shorter ones
+hold nothing at a chunk's end).  8 * 2^-16 = 2^-13 per token, 2^-17 in fp32; twice that, as half a step is not the error's only
+source.  One decay for a head adds up its tokens: within 8 chunks the error of c is one number for all of them, while the
+gradients themselves add up as tau-long stretches: another factor sqrt(512 / tau) < 8.
+"""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    import gdn_lib
+    gdn_lib.load()
+    return torch.device("cuda:0")
+
+
+def tolerance(dtype):
+    """(per token, per head)"""
+    t = 2.0 ** -12 if dtype == torch.bfloat16 else 2.0 ** -16
+    return t, 8 * t
+
+
+def decays64(q, k, v, g, state, scale, dy, dlast=None):
+    """dL/dg of every token [B, T, Hv], float64: no state but the present one is kept, as dg_t = dg_{t+1} + q_t . dq_t - k_t . dk_t
+    and the rounding of 64 bits leaves room for the differences."""
+    q, k, v, g, dy = (t.detach().double() for t in (q, k, v, g, dy))
+    B, T, Hk, Dk = q.shape
+    Hv = v.shape[2]
+    a = g.expand(B, T, Hv).exp()[..., None, None]
+    q, k = (x.repeat_interleave(Hv // Hk, 2).transpose(0, 1).contiguous() for x in (q, k))
+    v, dy = v.transpose(0, 1).contiguous(), dy.transpose(0, 1).contiguous()
+    S = q.new_zeros(B, Hv, v.shape[-1], Dk) if state is None else state.detach().double().clone()
+    out = q.new_empty(T, B, Hv)
+    for t in range(T):
+        S = a[:, t] * S + v[t, ..., None] * k[t, ..., None, :]
+        out[t] = scale * ((S * dy[t, ..., None]).sum(-2) * q[t]).sum(-1)
+    D = torch.zeros_like(S) if dlast is None else dlast.double().clone()
+    run = (D * S).sum((-1, -2))
+    for t in range(T - 1, -1, -1):
+        D = D + scale * dy[t, ..., None] * q[t, ..., None, :]
+        run = run + out[t] - ((D * v[t, ..., None]).sum(-2) * k[t]).sum(-1)
+        out[t] = run
+        D = a[:, t] * D
+    return out.transpose(0, 1)
+
+
+def states64(q, k, v, g, state, scale, dy, dlast=None):
+    """The same from the states of all tokens, for short sequences: exact where single terms are large."""
+    q, k, v, g, dy = (t.detach().double() for t in (q, k, v, g, dy))
+    B, T, Hk, Dk = q.shape
+    Hv = v.shape[2]
+    q, k = (x.repeat_interleave(Hv // Hk, 2) for x in (q, k))
+    a = g.expand(B, T, Hv).exp()[..., None, None]
+    S = [q.new_zeros(B, Hv, v.shape[-1], Dk) if state is None else state.detach().double()]
+    for t in range(T):
+        S.append(a[:, t] * S[-1] + v[:, t, :, :, None] * k[:, t, :, None, :])
+    D = torch.zeros_like(S[0]) if dlast is None else dlast.double()
+    out = q.new_empty(B, T, Hv)
+    for t in range(T - 1, -1, -1):
+        D = D + scale * dy[:, t, :, :, None] * q[:, t, :, None, :]
+        out[:, t] = (D * S[t]).sum((-1, -2)) * a[:, t, :, 0, 0]
+        D = a[:, t] * D
+    return out
+
+
+def each_head(got, want, rel, what):
+    """2-norms over everything but the last axis."""
+    got, want = got.detach().double().flatten(0, -2), want.flatten(0, -2)
+    assert bool(torch.isfinite(got).all()), what
+    err = (got - want).norm(dim=0) / want.norm(dim=0).clamp_min(1e-30)
+    print(what, f"{float(err.max()):.3g} of {rel:.3g}", flush=True)
+    assert float(err.max()) <= rel, (what, err.tolist(), rel)
+
+
+def inputs(dev, B, T, Hk, Hv, Dk, Dv, dtype, seed):
+    gen = torch.Generator(device=dev)
+    gen.manual_seed(seed)
+    n = lambda *s: torch.randn(*s, device=dev, generator=gen)  # noqa: E731
+    q, k, v = n(B, T, Hk, Dk).to(dtype), n(B, T, Hk, Dk).to(dtype), n(B, T, Hv, Dv).to(dtype)
+    g = -torch.exp2(-torch.linspace(0.0, 12.0, Hv, device=dev))  # memories of one token to thousands
+    return q, k, v, g, n(B, Hv, Dv, Dk), n(B, T, Hv, Dv).to(dtype), n(B, Hv, Dv, Dk)
+
+
+def gradient(q, k, v, g, state, dy, dlast=None):
+    from linear_attention import linear_attention
+    g = g.detach().clone().requires_grad_(True)
+    y, last = linear_attention(q, k, v, g, state)
+    outs, cots = ([y], [dy]) if dlast is None else ([y, last], [dy, dlast])
+    return torch.autograd.grad(outs, g, cots)[0]
