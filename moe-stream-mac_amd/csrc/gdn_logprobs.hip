@@ -396,7 +396,7 @@ __global__ __launch_bounds__(NT) void bwd_kernel(Bwd b) {
     const int64_t left = b.a.V - v0, y = b.target[row];
     const bool live = y != b.ignore;
     float d = live && b.dlogp ? b.dlogp[row] : 0.f;
-    if (live && (y < 0 || y >= b.a.V)) d = __builtin_nanf("");  // as its logp
+    if (live && b.dlogp && (y < 0 || y >= b.a.V)) d = __builtin_nanf("");  // as its logp, where that is in the loss
     const float e = ENT ? b.dent[row] : 0.f;
     const int64_t out = row * b.a.V + v0;
     float x[E] = {};

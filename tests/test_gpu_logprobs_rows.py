@@ -1,4 +1,5 @@
-"""GPU checks of the log probabilities of rows that hold NaN, and of their gradients, against a plain 64-bit form.
+"""GPU checks of the log probabilities of rows that hold NaN and of targets outside the vocabulary, and of their gradients,
+against plain 64-bit forms.
 
 A row with a NaN logit has no log probability, entropy or gradient that is a number, whatever else it holds: its sum is NaN.
 Rows of nothing but -inf (banned tokens) are something else: log probabilities -inf, entropy 0, no gradient.
@@ -59,3 +60,26 @@ def test_rows_of_nan(dev, V, dtype):
         assert bool(torch.isfinite(dz[[5, 8]]).all()) and bool(dz[[5, 8]].any(-1).all())
         if len(loss) == 1 and loss[0] is r.logp:
             assert not bool(dz[6].any())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_targets_outside_the_vocabulary(dev, dtype):
+    """They make their own log probability NaN and the gradient of a loss that it is part of; the entropy of the row does not
+    depend on its target, nor does the entropy's gradient.  Bound: as in the other tests of dlogits, a few 2^-23 of the terms
+    (each below |x| + H < 40 times its probability) and the output's own rounding."""
+    from token_logprobs import token_logprobs
+    z = (3 * torch.randn(4, 9001, device=dev)).to(dtype).requires_grad_(True)
+    y = torch.tensor([9001, -1, 7, -100], device=dev)
+    w = torch.randn(4, device=dev)
+    r = token_logprobs(z, y, entropy=True)
+    assert r.logp.isnan().tolist() == [True, True, False, False] and bool(torch.isfinite(r.entropy).all())
+    (dz,) = torch.autograd.grad([r.entropy], [z], [w], retain_graph=True)
+    lp = torch.log_softmax(z.detach().double(), -1)
+    p = lp.exp()
+    H = -(p * lp).sum(-1, keepdim=True)
+    want = -w.double()[:, None] * p * (lp + H)
+    room = w.double().abs()[:, None] * p * 40 * 2 ** -16 + want.abs() * torch.finfo(dtype).eps / 2
+    room = room + torch.finfo(dtype).smallest_normal
+    assert bool(((dz.double() - want).abs() <= room).all())
+    (dz,) = torch.autograd.grad([r.logp, r.entropy], [z], [w, w])
+    assert bool(dz[:2].isnan().all()) and bool(torch.isfinite(dz[2:]).all())
