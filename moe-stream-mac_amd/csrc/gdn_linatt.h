@@ -394,7 +394,7 @@ struct Shared {
     float total[G], dot[DOT ? G : 1][DOT ? NW : 1][DOT ? C : 1];
     static constexpr bool SUM_OVER_Q = SUM * sizeof(float4) <= G * C * LK::LD * sizeof(ET);
     float4 own_sum[G == 2 && !SUM_OVER_Q ? SUM : 1];
-    // where Q' was, once it is used: the waves' sums of M, [NW][C]
+    // where Q' was, once it is used: the waves' sums of M for each token, [NW][C]
     using Cross = std::conditional_t<std::is_same_v<ET, float>, double, float>;
     __device__ __forceinline__ Cross *cross() { return reinterpret_cast<Cross *>(Q[0] + (TAKEN ? C * LP::LD + C * LV::LD : 0)); }
     __device__ __forceinline__ ET *p(int i) { return TAKEN ? Q[0] : own_p[i]; }
@@ -536,6 +536,25 @@ __device__ __forceinline__ double sum16(double x) {
     x += dpp_mov_f64<DPP_ROW_HALF_MIRROR>(x);
     return x + dpp_mov_f64<DPP_ROW_MIRROR>(x);
 }
+// Lane i of 16 receives lane i - 1 (lane 0: 0); the sum over the lanes up to its own.
+__device__ __forceinline__ float row_shr1(float x) { return dpp_mov<0x111>(x); }
+__device__ __forceinline__ double row_shr1(double x) { return dpp_mov_f64<0x111>(x); }
+__device__ __forceinline__ float prefix16(float x) {
+    x += dpp_mov<0x111>(x);
+    x += dpp_mov<0x112>(x);
+    x += dpp_mov<0x114>(x);
+    return x + dpp_mov<0x118>(x);
+}
+__device__ __forceinline__ double prefix16(double x) {
+    x += dpp_mov_f64<0x111>(x);
+    x += dpp_mov_f64<0x112>(x);
+    x += dpp_mov_f64<0x114>(x);
+    return x + dpp_mov_f64<0x118>(x);
+}
+__device__ __forceinline__ float xor16(float x) { return lane_xor16(x); }
+__device__ __forceinline__ float xor32(float x) { return lane_xor32(x); }
+__device__ __forceinline__ double xor16(double x) { return __shfl_xor(x, 16); }
+__device__ __forceinline__ double xor32(double x) { return __shfl_xor(x, 32); }
 
 // Waves to a SIMD that the registers have to allow.
 template <typename ET, int D>
@@ -729,34 +748,42 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
         }
         __syncthreads();
         if (i < last) fetch(after, 2);
-        // M of the same blocks, its sums over outputs and sources apart (fp32 inputs: in 64 bits): their difference from a token
-        // on is the sum of the pairs that cross it
+        // M of the same blocks, and for every token t the sum of the pairs that cross it, an output before t with a source from t
+        // on (fp32 inputs: in 64 bits).  Only those are added, none is added and taken away again: what later pairs are, large
+        // or NaN, has no part in it.  Lane t of a wave sums its blocks' part.
         if constexpr (KIND == DV) {
             using Cross = typename Shared<ET, D, NV, NW, KIND, G>::Cross;
             const int lv = LV::row_lane(li, g);
-            Cross *cross = sh.cross() + w * C;
-            cross[l] = 0;
+            Cross mine = 0;
 #pragma unroll
             for (int e = 0; e < BLOCKS; ++e) {
-                if (e == BLOCKS - 1 && !last_block) continue;
                 const Block k = block<REV>(w + NW * e);
+                if ((e == BLOCKS - 1 && !last_block) || k.s0 < k.r0) continue;
                 f4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < 16 * NV * NW; i += 32)
                     x = mma(row_frag<LV>(sh.V, lv, k.s0, i), row_frag<LV>(sh.x(), lv, k.r0, i), x);
-                Cross out = 0;
+                const bool diagonal = k.s0 == k.r0;
+                // the lane's output (column li) with its sources from each of the lane's four on
+                Cross from[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int s = k.s0 + 4 * g + j;
-                    const Cross p = (Cross)x[j] * (Cross)acc[e][j], m = s > k.r0 + li ? p : 0;
-                    out += m;
-                    const Cross sum = sum16(m);
-                    if (li == 0) cross[s] += sum;
+                for (int j = 3; j >= 0; --j) {
+                    const Cross p = (Cross)x[j] * (Cross)acc[e][j];
+                    from[j] = (!diagonal || 4 * g + j > li ? p : 0) + (j < 3 ? from[(j + 1) & 3] : 0);
                 }
-                out += __shfl_xor(out, 16);
-                out += __shfl_xor(out, 32);
-                if (g == 0) cross[k.r0 + li] -= out;
+                const Cross beside = xor16(from[0]), two = from[0] + beside, others = xor32(two);
+                const Cross after = (g & 1 ? 0 : beside) + (g < 2 ? others : 0);
+                // t among the sources: their sums over all outputs (of its own block: those before t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) from[j] = sum16(!diagonal || li < 4 * g + j ? from[j] + after : (Cross)0);
+                const Cross own = li & 2 ? (li & 1 ? from[3] : from[2]) : (li & 1 ? from[1] : from[0]);
+                const Cross sources = __shfl(own, 16 * (li >> 2) + (li & 3));
+                // t among the outputs: those before it with all sources; t in a block between: all of both
+                const Cross outputs = prefix16(two + others), before = row_shr1(outputs), all = sum16(two + others);
+                const int t0 = l & 48;
+                mine += t0 == k.s0 ? sources : t0 == k.r0 ? before : t0 > k.r0 && t0 < k.s0 ? all : (Cross)0;
             }
+            sh.cross()[w * C + l] = mine;
         }
         const float total = sh.total[grp];
         const int lp = LP::row_lane(li, g), lkc = LK::template col_lane<8>(li, g);
@@ -853,13 +880,10 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
         if constexpr (KIND == DV) {
             __syncthreads();
             if (w == 0) {
-                const int t = C - 1 - l;
-                const auto *const x0 = sh.cross() + t;
                 double x = 0.;
 #pragma unroll
-                for (int i = 0; i < NW; ++i) x += (double)x0[i * C];
-                const double s = wave_prefix_sum(x);
-                if (t < n) a.dot[at + t] = (float)s;
+                for (int i = 0; i < NW; ++i) x += (double)sh.cross()[i * C + l];
+                if (l < n) a.dot[at + l] = (float)x;
             }
         }
     }

@@ -104,3 +104,19 @@ def gradient(q, k, v, g, state, dy, dlast=None):
     y, last = linear_attention(q, k, v, g, state)
     outs, cots = ([y], [dy]) if dlast is None else ([y, last], [dy, dlast])
     return torch.autograd.grad(outs, g, cots)[0]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T,t0", [(64, 40), (61, 16), (33, 32), (64, 5)])
+def test_large_pairs_after_a_token_leave_its_gradient_alone(dev, T, t0, dtype):
+    """Values and queries 2^10 times larger from t0 on: the pairs among those tokens are 2^20 times the size of the others, and
+    dg before t0 holds none of them."""
+    q, k, v, g, _, dy, _ = inputs(dev, 2, T, 1, 3, 64, 64, dtype, T + t0)
+    late = torch.arange(T, device=dev) >= t0
+    v = torch.where(late[:, None, None], v * 2 ** 10, v)
+    k = torch.where(late[:, None, None], k * 2 ** 10, k)
+    g = g.expand(2, T, 3) * torch.rand(2, T, 3, device=dev)
+    dg = gradient(q, k, v, g, None, dy)
+    want = states64(q, k, v, g, None, 0.125, dy)
+    each_head(dg[:, 1:t0], want[:, 1:t0], tolerance(dtype)[0], f"dg before {t0} of {T}, {dtype}")
+    each_head(dg, want, tolerance(dtype)[0], f"dg of {T}, {dtype}")
