@@ -11,9 +11,11 @@
 // dg_t is what the loss draws from everything before t through everything from t on.  In t's chunk, with a_r = q_r . (dq_r
 // from the state entering it), b_s = k_s . (dk_s from the cotangent of the state leaving it) and M_rs = P_rs (dy_r . v_s):
 //   dg_t = c + sum_{r >= t} a_r + sum_{s < t} b_s + sum_{r >= t > s} M_rs,   c = e^{G_C} <dS', S>,
-// sums without cancellation, and c by the chain c = D - sum b, D of the chunk before = c + sum a, from D = <dS_T, S_T> on.  So
-// that rounding errors do not outlive what they belong to, every segment (below) starts from a D of its own, the product of the
-// states at its end, and a chunk whose decay is below 2^-30 from c = 0, which is nearer than the difference of two fp32 sums.
+// sums without cancellation.  c comes by a chain, from D, the product <dS, S> of the states between two chunks: c = D - sum b of
+// the chunk before it, c = D - sum a of the chunk after it, and D goes on as c + sum a backwards, c + sum b forwards.  Rounding
+// errors of a chain stay while what they belong to fades, so every MARK chunks DQ leaves its state and DK multiplies its own
+// with it: a chain runs at most that far, wherever the sequence is cut, and from the end whose terms are smaller.  Through a
+// chunk whose decay is below the errors of a and b nothing is passed on: c = 0.
 // So one kernel, pass_kernel, computes all four.  Where there are few heads, the sequence is cut into segments: seg_kernel
 // sums each segment's state from nothing, scan_kernel joins them to the states entering each segment, and the passes run all
 // segments at once.
@@ -46,6 +48,7 @@ namespace la {
 
 constexpr int NT = 256;
 constexpr int C = 64;  // tokens of a chunk
+constexpr int MARK = 8;  // chunks between two products of the states (512 KB of states for 4096 tokens of a head of 128 x 128)
 constexpr double LOG2E = 1.4426950408889634074;
 
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -370,6 +373,10 @@ struct Pass {
     int64_t s_head, s_seg;
     int s_t;            // states are [v'][k'] (0) or [k'][v'] (1)
     void *o;            // [B][T][heads][dv] contiguous
+    float *marks;       // DQ writes, DK reads: the states entering chunks 0, MARK, 2 MARK, .., as the lanes hold them,
+                        // [B][Hv][nm][slices][D / 16][NV][64 NW][4]
+    double *ends;       // DK: their products with the cotangents there, [B][Hv][nm][slices][NW], a wave's part each
+    int nm, mark0;      // marks of the sequence; the first that is taken (1 where the state before the first token is zero)
     float *dot;         // per token [slices][B][Hv][T]: DQ, DK X . (O from the state); DV the pairs that cross it, X = v
     int B, T, Hv, dk, dv, slices, nseg, cps, nc;  // cps: chunks of a segment, nc: of the sequence
     int dt, o_dt, pair;  // pair: two heads to a workgroup, whose outputs are added
@@ -488,6 +495,36 @@ struct State {
                 for (int e = 0; e < 8; ++e)
                     if (k + e < dk) p[tr ? (k + e) * dv + v : v * dk + k + e] = s[2 * T + e / 4][n][e % 4];
             }
+    }
+    // the state as the lanes hold it, lane `tid` of the head's
+    __device__ __forceinline__ void put(float *p, int tid) const {
+        f4 *const m = reinterpret_cast<f4 *>(p) + tid;
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+            for (int n = 0; n < NV; ++n) m[(t * NV + n) * 64 * NW] = s[t][n];
+    }
+    // the lane's part of the product with a state put there, a few loads at a time (registers)
+    __device__ __forceinline__ double product(const float *p, int tid) const {
+        const f4 *const m = reinterpret_cast<const f4 *>(p) + tid;
+        constexpr int STEP = 4 / NV;
+        double x = 0.;
+#pragma unroll
+        for (int t0 = 0; t0 < D / 16; t0 += STEP) {
+            f4 y[STEP][NV];
+#pragma unroll
+            for (int t = 0; t < STEP; ++t)
+#pragma unroll
+                for (int n = 0; n < NV; ++n) y[t][n] = m[((t0 + t) * NV + n) * 64 * NW];
+#pragma unroll
+            for (int t = 0; t < STEP; ++t)
+#pragma unroll
+                for (int n = 0; n < NV; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x = fma((double)s[t0 + t][n][e], (double)y[t][n][e], x);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        return x;
     }
     // s += K'^T diag(weights) V' over 32 rows, tile by tile, between(t) behind the products of each
     template <int NS, typename ET, typename F>
@@ -622,6 +659,11 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
         // opaque: addresses in LDS are formed where they are used, not hoisted out of the loop and spilled
         const int tid = opaque(threadIdx.x), l = tid & 63, li = l & 15, g = l >> 4;
         const int col = c0 + 16 * NV * w + 4 * NV * g;  // the lane's first column of O
+        const bool marked = DOT && c % MARK == 0 && c / MARK >= a.mark0;
+        const int64_t mark = marked ? (head * a.nm + c / MARK) * a.slices + slice : 0;
+        if constexpr (KIND == DQ) {
+            if (marked) S.put(a.marks + mark * (D * 16 * NV * NW), w * 64 + l);
+        }
         __syncthreads();
         tq.store(sh.Q[grp], n, a.dk, a.dt);
         tk.store(sh.K[grp], n, a.dk, a.dt);
@@ -867,6 +909,12 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
                 }
             }
         }
+        if constexpr (KIND == DK) {
+            if (marked) {
+                const double x = wave_prefix_sum(S.product(a.marks + mark * (D * 16 * NV * NW), w * 64 + l));
+                if (l == 63) a.ends[mark * NW + w] = x;
+            }
+        }
         const int64_t at = (((int64_t)slice * a.B + b) * a.Hv + h) * a.T + t0;
         if constexpr (DOT) {
             __syncthreads();
@@ -966,6 +1014,9 @@ __global__ __launch_bounds__(64 * NW, (waves<ET, D>())) void seg_kernel(const Se
 
 // Columns of V' to a workgroup: 64, or 128 where the state of 128 fits the registers beside the tiles.
 inline int cols_of(int dk, int dv) { return dv <= 64 || dk > 128 ? 64 : 128; }
+// Of a pass: K' channels that a kernel's tiles hold, and waves to a head.
+inline int rows_of(int dk) { return dk <= 64 ? 64 : dk <= 128 ? 128 : 256; }
+inline int waves_of(int dk, int dv, int dt) { return cols_of(dk, dv) == 128 && dt != DT_BF16 ? 8 : 4; }
 // For segment sums in bf16 always 64: three quarters of two workgroups for each compute unit become three halves, which share
 // out evenly, three waves to a SIMD (B=4, T=4096, Hv=32: 67 us against 79; two LDS buffers at 128 columns gained nothing).
 inline int seg_cols(int dk, int dv, int dt) { return dt == DT_BF16 ? 64 : cols_of(dk, dv); }

@@ -36,34 +36,22 @@ __device__ __forceinline__ double block_sum(double x, double *red, int waves) {
     return r;
 }
 
-// The segments' sums become the states entering them: from s0 (or nothing) on, in place.  With `at` (reverse), the states
-// entering the segments forwards, also the products of both at the segments' ends, <dS, S>: part [heads][nseg][blocks].
-// Streaming: 34 MB of states in and out, 12 us, and as much again to read in reverse, 20 us (128 heads of 128 x 128, four
-// segments).
+// The segments' sums become the states entering them (reverse: the cotangents, from the end): from s0 (or nothing) on, in
+// place.  Streaming: 34 MB of states in and out, 10 us (128 heads of 128 x 128, four segments).
 template <bool REV, int V>
-__global__ __launch_bounds__(NT) void scan_kernel(float *s, const float *decay, const float *s0, const float *at, double *part,
-                                                  int nseg, int64_t size) {
-    __shared__ double red[NT / 64];
+__global__ __launch_bounds__(NT) void scan_kernel(float *s, const float *decay, const float *s0, int nseg, int64_t size) {
     const int64_t head = blockIdx.y, i = ((int64_t)blockIdx.x * NT + threadIdx.x) * V;
-    const bool in = i < size;
+    if (i >= size) return;
     float cur[V] = {};
-    if (s0 && in)
+    if (s0)
         for (int e = 0; e < V; ++e) cur[e] = s0[head * size + i + e];  // at any alignment
     for (int j = 0; j < nseg; ++j) {
         const int seg = REV ? nseg - 1 - j : j;
         const int64_t p = (head * nseg + seg) * size + i;
         const float f = j < nseg - 1 ? decay[head * nseg + seg] : 0.f;
-        float add[V] = {}, S[V] = {};
-        if (j < nseg - 1 && in) ops::loadv<V>(s, p, DT_F32, add);
-        if (in) ops::storev<V>(s, p, DT_F32, cur);
-        if (REV && at && j > 0) {  // the last segment's end is the sequence's
-            if (in) ops::loadv<V>(at, p + size, DT_F32, S);
-            double x = 0.;
-#pragma unroll
-            for (int e = 0; e < V; ++e) x = fma((double)cur[e], (double)S[e], x);
-            x = block_sum(x, red, NT / 64);
-            if (threadIdx.x == 0) part[(head * nseg + seg) * gridDim.x + blockIdx.x] = x;
-        }
+        float add[V] = {};
+        if (j < nseg - 1) ops::loadv<V>(s, p, DT_F32, add);
+        ops::storev<V>(s, p, DT_F32, cur);
 #pragma unroll
         for (int e = 0; e < V; ++e) cur[e] = fmaf(f, cur[e], add[e]);
     }
@@ -85,91 +73,91 @@ struct DecayGrad {
     const float *a, *b, *cross;  // [slices][B][Hv][T]; cross: [cross_slices]
     const float *decays;         // [B][Hv][nc][DECAYS]
     const float *dlast, *last;   // [B][Hv][size], or dlast NULL
-    const double *ends;          // <dS, S> at the segments' ends but the last, [B][Hv][nseg][blocks]
-    void *dg;                    // [B][T][Hv], or [Hv]
-    int B, T, Hv, slices, cross_slices, per_head, dt, nc, cps, nseg, blocks;
+    const double *ends;          // <dS, S> before chunks 0, MARK, .., from mark0 on, [B][Hv][nm][parts]
+    void *dg;                    // [B][T][Hv]
+    double *sums;                // or with one decay per head [Hv][B][nm]
+    int B, T, Hv, slices, cross_slices, per_head, dt, nc, nm, mark0, parts;
+    float none;                  // a chunk's decay below which it passes nothing on
     int64_t size;
 };
 
-constexpr int DW = 16;  // waves
-
-// dg of one value head, from the end of each sequence backwards, in 64 bits: a wave sums one chunk, the chunks chain, sixteen
-// to a turn.  grid (Hv, B), or (Hv) per head.  Bound by the latency of its turns: 26 us at T = 4096 (four turns and <dS, S> at
-// the end; 31 before a turn's loads were issued during the one before), 14 at T = 2047.
-__global__ __launch_bounds__(64 * DW) void dg_kernel(const DecayGrad a) {
-    __shared__ double sumA[DW], sumB[DW], own[DW], red[DW];
-    __shared__ int anew[DW], ends[DW];
-    const int h = blockIdx.x, l = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t heads = (int64_t)a.B * a.Hv;
-    double sum = 0.;
-    for (int b = a.per_head ? 0 : blockIdx.y; b < (a.per_head ? a.B : (int)blockIdx.y + 1); ++b) {
-        const int64_t head = (int64_t)b * a.Hv + h;
-        double D = 0.;
-        if (a.dlast) {
-            const float *x = a.dlast + head * a.size, *y = a.last + head * a.size;
+// dg between two marks, in 64 bits: a wave sums one chunk; c by the chain from either end.  Its errors are those of the numbers
+// that it adds, so the end is taken whose magnitudes add up to less.  grid (nm, Hv, B).
+__global__ __launch_bounds__(64 * MARK) void dg_kernel(const DecayGrad a) {
+    __shared__ double A[MARK], B[MARK], red[MARK], D0, D1;
+    __shared__ float absA[MARK], absB[MARK];
+    __shared__ int anew[MARK];
+    const int m = blockIdx.x, h = blockIdx.y, b = blockIdx.z, l = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t heads = (int64_t)a.B * a.Hv, head = (int64_t)b * a.Hv + h;
+    const int n = min(MARK, a.nc - m * MARK), c = m * MARK + w;  // chunks here, the wave's
+    const int64_t t = (int64_t)c * C + C - 1 - l;                 // later tokens in lower lanes
+    const bool in = w < n && t < a.T;
+    double xa = 0., xb = 0., x = 0.;
+    if (in) {
+        for (int s = 0; s < a.slices; ++s) {
+            xa += (double)a.a[(s * heads + head) * a.T + t];
+            xb += (double)a.b[(s * heads + head) * a.T + t];
+        }
+        for (int s = 0; s < a.cross_slices; ++s) x += (double)a.cross[(s * heads + head) * a.T + t];
+    }
+    double end = 0.;
+    if (m == a.nm - 1 && a.dlast) {
+        const float *const p = a.dlast + head * a.size, *const q = a.last + head * a.size;
 #pragma unroll 8
-            for (int i = threadIdx.x; i < (int)a.size; i += 64 * DW) D = fma((double)x[i], (double)y[i], D);
-            D = block_sum(D, red, DW);
-        }
-        // the first slices' numbers of a turn are loaded during the turn before
-        float na, nb, nx;
-        const auto fetch = [&](int c) {
-            const int64_t t = (int64_t)c * C + C - 1 - l, at = head * a.T + (c >= 0 && t < a.T ? t : 0);
-            na = a.a[at];
-            nb = a.b[at];
-            nx = a.cross[at];
-        };
-        fetch(a.nc - 1 - w);
-        for (int c1 = a.nc - 1; c1 >= 0; c1 -= DW) {
-            const int c = c1 - w;  // later chunks in lower waves, later tokens in lower lanes
-            const int64_t t = (int64_t)c * C + C - 1 - l;
-            const bool in = c >= 0 && t < a.T;
-            double xa = in ? na : 0., xb = in ? nb : 0., x = in ? nx : 0.;
-            if (c1 >= DW) fetch(c - DW);
-            if (in) {
-                for (int s = 1; s < a.slices; ++s) {
-                    xa += (double)a.a[(s * heads + head) * a.T + t];
-                    xb += (double)a.b[(s * heads + head) * a.T + t];
-                }
-                for (int s = 1; s < a.cross_slices; ++s) x += (double)a.cross[(s * heads + head) * a.T + t];
-            }
-            xa = wave_prefix_sum(xa);
-            xb = wave_prefix_sum(xb);
-            const double B = readlane_f64(xb, 63);
-            const int seg = c / a.cps;
-            const bool end = c >= 0 && seg < a.nseg - 1 && (c + 1) % a.cps == 0;
-            double e = 0.;
-            if (end) {
-                for (int i = l; i < a.blocks; i += 64) e += a.ends[(head * a.nseg + seg) * a.blocks + i];
-                e = wave_prefix_sum(e);
-            }
-            if (l == 63) {
-                ends[w] = end;
-                own[w] = e;
-                sumA[w] = xa;
-                sumB[w] = xb;
-                anew[w] = c >= 0 && a.decays[(head * a.nc + c) * DECAYS + 3 * C - 1] < 0x1p-30f;  // e^{G_C}
-            }
-            __syncthreads();
-            double mine = 0.;
-            for (int i = 0; i < DW; ++i) {
-                if (ends[i]) D = own[i];
-                const double c0 = anew[i] ? 0. : D - sumB[i];
-                if (i == w) mine = c0;
-                D = c0 + sumA[i];
-            }
-            x += mine + xa + (B - xb);
-            if (in) {
-                if (a.per_head) sum += x;
-                else store_from_f32(a.dg, (b * (int64_t)a.T + t) * a.Hv + h, (float)x, a.dt);
-            }
-            __syncthreads();
-        }
+        for (int i = threadIdx.x; i < (int)a.size; i += 64 * MARK) end = fma((double)p[i], (double)q[i], end);
+        end = block_sum(end, red, MARK);
     }
-    if (a.per_head) {
-        sum = block_sum(sum, red, DW);
-        if (threadIdx.x == 0) store_from_f32(a.dg, h, (float)sum, a.dt);
+    if (w < 2) {
+        const int at = m + w;
+        double e = 0.;
+        if (at >= a.mark0 && at < a.nm)
+            for (int i = l; i < a.parts; i += 64) e += a.ends[(head * a.nm + at) * a.parts + i];
+        e = wave_prefix_sum(e);
+        if (l == 63) (w ? D1 : D0) = at < a.nm ? e : end;
     }
+    const float fa = ops::group_sum<64>((float)fabs(xa)), fb = ops::group_sum<64>((float)fabs(xb));
+    xa = wave_prefix_sum(xa);
+    xb = wave_prefix_sum(xb);
+    if (l == 63) {
+        A[w] = xa;
+        B[w] = xb;
+        absA[w] = fa;
+        absB[w] = fb;
+        anew[w] = w < n && a.decays[(head * a.nc + c) * DECAYS + 3 * C - 1] < a.none;  // e^{G_C}
+    }
+    __syncthreads();
+    double from_start = 0., from_end = 0., D = D0;
+    float size_start = 0.f, size_end = 0.f, size = fabsf((float)D0);
+    for (int i = 0; i < n && i <= w; ++i) {
+        from_start = anew[i] ? 0. : D - A[i];
+        size_start = anew[i] ? 0.f : size + absA[i];
+        D = from_start + B[i];
+        size = size_start + absB[i];
+    }
+    D = D1;
+    size = fabsf((float)D1);
+    for (int i = n - 1; i >= w; --i) {
+        from_end = anew[i] ? 0. : D - B[i];
+        size_end = anew[i] ? 0.f : size + absB[i];
+        D = from_end + A[i];
+        size = size_end + absA[i];
+    }
+    x += (size_start <= size_end ? from_start : from_end) + xa + (B[w] - xb);
+    if (!a.per_head) {
+        if (in) store_from_f32(a.dg, (b * (int64_t)a.T + t) * a.Hv + h, (float)x, a.dt);
+        return;
+    }
+    x = block_sum(in ? x : 0., red, MARK);
+    if (threadIdx.x == 0) a.sums[((int64_t)h * a.B + b) * a.nm + m] = x;
+}
+
+// One decay per head: the sums over n stretches of all sequences, in a fixed order.
+__global__ __launch_bounds__(NT) void dg_head_kernel(const double *sums, void *dg, int64_t n, int dt) {
+    __shared__ double red[NT / 64];
+    double x = 0.;
+    for (int64_t i = threadIdx.x; i < n; i += NT) x += sums[blockIdx.x * n + i];
+    x = block_sum(x, red, NT / 64);
+    if (threadIdx.x == 0) store_from_f32(dg, blockIdx.x, (float)x, dt);
 }
 
 // One token: y = scale S' q, S' = e^g S + v k^T, in place.  `lanes` lanes share a row of the state, V channels each at a time,
@@ -255,9 +243,8 @@ static int run_pass(Pass a, Kind kind, hipStream_t st) {
 
 // The states entering each segment (nseg > 1), from s0 on (reverse: the cotangents, from the end).
 static int scan_width(int64_t size) { return size % 4 ? 1 : 4; }
-static int scan_blocks(int64_t size) { return (int)((size + NT * scan_width(size) - 1) / (NT * scan_width(size))); }
 template <bool REV>
-static int run_segments(Seg a, const float *s0, const float *at, double *part, hipStream_t st) {
+static int run_segments(Seg a, const float *s0, hipStream_t st) {
     const int cols = seg_cols(a.dk, a.dv, a.dt);
     a.slices = (a.dv + cols - 1) / cols;
     {
@@ -270,17 +257,19 @@ static int run_segments(Seg a, const float *s0, const float *at, double *part, h
     const int64_t size = (int64_t)a.dk * a.dv;
     {
         Timed tm("linatt_scan", st);
-        const dim3 grid((unsigned)scan_blocks(size), (unsigned)(a.B * a.Hv));
+        const int per = NT * scan_width(size);
+        const dim3 grid((unsigned)((size + per - 1) / per), (unsigned)(a.B * a.Hv));
         if (scan_width(size) == 4)
-            hipLaunchKernelGGL((scan_kernel<REV, 4>), grid, dim3(NT), 0, st, a.s, a.decay, s0, at, part, a.nseg, size);
+            hipLaunchKernelGGL((scan_kernel<REV, 4>), grid, dim3(NT), 0, st, a.s, a.decay, s0, a.nseg, size);
         else
-            hipLaunchKernelGGL((scan_kernel<REV, 1>), grid, dim3(NT), 0, st, a.s, a.decay, s0, at, part, a.nseg, size);
+            hipLaunchKernelGGL((scan_kernel<REV, 1>), grid, dim3(NT), 0, st, a.s, a.decay, s0, a.nseg, size);
     }
     return check_launch(st, "linear attention (scan)");
 }
 
 struct Sizes {
-    size_t decays, state, decay, saved, part, dot, cross, ends, bwd;
+    size_t decays, state, decay, saved, part, dot, cross, marks, ends, sums, bwd;
+    int nm, parts;
 };
 // value heads of a key head whose dq and dk are added after the passes: all, or the pairs of pair_heads()
 static bool pair_heads(int r, int Dv, int dtype) { return dtype == DT_BF16 && Dv <= 128 && r % 2 == 0; }
@@ -299,8 +288,15 @@ static Sizes sizes(int B, int T, int Hk, int Hv, int Dk, int Dv, int dtype = DT_
     const size_t rows = (size_t)B * Hv * T * sizeof(float);
     s.dot = align_up256(rows * slices_of(Dv, Dk));
     s.cross = align_up256(rows * slices_of(Dk, Dv));
-    if (p.nseg > 1) s.ends = align_up256((size_t)B * Hv * p.nseg * scan_blocks((int64_t)Dk * Dv) * sizeof(double));
-    s.bwd = s.state + s.decay + s.part + 2 * s.dot + s.cross + s.ends;
+    // of the passes that write dq and dk, whose K' are the value channels
+    const int slices = slices_of(Dv, Dk);
+    s.nm = (p.nc + MARK - 1) / MARK;
+    s.parts = slices * waves_of(Dv, Dk, dtype);
+    const size_t marks = (size_t)B * Hv * s.nm;
+    s.marks = align_up256(marks * slices * rows_of(Dv) * cols_of(Dv, Dk) * sizeof(float));
+    s.ends = align_up256(marks * s.parts * sizeof(double));
+    s.sums = align_up256(marks * sizeof(double));
+    s.bwd = s.state + s.decay + s.part + 2 * s.dot + s.cross + s.marks + s.ends + s.sums;
     return s;
 }
 
@@ -375,7 +371,7 @@ extern "C" int gdn_linatt_fwd(const void *q, const void *k, const void *v, const
     p.s_out = state_T;
     if (pl.nseg > 1) {
         const la::Seg a{p.K, p.V, decays, states, seg_decay, B, T, Hv, Dk, Dv, 0, pl.nseg, pl.cps, pl.nc, dtype, scale};
-        rc = la::run_segments<false>(a, state0, nullptr, nullptr, st);
+        rc = la::run_segments<false>(a, state0, st);
         if (rc) return rc;
         p.s_in = states;
         p.s_seg = p.s_head;
@@ -412,7 +408,8 @@ extern "C" int gdn_linatt_bwd(const void *q, const void *k, const void *v, const
     };
     float *ds = take(sz.state), *decay = take(sz.decay), *part = take(sz.part);
     float *sa = take(sz.dot), *sb = take(sz.dot), *cross = take(sz.cross);
-    double *ends = reinterpret_cast<double *>(take(sz.ends));
+    float *marks = take(sz.marks);
+    double *ends = reinterpret_cast<double *>(take(sz.ends)), *sums = reinterpret_cast<double *>(take(sz.sums));
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int r = Hv / Hk;
     const int64_t dys[3] = {(int64_t)T * Hv * Dv, (int64_t)Hv * Dv, Dv}, size = (int64_t)Dk * Dv;
@@ -423,6 +420,10 @@ extern "C" int gdn_linatt_bwd(const void *q, const void *k, const void *v, const
     p.B = B; p.T = T; p.Hv = Hv; p.nseg = pl.nseg; p.cps = pl.cps; p.nc = pl.nc;
     p.dt = dtype;
     p.scale = scale;
+    p.marks = marks;
+    p.ends = ends;
+    p.nm = sz.nm;
+    p.mark0 = state0 ? 0 : 1;
     const int64_t n = (int64_t)B * T * Hk * Dk;
     // value heads that share a key head: two to a workgroup, or each for itself, the rest added afterwards
     const int pair = la::pair_heads(r, Dv, dtype), group = pair ? r / 2 : r;
@@ -452,7 +453,7 @@ extern "C" int gdn_linatt_bwd(const void *q, const void *k, const void *v, const
     const float *s_in = dstate_T;
     if (pl.nseg > 1) {
         const la::Seg a{tq, tdy, decays, ds, decay, B, T, Hv, Dk, Dv, 0, pl.nseg, pl.cps, pl.nc, dtype, scale};
-        rc = la::run_segments<true>(a, dstate_T, states, ends, st);
+        rc = la::run_segments<true>(a, dstate_T, st);
         if (rc) return rc;
         s_in = ds;
     }
@@ -473,12 +474,15 @@ extern "C" int gdn_linatt_bwd(const void *q, const void *k, const void *v, const
     p.s_out = dstate0;
     rc = la::run_pass(p, la::DV, st);
     if (rc) return rc;
-    const la::DecayGrad d{sa, sb, cross, decays, dstate_T, state_T, ends, dg, B, T, Hv, la::slices_of(Dv, Dk),
-                          la::slices_of(Dk, Dv), g_per_head != 0, g_dtype, pl.nc, pl.cps, pl.nseg, la::scan_blocks(size), size};
+    const la::DecayGrad d{sa, sb, cross, decays, dstate_T, state_T, ends, dg, sums, B, T, Hv, la::slices_of(Dv, Dk),
+                          la::slices_of(Dk, Dv), g_per_head != 0, g_dtype, pl.nc, sz.nm, p.mark0, sz.parts,
+                          // an eighth of the relative errors of a and b
+                          dtype == GDN_BF16 ? 0x1p-20f : 0x1p-26f, size};
     {
         Timed tm("linatt_dg", st);
-        hipLaunchKernelGGL(la::dg_kernel, dim3((unsigned)Hv, g_per_head ? 1u : (unsigned)B), dim3(64 * la::DW), 0,
-                           st, d);
+        hipLaunchKernelGGL(la::dg_kernel, dim3((unsigned)sz.nm, (unsigned)Hv, (unsigned)B), dim3(64 * la::MARK), 0, st, d);
+        if (g_per_head)
+            hipLaunchKernelGGL(la::dg_head_kernel, dim3((unsigned)Hv), dim3(la::NT), 0, st, sums, dg, (int64_t)B * sz.nm, g_dtype);
     }
     return check_launch(st, "linear attention (dg)");
 }

@@ -37,32 +37,9 @@ def tolerance(dtype):
     return t, 8 * t
 
 
-def decays64(q, k, v, g, state, scale, dy, dlast=None):
-    """dL/dg of every token [B, T, Hv], float64: no state but the present one is kept, as dg_t = dg_{t+1} + q_t . dq_t - k_t . dk_t
-    and the rounding of 64 bits leaves room for the differences."""
-    q, k, v, g, dy = (t.detach().double() for t in (q, k, v, g, dy))
-    B, T, Hk, Dk = q.shape
-    Hv = v.shape[2]
-    a = g.expand(B, T, Hv).exp()[..., None, None]
-    q, k = (x.repeat_interleave(Hv // Hk, 2).transpose(0, 1).contiguous() for x in (q, k))
-    v, dy = v.transpose(0, 1).contiguous(), dy.transpose(0, 1).contiguous()
-    S = q.new_zeros(B, Hv, v.shape[-1], Dk) if state is None else state.detach().double().clone()
-    out = q.new_empty(T, B, Hv)
-    for t in range(T):
-        S = a[:, t] * S + v[t, ..., None] * k[t, ..., None, :]
-        out[t] = scale * ((S * dy[t, ..., None]).sum(-2) * q[t]).sum(-1)
-    D = torch.zeros_like(S) if dlast is None else dlast.double().clone()
-    run = (D * S).sum((-1, -2))
-    for t in range(T - 1, -1, -1):
-        D = D + scale * dy[t, ..., None] * q[t, ..., None, :]
-        run = run + out[t] - ((D * v[t, ..., None]).sum(-2) * k[t]).sum(-1)
-        out[t] = run
-        D = a[:, t] * D
-    return out.transpose(0, 1)
-
-
 def states64(q, k, v, g, state, scale, dy, dlast=None):
-    """The same from the states of all tokens, for short sequences: exact where single terms are large."""
+    """dL/dg of every token [B, T, Hv] = a_t <dS_t, S_{t-1}>, float64, from the states of all tokens (sums of q . dq - k . dk,
+    which need no states, lose what has faded)."""
     q, k, v, g, dy = (t.detach().double() for t in (q, k, v, g, dy))
     B, T, Hk, Dk = q.shape
     Hv = v.shape[2]
@@ -120,3 +97,41 @@ def test_large_pairs_after_a_token_leave_its_gradient_alone(dev, T, t0, dtype):
     want = states64(q, k, v, g, None, 0.125, dy)
     each_head(dg[:, 1:t0], want[:, 1:t0], tolerance(dtype)[0], f"dg before {t0} of {T}, {dtype}")
     each_head(dg, want, tolerance(dtype)[0], f"dg of {T}, {dtype}")
+
+
+# as many sequences and heads as fill the card without cutting the sequence, and few heads, whose sequence is cut
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,T,Hk,Hv,D", [(16, 6001, 2, 32, 32), (2, 6001, 2, 16, 64)])
+def test_long_sequences(dev, B, T, Hk, Hv, D, dtype):
+    """A decay for every token, then the same decays one for each head: the errors of many chunks do not add up.  Per head: of
+    the sequences' sums."""
+    q, k, v, g, state, dy, dlast = inputs(dev, B, T, Hk, Hv, D, D, dtype, B)
+    want = states64(q, k, v, g, state, D ** -0.5, dy, dlast)
+    per_token, per_head = tolerance(dtype)
+    each_head(gradient(q, k, v, g.expand(B, T, Hv), state, dy, dlast), want, per_token, f"dg of {B} x {T}, {dtype}")
+    got = gradient(q, k, v, g, state, dy, dlast).double()
+    size = want.sum(1).norm(dim=0)  # of the B sums that a head's gradient adds
+    err = (got - want.sum((0, 1))).abs() / size
+    print(f"per head {float(err.max()):.3g}", flush=True)
+    assert float(err.max()) <= per_head, err.tolist()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,T,Hk,Hv,D", [(16, 4100, 2, 32, 32), (1, 4100, 1, 8, 64)])
+def test_loss_of_the_last_tokens(dev, B, T, Hk, Hv, D, dtype):
+    """Nothing but the last ten outputs in the loss: what they draw from thousands of tokens earlier fades, and so does the
+    error.  Per token, every 512 tokens for themselves where the gradient is above 2^-40 of the last one."""
+    q, k, v, g, state, dy, _ = inputs(dev, B, T, Hk, Hv, D, D, dtype, 7)
+    dy[:, :-10] = 0
+    want = states64(q, k, v, g, state, D ** -0.5, dy)
+    got = gradient(q, k, v, g.expand(B, T, Hv), state, dy).double()
+    per_token, per_head = tolerance(dtype)
+    each_head(got, want, per_token, f"dg of the last tokens, {B} x {T}, {dtype}")
+    size = want.norm(dim=(0, 1))
+    for t in range(0, T, 512):
+        part, err = want[:, t:t + 512].norm(dim=(0, 1)), (got - want)[:, t:t + 512].norm(dim=(0, 1))
+        on = part > 2.0 ** -40 * size
+        assert bool((err[on] <= per_token * part[on]).all()), (t, (err / part).tolist())
+    err = (gradient(q, k, v, g, state, dy).double() - want.sum((0, 1))).abs() / want.sum(1).norm(dim=0)
+    print(f"per head {float(err.max()):.3g}", flush=True)
+    assert float(err.max()) <= per_head, err.tolist()
