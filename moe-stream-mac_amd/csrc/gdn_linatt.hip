@@ -82,7 +82,9 @@ struct DecayGrad {
 };
 
 // dg between two marks, in 64 bits: a wave sums one chunk; c by the chain from either end.  Its errors are those of the numbers
-// that it adds, so the end is taken whose magnitudes add up to less.  grid (nm, Hv, B).
+// that it adds, so the end is taken whose magnitudes add up to less.  A NaN or infinite value or key makes the states after it
+// odd, a query or cotangent those before it: of the two ends, and of the two sums over a chunk's tokens, each is formed from one
+// side alone, so that gradients between a state and a cotangent that are both finite are, too.  grid (nm, Hv, B).
 __global__ __launch_bounds__(64 * MARK) void dg_kernel(const DecayGrad a) {
     __shared__ double A[MARK], B[MARK], red[MARK], D0, D1;
     __shared__ float absA[MARK], absB[MARK];
@@ -90,14 +92,13 @@ __global__ __launch_bounds__(64 * MARK) void dg_kernel(const DecayGrad a) {
     const int m = blockIdx.x, h = blockIdx.y, b = blockIdx.z, l = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int64_t heads = (int64_t)a.B * a.Hv, head = (int64_t)b * a.Hv + h;
     const int n = min(MARK, a.nc - m * MARK), c = m * MARK + w;  // chunks here, the wave's
-    const int64_t t = (int64_t)c * C + C - 1 - l;                 // later tokens in lower lanes
+    const int64_t t = (int64_t)c * C + l, last = (int64_t)c * C + C - 1 - l;
     const bool in = w < n && t < a.T;
-    double xa = 0., xb = 0., x = 0.;
+    double xa = 0., xb = 0., x = 0.;  // a of token `last`, b and the pairs of token t
+    if (w < n && last < a.T)
+        for (int s = 0; s < a.slices; ++s) xa += (double)a.a[(s * heads + head) * a.T + last];
     if (in) {
-        for (int s = 0; s < a.slices; ++s) {
-            xa += (double)a.a[(s * heads + head) * a.T + t];
-            xb += (double)a.b[(s * heads + head) * a.T + t];
-        }
+        for (int s = 0; s < a.slices; ++s) xb += (double)a.b[(s * heads + head) * a.T + t];
         for (int s = 0; s < a.cross_slices; ++s) x += (double)a.cross[(s * heads + head) * a.T + t];
     }
     double end = 0.;
@@ -142,7 +143,9 @@ __global__ __launch_bounds__(64 * MARK) void dg_kernel(const DecayGrad a) {
         D = from_end + A[i];
         size = size_end + absA[i];
     }
-    x += (size_start <= size_end ? from_start : from_end) + xa + (B[w] - xb);
+    const bool start = isfinite(from_start) && (size_start <= size_end || !isfinite(from_end));
+    // a from t on, b before t
+    x += (start ? from_start : from_end) + __shfl(xa, C - 1 - l) + dpp_mov_f64<0x138>(xb);
     if (!a.per_head) {
         if (in) store_from_f32(a.dg, (b * (int64_t)a.T + t) * a.Hv + h, (float)x, a.dt);
         return;

@@ -135,3 +135,43 @@ def test_loss_of_the_last_tokens(dev, B, T, Hk, Hv, D, dtype):
     err = (gradient(q, k, v, g, state, dy).double() - want.sum((0, 1))).abs() / want.sum(1).norm(dim=0)
     print(f"per head {float(err.max()):.3g}", flush=True)
     assert float(err.max()) <= per_head, err.tolist()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sizes", [(2, 2, 4, 128, 128), (1, 1, 3, 64, 40), (1, 1, 1, 256, 33), (40, 1, 16, 32, 32)])
+def test_odd_tokens_do_not_reach_decays_they_have_no_part_in(dev, sizes, dtype):
+    """A NaN or infinite value or key of token t is in no state before t: dg up to t is the clean one.  A NaN or infinite query or
+    cotangent of token t is in no cotangent of a state after t: dg from t + 1 on is.  Both with and without the final state in
+    the loss, in sequences of several chunks and of several segments (few heads) or one (many)."""
+    B, Hk, Hv, Dk, Dv = sizes
+    T = 1300
+    q, k, v, g, state, dy, dlast = inputs(dev, B, T, Hk, Hv, Dk, Dv, dtype, 3)
+    g = g.expand(B, T, Hv) * (0.5 + torch.rand(B, T, Hv, device=dev))
+    for with_last in (True, False):
+        end = dlast if with_last else None
+        clean = gradient(q, k, v, g, state, dy, end).double()
+        for t in (0, 5, 63, 64, 700, 1151, 1299):
+            for what, bad in (("v", math.nan), ("v", math.inf), ("k", math.nan), ("q", math.nan), ("dy", math.nan),
+                              ("dy", -math.inf)):
+                x = dict(q=q.clone(), k=k.clone(), v=v.clone(), dy=dy.clone())
+                x[what][:, t, 0] = bad
+                dg = gradient(x["q"], x["k"], x["v"], g, state, x["dy"], end)
+                part = slice(0, t + 1) if what in ("v", "k") else slice(t + 1, T)
+                if clean[:, part].numel():
+                    # two results, each within its tolerance of the exact ones
+                    each_head(dg[:, part], clean[:, part], 2 * tolerance(dtype)[0], (what, bad, t, with_last))
+                each_head(dg[..., Hv // Hk:], clean[..., Hv // Hk:], 2 * tolerance(dtype)[0], "other heads") if Hk > 1 else None
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_nan_where_no_loss_is_left(dev, dtype):
+    """A NaN key from which on nothing is in the loss: the gradients of the decays up to it are the clean ones."""
+    q, k, v, g, state, dy, _ = inputs(dev, 1, 900, 1, 2, 64, 64, dtype, 4)
+    g = g.expand(1, 900, 2)
+    for t in (30, 64, 511, 899):
+        cut = dy.clone()
+        cut[:, t:] = 0
+        bad = k.clone()
+        bad[:, t] = math.nan
+        each_head(gradient(q, bad, v, g, state, cut)[:, :t + 1], gradient(q, k, v, g, state, cut)[:, :t + 1].double(),
+                  2 * tolerance(dtype)[0], t)
