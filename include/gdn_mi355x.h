@@ -290,7 +290,8 @@ int gdn_gated_rmsnorm_bwd(const void *y, const void *z, const float *w, const vo
  * holds the element strides over batch, tokens and heads of q, k, v and g, 12 numbers; channels are contiguous.  One log
  * decay per head: strides of 0 over batch and tokens.  A log decay of -inf keeps nothing of the state.  state0 [B][Hv][Dv][Dk]
  * fp32, or NULL for zeros; y [B][T][Hv][Dv] contiguous, of dtype; state_T as state0 (may be NULL).  Dk, Dv <= 256,
- * B * Hv <= 65535, Hv * max(Dk, Dv) < 2^22, T > 0; tokens of q, k and v 0 to 2^22 - 1 elements apart.
+ * B * Hv <= 65535, Hv * max(Dk, Dv) < 2^22, B * T * Hv * max(Dk, Dv) < 2^39, T > 0; tokens of q, k and v
+ * 0 to 2^22 - 1 elements apart.
  *
  * saved (gdn_linatt_saved_bytes) holds the decays' sums and the states entering each segment of the sequence; gdn_linatt_bwd
  * reads it.  From the cotangents dy (contiguous, of dtype) and dstate_T (fp32, or NULL for zeros; needs state_T) it writes dq,
@@ -330,7 +331,7 @@ int gdn_rotary(const void *q, const void *k, void *q_out, void *k_out, const voi
  *   stat [rows][2]   what gdn_logprobs_bwd needs (may be NULL)
  *   top_ids, top_logp [rows][top]  the largest log probabilities, equal ones by index (NULL with top = 0; top <= 64)
  * fp32 outputs.  Logits of -inf have probability 0; a row with nothing else has log probabilities -inf, entropy 0 and no
- * gradient.  At most 2^24 pieces of 8192 logits over all rows, and top * ceil(V / 8192) <= 8192.
+ * gradient.  Less than 2^24 pieces of 8192 logits over all rows, and top * ceil(V / 8192) <= 8192.
  *
  * gdn_logprobs_bwd: dlogits [rows][V] contiguous (dtype) from the cotangents dlogp and dentropy [rows] (either may be
  * NULL; dentropy needs the forward's entropy). */

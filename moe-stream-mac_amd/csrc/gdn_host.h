@@ -25,6 +25,14 @@ struct Timed {
     Timed &operator=(const Timed &) = delete;
 };
 
+// A launch has less than 2^32 threads along a dimension: a grid of `blocks` workgroups (less than 2^32), in rows if they are
+// many.  The last row may be longer than what is left; block_index() of those is `blocks` or more.
+inline dim3 grid_of(int64_t blocks) {
+    constexpr int64_t ROW = 1 << 16;
+    return blocks <= 1 << 21 ? dim3((unsigned)blocks) : dim3((unsigned)ROW, (unsigned)((blocks + ROW - 1) / ROW));
+}
+__device__ __forceinline__ int64_t block_index() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 inline size_t align_up256(size_t x) { return (x + 255) & ~(size_t)255; }
 inline bool aligned_to(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 

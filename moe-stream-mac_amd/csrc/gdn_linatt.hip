@@ -12,7 +12,7 @@ constexpr int MAX_D = 256;
 // The decays of every chunk, a wave to a chunk, once for the five or six kernels that use them (a wave of each pass would
 // spend two 64-bit exponentials a chunk).  Sums run in 64 bits.  9 us at B=4, T=4096, Hv=32: latency.
 __global__ __launch_bounds__(NT) void decay_kernel(Gate g, float *o, int B, int T, int Hv, int nc) {
-    const int64_t id = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
+    const int64_t id = block_index() * (NT / 64) + (threadIdx.x >> 6);
     const int l = threadIdx.x & 63;
     if (id >= (int64_t)B * Hv * nc) return;
     const int h = id % Hv, c = (id / Hv) % nc, b = id / Hv / nc;  // heads side by side: their decays are, in memory
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(NT) void scan_kernel(float *s, const float *decay, 
 // The heads of a group added in order: part [rows][group][D] to o [rows][D].  13 us for 2047 tokens of 2 x 16 heads of 128 in
 // fp32 (50 MB).  Atomics into o would round and order the sums differently every time.
 __global__ __launch_bounds__(NT) void group_kernel(const float *part, void *o, int64_t n, int group, int D, int dt) {
-    const int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x;
+    const int64_t i = block_index() * NT + threadIdx.x;
     if (i >= n) return;
     const int64_t row = i / D;
     const float *p = part + row * group * D + i % D;
@@ -315,6 +315,8 @@ static int check(const int64_t *strides, int B, int T, int Hk, int Hv, int Dk, i
             return fail(GDN_ERR_UNSUPPORTED, "tokens of q, k and v must be less than 2^22 elements apart");
     if ((int64_t)B * Hv > 65535 || Hv > 65535) return fail(GDN_ERR_UNSUPPORTED, "more than 65535 heads over the batch");
     if ((int64_t)Hv * (Dk > Dv ? Dk : Dv) >= 1 << 22) return fail(GDN_ERR_UNSUPPORTED, "a token of more than 2^22 elements");
+    if ((int64_t)B * Hv * T * (Dk > Dv ? Dk : Dv) >= (int64_t)1 << 39)  // grids of 2^31 workgroups
+        return fail(GDN_ERR_UNSUPPORTED, "2^39 elements or more over the value heads");
     return 0;
 }
 
@@ -355,8 +357,7 @@ extern "C" int gdn_linatt_fwd(const void *q, const void *k, const void *v, const
     {
         Timed tm("linatt_decays", st);
         const int64_t waves = (int64_t)B * Hv * pl.nc;
-        hipLaunchKernelGGL(la::decay_kernel, dim3((unsigned)((waves + 3) / 4)), dim3(la::NT), 0, st, gate, decays, B, T, Hv,
-                           pl.nc);
+        hipLaunchKernelGGL(la::decay_kernel, grid_of((waves + 3) / 4), dim3(la::NT), 0, st, gate, decays, B, T, Hv, pl.nc);
     }
     rc = check_launch(st, "linear attention (decays)");
     if (rc) return rc;
@@ -438,8 +439,8 @@ extern "C" int gdn_linatt_bwd(const void *q, const void *k, const void *v, const
         if (e || group == 1) return e;
         {
             Timed tm("linatt_group", st);
-            hipLaunchKernelGGL(la::group_kernel, dim3((unsigned)((n + la::NT - 1) / la::NT)), dim3(la::NT), 0, st, part, out, n,
-                               group, Dk, dtype);
+            hipLaunchKernelGGL(la::group_kernel, grid_of((n + la::NT - 1) / la::NT), dim3(la::NT), 0, st, part, out, n, group, Dk,
+                               dtype);
         }
         return check_launch(st, "linear attention (groups)");
     };

@@ -439,8 +439,9 @@ static int check(int64_t outer, int64_t inner, int64_t V, int dtype) {
     if (outer < 0 || inner < 0 || V <= 0) return fail(GDN_ERR_INVALID, "row counts must be >= 0 and V > 0");
     if (dtype != GDN_F32 && dtype != GDN_BF16 && dtype != GDN_F16) return fail(GDN_ERR_INVALID, "unknown dtype code");
     if (outer == 0 || inner == 0) return 1;
-    if (V > 0x7fffffff || inner > 0x7fffffff || outer > (1 << 24) / inner || pieces_of(V) > (1 << 24) / (outer * inner))
-        return fail(GDN_ERR_UNSUPPORTED, "more than 2^24 pieces of %d logits are not supported", PIECE);
+    constexpr int64_t MOST = (1 << 24) - 1;  // workgroups of 256 threads: a launch has less than 2^32
+    if (V > 0x7fffffff || inner > MOST || outer > MOST / inner || pieces_of(V) > MOST / (outer * inner))
+        return fail(GDN_ERR_UNSUPPORTED, "2^24 or more pieces of %d logits are not supported", PIECE);
     return 0;
 }
 

@@ -84,7 +84,8 @@ __global__ __launch_bounds__(NT) void rotary_kernel(const Args a) {
     extern __shared__ float2 cs[];  // [tok][R / 2]
     __shared__ int64_t from[MAX_TOK][2];
     const int tid = threadIdx.x, half = a.R / 2;
-    const int64_t t0 = (int64_t)blockIdx.x * a.tok;
+    const int64_t t0 = block_index() * a.tok;
+    if (t0 >= a.tokens) return;
     const int ntok = (int)min((int64_t)a.tok, a.tokens - t0);
     if (tid < ntok) {
         const int64_t b = (t0 + tid) / a.T, t = (t0 + tid) % a.T;
@@ -182,7 +183,7 @@ extern "C" int gdn_rotary(const void *q, const void *k, void *q_out, void *k_out
     hipStream_t st = static_cast<hipStream_t>(stream);
     {
         Timed tm("rotary", st);
-        const dim3 grid((unsigned)blocks), block(rope::NT);
+        const dim3 grid = grid_of(blocks), block(rope::NT);
 #define GDN_ROTARY(DT)                                                                                      \
     if (V == 8) hipLaunchKernelGGL((rope::rotary_kernel<8, DT>), grid, block, lds, st, a);                   \
     else if (V == 4) hipLaunchKernelGGL((rope::rotary_kernel<4, DT>), grid, block, lds, st, a);              \
