@@ -299,7 +299,7 @@ int gdn_gated_rmsnorm_bwd(const void *y, const void *z, const float *w, const vo
  * dstate0 (may be NULL).
  *
  * gdn_linatt_step: one token of B sequences; q, k [B][Hk][Dk], v, y [B][Hv][Dv] contiguous, g with element strides over
- * batch and heads, state [B][Hv][Dv][Dk] fp32 updated in place. */
+ * batch and heads, state [B][Hv][Dv][Dk] fp32 updated in place.  B, Hv <= 65535 each. */
 size_t gdn_linatt_saved_bytes(int B, int T, int Hk, int Hv, int Dk, int Dv);
 size_t gdn_linatt_bwd_workspace_bytes(int B, int T, int Hk, int Hv, int Dk, int Dv, int dtype);
 int gdn_linatt_fwd(const void *q, const void *k, const void *v, const void *g, const float *state0, void *y,

@@ -303,17 +303,24 @@ static Sizes sizes(int B, int T, int Hk, int Hv, int Dk, int Dv, int dtype = DT_
     return s;
 }
 
-static int check(const int64_t *strides, int B, int T, int Hk, int Hv, int Dk, int Dv, int dtype, int g_dtype) {
+// What whole sequences and single tokens share.
+static int check_sizes(int B, int T, int Hk, int Hv, int Dk, int Dv, int dtype, int g_dtype) {
     if (B < 0 || T < 0) return fail(GDN_ERR_INVALID, "B and T must be >= 0");
     if (Hk <= 0 || Hv <= 0 || Dk <= 0 || Dv <= 0) return fail(GDN_ERR_INVALID, "head counts and sizes must be positive");
     if (Hv % Hk) return fail(GDN_ERR_INVALID, "the key heads (%d) must divide the value heads (%d)", Hk, Hv);
     for (int d : {dtype, g_dtype})
         if (d != GDN_F32 && d != GDN_BF16 && d != GDN_F16) return fail(GDN_ERR_INVALID, "unknown dtype code");
     if (Dk > MAX_D || Dv > MAX_D) return fail(GDN_ERR_UNSUPPORTED, "heads of more than %d channels are not supported", MAX_D);
+    return 0;
+}
+
+static int check(const int64_t *strides, int B, int T, int Hk, int Hv, int Dk, int Dv, int dtype, int g_dtype) {
+    const int rc = check_sizes(B, T, Hk, Hv, Dk, Dv, dtype, g_dtype);
+    if (rc) return rc;
     for (int i = 0; strides && i < 9; i += 3)
         if (strides[i + 1] < 0 || strides[i + 1] >= 1 << 22)  // a chunk's rows are addressed in 32 bits
             return fail(GDN_ERR_UNSUPPORTED, "tokens of q, k and v must be less than 2^22 elements apart");
-    if ((int64_t)B * Hv > 65535 || Hv > 65535) return fail(GDN_ERR_UNSUPPORTED, "more than 65535 heads over the batch");
+    if ((int64_t)B * Hv > 65535) return fail(GDN_ERR_UNSUPPORTED, "more than 65535 heads over the batch");
     if ((int64_t)Hv * (Dk > Dv ? Dk : Dv) >= 1 << 22) return fail(GDN_ERR_UNSUPPORTED, "a token of more than 2^22 elements");
     if ((int64_t)B * Hv * T * (Dk > Dv ? Dk : Dv) >= (int64_t)1 << 39)  // grids of 2^31 workgroups
         return fail(GDN_ERR_UNSUPPORTED, "2^39 elements or more over the value heads");
@@ -495,8 +502,9 @@ extern "C" int gdn_linatt_step(const void *q, const void *k, const void *v, cons
                                int64_t gs_h, int B, int Hk, int Hv, int Dk, int Dv, float scale, int dtype, int g_dtype,
                                void *stream) {
     clear_error();
-    const int rc = la::check(nullptr, B, 1, Hk, Hv, Dk, Dv, dtype, g_dtype);
+    const int rc = la::check_sizes(B, 1, Hk, Hv, Dk, Dv, dtype, g_dtype);
     if (rc) return rc;
+    if (B > 65535 || Hv > 65535) return fail(GDN_ERR_UNSUPPORTED, "more than 65535 sequences or heads");
     if (B == 0) return GDN_OK;
     if (!q || !k || !v || !g || !state || !y) return fail(GDN_ERR_INVALID, "null pointer");
     const bool vec = Dk % 4 == 0 && aligned_to(q, 16) && aligned_to(k, 16) && aligned_to(state, 16);

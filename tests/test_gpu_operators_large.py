@@ -54,3 +54,20 @@ def test_heads_added_over_many_elements(dev):
         got = got[:, -n:].double()
         assert bool(torch.isfinite(got).all())
         assert float((got - w).norm() / w.norm()) <= 2 ** -16 + 2 ** -11
+
+
+def test_step_of_many_sequences(dev):
+    """More than 65535 heads over the batch.  States: one rounded product and sum (2^-23 of the terms); outputs sums of 16 of
+    their products."""
+    from linear_attention import linear_attention_step
+    B, Hk, Hv, D = 2100, 2, 32, 16
+    q, k = torch.randn(B, Hk, D, device=dev), torch.randn(B, Hk, D, device=dev)
+    v, g, S = torch.randn(B, Hv, D, device=dev), -torch.rand(B, Hv, device=dev), torch.randn(B, Hv, D, D, device=dev)
+    q64, k64 = (x.double().repeat_interleave(Hv // Hk, 1) for x in (q, k))
+    old = S.double() * g.double().exp()[..., None, None]
+    want, add = old + v.double()[..., None] * k64[..., None, :], v.double()[..., None] * k64[..., None, :]
+    y = linear_attention_step(q, k, v, g, S)
+    size = old.abs() + add.abs()
+    assert bool(((S.double() - want).abs() <= 2.0 ** -21 * size).all())
+    assert bool(((y.double() - 0.25 * (want * q64[..., None, :]).sum(-1)).abs()
+                 <= 2.0 ** -20 * (size * q64[..., None, :].abs()).sum(-1)).all())

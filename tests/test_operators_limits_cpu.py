@@ -33,3 +33,11 @@ def test_linear_attention_elements():
     for size in ((60000, (1 << 31) - 1, 1, 256), (1 << 8, 1 << 30, 2, 1), (2, 1 << 30, 1, 256)):
         assert fwd(*size) == L.GDN_ERR_UNSUPPORTED, size
     assert fwd(1, 1 << 30, 1, 256) == L.GDN_ERR_INVALID  # null pointers
+
+
+def test_steps_of_many_sequences():
+    """A step's sequences and heads are counted apart: 4096 sequences of 32 heads pass (and fail for their null pointers)."""
+    lib = L.load()
+    step = lambda B, Hv: lib.gdn_linatt_step(*[None] * 6, 1, 1, B, 1, Hv, 64, 64, 1.0, 0, 0, None)  # noqa: E731
+    assert step(4096, 32) == L.GDN_ERR_INVALID and step(65535, 65535) == L.GDN_ERR_INVALID
+    assert step(65536, 1) == L.GDN_ERR_UNSUPPORTED and step(1, 65536) == L.GDN_ERR_UNSUPPORTED
