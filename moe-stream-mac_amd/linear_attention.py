@@ -8,6 +8,7 @@ backward pass, and a recurrent step for decoding.  Tensors must live on a ROCm d
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import Optional
 
@@ -122,14 +123,33 @@ def linear_attention(q: Array, k: Array, v: Array, g: Array, state: Optional[Arr
     return _forward(q, k, v, g, state, scale)[:2]
 
 
+class _NoGradient(torch.autograd.Function):
+    """A result of a step as autograd sees it: it depends on the step's inputs, and a gradient through it is refused."""
+
+    @staticmethod
+    def forward(ctx, result, *inputs):
+        ctx.mark_dirty(result)
+        return result
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("linear_attention_step is not differentiable; use linear_attention")
+
+
 def linear_attention_step(q: Array, k: Array, v: Array, g: Array, state: Array, *,
                           scale: Optional[float] = None) -> Array:
     """One token of B sequences: q, k [B, Hk, Dk], v [B, Hv, Dv], g [B, Hv] or [Hv].  Updates ``state`` [B, Hv, Dv, Dk]
-    (contiguous float32) in place and returns y [B, Hv, Dv].  Not differentiable."""
+    (contiguous float32) in place and returns y [B, Hv, Dv].  Not differentiable: with gradients enabled, a backward pass
+    that reaches a step whose inputs require them raises."""
     _check(q, k, v, g, state, 1)
     if state.dtype != torch.float32 or not state.is_contiguous():
         raise ValueError("state must be contiguous float32: it is updated in place")
     (B, Hk, Dk), (Hv, Dv), dev = q.shape, v.shape[1:], q.device
+    inputs = (q, k, v, g, state) if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, g, state)) else None
+    if inputs:
+        # torch itself refuses leaves and views made without gradients, whose earlier uses the change of version guards
+        with contextlib.suppress(RuntimeError):
+            _NoGradient.apply(state, q, k, v, g)
     # the copies stay referenced until the launch is enqueued
     q, k, v, g = q.detach().contiguous(), k.detach().contiguous(), v.detach().contiguous(), g.detach()
     y = torch.empty((B, Hv, Dv), dtype=q.dtype, device=dev)
@@ -140,4 +160,4 @@ def linear_attention_step(q: Array, k: Array, v: Array, g: Array, state: Array, 
                                          Dk ** -0.5 if scale is None else float(scale), L.DTYPE_CODE[q.dtype],
                                          L.DTYPE_CODE[g.dtype], L.stream_handle(dev)))
     L.written((state,))
-    return y
+    return _NoGradient.apply(y, *inputs) if inputs else y
