@@ -63,13 +63,19 @@ class LinearLM(torch.nn.Module):
         self.head = torch.nn.Linear(hidden, vocab, bias=False)
         self.register_buffer("inv_freq", rotary_frequencies(head_dim // 2)[0], persistent=False)
 
+    def _apply(self, fn, *args, **kw):
+        """Moves and casts of the whole model: the frequencies go along and keep their 64 bits."""
+        inv = self.inv_freq
+        super()._apply(fn, *args, **kw)
+        self.inv_freq = inv.to(self.inv_freq.device)
+        return self
+
     def forward(self, ids: Array, start: int = 0, states: Optional[list] = None) -> tuple[Array, list]:
         """(logits [B, T, vocab], the layers' states after the last token) of ids [B, T] at positions start on."""
         positions = torch.arange(start, start + ids.shape[1], device=ids.device)
-        inv = self.inv_freq.double()
         x, out = self.embed(ids), []
         for i, (mixer, mlp) in enumerate(zip(self.mixers, self.mlps)):
-            y, state = mixer(self.norms[2 * i](x), positions, inv, None if states is None else states[i])
+            y, state = mixer(self.norms[2 * i](x), positions, self.inv_freq, None if states is None else states[i])
             out.append(state)
             x = x + y
             x = x + mlp(self.norms[2 * i + 1](x))
@@ -125,7 +131,6 @@ def main(argv: list[str] | None = None) -> int:
     torch.manual_seed(args.seed)
     model = LinearLM(args.vocab, args.hidden, args.layers, args.key_heads, args.value_heads, args.head_dim)
     model = model.to(device=dev, dtype=torch.bfloat16 if args.bf16 else torch.float32)
-    model.inv_freq = rotary_frequencies(args.head_dim // 2, device=dev)[0]  # float64, also in a bf16 model
     opt = torch.optim.AdamW(model.parameters(), lr=args.lr)
     ids = torch.randint(0, args.vocab, (args.batch, args.tokens + 1), device=dev)
     torch.cuda.synchronize(dev)
