@@ -21,10 +21,11 @@
 // segments at once.
 //
 // Inputs in bf16 use v_mfma_f32_16x16x32_bf16, whose operands q, k, v and dy are exact; fp32 and fp16 inputs are held as fp32
-// and use v_mfma_f32_16x16x4_f32.  Sums and states are fp32, decays' sums fp64.  What bf16 rounds besides:
-//   P and the state as operands of Y, once (2^-8 of an element at most, as the output's own rounding);
-//   the state in the passes that a and b are formed from, in two terms (2^-17): the chain subtracts them;
-//   e^{G_C - G_s} v_s in three terms (2^-26): the final state is an fp32 output.
+// and use v_mfma_f32_16x16x4_f32.  Sums and states are fp32, decays' sums fp64.  What bf16 rounds besides is split into terms:
+//   P and the state as operands of outputs and gradients, and of a and b, which a chain subtracts: two (2^-17).  In one term (2^-8)
+//     Y and DV of 4 sequences of 4096 tokens were 1.4 times as far from 64 bits as sums of 32 bits rounded once, short ones up
+//     to 1.6 times, now 1.0, for 6 % of a training step's time and 12 % of a prompt's;
+//   e^{G_C - G_s} v_s: three (2^-26), as the final state is an fp32 output.
 //
 // What bounds the passes is the issue of instructions and the waits between them, not memory: 4 sequences of 4096 tokens, 16
 // key and 32 value heads of 128 channels, bf16: Y 155 us, DQ and DK 186 each, DV 190, a segment sum 68 (up to 5% less on
@@ -145,6 +146,32 @@ __device__ __forceinline__ F32Frag col_frag(const float *t, int lane, int k0, in
     for (int j = 0; j < 8; ++j) f.v[j] = p[j * L::LD];
     return f;
 }
+
+// P in LDS, [outputs][sources].  fp32: a tile of C columns.  bf16: two terms of every element, of the six pieces of 16 outputs by
+// 32 sources that hold pairs (whole tiles would leave no room for DV's second workgroup).  A term of a piece is 1 KB, its 16-byte
+// chunks permuted so that reads of an operand and writes of a block of products meet no conflict.
+template <typename ET, bool REV>
+struct Pairs {
+    static constexpr bool F32 = std::is_same_v<ET, float>;
+    using L = Lds<ET, C>;
+    static constexpr int TERMS = F32 ? 1 : 2, TERM = 512, SIZE = F32 ? C * L::LD : 6 * TERMS * TERM;
+    // where the piece of outputs r0 (a multiple of 16) and sources s0 (of 32) begins
+    static __device__ __forceinline__ int piece(int r0, int s0) {
+        const int r = r0 >> 4;
+        return ((s0 >> 5) == (REV ? 1 : 0) ? r : REV ? 4 + r : 2 + r) * TERMS * TERM;
+    }
+    // 4 sources from s on, a multiple of 4
+    static __device__ __forceinline__ int at(int r, int s) {
+        if constexpr (F32) return L::at4(r, s);
+        else return piece(r & ~15, s & ~31) + (r & 15) * 32 + ((((s >> 3) & 3) ^ ((r >> 2) & 3)) << 3) + (s & 7);
+    }
+    // the operand: row li, sources 8 g on
+    static __device__ __forceinline__ int lane(int li, int g) { return F32 ? L::row_lane(li, g) : li * 32 + ((g ^ (li >> 2)) << 3); }
+    static __device__ __forceinline__ Frag<ET> frag(const ET *p, int lane, int r0, int s0, int term) {
+        if constexpr (F32) return row_frag<L>(p, lane, r0, s0);
+        else return *reinterpret_cast<const bf8 *>(p + piece(r0, s0) + term * TERM + lane);
+    }
+};
 
 // Two numbers rounded to bf16 by one instruction, and back.
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
@@ -392,20 +419,20 @@ template <typename ET, int D, int NV, int NW, int KIND, int G>
 struct Shared {
     using LK = Lds<ET, D>;        // tiles Q' and K'
     using LV = Lds<ET, 16 * NV * NW>;  // V' and X
-    using LP = Lds<ET, C>;        // P
+    using P = Pairs<ET, (KIND >= DK)>;
     static constexpr bool TAKEN = p_over_q<ET, D>(), DOT = KIND == DQ || KIND == DK;
     static constexpr int SUM = 4 * NV * 64 * NW;  // float4s of a head's outputs
     ET Q[G][C * LK::LD], K[G][C * LK::LD], V[C * LV::LD];
-    ET own_p[G][TAKEN ? 8 : C * LP::LD], own_x[KIND == DV && !TAKEN ? C * LV::LD : 8];
+    ET own_p[G][TAKEN ? 8 : P::SIZE], own_x[KIND == DV && !TAKEN ? C * LV::LD : 8];
     Decays d[G];
     float total[G], dot[DOT ? G : 1][DOT ? NW : 1][DOT ? C : 1];
     static constexpr bool SUM_OVER_Q = SUM * sizeof(float4) <= G * C * LK::LD * sizeof(ET);
     float4 own_sum[G == 2 && !SUM_OVER_Q ? SUM : 1];
     // where Q' was, once it is used: the waves' sums of M for each token, [NW][C]
     using Cross = std::conditional_t<std::is_same_v<ET, float>, double, float>;
-    __device__ __forceinline__ Cross *cross() { return reinterpret_cast<Cross *>(Q[0] + (TAKEN ? C * LP::LD + C * LV::LD : 0)); }
+    __device__ __forceinline__ Cross *cross() { return reinterpret_cast<Cross *>(Q[0] + (TAKEN ? P::SIZE + C * LV::LD : 0)); }
     __device__ __forceinline__ ET *p(int i) { return TAKEN ? Q[0] : own_p[i]; }
-    __device__ __forceinline__ ET *x() { return TAKEN ? Q[0] + C * LP::LD : own_x; }
+    __device__ __forceinline__ ET *x() { return TAKEN ? Q[0] + P::SIZE : own_x; }
     __device__ __forceinline__ float4 *sum() { return SUM_OVER_Q ? reinterpret_cast<float4 *>(Q[0]) : own_sum; }
 };
 
@@ -604,11 +631,11 @@ constexpr int waves() { return std::is_same_v<ET, bf16> && D <= 128 ? 2 : 1; }
 template <typename ET, int D, int NV, int NW, int KIND, int G, bool VEC>
 __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(const Pass a) {
     constexpr bool F32 = std::is_same_v<ET, float>, REV = KIND >= DK, DOT = KIND == DQ || KIND == DK;
-    constexpr int NS = F32 ? 1 : 3, NH = F32 || !DOT ? 1 : 2;  // terms of the weighted V', of the state as an operand
+    constexpr int NS = F32 ? 1 : 3, NH = F32 ? 1 : 2;  // terms of the weighted V', of the state as an operand
     constexpr int RT = C / 16;
     using LK = Lds<ET, D>;
     using LV = Lds<ET, 16 * NV * NW>;
-    using LP = Lds<ET, C>;
+    using P = Pairs<ET, REV>;
     constexpr bool TAKEN = Shared<ET, D, NV, NW, KIND, G>::TAKEN;
     __shared__ __attribute__((aligned(16))) Shared<ET, D, NV, NW, KIND, G> sh;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & (NW - 1), grp = wave / NW;
@@ -771,9 +798,15 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
         if constexpr (KIND == DV) tx.store(sh.x(), n, a.dv - c0, a.dt);
         if constexpr (KIND == DV) read_decays();
         const auto put = [&](int r, int s, const f4 &p) {
-            ET *o = sP + LP::at4(r, s);
-            if constexpr (F32) *reinterpret_cast<f4 *>(o) = p;
-            else *reinterpret_cast<uint2 *>(o) = make_uint2(pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]));
+            ET *o = sP + P::at(r, s);
+            if constexpr (F32) {
+                *reinterpret_cast<f4 *>(o) = p;
+            } else {
+                const uint32_t a = pack_bf16(p[0], p[1]), b = pack_bf16(p[2], p[3]);
+                *reinterpret_cast<uint2 *>(o) = make_uint2(a, b);
+                *reinterpret_cast<uint2 *>(o + P::TERM) = make_uint2(pack_bf16(p[0] - low_bf16(a), p[1] - high_bf16(a)),
+                                                                     pack_bf16(p[2] - low_bf16(b), p[3] - high_bf16(b)));
+            }
         };
 #pragma unroll
         for (int e = 0; e < BLOCKS; ++e) {
@@ -828,7 +861,7 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
             sh.cross()[w * C + l] = mine;
         }
         const float total = sh.total[grp];
-        const int lp = LP::row_lane(li, g), lkc = LK::template col_lane<8>(li, g);
+        const int lp = P::lane(li, g), lkc = LK::template col_lane<8>(li, g);
         const auto pairs_of = [&](int k0, const Frag<ET> (&v)[NV]) {
             // an infinite or NaN source of a later token (reverse: an earlier one) must not reach an output through its weight
             // of 0: where a product with zeros shows one, the sum takes the pairs that count one by one (looking costs a pass
@@ -842,7 +875,8 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
 #pragma unroll 1
                     for (int s = k0; s < k0 + 32; ++s) {
                         if (REV ? s < 16 * rt + li : s > 16 * rt + li) continue;
-                        const float p = (float)sP[LP::at4(16 * rt + li, s & ~3) + (s & 3)];
+                        const ET *const ps = sP + P::at(16 * rt + li, s & ~3) + (s & 3);
+                        const float p = F32 ? (float)ps[0] : (float)ps[0] + (float)ps[P::TERM];
                         const ET *const vs = sh.V + LV::at4(s, col - c0);
 #pragma unroll
                         for (int j = 0; j < 4 * NV; ++j) O[rt][j / 4][j % 4] = fmaf(p, (float)vs[j], O[rt][j / 4][j % 4]);
@@ -852,9 +886,12 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
                 if (REV ? 16 * rt >= k0 + 32 : 16 * rt + 16 <= k0) continue;
-                const Frag<ET> p = row_frag<LP>(sP, lp, 16 * rt, k0);
 #pragma unroll
-                for (int x = 0; x < NV; ++x) O[rt][x] = mma(v[x], p, O[rt][x]);
+                for (int n = 0; n < P::TERMS; ++n) {
+                    const Frag<ET> p = P::frag(sP, lp, 16 * rt, k0, n);
+#pragma unroll
+                    for (int x = 0; x < NV; ++x) O[rt][x] = mma(v[x], p, O[rt][x]);
+                }
             }
         };
         Weighted<ET, NV, NS> next;
