@@ -13,7 +13,7 @@
 //   dg_t = c + sum_{r >= t} a_r + sum_{s < t} b_s + sum_{r >= t > s} M_rs,   c = e^{G_C} <dS', S>,
 // sums without cancellation.  c comes by a chain, from D, the product <dS, S> of the states between two chunks: c = D - sum b of
 // the chunk before it, c = D - sum a of the chunk after it, and D goes on as c + sum a backwards, c + sum b forwards.  Rounding
-// errors of a chain stay while what they belong to fades, so every MARK chunks DQ leaves its state and DK multiplies its own
+// errors of a chain stay while what they belong to fades, so every few chunks (mark_of) DQ leaves its state and DK multiplies its own
 // with it: a chain runs at most that far, wherever the sequence is cut, and from the end whose terms are smaller.  Through a
 // chunk whose decay is below the errors of a and b nothing is passed on: c = 0.
 // So one kernel, pass_kernel, computes all four.  Where there are few heads, the sequence is cut into segments: seg_kernel
@@ -49,7 +49,6 @@ namespace la {
 
 constexpr int NT = 256;
 constexpr int C = 64;  // tokens of a chunk
-constexpr int MARK = 8;  // chunks between two products of the states (512 KB of states for 4096 tokens of a head of 128 x 128)
 constexpr double LOG2E = 1.4426950408889634074;
 
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -392,6 +391,11 @@ static_assert(DECAYS == NT, "one float to a thread");
 
 enum Kind { Y, DQ, DK, DV };  // what a pass computes
 
+// Chunks between two products of the states.  Eight: 512 KB of states for 4096 tokens of a head of 128 x 128; four take 2.4 % of
+// a bf16 step's time, whose a and b have 17 bits.  fp32 and fp16 inputs, whose a and b have more, take four: one decay for a
+// head of 2047 tokens is 5e-7 off (8e-7 with eight; 32-bit chunks in plain form 7e-7), for 0.7 % of the time.
+constexpr int mark_of(bool f32) { return f32 ? 4 : 8; }
+
 struct Pass {
     Ten Q, K, V, X;
     const float *decays;  // [B][Hv][nc][DECAYS]
@@ -400,7 +404,7 @@ struct Pass {
     int64_t s_head, s_seg;
     int s_t;            // states are [v'][k'] (0) or [k'][v'] (1)
     void *o;            // [B][T][heads][dv] contiguous
-    float *marks;       // DQ writes, DK reads: the states entering chunks 0, MARK, 2 MARK, .., as the lanes hold them,
+    float *marks;       // DQ writes, DK reads: the states entering every mark_of() chunks, from the first on, as the lanes hold them,
                         // [B][Hv][nm][slices][D / 16][NV][64 NW][4]
     double *ends;       // DK: their products with the cotangents there, [B][Hv][nm][slices][NW], a wave's part each
     int nm, mark0;      // marks of the sequence; the first that is taken (1 where the state before the first token is zero)
@@ -686,8 +690,9 @@ __global__ __launch_bounds__(64 * NW * G, (waves<ET, D>())) void pass_kernel(con
         // opaque: addresses in LDS are formed where they are used, not hoisted out of the loop and spilled
         const int tid = opaque(threadIdx.x), l = tid & 63, li = l & 15, g = l >> 4;
         const int col = c0 + 16 * NV * w + 4 * NV * g;  // the lane's first column of O
-        const bool marked = DOT && c % MARK == 0 && c / MARK >= a.mark0;
-        const int64_t mark = marked ? (head * a.nm + c / MARK) * a.slices + slice : 0;
+        constexpr int M = mark_of(F32);
+        const bool marked = DOT && c % M == 0 && c / M >= a.mark0;
+        const int64_t mark = marked ? (head * a.nm + c / M) * a.slices + slice : 0;
         if constexpr (KIND == DQ) {
             if (marked) S.put(a.marks + mark * (D * 16 * NV * NW), w * 64 + l);
         }

@@ -73,7 +73,7 @@ struct DecayGrad {
     const float *a, *b, *cross;  // [slices][B][Hv][T]; cross: [cross_slices]
     const float *decays;         // [B][Hv][nc][DECAYS]
     const float *dlast, *last;   // [B][Hv][size], or dlast NULL
-    const double *ends;          // <dS, S> before chunks 0, MARK, .., from mark0 on, [B][Hv][nm][parts]
+    const double *ends;          // <dS, S> before every mark_of() chunks, from mark0 on, [B][Hv][nm][parts]
     void *dg;                    // [B][T][Hv]
     double *sums;                // or with one decay per head [Hv][B][nm]
     int B, T, Hv, slices, cross_slices, per_head, dt, nc, nm, mark0, parts;
@@ -85,6 +85,7 @@ struct DecayGrad {
 // that it adds, so the end is taken whose magnitudes add up to less.  A NaN or infinite value or key makes the states after it
 // odd, a query or cotangent those before it: of the two ends, and of the two sums over a chunk's tokens, each is formed from one
 // side alone, so that gradients between a state and a cotangent that are both finite are, too.  grid (nm, Hv, B).
+template <int MARK>
 __global__ __launch_bounds__(64 * MARK) void dg_kernel(const DecayGrad a) {
     __shared__ double A[MARK], B[MARK], red[MARK], D0, D1;
     __shared__ float absA[MARK], absB[MARK];
@@ -293,7 +294,8 @@ static Sizes sizes(int B, int T, int Hk, int Hv, int Dk, int Dv, int dtype = DT_
     s.cross = align_up256(rows * slices_of(Dk, Dv));
     // of the passes that write dq and dk, whose K' are the value channels
     const int slices = slices_of(Dv, Dk);
-    s.nm = (p.nc + MARK - 1) / MARK;
+    const int mark = mark_of(dtype != DT_BF16);
+    s.nm = (p.nc + mark - 1) / mark;
     s.parts = slices * waves_of(Dv, Dk, dtype);
     const size_t marks = (size_t)B * Hv * s.nm;
     s.marks = align_up256(marks * slices * rows_of(Dv) * cols_of(Dv, Dk) * sizeof(float));
@@ -491,7 +493,10 @@ extern "C" int gdn_linatt_bwd(const void *q, const void *k, const void *v, const
                           dtype == GDN_BF16 ? 0x1p-20f : 0x1p-26f, size};
     {
         Timed tm("linatt_dg", st);
-        hipLaunchKernelGGL(la::dg_kernel, dim3((unsigned)sz.nm, (unsigned)Hv, (unsigned)B), dim3(64 * la::MARK), 0, st, d);
+        const dim3 grid((unsigned)sz.nm, (unsigned)Hv, (unsigned)B);
+        constexpr int M16 = la::mark_of(false), M32 = la::mark_of(true);
+        if (dtype == GDN_BF16) hipLaunchKernelGGL(la::dg_kernel<M16>, grid, dim3(64 * M16), 0, st, d);
+        else hipLaunchKernelGGL(la::dg_kernel<M32>, grid, dim3(64 * M32), 0, st, d);
         if (g_per_head)
             hipLaunchKernelGGL(la::dg_head_kernel, dim3((unsigned)Hv), dim3(la::NT), 0, st, sums, dg, (int64_t)B * sz.nm, g_dtype);
     }

@@ -175,3 +175,18 @@ def test_nan_where_no_loss_is_left(dev, dtype):
         bad[:, t] = math.nan
         each_head(gradient(q, bad, v, g, state, cut)[:, :t + 1], gradient(q, k, v, g, state, cut)[:, :t + 1].double(),
                   2 * tolerance(dtype)[0], t)
+
+
+def test_one_decay_for_a_head_in_32_bits(dev):
+    """fp32: products of the states at most four chunks apart, two chunks of a's and b's from the nearer end.  As in the head of
+    this file, with e = 2^-22 (sums of 128 terms, 2^-24 each, independent) and 256 in the place of 512: e * 256 / tau of the
+    size of a head's sums, for the three longest of these memories (tau = 64 to 256) 2^-20.  Over eight sequences, one by one."""
+    B, T, Hv, D = 8, 2047, 3, 128
+    q, k, v, _, state, dy, dlast = inputs(dev, B, T, 1, Hv, D, D, torch.float32, 9)
+    g = -torch.exp2(-torch.tensor([6.0, 7.0, 8.0], device=dev))
+    want = states64(q, k, v, g, state, D ** -0.5, dy, dlast).sum(1)
+    got = torch.stack([gradient(q[b:b + 1], k[b:b + 1], v[b:b + 1], g, state[b:b + 1], dy[b:b + 1], dlast[b:b + 1])
+                       for b in range(B)]).double()
+    err = (got - want).norm(dim=0) / want.norm(dim=0)
+    print("one decay for a head", err.tolist(), flush=True)
+    assert float(err.max()) <= 2.0 ** -20, err.tolist()
