@@ -89,8 +89,12 @@ template <typename ET, int W>
 struct Lds {
     static constexpr bool F32 = std::is_same_v<ET, float>;
     static constexpr int LD = W + (F32 ? 4 : 0);
+    static __device__ __forceinline__ int quad(int r) {
+        const int q = (r >> 2) & 3;
+        return ((q ^ (q << 1)) & 2) | (q >> 1);  // 0, 2, 3, 1
+    }
     static __device__ __forceinline__ int swz(int r) {
-        const int q = (r >> 2) & 3, low = ((q ^ (q << 1)) & 2) | (q >> 1);  // 0, 2, 3, 1
+        const int low = quad(r);
         return W == 64 ? ((r & 2) << 1) | low : ((r & 3) << 2) | low;
     }
     static __device__ __forceinline__ int add(int o, int x) { return F32 ? o + x : o ^ x; }
@@ -162,10 +166,10 @@ struct Pairs {
     // 4 sources from s on, a multiple of 4
     static __device__ __forceinline__ int at(int r, int s) {
         if constexpr (F32) return L::at4(r, s);
-        else return piece(r & ~15, s & ~31) + (r & 15) * 32 + ((((s >> 3) & 3) ^ ((r >> 2) & 3)) << 3) + (s & 7);
+        else return piece(r & ~15, s & ~31) + (r & 15) * 32 + ((((s >> 3) & 3) ^ L::quad(r)) << 3) + (s & 7);
     }
     // the operand: row li, sources 8 g on
-    static __device__ __forceinline__ int lane(int li, int g) { return F32 ? L::row_lane(li, g) : li * 32 + ((g ^ (li >> 2)) << 3); }
+    static __device__ __forceinline__ int lane(int li, int g) { return F32 ? L::row_lane(li, g) : li * 32 + ((g ^ L::quad(li)) << 3); }
     static __device__ __forceinline__ Frag<ET> frag(const ET *p, int lane, int r0, int s0, int term) {
         if constexpr (F32) return row_frag<L>(p, lane, r0, s0);
         else return *reinterpret_cast<const bf8 *>(p + piece(r0, s0) + term * TERM + lane);
