@@ -8,7 +8,9 @@
 // time.  Squares are summed in 64 bits: neither their range (1e20^2 overflows 32 bits) nor the length of the sum
 // matters, and one 64-bit FMA per element stays well under the time of its load.  HBM-bound: one read for the norm, one
 // read (from the Infinity Cache where the tensors fit) and one write for the scaling.  1.41 GB of bf16 in
-// 84 tensors: 843 us, 5.0 TB/s over the three passes.  320 small fp32 tensors (79 MB): 76 us of kernels.
+// 84 tensors: 846 us, 5.0 TB/s over the three passes.  320 small fp32 tensors (80 MB): 64 us of kernels, in seven launches.
+// Tensors at addresses that are no multiple of 16 bytes go element by element: 80 MB of bf16, norm 38 us against 17, scaling 46
+// against 28.
 #include <algorithm>
 #include <vector>
 

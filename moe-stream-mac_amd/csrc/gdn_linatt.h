@@ -24,18 +24,20 @@
 // and use v_mfma_f32_16x16x4_f32.  Sums and states are fp32, decays' sums fp64.  What bf16 rounds besides is split into terms:
 //   P and the state as operands of outputs and gradients, and of a and b, which a chain subtracts: two (2^-17).  In one term (2^-8)
 //     Y and DV of 4 sequences of 4096 tokens were 1.4 times as far from 64 bits as sums of 32 bits rounded once, short ones up
-//     to 1.6 times, now 1.0, for 6 % of a training step's time and 12 % of a prompt's;
+//     to 1.6 times, now 1.0, for 6 % of a training step's time and 7 % of a prompt's;
 //   e^{G_C - G_s} v_s: three (2^-26), as the final state is an fp32 output.
 //
 // What bounds the passes is the issue of instructions and the waits between them, not memory: 4 sequences of 4096 tokens, 16
-// key and 32 value heads of 128 channels, bf16: Y 155 us, DQ and DK 186 each, DV 190, a segment sum 68 (up to 5% less on
-// other cards), for 0.3 to 0.5 GB of traffic each (60 to 100 us at the card's copy rate).  A wave's matrix instructions (Y:
-// 156 of 16 cycles in a chunk) and its vector instructions (some 770: decays, the state and V' split into bf16 terms, tiles
-// to LDS) take the SIMD's time one after the other, and each of its two waves spends a third of its time on a dependency and
-// a quarter at barriers.  Measured along the way: loads under branches, each waited for where it stands, and one workgroup
-// to a CU: Y 295 us, DQ 367.  LDS rows padded instead of permuted (three times the conflicts) and X loaded behind the next
-// tiles: DQ 269, DV 245.  P in sixteen blocks instead of the twelve that count, weights formed ahead of all products instead
-// of between them, and a chunk's loads all at one place: Y 161, DQ 208, DV 203.
+// key and 32 value heads of 128 channels, bf16: Y 179 us, DQ 210, DK 217, DV 213, a segment sum 66 to 70 (medians of one run on
+// one card; its shortest launches, and other cards, take 10 to 15 % less), for 0.3 to 0.6 GB of traffic each (60 to 110 us at the
+// card's copy rate).  In a chunk of Y a wave has 200 matrix instructions of 16 cycles and some 970 vector instructions (decays,
+// P, the state and V' split into bf16 terms, tiles to LDS), which take the SIMD's time one after the other.  Of the passes' wave
+// cycles 27 to 36 % wait for an instruction's issue (SQ_WAIT_INST_ANY) and 24 to 40 % for anything else, loads, LDS or barriers,
+// which no counter tells apart (SQ_WAIT_ANY); matrix units are busy 24 to 29 %.  Measured along the way, when P and the state of Y
+// and DV were rounded to one term: loads under branches, each waited for where it stands, and one workgroup to a CU: Y 295 us, DQ
+// 367.  LDS rows padded instead of permuted (three times the conflicts) and X loaded behind the next tiles: DQ 269, DV 245.  P in
+// sixteen blocks instead of the twelve that count, weights formed ahead of all products instead of between them, and a chunk's
+// loads all at one place: Y 161, DQ 208, DV 203, and without them 155, 186, 190.
 #pragma once
 
 #include <type_traits>
@@ -994,7 +996,7 @@ struct Seg {
 };
 
 // What a segment adds to a state that starts from nothing, and its decay.  The segment that the chain ends with is left out
-// (the last; reverse: the first).  Three quarters of the sequence's state products once more (67 us at B=4, T=4096, Hv=32), for
+// (the last; reverse: the first).  Three quarters of the sequence's state products once more (66 us at B=4, T=4096, Hv=32), for
 // four times as many workgroups in every pass: unsplit, 128 heads leave half of 256 CUs without work.
 template <typename ET, int D, int NV, int NW, bool REV, bool VEC>
 __global__ __launch_bounds__(64 * NW, (waves<ET, D>())) void seg_kernel(const Seg a) {
@@ -1107,7 +1109,7 @@ void launch_seg(const Seg &a, bool rev, hipStream_t st) {
     else hipLaunchKernelGGL((seg_kernel<ET, D, NV, NW, false, VEC>), grid, block, 0, st, a);
 }
 // 128 columns of V' go to four waves of 32 in bf16 (eight of 16 read the K' and Q' tiles twice as often: 171 us against 144
-// for two sequences of 8100 tokens, 32 heads, when both were tried; now 137), to eight of 16 in fp32 (two waves to a SIMD: 83 us
+// for two sequences of 8100 tokens, 32 heads, when both were tried, with one term of P and the state), to eight of 16 in fp32 (two waves to a SIMD: 83 us
 // against 87 for 2047 tokens; now 80).
 template <typename ET>
 constexpr int wide_columns() { return std::is_same_v<ET, bf16> ? 2 : 1; }

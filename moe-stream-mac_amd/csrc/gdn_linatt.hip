@@ -10,7 +10,7 @@ namespace la {
 constexpr int MAX_D = 256;
 
 // The decays of every chunk, a wave to a chunk, once for the five or six kernels that use them (a wave of each pass would
-// spend two 64-bit exponentials a chunk).  Sums run in 64 bits.  9 us at B=4, T=4096, Hv=32: latency.
+// spend two 64-bit exponentials a chunk).  Sums run in 64 bits.  7 us at B=4, T=4096, Hv=32: latency.
 __global__ __launch_bounds__(NT) void decay_kernel(Gate g, float *o, int B, int T, int Hv, int nc) {
     const int64_t id = block_index() * (NT / 64) + (threadIdx.x >> 6);
     const int l = threadIdx.x & 63;
@@ -57,7 +57,7 @@ __global__ __launch_bounds__(NT) void scan_kernel(float *s, const float *decay, 
     }
 }
 
-// The heads of a group added in order: part [rows][group][D] to o [rows][D].  13 us for 2047 tokens of 2 x 16 heads of 128 in
+// The heads of a group added in order: part [rows][group][D] to o [rows][D].  11 us for 2047 tokens of 2 x 16 heads of 128 in
 // fp32 (50 MB).  Atomics into o would round and order the sums differently every time.
 __global__ __launch_bounds__(NT) void group_kernel(const float *part, void *o, int64_t n, int group, int D, int dt) {
     const int64_t i = block_index() * NT + threadIdx.x;
@@ -84,7 +84,8 @@ struct DecayGrad {
 // dg between two marks, in 64 bits: a wave sums one chunk; c by the chain from either end.  Its errors are those of the numbers
 // that it adds, so the end is taken whose magnitudes add up to less.  A NaN or infinite value or key makes the states after it
 // odd, a query or cotangent those before it: of the two ends, and of the two sums over a chunk's tokens, each is formed from one
-// side alone, so that gradients between a state and a cotangent that are both finite are, too.  grid (nm, Hv, B).
+// side alone, so that gradients between a state and a cotangent that are both finite are, too.  grid (nm, Hv, B).  22 us at B=4, T=4096, Hv=32, 9 at B=1, T=2047 (and 5 for
+// the sums of one decay per head): latency, a workgroup's loads, sums and one barrier after the other.
 template <int MARK>
 __global__ __launch_bounds__(64 * MARK) void dg_kernel(const DecayGrad a) {
     __shared__ double A[MARK], B[MARK], red[MARK], D0, D1;
@@ -166,8 +167,9 @@ __global__ __launch_bounds__(NT) void dg_head_kernel(const double *sums, void *d
 
 // One token: y = scale S' q, S' = e^g S + v k^T, in place.  `lanes` lanes share a row of the state, V channels each at a time,
 // and walk STEP_ROWS rows side by side, all of whose loads are under way before the first is used: the state, read and
-// written once, is the kernel's traffic.  64 sequences of 32 states of 128 x 128: 268 MB in 52.7 us, 5.1 TB/s, what a copy
-// reaches.
+// written once, is the kernel's traffic.  64 sequences of 32 states of 128 x 128: 268 MB in 52.8 us, 5.1 TB/s, what a copy
+// reaches (44 us where the same states come again and part of them lies in the Infinity Cache).  One channel at a time, for states
+// at any address: 66 us against 45.
 constexpr int STEP_ROWS = 4;
 struct Step {
     const void *q, *k, *v;
@@ -220,7 +222,7 @@ struct Plan {
 };
 // Segments: two workgroups for each compute unit (their LDS leaves room for no more), and at least four chunks of work for
 // each, as a segment costs its state's way through memory and its part of the sums (a single sequence of 2047 tokens, 32 fp32
-// heads: eight segments, the forward pass 80 us).
+// heads: eight segments, the forward pass 81 us).
 static Plan plan(int B, int T, int Hv, int Dk, int Dv) {
     const int64_t wgs = (int64_t)B * Hv * slices_of(Dk, Dv), nc = ((int64_t)T + C - 1) / C;
     int64_t want = (512 + wgs - 1) / wgs;

@@ -14,8 +14,8 @@
 // Gradient: dz_j = d ([j = target] - p_j) - e p_j (log p_j + H) for the cotangents d of logp and e of H.  Streaming:
 // logits in, gradient out.
 //
-// Measured: 8192 rows of 32000 bf16 logits (524 MB): pieces 128 us (4.1 TB/s; 136 with a group of 8 loaded after the other),
-// join 8, gradient 161 (1.05 GB less what ignored rows need not read).  64 rows of 131072 with entropy and 20 alternatives
+// Measured: 8192 rows of 32000 bf16 logits (524 MB): pieces 126 us (4.2 TB/s; 136 with a group of 8 loaded after the other),
+// join 6, gradient 159 (1.05 GB less what ignored rows need not read).  64 rows of 131072 with entropy and 20 alternatives
 // 22.5 us: 26 with one lane to a key in the ranking, 30 with every thread's largest key ranked first.
 #include "gdn_common.h"
 #include "gdn_host.h"

@@ -8,7 +8,10 @@
 // Angles of far positions lose everything in 32 bits (p = 10^6: half an ulp is 0.03 rad), so turns p * inv_freq / 2 pi
 // are formed and reduced to [-1/2, 1/2] in 64 bits; sine and cosine of what is left are 32-bit.  That is R/2 pairs per
 // token, shared by its heads through LDS.  The rest is a copy: 2 x 8192 tokens of 48 heads of 128 bf16 channels, 0.40 GB, in
-// 85 us (4.7 TB/s; a plain copy 5.1).  One head and one vector at a time took 159 us, the type looked up per load 120.
+// 87 us (4.6 TB/s; a plain copy 5.1).  One head and one vector at a time took 159 us, the type looked up per load 120.
+//
+// Loads are as wide as sizes, strides and addresses allow: 89 us a launch of that size with 8 channels each, 100 with 4 (rows of
+// the projection 4 channels longer), 226 with one (an odd row, as of a projection of q, k, v and an odd number of decays).
 #include "gdn_common.h"
 #include "gdn_host.h"
 #include "gdn_vec.h"

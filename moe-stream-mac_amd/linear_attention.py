@@ -108,8 +108,12 @@ def linear_attention(q: Array, k: Array, v: Array, g: Array, state: Optional[Arr
     and the log decays ``g`` [B, T, Hv], or [Hv] for one of each head; value head h reads key head h / (Hv / Hk).
 
     ``state`` is the state before the first token (None: zeros), ``scale`` defaults to Dk^-1/2.  A log decay of -inf keeps
-    nothing of the state.  A token's infinite or NaN values do not reach earlier outputs.  q, k, v and g may be strided views; heads have at most 256 channels.  Differentiable in q, k, v,
-    g and state (once: no second derivatives); gradients have their inputs' types."""
+    nothing of the state.  q, k, v and g may be strided views; heads have at most 256 channels.  Differentiable in q, k, v, g
+    and state (once: no second derivatives); gradients have their inputs' types.
+
+    An infinite or NaN input of one token does not reach the outputs before it, nor gradients that it has no part in; what it
+    has a part in may be NaN where the formula gives an infinity.  Decays' gradients that lie between two such tokens less than
+    512 apart may be NaN as well, and one log decay for a head has the sum of all its tokens' gradients."""
     _check(q, k, v, g, state, 2)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if q.shape[0] == 0 or q.shape[1] == 0:  # no token: the state passes through
