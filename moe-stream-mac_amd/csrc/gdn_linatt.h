@@ -13,9 +13,9 @@
 //   dg_t = c + sum_{r >= t} a_r + sum_{s < t} b_s + sum_{r >= t > s} M_rs,   c = e^{G_C} <dS', S>,
 // sums without cancellation.  c comes by a chain, from D, the product <dS, S> of the states between two chunks: c = D - sum b of
 // the chunk before it, c = D - sum a of the chunk after it, and D goes on as c + sum a backwards, c + sum b forwards.  Rounding
-// errors of a chain stay while what they belong to fades, so every few chunks (mark_of) DQ leaves its state and DK multiplies its own
-// with it: a chain runs at most that far, wherever the sequence is cut, and from the end whose terms are smaller.  Through a
-// chunk whose decay is below the errors of a and b nothing is passed on: c = 0.
+// errors of a chain stay while what they belong to fades, so every few chunks (mark_of) DQ leaves its state and DK multiplies
+// its own with it: a chain runs at most that far, wherever the sequence is cut, and from the end whose terms are smaller.
+// Through a chunk whose decay is below the errors of a and b nothing is passed on: c = 0.
 // So one kernel, pass_kernel, computes all four.  Where there are few heads, the sequence is cut into segments: seg_kernel
 // sums each segment's state from nothing, scan_kernel joins them to the states entering each segment, and the passes run all
 // segments at once.
@@ -171,7 +171,9 @@ struct Pairs {
         else return piece(r & ~15, s & ~31) + (r & 15) * 32 + ((((s >> 3) & 3) ^ L::quad(r)) << 3) + (s & 7);
     }
     // the operand: row li, sources 8 g on
-    static __device__ __forceinline__ int lane(int li, int g) { return F32 ? L::row_lane(li, g) : li * 32 + ((g ^ L::quad(li)) << 3); }
+    static __device__ __forceinline__ int lane(int li, int g) {
+        return F32 ? L::row_lane(li, g) : li * 32 + ((g ^ L::quad(li)) << 3);
+    }
     static __device__ __forceinline__ Frag<ET> frag(const ET *p, int lane, int r0, int s0, int term) {
         if constexpr (F32) return row_frag<L>(p, lane, r0, s0);
         else return *reinterpret_cast<const bf8 *>(p + piece(r0, s0) + term * TERM + lane);
@@ -410,8 +412,8 @@ struct Pass {
     int64_t s_head, s_seg;
     int s_t;            // states are [v'][k'] (0) or [k'][v'] (1)
     void *o;            // [B][T][heads][dv] contiguous
-    float *marks;       // DQ writes, DK reads: the states entering every mark_of() chunks, from the first on, as the lanes hold them,
-                        // [B][Hv][nm][slices][D / 16][NV][64 NW][4]
+    float *marks;       // DQ writes, DK reads: the states entering every mark_of() chunks, from the first on, as the lanes hold
+                        // them, [B][Hv][nm][slices][D / 16][NV][64 NW][4]
     double *ends;       // DK: their products with the cotangents there, [B][Hv][nm][slices][NW], a wave's part each
     int nm, mark0;      // marks of the sequence; the first that is taken (1 where the state before the first token is zero)
     float *dot;         // per token [slices][B][Hv][T]: DQ, DK X . (O from the state); DV the pairs that cross it, X = v
@@ -1109,8 +1111,8 @@ void launch_seg(const Seg &a, bool rev, hipStream_t st) {
     else hipLaunchKernelGGL((seg_kernel<ET, D, NV, NW, false, VEC>), grid, block, 0, st, a);
 }
 // 128 columns of V' go to four waves of 32 in bf16 (eight of 16 read the K' and Q' tiles twice as often: 171 us against 144
-// for two sequences of 8100 tokens, 32 heads, when both were tried, with one term of P and the state), to eight of 16 in fp32 (two waves to a SIMD: 83 us
-// against 87 for 2047 tokens; now 80).
+// for two sequences of 8100 tokens, 32 heads, when both were tried, with one term of P and the state), to eight of 16 in fp32
+// (two waves to a SIMD: 83 us against 87 for 2047 tokens; now 80).
 template <typename ET>
 constexpr int wide_columns() { return std::is_same_v<ET, bf16> ? 2 : 1; }
 template <typename ET, int D, bool VEC>

@@ -84,8 +84,9 @@ struct DecayGrad {
 // dg between two marks, in 64 bits: a wave sums one chunk; c by the chain from either end.  Its errors are those of the numbers
 // that it adds, so the end is taken whose magnitudes add up to less.  A NaN or infinite value or key makes the states after it
 // odd, a query or cotangent those before it: of the two ends, and of the two sums over a chunk's tokens, each is formed from one
-// side alone, so that gradients between a state and a cotangent that are both finite are, too.  grid (nm, Hv, B).  22 us at B=4, T=4096, Hv=32, 9 at B=1, T=2047 (and 5 for
-// the sums of one decay per head): latency, a workgroup's loads, sums and one barrier after the other.
+// side alone, so that gradients between a state and a cotangent that are both finite are, too.  grid (nm, Hv, B).  22 us at
+// B=4, T=4096, Hv=32, 9 at B=1, T=2047 (and 5 for the sums of one decay per head): latency, a workgroup's loads, sums and one
+// barrier after the other.
 template <int MARK>
 __global__ __launch_bounds__(64 * MARK) void dg_kernel(const DecayGrad a) {
     __shared__ double A[MARK], B[MARK], red[MARK], D0, D1;
