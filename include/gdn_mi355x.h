@@ -354,6 +354,37 @@ int gdn_clip_grad_norm(const void *const *x, void *const *y, const int64_t *nume
                        int norm_inf, double max_norm, double eps, float *norm, void *workspace, size_t workspace_bytes,
                        void *stream);
 
+/* Cross entropy of the logits z = x w^T, which are never kept.  x [N][H] and w [V][H] (dtype; row strides in elements, channels
+ * contiguous), targets [N]:
+ *   loss [N]      log sum_v e^{z_v} - z_target; 0 where targets == ignore_index; NaN where the target is outside [0, V)
+ *   stat [N][2]   what gdn_linear_loss_bwd needs (may be NULL)
+ *   total [1]     reduction 1: the losses' sum; 2: their mean over the tokens that count (0 if none does)
+ *   factor [1]    what takes the cotangent of that to a token's.  reduction 0: neither is written, both may be NULL
+ * fp32 outputs.  What x holds at ignored tokens does not reach any other token, nor w's gradient.
+ *
+ * gdn_linear_loss_bwd: dx [N][H] and dw [V][H], contiguous (dtype; either may be NULL), from the cotangents dloss (fp32;
+ * dloss_stride 1: one for each token, 0: one for all), times factor [0] (NULL for 1); dx is 0 at ignored tokens.
+ * N, V <= 2^24, H <= 2^17.  The workspace of the forward pass: want_dx = want_dw = 0.  aligned: both operands lie on 16 bytes,
+ * with rows a multiple of 16 bytes apart; without it there is room for copies of them. */
+size_t gdn_linear_loss_workspace_bytes(int64_t N, int64_t H, int64_t V, int dtype, int aligned, int want_dx, int want_dw);
+int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *targets, float *loss, float *stat, float *total,
+                        float *factor, void *workspace, size_t workspace_bytes, int64_t N, int64_t H, int64_t V, int64_t x_stride,
+                        int64_t w_stride, int64_t ignore_index, int reduction, int dtype, void *stream);
+int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *targets, const float *stat, const float *dloss,
+                        int64_t dloss_stride, const float *factor, void *dx, void *dw, void *workspace,
+                        size_t workspace_bytes, int64_t N, int64_t H, int64_t V, int64_t x_stride, int64_t w_stride,
+                        int64_t ignore_index, int dtype, void *stream);
+
+/* Rows of a table: y [N][H] = scale * w[ids[n]] (dtype; w_stride elements from row to row, channels contiguous); rows of NaN
+ * where an id lies outside [0, V).  Backward: dw [V][H] (contiguous, every row written) = scale times the sum of dy [N][H]
+ * (dtype, dy_stride elements from row to row) over the tokens of each word, in their order, in 64 bits; without the tokens
+ * equal to padding_idx (-1 for none) and those outside the table.  N, V <= 2^26, H <= 2^20. */
+int gdn_embedding_fwd(const int64_t *ids, const void *w, void *y, int64_t N, int64_t V, int64_t H, int64_t w_stride,
+                      double scale, int dtype, void *stream);
+size_t gdn_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t H);
+int gdn_embedding_bwd(const int64_t *ids, const void *dy, void *dw, void *workspace, size_t workspace_bytes, int64_t N,
+                      int64_t V, int64_t H, int64_t dy_stride, int64_t padding_idx, double scale, int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,585 @@
+// Cross entropy of the logits z = x W^T without keeping them, and its gradients, for gfx950.
+//
+// For token i and word v, z_iv = <x_i, W_v>, M_i = max_v z_iv, s_i = sum_v e^{z_iv - M_i}, target t_i:
+//   loss_i = log s_i + M_i - z_{i,t_i},    p_iv = e^{z_iv - M_i} / s_i,
+//   dx_i = d_i sum_v (p_iv - [v = t_i]) W_v,    dW_v = sum_i d_i (p_iv - [v = t_i]) x_i
+// for the cotangents d_i of the losses.
+//
+// Forward: one product whose tiles of logits end in registers, each as the maximum and the sum of exponentials of its words
+// per token; a second kernel joins them.  Backward: the words in pieces; of each piece the logits again (their normaliser is
+// known only after the last word), from them the differences p - [v = t] as fp16 numbers, then two more products.  What
+// is stored at any time is one piece of differences, at most 2^26 of them.
+//
+// Words lie along registers and tokens along lanes, so that maxima and sums run within a lane.
+//
+// Precision.  Differences lie in [-1, 1] and have 11 bits as fp16 numbers times 2^15 (those below 2^-29 fewer); bf16 would
+// leave 8, as many as the results have, and make bf16 gradients up to 1.4 times as far from the exact ones.  W and x are fp16
+// numbers times a power of two then (gdn_terms.hip), which holds bf16 numbers exactly.  The differences for dW carry the
+// token's cotangent relative to the largest; those for dx do not, since it can be applied to the sum.  With fp32 inputs every
+// operand is two fp16 terms (2^-22) and every product three; a difference's second term is stored times 2^11, so that small
+// probabilities keep their bits (2^-22 of them down to 2^-29, 2^-51 below; in one term 2^-11 and 2^-40).
+#include "gdn_common.h"
+#include "gdn_host.h"
+#include "gdn_product.h"
+#include "gdn_terms.h"
+#include "../../include/gdn_mi355x.h"
+
+namespace gdn {
+namespace ll {
+
+using namespace mm;
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int NT = 256;
+constexpr int64_t KEPT = 1 << 26;  // differences of a piece; statistics of the parts of the words
+constexpr int SHIFT = 15;          // differences are stored times 2^15
+constexpr int TOP = 14;            // largest magnitudes of scaled operands: [2^14, 2^15)
+
+enum : int { E_X = 0, E_W = 1, E_D = 2 };
+
+// ------------------------------------------------------------------------------------------------ forward
+
+struct StatArgs {
+    const int64_t *targets;
+    float2 *part;  // [parts][N]: maximum and sum of a part of the words
+    float *zt;     // [N] the target's logit
+    const int *exps;
+    int64_t N, V, v0;  // word of the operand's first row
+    int part0;
+};
+
+// Waves leave the statistics of their own words.
+template <class S, bool F16, bool SCALED>
+__global__ __launch_bounds__(S::NT, S::WAVES_EU) void stat_kernel(const Args g, const StatArgs a) {
+    __shared__ __attribute__((aligned(16))) char lds[S::LDS];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, wm = w / S::WN, wn = w % S::WN;
+    products<S, F16>(g, lds, [&](int tm, int tn, acc_t(&acc)[S::TM][S::TN]) {
+        const int64_t m0 = (int64_t)tm * S::BM + wm * (S::BM / S::WM);  // of the operand's rows
+        const int words = (int)min((int64_t)(S::BM / S::WM), g.a.rows - m0);
+        const int e = SCALED ? -(a.exps[E_X] + a.exps[E_W]) : 0;
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j) {
+            const int64_t n = (int64_t)tn * S::BN + wn * (S::BN / S::WN) + 32 * j + (lane & 31);
+            const bool live = n < a.N;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+                for (int q = 0; q < 16; ++q) {
+                    if constexpr (SCALED) acc[i][j][q] = ldexpf(acc[i][j][q], e);
+                    if (words < S::BM / S::WM && 32 * i + 8 * (q / 4) + 4 * (lane >> 5) + q % 4 >= words) acc[i][j][q] = -INFINITY;
+                    mx = fmaxf(mx, acc[i][j][q]);
+                }
+            mx = fmaxf(mx, lane_xor32(mx));
+            const float ref = mx == -INFINITY ? 0.f : mx;
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+                for (int q = 0; q < 16; ++q) s += __builtin_amdgcn_exp2f((acc[i][j][q] - ref) * LOG2E);
+            s += lane_xor32(s);
+            if (live && lane < 32) a.part[(int64_t)(a.part0 + tm * S::WM + wm) * a.N + n] = make_float2(mx, s);
+            const int64_t t = live ? a.targets[n] - a.v0 - m0 : -1;
+            const bool here = t >= 0 && t < words && ((t >> 2 & 1) == (lane >> 5));
+            if (__any(here)) {
+                const int tl = here ? (int)t - 4 * (lane >> 5) : -1;
+                float z = 0.f;
+#pragma unroll
+                for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+                    for (int q = 0; q < 16; ++q)
+                        if (tl == 32 * i + 8 * (q / 4) + q % 4) z = acc[i][j][q];
+                if (here) a.zt[n] = z;
+            }
+        }
+    });
+}
+
+// Joins a token's parts: 16 tokens to a workgroup, 16 threads to a token.
+__global__ __launch_bounds__(NT) void join_kernel(const int64_t *targets, const float2 *part, int parts, const float *zt,
+                                                  int64_t N, int64_t V, int64_t ignore, float *loss, float2 *stat) {
+    __shared__ float2 red[16][16];
+    const int tl = threadIdx.x & 15, p0 = threadIdx.x >> 4;
+    const int64_t n = block_index() * 16 + tl;
+    float m = -INFINITY, s = 0.f;
+    if (n < N) {
+#pragma unroll 8
+        for (int p = p0; p < parts; p += 16) {
+            const float2 o = part[(int64_t)p * N + n];
+            const float b = fmaxf(m, o.x), r = b == -INFINITY ? 0.f : b;
+            s = s * __builtin_amdgcn_exp2f((m - r) * LOG2E) + o.y * __builtin_amdgcn_exp2f((o.x - r) * LOG2E);
+            m = b;
+        }
+    }
+    red[p0][tl] = make_float2(m, s);
+    __syncthreads();
+    if (p0 || n >= N) return;
+    float M = -INFINITY;
+    for (int p = 0; p < 16; ++p) M = fmaxf(M, red[p][tl].x);
+    const float r = M == -INFINITY ? 0.f : M;
+    s = 0.f;
+    for (int p = 0; p < 16; ++p) s += red[p][tl].y * __builtin_amdgcn_exp2f((red[p][tl].x - r) * LOG2E);
+    const int64_t t = targets[n];
+    float l = logf(s) - (zt[n] - M);
+    if (t < 0 || t >= V) l = NAN;
+    if (t == ignore) l = 0.f;
+    loss[n] = l;
+    if (stat) stat[n] = make_float2(M, 1.f / s);
+}
+
+// The losses' sum, or mean over the tokens that count, and what a token's cotangent is multiplied by.
+__global__ __launch_bounds__(1024) void total_kernel(const float *loss, const int64_t *targets, int64_t N, int64_t ignore,
+                                                     int mean, float *total, float *factor) {
+    __shared__ double red[1024];
+    __shared__ int64_t count[1024];
+    double s = 0.;
+    int64_t c = 0;
+    for (int64_t i = threadIdx.x; i < N; i += 1024) {
+        s += (double)loss[i];
+        c += targets[i] != ignore;
+    }
+    red[threadIdx.x] = s;
+    count[threadIdx.x] = c;
+    __syncthreads();
+    for (int h = 512; h >= 1; h >>= 1) {
+        if ((int)threadIdx.x < h) {
+            red[threadIdx.x] += red[threadIdx.x + h];
+            count[threadIdx.x] += count[threadIdx.x + h];
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) {
+        const double n = mean ? (double)(count[0] > 0 ? count[0] : 1) : 1.;
+        total[0] = (float)(red[0] / n);
+        factor[0] = (float)(1. / n);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ backward
+
+// d[n] = the token's cotangent: 0 where it does not count, NaN where its target is no word.  part = partial maxima of |d|.
+__global__ __launch_bounds__(NT) void cotangent_kernel(const int64_t *targets, const float *dloss, int64_t stride,
+                                                       const float *factor, int64_t N, int64_t V, int64_t ignore, float *d,
+                                                       float *part) {
+    __shared__ float red[NT];
+    float m = 0.f;
+    for (int64_t n = (int64_t)blockIdx.x * NT + threadIdx.x; n < N; n += (int64_t)PARTS * NT) {
+        const int64_t t = targets[n];
+        float x = dloss[n * stride];
+        if (factor) x *= factor[0];
+        if (t < 0 || t >= V) x = NAN;
+        if (t == ignore) x = 0.f;
+        d[n] = x;
+        const float a = fabsf(x);
+        m = fmaxf(m, a <= 3.4028234e38f ? a : 0.f);
+    }
+    red[threadIdx.x] = m;
+    __syncthreads();
+    for (int h = NT / 2; h >= 1; h >>= 1) {
+        if ((int)threadIdx.x < h) red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + h]);
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) part[blockIdx.x] = red[0];
+}
+
+struct DiffArgs {
+    const int64_t *targets;
+    const float2 *stat;
+    const float *d;
+    const int *exps;  // with fp32 inputs also the logits' scale
+    uint16_t *p, *pt; // [N][terms * kp], [words][terms * np]; either may be NULL
+    int64_t N, v0, kp, np;
+};
+
+__device__ __forceinline__ uint32_t half_bits(float x) { return __half_as_ushort(__float2half(x)); }
+
+// The differences of a piece of words, 2^15 (p - [v = t]), and times d / (the power of two over the largest |d|) for dW.
+template <class S, bool F16, int TERMS, bool DX, bool DW>
+__global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, const DiffArgs a) {
+    __shared__ __attribute__((aligned(16))) char lds[S::LDS];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, wm = w / S::WN, wn = w % S::WN;
+    products<S, F16>(g, lds, [&](int tm, int tn, const acc_t(&acc)[S::TM][S::TN]) {
+        const int64_t m0 = (int64_t)tm * S::BM + wm * (S::BM / S::WM) + 4 * (lane >> 5);
+        const int64_t words = g.a.rows;
+        const int e = TERMS > 1 ? -(a.exps[E_X] + a.exps[E_W]) : 0;
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j) {
+            const int64_t n = (int64_t)tn * S::BN + wn * (S::BN / S::WN) + 32 * j + (lane & 31);
+            const bool live = n < a.N;
+            const float2 st = live ? a.stat[n] : make_float2(0.f, 0.f);
+            const float d = live ? a.d[n] : 0.f, r = DW ? ldexpf(d, a.exps[E_D]) : 0.f;
+            const float inv = st.y * (float)(1 << SHIFT);
+            const int64_t hot = live ? a.targets[n] - a.v0 - m0 : -1;
+#pragma unroll
+            for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int64_t m = m0 + 32 * i + 8 * q;
+                    float x[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        float z = acc[i][j][4 * q + k];
+                        if constexpr (TERMS > 1) z = ldexpf(z, e);
+                        x[k] = __builtin_amdgcn_exp2f((z - st.x) * LOG2E) * inv;
+                        if (hot == 32 * i + 8 * q + k) x[k] -= (float)(1 << SHIFT);
+                        if (m + k >= words) x[k] = 0.f;
+                    }
+                    if constexpr (DX) {
+                        if (live && m < a.kp) {
+                            uint16_t *to = a.p + n * (TERMS * a.kp) + m;
+                            float y[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                            for (int t = 0; t < TERMS; ++t) {
+                                uint32_t b[4];
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    b[k] = half_bits(y[k]);
+                                    y[k] = (y[k] - __half2float(__ushort_as_half((unsigned short)b[k]))) * (float)(1 << LOW);
+                                }
+                                *reinterpret_cast<uint2 *>(to + t * a.kp) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+                            }
+                        }
+                    }
+                    if constexpr (DW) {
+                        if (n < a.np) {
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                if (m + k >= words) continue;
+                                float y = r == 0.f ? 0.f : x[k] * r;
+                                uint16_t *to = a.pt + (m + k) * (TERMS * a.np) + n;
+#pragma unroll
+                                for (int t = 0; t < TERMS; ++t) {
+                                    const uint32_t b = half_bits(y);
+                                    to[t * a.np] = (uint16_t)b;
+                                    y = (y - __half2float(__ushort_as_half((unsigned short)b))) * (float)(1 << LOW);
+                                }
+                            }
+                        }
+                    }
+                }
+        }
+    });
+}
+
+// ------------------------------------------------------------------------------------------------ host
+
+// The segments of a product of operands with `terms` terms, kp elements each: all pairs but the least.  `across`: a has the
+// slots of terms_across and b's second term is stored times 2^LOW.
+static void segments(Args &g, int terms, int64_t kp, bool across) {
+    g.kit = (int)(kp / BK);
+    g.nseg = terms == 1 ? 1 : 3;
+    for (int s = 0; s < 3; ++s) g.a.off[s] = g.b.off[s] = 0;
+    if (terms > 1) {
+        g.a.off[1] = kp * 2;
+        g.b.off[2] = kp * 2;
+        if (across) g.a.off[2] = 2 * kp * 2;
+    }
+    g.a.ld = (across ? across_slots(terms) : terms) * kp * 2;
+    g.b.ld = terms * kp * 2;
+}
+
+struct Sizes {
+    int64_t N, H, V, hp, np, piece, pieces;  // hp, np: H and N in whole blocks; piece: words at a time
+    int terms;
+    bool direct_x, direct_w;  // the operand is used as it lies
+    int64_t parts, tokens;  // parts of the words with statistics of their own; tokens at a time in the forward pass
+    Plan px, pw;
+};
+
+static bool direct(const void *p, int64_t ld, int64_t H, int dt) {
+    return dt != GDN_F32 && H % BK == 0 && ld % 8 == 0 && aligned_to(p, 16) && pitch_fits(ld * 2);
+}
+
+static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt) {
+    Sizes s{};
+    s.N = N; s.H = H; s.V = V;
+    s.hp = padded(H);
+    s.np = padded(N);
+    s.terms = dt == GDN_F32 ? 2 : 1;
+    int64_t most = KEPT / s.np / 256 * 256;
+    if (most < 256) most = 256;
+    s.pieces = (V + most - 1) / most;
+    s.piece = ((V + s.pieces - 1) / s.pieces + 255) / 256 * 256;
+    s.pieces = (V + s.piece - 1) / s.piece;
+    s.parts = 2 * s.pieces * ((s.piece + 127) / 128);  // two waves to 128 words at most
+    s.tokens = KEPT / s.parts / 256 * 256;
+    if (s.tokens < 256) s.tokens = 256;
+    if (s.tokens > N) s.tokens = N;
+    const int64_t seg = s.terms == 1 ? 1 : 3;
+    const int64_t words = s.piece < V ? s.piece : V;
+    s.px = plan(N, H, seg * padded(words) / BK, 16);
+    s.pw = plan(words, H, seg * s.np / BK, 8);
+    return s;
+}
+
+struct Space {
+    char *base;
+    size_t at = 0;
+    template <class T>
+    T *take(int64_t n) {
+        T *p = base ? reinterpret_cast<T *>(base + at) : nullptr;
+        at += align_up256((size_t)n * sizeof(T));
+        return p;
+    }
+};
+
+struct Buffers {
+    uint16_t *x, *w, *wt, *xt, *p, *pt;
+    float *part, *zt, *d, *acc_x, *acc_w;
+    float2 *stats;
+    int *exps;
+};
+
+static Buffers place(Space &sp, const Sizes &s, bool dx, bool dw, bool bwd, bool copy_x, bool copy_w) {
+    Buffers b{};
+    const int t = s.terms;
+    const int64_t words = s.piece < s.V ? s.piece : s.V;
+    b.exps = sp.take<int>(4);
+    b.part = sp.take<float>(3 * PARTS);
+    if (copy_x) b.x = sp.take<uint16_t>(s.N * t * s.hp);
+    if (copy_w) b.w = sp.take<uint16_t>(words * t * s.hp);
+    if (!bwd) {
+        b.stats = sp.take<float2>(s.parts * s.tokens);
+        b.zt = sp.take<float>(s.tokens);
+        return b;
+    }
+    b.d = sp.take<float>(s.N);
+    if (dx) {
+        b.wt = sp.take<uint16_t>(s.H * across_slots(t) * padded(words));
+        b.p = sp.take<uint16_t>(s.N * t * padded(words));
+        b.acc_x = sp.take<float>((int64_t)s.px.splits * s.N * s.H);
+    }
+    if (dw) {
+        b.xt = sp.take<uint16_t>(s.H * across_slots(t) * s.np);
+        b.pt = sp.take<uint16_t>(words * t * s.np);
+        if (s.pw.splits > 1) b.acc_w = sp.take<float>((int64_t)s.pw.splits * words * s.H);
+    }
+    return b;
+}
+
+static int check(int64_t N, int64_t H, int64_t V, int64_t x_ld, int64_t w_ld, int dt) {
+    if (N < 0 || H <= 0 || V <= 0) return fail(GDN_ERR_INVALID, "N must be >= 0, H and V > 0");
+    if (dt != GDN_F32 && dt != GDN_BF16 && dt != GDN_F16) return fail(GDN_ERR_INVALID, "unknown dtype code");
+    if (N > 1 << 24 || V > 1 << 24 || H > 1 << 17)
+        return fail(GDN_ERR_UNSUPPORTED, "more than 2^24 tokens or words, or 2^17 channels are not supported");
+    if ((N > 1 && x_ld < H) || (V > 1 && w_ld < H)) return fail(GDN_ERR_INVALID, "rows overlap");
+    return GDN_OK;
+}
+
+template <class S, bool F16>
+static void launch_stat(Args &g, const StatArgs &a, bool scaled, hipStream_t st) {
+    const dim3 grid = tiles_of<S>(g, 1);
+    if (scaled) hipLaunchKernelGGL((stat_kernel<S, F16, true>), grid, dim3(S::NT), 0, st, g, a);
+    else hipLaunchKernelGGL((stat_kernel<S, F16, false>), grid, dim3(S::NT), 0, st, g, a);
+}
+
+template <class S, bool F16, int TERMS>
+static void launch_diff(Args &g, const DiffArgs &a, hipStream_t st) {
+    const dim3 grid = tiles_of<S>(g, 1);
+    if (a.p && a.pt) hipLaunchKernelGGL((diff_kernel<S, F16, TERMS, true, true>), grid, dim3(S::NT), 0, st, g, a);
+    else if (a.p) hipLaunchKernelGGL((diff_kernel<S, F16, TERMS, true, false>), grid, dim3(S::NT), 0, st, g, a);
+    else hipLaunchKernelGGL((diff_kernel<S, F16, TERMS, false, true>), grid, dim3(S::NT), 0, st, g, a);
+}
+
+// 16-bit inputs as they are, fp32 inputs as two fp16 terms.
+template <class S>
+static void launch_stat_of(Args &g, const StatArgs &a, int dt, hipStream_t st) {
+    if (dt == GDN_BF16) launch_stat<S, false>(g, a, false, st);
+    else launch_stat<S, true>(g, a, dt == GDN_F32, st);
+}
+template <class S>
+static void launch_diff_of(Args &g, const DiffArgs &a, int dt, hipStream_t st) {
+    if (dt == GDN_BF16) launch_diff<S, false, 1>(g, a, st);
+    else if (dt == GDN_F16) launch_diff<S, true, 1>(g, a, st);
+    else launch_diff<S, true, 2>(g, a, st);
+}
+
+#define GDN_BY_SHAPE(shape, call)              \
+    switch (shape) {                           \
+        case BIG: call(Big); break;            \
+        case MID: call(Mid); break;            \
+        case FEW: call(Few); break;            \
+        default: call(One); break;             \
+    }
+
+}  // namespace ll
+}  // namespace gdn
+
+using namespace gdn;
+using namespace gdn::ll;
+
+static size_t need(const Sizes &s, bool dx, bool dw, bool bwd, bool copy_x, bool copy_w) {
+    Space sp{nullptr};
+    place(sp, s, dx, dw, bwd, copy_x, copy_w);
+    return sp.at;
+}
+
+extern "C" size_t gdn_linear_loss_workspace_bytes(int64_t N, int64_t H, int64_t V, int dtype, int aligned, int want_dx,
+                                                  int want_dw) {
+    if (N <= 0 || H <= 0 || V <= 0 || N > 1 << 24 || V > 1 << 24 || H > 1 << 17) return 0;
+    const bool copy = !aligned || dtype == GDN_F32 || H % BK;
+    return need(sizes(N, H, V, dtype), want_dx, want_dw, want_dx || want_dw, copy, copy);
+}
+
+extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *targets, float *loss, float *stat, float *total,
+                                   float *factor, void *workspace, size_t workspace_bytes, int64_t N, int64_t H, int64_t V, int64_t x_stride,
+                                   int64_t w_stride, int64_t ignore_index, int reduction, int dtype, void *stream) {
+    clear_error();
+    if (const int rc = check(N, H, V, x_stride, w_stride, dtype)) return rc;
+    if (reduction < 0 || reduction > 2) return fail(GDN_ERR_INVALID, "unknown reduction");
+    if (reduction && (!total || !factor)) return fail(GDN_ERR_INVALID, "null pointer");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (N == 0 && !reduction) return GDN_OK;
+    if (N > 0) {
+        if (!x || !w || !targets || !loss || !workspace) return fail(GDN_ERR_INVALID, "null pointer");
+        const Sizes s = sizes(N, H, V, dtype);
+        const bool dx = direct(x, x_stride, H, dtype), dw = direct(w, w_stride, H, dtype);
+        const size_t bytes = need(s, false, false, false, !dx, !dw);
+        if (workspace_bytes < bytes)
+            return fail(GDN_ERR_WORKSPACE, "the workspace holds %zu bytes, %zu are needed", workspace_bytes, bytes);
+        Space sp{static_cast<char *>(workspace)};
+        const Buffers b = place(sp, s, false, false, false, !dx, !dw);
+        const bool f16 = dtype != GDN_BF16;
+        const int *exps = nullptr;
+        const Source sx{x, dtype, N, H, x_stride, targets, ignore_index}, sw{w, dtype, V, H, w_stride, nullptr, 0};
+        if (dtype == GDN_F32) {
+            maxima(sx, b.part + E_X * PARTS, st);
+            maxima(sw, b.part + E_W * PARTS, st);
+            exponents(b.part, 2, TOP, b.exps, st);
+            exps = b.exps;
+        }
+        if (!dx) terms(sx, s.terms, f16, exps, E_X, b.x, st);
+        // operands that are used as they lie need no pieces
+        const int64_t step = dw ? V : s.piece;
+        for (int64_t n0 = 0; n0 < N; n0 += s.tokens) {
+            const int64_t tokens = N - n0 < s.tokens ? N - n0 : s.tokens;
+            const int shape = plan(tokens, V, 1, 1).shape;
+            int parts = 0;
+            for (int64_t v0 = 0; v0 < V; v0 += step) {
+                const int64_t words = V - v0 < step ? V - v0 : step;
+                Args g{};
+                segments(g, s.terms, s.hp, false);
+                g.a.rows = words;
+                g.b.rows = tokens;
+                g.a.p = reinterpret_cast<const char *>(b.w);
+                g.b.p = reinterpret_cast<const char *>(b.x) + n0 * s.terms * s.hp * 2;
+                if (dw) {
+                    g.a.p = static_cast<const char *>(w);
+                    g.a.ld = w_stride * 2;
+                } else {
+                    Source part = sw;
+                    part.p = static_cast<const char *>(w) + v0 * w_stride * (dtype == GDN_F32 ? 4 : 2);
+                    part.rows = words;
+                    terms(part, s.terms, f16, exps, E_W, b.w, st);
+                }
+                if (dx) {
+                    g.b.p = static_cast<const char *>(x) + n0 * x_stride * 2;
+                    g.b.ld = x_stride * 2;
+                }
+                const StatArgs a{targets + n0, b.stats, b.zt, exps, tokens, V, v0, parts};
+                Timed tm("loss_stat", st);
+#define GDN_STAT(S)                                \
+    launch_stat_of<S>(g, a, dtype, st);            \
+    parts += g.mt * S::WM
+                GDN_BY_SHAPE(shape, GDN_STAT)
+#undef GDN_STAT
+            }
+            Timed tm("loss_join", st);
+            hipLaunchKernelGGL(join_kernel, grid_of((tokens + 15) / 16), dim3(NT), 0, st, targets + n0, b.stats, parts, b.zt,
+                               tokens, V, ignore_index, loss + n0, stat ? reinterpret_cast<float2 *>(stat) + n0 : nullptr);
+        }
+    }
+    if (reduction)
+        hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, st, loss, targets, N, ignore_index, reduction == 2, total,
+                           factor);
+    return check_launch(st, "gdn_linear_loss_fwd");
+}
+
+extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *targets, const float *stat, const float *dloss,
+                                   int64_t dloss_stride, const float *factor, void *dx, void *dw, void *workspace,
+                                   size_t workspace_bytes, int64_t N, int64_t H, int64_t V, int64_t x_stride, int64_t w_stride,
+                                   int64_t ignore_index, int dtype, void *stream) {
+    clear_error();
+    if (const int rc = check(N, H, V, x_stride, w_stride, dtype)) return rc;
+    if (dloss_stride < 0 || dloss_stride > 1) return fail(GDN_ERR_INVALID, "the cotangents' stride must be 0 or 1");
+    if (!dx && !dw) return GDN_OK;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (N == 0) return fail(GDN_ERR_INVALID, "no tokens: the gradients are zeros, which this call does not write");
+    if (!x || !w || !targets || !stat || !dloss || !workspace) return fail(GDN_ERR_INVALID, "null pointer");
+    const Sizes s = sizes(N, H, V, dtype);
+    const bool direct_x = direct(x, x_stride, H, dtype), direct_w = direct(w, w_stride, H, dtype);
+    const size_t bytes = need(s, dx, dw, true, !direct_x, !direct_w);
+    if (workspace_bytes < bytes)
+        return fail(GDN_ERR_WORKSPACE, "the workspace holds %zu bytes, %zu are needed", workspace_bytes, bytes);
+    Space sp{static_cast<char *>(workspace)};
+    const Buffers b = place(sp, s, dx, dw, true, !direct_x, !direct_w);
+    const bool f16 = dtype != GDN_BF16;
+    const int elem = dtype == GDN_F32 ? 4 : 2, t = s.terms;
+    const Source sx{x, dtype, N, H, x_stride, targets, ignore_index}, sw{w, dtype, V, H, w_stride, nullptr, 0};
+    hipLaunchKernelGGL(cotangent_kernel, dim3(PARTS), dim3(NT), 0, st, targets, dloss, dloss_stride, factor, N, V, ignore_index,
+                       b.d, b.part + E_D * PARTS);
+    maxima(sx, b.part + E_X * PARTS, st);
+    maxima(sw, b.part + E_W * PARTS, st);
+    exponents(b.part, 2, TOP, b.exps, st);
+    exponents(b.part + E_D * PARTS, 1, -1, b.exps + E_D, st);  // |d| below 1
+    const int *exps = dtype == GDN_F32 ? b.exps : nullptr;
+    if (!direct_x) terms(sx, t, f16, exps, E_X, b.x, st);
+    if (dw) terms_across(sx, t, true, b.exps, E_X, b.xt, st);
+    const int shape = plan(dw ? s.np : N, s.piece, 1, 1).shape;  // tiles that cover the columns that dW's product reads
+    for (int64_t v0 = 0; v0 < V; v0 += s.piece) {
+        const int64_t words = V - v0 < s.piece ? V - v0 : s.piece, kp = padded(words);
+        Source part = sw;
+        part.p = static_cast<const char *>(w) + v0 * w_stride * elem;
+        part.rows = words;
+        Args g{};
+        segments(g, t, s.hp, false);
+        g.a.rows = words;
+        g.b.rows = N;
+        g.a.p = reinterpret_cast<const char *>(b.w);
+        g.b.p = reinterpret_cast<const char *>(b.x);
+        if (direct_w) {
+            g.a.p = static_cast<const char *>(part.p);
+            g.a.ld = w_stride * 2;
+        } else {
+            terms(part, t, f16, exps, E_W, b.w, st);
+        }
+        if (direct_x) {
+            g.b.p = static_cast<const char *>(x);
+            g.b.ld = x_stride * 2;
+        }
+        const DiffArgs a{targets, reinterpret_cast<const float2 *>(stat), b.d, b.exps, b.p, b.pt, N, v0, kp, s.np};
+        {
+            Timed tm("loss_diff", st);
+#define GDN_DIFF(S) launch_diff_of<S>(g, a, dtype, st)
+            GDN_BY_SHAPE(shape, GDN_DIFF)
+#undef GDN_DIFF
+        }
+        if (dx) {
+            terms_across(part, t, true, b.exps, E_W, b.wt, st);
+            Args h{};
+            segments(h, t, kp, true);
+            h.a.p = reinterpret_cast<const char *>(b.wt);
+            h.a.rows = H;
+            h.b.p = reinterpret_cast<const char *>(b.p);
+            h.b.rows = N;
+            const Plan pl = s.px;  // parts without a block of the last piece add nothing
+            Result r{dx, H, dtype, b.d, b.exps, -SHIFT, {0, -1, 0}, nullptr, v0 > 0};
+            if (s.pieces > 1 || pl.splits > 1) r.acc = b.acc_x;
+            multiply(h, true, pl, r, st);
+            if (r.acc && v0 + words == V) finish(r, pl.splits, N, H, st);
+        }
+        if (dw) {
+            Args h{};
+            segments(h, t, s.np, true);
+            h.a.p = reinterpret_cast<const char *>(b.xt);
+            h.a.rows = H;
+            h.b.p = reinterpret_cast<const char *>(b.pt);
+            h.b.rows = words;
+            Result r{static_cast<char *>(dw) + v0 * H * elem, H, dtype, nullptr, b.exps, -SHIFT, {-1, 0, -1}, nullptr, 0};
+            if (s.pw.splits > 1) r.acc = b.acc_w;
+            multiply(h, true, s.pw, r, st);
+            if (r.acc) finish(r, s.pw.splits, words, H, st);
+        }
+    }
+    return check_launch(st, "gdn_linear_loss_bwd");
+}

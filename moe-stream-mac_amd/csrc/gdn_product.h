@@ -1,0 +1,367 @@
+// The matrix product of the operators that are not bound by memory: C[n][m] = sum_k B[n][k] A[m][k] with 16-bit operands
+// that both lie along the contraction, 32-bit sums on the matrix cores, for gfx950.
+//
+// Operands in one order only: whoever has another order, type or an odd size lays its operand out in a pass of its own
+// (gdn_terms.h), which costs a percent or two of a large product and leaves one loop to make fast.  fp32 operands become
+// sums of 16-bit terms, side by side along the contraction; the product then walks pairs of terms ("segments").
+//
+// A workgroup forms a BM x BN tile, BK = 64 at a time: rows of 128 bytes go from memory to LDS without passing through
+// registers, two stages deep.  Chunk c of 16 bytes of row r lies in place c ^ (r / 2 & 7): sixteen rows of one chunk, which an
+// LDS read serves at once, fill all 64 banks (with r & 7 half of the read cycles were conflicts).  The global addresses are
+// permuted to that end, since LDS is filled in order.
+//
+// The barrier of a stage stands before its last quarter: by then that quarter's fragments are in registers, so after it
+// the stage's LDS may be overwritten and the next stage's first fragments are read under the last quarter's products.
+// Loads thus have three quarters of a stage to arrive, and no product waits for LDS.
+//
+// Lanes hold the columns of an MFMA's result and registers its rows: A's rows (m) run over registers, B's (n) over lanes.
+// Sums over m, such as those of a softmax over words, stay within a lane and its partner 32 lanes on.
+#pragma once
+
+#include "gdn_common.h"
+#include "gdn_host.h"
+#include "gdn_vec.h"
+
+namespace gdn {
+namespace mm {
+
+typedef float acc_t __attribute__((ext_vector_type(16)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 hf8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+constexpr int BK = 64;
+
+template <bool F16>
+__device__ __forceinline__ acc_t mfma(u4 a, u4 b, acc_t c) {
+    if constexpr (F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(hf8, a), __builtin_bit_cast(hf8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+}
+
+// A matrix of `rows` rows, `ld` bytes apart, of `off[s]` bytes to the term that segment s takes.
+struct Operand {
+    const char *p;
+    int64_t ld, rows;
+    int64_t off[3];
+};
+struct Args {
+    Operand a, b;
+    int kit;     // BK-blocks of a term
+    int nseg;    // 1 to 3
+    int splits;  // the nseg * kit blocks in this many parts (grid.z)
+    int mt, nt;  // tiles
+};
+
+// BM x BN tile of WM x WN waves.
+template <int BM_, int BN_, int WM_, int WN_, int PER_CU_>
+struct Shape {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NT = 64 * WM_ * WN_;
+    static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
+    static constexpr int A_BYTES = BM * BK * 2, STAGE = (BM + BN) * BK * 2, LDS = 2 * STAGE;
+    static constexpr int RA = BM * 8 / NT, RB = BN * 8 / NT;  // 16-byte loads of a thread for a stage
+    static constexpr int PER_CU = PER_CU_;
+    static constexpr int WAVES_EU = PER_CU_ * NT / 256;
+    static_assert(RA >= 1 && RB >= 1 && TM % 2 == 0 && TN >= 1, "tile");
+};
+typedef Shape<256, 256, 2, 4, 1> Big;
+typedef Shape<128, 128, 2, 2, 2> Mid;
+typedef Shape<128, 64, 2, 2, 3> Few;
+typedef Shape<128, 32, 2, 1, 4> One;
+
+typedef __attribute__((address_space(1))) const void gvoid;
+typedef __attribute__((address_space(3))) void lvoid;
+
+// Tile of a workgroup.  Workgroups go round the 8 XCDs in turn: each XCD takes a run of tiles of its own, and a run walks
+// groups of 8 tiles along m, so that the tiles under way on an XCD share rows of both operands in its L2.
+__device__ __forceinline__ void tile_of(int id, int mt, int nt, int &tm, int &tn) {
+    const int total = mt * nt, xcd = id & 7, in = id >> 3;
+    const int q = total >> 3, rest = total & 7;
+    const int t = xcd * q + min(xcd, rest) + in;
+    const int per = 8 * nt, g = t / per, first = g * 8, width = min(8, mt - first), r = t - g * per;
+    tm = first + r % width;
+    tn = r / width;
+}
+
+// A workgroup's walk over its tiles and their blocks: tiles blockIdx.x, blockIdx.x + gridDim.x, ..., each from block `first`
+// to `end`.  It runs two blocks ahead of the products, over the border between two tiles too, so that the next tile's first
+// loads are under way while results are written.
+template <class S>
+struct Loader {
+    const char *pa, *pb;  // of the block to load next
+    uint32_t va, vb, na, nb;  // this thread's offset in a tile, and the bytes that loads may reach: none behind the last row
+    uint32_t step_a, step_b;  // from one load's rows to the next one's
+    int left, seg_left, seg, tile, tiles, w;  // blocks left of the tile and of the segment
+
+    __device__ __forceinline__ void start(const Args &g, int first, int end) {  // of a tile
+        int tm, tn;
+        tile_of(tile, g.mt, g.nt, tm, tn);
+        const int lane = threadIdx.x & 63, r0 = (threadIdx.x >> 3);
+        const uint32_t chunk = ((lane & 7) ^ (r0 >> 1 & 7)) << 4;
+        const int ma = (int)min((int64_t)S::BM, g.a.rows - (int64_t)tm * S::BM);
+        const int mb = (int)min((int64_t)S::BN, g.b.rows - (int64_t)tn * S::BN);
+        va = (uint32_t)r0 * (uint32_t)g.a.ld + chunk;
+        vb = (uint32_t)r0 * (uint32_t)g.b.ld + chunk;
+        na = (uint32_t)(ma - 1) * (uint32_t)g.a.ld + BK * 2;
+        nb = (uint32_t)(mb - 1) * (uint32_t)g.b.ld + BK * 2;
+        step_a = (uint32_t)(S::NT / 8) * (uint32_t)g.a.ld;
+        step_b = (uint32_t)(S::NT / 8) * (uint32_t)g.b.ld;
+        left = end - first;
+        seg = first / g.kit;
+        const int kk = first - seg * g.kit;
+        seg_left = g.kit - kk;
+        pa = g.a.p + (int64_t)tm * S::BM * g.a.ld + g.a.off[seg] + (int64_t)kk * (BK * 2);
+        pb = g.b.p + (int64_t)tn * S::BN * g.b.ld + g.b.off[seg] + (int64_t)kk * (BK * 2);
+    }
+    // Loads [R0, R1) of a block's RA + RB.  Rows behind the last read as zeros.
+    template <int R0, int R1>
+    __device__ __forceinline__ void load(char *__restrict__ dst) const {
+#ifdef __HIP_DEVICE_COMPILE__  // the host's pass does not know buffer resources
+        constexpr int RAW = 0x00020000;
+        const auto a = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(pa), 0, na, RAW);
+        const auto b = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(pb), 0, nb, RAW);
+#pragma unroll
+        for (int r = R0; r < R1; ++r) {
+            lvoid *to = (lvoid *)(dst + r * (S::NT * 16) + w * 1024);
+            if (r < S::RA)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(a, to, 16, va + r * step_a, 0, 0, 0);
+            else
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(b, to, 16, vb + (r - S::RA) * step_b, 0, 0, 0);
+        }
+#endif
+    }
+    // On to the next block; after the very last one it stays there, so that loads need no branch around them.
+    __device__ __forceinline__ void next(const Args &g, int first, int end) {
+        if (left > 1) {
+            pa += BK * 2;
+            pb += BK * 2;
+            --left;
+            if (--seg_left == 0) {
+                seg_left = g.kit;
+                pa += g.a.off[seg + 1] - g.a.off[seg] - (int64_t)g.kit * (BK * 2);
+                pb += g.b.off[seg + 1] - g.b.off[seg] - (int64_t)g.kit * (BK * 2);
+                ++seg;
+            }
+        } else if (tile + (int)gridDim.x < tiles) {
+            tile += gridDim.x;
+            start(g, first, end);
+        }
+    }
+};
+
+// Every load into LDS has landed and every fragment read has returned, of all waves.
+__device__ __forceinline__ void stage_barrier() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// The fragments of a block: four steps of 16 along the contraction; A's rows in two halves.
+template <class S>
+struct Frags {
+    static constexpr int H = S::TM / 2;
+    u4 lo[4][H], hi[4][H], b[4][S::TN];
+    __device__ __forceinline__ void read_lo(const char *__restrict__ lds, const uint32_t (&at_a)[4], int k) {
+#pragma unroll
+        for (int i = 0; i < H; ++i) lo[k][i] = *reinterpret_cast<const u4 *>(lds + at_a[k] + i * 32 * BK * 2);
+    }
+    __device__ __forceinline__ void read_hi(const char *__restrict__ lds, const uint32_t (&at_a)[4], int k) {
+#pragma unroll
+        for (int i = 0; i < H; ++i) hi[k][i] = *reinterpret_cast<const u4 *>(lds + at_a[k] + (H + i) * 32 * BK * 2);
+    }
+    __device__ __forceinline__ void read_b(const char *__restrict__ lds, const uint32_t (&at_b)[4], int k) {
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j) b[k][j] = *reinterpret_cast<const u4 *>(lds + at_b[k] + j * 32 * BK * 2);
+    }
+    template <bool F16>
+    __device__ __forceinline__ void mul_lo(acc_t (&acc)[S::TM][S::TN], int k) const {
+#pragma unroll
+        for (int i = 0; i < H; ++i)
+#pragma unroll
+            for (int j = 0; j < S::TN; ++j) acc[i][j] = mfma<F16>(lo[k][i], b[k][j], acc[i][j]);
+    }
+    template <bool F16>
+    __device__ __forceinline__ void mul_hi(acc_t (&acc)[S::TM][S::TN], int k) const {
+#pragma unroll
+        for (int i = 0; i < H; ++i)
+#pragma unroll
+            for (int j = 0; j < S::TN; ++j) acc[H + i][j] = mfma<F16>(hi[k][i], b[k][j], acc[H + i][j]);
+    }
+};
+
+// One step's products with LOADS loads and READS reads from LDS between them.
+template <class S, int LOADS, int READS>
+__device__ __forceinline__ void interleave() {
+    constexpr int PRODUCTS = Frags<S>::H * S::TN, L = (LOADS + PRODUCTS - 1) / PRODUCTS, R = (READS + PRODUCTS - 1) / PRODUCTS;
+#pragma unroll
+    for (int i = 0; i < PRODUCTS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x020, L, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// First half of a block: the products of A's lower rows, while the rest of the block's fragments are read.
+template <class S, bool F16>
+__device__ __forceinline__ void first_half(const char *__restrict__ rd, const uint32_t (&at_a)[4], const uint32_t (&at_b)[4],
+                                           Frags<S> &f, acc_t (&acc)[S::TM][S::TN]) {
+    f.template mul_lo<F16>(acc, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    f.read_b(rd, at_b, 3);
+    f.read_hi(rd, at_a, 0);
+    f.read_hi(rd, at_a, 1);
+    f.read_hi(rd, at_a, 2);
+    f.read_hi(rd, at_a, 3);
+    f.template mul_lo<F16>(acc, 1);
+    f.template mul_lo<F16>(acc, 2);
+    constexpr int READS = S::TN + 4 * Frags<S>::H, PRODUCTS = Frags<S>::H * S::TN;
+#pragma unroll
+    for (int i = 0; i < (READS + 1) / 2; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, 2 * PRODUCTS, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    f.template mul_lo<F16>(acc, 3);
+}
+
+// Second half: the products of A's upper rows, while the block after the next is loaded into this one's LDS and the
+// next one's fragments are read in the place of those that no product needs any more.  A load takes the memory pipe 16
+// cycles for each of the workgroup's waves, so loads stand between products: in one run they held the products up.
+template <class S, bool F16>
+__device__ __forceinline__ void second_half(const char *__restrict__ rd, char *__restrict__ wr, const Loader<S> &ld,
+                                            const uint32_t (&at_a)[4], const uint32_t (&at_b)[4], Frags<S> &f,
+                                            acc_t (&acc)[S::TM][S::TN]) {
+    constexpr int R = S::RA + S::RB;
+    ld.template load<0, R / 4>(wr);
+    f.template mul_hi<F16>(acc, 0);
+    f.read_lo(rd, at_a, 0);
+    f.read_lo(rd, at_a, 3);
+    interleave<S, R / 4, 2 * Frags<S>::H>();
+    ld.template load<R / 4, R / 2>(wr);
+    f.template mul_hi<F16>(acc, 1);
+    f.read_b(rd, at_b, 0);
+    f.read_lo(rd, at_a, 1);
+    interleave<S, R / 2 - R / 4, Frags<S>::H + S::TN>();
+    ld.template load<R / 2, 3 * R / 4>(wr);
+    f.template mul_hi<F16>(acc, 2);
+    f.read_b(rd, at_b, 1);
+    f.read_lo(rd, at_a, 2);
+    interleave<S, 3 * R / 4 - R / 2, Frags<S>::H + S::TN>();
+    ld.template load<3 * R / 4, R>(wr);
+    f.template mul_hi<F16>(acc, 3);
+    f.read_b(rd, at_b, 2);
+    interleave<S, R - 3 * R / 4, S::TN>();
+}
+
+// Forms the workgroup's tiles and hands each to epilogue(tm, tn, acc).
+// acc[i][j]: rows m = 32 i + 8 (q / 4) + 4 (lane / 32) + q % 4 of this wave's part for register q, column n = 32 j + lane % 32.
+template <class S, bool F16, class E>
+__device__ __forceinline__ void products(const Args &g, char *lds, E &&epilogue) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, wm = w / S::WN, wn = w % S::WN;
+    const int total = g.kit * g.nseg;
+    const int first = (int)((int64_t)total * blockIdx.z / g.splits), end = (int)((int64_t)total * (blockIdx.z + 1) / g.splits);
+    const int blocks = end - first, mt = g.mt, nt = g.nt;
+    Loader<S> ld;
+    ld.tile = blockIdx.x;
+    ld.tiles = mt * nt;
+    ld.w = __builtin_amdgcn_readfirstlane(w);
+    if (ld.tile >= ld.tiles || blocks == 0) return;
+    ld.start(g, first, end);
+    uint32_t at_a[4], at_b[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t c = ((k * 2 + (lane >> 5)) ^ (lane >> 1 & 7)) << 4;
+        at_a[k] = (wm * (S::BM / S::WM) + (lane & 31)) * BK * 2 + c;
+        at_b[k] = S::A_BYTES + (wn * (S::BN / S::WN) + (lane & 31)) * BK * 2 + c;
+    }
+    char *cur = lds, *other = lds + S::STAGE;
+    ld.template load<0, S::RA + S::RB>(cur);
+    ld.next(g, first, end);
+    stage_barrier();
+    ld.template load<0, S::RA + S::RB>(other);
+    ld.next(g, first, end);
+    for (int t = blockIdx.x; t < mt * nt; t += gridDim.x) {
+        acc_t acc[S::TM][S::TN];
+#pragma unroll
+        for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+            for (int j = 0; j < S::TN; ++j)
+#pragma unroll
+                for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
+        // read anew for each tile, so that their registers are free while results are written
+        Frags<S> f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            f.read_lo(cur, at_a, k);
+            if (k < 3) f.read_b(cur, at_b, k);
+        }
+        for (int n = 0; n < blocks; ++n) {
+            first_half<S, F16>(cur, at_a, at_b, f, acc);
+            stage_barrier();
+            // after a tile's last block no product uses what this reads
+            second_half<S, F16>(other, cur, ld, at_a, at_b, f, acc);
+            ld.next(g, first, end);
+            char *x = cur;
+            cur = other;
+            other = x;
+        }
+        int tm, tn;
+        tile_of(t, mt, nt, tm, tn);
+        epilogue(tm, tn, acc);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): no load into this LDS outlives the workgroup
+}
+
+// Whether a product takes operands with this row pitch: offsets within a tile stay below 2^31.
+inline bool pitch_fits(int64_t ld_bytes) { return ld_bytes > 0 && ld_bytes <= (1 << 22); }
+
+// What becomes of a product: C[n][m] -> 2^e row[n] C[n][m], rounded to dt, y rows ldy elements apart.  e = base + sum of
+// sign[i] exps[i]; a row factor of 0 makes zeros of whatever the row holds.  With acc (fp32 [splits][rows][cols]) the parts
+// of a split contraction go there as they are, added to what is there with `add`; finish() turns them into y.
+struct Result {
+    void *y;
+    int64_t ldy;
+    int dt;
+    const float *row;
+    const int *exps;
+    int base, sign[3];
+    float *acc;
+    int add;
+};
+
+enum : int { BIG = 0, MID = 1, FEW = 2, ONE = 3 };
+struct Plan {
+    int shape, splits;
+};
+// The tile and the split of the contraction (at most max_splits) for rows x cols results of `blocks` BK-blocks.
+Plan plan(int64_t rows, int64_t cols, int64_t blocks, int max_splits);
+
+// Fills in the tiles of g and the grid of a launch.
+template <class S>
+inline dim3 tiles_of(Args &g, int splits) {
+    g.mt = (int)((g.a.rows + S::BM - 1) / S::BM);
+    g.nt = (int)((g.b.rows + S::BN - 1) / S::BN);
+    g.splits = splits;
+    const int64_t tiles = (int64_t)g.mt * g.nt;
+    int64_t most = 256 * S::PER_CU / splits / 8 * 8;  // whole rounds of the XCDs
+    if (most < 8) most = 8;
+    return dim3((unsigned)(tiles < most ? tiles : most), 1, (unsigned)splits);
+}
+
+void multiply(Args g, bool f16, const Plan &p, const Result &r, hipStream_t st);
+void finish(const Result &r, int splits, int64_t rows, int64_t cols, hipStream_t st);
+
+__device__ __forceinline__ int exponent_of(const Result &r) {
+    int e = r.base;
+    if (r.exps) e += r.sign[0] * r.exps[0] + r.sign[1] * r.exps[1] + r.sign[2] * r.exps[2];
+    return e;
+}
+
+}  // namespace mm
+}  // namespace gdn

@@ -1,0 +1,41 @@
+// Operands of the matrix products (gdn_product.h) in the order and type that these take: 16-bit terms along the contraction.
+#pragma once
+
+#include "gdn_host.h"
+
+namespace gdn {
+namespace mm {
+
+// A matrix as the caller has it: rows of `cols` elements of type dt, ld elements apart.  With targets, rows whose target is
+// `ignore` count as zeros, whatever they hold.
+struct Source {
+    const void *p;
+    int dt;
+    int64_t rows, cols, ld;
+    const int64_t *targets;
+    int64_t ignore;
+};
+
+constexpr int PARTS = 256;  // partial maxima of one matrix
+
+// Elements of a row of `cols`, filled up to whole blocks of the contraction.
+inline int64_t padded(int64_t cols) { return (cols + 63) / 64 * 64; }
+
+// part[PARTS] = partial maxima of the finite magnitudes of s (of v[n] where targets[n] != ignore for maxima_of).
+void maxima(const Source &s, float *part, hipStream_t st);
+
+// exps[i] = the exponent e_i that takes the largest of part[i][PARTS] to [2^top, 2^(top + 1)), for i < n; 0 for zeros.
+void exponents(const float *part, int n, int top, int *exps, hipStream_t st);
+
+// dst[r][t * padded(cols) + c] = term t of 2^e s[r][c], e = exps[which] (0 without exps), zeros behind the last column: x is
+// the sum of its terms up to the last one's rounding.  f16 or bf16 terms.
+void terms(const Source &s, int nterms, bool f16, const int *exps, int which, void *dst, hipStream_t st);
+
+// The same transposed: dst[c][t * padded(rows) + r].  Of two terms there is a third slot with the first one times 2^-LOW, the
+// partner of a second term that is stored times 2^LOW.
+constexpr int LOW = 11;
+inline int across_slots(int nterms) { return nterms == 2 ? 3 : 1; }
+void terms_across(const Source &s, int nterms, bool f16, const int *exps, int which, void *dst, hipStream_t st);
+
+}  // namespace mm
+}  // namespace gdn

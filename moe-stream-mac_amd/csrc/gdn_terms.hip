@@ -1,0 +1,191 @@
+// Operands of the matrix products laid out in 16-bit terms along the contraction, straight or transposed, for gfx950.
+//
+// A number of more bits than a 16-bit type holds is a sum of terms, each the rounding of what the earlier ones leave:
+// fp32 = 2 fp16 terms up to 2^-22 of it (or 3 bf16 terms, 2^-24).  fp16 has 5 bits of exponent, so a whole matrix is first
+// multiplied by the power of two that takes its largest magnitude to 2^14: a bf16 number (8 bits) is then exact down to
+// 2^-32 of the largest, and what is smaller is off by 2^-40 of it at most.
+#include "gdn_common.h"
+#include "gdn_terms.h"
+#include "gdn_vec.h"
+
+namespace gdn {
+namespace mm {
+
+constexpr int NT = 256;
+
+__device__ __forceinline__ bool skipped(const Source &s, int64_t r) { return s.targets && s.targets[r] == s.ignore; }
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) x = fmaxf(x, __shfl_xor(x, o));
+    return x;
+}
+
+__device__ __forceinline__ float magnitude(float x) {
+    const float a = fabsf(x);
+    return a <= 3.4028234e38f ? a : 0.f;  // neither infinite nor NaN
+}
+
+template <int V>
+__global__ __launch_bounds__(NT) void maxima_kernel(const Source s, float *part) {
+    __shared__ float red[NT / 64];
+    const int64_t per = (s.cols + V - 1) / V, total = s.rows * per;
+    float m = 0.f;
+    for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < total; i += (int64_t)PARTS * NT) {
+        const int64_t r = i / per, c = (i - r * per) * V;
+        if (skipped(s, r)) continue;
+        float x[V];
+        ops::loadv<V>(s.p, r * s.ld + c, s.dt, x);
+#pragma unroll
+        for (int j = 0; j < V; ++j) m = fmaxf(m, magnitude(x[j]));
+    }
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+__global__ __launch_bounds__(64) void exponents_kernel(const float *part, int top, int *exps) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < PARTS / 64; ++i) m = fmaxf(m, part[blockIdx.x * PARTS + i * 64 + threadIdx.x]);
+    m = wave_max(m);
+    if (threadIdx.x == 0) {
+        int e = 0;
+        if (m > 0.f) (void)frexpf(m, &e);  // m in [2^(e - 1), 2^e)
+        exps[blockIdx.x] = m > 0.f ? top + 1 - e : 0;
+    }
+}
+
+// Term `t` of y: what the terms before it leave, rounded; an infinite or NaN number is its first term.
+template <bool F16>
+__device__ __forceinline__ uint16_t next_term(float &y) {
+    uint16_t b;
+    float back;
+    if constexpr (F16) {
+        const __half h = __float2half(y);
+        b = __half_as_ushort(h);
+        back = __half2float(h);
+    } else {
+        b = f32_to_bf16_cvt(y);
+        back = bf16_to_f32(b);
+    }
+    y = fabsf(back) <= 3.4028234e38f ? y - back : 0.f;
+    return b;
+}
+
+__device__ __forceinline__ uint4 pack8(const uint16_t (&b)[8]) {
+    return make_uint4(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16, b[4] | (uint32_t)b[5] << 16,
+                      b[6] | (uint32_t)b[7] << 16);
+}
+
+// Eight elements of a row to a thread.
+template <bool F16, bool WIDE>
+__global__ __launch_bounds__(NT) void terms_kernel(const Source s, int nterms, const int *exps, int which, uint16_t *dst,
+                                                   int64_t kp) {
+    const int64_t i = block_index() * NT + threadIdx.x, per = kp / 8, r = i / per, c = (i - r * per) * 8;
+    if (r >= s.rows) return;
+    const int e = exps ? exps[which] : 0;
+    float x[8];
+    const bool none = skipped(s, r);
+    if (WIDE && c + 8 <= s.cols) {
+        ops::loadv<8>(s.p, r * s.ld + c, s.dt, x);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = c + j < s.cols ? load_as_f32(s.p, r * s.ld + c + j, s.dt) : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = none ? 0.f : ldexpf(x[j], e);
+    for (int t = 0; t < nterms; ++t) {
+        uint16_t b[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b[j] = next_term<F16>(x[j]);
+        *reinterpret_cast<uint4 *>(dst + r * (kp * nterms) + t * kp + c) = pack8(b);
+    }
+}
+
+// 64 x 64 elements to a workgroup, turned over in LDS.
+template <bool F16, bool WIDE>
+__global__ __launch_bounds__(NT) void across_kernel(const Source s, int slots, const int *exps, int which, uint16_t *dst,
+                                                    int64_t kp, int64_t tiles_c, int64_t tiles) {
+    __shared__ float tile[64][65];
+    const int64_t t0 = block_index();
+    if (t0 >= tiles) return;
+    const int64_t r0 = t0 / tiles_c * 64, c0 = t0 % tiles_c * 64;
+    const int e = exps ? exps[which] : 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int rl = h * 32 + threadIdx.x / 8, cl = threadIdx.x % 8 * 8;
+        const int64_t r = r0 + rl, c = c0 + cl;
+        float x[8];
+        const bool live = r < s.rows && !skipped(s, r);
+        if (WIDE && live && c + 8 <= s.cols) {
+            ops::loadv<8>(s.p, r * s.ld + c, s.dt, x);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = live && c + j < s.cols ? load_as_f32(s.p, r * s.ld + c + j, s.dt) : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) tile[rl][cl + j] = ldexpf(x[j], e);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int cl = h * 32 + threadIdx.x / 8, rl = threadIdx.x % 8 * 8;
+        if (c0 + cl >= s.cols) continue;
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = tile[rl + j][cl];
+        uint16_t *to = dst + (c0 + cl) * (kp * slots) + r0 + rl;
+        for (int t = 0; t < slots; ++t) {
+            uint16_t b[8];
+            if (t == 2) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[j] = ldexpf(tile[rl + j][cl], -LOW);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) b[j] = next_term<F16>(x[j]);
+            *reinterpret_cast<uint4 *>(to + t * kp) = pack8(b);
+        }
+    }
+}
+
+static bool wide(const Source &s) { return s.ld % 8 == 0 && aligned_to(s.p, 16); }
+
+void maxima(const Source &s, float *part, hipStream_t st) {
+    Timed tm("maxima", st);
+    if (wide(s) && s.cols % 8 == 0)
+        hipLaunchKernelGGL((maxima_kernel<8>), dim3(PARTS), dim3(NT), 0, st, s, part);
+    else
+        hipLaunchKernelGGL((maxima_kernel<1>), dim3(PARTS), dim3(NT), 0, st, s, part);
+}
+
+void exponents(const float *part, int n, int top, int *exps, hipStream_t st) {
+    hipLaunchKernelGGL(exponents_kernel, dim3(n), dim3(64), 0, st, part, top, exps);
+}
+
+#define GDN_TERMS(KERNEL, ...)                                                                                        \
+    if (f16 && w) hipLaunchKernelGGL((KERNEL<true, true>), grid, dim3(NT), 0, st, __VA_ARGS__);                        \
+    else if (f16) hipLaunchKernelGGL((KERNEL<true, false>), grid, dim3(NT), 0, st, __VA_ARGS__);                       \
+    else if (w) hipLaunchKernelGGL((KERNEL<false, true>), grid, dim3(NT), 0, st, __VA_ARGS__);                         \
+    else hipLaunchKernelGGL((KERNEL<false, false>), grid, dim3(NT), 0, st, __VA_ARGS__)
+
+void terms(const Source &s, int nterms, bool f16, const int *exps, int which, void *dst, hipStream_t st) {
+    Timed tm("terms", st);
+    const int64_t kp = padded(s.cols);
+    const bool w = wide(s);
+    const dim3 grid = grid_of((s.rows * (kp / 8) + NT - 1) / NT);
+    GDN_TERMS(terms_kernel, s, nterms, exps, which, static_cast<uint16_t *>(dst), kp);
+}
+
+void terms_across(const Source &s, int nterms, bool f16, const int *exps, int which, void *dst, hipStream_t st) {
+    Timed tm("terms_across", st);
+    const int64_t kp = padded(s.rows), tc = (s.cols + 63) / 64, tiles = kp / 64 * tc;
+    const bool w = wide(s);
+    const dim3 grid = grid_of(tiles);
+    GDN_TERMS(across_kernel, s, across_slots(nterms), exps, which, static_cast<uint16_t *>(dst), kp, tc, tiles);
+}
+#undef GDN_TERMS
+
+}  // namespace mm
+}  // namespace gdn

@@ -59,6 +59,12 @@ _SIGS = {
     "gdn_linatt_fwd": ([_vp] * 8 + [_sz, _vp] + [_i] * 6 + [_f, _i, _i, _vp], _i),
     "gdn_linatt_bwd": ([_vp] * 7 + [_sz] + [_vp] * 8 + [_sz, _vp] + [_i] * 6 + [_f, _i, _i, _i, _vp], _i),
     "gdn_linatt_step": ([_vp] * 6 + [_i64, _i64] + [_i] * 5 + [_f, _i, _i, _vp], _i),
+    "gdn_linear_loss_workspace_bytes": ([_i64] * 3 + [_i] * 4, _sz),
+    "gdn_linear_loss_fwd": ([_vp] * 8 + [_sz] + [_i64] * 6 + [_i, _i, _vp], _i),
+    "gdn_linear_loss_bwd": ([_vp] * 5 + [_i64] + [_vp] * 4 + [_sz] + [_i64] * 6 + [_i, _vp], _i),
+    "gdn_embedding_fwd": ([_vp] * 3 + [_i64] * 4 + [_d, _i, _vp], _i),
+    "gdn_embedding_bwd_workspace_bytes": ([_i64] * 3, _sz),
+    "gdn_embedding_bwd": ([_vp] * 4 + [_sz] + [_i64] * 5 + [_d, _i, _vp], _i),
     "gdn_version": ([], _i),
     "gdn_last_error": ([], ctypes.c_char_p),
     "gdn_num_snapshots": ([_i, _i], ctypes.c_int64),
