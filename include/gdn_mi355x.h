@@ -364,7 +364,7 @@ int gdn_clip_grad_norm(const void *const *x, void *const *y, const int64_t *nume
  *
  * gdn_linear_loss_bwd: dx [N][H] and dw [V][H], contiguous (dtype; either may be NULL), from the cotangents dloss (fp32;
  * dloss_stride 1: one for each token, 0: one for all), times factor [0] (NULL for 1); dx is 0 at ignored tokens.
- * N, V <= 2^24, H <= 2^17.  The workspace of the forward pass: want_dx = want_dw = 0.  aligned: both operands lie on 16 bytes,
+ * N <= 2^20, V <= 2^24, H <= 2^17.  The workspace of the forward pass: want_dx = want_dw = 0.  aligned: both operands lie on 16 bytes,
  * with rows a multiple of 16 bytes apart; without it there is room for copies of them. */
 size_t gdn_linear_loss_workspace_bytes(int64_t N, int64_t H, int64_t V, int dtype, int aligned, int want_dx, int want_dw);
 int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *targets, float *loss, float *stat, float *total,
@@ -384,6 +384,25 @@ int gdn_embedding_fwd(const int64_t *ids, const void *w, void *y, int64_t N, int
 size_t gdn_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t H);
 int gdn_embedding_bwd(const int64_t *ids, const void *dy, void *dw, void *workspace, size_t workspace_bytes, int64_t N,
                       int64_t V, int64_t H, int64_t dy_stride, int64_t padding_idx, double scale, int dtype, void *stream);
+
+/* Weights in microscaled 4-bit floating point (MXFP4).  w [N][K] is cut along K into blocks of 32 (K filled up with zeros):
+ * codes [N][ceil(K / 32) * 16], on 16 bytes: two elements to a byte, the even one low, each a sign and one of 0, 0.5, 1, 1.5, 2,
+ * 3, 4, 6; scales [N][ceil(K / 32)]: biased exponents of a block's power of two, 255 for NaN.  Quantisation takes a block's
+ * largest magnitude to [4, 8), rounds to the nearest (ties to the even code) and ends at 6; a block with an infinite or NaN
+ * element has scale 255.  gdn_mxfp4_dequantize writes the values, contiguous (dtype, on 16 bytes).
+ *
+ * gdn_mxfp4_linear: y [M][N] = x w^T, gdn_mxfp4_linear_bwd: dx [M][K] = dy w (x, dy of dtype, rows x_stride or dy_stride
+ * elements apart; y, dx contiguous, of dtype); the weight's values and every bit of x or dy enter 32-bit sums.  A forward call
+ * of at most 64 tokens needs no workspace.  aligned: x or dy lies on 16 bytes, with rows a multiple of 16 bytes apart.
+ * M, N <= 2^24, K <= 2^18. */
+int gdn_mxfp4_quantize(const void *w, void *codes, void *scales, int64_t N, int64_t K, int64_t w_stride, int dtype,
+                       void *stream);
+int gdn_mxfp4_dequantize(const void *codes, const void *scales, void *out, int64_t N, int64_t K, int dtype, void *stream);
+size_t gdn_mxfp4_linear_workspace_bytes(int64_t M, int64_t K, int64_t N, int dtype, int aligned, int backward);
+int gdn_mxfp4_linear(const void *x, const void *codes, const void *scales, void *y, void *workspace, size_t workspace_bytes,
+                     int64_t M, int64_t K, int64_t N, int64_t x_stride, int dtype, void *stream);
+int gdn_mxfp4_linear_bwd(const void *dy, const void *codes, const void *scales, void *dx, void *workspace,
+                         size_t workspace_bytes, int64_t M, int64_t K, int64_t N, int64_t dy_stride, int dtype, void *stream);
 
 #ifdef __cplusplus
 }

@@ -32,6 +32,7 @@ using namespace mm;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int NT = 256;
 constexpr int64_t KEPT = 1 << 26;  // differences of a piece; statistics of the parts of the words
+constexpr int64_t MOST_TOKENS = 1 << 20;  // three slots of 16 bits for each are a row pitch that a product takes
 constexpr int SHIFT = 15;          // differences are stored times 2^15
 constexpr int TOP = 14;            // largest magnitudes of scaled operands: [2^14, 2^15)
 
@@ -360,8 +361,8 @@ static Buffers place(Space &sp, const Sizes &s, bool dx, bool dw, bool bwd, bool
 static int check(int64_t N, int64_t H, int64_t V, int64_t x_ld, int64_t w_ld, int dt) {
     if (N < 0 || H <= 0 || V <= 0) return fail(GDN_ERR_INVALID, "N must be >= 0, H and V > 0");
     if (dt != GDN_F32 && dt != GDN_BF16 && dt != GDN_F16) return fail(GDN_ERR_INVALID, "unknown dtype code");
-    if (N > 1 << 24 || V > 1 << 24 || H > 1 << 17)
-        return fail(GDN_ERR_UNSUPPORTED, "more than 2^24 tokens or words, or 2^17 channels are not supported");
+    if (N > MOST_TOKENS || V > 1 << 24 || H > 1 << 17)
+        return fail(GDN_ERR_UNSUPPORTED, "more than 2^20 tokens, 2^24 words or 2^17 channels are not supported");
     if ((N > 1 && x_ld < H) || (V > 1 && w_ld < H)) return fail(GDN_ERR_INVALID, "rows overlap");
     return GDN_OK;
 }
@@ -416,7 +417,7 @@ static size_t need(const Sizes &s, bool dx, bool dw, bool bwd, bool copy_x, bool
 
 extern "C" size_t gdn_linear_loss_workspace_bytes(int64_t N, int64_t H, int64_t V, int dtype, int aligned, int want_dx,
                                                   int want_dw) {
-    if (N <= 0 || H <= 0 || V <= 0 || N > 1 << 24 || V > 1 << 24 || H > 1 << 17) return 0;
+    if (N <= 0 || H <= 0 || V <= 0 || N > MOST_TOKENS || V > 1 << 24 || H > 1 << 17) return 0;
     const bool copy = !aligned || dtype == GDN_F32 || H % BK;
     return need(sizes(N, H, V, dtype), want_dx, want_dw, want_dx || want_dw, copy, copy);
 }

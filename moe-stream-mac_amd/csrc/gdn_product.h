@@ -318,8 +318,8 @@ __device__ __forceinline__ void products(const Args &g, char *lds, E &&epilogue)
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): no load into this LDS outlives the workgroup
 }
 
-// Whether a product takes operands with this row pitch: offsets within a tile stay below 2^31.
-inline bool pitch_fits(int64_t ld_bytes) { return ld_bytes > 0 && ld_bytes <= (1 << 22); }
+// Whether a product takes operands with this row pitch: offsets within a tile of 256 rows stay below 2^31.
+inline bool pitch_fits(int64_t ld_bytes) { return ld_bytes > 0 && ld_bytes <= (1 << 23); }
 
 // What becomes of a product: C[n][m] -> 2^e row[n] C[n][m], rounded to dt, y rows ldy elements apart.  e = base + sum of
 // sign[i] exps[i]; a row factor of 0 makes zeros of whatever the row holds.  With acc (fp32 [splits][rows][cols]) the parts

@@ -1,7 +1,7 @@
 // Operands of the matrix products laid out in 16-bit terms along the contraction, straight or transposed, for gfx950.
 //
 // A number of more bits than a 16-bit type holds is a sum of terms, each the rounding of what the earlier ones leave:
-// fp32 = 2 fp16 terms up to 2^-22 of it (or 3 bf16 terms, 2^-24).  fp16 has 5 bits of exponent, so a whole matrix is first
+// fp32 = 2 fp16 terms up to 2^-22 of it, or 3 bf16 terms.  fp16 has 5 bits of exponent, so a whole matrix is first
 // multiplied by the power of two that takes its largest magnitude to 2^14: a bf16 number (8 bits) is then exact down to
 // 2^-32 of the largest, and what is smaller is off by 2^-40 of it at most.
 #include "gdn_common.h"
@@ -57,7 +57,8 @@ __global__ __launch_bounds__(64) void exponents_kernel(const float *part, int to
     }
 }
 
-// Term `t` of y: what the terms before it leave, rounded; an infinite or NaN number is its first term.
+// The next term of y, which keeps the rest: rounded (fp16) or cut off (bf16: three take the 24 bits of an fp32 number as they
+// are, and none becomes infinite).  An infinite or NaN number is its first term.
 template <bool F16>
 __device__ __forceinline__ uint16_t next_term(float &y) {
     uint16_t b;
@@ -67,7 +68,7 @@ __device__ __forceinline__ uint16_t next_term(float &y) {
         b = __half_as_ushort(h);
         back = __half2float(h);
     } else {
-        b = f32_to_bf16_cvt(y);
+        b = (uint16_t)(__float_as_uint(y) >> 16 | (y != y ? 0x40u : 0u));
         back = bf16_to_f32(b);
     }
     y = fabsf(back) <= 3.4028234e38f ? y - back : 0.f;

@@ -65,6 +65,11 @@ _SIGS = {
     "gdn_embedding_fwd": ([_vp] * 3 + [_i64] * 4 + [_d, _i, _vp], _i),
     "gdn_embedding_bwd_workspace_bytes": ([_i64] * 3, _sz),
     "gdn_embedding_bwd": ([_vp] * 4 + [_sz] + [_i64] * 5 + [_d, _i, _vp], _i),
+    "gdn_mxfp4_quantize": ([_vp] * 3 + [_i64] * 3 + [_i, _vp], _i),
+    "gdn_mxfp4_dequantize": ([_vp] * 3 + [_i64] * 2 + [_i, _vp], _i),
+    "gdn_mxfp4_linear_workspace_bytes": ([_i64] * 3 + [_i] * 3, _sz),
+    "gdn_mxfp4_linear": ([_vp] * 5 + [_sz] + [_i64] * 4 + [_i, _vp], _i),
+    "gdn_mxfp4_linear_bwd": ([_vp] * 5 + [_sz] + [_i64] * 4 + [_i, _vp], _i),
     "gdn_version": ([], _i),
     "gdn_last_error": ([], ctypes.c_char_p),
     "gdn_num_snapshots": ([_i, _i], ctypes.c_int64),

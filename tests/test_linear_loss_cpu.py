@@ -18,7 +18,7 @@ def test_abi_refusals():
     for kw in (dict(N=-1), dict(H=0), dict(V=0), dict(dt=3), dict(red=3), dict(red=1, total=None), dict(p=None), dict(xs=63),
                dict(ws=10)):
         assert fwd(**kw) == L.GDN_ERR_INVALID, kw
-    for kw in (dict(N=(1 << 24) + 1), dict(V=(1 << 24) + 1), dict(H=(1 << 17) + 1, xs=1 << 18, ws=1 << 18)):
+    for kw in (dict(N=(1 << 20) + 1), dict(V=(1 << 24) + 1), dict(H=(1 << 17) + 1, xs=1 << 18, ws=1 << 18)):
         assert fwd(**kw) == L.GDN_ERR_UNSUPPORTED, kw
     need = lib.gdn_linear_loss_workspace_bytes(4, 64, 100, 1, 1, 0, 0)
     assert need > 0 and fwd(room=need - 1) == L.GDN_ERR_WORKSPACE and b"workspace" in lib.gdn_last_error()
@@ -40,7 +40,7 @@ def test_workspace_stays_bounded():
     """Forward 2^26 statistics or 256 tokens' (and room for copies of what is not aligned); backward 2^26 differences, in 16 bits
     for each gradient, or 256 words', the operands of their products and fp32 sums of dx in parts."""
     f, H, MB = L.load().gdn_linear_loss_workspace_bytes, 2048, 1 << 20
-    for N, V in ((8192, 131072), (1 << 20, 131072), (1 << 24, 1000), (100, 1 << 24)):
+    for N, V in ((8192, 131072), (1 << 20, 131072), (1 << 20, 1000), (100, 1 << 24)):
         stats = 8 * max(1 << 26, 256 * (V // 64 + 512))
         assert f(N, H, V, 1, 1, 0, 0) <= stats + 4 * N + MB, (N, V)
         assert f(N, H, V, 1, 0, 0, 0) <= stats + 4 * N + 2 * H * (N + min(V, (1 << 26) // N + 512)) + MB
