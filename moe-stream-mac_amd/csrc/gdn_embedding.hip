@@ -26,23 +26,24 @@ constexpr int CHUNK = 32;   // tokens summed by one workgroup
 
 // ------------------------------------------------------------------------------------------------ forward
 
-// V elements to a thread, `per` of these to a row.
-template <int V>
+template <int DT>
+struct Width { static constexpr int V = DT == DT_F32 ? 4 : 8; };  // elements to a thread: 16 bytes
+
+// `per` vectors to a row.
+template <int DT>
 __global__ __launch_bounds__(NT) void rows_kernel(const int64_t *ids, const void *w, void *y, int64_t N, int64_t words, int H,
-                                                  int64_t ld, double scale, int dt, int per) {
-    const int64_t i = block_index() * NT + threadIdx.x, n = i / per;
+                                                  int64_t ld, double scale, uint32_t per) {
+    constexpr int V = Width<DT>::V;
+    const int64_t i = block_index() * NT + threadIdx.x;
+    const int64_t n = i >> 32 ? i / per : (uint32_t)i / per;
     if (n >= N) return;
     const int64_t c = (i - n * per) * V, id = ids[n];
     float x[V];
-    if (id >= 0 && id < words) {
-        ops::loadv<V>(w, id * ld + c, dt, x);
+    const bool in = id >= 0 && id < words;
+    ops::load_first<V, DT>(w, (in ? id : 0) * ld + c, H - c, x);
 #pragma unroll
-        for (int j = 0; j < V; ++j) x[j] = (float)(x[j] * scale);
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) x[j] = NAN;
-    }
-    ops::storev<V>(y, n * H + c, dt, x);
+    for (int j = 0; j < V; ++j) x[j] = in ? (float)(x[j] * scale) : NAN;
+    ops::store_first<V, DT>(y, n * H + c, H - c, x);
 }
 
 // ------------------------------------------------------------------------------------------------ order
@@ -105,37 +106,38 @@ struct SumArgs {
     double *part;   // [chunks][H] of chunks within one word's run
     int *starts;    // [words + 1] the first place of each word's run
     int64_t N, words, ld;
-    int H, dt, lanes;  // lanes: threads to a row, a power of two
+    int H, lanes;  // lanes: threads to a row, a power of two
     double scale;
 };
 
 __device__ __forceinline__ int64_t word(uint64_t key) { return (int64_t)(key >> 32); }
 __device__ __forceinline__ int64_t token(uint64_t key) { return (int64_t)(key & 0xffffffffull); }
 
-// x += rows of the tokens [a, b) of the sorted list, four under way.
-template <int V>
+// x += rows of the tokens [a, b) of the sorted list, U under way.
+template <int DT, int U, int V>
 __device__ __forceinline__ void add_tokens(const SumArgs &s, int64_t a, int64_t b, int64_t c, double (&x)[V]) {
     int64_t i = a;
-    for (; i + 4 <= b; i += 4) {
-        float v[4][V];
+    for (; i + U <= b; i += U) {
+        float v[U][V];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) ops::loadv<V>(s.dy, token(s.keys[i + u]) * s.ld + c, s.dt, v[u]);
+        for (int u = 0; u < U; ++u) ops::load_first<V, DT>(s.dy, token(s.keys[i + u]) * s.ld + c, s.H - c, v[u]);
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int j = 0; j < V; ++j) x[j] += v[u][j];
     }
     for (; i < b; ++i) {
         float v[V];
-        ops::loadv<V>(s.dy, token(s.keys[i]) * s.ld + c, s.dt, v);
+        ops::load_first<V, DT>(s.dy, token(s.keys[i]) * s.ld + c, s.H - c, v);
 #pragma unroll
         for (int j = 0; j < V; ++j) x[j] += v[j];
     }
 }
 
 // The first `chunks` workgroups: sums of whole chunks.  The others: the words' first places.
-template <int V>
+template <int DT>
 __global__ __launch_bounds__(NT) void chunk_kernel(const SumArgs s, int64_t chunks) {
+    constexpr int V = Width<DT>::V;
     const int64_t g = block_index();
     if (g < chunks) {
         const int64_t a = g * CHUNK, b = a + CHUNK;
@@ -146,9 +148,10 @@ __global__ __launch_bounds__(NT) void chunk_kernel(const SumArgs s, int64_t chun
             double x[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) x[j] = 0.;
-            add_tokens<V>(s, a, b, c, x);
+            add_tokens<DT, 8>(s, a, b, c, x);
 #pragma unroll
-            for (int j = 0; j < V; ++j) s.part[g * s.H + c + j] = x[j];
+            for (int j = 0; j < V; ++j)
+                if (c + j < s.H) s.part[g * s.H + c + j] = x[j];
         }
         return;
     }
@@ -165,8 +168,9 @@ __global__ __launch_bounds__(NT) void chunk_kernel(const SumArgs s, int64_t chun
     s.starts[v] = (int)lo;
 }
 
-template <int V>
+template <int DT>
 __global__ __launch_bounds__(NT) void words_kernel(const SumArgs s) {
+    constexpr int V = Width<DT>::V;
     const int lane = threadIdx.x & (s.lanes - 1);
     const int64_t v = block_index() * (NT / s.lanes) + threadIdx.x / s.lanes;
     if (v >= s.words) return;
@@ -175,21 +179,23 @@ __global__ __launch_bounds__(NT) void words_kernel(const SumArgs s) {
         double x[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) x[j] = 0.;
-        const int64_t c0 = (a + CHUNK - 1) / CHUNK, c1 = b / CHUNK;  // whole chunks
-        if (c0 < c1) {
-            add_tokens<V>(s, a, c0 * CHUNK, c, x);
-#pragma unroll 4
+        // tokens up to the first whole chunk, whole chunks, tokens after them; or tokens alone
+        const int64_t c0 = (a + CHUNK - 1) / CHUNK, c1 = b / CHUNK;
+        int64_t from = a, to = c0 < c1 ? c0 * CHUNK : b;
+        while (from < b) {
+            add_tokens<DT, 4>(s, from, to, c, x);
+            if (to == b) break;
+#pragma unroll 2
             for (int64_t k = c0; k < c1; ++k)
 #pragma unroll
-                for (int j = 0; j < V; ++j) x[j] += s.part[k * s.H + c + j];
-            add_tokens<V>(s, c1 * CHUNK, b, c, x);
-        } else {
-            add_tokens<V>(s, a, b, c, x);
+                for (int j = 0; j < V; ++j) x[j] += c + j < s.H ? s.part[k * s.H + c + j] : 0.;
+            from = c1 * CHUNK;
+            to = b;
         }
         float y[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) y[j] = (float)(x[j] * s.scale);
-        ops::storev<V>(s.dw, v * s.H + c, s.dt, y);
+        ops::store_first<V, DT>(s.dw, v * s.H + c, s.H - c, y);
     }
 }
 
@@ -201,12 +207,12 @@ static int check(int64_t N, int64_t V, int64_t H, int dt) {
     return GDN_OK;
 }
 
-// Elements to a load: 16 bytes of 16-bit data, or 4 or 1 where sizes, strides and addresses ask for it.
-static int width(int64_t H, int64_t ld, const void *a, const void *b) {
-    for (int v = 8; v > 1; v /= 2)
-        if (v != 2 && H % v == 0 && ld % v == 0 && aligned_to(a, 16) && aligned_to(b, 16)) return v;
-    return 1;
-}
+#define GDN_BY_TYPE(dtype, call)                  \
+    if (dtype == GDN_F32) { call(DT_F32); }       \
+    else if (dtype == GDN_BF16) { call(DT_BF16); } \
+    else { call(DT_F16); }
+
+static int width(int dtype) { return dtype == GDN_F32 ? emb::Width<DT_F32>::V : emb::Width<DT_BF16>::V; }
 
 }  // namespace emb
 }  // namespace gdn
@@ -220,15 +226,13 @@ extern "C" int gdn_embedding_fwd(const int64_t *ids, const void *w, void *y, int
     if (N == 0) return GDN_OK;
     if (!ids || !w || !y) return fail(GDN_ERR_INVALID, "null pointer");
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const int v = emb::width(H, w_stride, w, y), per = (int)(H / v);
-    const dim3 grid = grid_of((N * per + emb::NT - 1) / emb::NT), block(emb::NT);
+    const int64_t per = (H + emb::width(dtype) - 1) / emb::width(dtype);
     {
         Timed tm("embedding", st);
-#define GDN_ROWS(V_)                                                                                                   \
-    hipLaunchKernelGGL((emb::rows_kernel<V_>), grid, block, 0, st, ids, w, y, N, V, (int)H, w_stride, scale, dtype, per)
-        if (v == 8) GDN_ROWS(8);
-        else if (v == 4) GDN_ROWS(4);
-        else GDN_ROWS(1);
+#define GDN_ROWS(DT)                                                                                                    \
+    hipLaunchKernelGGL((emb::rows_kernel<DT>), grid_of((N * per + emb::NT - 1) / emb::NT), dim3(emb::NT), 0, st, ids, w, y, N, \
+                       V, (int)H, w_stride, scale, (uint32_t)per)
+        GDN_BY_TYPE(dtype, GDN_ROWS)
 #undef GDN_ROWS
     }
     return check_launch(st, "gdn_embedding_fwd");
@@ -267,23 +271,18 @@ extern "C" int gdn_embedding_bwd(const int64_t *ids, const void *dy, void *dw, v
         }
     }
     s.keys = keys; s.dy = dy; s.dw = dw;
-    s.N = N; s.words = V; s.ld = dy_stride; s.H = (int)H; s.dt = dtype; s.scale = scale;
-    const int v = emb::width(H, dy_stride, dy, dw);
+    s.N = N; s.words = V; s.ld = dy_stride; s.H = (int)H; s.scale = scale;
     s.lanes = 1;
-    while (s.lanes < emb::NT && s.lanes * v < H) s.lanes *= 2;
+    while (s.lanes < emb::NT && s.lanes * emb::width(dtype) < H) s.lanes *= 2;
     const int64_t chunks = N / emb::CHUNK;
     const dim3 block(emb::NT), some = grid_of(chunks + (V + emb::NT) / emb::NT);
     const dim3 all = grid_of((V + emb::NT / s.lanes - 1) / (emb::NT / s.lanes));
     {
         Timed tm("embedding_sum", st);
-#define GDN_SUMS(V_)                                                                      \
-    do {                                                                                  \
-        hipLaunchKernelGGL((emb::chunk_kernel<V_>), some, block, 0, st, s, chunks);       \
-        hipLaunchKernelGGL((emb::words_kernel<V_>), all, block, 0, st, s);                \
-    } while (0)
-        if (v == 8) GDN_SUMS(8);
-        else if (v == 4) GDN_SUMS(4);
-        else GDN_SUMS(1);
+#define GDN_SUMS(DT)                                                                  \
+    hipLaunchKernelGGL((emb::chunk_kernel<DT>), some, block, 0, st, s, chunks);       \
+    hipLaunchKernelGGL((emb::words_kernel<DT>), all, block, 0, st, s)
+        GDN_BY_TYPE(dtype, GDN_SUMS)
 #undef GDN_SUMS
     }
     return check_launch(st, "gdn_embedding_bwd");

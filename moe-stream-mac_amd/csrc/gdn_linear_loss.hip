@@ -53,8 +53,9 @@ struct StatArgs {
 template <class S, bool F16, bool SCALED>
 __global__ __launch_bounds__(S::NT, S::WAVES_EU) void stat_kernel(const Args g, const StatArgs a) {
     __shared__ __attribute__((aligned(16))) char lds[S::LDS];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, wm = w / S::WN, wn = w % S::WN;
+    const int w = wave_index(), wm = w / S::WN, wn = w % S::WN;
     products<S, F16>(g, lds, [&](int tm, int tn, acc_t(&acc)[S::TM][S::TN]) {
+        const int lane = lane_here();
         const int64_t m0 = (int64_t)tm * S::BM + wm * (S::BM / S::WM);  // of the operand's rows
         const int words = (int)min((int64_t)(S::BM / S::WM), g.a.rows - m0);
         const int e = SCALED ? -(a.exps[E_X] + a.exps[E_W]) : 0;
@@ -96,16 +97,18 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void stat_kernel(const Args g, 
     });
 }
 
-// Joins a token's parts: 16 tokens to a workgroup, 16 threads to a token.
+// Joins a token's parts: TOKENS tokens to a workgroup, NT / TOKENS threads to a token.
+template <int TOKENS>
 __global__ __launch_bounds__(NT) void join_kernel(const int64_t *targets, const float2 *part, int parts, const float *zt,
                                                   int64_t N, int64_t V, int64_t ignore, float *loss, float2 *stat) {
-    __shared__ float2 red[16][16];
-    const int tl = threadIdx.x & 15, p0 = threadIdx.x >> 4;
-    const int64_t n = block_index() * 16 + tl;
+    constexpr int P = NT / TOKENS;
+    __shared__ float2 red[P][TOKENS];
+    const int tl = threadIdx.x % TOKENS, p0 = threadIdx.x / TOKENS;
+    const int64_t n = block_index() * TOKENS + tl;
     float m = -INFINITY, s = 0.f;
     if (n < N) {
 #pragma unroll 8
-        for (int p = p0; p < parts; p += 16) {
+        for (int p = p0; p < parts; p += P) {
             const float2 o = part[(int64_t)p * N + n];
             const float b = fmaxf(m, o.x), r = b == -INFINITY ? 0.f : b;
             s = s * __builtin_amdgcn_exp2f((m - r) * LOG2E) + o.y * __builtin_amdgcn_exp2f((o.x - r) * LOG2E);
@@ -114,18 +117,24 @@ __global__ __launch_bounds__(NT) void join_kernel(const int64_t *targets, const 
     }
     red[p0][tl] = make_float2(m, s);
     __syncthreads();
+#pragma unroll
+    for (int h = P / 2; h >= 1; h /= 2) {
+        if (p0 < h) {
+            const float2 o = red[p0 + h][tl];
+            const float b = fmaxf(m, o.x), r = b == -INFINITY ? 0.f : b;
+            s = s * __builtin_amdgcn_exp2f((m - r) * LOG2E) + o.y * __builtin_amdgcn_exp2f((o.x - r) * LOG2E);
+            m = b;
+            red[p0][tl] = make_float2(m, s);
+        }
+        __syncthreads();
+    }
     if (p0 || n >= N) return;
-    float M = -INFINITY;
-    for (int p = 0; p < 16; ++p) M = fmaxf(M, red[p][tl].x);
-    const float r = M == -INFINITY ? 0.f : M;
-    s = 0.f;
-    for (int p = 0; p < 16; ++p) s += red[p][tl].y * __builtin_amdgcn_exp2f((red[p][tl].x - r) * LOG2E);
     const int64_t t = targets[n];
-    float l = logf(s) - (zt[n] - M);
+    float l = logf(s) - (zt[n] - m);
     if (t < 0 || t >= V) l = NAN;
     if (t == ignore) l = 0.f;
     loss[n] = l;
-    if (stat) stat[n] = make_float2(M, 1.f / s);
+    if (stat) stat[n] = make_float2(m, 1.f / s);
 }
 
 // The losses' sum, or mean over the tokens that count, and what a token's cotangent is multiplied by.
@@ -192,72 +201,112 @@ struct DiffArgs {
     int64_t N, v0, kp, np;
 };
 
-__device__ __forceinline__ uint32_t half_bits(float x) { return __half_as_ushort(__float2half(x)); }
+// x as it was rounded: the compiler may round a product or sum to 16 bits at once in one place and in two steps in another, and
+// terms that are taken in two places have to belong to the same number.
+__device__ __forceinline__ float as_rounded(float x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// What a term leaves of x, times 2^LOW: the next term.
+__device__ __forceinline__ float left_of(float x) {
+    return (x - __half2float(__float2half(x))) * (float)(1 << LOW);
+}
 
 // The differences of a piece of words, 2^15 (p - [v = t]), and times d / (the power of two over the largest |d|) for dW.
 template <class S, bool F16, int TERMS, bool DX, bool DW>
 __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, const DiffArgs a) {
-    __shared__ __attribute__((aligned(16))) char lds[S::LDS];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, wm = w / S::WN, wn = w % S::WN;
-    products<S, F16>(g, lds, [&](int tm, int tn, const acc_t(&acc)[S::TM][S::TN]) {
-        const int64_t m0 = (int64_t)tm * S::BM + wm * (S::BM / S::WM) + 4 * (lane >> 5);
-        const int64_t words = g.a.rows;
+    __shared__ __attribute__((aligned(16))) char lds[S::LDS + S::STORE];
+    const int w = wave_index(), wm = w / S::WN, wn = w % S::WN;
+    char *store = lds + S::LDS + w * 4096;
+    products<S, F16>(g, lds, [&](int tm, int tn, acc_t(&acc)[S::TM][S::TN]) {
+        const int lane = lane_here();
+        const int64_t m0 = (int64_t)tm * S::BM + wm * (S::BM / S::WM), n0 = (int64_t)tn * S::BN + wn * (S::BN / S::WN);
+        const int words = (int)min((int64_t)(S::BM / S::WM), g.a.rows - m0);  // of this wave's; may be negative
         const int e = TERMS > 1 ? -(a.exps[E_X] + a.exps[E_W]) : 0;
+        float r[S::TN];
 #pragma unroll
         for (int j = 0; j < S::TN; ++j) {
-            const int64_t n = (int64_t)tn * S::BN + wn * (S::BN / S::WN) + 32 * j + (lane & 31);
+            const int64_t n = n0 + 32 * j + (lane & 31);
             const bool live = n < a.N;
             const float2 st = live ? a.stat[n] : make_float2(0.f, 0.f);
-            const float d = live ? a.d[n] : 0.f, r = DW ? ldexpf(d, a.exps[E_D]) : 0.f;
+            r[j] = DW && live ? ldexpf(a.d[n], a.exps[E_D]) : 0.f;
             const float inv = st.y * (float)(1 << SHIFT);
-            const int64_t hot = live ? a.targets[n] - a.v0 - m0 : -1;
+            const int64_t hot = live ? a.targets[n] - a.v0 - m0 - 4 * (lane >> 5) : -1;
 #pragma unroll
             for (int i = 0; i < S::TM; ++i)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int64_t m = m0 + 32 * i + 8 * q;
-                    float x[4];
+                for (int q = 0; q < 16; ++q) {
+                    const int m = 32 * i + 8 * (q / 4) + q % 4;
+                    float z = acc[i][j][q];
+                    if constexpr (TERMS > 1) z = ldexpf(z, e);
+                    float x = __builtin_amdgcn_exp2f((z - st.x) * LOG2E) * inv;
+                    if (hot == m) x -= (float)(1 << SHIFT);
+                    if (words < S::BM / S::WM && m + 4 * (lane >> 5) >= words) x = 0.f;
+                    acc[i][j][q] = TERMS > 1 ? as_rounded(x) : x;
+                }
+        }
+        if constexpr (DX) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        float z = acc[i][j][4 * q + k];
-                        if constexpr (TERMS > 1) z = ldexpf(z, e);
-                        x[k] = __builtin_amdgcn_exp2f((z - st.x) * LOG2E) * inv;
-                        if (hot == 32 * i + 8 * q + k) x[k] -= (float)(1 << SHIFT);
-                        if (m + k >= words) x[k] = 0.f;
-                    }
-                    if constexpr (DX) {
-                        if (live && m < a.kp) {
-                            uint16_t *to = a.p + n * (TERMS * a.kp) + m;
-                            float y[4] = {x[0], x[1], x[2], x[3]};
+            for (int j = 0; j < S::TN; ++j) {
+                const int64_t n = n0 + 32 * j, rows = a.N - n;
+                if (rows <= 0) break;
 #pragma unroll
-                            for (int t = 0; t < TERMS; ++t) {
-                                uint32_t b[4];
+                for (int i = 0; i < S::TM; i += 2) {
+                    const int64_t m = m0 + 32 * i;
+                    if (m >= a.kp) break;
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    b[k] = half_bits(y[k]);
-                                    y[k] = (y[k] - __half2float(__ushort_as_half((unsigned short)b[k]))) * (float)(1 << LOW);
-                                }
-                                *reinterpret_cast<uint2 *>(to + t * a.kp) = make_uint2(b[0] | b[1] << 16, b[2] | b[3] << 16);
+                    for (int t = 0; t < TERMS; ++t) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                float y[4];
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) y[k] = t ? left_of(acc[i + h][j][4 * q + k]) : acc[i + h][j][4 * q + k];
+                                put16(lane, store, h, q, ops::pack2(y[0], y[1], DT_F16), ops::pack2(y[2], y[3], DT_F16));
                             }
-                        }
-                    }
-                    if constexpr (DW) {
-                        if (n < a.np) {
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                if (m + k >= words) continue;
-                                float y = r == 0.f ? 0.f : x[k] * r;
-                                uint16_t *to = a.pt + (m + k) * (TERMS * a.np) + n;
-#pragma unroll
-                                for (int t = 0; t < TERMS; ++t) {
-                                    const uint32_t b = half_bits(y);
-                                    to[t * a.np] = (uint16_t)b;
-                                    y = (y - __half2float(__ushort_as_half((unsigned short)b))) * (float)(1 << LOW);
-                                }
-                            }
-                        }
+                        store_rows(lane, store, reinterpret_cast<char *>(a.p + n * (TERMS * a.kp) + t * a.kp + m),
+                                   (uint32_t)(TERMS * a.kp * 2), rows, (a.kp - m) * 2, 2);
                     }
                 }
+            }
+        }
+        if constexpr (DW) {
+            constexpr int W = S::TN < 2 ? 1 : 2;  // tiles of tokens side by side
+#pragma unroll
+            for (int j = 0; j < S::TN; j += W) {
+                const int64_t n = n0 + 32 * j;
+                if (n >= a.np) break;
+#pragma unroll
+                for (int i = 0; i < S::TM; ++i) {
+                    if (32 * i >= words) break;
+#pragma unroll
+                    for (int t = 0; t < TERMS; ++t) {
+#pragma unroll
+                        for (int h = 0; h < W; ++h)
+#pragma unroll
+                            for (int q = 0; q < 16; q += 2) {
+                                float y[2];
+#pragma unroll
+                                for (int k = 0; k < 2; ++k) {
+                                    y[k] = r[j + h] == 0.f ? 0.f : acc[i][j + h][q + k] * r[j + h];
+                                    if (TERMS > 1) y[k] = as_rounded(y[k]);
+                                    if (t) y[k] = left_of(y[k]);
+                                }
+                                // two words of a token become two tokens of a word, with the neighbouring lane
+                                const uint32_t own = ops::pack2(y[0], y[1], DT_F16);
+                                const uint32_t its = __builtin_amdgcn_update_dpp(0, (int)own, DPP_QUAD_1032, 0xF, 0xF, false);
+                                const uint32_t v = lane & 1 ? (its >> 16) | (own & 0xffff0000u) : (own & 0xffffu) | (its << 16);
+                                const int row = 8 * (q / 4) + 4 * (lane >> 5) + q % 4 + (lane & 1), col = 32 * h + (lane & 30);
+                                *reinterpret_cast<uint32_t *>(store_chunk(store, row, col >> 3) + (col & 7) * 2) = v;
+                            }
+                        const int64_t left = (a.np - n) * 2;
+                        store_rows(lane, store, reinterpret_cast<char *>(a.pt + (m0 + 32 * i) * (TERMS * a.np) + t * a.np + n),
+                                   (uint32_t)(TERMS * a.np * 2), words - 32 * i, left < W * 64 ? left : W * 64, 2);
+                    }
+                }
+            }
         }
     });
 }
@@ -348,12 +397,12 @@ static Buffers place(Space &sp, const Sizes &s, bool dx, bool dw, bool bwd, bool
     if (dx) {
         b.wt = sp.take<uint16_t>(s.H * across_slots(t) * padded(words));
         b.p = sp.take<uint16_t>(s.N * t * padded(words));
-        b.acc_x = sp.take<float>((int64_t)s.px.splits * s.N * s.H);
+        b.acc_x = sp.take<float>((int64_t)s.px.splits * s.N * columns_of(s.H));
     }
     if (dw) {
         b.xt = sp.take<uint16_t>(s.H * across_slots(t) * s.np);
         b.pt = sp.take<uint16_t>(words * t * s.np);
-        if (s.pw.splits > 1) b.acc_w = sp.take<float>((int64_t)s.pw.splits * words * s.H);
+        if (s.pw.splits > 1) b.acc_w = sp.take<float>((int64_t)s.pw.splits * words * columns_of(s.H));
     }
     return b;
 }
@@ -486,8 +535,14 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
 #undef GDN_STAT
             }
             Timed tm("loss_join", st);
-            hipLaunchKernelGGL(join_kernel, grid_of((tokens + 15) / 16), dim3(NT), 0, st, targets + n0, b.stats, parts, b.zt,
-                               tokens, V, ignore_index, loss + n0, stat ? reinterpret_cast<float2 *>(stat) + n0 : nullptr);
+            float2 *to = stat ? reinterpret_cast<float2 *>(stat) + n0 : nullptr;
+            // 128 bytes of a part's tokens at a time, or all threads on the parts of one of few
+            if (tokens > 64)
+                hipLaunchKernelGGL((join_kernel<16>), grid_of((tokens + 15) / 16), dim3(NT), 0, st, targets + n0, b.stats, parts,
+                                   b.zt, tokens, V, ignore_index, loss + n0, to);
+            else
+                hipLaunchKernelGGL((join_kernel<1>), grid_of(tokens), dim3(NT), 0, st, targets + n0, b.stats, parts, b.zt, tokens,
+                                   V, ignore_index, loss + n0, to);
         }
     }
     if (reduction)
@@ -564,7 +619,7 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
             h.b.p = reinterpret_cast<const char *>(b.p);
             h.b.rows = N;
             const Plan pl = s.px;  // parts without a block of the last piece add nothing
-            Result r{dx, H, dtype, b.d, b.exps, -SHIFT, {0, -1, 0}, nullptr, v0 > 0};
+            Result r{dx, H, dtype, b.d, b.exps, -SHIFT, {0, -1, 0}, nullptr, columns_of(H), v0 > 0};
             if (s.pieces > 1 || pl.splits > 1) r.acc = b.acc_x;
             multiply(h, true, pl, r, st);
             if (r.acc && v0 + words == V) finish(r, pl.splits, N, H, st);
@@ -576,7 +631,7 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
             h.a.rows = H;
             h.b.p = reinterpret_cast<const char *>(b.pt);
             h.b.rows = words;
-            Result r{static_cast<char *>(dw) + v0 * H * elem, H, dtype, nullptr, b.exps, -SHIFT, {-1, 0, -1}, nullptr, 0};
+            Result r{static_cast<char *>(dw) + v0 * H * elem, H, dtype, nullptr, b.exps, -SHIFT, {-1, 0, -1}, nullptr, columns_of(H), 0};
             if (s.pw.splits > 1) r.acc = b.acc_w;
             multiply(h, true, s.pw, r, st);
             if (r.acc) finish(r, s.pw.splits, words, H, st);

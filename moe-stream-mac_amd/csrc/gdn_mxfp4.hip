@@ -306,7 +306,7 @@ static Buffers place(Space &sp, const Sizes &s, int64_t M, int64_t K, bool back,
     b.w = sp.take((size_t)(back ? K : s.piece) * s.kp * 2);
     if (copy) b.x = sp.take((size_t)M * s.terms * s.kp * 2);
     const bool parts = s.plan.splits > 1 || (back && s.pieces > 1);
-    if (parts) b.acc = reinterpret_cast<float *>(sp.take((size_t)s.plan.splits * M * (back ? K : s.piece) * 4));
+    if (parts) b.acc = reinterpret_cast<float *>(sp.take((size_t)s.plan.splits * M * columns_of(back ? K : s.piece) * 4));
     return b;
 }
 
@@ -427,7 +427,7 @@ extern "C" int gdn_mxfp4_linear(const void *x, const void *codes, const void *sc
                                    static_cast<const uint8_t *>(scales) + n0 * blocks, b.w, rows, K, blocks, s.kp, 0);
             }
             g.a = Operand{b.w, s.kp * 2, rows, {0, 0, 0}};
-            const Result r{static_cast<char *>(y) + n0 * elem, N, dtype, nullptr, nullptr, 0, {0, 0, 0}, b.acc, 0};
+            const Result r{static_cast<char *>(y) + n0 * elem, N, dtype, nullptr, nullptr, 0, {0, 0, 0}, b.acc, columns_of(rows), 0};
             multiply(g, false, s.plan, r, st);
             if (r.acc) finish(r, s.plan.splits, M, rows, st);
         }
@@ -465,7 +465,7 @@ extern "C" int gdn_mxfp4_linear_bwd(const void *dy, const void *codes, const voi
                                blocks, np, tiles_k, tiles);
         }
         g.a = Operand{b.w, np * 2, K, {0, 0, 0}};
-        const Result r{dx, K, dtype, nullptr, nullptr, 0, {0, 0, 0}, b.acc, n0 > 0};
+        const Result r{dx, K, dtype, nullptr, nullptr, 0, {0, 0, 0}, b.acc, columns_of(K), n0 > 0};
         multiply(g, false, s.plan, r, st);
         if (r.acc && n0 + rows == N) finish(r, s.plan.splits, M, K, st);
     }

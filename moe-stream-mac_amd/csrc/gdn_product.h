@@ -60,15 +60,27 @@ struct Shape {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NT = 64 * WM_ * WN_;
     static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
     static constexpr int A_BYTES = BM * BK * 2, STAGE = (BM + BN) * BK * 2, LDS = 2 * STAGE;
+    static constexpr int STORE = WM * WN * 4096;  // LDS through which a wave's results leave, 4 KB each
     static constexpr int RA = BM * 8 / NT, RB = BN * 8 / NT;  // 16-byte loads of a thread for a stage
     static constexpr int PER_CU = PER_CU_;
     static constexpr int WAVES_EU = PER_CU_ * NT / 256;
     static_assert(RA >= 1 && RB >= 1 && TM % 2 == 0 && TN >= 1, "tile");
 };
+// The lane, as a value that is worked out where it stands: what an epilogue derives from it would otherwise be kept in registers
+// through the whole product, which has none to spare.
+__device__ __forceinline__ int lane_here() {
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
+// This wave's number, known to be the same for all its lanes.
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+
 typedef Shape<256, 256, 2, 4, 1> Big;
 typedef Shape<128, 128, 2, 2, 2> Mid;
-typedef Shape<128, 64, 2, 2, 3> Few;
-typedef Shape<128, 32, 2, 1, 4> One;
+typedef Shape<128, 64, 2, 2, 2> Few;
+typedef Shape<128, 32, 2, 1, 3> One;
 
 typedef __attribute__((address_space(1))) const void gvoid;
 typedef __attribute__((address_space(3))) void lvoid;
@@ -263,14 +275,14 @@ __device__ __forceinline__ void second_half(const char *__restrict__ rd, char *_
 // acc[i][j]: rows m = 32 i + 8 (q / 4) + 4 (lane / 32) + q % 4 of this wave's part for register q, column n = 32 j + lane % 32.
 template <class S, bool F16, class E>
 __device__ __forceinline__ void products(const Args &g, char *lds, E &&epilogue) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, wm = w / S::WN, wn = w % S::WN;
+    const int lane = threadIdx.x & 63, w = wave_index(), wm = w / S::WN, wn = w % S::WN;
     const int total = g.kit * g.nseg;
     const int first = (int)((int64_t)total * blockIdx.z / g.splits), end = (int)((int64_t)total * (blockIdx.z + 1) / g.splits);
     const int blocks = end - first, mt = g.mt, nt = g.nt;
     Loader<S> ld;
     ld.tile = blockIdx.x;
     ld.tiles = mt * nt;
-    ld.w = __builtin_amdgcn_readfirstlane(w);
+    ld.w = w;
     if (ld.tile >= ld.tiles || blocks == 0) return;
     ld.start(g, first, end);
     uint32_t at_a[4], at_b[4];
@@ -318,12 +330,71 @@ __device__ __forceinline__ void products(const Args &g, char *lds, E &&epilogue)
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): no load into this LDS outlives the workgroup
 }
 
+// A wave's results leave through 4 KB of LDS, 32 rows of 128 bytes at a time (chunk c of 16 bytes of row r in place c ^ (r & 7)):
+// eight lanes then store 128 bytes of one row, where registers hold 8 or 16 bytes of 32 rows.  At 8192 x 8192 x 2048 the
+// product takes 215 us so, 231 to 280 with stores from registers.
+__device__ __forceinline__ char *store_chunk(char *st, int row, int chunk) { return st + row * 128 + ((chunk ^ (row & 7)) << 4); }
+
+// Rows [0, rows) of the 32 in LDS to memory, ld bytes apart (32 of them less than 2^32 bytes), of which the first `bytes` of
+// each count.  to, ld, rows and bytes are the same for the whole wave.
+__device__ __forceinline__ void store_rows(int lane, const char *st, char *to, uint32_t ld, int64_t rows, int64_t bytes,
+                                           int elem) {
+    typedef u4 any4 __attribute__((aligned(2)));
+    const int c = lane & 7;
+    asm volatile("" ::: "memory");  // what other lanes have put there: LDS keeps a wave's order, the compiler has to
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const int r = t * 8 + (lane >> 3);
+        const u4 v = *reinterpret_cast<const u4 *>(store_chunk(const_cast<char *>(st), r, c));
+        if (r >= rows) continue;
+        char *at = to + ((uint32_t)r * ld + (uint32_t)c * 16);
+        if (c * 16 + 16 <= bytes) {
+            *reinterpret_cast<any4 *>(at) = v;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {  // by 16 bits; an fp32 element is two
+                const uint16_t h = (uint16_t)(v[j / 2] >> (16 * (j % 2)));
+                if (c * 16 + j / (elem / 2) * elem + elem <= bytes) reinterpret_cast<uint16_t *>(at)[j] = h;
+            }
+        }
+    }
+    asm volatile("" ::: "memory");
+}
+
+// Adds the 32 rows in memory, ld bytes apart and padded to 16, to the fp32 numbers in LDS.
+__device__ __forceinline__ void add_rows(int lane, char *st, const char *from, uint32_t ld, int64_t rows, int64_t bytes) {
+    const int c = lane & 7;
+    asm volatile("" ::: "memory");
+    float4 v[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const int r = t * 8 + (lane >> 3);
+        v[t] = r < rows && c * 16 < bytes ? *reinterpret_cast<const float4 *>(from + ((uint32_t)r * ld + (uint32_t)c * 16)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        float4 &x = *reinterpret_cast<float4 *>(store_chunk(st, t * 8 + (lane >> 3), c));
+        x = make_float4(x.x + v[t].x, x.y + v[t].y, x.z + v[t].z, x.w + v[t].w);
+    }
+}
+
+// Registers 4 q to 4 q + 3 of two 32 x 32 tiles side by side along m (h = 0, 1) as 16-bit numbers: one row of 128 bytes to a lane
+// pair.
+__device__ __forceinline__ void put16(int lane, char *st, int h, int q, uint32_t lo, uint32_t hi) {
+    *reinterpret_cast<uint2 *>(store_chunk(st, lane & 31, h * 4 + q) + 8 * (lane >> 5)) = make_uint2(lo, hi);
+}
+// The same of one tile as fp32 numbers.
+__device__ __forceinline__ void put32(int lane, char *st, int q, const float (&x)[4]) {
+    *reinterpret_cast<float4 *>(store_chunk(st, lane & 31, 2 * q + (lane >> 5))) = make_float4(x[0], x[1], x[2], x[3]);
+}
+
 // Whether a product takes operands with this row pitch: offsets within a tile of 256 rows stay below 2^31.
 inline bool pitch_fits(int64_t ld_bytes) { return ld_bytes > 0 && ld_bytes <= (1 << 23); }
 
 // What becomes of a product: C[n][m] -> 2^e row[n] C[n][m], rounded to dt, y rows ldy elements apart.  e = base + sum of
-// sign[i] exps[i]; a row factor of 0 makes zeros of whatever the row holds.  With acc (fp32 [splits][rows][cols]) the parts
-// of a split contraction go there as they are, added to what is there with `add`; finish() turns them into y.
+// sign[i] exps[i]; a row factor of 0 makes zeros of whatever the row holds.  With acc (fp32 [splits][rows][ldp], ldp columns_of
+// the columns) the parts of a split contraction go there as they are, added to what is there with `add`; finish() turns them
+// into y.
 struct Result {
     void *y;
     int64_t ldy;
@@ -332,8 +403,10 @@ struct Result {
     const int *exps;
     int base, sign[3];
     float *acc;
+    int64_t ldp;
     int add;
 };
+inline int64_t columns_of(int64_t cols) { return (cols + 3) / 4 * 4; }  // whole 16 bytes
 
 enum : int { BIG = 0, MID = 1, FEW = 2, ONE = 3 };
 struct Plan {

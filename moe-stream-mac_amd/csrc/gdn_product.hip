@@ -4,83 +4,101 @@
 namespace gdn {
 namespace mm {
 
-// Lanes hold rows of the result and registers its columns: four consecutive columns to a store.
-template <class S, bool F16, bool ACC>
+enum : int { OUT16 = 0, OUT32 = 1, PARTS = 2 };
+
+template <class S, bool F16, int KIND>
 __global__ __launch_bounds__(S::NT, S::WAVES_EU) void product_kernel(const Args g, const Result r) {
-    __shared__ __attribute__((aligned(16))) char lds[S::LDS];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, wm = w / S::WN, wn = w % S::WN;
-    products<S, F16>(g, lds, [&](int tm, int tn, const acc_t(&acc)[S::TM][S::TN]) {
-        const int64_t m0 = (int64_t)tm * S::BM + wm * (S::BM / S::WM) + 4 * (lane >> 5);
-        const int64_t n0 = (int64_t)tn * S::BN + wn * (S::BN / S::WN) + (lane & 31);
-        const int e = ACC ? 0 : exponent_of(r);
+    __shared__ __attribute__((aligned(16))) char lds[S::LDS + S::STORE];
+    const int w = wave_index(), wm = w / S::WN, wn = w % S::WN;
+    char *st = lds + S::LDS + w * 4096;
+    products<S, F16>(g, lds, [&](int tm, int tn, acc_t(&acc)[S::TM][S::TN]) {
+        const int lane = lane_here();
+        const int64_t m0 = (int64_t)tm * S::BM + wm * (S::BM / S::WM), n0 = (int64_t)tn * S::BN + wn * (S::BN / S::WN);
+        const int e = KIND == PARTS ? 0 : exponent_of(r);
 #pragma unroll
         for (int j = 0; j < S::TN; ++j) {
-            const int64_t n = n0 + 32 * j;
-            if (n >= g.b.rows) continue;
+            const int64_t n = n0 + 32 * j, rows = g.b.rows - n;
+            if (rows <= 0) break;
             float f = 1.f;
-            if constexpr (!ACC) f = r.row ? r.row[n] : 1.f;
+            if constexpr (KIND != PARTS)
+                if (r.row) f = r.row[n + min((int64_t)(lane & 31), rows - 1)];
+            const auto scaled = [&](float x) { return f == 0.f ? 0.f : ldexpf(x, e) * f; };
+            if constexpr (KIND == OUT16) {
 #pragma unroll
-            for (int i = 0; i < S::TM; ++i)
+                for (int i = 0; i < S::TM; i += 2) {
+                    const int64_t m = m0 + 32 * i;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int64_t m = m0 + 32 * i + 8 * q;
-                    float x[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                    if constexpr (ACC) {
-                        float *to = r.acc + ((int64_t)blockIdx.z * g.b.rows + n) * g.a.rows + m;
-                        if (m + 3 < g.a.rows && g.a.rows % 4 == 0) {
-                            float4 v = make_float4(x[0], x[1], x[2], x[3]);
-                            if (r.add) {
-                                const float4 o = *reinterpret_cast<const float4 *>(to);
-                                v = make_float4(o.x + v.x, o.y + v.y, o.z + v.z, o.w + v.w);
-                            }
-                            *reinterpret_cast<float4 *>(to) = v;
-                        } else {
-                            for (int k = 0; k < 4; ++k)
-                                if (m + k < g.a.rows) to[k] = r.add ? to[k] + x[k] : x[k];
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const acc_t &x = acc[i + h][j];
+                            put16(lane, st, h, q, ops::pack2_cvt(scaled(x[4 * q]), scaled(x[4 * q + 1]), r.dt),
+                                  ops::pack2_cvt(scaled(x[4 * q + 2]), scaled(x[4 * q + 3]), r.dt));
                         }
+                    store_rows(lane, st, static_cast<char *>(r.y) + (n * r.ldy + m) * 2, (uint32_t)(r.ldy * 2), rows, (g.a.rows - m) * 2, 2);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < S::TM; ++i) {
+                    const int64_t m = m0 + 32 * i;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        float x[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) x[k] = KIND == PARTS ? acc[i][j][4 * q + k] : scaled(acc[i][j][4 * q + k]);
+                        put32(lane, st, q, x);
+                    }
+                    if constexpr (KIND == OUT32) {
+                        store_rows(lane, st, static_cast<char *>(r.y) + (n * r.ldy + m) * 4, (uint32_t)(r.ldy * 4), rows, (g.a.rows - m) * 4, 4);
                     } else {
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) x[k] = f == 0.f ? 0.f : ldexpf(x[k], e) * f;
-                        const int64_t at = n * r.ldy + m;
-                        if (m + 3 < g.a.rows && r.ldy % 4 == 0) {
-                            store4_from_f32(r.y, at, make_float4(x[0], x[1], x[2], x[3]), r.dt);
-                        } else {
-                            for (int k = 0; k < 4; ++k)
-                                if (m + k < g.a.rows) store_from_f32(r.y, at + k, x[k], r.dt);
-                        }
+                        char *to = reinterpret_cast<char *>(r.acc + ((int64_t)blockIdx.z * g.b.rows + n) * r.ldp + m);
+                        if (r.add) add_rows(lane, st, to, (uint32_t)(r.ldp * 4), rows, (r.ldp - m) * 4);
+                        store_rows(lane, st, to, (uint32_t)(r.ldp * 4), rows, (r.ldp - m) * 4, 4);
                     }
                 }
+            }
         }
     });
 }
 
 constexpr int NT = 256;
 
+// Four columns to a thread.
+template <int DT>
 __global__ __launch_bounds__(NT) void finish_kernel(const Result r, int splits, int64_t rows, int64_t cols) {
-    const int64_t i = (block_index() * NT + threadIdx.x) * 4, size = rows * cols;
-    if (i >= size) return;
+    const int64_t per = r.ldp / 4, i = block_index() * NT + threadIdx.x, n = i / per, m = (i - n * per) * 4;
+    if (n >= rows) return;
     const int e = exponent_of(r);
-    for (int64_t k = i; k < min(i + 4, size); ++k) {
-        float s = 0.f;
-        for (int z = 0; z < splits; ++z) s += r.acc[z * size + k];
-        const int64_t n = k / cols;
-        const float f = r.row ? r.row[n] : 1.f;
-        store_from_f32(r.y, n * r.ldy + (k - n * cols), f == 0.f ? 0.f : ldexpf(s, e) * f, r.dt);
+    const float f = r.row ? r.row[n] : 1.f;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int z = 0; z < splits; ++z) {
+        const float4 v = *reinterpret_cast<const float4 *>(r.acc + (z * rows + n) * r.ldp + m);
+        s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s[k] = f == 0.f ? 0.f : ldexpf(s[k], e) * f;
+    ops::store_first<4, DT>(r.y, n * r.ldy + m, cols - m, s);
 }
 
 void finish(const Result &r, int splits, int64_t rows, int64_t cols, hipStream_t st) {
     Timed tm("product_join", st);
-    hipLaunchKernelGGL(finish_kernel, grid_of((rows * cols + 4 * NT - 1) / (4 * NT)), dim3(NT), 0, st, r, splits, rows, cols);
+    const dim3 grid = grid_of((rows * (r.ldp / 4) + NT - 1) / NT), block(NT);
+    if (r.dt == DT_F32) hipLaunchKernelGGL((finish_kernel<DT_F32>), grid, block, 0, st, r, splits, rows, cols);
+    else if (r.dt == DT_BF16) hipLaunchKernelGGL((finish_kernel<DT_BF16>), grid, block, 0, st, r, splits, rows, cols);
+    else hipLaunchKernelGGL((finish_kernel<DT_F16>), grid, block, 0, st, r, splits, rows, cols);
 }
 
+template <class S, bool F16>
+static void launch(Args &g, int splits, const Result &r, hipStream_t st) {
+    const dim3 grid = tiles_of<S>(g, splits);
+    if (r.acc) hipLaunchKernelGGL((product_kernel<S, F16, PARTS>), grid, dim3(S::NT), 0, st, g, r);
+    else if (r.dt == DT_F32) hipLaunchKernelGGL((product_kernel<S, F16, OUT32>), grid, dim3(S::NT), 0, st, g, r);
+    else hipLaunchKernelGGL((product_kernel<S, F16, OUT16>), grid, dim3(S::NT), 0, st, g, r);
+}
 template <class S>
 static void launch(Args &g, bool f16, int splits, const Result &r, hipStream_t st) {
-    const dim3 grid = tiles_of<S>(g, splits);
-    if (f16 && r.acc) hipLaunchKernelGGL((product_kernel<S, true, true>), grid, dim3(S::NT), 0, st, g, r);
-    else if (f16) hipLaunchKernelGGL((product_kernel<S, true, false>), grid, dim3(S::NT), 0, st, g, r);
-    else if (r.acc) hipLaunchKernelGGL((product_kernel<S, false, true>), grid, dim3(S::NT), 0, st, g, r);
-    else hipLaunchKernelGGL((product_kernel<S, false, false>), grid, dim3(S::NT), 0, st, g, r);
+    if (f16) launch<S, true>(g, splits, r, st);
+    else launch<S, false>(g, splits, r, st);
 }
 
 void multiply(Args g, bool f16, const Plan &p, const Result &r, hipStream_t st) {

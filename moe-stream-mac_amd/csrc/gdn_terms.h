@@ -16,7 +16,7 @@ struct Source {
     int64_t ignore;
 };
 
-constexpr int PARTS = 256;  // partial maxima of one matrix
+constexpr int PARTS = 512;  // partial maxima of one matrix
 
 // Elements of a row of `cols`, filled up to whole blocks of the contraction.
 inline int64_t padded(int64_t cols) { return (cols + 63) / 64 * 64; }

@@ -26,23 +26,33 @@ __device__ __forceinline__ float magnitude(float x) {
     return a <= 3.4028234e38f ? a : 0.f;  // neither infinite nor NaN
 }
 
-template <int V>
-__global__ __launch_bounds__(NT) void maxima_kernel(const Source s, float *part) {
-    __shared__ float red[NT / 64];
-    const int64_t per = (s.cols + V - 1) / V, total = s.rows * per;
+// A wave to a row, 2048 elements at a time.
+template <int DT>
+__global__ __launch_bounds__(1024) void maxima_kernel(const Source s, float *part) {
+    constexpr int WAVES = 16, U = 4;
+    __shared__ float red[WAVES];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float m = 0.f;
-    for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < total; i += (int64_t)PARTS * NT) {
-        const int64_t r = i / per, c = (i - r * per) * V;
+    for (int64_t r = blockIdx.x * WAVES + w; r < s.rows; r += PARTS * WAVES) {
         if (skipped(s, r)) continue;
-        float x[V];
-        ops::loadv<V>(s.p, r * s.ld + c, s.dt, x);
+        for (int64_t c = lane * 8; c < s.cols; c += U * 512) {
+            float x[U][8];
 #pragma unroll
-        for (int j = 0; j < V; ++j) m = fmaxf(m, magnitude(x[j]));
+            for (int u = 0; u < U; ++u) ops::load_first<8, DT>(s.p, r * s.ld + c + u * 512, s.cols - c - u * 512, x[u]);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = fmaxf(m, magnitude(x[u][j]));
+        }
     }
     m = wave_max(m);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
+    if (lane == 0) red[w] = m;
     __syncthreads();
-    if (threadIdx.x == 0) part[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int i = 1; i < WAVES; ++i) m = fmaxf(m, red[i]);
+        part[blockIdx.x] = m;
+    }
 }
 
 __global__ __launch_bounds__(64) void exponents_kernel(const float *part, int top, int *exps) {
@@ -81,20 +91,17 @@ __device__ __forceinline__ uint4 pack8(const uint16_t (&b)[8]) {
 }
 
 // Eight elements of a row to a thread.
-template <bool F16, bool WIDE>
+template <bool F16, int DT>
 __global__ __launch_bounds__(NT) void terms_kernel(const Source s, int nterms, const int *exps, int which, uint16_t *dst,
                                                    int64_t kp) {
-    const int64_t i = block_index() * NT + threadIdx.x, per = kp / 8, r = i / per, c = (i - r * per) * 8;
+    const int64_t i = block_index() * NT + threadIdx.x;
+    const uint32_t per = (uint32_t)(kp / 8);
+    const int64_t r = i >> 32 ? i / per : (uint32_t)i / per, c = (i - r * per) * 8;
     if (r >= s.rows) return;
     const int e = exps ? exps[which] : 0;
     float x[8];
     const bool none = skipped(s, r);
-    if (WIDE && c + 8 <= s.cols) {
-        ops::loadv<8>(s.p, r * s.ld + c, s.dt, x);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = c + j < s.cols ? load_as_f32(s.p, r * s.ld + c + j, s.dt) : 0.f;
-    }
+    ops::load_first<8, DT>(s.p, r * s.ld + c, s.cols - c, x);
 #pragma unroll
     for (int j = 0; j < 8; ++j) x[j] = none ? 0.f : ldexpf(x[j], e);
     for (int t = 0; t < nterms; ++t) {
@@ -106,7 +113,7 @@ __global__ __launch_bounds__(NT) void terms_kernel(const Source s, int nterms, c
 }
 
 // 64 x 64 elements to a workgroup, turned over in LDS.
-template <bool F16, bool WIDE>
+template <bool F16, int DT>
 __global__ __launch_bounds__(NT) void across_kernel(const Source s, int slots, const int *exps, int which, uint16_t *dst,
                                                     int64_t kp, int64_t tiles_c, int64_t tiles) {
     __shared__ float tile[64][65];
@@ -120,12 +127,7 @@ __global__ __launch_bounds__(NT) void across_kernel(const Source s, int slots, c
         const int64_t r = r0 + rl, c = c0 + cl;
         float x[8];
         const bool live = r < s.rows && !skipped(s, r);
-        if (WIDE && live && c + 8 <= s.cols) {
-            ops::loadv<8>(s.p, r * s.ld + c, s.dt, x);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = live && c + j < s.cols ? load_as_f32(s.p, r * s.ld + c + j, s.dt) : 0.f;
-        }
+        ops::load_first<8, DT>(s.p, r * s.ld + c, live ? s.cols - c : 0, x);
 #pragma unroll
         for (int j = 0; j < 8; ++j) tile[rl][cl + j] = ldexpf(x[j], e);
     }
@@ -151,30 +153,35 @@ __global__ __launch_bounds__(NT) void across_kernel(const Source s, int slots, c
     }
 }
 
-static bool wide(const Source &s) { return s.ld % 8 == 0 && aligned_to(s.p, 16); }
-
-void maxima(const Source &s, float *part, hipStream_t st) {
+void maxima(const Source &s0, float *part, hipStream_t st) {
     Timed tm("maxima", st);
-    if (wide(s) && s.cols % 8 == 0)
-        hipLaunchKernelGGL((maxima_kernel<8>), dim3(PARTS), dim3(NT), 0, st, s, part);
-    else
-        hipLaunchKernelGGL((maxima_kernel<1>), dim3(PARTS), dim3(NT), 0, st, s, part);
+    constexpr int64_t LONG = 8192;
+    Source s = s0;
+    if (s.ld == s.cols && !s.targets && s.rows * s.cols % LONG == 0) {  // rows in one piece: of any length
+        s.rows = s.rows * s.cols / LONG;
+        s.ld = s.cols = LONG;
+    }
+    const dim3 grid(PARTS), block(1024);
+    if (s.dt == DT_F32) hipLaunchKernelGGL((maxima_kernel<DT_F32>), grid, block, 0, st, s, part);
+    else if (s.dt == DT_BF16) hipLaunchKernelGGL((maxima_kernel<DT_BF16>), grid, block, 0, st, s, part);
+    else hipLaunchKernelGGL((maxima_kernel<DT_F16>), grid, block, 0, st, s, part);
 }
 
 void exponents(const float *part, int n, int top, int *exps, hipStream_t st) {
     hipLaunchKernelGGL(exponents_kernel, dim3(n), dim3(64), 0, st, part, top, exps);
 }
 
-#define GDN_TERMS(KERNEL, ...)                                                                                        \
-    if (f16 && w) hipLaunchKernelGGL((KERNEL<true, true>), grid, dim3(NT), 0, st, __VA_ARGS__);                        \
-    else if (f16) hipLaunchKernelGGL((KERNEL<true, false>), grid, dim3(NT), 0, st, __VA_ARGS__);                       \
-    else if (w) hipLaunchKernelGGL((KERNEL<false, true>), grid, dim3(NT), 0, st, __VA_ARGS__);                         \
-    else hipLaunchKernelGGL((KERNEL<false, false>), grid, dim3(NT), 0, st, __VA_ARGS__)
+#define GDN_TERMS_OF(KERNEL, F16, ...)                                                                                \
+    if (s.dt == DT_F32) hipLaunchKernelGGL((KERNEL<F16, DT_F32>), grid, dim3(NT), 0, st, __VA_ARGS__);                 \
+    else if (s.dt == DT_BF16) hipLaunchKernelGGL((KERNEL<F16, DT_BF16>), grid, dim3(NT), 0, st, __VA_ARGS__);          \
+    else hipLaunchKernelGGL((KERNEL<F16, DT_F16>), grid, dim3(NT), 0, st, __VA_ARGS__)
+#define GDN_TERMS(KERNEL, ...)                             \
+    if (f16) { GDN_TERMS_OF(KERNEL, true, __VA_ARGS__); }   \
+    else { GDN_TERMS_OF(KERNEL, false, __VA_ARGS__); }
 
 void terms(const Source &s, int nterms, bool f16, const int *exps, int which, void *dst, hipStream_t st) {
     Timed tm("terms", st);
     const int64_t kp = padded(s.cols);
-    const bool w = wide(s);
     const dim3 grid = grid_of((s.rows * (kp / 8) + NT - 1) / NT);
     GDN_TERMS(terms_kernel, s, nterms, exps, which, static_cast<uint16_t *>(dst), kp);
 }
@@ -182,11 +189,11 @@ void terms(const Source &s, int nterms, bool f16, const int *exps, int which, vo
 void terms_across(const Source &s, int nterms, bool f16, const int *exps, int which, void *dst, hipStream_t st) {
     Timed tm("terms_across", st);
     const int64_t kp = padded(s.rows), tc = (s.cols + 63) / 64, tiles = kp / 64 * tc;
-    const bool w = wide(s);
     const dim3 grid = grid_of(tiles);
     GDN_TERMS(across_kernel, s, across_slots(nterms), exps, which, static_cast<uint16_t *>(dst), kp, tc, tiles);
 }
 #undef GDN_TERMS
+#undef GDN_TERMS_OF
 
 }  // namespace mm
 }  // namespace gdn

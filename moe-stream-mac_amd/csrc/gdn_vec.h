@@ -107,5 +107,85 @@ __device__ __forceinline__ void storev(void *p, size_t i, int dt, const float (&
     }
 }
 
+// The same from any element on: the card takes vector accesses at every address, and 16 bytes across a border cost less than
+// element by element.
+template <int V, int DT>
+__device__ __forceinline__ void loadv_any(const void *p, int64_t i, float (&o)[V]) {
+    static_assert(V == 4 || V == 8, "V is 4 or 8");
+    typedef uint32_t w4 __attribute__((ext_vector_type(4)));
+    typedef uint32_t w2 __attribute__((ext_vector_type(2)));
+    typedef w4 any4 __attribute__((aligned(2)));
+    typedef w2 any2 __attribute__((aligned(2)));
+    if constexpr (DT == DT_F32) {
+#pragma unroll
+        for (int h = 0; h < V / 4; ++h) {
+            const w4 u = *reinterpret_cast<const any4 *>(static_cast<const float *>(p) + i + 4 * h);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[4 * h + j] = __uint_as_float(u[j]);
+        }
+    } else {
+        uint32_t w[V / 2];
+        if constexpr (V == 8) {
+            const w4 u = *reinterpret_cast<const any4 *>(static_cast<const uint16_t *>(p) + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = u[j];
+        } else {
+            const w2 u = *reinterpret_cast<const any2 *>(static_cast<const uint16_t *>(p) + i);
+            w[0] = u[0];
+            w[1] = u[1];
+        }
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) {
+            o[2 * j] = DT == DT_BF16 ? __uint_as_float(w[j] << 16) : half_bits_to_f32(w[j]);
+            o[2 * j + 1] = DT == DT_BF16 ? __uint_as_float(w[j] & 0xffff0000u) : half_bits_to_f32(w[j] >> 16);
+        }
+    }
+}
+
+template <int V, int DT>
+__device__ __forceinline__ void storev_any(void *p, int64_t i, const float (&o)[V]) {
+    static_assert(V == 4 || V == 8, "V is 4 or 8");
+    typedef uint32_t w4 __attribute__((ext_vector_type(4)));
+    typedef uint32_t w2 __attribute__((ext_vector_type(2)));
+    typedef w4 any4 __attribute__((aligned(2)));
+    typedef w2 any2 __attribute__((aligned(2)));
+    if constexpr (DT == DT_F32) {
+#pragma unroll
+        for (int h = 0; h < V / 4; ++h)
+            *reinterpret_cast<any4 *>(static_cast<float *>(p) + i + 4 * h) =
+                w4{__float_as_uint(o[4 * h]), __float_as_uint(o[4 * h + 1]), __float_as_uint(o[4 * h + 2]),
+                   __float_as_uint(o[4 * h + 3])};
+    } else {
+        uint32_t w[V / 2];
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) w[j] = pack2_cvt(o[2 * j], o[2 * j + 1], DT);
+        if constexpr (V == 8)
+            *reinterpret_cast<any4 *>(static_cast<uint16_t *>(p) + i) = w4{w[0], w[1], w[2], w[3]};
+        else
+            *reinterpret_cast<any2 *>(static_cast<uint16_t *>(p) + i) = w2{w[0], w[1]};
+    }
+}
+
+// The first n of V elements (n may be V or more, or less than one); the rest are zeros, or not stored.
+template <int V, int DT>
+__device__ __forceinline__ void load_first(const void *p, int64_t i, int64_t n, float (&o)[V]) {
+    if (n >= V) {
+        loadv_any<V, DT>(p, i, o);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = j < n ? load_as_f32(p, i + j, DT) : 0.f;
+    }
+}
+template <int V, int DT>
+__device__ __forceinline__ void store_first(void *p, int64_t i, int64_t n, const float (&o)[V]) {
+    if (n >= V) {
+        storev_any<V, DT>(p, i, o);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (j < n) store_from_f32(p, i + j, o[j], DT);
+    }
+}
+
 }  // namespace ops
 }  // namespace gdn
