@@ -61,36 +61,38 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void stat_kernel(const Args g, 
         const int e = SCALED ? -(a.exps[E_X] + a.exps[E_W]) : 0;
 #pragma unroll
         for (int j = 0; j < S::TN; ++j) {
-            const int64_t n = (int64_t)tn * S::BN + wn * (S::BN / S::WN) + 32 * j + (lane & 31);
+            const int64_t n = (int64_t)tn * S::BN + wn * (S::BN / S::WN) + 16 * j + (lane & 15);
             const bool live = n < a.N;
             float mx = -INFINITY;
 #pragma unroll
             for (int i = 0; i < S::TM; ++i)
 #pragma unroll
-                for (int q = 0; q < 16; ++q) {
+                for (int q = 0; q < 4; ++q) {
                     if constexpr (SCALED) acc[i][j][q] = ldexpf(acc[i][j][q], e);
-                    if (words < S::BM / S::WM && 32 * i + 8 * (q / 4) + 4 * (lane >> 5) + q % 4 >= words) acc[i][j][q] = -INFINITY;
+                    if (words < S::BM / S::WM && 16 * i + 4 * (lane >> 4) + q >= words) acc[i][j][q] = -INFINITY;
                     mx = fmaxf(mx, acc[i][j][q]);
                 }
+            mx = fmaxf(mx, lane_xor16(mx));
             mx = fmaxf(mx, lane_xor32(mx));
             const float ref = mx == -INFINITY ? 0.f : mx;
             float s = 0.f;
 #pragma unroll
             for (int i = 0; i < S::TM; ++i)
 #pragma unroll
-                for (int q = 0; q < 16; ++q) s += __builtin_amdgcn_exp2f((acc[i][j][q] - ref) * LOG2E);
+                for (int q = 0; q < 4; ++q) s += __builtin_amdgcn_exp2f((acc[i][j][q] - ref) * LOG2E);
+            s += lane_xor16(s);
             s += lane_xor32(s);
-            if (live && lane < 32) a.part[(int64_t)(a.part0 + tm * S::WM + wm) * a.N + n] = make_float2(mx, s);
+            if (live && lane < 16) a.part[(int64_t)(a.part0 + tm * S::WM + wm) * a.N + n] = make_float2(mx, s);
             const int64_t t = live ? a.targets[n] - a.v0 - m0 : -1;
-            const bool here = t >= 0 && t < words && ((t >> 2 & 1) == (lane >> 5));
+            const bool here = t >= 0 && t < words && ((t >> 2 & 3) == (lane >> 4));
             if (__any(here)) {
-                const int tl = here ? (int)t - 4 * (lane >> 5) : -1;
+                const int tl = here ? (int)t - 4 * (lane >> 4) : -1;
                 float z = 0.f;
 #pragma unroll
                 for (int i = 0; i < S::TM; ++i)
 #pragma unroll
-                    for (int q = 0; q < 16; ++q)
-                        if (tl == 32 * i + 8 * (q / 4) + q % 4) z = acc[i][j][q];
+                    for (int q = 0; q < 4; ++q)
+                        if (tl == 16 * i + q) z = acc[i][j][q];
                 if (here) a.zt[n] = z;
             }
         }
@@ -227,44 +229,44 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
         float r[S::TN];
 #pragma unroll
         for (int j = 0; j < S::TN; ++j) {
-            const int64_t n = n0 + 32 * j + (lane & 31);
+            const int64_t n = n0 + 16 * j + (lane & 15);
             const bool live = n < a.N;
             const float2 st = live ? a.stat[n] : make_float2(0.f, 0.f);
             r[j] = DW && live ? ldexpf(a.d[n], a.exps[E_D]) : 0.f;
             const float inv = st.y * (float)(1 << SHIFT);
-            const int64_t hot = live ? a.targets[n] - a.v0 - m0 - 4 * (lane >> 5) : -1;
+            const int64_t hot = live ? a.targets[n] - a.v0 - m0 - 4 * (lane >> 4) : -1;
 #pragma unroll
             for (int i = 0; i < S::TM; ++i)
 #pragma unroll
-                for (int q = 0; q < 16; ++q) {
-                    const int m = 32 * i + 8 * (q / 4) + q % 4;
+                for (int q = 0; q < 4; ++q) {
+                    const int m = 16 * i + q;
                     float z = acc[i][j][q];
                     if constexpr (TERMS > 1) z = ldexpf(z, e);
                     float x = __builtin_amdgcn_exp2f((z - st.x) * LOG2E) * inv;
                     if (hot == m) x -= (float)(1 << SHIFT);
-                    if (words < S::BM / S::WM && m + 4 * (lane >> 5) >= words) x = 0.f;
+                    if (words < S::BM / S::WM && m + 4 * (lane >> 4) >= words) x = 0.f;
                     acc[i][j][q] = TERMS > 1 ? as_rounded(x) : x;
                 }
         }
         if constexpr (DX) {
 #pragma unroll
-            for (int j = 0; j < S::TN; ++j) {
-                const int64_t n = n0 + 32 * j, rows = a.N - n;
+            for (int j = 0; j < S::TN; j += 2) {
+                const int64_t n = n0 + 16 * j, rows = a.N - n;
                 if (rows <= 0) break;
 #pragma unroll
-                for (int i = 0; i < S::TM; i += 2) {
-                    const int64_t m = m0 + 32 * i;
+                for (int i = 0; i < S::TM; i += 4) {
+                    const int64_t m = m0 + 16 * i;
                     if (m >= a.kp) break;
 #pragma unroll
                     for (int t = 0; t < TERMS; ++t) {
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
+                        for (int ii = 0; ii < 4; ++ii)
 #pragma unroll
-                            for (int q = 0; q < 4; ++q) {
+                            for (int jj = 0; jj < 2; ++jj) {
                                 float y[4];
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) y[k] = t ? left_of(acc[i + h][j][4 * q + k]) : acc[i + h][j][4 * q + k];
-                                put16(lane, store, h, q, ops::pack2(y[0], y[1], DT_F16), ops::pack2(y[2], y[3], DT_F16));
+                                for (int k = 0; k < 4; ++k) y[k] = t ? left_of(acc[i + ii][j + jj][k]) : acc[i + ii][j + jj][k];
+                                put16(lane, store, ii, jj, ops::pack2(y[0], y[1], DT_F16), ops::pack2(y[2], y[3], DT_F16));
                             }
                         store_rows(lane, store, reinterpret_cast<char *>(a.p + n * (TERMS * a.kp) + t * a.kp + m),
                                    (uint32_t)(TERMS * a.kp * 2), rows, (a.kp - m) * 2, 2);
@@ -273,37 +275,39 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
             }
         }
         if constexpr (DW) {
-            constexpr int W = S::TN < 2 ? 1 : 2;  // tiles of tokens side by side
+            constexpr int W = S::TN < 4 ? 2 : 4;  // tiles of tokens side by side
 #pragma unroll
             for (int j = 0; j < S::TN; j += W) {
-                const int64_t n = n0 + 32 * j;
+                const int64_t n = n0 + 16 * j;
                 if (n >= a.np) break;
 #pragma unroll
-                for (int i = 0; i < S::TM; ++i) {
-                    if (32 * i >= words) break;
+                for (int i = 0; i < S::TM; i += 2) {
+                    if (16 * i >= words) break;
 #pragma unroll
                     for (int t = 0; t < TERMS; ++t) {
 #pragma unroll
-                        for (int h = 0; h < W; ++h)
+                        for (int ii = 0; ii < 2; ++ii)
 #pragma unroll
-                            for (int q = 0; q < 16; q += 2) {
-                                float y[2];
+                            for (int h = 0; h < W; ++h)
 #pragma unroll
-                                for (int k = 0; k < 2; ++k) {
-                                    y[k] = r[j + h] == 0.f ? 0.f : acc[i][j + h][q + k] * r[j + h];
-                                    if (TERMS > 1) y[k] = as_rounded(y[k]);
-                                    if (t) y[k] = left_of(y[k]);
+                                for (int q = 0; q < 4; q += 2) {
+                                    float y[2];
+#pragma unroll
+                                    for (int k = 0; k < 2; ++k) {
+                                        y[k] = r[j + h] == 0.f ? 0.f : acc[i + ii][j + h][q + k] * r[j + h];
+                                        if (TERMS > 1) y[k] = as_rounded(y[k]);
+                                        if (t) y[k] = left_of(y[k]);
+                                    }
+                                    // two words of a token become two tokens of a word, with the neighbouring lane
+                                    const uint32_t own = ops::pack2(y[0], y[1], DT_F16);
+                                    const uint32_t its = __builtin_amdgcn_update_dpp(0, (int)own, DPP_QUAD_1032, 0xF, 0xF, false);
+                                    const uint32_t v = lane & 1 ? (its >> 16) | (own & 0xffff0000u) : (own & 0xffffu) | (its << 16);
+                                    const int row = 16 * ii + 4 * (lane >> 4) + q + (lane & 1), col = 16 * h + (lane & 14);
+                                    *reinterpret_cast<uint32_t *>(store_chunk(store, row, col >> 3) + (col & 7) * 2) = v;
                                 }
-                                // two words of a token become two tokens of a word, with the neighbouring lane
-                                const uint32_t own = ops::pack2(y[0], y[1], DT_F16);
-                                const uint32_t its = __builtin_amdgcn_update_dpp(0, (int)own, DPP_QUAD_1032, 0xF, 0xF, false);
-                                const uint32_t v = lane & 1 ? (its >> 16) | (own & 0xffff0000u) : (own & 0xffffu) | (its << 16);
-                                const int row = 8 * (q / 4) + 4 * (lane >> 5) + q % 4 + (lane & 1), col = 32 * h + (lane & 30);
-                                *reinterpret_cast<uint32_t *>(store_chunk(store, row, col >> 3) + (col & 7) * 2) = v;
-                            }
                         const int64_t left = (a.np - n) * 2;
-                        store_rows(lane, store, reinterpret_cast<char *>(a.pt + (m0 + 32 * i) * (TERMS * a.np) + t * a.np + n),
-                                   (uint32_t)(TERMS * a.np * 2), words - 32 * i, left < W * 64 ? left : W * 64, 2);
+                        store_rows(lane, store, reinterpret_cast<char *>(a.pt + (m0 + 16 * i) * (TERMS * a.np) + t * a.np + n),
+                                   (uint32_t)(TERMS * a.np * 2), words - 16 * i, left < W * 32 ? left : W * 32, 2);
                     }
                 }
             }

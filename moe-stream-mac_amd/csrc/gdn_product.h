@@ -10,12 +10,16 @@
 // LDS read serves at once, fill all 64 banks (with r & 7 half of the read cycles were conflicts).  The global addresses are
 // permuted to that end, since LDS is filled in order.
 //
-// The barrier of a stage stands before its last quarter: by then that quarter's fragments are in registers, so after it
-// the stage's LDS may be overwritten and the next stage's first fragments are read under the last quarter's products.
-// Loads thus have three quarters of a stage to arrive, and no product waits for LDS.
+// The barrier of a stage stands in its middle: by then all of its fragments are in registers, so after it the stage's LDS may be
+// overwritten, and the next stage's fragments are read under the second half's products.  Loads thus have a whole stage to
+// arrive, and no product waits for LDS.
 //
-// Lanes hold the columns of an MFMA's result and registers its rows: A's rows (m) run over registers, B's (n) over lanes.
-// Sums over m, such as those of a softmax over words, stay within a lane and its partner 32 lanes on.
+// Lanes hold the columns of a matrix instruction's result and registers its rows: A's rows (m) run over registers, B's (n) over
+// lanes.  Sums over m, such as those of a softmax over words, stay within a lane and its three partners 16 lanes apart.
+//
+// Measured, bf16: 8192 x 2048 x 8192 1.48 PFLOP/s, 8192 x 8192 x 2048 1.40 (a large library product 1.53).  The card lowers its
+// clock under this load, to 1.9 GHz: with 32 x 32 x 16 instructions, which move twice the sums through registers, to 1.7 and
+// 1.39 PFLOP/s.
 #pragma once
 
 #include "gdn_common.h"
@@ -25,7 +29,7 @@
 namespace gdn {
 namespace mm {
 
-typedef float acc_t __attribute__((ext_vector_type(16)));
+typedef float acc_t __attribute__((ext_vector_type(4)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 hf8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
@@ -35,9 +39,9 @@ constexpr int BK = 64;
 template <bool F16>
 __device__ __forceinline__ acc_t mfma(u4 a, u4 b, acc_t c) {
     if constexpr (F16)
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(hf8, a), __builtin_bit_cast(hf8, b), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(hf8, a), __builtin_bit_cast(hf8, b), c, 0, 0, 0);
     else
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
 }
 
 // A matrix of `rows` rows, `ld` bytes apart, of `off[s]` bytes to the term that segment s takes.
@@ -58,13 +62,13 @@ struct Args {
 template <int BM_, int BN_, int WM_, int WN_, int PER_CU_>
 struct Shape {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NT = 64 * WM_ * WN_;
-    static constexpr int TM = BM / WM / 32, TN = BN / WN / 32;
+    static constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
     static constexpr int A_BYTES = BM * BK * 2, STAGE = (BM + BN) * BK * 2, LDS = 2 * STAGE;
     static constexpr int STORE = WM * WN * 4096;  // LDS through which a wave's results leave, 4 KB each
     static constexpr int RA = BM * 8 / NT, RB = BN * 8 / NT;  // 16-byte loads of a thread for a stage
     static constexpr int PER_CU = PER_CU_;
     static constexpr int WAVES_EU = PER_CU_ * NT / 256;
-    static_assert(RA >= 1 && RB >= 1 && TM % 2 == 0 && TN >= 1, "tile");
+    static_assert(RA >= 1 && RB >= 1 && TM % 4 == 0 && TN % 2 == 0 && TN >= 1, "tile");
 };
 // The lane, as a value that is worked out where it stands: what an epilogue derives from it would otherwise be kept in registers
 // through the whole product, which has none to spare.
@@ -172,22 +176,22 @@ __device__ __forceinline__ void stage_barrier() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// The fragments of a block: four steps of 16 along the contraction; A's rows in two halves.
+// The fragments of a block: two steps of 32 along the contraction; A's rows in two halves.
 template <class S>
 struct Frags {
     static constexpr int H = S::TM / 2;
-    u4 lo[4][H], hi[4][H], b[4][S::TN];
-    __device__ __forceinline__ void read_lo(const char *__restrict__ lds, const uint32_t (&at_a)[4], int k) {
+    u4 lo[2][H], hi[2][H], b[2][S::TN];
+    __device__ __forceinline__ void read_lo(const char *__restrict__ lds, const uint32_t (&at_a)[2], int k) {
 #pragma unroll
-        for (int i = 0; i < H; ++i) lo[k][i] = *reinterpret_cast<const u4 *>(lds + at_a[k] + i * 32 * BK * 2);
+        for (int i = 0; i < H; ++i) lo[k][i] = *reinterpret_cast<const u4 *>(lds + at_a[k] + i * 16 * BK * 2);
     }
-    __device__ __forceinline__ void read_hi(const char *__restrict__ lds, const uint32_t (&at_a)[4], int k) {
+    __device__ __forceinline__ void read_hi(const char *__restrict__ lds, const uint32_t (&at_a)[2], int k) {
 #pragma unroll
-        for (int i = 0; i < H; ++i) hi[k][i] = *reinterpret_cast<const u4 *>(lds + at_a[k] + (H + i) * 32 * BK * 2);
+        for (int i = 0; i < H; ++i) hi[k][i] = *reinterpret_cast<const u4 *>(lds + at_a[k] + (H + i) * 16 * BK * 2);
     }
-    __device__ __forceinline__ void read_b(const char *__restrict__ lds, const uint32_t (&at_b)[4], int k) {
+    __device__ __forceinline__ void read_b(const char *__restrict__ lds, const uint32_t (&at_b)[2], int k) {
 #pragma unroll
-        for (int j = 0; j < S::TN; ++j) b[k][j] = *reinterpret_cast<const u4 *>(lds + at_b[k] + j * 32 * BK * 2);
+        for (int j = 0; j < S::TN; ++j) b[k][j] = *reinterpret_cast<const u4 *>(lds + at_b[k] + j * 16 * BK * 2);
     }
     template <bool F16>
     __device__ __forceinline__ void mul_lo(acc_t (&acc)[S::TM][S::TN], int k) const {
@@ -205,74 +209,61 @@ struct Frags {
     }
 };
 
-// One step's products with LOADS loads and READS reads from LDS between them.
-template <class S, int LOADS, int READS>
-__device__ __forceinline__ void interleave() {
-    constexpr int PRODUCTS = Frags<S>::H * S::TN, L = (LOADS + PRODUCTS - 1) / PRODUCTS, R = (READS + PRODUCTS - 1) / PRODUCTS;
-#pragma unroll
-    for (int i = 0; i < PRODUCTS; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x020, L, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-}
-
-// First half of a block: the products of A's lower rows, while the rest of the block's fragments are read.
+// First half of a block: the products of A's lower rows, while the rest of the block's fragments are read, one between two
+// products, and the first product before them (its wait is for what the last half has read).
 template <class S, bool F16>
-__device__ __forceinline__ void first_half(const char *__restrict__ rd, const uint32_t (&at_a)[4], const uint32_t (&at_b)[4],
+__device__ __forceinline__ void first_half(const char *__restrict__ rd, const uint32_t (&at_a)[2], const uint32_t (&at_b)[2],
                                            Frags<S> &f, acc_t (&acc)[S::TM][S::TN]) {
+    constexpr int READS = S::TN + 2 * Frags<S>::H, PRODUCTS = Frags<S>::H * S::TN;
     f.template mul_lo<F16>(acc, 0);
-    __builtin_amdgcn_sched_barrier(0);
-    f.read_b(rd, at_b, 3);
+    f.read_b(rd, at_b, 1);
     f.read_hi(rd, at_a, 0);
     f.read_hi(rd, at_a, 1);
-    f.read_hi(rd, at_a, 2);
-    f.read_hi(rd, at_a, 3);
-    f.template mul_lo<F16>(acc, 1);
-    f.template mul_lo<F16>(acc, 2);
-    constexpr int READS = S::TN + 4 * Frags<S>::H, PRODUCTS = Frags<S>::H * S::TN;
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
 #pragma unroll
-    for (int i = 0; i < (READS + 1) / 2; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    for (int i = 0; i < READS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        if (i < PRODUCTS - 1) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
     }
-    __builtin_amdgcn_sched_group_barrier(0x008, 2 * PRODUCTS, 0);
+    __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
     __builtin_amdgcn_sched_barrier(0);
-    f.template mul_lo<F16>(acc, 3);
+    f.template mul_lo<F16>(acc, 1);
+    __builtin_amdgcn_sched_barrier(0);
 }
 
-// Second half: the products of A's upper rows, while the block after the next is loaded into this one's LDS and the
-// next one's fragments are read in the place of those that no product needs any more.  A load takes the memory pipe 16
-// cycles for each of the workgroup's waves, so loads stand between products: in one run they held the products up.
+// Second half: the products of A's upper rows, while the block after the next is loaded into this one's LDS and the next
+// one's fragments are read in the place of those that no product needs any more.  A load takes the memory pipe 16 cycles for
+// each of the workgroup's waves, so loads stand between products: in one run they held the products up.
 template <class S, bool F16>
 __device__ __forceinline__ void second_half(const char *__restrict__ rd, char *__restrict__ wr, const Loader<S> &ld,
-                                            const uint32_t (&at_a)[4], const uint32_t (&at_b)[4], Frags<S> &f,
+                                            const uint32_t (&at_a)[2], const uint32_t (&at_b)[2], Frags<S> &f,
                                             acc_t (&acc)[S::TM][S::TN]) {
-    constexpr int R = S::RA + S::RB;
-    ld.template load<0, R / 4>(wr);
+    constexpr int R = S::RA + S::RB, P = Frags<S>::H * S::TN, READS = 2 * Frags<S>::H;
+    ld.template load<0, R / 2>(wr);
     f.template mul_hi<F16>(acc, 0);
     f.read_lo(rd, at_a, 0);
-    f.read_lo(rd, at_a, 3);
-    interleave<S, R / 4, 2 * Frags<S>::H>();
-    ld.template load<R / 4, R / 2>(wr);
-    f.template mul_hi<F16>(acc, 1);
-    f.read_b(rd, at_b, 0);
     f.read_lo(rd, at_a, 1);
-    interleave<S, R / 2 - R / 4, Frags<S>::H + S::TN>();
-    ld.template load<R / 2, 3 * R / 4>(wr);
-    f.template mul_hi<F16>(acc, 2);
-    f.read_b(rd, at_b, 1);
-    f.read_lo(rd, at_a, 2);
-    interleave<S, 3 * R / 4 - R / 2, Frags<S>::H + S::TN>();
-    ld.template load<3 * R / 4, R>(wr);
-    f.template mul_hi<F16>(acc, 3);
-    f.read_b(rd, at_b, 2);
-    interleave<S, R - 3 * R / 4, S::TN>();
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x020, (R / 2 + P / 2 - 1) / (P / 2), 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, (READS + P / 2 - 1) / (P / 2), 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    ld.template load<R / 2, R>(wr);
+    f.read_b(rd, at_b, 0);
+    f.template mul_hi<F16>(acc, 1);
+#pragma unroll
+    for (int i = 0; i < P / 2; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x020, (R - R / 2 + P / 2 - 1) / (P / 2), 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // Forms the workgroup's tiles and hands each to epilogue(tm, tn, acc).
-// acc[i][j]: rows m = 32 i + 8 (q / 4) + 4 (lane / 32) + q % 4 of this wave's part for register q, column n = 32 j + lane % 32.
+// acc[i][j]: rows m = 16 i + 4 (lane / 16) + q of this wave's part for register q, column n = 16 j + lane % 16.
 template <class S, bool F16, class E>
 __device__ __forceinline__ void products(const Args &g, char *lds, E &&epilogue) {
     const int lane = threadIdx.x & 63, w = wave_index(), wm = w / S::WN, wn = w % S::WN;
@@ -285,12 +276,12 @@ __device__ __forceinline__ void products(const Args &g, char *lds, E &&epilogue)
     ld.w = w;
     if (ld.tile >= ld.tiles || blocks == 0) return;
     ld.start(g, first, end);
-    uint32_t at_a[4], at_b[4];
+    uint32_t at_a[2], at_b[2];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const uint32_t c = ((k * 2 + (lane >> 5)) ^ (lane >> 1 & 7)) << 4;
-        at_a[k] = (wm * (S::BM / S::WM) + (lane & 31)) * BK * 2 + c;
-        at_b[k] = S::A_BYTES + (wn * (S::BN / S::WN) + (lane & 31)) * BK * 2 + c;
+    for (int k = 0; k < 2; ++k) {
+        const uint32_t c = ((k * 4 + (lane >> 4)) ^ (lane >> 1 & 7)) << 4;
+        at_a[k] = (wm * (S::BM / S::WM) + (lane & 15)) * BK * 2 + c;
+        at_b[k] = S::A_BYTES + (wn * (S::BN / S::WN) + (lane & 15)) * BK * 2 + c;
     }
     char *cur = lds, *other = lds + S::STAGE;
     ld.template load<0, S::RA + S::RB>(cur);
@@ -305,13 +296,13 @@ __device__ __forceinline__ void products(const Args &g, char *lds, E &&epilogue)
 #pragma unroll
             for (int j = 0; j < S::TN; ++j)
 #pragma unroll
-                for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
+                for (int q = 0; q < 4; ++q) acc[i][j][q] = 0.f;
         // read anew for each tile, so that their registers are free while results are written
         Frags<S> f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 2; ++k) {
             f.read_lo(cur, at_a, k);
-            if (k < 3) f.read_b(cur, at_b, k);
+            if (k < 1) f.read_b(cur, at_b, k);
         }
         for (int n = 0; n < blocks; ++n) {
             first_half<S, F16>(cur, at_a, at_b, f, acc);
@@ -378,14 +369,14 @@ __device__ __forceinline__ void add_rows(int lane, char *st, const char *from, u
     }
 }
 
-// Registers 4 q to 4 q + 3 of two 32 x 32 tiles side by side along m (h = 0, 1) as 16-bit numbers: one row of 128 bytes to a lane
-// pair.
-__device__ __forceinline__ void put16(int lane, char *st, int h, int q, uint32_t lo, uint32_t hi) {
-    *reinterpret_cast<uint2 *>(store_chunk(st, lane & 31, h * 4 + q) + 8 * (lane >> 5)) = make_uint2(lo, hi);
+// The registers of tile (ii, jj) of 4 x 2 tiles, 64 columns (m) of 32 rows (n), as 16-bit numbers.
+__device__ __forceinline__ void put16(int lane, char *st, int ii, int jj, uint32_t lo, uint32_t hi) {
+    char *at = store_chunk(st, 16 * jj + (lane & 15), 2 * ii + (lane >> 5));
+    *reinterpret_cast<uint2 *>(at + 8 * (lane >> 4 & 1)) = make_uint2(lo, hi);
 }
-// The same of one tile as fp32 numbers.
-__device__ __forceinline__ void put32(int lane, char *st, int q, const float (&x)[4]) {
-    *reinterpret_cast<float4 *>(store_chunk(st, lane & 31, 2 * q + (lane >> 5))) = make_float4(x[0], x[1], x[2], x[3]);
+// The same of 2 x 2 tiles as fp32 numbers.
+__device__ __forceinline__ void put32(int lane, char *st, int ii, int jj, const float (&x)[4]) {
+    *reinterpret_cast<float4 *>(store_chunk(st, 16 * jj + (lane & 15), 4 * ii + (lane >> 4))) = make_float4(x[0], x[1], x[2], x[3]);
 }
 
 // Whether a product takes operands with this row pitch: offsets within a tile of 256 rows stay below 2^31.

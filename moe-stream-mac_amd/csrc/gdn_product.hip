@@ -16,40 +16,48 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void product_kernel(const Args 
         const int64_t m0 = (int64_t)tm * S::BM + wm * (S::BM / S::WM), n0 = (int64_t)tn * S::BN + wn * (S::BN / S::WN);
         const int e = KIND == PARTS ? 0 : exponent_of(r);
 #pragma unroll
-        for (int j = 0; j < S::TN; ++j) {
-            const int64_t n = n0 + 32 * j, rows = g.b.rows - n;
+        for (int j = 0; j < S::TN; j += 2) {
+            const int64_t n = n0 + 16 * j, rows = g.b.rows - n;
             if (rows <= 0) break;
-            float f = 1.f;
+            float f[2] = {1.f, 1.f};
             if constexpr (KIND != PARTS)
-                if (r.row) f = r.row[n + min((int64_t)(lane & 31), rows - 1)];
-            const auto scaled = [&](float x) { return f == 0.f ? 0.f : ldexpf(x, e) * f; };
+                if (r.row) {
+#pragma unroll
+                    for (int jj = 0; jj < 2; ++jj) f[jj] = r.row[n + min((int64_t)(16 * jj + (lane & 15)), rows - 1)];
+                }
+            const auto scaled = [&](float x, int jj) { return f[jj] == 0.f ? 0.f : ldexpf(x, e) * f[jj]; };
             if constexpr (KIND == OUT16) {
 #pragma unroll
-                for (int i = 0; i < S::TM; i += 2) {
-                    const int64_t m = m0 + 32 * i;
+                for (int i = 0; i < S::TM; i += 4) {
+                    const int64_t m = m0 + 16 * i;
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                    for (int ii = 0; ii < 4; ++ii)
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const acc_t &x = acc[i + h][j];
-                            put16(lane, st, h, q, ops::pack2_cvt(scaled(x[4 * q]), scaled(x[4 * q + 1]), r.dt),
-                                  ops::pack2_cvt(scaled(x[4 * q + 2]), scaled(x[4 * q + 3]), r.dt));
+                        for (int jj = 0; jj < 2; ++jj) {
+                            const acc_t &x = acc[i + ii][j + jj];
+                            put16(lane, st, ii, jj, ops::pack2_cvt(scaled(x[0], jj), scaled(x[1], jj), r.dt),
+                                  ops::pack2_cvt(scaled(x[2], jj), scaled(x[3], jj), r.dt));
                         }
-                    store_rows(lane, st, static_cast<char *>(r.y) + (n * r.ldy + m) * 2, (uint32_t)(r.ldy * 2), rows, (g.a.rows - m) * 2, 2);
+                    store_rows(lane, st, static_cast<char *>(r.y) + (n * r.ldy + m) * 2, (uint32_t)(r.ldy * 2), rows,
+                               (g.a.rows - m) * 2, 2);
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < S::TM; ++i) {
-                    const int64_t m = m0 + 32 * i;
+                for (int i = 0; i < S::TM; i += 2) {
+                    const int64_t m = m0 + 16 * i;
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        float x[4];
+                    for (int ii = 0; ii < 2; ++ii)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) x[k] = KIND == PARTS ? acc[i][j][4 * q + k] : scaled(acc[i][j][4 * q + k]);
-                        put32(lane, st, q, x);
-                    }
+                        for (int jj = 0; jj < 2; ++jj) {
+                            float x[4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                x[k] = KIND == PARTS ? acc[i + ii][j + jj][k] : scaled(acc[i + ii][j + jj][k], jj);
+                            put32(lane, st, ii, jj, x);
+                        }
                     if constexpr (KIND == OUT32) {
-                        store_rows(lane, st, static_cast<char *>(r.y) + (n * r.ldy + m) * 4, (uint32_t)(r.ldy * 4), rows, (g.a.rows - m) * 4, 4);
+                        store_rows(lane, st, static_cast<char *>(r.y) + (n * r.ldy + m) * 4, (uint32_t)(r.ldy * 4), rows,
+                                   (g.a.rows - m) * 4, 4);
                     } else {
                         char *to = reinterpret_cast<char *>(r.acc + ((int64_t)blockIdx.z * g.b.rows + n) * r.ldp + m);
                         if (r.add) add_rows(lane, st, to, (uint32_t)(r.ldp * 4), rows, (r.ldp - m) * 4);
