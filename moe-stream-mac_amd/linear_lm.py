@@ -3,6 +3,9 @@ operators of ``linear_attention``, ``rotary``, ``token_logprobs`` and ``grad_cli
 
     python moe-stream-mac_amd/linear_lm.py --steps 4 --tokens 512 --decode 16
 
+``--lean`` trains without logits (``linear_loss``) and with the embedding's gradient by sorted tokens (``embedding``); ``--tied``
+uses the embedding as the head as well, its rows scaled by the root of their size on the way in.
+
 The model is random-initialised and trained with AdamW on synthetic next-token data.  Prints the loss and the gradients'
 norm of every step, then for every decoded token its log probability, the entropy it was drawn from and its best
 alternative.
@@ -18,8 +21,10 @@ from typing import Optional
 import torch
 import torch.nn.functional as F
 
+from embedding import Embedding
 from grad_clip import clip_grad_norm
 from linear_attention import linear_attention, linear_attention_step
+from linear_loss import linear_cross_entropy
 from rotary import rotary, rotary_frequencies
 from token_logprobs import token_logprobs
 
@@ -52,15 +57,23 @@ class Mixer(torch.nn.Module):
 
 
 class LinearLM(torch.nn.Module):
-    def __init__(self, vocab: int, hidden: int, layers: int, key_heads: int, value_heads: int, head_dim: int):
+    def __init__(self, vocab: int, hidden: int, layers: int, key_heads: int, value_heads: int, head_dim: int,
+                 lean: bool = False, tied: bool = False):
         super().__init__()
-        self.embed = torch.nn.Embedding(vocab, hidden)
+        self.lean = lean or tied
+        if self.lean:
+            self.embed = Embedding(vocab, hidden, scale=hidden ** 0.5 if tied else 1.0)
+        else:
+            self.embed = torch.nn.Embedding(vocab, hidden)
         self.norms = torch.nn.ModuleList(torch.nn.LayerNorm(hidden) for _ in range(2 * layers + 1))
         self.mixers = torch.nn.ModuleList(Mixer(hidden, key_heads, value_heads, head_dim) for _ in range(layers))
         self.mlps = torch.nn.ModuleList(
             torch.nn.Sequential(torch.nn.Linear(hidden, 4 * hidden), torch.nn.GELU(), torch.nn.Linear(4 * hidden, hidden))
             for _ in range(layers))
         self.head = torch.nn.Linear(hidden, vocab, bias=False)
+        if tied:
+            torch.nn.init.normal_(self.embed.weight, std=hidden ** -0.5)
+            self.head.weight = self.embed.weight
         self.register_buffer("inv_freq", rotary_frequencies(head_dim // 2)[0], persistent=False)
 
     def _apply(self, fn, *args, **kw):
@@ -70,8 +83,8 @@ class LinearLM(torch.nn.Module):
         self.inv_freq = inv.to(self.inv_freq.device)
         return self
 
-    def forward(self, ids: Array, start: int = 0, states: Optional[list] = None) -> tuple[Array, list]:
-        """(logits [B, T, vocab], the layers' states after the last token) of ids [B, T] at positions start on."""
+    def hidden(self, ids: Array, start: int = 0, states: Optional[list] = None) -> tuple[Array, list]:
+        """(what the head takes [B, T, hidden], the layers' states after the last token) of ids [B, T] at positions start on."""
         positions = torch.arange(start, start + ids.shape[1], device=ids.device)
         x, out = self.embed(ids), []
         for i, (mixer, mlp) in enumerate(zip(self.mixers, self.mlps)):
@@ -79,13 +92,21 @@ class LinearLM(torch.nn.Module):
             out.append(state)
             x = x + y
             x = x + mlp(self.norms[2 * i + 1](x))
-        return self.head(self.norms[-1](x)), out
+        return self.norms[-1](x), out
+
+    def forward(self, ids: Array, start: int = 0, states: Optional[list] = None) -> tuple[Array, list]:
+        """(logits [B, T, vocab], the layers' states after the last token) of ids [B, T] at positions start on."""
+        x, out = self.hidden(ids, start, states)
+        return self.head(x), out
 
 
 def train_step(model: LinearLM, opt, ids: Array, max_norm: float) -> tuple[Array, Array]:
     """(loss, the gradients' norm before clipping) of one step on ids [B, T + 1]."""
-    logits, _ = model(ids[:, :-1])
-    loss = -token_logprobs(logits, ids[:, 1:]).logp.mean()
+    if model.lean:
+        loss = linear_cross_entropy(model.hidden(ids[:, :-1])[0], model.head.weight, ids[:, 1:])
+    else:
+        logits, _ = model(ids[:, :-1])
+        loss = -token_logprobs(logits, ids[:, 1:]).logp.mean()
     opt.zero_grad(set_to_none=True)
     loss.backward()
     norm = clip_grad_norm([p.grad for p in model.parameters() if p.grad is not None], max_norm)
@@ -120,6 +141,8 @@ def main(argv: list[str] | None = None) -> int:
     p.add_argument("--lr", type=float, default=1e-3)
     p.add_argument("--max-norm", type=float, default=1.0)
     p.add_argument("--bf16", action="store_true")
+    p.add_argument("--lean", action="store_true")
+    p.add_argument("--tied", action="store_true")
     p.add_argument("--seed", type=int, default=0)
     args = p.parse_args(argv)
     if args.steps < 0 or args.tokens < 1 or args.decode < 0:
@@ -129,7 +152,8 @@ def main(argv: list[str] | None = None) -> int:
         return 1
     dev = torch.device("cuda:0")
     torch.manual_seed(args.seed)
-    model = LinearLM(args.vocab, args.hidden, args.layers, args.key_heads, args.value_heads, args.head_dim)
+    model = LinearLM(args.vocab, args.hidden, args.layers, args.key_heads, args.value_heads, args.head_dim,
+                     args.lean, args.tied)
     model = model.to(device=dev, dtype=torch.bfloat16 if args.bf16 else torch.float32)
     opt = torch.optim.AdamW(model.parameters(), lr=args.lr)
     ids = torch.randint(0, args.vocab, (args.batch, args.tokens + 1), device=dev)

@@ -6,6 +6,7 @@
 GDN_CHECKPOINT (default "1") installs gdn_checkpoint, GDN_VJP (default "0") installs gdn_vjp and
 FROZEN_GDN_KERNEL (default "0") marks the frozen lower GDN layers with frozen_gdn, in the reference's order.
 The model is random-initialised (no checkpoint is loaded) and trained with AdamW on synthetic next-token data.
+``--lean`` takes the loss without logits and the embedding by sorted tokens, ``--base-bits 4`` keeps the frozen layers in MXFP4.
 Prints the reference's timing line and peak memory (torch's HIP caching-allocator counter).
 """
 
@@ -31,7 +32,12 @@ def build_model(args: argparse.Namespace, dev: torch.device) -> Q.Model:
                         full_attention_interval=args.full_attention_interval)
     model = Q.Model(margs)
     Q.linear_to_lora_layers(model, args.lora_layers, rank=args.rank, scale=args.scale)
-    return model.to(device=dev, dtype=torch.bfloat16 if args.bf16 else torch.float32)
+    model = model.to(device=dev, dtype=torch.bfloat16 if args.bf16 else torch.float32)
+    if args.lean:
+        Q.sorted_embedding(model)
+    if args.base_bits == 4:
+        Q.quantize_frozen(model)
+    return model
 
 
 def install_from_env(model: Q.Model) -> list[str]:
@@ -69,6 +75,8 @@ def main(argv: list[str] | None = None) -> int:
     p.add_argument("--scale", type=float, default=20.0)
     p.add_argument("--lr", type=float, default=1e-4)
     p.add_argument("--bf16", action="store_true")
+    p.add_argument("--lean", action="store_true")
+    p.add_argument("--base-bits", type=int, choices=(4, 16), default=16)
     p.add_argument("--seed", type=int, default=0)
     args = p.parse_args(argv)
     if args.steps <= 0 or args.tokens <= 1:
@@ -91,7 +99,10 @@ def main(argv: list[str] | None = None) -> int:
     torch.cuda.synchronize(dev)
     started = time.perf_counter()
     for step in range(args.steps):
-        loss = F.cross_entropy(model(inputs).float().flatten(0, 1), targets.flatten())
+        if args.lean:
+            loss = model.loss(inputs, targets)
+        else:
+            loss = F.cross_entropy(model(inputs).float().flatten(0, 1), targets.flatten())
         opt.zero_grad(set_to_none=True)
         loss.backward()
         opt.step()

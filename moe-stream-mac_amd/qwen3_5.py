@@ -29,7 +29,10 @@ import gated_delta
 import gdn_block
 import gdn_engine
 import gdn_lib as L
+import mxfp4
+from embedding import Embedding
 from gated_delta import gated_delta_update, normalize_qk  # noqa: F401  (rebound by install())
+from linear_loss import linear_cross_entropy
 
 Array = torch.Tensor
 
@@ -97,7 +100,7 @@ class GatedDeltaNet(nn.Module):
         projs = (self.in_proj_qkv, self.in_proj_z, self.in_proj_b, self.in_proj_a)
         if T == 1 and cache is not None and mask is None and not torch.is_grad_enabled() and self._decodes_fused(x, cache):
             return self._decode_token(x, cache)
-        if all(isinstance(m, LoRALinear) and m.base.bias is None for m in projs):
+        if all(isinstance(m, LoRALinear) and m.groups for m in projs):
             qkv, z, b, a = lora_group(x, projs)  # the four adapters share one pass over x
         else:
             qkv, z, b, a = (m(x) for m in projs)
@@ -304,6 +307,10 @@ class Model(nn.Module):
     def forward(self, tokens: Array, mask: Optional[Array] = None, cache: Optional[list] = None) -> Array:
         return self.lm_head(self.model(tokens, mask, cache))
 
+    def loss(self, tokens: Array, targets: Array, mask: Optional[Array] = None, ignore_index: int = -100) -> Array:
+        """Mean cross entropy of ``targets`` (those that are not ``ignore_index``) without the logits."""
+        return linear_cross_entropy(self.model(tokens, mask), self.lm_head.weight, targets, ignore_index=ignore_index)
+
 
 Qwen3_5TextModel = TextModel
 
@@ -403,8 +410,13 @@ class LoRALinear(nn.Module):
     def weight(self):
         return self.base.weight
 
+    @property
+    def groups(self) -> bool:
+        """Whether the base is a dense layer without bias, as lora_group takes them."""
+        return isinstance(self.base, nn.Linear) and self.base.bias is None
+
     def forward(self, x: Array) -> Array:
-        if self.base.bias is None:
+        if self.groups:
             return lora_group(x, (self,))[0]
         u = F.linear(x, self.lora_a.to(x.dtype)).flatten(0, -2)
         y = torch.addmm(self.base(x).flatten(0, -2), u, self.lora_b.to(x.dtype).t(), alpha=self.scale)
@@ -425,3 +437,25 @@ def linear_to_lora_layers(model: Model, num_layers: int, rank: int = 2, scale: f
             for child_name, child in list(mod.named_children()):
                 if isinstance(child, nn.Linear):
                     setattr(mod, child_name, LoRALinear(child, rank, scale))
+
+
+def quantize_frozen(model: Model) -> int:
+    """The frozen bias-free Linear layers of the decoder layers, under adapters or not, in 4 bits (``mxfp4.MXFP4Linear``): where
+    the reference trains adapters on a 4-bit base.  Returns how many there were.  Layers must be on the GPU; those that train
+    keep their weights."""
+    count = 0
+    for layer in model.layers:
+        for mod in list(layer.modules()):
+            for name, child in list(mod.named_children()):
+                if type(child) is nn.Linear and child.bias is None and not child.weight.requires_grad:
+                    setattr(mod, name, mxfp4.MXFP4Linear.of(child))
+                    count += 1
+    return count
+
+
+def sorted_embedding(model: Model) -> None:
+    """The model's embedding as ``embedding.Embedding``, with the same parameter."""
+    old = model.model.embed_tokens
+    new = Embedding(old.num_embeddings, old.embedding_dim, old.padding_idx, device="meta")
+    new.weight = old.weight
+    model.model.embed_tokens = new
