@@ -108,8 +108,10 @@ def test_decoding_on_a_4_bit_base(dev):
 
 
 @pytest.mark.parametrize("extra", [["--lean"], ["--lean", "--base-bits", "4", "--bf16"], ["--base-bits", "4"]])
-def test_lora_step(dev, extra, capsys):
+def test_lora_step(dev, extra, capsys, monkeypatch):
     import lora_step
+    for name in ("GDN_CHECKPOINT", "GDN_VJP", "FROZEN_GDN_KERNEL"):
+        monkeypatch.setenv(name, "0")  # installs stay for the process
     assert lora_step.main(["--steps", "2", "--tokens", "100", "--hidden", "128", "--head-dim", "64", *extra]) == 0
     assert sum(l.startswith("step") for l in capsys.readouterr().out.splitlines()) == 2
 
