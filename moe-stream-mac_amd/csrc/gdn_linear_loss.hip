@@ -12,6 +12,11 @@
 //
 // Words lie along registers and tokens along lanes, so that maxima and sums run within a lane.
 //
+// Tokens that do not count (prompts, padding) are left out: from COMPACT tokens on, the others' hidden states are gathered into
+// the workspace, in their order, and every product forms the tiles of these alone.  How many there are only the device knows,
+// so launches are for all of them and workgroups without a token end at once.  Fewer tokens are taken as they lie: the
+// gathering, 20 us in all, would cost more than a few tokens less give.
+//
 // Precision.  Differences lie in [-1, 1] and have 11 bits as fp16 numbers times 2^15 (those below 2^-29 fewer); bf16 would
 // leave 8, as many as the results have, and make bf16 gradients up to 1.4 times as far from the exact ones.  W and x are fp16
 // numbers times a power of two then (gdn_terms.hip), which holds bf16 numbers exactly.  The differences for dW carry the
@@ -31,12 +36,54 @@ using namespace mm;
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int NT = 256;
+constexpr int64_t COMPACT = 2048;
 constexpr int64_t KEPT = 1 << 26;  // differences of a piece; statistics of the parts of the words
 constexpr int64_t MOST_TOKENS = 1 << 20;  // three slots of 16 bits for each are a row pitch that a product takes
 constexpr int SHIFT = 15;          // differences are stored times 2^15
 constexpr int TOP = 14;            // largest magnitudes of scaled operands: [2^14, 2^15)
 
 enum : int { E_X = 0, E_W = 1, E_D = 2 };
+
+// ------------------------------------------------------------------------------------------------ tokens that count
+
+struct Tokens {      // of COMPACT tokens and more
+    int *count;      // how many count
+    int *index;      // [N] their places
+    int *place;      // [N] a token's place among them, -1 for one that does not count
+    int64_t *target; // [N] their targets
+};
+
+// One workgroup, a run of tokens to each thread.  Tokens that do not count have loss 0.
+__global__ __launch_bounds__(1024) void tokens_kernel(const int64_t *targets, int64_t N, int64_t ignore, Tokens t, float *loss) {
+    __shared__ int sums[16];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t per = (N + 1023) / 1024, n0 = min(N, threadIdx.x * per), n1 = min(N, n0 + per);
+    int own = 0;
+    for (int64_t n = n0; n < n1; ++n) own += targets[n] != ignore;
+    int before = own;  // of the threads up to this one
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const int v = __shfl_up(before, o);
+        if (lane >= o) before += v;
+    }
+    if (lane == 63) sums[w] = before;
+    __syncthreads();
+    int c = before - own;
+    for (int i = 0; i < w; ++i) c += sums[i];
+    for (int64_t n = n0; n < n1; ++n) {
+        const int64_t v = targets[n];
+        const bool live = v != ignore;
+        t.place[n] = live ? c : -1;
+        if (live) {
+            t.index[c] = (int)n;
+            t.target[c] = v;
+            ++c;
+        } else if (loss) {
+            loss[n] = 0.f;
+        }
+    }
+    if (threadIdx.x == 1023) *t.count = c;
+}
 
 // ------------------------------------------------------------------------------------------------ forward
 
@@ -54,7 +101,8 @@ template <class S, bool F16, bool SCALED>
 __global__ __launch_bounds__(S::NT, S::WAVES_EU) void stat_kernel(const Args g, const StatArgs a) {
     __shared__ __attribute__((aligned(16))) char lds[S::LDS];
     const int w = wave_index(), wm = w / S::WN, wn = w % S::WN;
-    products<S, F16>(g, lds, [&](int tm, int tn, acc_t(&acc)[S::TM][S::TN]) {
+    const Extent ext = extent_of<S>(g);
+    products<S, F16>(g, ext, lds, [&](int tm, int tn, acc_t(&acc)[S::TM][S::TN]) {
         const int lane = lane_here();
         const int64_t m0 = (int64_t)tm * S::BM + wm * (S::BM / S::WM);  // of the operand's rows
         const int words = (int)min((int64_t)(S::BM / S::WM), g.a.rows - m0);
@@ -62,7 +110,7 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void stat_kernel(const Args g, 
 #pragma unroll
         for (int j = 0; j < S::TN; ++j) {
             const int64_t n = (int64_t)tn * S::BN + wn * (S::BN / S::WN) + 16 * j + (lane & 15);
-            const bool live = n < a.N;
+            const bool live = n < ext.rows_b;
             float mx = -INFINITY;
 #pragma unroll
             for (int i = 0; i < S::TM; ++i)
@@ -102,13 +150,15 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void stat_kernel(const Args g, 
 // Joins a token's parts: TOKENS tokens to a workgroup, NT / TOKENS threads to a token.
 template <int TOKENS>
 __global__ __launch_bounds__(NT) void join_kernel(const int64_t *targets, const float2 *part, int parts, const float *zt,
-                                                  int64_t N, int64_t V, int64_t ignore, float *loss, float2 *stat) {
+                                                  int64_t N, int64_t V, int64_t ignore, float *loss, float2 *stat,
+                                                  const int *index, const int *count, int64_t n0) {
     constexpr int P = NT / TOKENS;
     __shared__ float2 red[P][TOKENS];
     const int tl = threadIdx.x % TOKENS, p0 = threadIdx.x / TOKENS;
     const int64_t n = block_index() * TOKENS + tl;
+    const bool any = n < N && (!count || n0 + n < *count);
     float m = -INFINITY, s = 0.f;
-    if (n < N) {
+    if (any) {
 #pragma unroll 8
         for (int p = p0; p < parts; p += P) {
             const float2 o = part[(int64_t)p * N + n];
@@ -130,12 +180,12 @@ __global__ __launch_bounds__(NT) void join_kernel(const int64_t *targets, const 
         }
         __syncthreads();
     }
-    if (p0 || n >= N) return;
+    if (p0 || !any) return;
     const int64_t t = targets[n];
     float l = logf(s) - (zt[n] - m);
     if (t < 0 || t >= V) l = NAN;
     if (t == ignore) l = 0.f;
-    loss[n] = l;
+    loss[index ? index[n] : n] = l;
     if (stat) stat[n] = make_float2(m, 1.f / s);
 }
 
@@ -172,12 +222,13 @@ __global__ __launch_bounds__(1024) void total_kernel(const float *loss, const in
 // d[n] = the token's cotangent: 0 where it does not count, NaN where its target is no word.  part = partial maxima of |d|.
 __global__ __launch_bounds__(NT) void cotangent_kernel(const int64_t *targets, const float *dloss, int64_t stride,
                                                        const float *factor, int64_t N, int64_t V, int64_t ignore, float *d,
-                                                       float *part) {
+                                                       float *part, const int *index, const int *count) {
     __shared__ float red[NT];
     float m = 0.f;
+    if (count) N = *count;
     for (int64_t n = (int64_t)blockIdx.x * NT + threadIdx.x; n < N; n += (int64_t)PARTS * NT) {
         const int64_t t = targets[n];
-        float x = dloss[n * stride];
+        float x = dloss[(index ? index[n] : n) * stride];
         if (factor) x *= factor[0];
         if (t < 0 || t >= V) x = NAN;
         if (t == ignore) x = 0.f;
@@ -200,7 +251,7 @@ struct DiffArgs {
     const float *d;
     const int *exps;  // with fp32 inputs also the logits' scale
     uint16_t *p, *pt; // [N][terms * kp], [words][terms * np]; either may be NULL
-    int64_t N, v0, kp, np;
+    int64_t v0, kp, np;
 };
 
 // x as it was rounded: the compiler may round a product or sum to 16 bits at once in one place and in two steps in another, and
@@ -221,7 +272,8 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
     __shared__ __attribute__((aligned(16))) char lds[S::LDS + S::STORE];
     const int w = wave_index(), wm = w / S::WN, wn = w % S::WN;
     char *store = lds + S::LDS + w * 4096;
-    products<S, F16>(g, lds, [&](int tm, int tn, acc_t(&acc)[S::TM][S::TN]) {
+    const Extent ext = extent_of<S>(g);
+    products<S, F16>(g, ext, lds, [&](int tm, int tn, acc_t(&acc)[S::TM][S::TN]) {
         const int lane = lane_here();
         const int64_t m0 = (int64_t)tm * S::BM + wm * (S::BM / S::WM), n0 = (int64_t)tn * S::BN + wn * (S::BN / S::WN);
         const int words = (int)min((int64_t)(S::BM / S::WM), g.a.rows - m0);  // of this wave's; may be negative
@@ -230,7 +282,7 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
 #pragma unroll
         for (int j = 0; j < S::TN; ++j) {
             const int64_t n = n0 + 16 * j + (lane & 15);
-            const bool live = n < a.N;
+            const bool live = n < ext.rows_b;
             const float2 st = live ? a.stat[n] : make_float2(0.f, 0.f);
             r[j] = DW && live ? ldexpf(a.d[n], a.exps[E_D]) : 0.f;
             const float inv = st.y * (float)(1 << SHIFT);
@@ -251,13 +303,13 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
         if constexpr (DX) {
 #pragma unroll
             for (int j = 0; j < S::TN; j += 2) {
-                const int64_t n = n0 + 16 * j, rows = a.N - n;
+                const int64_t n = n0 + 16 * j, rows = ext.rows_b - n;
                 if (rows <= 0) break;
 #pragma unroll
                 for (int i = 0; i < S::TM; i += 4) {
                     const int64_t m = m0 + 16 * i;
                     if (m >= a.kp) break;
-#pragma unroll
+#pragma unroll 1
                     for (int t = 0; t < TERMS; ++t) {
 #pragma unroll
                         for (int ii = 0; ii < 4; ++ii)
@@ -283,7 +335,7 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
 #pragma unroll
                 for (int i = 0; i < S::TM; i += 2) {
                     if (16 * i >= words) break;
-#pragma unroll
+#pragma unroll 1
                     for (int t = 0; t < TERMS; ++t) {
 #pragma unroll
                         for (int ii = 0; ii < 2; ++ii)
@@ -335,7 +387,7 @@ static void segments(Args &g, int terms, int64_t kp, bool across) {
 struct Sizes {
     int64_t N, H, V, hp, np, piece, pieces;  // hp, np: H and N in whole blocks; piece: words at a time
     int terms;
-    bool direct_x, direct_w;  // the operand is used as it lies
+    bool compact;
     int64_t parts, tokens;  // parts of the words with statistics of their own; tokens at a time in the forward pass
     Plan px, pw;
 };
@@ -350,6 +402,7 @@ static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt) {
     s.hp = padded(H);
     s.np = padded(N);
     s.terms = dt == GDN_F32 ? 2 : 1;
+    s.compact = N >= COMPACT;
     int64_t most = KEPT / s.np / 256 * 256;
     if (most < 256) most = 256;
     s.pieces = (V + most - 1) / most;
@@ -382,6 +435,7 @@ struct Buffers {
     float *part, *zt, *d, *acc_x, *acc_w;
     float2 *stats;
     int *exps;
+    Tokens tokens;
 };
 
 static Buffers place(Space &sp, const Sizes &s, bool dx, bool dw, bool bwd, bool copy_x, bool copy_w) {
@@ -390,7 +444,13 @@ static Buffers place(Space &sp, const Sizes &s, bool dx, bool dw, bool bwd, bool
     const int64_t words = s.piece < s.V ? s.piece : s.V;
     b.exps = sp.take<int>(4);
     b.part = sp.take<float>(3 * PARTS);
-    if (copy_x) b.x = sp.take<uint16_t>(s.N * t * s.hp);
+    if (s.compact) {
+        b.tokens.count = sp.take<int>(1);
+        b.tokens.index = sp.take<int>(s.N);
+        b.tokens.place = sp.take<int>(s.N);
+        b.tokens.target = sp.take<int64_t>(s.N);
+    }
+    if (copy_x || s.compact) b.x = sp.take<uint16_t>(s.N * t * s.hp);
     if (copy_w) b.w = sp.take<uint16_t>(words * t * s.hp);
     if (!bwd) {
         b.stats = sp.take<float2>(s.parts * s.tokens);
@@ -487,7 +547,7 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
     if (N > 0) {
         if (!x || !w || !targets || !loss || !workspace) return fail(GDN_ERR_INVALID, "null pointer");
         const Sizes s = sizes(N, H, V, dtype);
-        const bool dx = direct(x, x_stride, H, dtype), dw = direct(w, w_stride, H, dtype);
+        const bool dx = !s.compact && direct(x, x_stride, H, dtype), dw = direct(w, w_stride, H, dtype);
         const size_t bytes = need(s, false, false, false, !dx, !dw);
         if (workspace_bytes < bytes)
             return fail(GDN_ERR_WORKSPACE, "the workspace holds %zu bytes, %zu are needed", workspace_bytes, bytes);
@@ -495,7 +555,12 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
         const Buffers b = place(sp, s, false, false, false, !dx, !dw);
         const bool f16 = dtype != GDN_BF16;
         const int *exps = nullptr;
-        const Source sx{x, dtype, N, H, x_stride, targets, ignore_index}, sw{w, dtype, V, H, w_stride, nullptr, 0};
+        const Tokens &tk = b.tokens;  // empty without
+        const int64_t *tt = s.compact ? tk.target : targets;
+        const Source sx{x, dtype, N, H, x_stride, s.compact ? nullptr : targets, ignore_index, tk.index, tk.count};
+        const Source sw{w, dtype, V, H, w_stride, nullptr, 0, nullptr, nullptr};
+        if (s.compact)
+            hipLaunchKernelGGL(tokens_kernel, dim3(1), dim3(1024), 0, st, targets, N, ignore_index, tk, loss);
         if (dtype == GDN_F32) {
             maxima(sx, b.part + E_X * PARTS, st);
             maxima(sw, b.part + E_W * PARTS, st);
@@ -515,6 +580,8 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
                 segments(g, s.terms, s.hp, false);
                 g.a.rows = words;
                 g.b.rows = tokens;
+                g.live = tk.count;
+                g.live0 = n0;
                 g.a.p = reinterpret_cast<const char *>(b.w);
                 g.b.p = reinterpret_cast<const char *>(b.x) + n0 * s.terms * s.hp * 2;
                 if (dw) {
@@ -530,7 +597,7 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
                     g.b.p = static_cast<const char *>(x) + n0 * x_stride * 2;
                     g.b.ld = x_stride * 2;
                 }
-                const StatArgs a{targets + n0, b.stats, b.zt, exps, tokens, V, v0, parts};
+                const StatArgs a{tt + n0, b.stats, b.zt, exps, tokens, V, v0, parts};
                 Timed tm("loss_stat", st);
 #define GDN_STAT(S)                                \
     launch_stat_of<S>(g, a, dtype, st);            \
@@ -540,13 +607,15 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
             }
             Timed tm("loss_join", st);
             float2 *to = stat ? reinterpret_cast<float2 *>(stat) + n0 : nullptr;
+            const int *index = s.compact ? tk.index + n0 : nullptr;
+            float *each = s.compact ? loss : loss + n0;
             // 128 bytes of a part's tokens at a time, or all threads on the parts of one of few
             if (tokens > 64)
-                hipLaunchKernelGGL((join_kernel<16>), grid_of((tokens + 15) / 16), dim3(NT), 0, st, targets + n0, b.stats, parts,
-                                   b.zt, tokens, V, ignore_index, loss + n0, to);
+                hipLaunchKernelGGL((join_kernel<16>), grid_of((tokens + 15) / 16), dim3(NT), 0, st, tt + n0, b.stats, parts, b.zt,
+                                   tokens, V, ignore_index, each, to, index, tk.count, n0);
             else
-                hipLaunchKernelGGL((join_kernel<1>), grid_of(tokens), dim3(NT), 0, st, targets + n0, b.stats, parts, b.zt, tokens,
-                                   V, ignore_index, loss + n0, to);
+                hipLaunchKernelGGL((join_kernel<1>), grid_of(tokens), dim3(NT), 0, st, tt + n0, b.stats, parts, b.zt, tokens, V,
+                                   ignore_index, each, to, index, tk.count, n0);
         }
     }
     if (reduction)
@@ -567,7 +636,7 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
     if (N == 0) return fail(GDN_ERR_INVALID, "no tokens: the gradients are zeros, which this call does not write");
     if (!x || !w || !targets || !stat || !dloss || !workspace) return fail(GDN_ERR_INVALID, "null pointer");
     const Sizes s = sizes(N, H, V, dtype);
-    const bool direct_x = direct(x, x_stride, H, dtype), direct_w = direct(w, w_stride, H, dtype);
+    const bool direct_x = !s.compact && direct(x, x_stride, H, dtype), direct_w = direct(w, w_stride, H, dtype);
     const size_t bytes = need(s, dx, dw, true, !direct_x, !direct_w);
     if (workspace_bytes < bytes)
         return fail(GDN_ERR_WORKSPACE, "the workspace holds %zu bytes, %zu are needed", workspace_bytes, bytes);
@@ -575,9 +644,13 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
     const Buffers b = place(sp, s, dx, dw, true, !direct_x, !direct_w);
     const bool f16 = dtype != GDN_BF16;
     const int elem = dtype == GDN_F32 ? 4 : 2, t = s.terms;
-    const Source sx{x, dtype, N, H, x_stride, targets, ignore_index}, sw{w, dtype, V, H, w_stride, nullptr, 0};
-    hipLaunchKernelGGL(cotangent_kernel, dim3(PARTS), dim3(NT), 0, st, targets, dloss, dloss_stride, factor, N, V, ignore_index,
-                       b.d, b.part + E_D * PARTS);
+    const Tokens &tk = b.tokens;  // empty without
+    const int64_t *tt = s.compact ? tk.target : targets;
+    const Source sx{x, dtype, N, H, x_stride, s.compact ? nullptr : targets, ignore_index, tk.index, tk.count};
+    const Source sw{w, dtype, V, H, w_stride, nullptr, 0, nullptr, nullptr};
+    if (s.compact) hipLaunchKernelGGL(tokens_kernel, dim3(1), dim3(1024), 0, st, targets, N, ignore_index, tk, nullptr);
+    hipLaunchKernelGGL(cotangent_kernel, dim3(PARTS), dim3(NT), 0, st, tt, dloss, dloss_stride, factor, N, V, ignore_index,
+                       b.d, b.part + E_D * PARTS, tk.index, tk.count);
     maxima(sx, b.part + E_X * PARTS, st);
     maxima(sw, b.part + E_W * PARTS, st);
     exponents(b.part, 2, TOP, b.exps, st);
@@ -595,6 +668,7 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
         segments(g, t, s.hp, false);
         g.a.rows = words;
         g.b.rows = N;
+        g.live = tk.count;
         g.a.p = reinterpret_cast<const char *>(b.w);
         g.b.p = reinterpret_cast<const char *>(b.x);
         if (direct_w) {
@@ -607,7 +681,7 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
             g.b.p = static_cast<const char *>(x);
             g.b.ld = x_stride * 2;
         }
-        const DiffArgs a{targets, reinterpret_cast<const float2 *>(stat), b.d, b.exps, b.p, b.pt, N, v0, kp, s.np};
+        const DiffArgs a{tt, reinterpret_cast<const float2 *>(stat), b.d, b.exps, b.p, b.pt, v0, kp, s.np};
         {
             Timed tm("loss_diff", st);
 #define GDN_DIFF(S) launch_diff_of<S>(g, a, dtype, st)
@@ -622,9 +696,10 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
             h.a.rows = H;
             h.b.p = reinterpret_cast<const char *>(b.p);
             h.b.rows = N;
+            h.live = tk.count;
             const Plan pl = s.px;  // parts without a block of the last piece add nothing
-            Result r{dx, H, dtype, b.d, b.exps, -SHIFT, {0, -1, 0}, nullptr, columns_of(H), v0 > 0};
-            if (s.pieces > 1 || pl.splits > 1) r.acc = b.acc_x;
+            Result r{dx, H, dtype, b.d, b.exps, -SHIFT, {0, -1, 0}, nullptr, columns_of(H), v0 > 0, tk.place};
+            if (s.compact || s.pieces > 1 || pl.splits > 1) r.acc = b.acc_x;
             multiply(h, true, pl, r, st);
             if (r.acc && v0 + words == V) finish(r, pl.splits, N, H, st);
         }
@@ -635,7 +710,9 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
             h.a.rows = H;
             h.b.p = reinterpret_cast<const char *>(b.pt);
             h.b.rows = words;
-            Result r{static_cast<char *>(dw) + v0 * H * elem, H, dtype, nullptr, b.exps, -SHIFT, {-1, 0, -1}, nullptr, columns_of(H), 0};
+            h.live = tk.count;
+            h.live_k = 1;
+            Result r{static_cast<char *>(dw) + v0 * H * elem, H, dtype, nullptr, b.exps, -SHIFT, {-1, 0, -1}, nullptr, columns_of(H), 0, nullptr};
             if (s.pw.splits > 1) r.acc = b.acc_w;
             multiply(h, true, s.pw, r, st);
             if (r.acc) finish(r, s.pw.splits, words, H, st);

@@ -416,7 +416,7 @@ extern "C" int gdn_mxfp4_linear(const void *x, const void *codes, const void *sc
             return fail(GDN_ERR_WORKSPACE, "the workspace holds %zu bytes, %zu are needed", workspace_bytes, need.at);
         const Buffers b = place(sp, s, M, K, false, !as_it_lies);
         Args g{};
-        operand(g, Source{x, dtype, M, K, x_stride, nullptr, 0}, s, b.x, as_it_lies, st);
+        operand(g, Source{x, dtype, M, K, x_stride, nullptr, 0, nullptr, nullptr}, s, b.x, as_it_lies, st);
         const int elem = dtype == GDN_F32 ? 4 : 2;
         for (int64_t n0 = 0; n0 < N; n0 += s.piece) {
             const int64_t rows = N - n0 < s.piece ? N - n0 : s.piece;
@@ -427,7 +427,7 @@ extern "C" int gdn_mxfp4_linear(const void *x, const void *codes, const void *sc
                                    static_cast<const uint8_t *>(scales) + n0 * blocks, b.w, rows, K, blocks, s.kp, 0);
             }
             g.a = Operand{b.w, s.kp * 2, rows, {0, 0, 0}};
-            const Result r{static_cast<char *>(y) + n0 * elem, N, dtype, nullptr, nullptr, 0, {0, 0, 0}, b.acc, columns_of(rows), 0};
+            const Result r{static_cast<char *>(y) + n0 * elem, N, dtype, nullptr, nullptr, 0, {0, 0, 0}, b.acc, columns_of(rows), 0, nullptr};
             multiply(g, false, s.plan, r, st);
             if (r.acc) finish(r, s.plan.splits, M, rows, st);
         }
@@ -457,7 +457,7 @@ extern "C" int gdn_mxfp4_linear_bwd(const void *dy, const void *codes, const voi
         const int64_t rows = N - n0 < s.piece ? N - n0 : s.piece, np = padded(rows), tiles_k = (K + 63) / 64;
         const int64_t tiles = np / 64 * tiles_k;
         Args g{};
-        operand(g, Source{static_cast<const char *>(dy) + n0 * elem, dtype, M, rows, dy_stride, nullptr, 0}, s, b.x, as_it_lies, st);
+        operand(g, Source{static_cast<const char *>(dy) + n0 * elem, dtype, M, rows, dy_stride, nullptr, 0, nullptr, nullptr}, s, b.x, as_it_lies, st);
         {
             Timed tm("mxfp4_across", st);
             hipLaunchKernelGGL(across_kernel, grid_of(tiles), dim3(NT), 0, st, static_cast<const uint32_t *>(codes) + n0 * blocks * 4,
@@ -465,7 +465,7 @@ extern "C" int gdn_mxfp4_linear_bwd(const void *dy, const void *codes, const voi
                                blocks, np, tiles_k, tiles);
         }
         g.a = Operand{b.w, np * 2, K, {0, 0, 0}};
-        const Result r{dx, K, dtype, nullptr, nullptr, 0, {0, 0, 0}, b.acc, columns_of(K), n0 > 0};
+        const Result r{dx, K, dtype, nullptr, nullptr, 0, {0, 0, 0}, b.acc, columns_of(K), n0 > 0, nullptr};
         multiply(g, false, s.plan, r, st);
         if (r.acc && n0 + rows == N) finish(r, s.plan.splits, M, K, st);
     }

@@ -56,7 +56,30 @@ struct Args {
     int nseg;    // 1 to 3
     int splits;  // the nseg * kit blocks in this many parts (grid.z)
     int mt, nt;  // tiles
+    // Sizes that only the device knows: `live` tokens count, of which these are those from live0 on.  They are b's rows, or with
+    // live_k the length of the contraction; tiles and blocks behind them are not formed.
+    const int *live;
+    int64_t live0;
+    int live_k;
 };
+struct Extent {
+    int64_t rows_b;
+    int nt, kit;
+};
+template <class S>
+__device__ __forceinline__ Extent extent_of(const Args &g) {
+    Extent x{g.b.rows, g.nt, g.kit};
+    if (g.live) {
+        const int64_t n = max((int64_t)0, (int64_t)*g.live - g.live0);
+        if (g.live_k) {
+            x.kit = (int)min((int64_t)g.kit, (n + BK - 1) / BK);
+        } else {
+            x.rows_b = min(g.b.rows, n);
+            x.nt = (int)((x.rows_b + S::BN - 1) / S::BN);
+        }
+    }
+    return x;
+}
 
 // BM x BN tile of WM x WN waves.
 template <int BM_, int BN_, int WM_, int WN_, int PER_CU_>
@@ -110,13 +133,13 @@ struct Loader {
     uint32_t step_a, step_b;  // from one load's rows to the next one's
     int left, seg_left, seg, tile, tiles, w;  // blocks left of the tile and of the segment
 
-    __device__ __forceinline__ void start(const Args &g, int first, int end) {  // of a tile
+    __device__ __forceinline__ void start(const Args &g, const Extent &x, int first, int end) {  // of a tile
         int tm, tn;
-        tile_of(tile, g.mt, g.nt, tm, tn);
+        tile_of(tile, g.mt, x.nt, tm, tn);
         const int lane = threadIdx.x & 63, r0 = (threadIdx.x >> 3);
         const uint32_t chunk = ((lane & 7) ^ (r0 >> 1 & 7)) << 4;
         const int ma = (int)min((int64_t)S::BM, g.a.rows - (int64_t)tm * S::BM);
-        const int mb = (int)min((int64_t)S::BN, g.b.rows - (int64_t)tn * S::BN);
+        const int mb = (int)min((int64_t)S::BN, x.rows_b - (int64_t)tn * S::BN);
         va = (uint32_t)r0 * (uint32_t)g.a.ld + chunk;
         vb = (uint32_t)r0 * (uint32_t)g.b.ld + chunk;
         na = (uint32_t)(ma - 1) * (uint32_t)g.a.ld + BK * 2;
@@ -124,9 +147,9 @@ struct Loader {
         step_a = (uint32_t)(S::NT / 8) * (uint32_t)g.a.ld;
         step_b = (uint32_t)(S::NT / 8) * (uint32_t)g.b.ld;
         left = end - first;
-        seg = first / g.kit;
-        const int kk = first - seg * g.kit;
-        seg_left = g.kit - kk;
+        seg = first / x.kit;
+        const int kk = first - seg * x.kit;
+        seg_left = x.kit - kk;
         pa = g.a.p + (int64_t)tm * S::BM * g.a.ld + g.a.off[seg] + (int64_t)kk * (BK * 2);
         pb = g.b.p + (int64_t)tn * S::BN * g.b.ld + g.b.off[seg] + (int64_t)kk * (BK * 2);
     }
@@ -148,20 +171,20 @@ struct Loader {
 #endif
     }
     // On to the next block; after the very last one it stays there, so that loads need no branch around them.
-    __device__ __forceinline__ void next(const Args &g, int first, int end) {
+    __device__ __forceinline__ void next(const Args &g, const Extent &x, int first, int end) {
         if (left > 1) {
             pa += BK * 2;
             pb += BK * 2;
             --left;
             if (--seg_left == 0) {
-                seg_left = g.kit;
-                pa += g.a.off[seg + 1] - g.a.off[seg] - (int64_t)g.kit * (BK * 2);
-                pb += g.b.off[seg + 1] - g.b.off[seg] - (int64_t)g.kit * (BK * 2);
+                seg_left = x.kit;
+                pa += g.a.off[seg + 1] - g.a.off[seg] - (int64_t)x.kit * (BK * 2);
+                pb += g.b.off[seg + 1] - g.b.off[seg] - (int64_t)x.kit * (BK * 2);
                 ++seg;
             }
         } else if (tile + (int)gridDim.x < tiles) {
             tile += gridDim.x;
-            start(g, first, end);
+            start(g, x, first, end);
         }
     }
 };
@@ -262,20 +285,27 @@ __device__ __forceinline__ void second_half(const char *__restrict__ rd, char *_
     __builtin_amdgcn_sched_barrier(0);
 }
 
+template <class S>
+__device__ __forceinline__ void clear(acc_t (&acc)[S::TM][S::TN]) {
+#pragma unroll
+    for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j) acc[i][j] = acc_t{0.f, 0.f, 0.f, 0.f};
+}
+
 // Forms the workgroup's tiles and hands each to epilogue(tm, tn, acc).
 // acc[i][j]: rows m = 16 i + 4 (lane / 16) + q of this wave's part for register q, column n = 16 j + lane % 16.
 template <class S, bool F16, class E>
-__device__ __forceinline__ void products(const Args &g, char *lds, E &&epilogue) {
+__device__ __forceinline__ void products(const Args &g, const Extent &x, char *lds, E &&epilogue) {
     const int lane = threadIdx.x & 63, w = wave_index(), wm = w / S::WN, wn = w % S::WN;
-    const int total = g.kit * g.nseg;
+    const int total = x.kit * g.nseg;
     const int first = (int)((int64_t)total * blockIdx.z / g.splits), end = (int)((int64_t)total * (blockIdx.z + 1) / g.splits);
-    const int blocks = end - first, mt = g.mt, nt = g.nt;
+    const int blocks = end - first, mt = g.mt, nt = x.nt;
     Loader<S> ld;
     ld.tile = blockIdx.x;
     ld.tiles = mt * nt;
     ld.w = w;
-    if (ld.tile >= ld.tiles || blocks == 0) return;
-    ld.start(g, first, end);
+    if (ld.tile >= ld.tiles) return;
     uint32_t at_a[2], at_b[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -284,19 +314,17 @@ __device__ __forceinline__ void products(const Args &g, char *lds, E &&epilogue)
         at_b[k] = S::A_BYTES + (wn * (S::BN / S::WN) + (lane & 15)) * BK * 2 + c;
     }
     char *cur = lds, *other = lds + S::STAGE;
-    ld.template load<0, S::RA + S::RB>(cur);
-    ld.next(g, first, end);
-    stage_barrier();
-    ld.template load<0, S::RA + S::RB>(other);
-    ld.next(g, first, end);
+    if (blocks > 0) {  // else empty sums
+        ld.start(g, x, first, end);
+        ld.template load<0, S::RA + S::RB>(cur);
+        ld.next(g, x, first, end);
+        stage_barrier();
+        ld.template load<0, S::RA + S::RB>(other);
+        ld.next(g, x, first, end);
+    }
     for (int t = blockIdx.x; t < mt * nt; t += gridDim.x) {
         acc_t acc[S::TM][S::TN];
-#pragma unroll
-        for (int i = 0; i < S::TM; ++i)
-#pragma unroll
-            for (int j = 0; j < S::TN; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) acc[i][j][q] = 0.f;
+        clear<S>(acc);
         // read anew for each tile, so that their registers are free while results are written
         Frags<S> f;
 #pragma unroll
@@ -309,10 +337,10 @@ __device__ __forceinline__ void products(const Args &g, char *lds, E &&epilogue)
             stage_barrier();
             // after a tile's last block no product uses what this reads
             second_half<S, F16>(other, cur, ld, at_a, at_b, f, acc);
-            ld.next(g, first, end);
-            char *x = cur;
+            ld.next(g, x, first, end);
+            char *c = cur;
             cur = other;
-            other = x;
+            other = c;
         }
         int tm, tn;
         tile_of(t, mt, nt, tm, tn);
@@ -396,6 +424,7 @@ struct Result {
     float *acc;
     int64_t ldp;
     int add;
+    const int *place;  // for finish(): the row of acc (and of `row`) that y's row n is, or -1 for zeros; NULL: row n
 };
 inline int64_t columns_of(int64_t cols) { return (cols + 3) / 4 * 4; }  // whole 16 bytes
 

@@ -11,13 +11,14 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void product_kernel(const Args 
     __shared__ __attribute__((aligned(16))) char lds[S::LDS + S::STORE];
     const int w = wave_index(), wm = w / S::WN, wn = w % S::WN;
     char *st = lds + S::LDS + w * 4096;
-    products<S, F16>(g, lds, [&](int tm, int tn, acc_t(&acc)[S::TM][S::TN]) {
+    const Extent ext = extent_of<S>(g);
+    products<S, F16>(g, ext, lds, [&](int tm, int tn, acc_t(&acc)[S::TM][S::TN]) {
         const int lane = lane_here();
         const int64_t m0 = (int64_t)tm * S::BM + wm * (S::BM / S::WM), n0 = (int64_t)tn * S::BN + wn * (S::BN / S::WN);
         const int e = KIND == PARTS ? 0 : exponent_of(r);
 #pragma unroll
         for (int j = 0; j < S::TN; j += 2) {
-            const int64_t n = n0 + 16 * j, rows = g.b.rows - n;
+            const int64_t n = n0 + 16 * j, rows = ext.rows_b - n;
             if (rows <= 0) break;
             float f[2] = {1.f, 1.f};
             if constexpr (KIND != PARTS)
@@ -77,10 +78,11 @@ __global__ __launch_bounds__(NT) void finish_kernel(const Result r, int splits, 
     const int64_t per = r.ldp / 4, i = block_index() * NT + threadIdx.x, n = i / per, m = (i - n * per) * 4;
     if (n >= rows) return;
     const int e = exponent_of(r);
-    const float f = r.row ? r.row[n] : 1.f;
+    const int64_t at = r.place ? r.place[n] : n;
+    const float f = at < 0 ? 0.f : r.row ? r.row[at] : 1.f;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int z = 0; z < splits; ++z) {
-        const float4 v = *reinterpret_cast<const float4 *>(r.acc + (z * rows + n) * r.ldp + m);
+    for (int z = 0; z < splits && at >= 0; ++z) {
+        const float4 v = *reinterpret_cast<const float4 *>(r.acc + (z * rows + at) * r.ldp + m);
         s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
     }
 #pragma unroll

@@ -7,13 +7,15 @@ namespace gdn {
 namespace mm {
 
 // A matrix as the caller has it: rows of `cols` elements of type dt, ld elements apart.  With targets, rows whose target is
-// `ignore` count as zeros, whatever they hold.
+// `ignore` count as zeros, whatever they hold.  With index and count, row r is the caller's row index[r], and rows from *count
+// on count as zeros (rows: how many there may be).
 struct Source {
     const void *p;
     int dt;
     int64_t rows, cols, ld;
     const int64_t *targets;
     int64_t ignore;
+    const int *index, *count;
 };
 
 constexpr int PARTS = 512;  // partial maxima of one matrix

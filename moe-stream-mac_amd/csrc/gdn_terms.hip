@@ -13,7 +13,11 @@ namespace mm {
 
 constexpr int NT = 256;
 
-__device__ __forceinline__ bool skipped(const Source &s, int64_t r) { return s.targets && s.targets[r] == s.ignore; }
+// The caller's row for row r, or -1 where it counts as zeros.
+__device__ __forceinline__ int64_t row_of(const Source &s, int64_t r) {
+    if (s.index) return r < *s.count ? s.index[r] : -1;
+    return s.targets && s.targets[r] == s.ignore ? -1 : r;
+}
 
 __device__ __forceinline__ float wave_max(float x) {
 #pragma unroll
@@ -34,11 +38,12 @@ __global__ __launch_bounds__(1024) void maxima_kernel(const Source s, float *par
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float m = 0.f;
     for (int64_t r = blockIdx.x * WAVES + w; r < s.rows; r += PARTS * WAVES) {
-        if (skipped(s, r)) continue;
+        const int64_t at = row_of(s, r);
+        if (at < 0) continue;
         for (int64_t c = lane * 8; c < s.cols; c += U * 512) {
             float x[U][8];
 #pragma unroll
-            for (int u = 0; u < U; ++u) ops::load_first<8, DT>(s.p, r * s.ld + c + u * 512, s.cols - c - u * 512, x[u]);
+            for (int u = 0; u < U; ++u) ops::load_first<8, DT>(s.p, at * s.ld + c + u * 512, s.cols - c - u * 512, x[u]);
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -100,10 +105,10 @@ __global__ __launch_bounds__(NT) void terms_kernel(const Source s, int nterms, c
     if (r >= s.rows) return;
     const int e = exps ? exps[which] : 0;
     float x[8];
-    const bool none = skipped(s, r);
-    ops::load_first<8, DT>(s.p, r * s.ld + c, s.cols - c, x);
+    const int64_t at = row_of(s, r);
+    ops::load_first<8, DT>(s.p, at * s.ld + c, at < 0 ? 0 : s.cols - c, x);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = none ? 0.f : ldexpf(x[j], e);
+    for (int j = 0; j < 8; ++j) x[j] = ldexpf(x[j], e);
     for (int t = 0; t < nterms; ++t) {
         uint16_t b[8];
 #pragma unroll
@@ -126,8 +131,8 @@ __global__ __launch_bounds__(NT) void across_kernel(const Source s, int slots, c
         const int rl = h * 32 + threadIdx.x / 8, cl = threadIdx.x % 8 * 8;
         const int64_t r = r0 + rl, c = c0 + cl;
         float x[8];
-        const bool live = r < s.rows && !skipped(s, r);
-        ops::load_first<8, DT>(s.p, r * s.ld + c, live ? s.cols - c : 0, x);
+        const int64_t at = r < s.rows ? row_of(s, r) : -1;
+        ops::load_first<8, DT>(s.p, at * s.ld + c, at < 0 ? 0 : s.cols - c, x);
 #pragma unroll
         for (int j = 0; j < 8; ++j) tile[rl][cl + j] = ldexpf(x[j], e);
     }
@@ -157,7 +162,7 @@ void maxima(const Source &s0, float *part, hipStream_t st) {
     Timed tm("maxima", st);
     constexpr int64_t LONG = 8192;
     Source s = s0;
-    if (s.ld == s.cols && !s.targets && s.rows * s.cols % LONG == 0) {  // rows in one piece: of any length
+    if (s.ld == s.cols && !s.targets && !s.index && s.rows * s.cols % LONG == 0) {  // rows in one piece: of any length
         s.rows = s.rows * s.cols / LONG;
         s.ld = s.cols = LONG;
     }

@@ -183,6 +183,38 @@ def test_masked_places_hold_anything(dev, dtype):
     assert torch.isnan(dw).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("share", [0.0, 0.3, 0.97, 1.0])
+@pytest.mark.parametrize("N,H,V", [(2048, 64, 300), (2111, 200, 1501)])
+def test_tokens_left_out(dev, N, H, V, share, dtype):
+    """Long batches, of which products see only the tokens that count: none left out, some, nearly all, all."""
+    from linear_loss import linear_cross_entropy
+    print("left out", N, H, V, share, dtype, flush=True)
+    x, w, t, d = inputs(dev, N, H, V, dtype, int(100 * share) + N, ignored=False)
+    out = torch.rand(N, device=dev) < share
+    t[out] = 7
+    x[out] = math.nan
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    want, tol = plain(x, w, t, d, 7)
+    loss = linear_cross_entropy(x, w, t, ignore_index=7, reduction="none")
+    dx, dw = torch.autograd.grad(loss, [x, w], d)
+    for got, a, b, what in zip((loss.detach(), dx, dw), want, tol, ("loss", "dx", "dw")):
+        within(got, a, b, what)
+    assert not dx[t == 7].any() and not loss[t == 7].any()
+    mean = linear_cross_entropy(x, w, t, ignore_index=7)
+    n = int((t != 7).sum())
+    assert abs(float(mean.detach()) - float(want[0].sum()) / max(1, n)) <= float(tol[0].sum()) / max(1, n) + U * abs(float(mean))
+    if share == 0.3:  # a target that is no word
+        t[(t != 7).nonzero()[3]] = V
+        x = x.detach().requires_grad_(True)
+        want, tol = plain(x, w, t, d, 7)
+        loss = linear_cross_entropy(x, w, t, ignore_index=7, reduction="none")
+        dx, = torch.autograd.grad(loss, [x], d)
+        within(loss.detach(), want[0], tol[0], "loss")
+        within(dx, want[1], tol[1], "dx")
+
+
 def test_views_and_magnitudes(dev):
     """Strided rows, unaligned bases, and inputs whose size fp16 does not hold."""
     from linear_loss import linear_cross_entropy
@@ -224,7 +256,12 @@ def test_difference_quotients(dev):
 def test_streams_graphs_and_repeats(dev):
     """Another stream than the tensors' own, and captured graphs replayed among eager calls, give the eager bits."""
     from linear_loss import linear_cross_entropy
-    x, w, t, _ = inputs(dev, 130, 128, 700, torch.bfloat16, 9)
+    for N in (130, 2300):
+        streams_graphs_and_repeats(dev, N, linear_cross_entropy)
+
+
+def streams_graphs_and_repeats(dev, N, linear_cross_entropy):
+    x, w, t, _ = inputs(dev, N, 128, 700, torch.bfloat16, 9)
 
     def both(x, w, t):
         x, w = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
@@ -247,7 +284,8 @@ def test_streams_graphs_and_repeats(dev):
             out = both(xs, w, t)
         graphs.append((graph, out))
     for seed in range(3):
-        x2 = inputs(dev, 130, 128, 700, torch.bfloat16, 20 + seed)[0]
+        x2, _, t2, _ = inputs(dev, N, 128, 700, torch.bfloat16, 20 + seed)
+        t.copy_(t2)  # others are left out
         want = both(x2, w, t)
         xs.copy_(x2)
         for graph, out in graphs:
