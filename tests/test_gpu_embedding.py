@@ -1,7 +1,7 @@
 """GPU checks of the embedding lookup and its gradient against plain 64-bit forms.
 
 A row of the lookup is a product in 64 bits, rounded to 32 and then to its type: half a step of each.  A gradient is a
-64-bit sum of n terms in chunks of 32, at most n / 32 + 64 additions one after the other, each off by 2^-53 of a partial sum,
+64-bit sum of n terms in chunks of 32, at most n / 32 + 66 additions one after the other, each off by 2^-53 of a partial sum,
 which sum |dy| bounds; then a product, and half a step of 32 bits and of its type.
 """
 
@@ -77,6 +77,19 @@ def test_a_million_tokens(dev):
     ids = torch.randint(0, 300, (3, 350001), device=dev, generator=g, dtype=torch.int32)
     ids[:, ::2] = 11
     run(dev, ids, 300, 8, torch.float32, 2.0, None, g)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_runs_against_chunks(dev, dtype):
+    """Words whose tokens begin and end at every place of a chunk of 32, cover chunks exactly, and groups of 64 chunks."""
+    g = torch.Generator(device=dev)
+    g.manual_seed(2)
+    for counts in (list(range(0, 70)), [32, 32, 64, 31, 1, 33, 63, 0, 96, 5], [2048, 2048, 4096, 2047, 1, 2049, 60000, 2048],
+                   [31, 70000, 3], [70000], [65536 - 2048, 2048]):
+        ids = torch.repeat_interleave(torch.arange(len(counts), device=dev), torch.tensor(counts, device=dev))
+        ids = ids[torch.randperm(len(ids), device=dev, generator=g)]
+        run(dev, ids, len(counts) + 1, 12, dtype, 1.5, None, g)
+        run(dev, ids, len(counts), 12, dtype, 1.0, 0, g)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
