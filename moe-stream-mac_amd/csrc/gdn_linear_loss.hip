@@ -23,6 +23,10 @@
 // token's cotangent relative to the largest; those for dx do not, since it can be applied to the sum.  With fp32 inputs every
 // operand is two fp16 terms (2^-22) and every product three; a difference's second term is stored times 2^11, so that small
 // probabilities keep their bits (2^-22 of them down to 2^-29, 2^-51 below; in one term 2^-11 and 2^-40).
+//
+// Few tokens (below DOWN) read the weight so often that its scaled copy, which lies along the words, costs more than the products:
+// dx is then formed from the weight as it lies (gdn_product.h), with fp16 weights by the differences as they are, with bf16 weights
+// by two bf16 terms of them (2^-17), rows of the same operand.
 #include "gdn_common.h"
 #include "gdn_host.h"
 #include "gdn_product.h"
@@ -37,6 +41,7 @@ using namespace mm;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int NT = 256;
 constexpr int64_t COMPACT = 2048;
+constexpr int64_t DOWN = 512;
 constexpr int64_t KEPT = 1 << 26;  // differences of a piece; statistics of the parts of the words
 constexpr int64_t MOST_TOKENS = 1 << 20;  // three slots of 16 bits for each are a row pitch that a product takes
 constexpr int SHIFT = 15;          // differences are stored times 2^15
@@ -266,9 +271,12 @@ __device__ __forceinline__ float left_of(float x) {
     return (x - __half2float(__float2half(x))) * (float)(1 << LOW);
 }
 
+enum : int { ONE16 = 1, TWO16 = 2, ROWS = 3 };  // differences for dx: one fp16 term, two (fp32 inputs), two bf16 terms as rows
+
 // The differences of a piece of words, 2^15 (p - [v = t]), and times d / (the power of two over the largest |d|) for dW.
-template <class S, bool F16, int TERMS, bool DX, bool DW>
+template <class S, bool F16, int KIND, bool DX, bool DW>
 __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, const DiffArgs a) {
+    constexpr int TERMS = KIND == TWO16 ? 2 : 1;  // side by side
     __shared__ __attribute__((aligned(16))) char lds[S::LDS + S::STORE];
     const int w = wave_index(), wm = w / S::WN, wn = w % S::WN;
     char *store = lds + S::LDS + w * 4096;
@@ -297,7 +305,7 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
                     float x = __builtin_amdgcn_exp2f((z - st.x) * LOG2E) * inv;
                     if (hot == m) x -= (float)(1 << SHIFT);
                     if (words < S::BM / S::WM && m + 4 * (lane >> 4) >= words) x = 0.f;
-                    acc[i][j][q] = TERMS > 1 ? as_rounded(x) : x;
+                    acc[i][j][q] = KIND != ONE16 ? as_rounded(x) : x;
                 }
         }
         if constexpr (DX) {
@@ -310,18 +318,23 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
                     const int64_t m = m0 + 16 * i;
                     if (m >= a.kp) break;
 #pragma unroll 1
-                    for (int t = 0; t < TERMS; ++t) {
+                    for (int t = 0; t < (KIND == ONE16 ? 1 : 2); ++t) {
 #pragma unroll
                         for (int ii = 0; ii < 4; ++ii)
 #pragma unroll
                             for (int jj = 0; jj < 2; ++jj) {
                                 float y[4];
+                                constexpr int DT = KIND == ROWS ? DT_BF16 : DT_F16;
 #pragma unroll
-                                for (int k = 0; k < 4; ++k) y[k] = t ? left_of(acc[i + ii][j + jj][k]) : acc[i + ii][j + jj][k];
-                                put16(lane, store, ii, jj, ops::pack2(y[0], y[1], DT_F16), ops::pack2(y[2], y[3], DT_F16));
+                                for (int k = 0; k < 4; ++k) {
+                                    y[k] = acc[i + ii][j + jj][k];
+                                    if (t) y[k] = KIND == ROWS ? y[k] - bf16_to_f32(f32_to_bf16_cvt(y[k])) : left_of(y[k]);
+                                }
+                                put16(lane, store, ii, jj, ops::pack2_cvt(y[0], y[1], DT), ops::pack2_cvt(y[2], y[3], DT));
                             }
-                        store_rows(lane, store, reinterpret_cast<char *>(a.p + n * (TERMS * a.kp) + t * a.kp + m),
-                                   (uint32_t)(TERMS * a.kp * 2), rows, (a.kp - m) * 2, 2);
+                        uint16_t *to = KIND == ROWS ? a.p + (t * g.b.rows + n) * a.kp : a.p + n * (TERMS * a.kp) + t * a.kp;
+                        store_rows(lane, store, reinterpret_cast<char *>(to + m), (uint32_t)(TERMS * a.kp * 2), rows, (a.kp - m) * 2,
+                                   2);
                     }
                 }
             }
@@ -388,6 +401,8 @@ struct Sizes {
     int64_t N, H, V, hp, np, piece, pieces;  // hp, np: H and N in whole blocks; piece: words at a time
     int terms;
     bool compact;
+    bool down;     // dx from the weight as it lies
+    int64_t prows; // rows of the differences for dx
     int64_t parts, tokens;  // parts of the words with statistics of their own; tokens at a time in the forward pass
     Plan px, pw;
 };
@@ -396,13 +411,15 @@ static bool direct(const void *p, int64_t ld, int64_t H, int dt) {
     return dt != GDN_F32 && H % BK == 0 && ld % 8 == 0 && aligned_to(p, 16) && pitch_fits(ld * 2);
 }
 
-static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt) {
+static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt, bool direct_w) {
     Sizes s{};
     s.N = N; s.H = H; s.V = V;
     s.hp = padded(H);
     s.np = padded(N);
     s.terms = dt == GDN_F32 ? 2 : 1;
     s.compact = N >= COMPACT;
+    s.down = N < DOWN && direct_w;
+    s.prows = s.down && dt == GDN_BF16 ? 2 * N : N;
     int64_t most = KEPT / s.np / 256 * 256;
     if (most < 256) most = 256;
     s.pieces = (V + most - 1) / most;
@@ -414,7 +431,7 @@ static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt) {
     if (s.tokens > N) s.tokens = N;
     const int64_t seg = s.terms == 1 ? 1 : 3;
     const int64_t words = s.piece < V ? s.piece : V;
-    s.px = plan(N, H, seg * padded(words) / BK, 16);
+    s.px = plan(s.prows, H, seg * padded(words) / BK, s.down ? 32 : 16);
     s.pw = plan(words, H, seg * s.np / BK, 8);
     return s;
 }
@@ -459,9 +476,9 @@ static Buffers place(Space &sp, const Sizes &s, bool dx, bool dw, bool bwd, bool
     }
     b.d = sp.take<float>(s.N);
     if (dx) {
-        b.wt = sp.take<uint16_t>(s.H * across_slots(t) * padded(words));
-        b.p = sp.take<uint16_t>(s.N * t * padded(words));
-        b.acc_x = sp.take<float>((int64_t)s.px.splits * s.N * columns_of(s.H));
+        if (!s.down) b.wt = sp.take<uint16_t>(s.H * across_slots(t) * padded(words));
+        b.p = sp.take<uint16_t>(s.prows * t * padded(words));
+        b.acc_x = sp.take<float>((int64_t)s.px.splits * s.prows * columns_of(s.H));
     }
     if (dw) {
         b.xt = sp.take<uint16_t>(s.H * across_slots(t) * s.np);
@@ -487,12 +504,12 @@ static void launch_stat(Args &g, const StatArgs &a, bool scaled, hipStream_t st)
     else hipLaunchKernelGGL((stat_kernel<S, F16, false>), grid, dim3(S::NT), 0, st, g, a);
 }
 
-template <class S, bool F16, int TERMS>
+template <class S, bool F16, int KIND>
 static void launch_diff(Args &g, const DiffArgs &a, hipStream_t st) {
     const dim3 grid = tiles_of<S>(g, 1);
-    if (a.p && a.pt) hipLaunchKernelGGL((diff_kernel<S, F16, TERMS, true, true>), grid, dim3(S::NT), 0, st, g, a);
-    else if (a.p) hipLaunchKernelGGL((diff_kernel<S, F16, TERMS, true, false>), grid, dim3(S::NT), 0, st, g, a);
-    else hipLaunchKernelGGL((diff_kernel<S, F16, TERMS, false, true>), grid, dim3(S::NT), 0, st, g, a);
+    if (a.p && a.pt) hipLaunchKernelGGL((diff_kernel<S, F16, KIND, true, true>), grid, dim3(S::NT), 0, st, g, a);
+    else if (a.p) hipLaunchKernelGGL((diff_kernel<S, F16, KIND, true, false>), grid, dim3(S::NT), 0, st, g, a);
+    else if constexpr (KIND != ROWS) hipLaunchKernelGGL((diff_kernel<S, F16, KIND, false, true>), grid, dim3(S::NT), 0, st, g, a);
 }
 
 // 16-bit inputs as they are, fp32 inputs as two fp16 terms.
@@ -502,10 +519,11 @@ static void launch_stat_of(Args &g, const StatArgs &a, int dt, hipStream_t st) {
     else launch_stat<S, true>(g, a, dt == GDN_F32, st);
 }
 template <class S>
-static void launch_diff_of(Args &g, const DiffArgs &a, int dt, hipStream_t st) {
-    if (dt == GDN_BF16) launch_diff<S, false, 1>(g, a, st);
-    else if (dt == GDN_F16) launch_diff<S, true, 1>(g, a, st);
-    else launch_diff<S, true, 2>(g, a, st);
+static void launch_diff_of(Args &g, const DiffArgs &a, int dt, bool rows, hipStream_t st) {
+    if (dt == GDN_F32) launch_diff<S, true, TWO16>(g, a, st);
+    else if (dt == GDN_F16) launch_diff<S, true, ONE16>(g, a, st);
+    else if (rows) launch_diff<S, false, ROWS>(g, a, st);
+    else launch_diff<S, false, ONE16>(g, a, st);
 }
 
 #define GDN_BY_SHAPE(shape, call)              \
@@ -532,7 +550,7 @@ extern "C" size_t gdn_linear_loss_workspace_bytes(int64_t N, int64_t H, int64_t 
                                                   int want_dw) {
     if (N <= 0 || H <= 0 || V <= 0 || N > MOST_TOKENS || V > 1 << 24 || H > 1 << 17) return 0;
     const bool copy = !aligned || dtype == GDN_F32 || H % BK;
-    return need(sizes(N, H, V, dtype), want_dx, want_dw, want_dx || want_dw, copy, copy);
+    return need(sizes(N, H, V, dtype, !copy), want_dx, want_dw, want_dx || want_dw, copy, copy);
 }
 
 extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *targets, float *loss, float *stat, float *total,
@@ -546,8 +564,9 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
     if (N == 0 && !reduction) return GDN_OK;
     if (N > 0) {
         if (!x || !w || !targets || !loss || !workspace) return fail(GDN_ERR_INVALID, "null pointer");
-        const Sizes s = sizes(N, H, V, dtype);
-        const bool dx = !s.compact && direct(x, x_stride, H, dtype), dw = direct(w, w_stride, H, dtype);
+        const bool dw = direct(w, w_stride, H, dtype);
+        const Sizes s = sizes(N, H, V, dtype, dw);
+        const bool dx = !s.compact && direct(x, x_stride, H, dtype);
         const size_t bytes = need(s, false, false, false, !dx, !dw);
         if (workspace_bytes < bytes)
             return fail(GDN_ERR_WORKSPACE, "the workspace holds %zu bytes, %zu are needed", workspace_bytes, bytes);
@@ -562,9 +581,8 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
         if (s.compact)
             hipLaunchKernelGGL(tokens_kernel, dim3(1), dim3(1024), 0, st, targets, N, ignore_index, tk, loss);
         if (dtype == GDN_F32) {
-            maxima(sx, b.part + E_X * PARTS, st);
-            maxima(sw, b.part + E_W * PARTS, st);
-            exponents(b.part, 2, TOP, b.exps, st);
+            maxima({sx, sw}, b.part, st);
+            exponents(b.part, Tops{{TOP, TOP, 0}}, b.exps, st);  // the third is not read
             exps = b.exps;
         }
         if (!dx) terms(sx, s.terms, f16, exps, E_X, b.x, st);
@@ -635,8 +653,9 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (N == 0) return fail(GDN_ERR_INVALID, "no tokens: the gradients are zeros, which this call does not write");
     if (!x || !w || !targets || !stat || !dloss || !workspace) return fail(GDN_ERR_INVALID, "null pointer");
-    const Sizes s = sizes(N, H, V, dtype);
-    const bool direct_x = !s.compact && direct(x, x_stride, H, dtype), direct_w = direct(w, w_stride, H, dtype);
+    const bool direct_w = direct(w, w_stride, H, dtype);
+    const Sizes s = sizes(N, H, V, dtype, direct_w);
+    const bool direct_x = !s.compact && direct(x, x_stride, H, dtype);
     const size_t bytes = need(s, dx, dw, true, !direct_x, !direct_w);
     if (workspace_bytes < bytes)
         return fail(GDN_ERR_WORKSPACE, "the workspace holds %zu bytes, %zu are needed", workspace_bytes, bytes);
@@ -651,10 +670,11 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
     if (s.compact) hipLaunchKernelGGL(tokens_kernel, dim3(1), dim3(1024), 0, st, targets, N, ignore_index, tk, nullptr);
     hipLaunchKernelGGL(cotangent_kernel, dim3(PARTS), dim3(NT), 0, st, tt, dloss, dloss_stride, factor, N, V, ignore_index,
                        b.d, b.part + E_D * PARTS, tk.index, tk.count);
-    maxima(sx, b.part + E_X * PARTS, st);
-    maxima(sw, b.part + E_W * PARTS, st);
-    exponents(b.part, 2, TOP, b.exps, st);
-    exponents(b.part + E_D * PARTS, 1, -1, b.exps + E_D, st);  // |d| below 1
+    Source mx = sx, mw = sw;  // what is stored times a power of two
+    if (!dw && dtype != GDN_F32) mx.rows = 0;
+    if ((!dx || s.down) && dtype != GDN_F32) mw.rows = 0;
+    if (mx.rows + mw.rows > 0) maxima({mx, mw}, b.part, st);
+    if (mx.rows + mw.rows > 0) exponents(b.part, Tops{{TOP, TOP, -1}}, b.exps, st);  // |d| below 1
     const int *exps = dtype == GDN_F32 ? b.exps : nullptr;
     if (!direct_x) terms(sx, t, f16, exps, E_X, b.x, st);
     if (dw) terms_across(sx, t, true, b.exps, E_X, b.xt, st);
@@ -684,24 +704,32 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
         const DiffArgs a{tt, reinterpret_cast<const float2 *>(stat), b.d, b.exps, b.p, b.pt, v0, kp, s.np};
         {
             Timed tm("loss_diff", st);
-#define GDN_DIFF(S) launch_diff_of<S>(g, a, dtype, st)
+#define GDN_DIFF(S) launch_diff_of<S>(g, a, dtype, s.down && dx, st)
             GDN_BY_SHAPE(shape, GDN_DIFF)
 #undef GDN_DIFF
         }
         if (dx) {
-            terms_across(part, t, true, b.exps, E_W, b.wt, st);
             Args h{};
-            segments(h, t, kp, true);
-            h.a.p = reinterpret_cast<const char *>(b.wt);
-            h.a.rows = H;
+            if (s.down) {
+                h.a = Operand{static_cast<const char *>(part.p), w_stride * 2, H, {0, 0, 0}};
+                h.b.ld = kp * 2;
+                h.kit = (int)(kp / BK);
+                h.nseg = 1;
+                h.down = words;
+            } else {
+                terms_across(part, t, true, b.exps, E_W, b.wt, st);
+                segments(h, t, kp, true);
+                h.a.p = reinterpret_cast<const char *>(b.wt);
+                h.a.rows = H;
+            }
             h.b.p = reinterpret_cast<const char *>(b.p);
-            h.b.rows = N;
+            h.b.rows = s.prows;
             h.live = tk.count;
             const Plan pl = s.px;  // parts without a block of the last piece add nothing
-            Result r{dx, H, dtype, b.d, b.exps, -SHIFT, {0, -1, 0}, nullptr, columns_of(H), v0 > 0, tk.place};
-            if (s.compact || s.pieces > 1 || pl.splits > 1) r.acc = b.acc_x;
-            multiply(h, true, pl, r, st);
-            if (r.acc && v0 + words == V) finish(r, pl.splits, N, H, st);
+            Result r{dx, H, dtype, b.d, b.exps, -SHIFT, {0, s.down ? 0 : -1, 0}, nullptr, columns_of(H), v0 > 0, tk.place};
+            if (s.down || s.compact || s.pieces > 1 || pl.splits > 1) r.acc = b.acc_x;
+            multiply(h, !s.down || dtype == GDN_F16, pl, r, st);
+            if (r.acc && v0 + words == V) finish(r, pl.splits * (int)(s.prows / N), N, H, st);  // terms are parts too
         }
         if (dw) {
             Args h{};

@@ -61,6 +61,7 @@ struct Args {
     const int *live;
     int64_t live0;
     int live_k;
+    int64_t down;  // not 0: A lies across the contraction, this many rows of a.rows columns; one segment, results in parts
 };
 struct Extent {
     int64_t rows_b;
@@ -123,14 +124,24 @@ __device__ __forceinline__ void tile_of(int id, int mt, int nt, int &tm, int &tn
     tn = r / width;
 }
 
+// A may also lie across the contraction (DOWN): rows of m, one for each k, read as they are and turned by LDS reads that transpose
+// 4 x 16 numbers.  32 bytes, what such a read takes of a row, lie in place (pair ^ down_swizzle(row)) of the row's, so that the
+// 16 rows of one read fill all banks twice.  Rows behind the last (g.down of them) read as zeros.
+__device__ __forceinline__ int down_swizzle(int row) { return (row & 3) | (row >> 3 & 1) << 2; }
+// The chunk of 16 bytes of a row that lies in place p.
+__device__ __forceinline__ int down_chunk(int p, int row) { return ((p >> 1) ^ down_swizzle(row)) << 1 | (p & 1); }
+
 // A workgroup's walk over its tiles and their blocks: tiles blockIdx.x, blockIdx.x + gridDim.x, ..., each from block `first`
 // to `end`.  It runs two blocks ahead of the products, over the border between two tiles too, so that the next tile's first
 // loads are under way while results are written.
-template <class S>
+template <class S, bool DOWN>
 struct Loader {
+    static constexpr int ROW = S::BM * 2, LANES = S::BM / 8, ROUND = S::NT / LANES;  // DOWN: a row's bytes, its lanes, rows a load
     const char *pa, *pb;  // of the block to load next
     uint32_t va, vb, na, nb;  // this thread's offset in a tile, and the bytes that loads may reach: none behind the last row
     uint32_t step_a, step_b;  // from one load's rows to the next one's
+    uint32_t va_odd;          // DOWN: va of odd loads
+    int64_t rest;             // DOWN: bytes from pa to the operand's end
     int left, seg_left, seg, tile, tiles, w;  // blocks left of the tile and of the segment
 
     __device__ __forceinline__ void start(const Args &g, const Extent &x, int first, int end) {  // of a tile
@@ -138,19 +149,32 @@ struct Loader {
         tile_of(tile, g.mt, x.nt, tm, tn);
         const int lane = threadIdx.x & 63, r0 = (threadIdx.x >> 3);
         const uint32_t chunk = ((lane & 7) ^ (r0 >> 1 & 7)) << 4;
-        const int ma = (int)min((int64_t)S::BM, g.a.rows - (int64_t)tm * S::BM);
         const int mb = (int)min((int64_t)S::BN, x.rows_b - (int64_t)tn * S::BN);
-        va = (uint32_t)r0 * (uint32_t)g.a.ld + chunk;
+        if constexpr (DOWN) {
+            const int r = threadIdx.x / LANES, p = threadIdx.x % LANES;
+            va = (uint32_t)r * (uint32_t)g.a.ld + down_chunk(p, r) * 16;
+            va_odd = (uint32_t)r * (uint32_t)g.a.ld + down_chunk(p, r + ROUND) * 16;
+            step_a = (uint32_t)ROUND * (uint32_t)g.a.ld;
+        } else {
+            const int ma = (int)min((int64_t)S::BM, g.a.rows - (int64_t)tm * S::BM);
+            va = (uint32_t)r0 * (uint32_t)g.a.ld + chunk;
+            na = (uint32_t)(ma - 1) * (uint32_t)g.a.ld + BK * 2;
+            step_a = (uint32_t)(S::NT / 8) * (uint32_t)g.a.ld;
+        }
         vb = (uint32_t)r0 * (uint32_t)g.b.ld + chunk;
-        na = (uint32_t)(ma - 1) * (uint32_t)g.a.ld + BK * 2;
         nb = (uint32_t)(mb - 1) * (uint32_t)g.b.ld + BK * 2;
-        step_a = (uint32_t)(S::NT / 8) * (uint32_t)g.a.ld;
         step_b = (uint32_t)(S::NT / 8) * (uint32_t)g.b.ld;
         left = end - first;
         seg = first / x.kit;
         const int kk = first - seg * x.kit;
         seg_left = x.kit - kk;
-        pa = g.a.p + (int64_t)tm * S::BM * g.a.ld + g.a.off[seg] + (int64_t)kk * (BK * 2);
+        if constexpr (DOWN) {
+            const int64_t at = (int64_t)kk * BK * g.a.ld + (int64_t)tm * S::BM * 2;
+            pa = g.a.p + at;
+            rest = (g.down - 1) * g.a.ld + g.a.rows * 2 - at;
+        } else {
+            pa = g.a.p + (int64_t)tm * S::BM * g.a.ld + g.a.off[seg] + (int64_t)kk * (BK * 2);
+        }
         pb = g.b.p + (int64_t)tn * S::BN * g.b.ld + g.b.off[seg] + (int64_t)kk * (BK * 2);
     }
     // Loads [R0, R1) of a block's RA + RB.  Rows behind the last read as zeros.
@@ -158,13 +182,14 @@ struct Loader {
     __device__ __forceinline__ void load(char *__restrict__ dst) const {
 #ifdef __HIP_DEVICE_COMPILE__  // the host's pass does not know buffer resources
         constexpr int RAW = 0x00020000;
-        const auto a = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(pa), 0, na, RAW);
+        const uint32_t la = DOWN ? (uint32_t)min(max(rest, (int64_t)0), (int64_t)1 << 31) : na;
+        const auto a = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(pa), 0, la, RAW);
         const auto b = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(pb), 0, nb, RAW);
 #pragma unroll
         for (int r = R0; r < R1; ++r) {
             lvoid *to = (lvoid *)(dst + r * (S::NT * 16) + w * 1024);
             if (r < S::RA)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(a, to, 16, va + r * step_a, 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(a, to, 16, (DOWN && r % 2 ? va_odd : va) + r * step_a, 0, 0, 0);
             else
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(b, to, 16, vb + (r - S::RA) * step_b, 0, 0, 0);
         }
@@ -173,12 +198,22 @@ struct Loader {
     // On to the next block; after the very last one it stays there, so that loads need no branch around them.
     __device__ __forceinline__ void next(const Args &g, const Extent &x, int first, int end) {
         if (left > 1) {
-            pa += BK * 2;
+            if constexpr (DOWN) {
+                pa += BK * g.a.ld;
+                rest -= BK * g.a.ld;
+            } else {
+                pa += BK * 2;
+            }
             pb += BK * 2;
             --left;
             if (--seg_left == 0) {
                 seg_left = x.kit;
-                pa += g.a.off[seg + 1] - g.a.off[seg] - (int64_t)x.kit * (BK * 2);
+                if constexpr (DOWN) {
+                    pa -= (int64_t)x.kit * BK * g.a.ld;
+                    rest += (int64_t)x.kit * BK * g.a.ld;
+                } else {
+                    pa += g.a.off[seg + 1] - g.a.off[seg] - (int64_t)x.kit * (BK * 2);
+                }
                 pb += g.b.off[seg + 1] - g.b.off[seg] - (int64_t)x.kit * (BK * 2);
                 ++seg;
             }
@@ -200,17 +235,32 @@ __device__ __forceinline__ void stage_barrier() {
 }
 
 // The fragments of a block: two steps of 32 along the contraction; A's rows in two halves.
-template <class S>
+template <class S, bool DOWN>
 struct Frags {
     static constexpr int H = S::TM / 2;
     u4 lo[2][H], hi[2][H], b[2][S::TN];
+    // Tile i of A: 16 bytes of a row, or DOWN two reads of four rows each, at_a[0] the lane's place in a row of tile 0 and at_a[1]
+    // its swizzle.
+    __device__ __forceinline__ static u4 read_a(const char *__restrict__ lds, const uint32_t (&at_a)[2], int k, int i) {
+        if constexpr (DOWN) {
+            typedef short s4 __attribute__((ext_vector_type(4)));
+            typedef short s8 __attribute__((ext_vector_type(8)));
+            typedef __attribute__((address_space(3))) s4 lds_s4;
+            const char *at = lds + at_a[0] + k * 32 * S::BM * 2 + ((uint32_t)(i * 32) ^ at_a[1]);
+            const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)at);
+            const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(at + 4 * S::BM * 2));
+            return __builtin_bit_cast(u4, (s8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            return *reinterpret_cast<const u4 *>(lds + at_a[k] + i * 16 * BK * 2);
+        }
+    }
     __device__ __forceinline__ void read_lo(const char *__restrict__ lds, const uint32_t (&at_a)[2], int k) {
 #pragma unroll
-        for (int i = 0; i < H; ++i) lo[k][i] = *reinterpret_cast<const u4 *>(lds + at_a[k] + i * 16 * BK * 2);
+        for (int i = 0; i < H; ++i) lo[k][i] = read_a(lds, at_a, k, i);
     }
     __device__ __forceinline__ void read_hi(const char *__restrict__ lds, const uint32_t (&at_a)[2], int k) {
 #pragma unroll
-        for (int i = 0; i < H; ++i) hi[k][i] = *reinterpret_cast<const u4 *>(lds + at_a[k] + (H + i) * 16 * BK * 2);
+        for (int i = 0; i < H; ++i) hi[k][i] = read_a(lds, at_a, k, H + i);
     }
     __device__ __forceinline__ void read_b(const char *__restrict__ lds, const uint32_t (&at_b)[2], int k) {
 #pragma unroll
@@ -234,10 +284,10 @@ struct Frags {
 
 // First half of a block: the products of A's lower rows, while the rest of the block's fragments are read, one between two
 // products, and the first product before them (its wait is for what the last half has read).
-template <class S, bool F16>
+template <class S, bool F16, bool DOWN>
 __device__ __forceinline__ void first_half(const char *__restrict__ rd, const uint32_t (&at_a)[2], const uint32_t (&at_b)[2],
-                                           Frags<S> &f, acc_t (&acc)[S::TM][S::TN]) {
-    constexpr int READS = S::TN + 2 * Frags<S>::H, PRODUCTS = Frags<S>::H * S::TN;
+                                           Frags<S, DOWN> &f, acc_t (&acc)[S::TM][S::TN]) {
+    constexpr int H = S::TM / 2, READS = S::TN + 2 * H * (DOWN ? 2 : 1), PRODUCTS = H * S::TN;
     f.template mul_lo<F16>(acc, 0);
     f.read_b(rd, at_b, 1);
     f.read_hi(rd, at_a, 0);
@@ -257,11 +307,11 @@ __device__ __forceinline__ void first_half(const char *__restrict__ rd, const ui
 // Second half: the products of A's upper rows, while the block after the next is loaded into this one's LDS and the next
 // one's fragments are read in the place of those that no product needs any more.  A load takes the memory pipe 16 cycles for
 // each of the workgroup's waves, so loads stand between products: in one run they held the products up.
-template <class S, bool F16>
-__device__ __forceinline__ void second_half(const char *__restrict__ rd, char *__restrict__ wr, const Loader<S> &ld,
-                                            const uint32_t (&at_a)[2], const uint32_t (&at_b)[2], Frags<S> &f,
+template <class S, bool F16, bool DOWN>
+__device__ __forceinline__ void second_half(const char *__restrict__ rd, char *__restrict__ wr, const Loader<S, DOWN> &ld,
+                                            const uint32_t (&at_a)[2], const uint32_t (&at_b)[2], Frags<S, DOWN> &f,
                                             acc_t (&acc)[S::TM][S::TN]) {
-    constexpr int R = S::RA + S::RB, P = Frags<S>::H * S::TN, READS = 2 * Frags<S>::H;
+    constexpr int R = S::RA + S::RB, P = S::TM / 2 * S::TN, READS = S::TM * (DOWN ? 2 : 1);
     ld.template load<0, R / 2>(wr);
     f.template mul_hi<F16>(acc, 0);
     f.read_lo(rd, at_a, 0);
@@ -295,13 +345,13 @@ __device__ __forceinline__ void clear(acc_t (&acc)[S::TM][S::TN]) {
 
 // Forms the workgroup's tiles and hands each to epilogue(tm, tn, acc).
 // acc[i][j]: rows m = 16 i + 4 (lane / 16) + q of this wave's part for register q, column n = 16 j + lane % 16.
-template <class S, bool F16, class E>
+template <class S, bool F16, bool DOWN = false, class E>
 __device__ __forceinline__ void products(const Args &g, const Extent &x, char *lds, E &&epilogue) {
     const int lane = threadIdx.x & 63, w = wave_index(), wm = w / S::WN, wn = w % S::WN;
     const int total = x.kit * g.nseg;
     const int first = (int)((int64_t)total * blockIdx.z / g.splits), end = (int)((int64_t)total * (blockIdx.z + 1) / g.splits);
     const int blocks = end - first, mt = g.mt, nt = x.nt;
-    Loader<S> ld;
+    Loader<S, DOWN> ld;
     ld.tile = blockIdx.x;
     ld.tiles = mt * nt;
     ld.w = w;
@@ -312,6 +362,11 @@ __device__ __forceinline__ void products(const Args &g, const Extent &x, char *l
         const uint32_t c = ((k * 4 + (lane >> 4)) ^ (lane >> 1 & 7)) << 4;
         at_a[k] = (wm * (S::BM / S::WM) + (lane & 15)) * BK * 2 + c;
         at_b[k] = S::A_BYTES + (wn * (S::BN / S::WN) + (lane & 15)) * BK * 2 + c;
+    }
+    if constexpr (DOWN) {
+        const int row = 8 * (lane >> 4) + (lane >> 2 & 3), first_pair = wm * S::TM;  // of a multiple of 4, a power of two
+        at_a[0] = row * S::BM * 2 + (lane & 3) * 8 + (first_pair & ~7) * 32;
+        at_a[1] = (uint32_t)(down_swizzle(row) ^ (first_pair & 7)) * 32;
     }
     char *cur = lds, *other = lds + S::STAGE;
     if (blocks > 0) {  // else empty sums
@@ -326,17 +381,17 @@ __device__ __forceinline__ void products(const Args &g, const Extent &x, char *l
         acc_t acc[S::TM][S::TN];
         clear<S>(acc);
         // read anew for each tile, so that their registers are free while results are written
-        Frags<S> f;
+        Frags<S, DOWN> f;
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             f.read_lo(cur, at_a, k);
             if (k < 1) f.read_b(cur, at_b, k);
         }
         for (int n = 0; n < blocks; ++n) {
-            first_half<S, F16>(cur, at_a, at_b, f, acc);
+            first_half<S, F16, DOWN>(cur, at_a, at_b, f, acc);
             stage_barrier();
             // after a tile's last block no product uses what this reads
-            second_half<S, F16>(other, cur, ld, at_a, at_b, f, acc);
+            second_half<S, F16, DOWN>(other, cur, ld, at_a, at_b, f, acc);
             ld.next(g, x, first, end);
             char *c = cur;
             cur = other;

@@ -6,13 +6,13 @@ namespace mm {
 
 enum : int { OUT16 = 0, OUT32 = 1, PARTS = 2 };
 
-template <class S, bool F16, int KIND>
+template <class S, bool F16, int KIND, bool DOWN>
 __global__ __launch_bounds__(S::NT, S::WAVES_EU) void product_kernel(const Args g, const Result r) {
     __shared__ __attribute__((aligned(16))) char lds[S::LDS + S::STORE];
     const int w = wave_index(), wm = w / S::WN, wn = w % S::WN;
     char *st = lds + S::LDS + w * 4096;
     const Extent ext = extent_of<S>(g);
-    products<S, F16>(g, ext, lds, [&](int tm, int tn, acc_t(&acc)[S::TM][S::TN]) {
+    products<S, F16, DOWN>(g, ext, lds, [&](int tm, int tn, acc_t(&acc)[S::TM][S::TN]) {
         const int lane = lane_here();
         const int64_t m0 = (int64_t)tm * S::BM + wm * (S::BM / S::WM), n0 = (int64_t)tn * S::BN + wn * (S::BN / S::WN);
         const int e = KIND == PARTS ? 0 : exponent_of(r);
@@ -81,7 +81,9 @@ __global__ __launch_bounds__(NT) void finish_kernel(const Result r, int splits, 
     const int64_t at = r.place ? r.place[n] : n;
     const float f = at < 0 ? 0.f : r.row ? r.row[at] : 1.f;
     float s[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int z = 0; z < splits && at >= 0; ++z) {
+    if (at < 0) splits = 0;
+#pragma unroll 8
+    for (int z = 0; z < splits; ++z) {
         const float4 v = *reinterpret_cast<const float4 *>(r.acc + (z * rows + at) * r.ldp + m);
         s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
     }
@@ -101,9 +103,10 @@ void finish(const Result &r, int splits, int64_t rows, int64_t cols, hipStream_t
 template <class S, bool F16>
 static void launch(Args &g, int splits, const Result &r, hipStream_t st) {
     const dim3 grid = tiles_of<S>(g, splits);
-    if (r.acc) hipLaunchKernelGGL((product_kernel<S, F16, PARTS>), grid, dim3(S::NT), 0, st, g, r);
-    else if (r.dt == DT_F32) hipLaunchKernelGGL((product_kernel<S, F16, OUT32>), grid, dim3(S::NT), 0, st, g, r);
-    else hipLaunchKernelGGL((product_kernel<S, F16, OUT16>), grid, dim3(S::NT), 0, st, g, r);
+    if (g.down) hipLaunchKernelGGL((product_kernel<S, F16, PARTS, true>), grid, dim3(S::NT), 0, st, g, r);
+    else if (r.acc) hipLaunchKernelGGL((product_kernel<S, F16, PARTS, false>), grid, dim3(S::NT), 0, st, g, r);
+    else if (r.dt == DT_F32) hipLaunchKernelGGL((product_kernel<S, F16, OUT32, false>), grid, dim3(S::NT), 0, st, g, r);
+    else hipLaunchKernelGGL((product_kernel<S, F16, OUT16, false>), grid, dim3(S::NT), 0, st, g, r);
 }
 template <class S>
 static void launch(Args &g, bool f16, int splits, const Result &r, hipStream_t st) {

@@ -23,11 +23,12 @@ constexpr int PARTS = 512;  // partial maxima of one matrix
 // Elements of a row of `cols`, filled up to whole blocks of the contraction.
 inline int64_t padded(int64_t cols) { return (cols + 63) / 64 * 64; }
 
-// part[PARTS] = partial maxima of the finite magnitudes of s (of v[n] where targets[n] != ignore for maxima_of).
-void maxima(const Source &s, float *part, hipStream_t st);
+// part[i][PARTS] = partial maxima of the finite magnitudes of s[i], i < 2, matrices of one type; without rows: zeros.
+void maxima(const Source (&s)[2], float *part, hipStream_t st);
 
-// exps[i] = the exponent e_i that takes the largest of part[i][PARTS] to [2^top, 2^(top + 1)), for i < n; 0 for zeros.
-void exponents(const float *part, int n, int top, int *exps, hipStream_t st);
+// exps[i] = the exponent e_i that takes the largest of part[i][PARTS] to [2^top[i], 2^(top[i] + 1)), for i < 3; 0 for zeros.
+struct Tops { int top[3]; };
+void exponents(const float *part, const Tops &top, int *exps, hipStream_t st);
 
 // dst[r][t * padded(cols) + c] = term t of 2^e s[r][c], e = exps[which] (0 without exps), zeros behind the last column: x is
 // the sum of its terms up to the last one's rounding.  f16 or bf16 terms.

@@ -30,14 +30,18 @@ __device__ __forceinline__ float magnitude(float x) {
     return a <= 3.4028234e38f ? a : 0.f;  // neither infinite nor NaN
 }
 
-// A wave to a row, 2048 elements at a time.
+struct Pair { Source s[2]; };
+
+// A wave to a row, 2048 elements at a time; the first PARTS workgroups for the first matrix.
 template <int DT>
-__global__ __launch_bounds__(1024) void maxima_kernel(const Source s, float *part) {
+__global__ __launch_bounds__(1024) void maxima_kernel(const Pair both, float *part) {
     constexpr int WAVES = 16, U = 4;
     __shared__ float red[WAVES];
+    const int which = blockIdx.x / PARTS, block = blockIdx.x % PARTS;
+    const Source &s = both.s[which];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     float m = 0.f;
-    for (int64_t r = blockIdx.x * WAVES + w; r < s.rows; r += PARTS * WAVES) {
+    for (int64_t r = block * WAVES + w; r < s.rows; r += PARTS * WAVES) {
         const int64_t at = row_of(s, r);
         if (at < 0) continue;
         for (int64_t c = lane * 8; c < s.cols; c += U * 512) {
@@ -60,15 +64,16 @@ __global__ __launch_bounds__(1024) void maxima_kernel(const Source s, float *par
     }
 }
 
-__global__ __launch_bounds__(64) void exponents_kernel(const float *part, int top, int *exps) {
+__global__ __launch_bounds__(64) void exponents_kernel(const float *part, const Tops tops, int *exps) {
+    const int i = blockIdx.x, top = i == 0 ? tops.top[0] : i == 1 ? tops.top[1] : tops.top[2];
     float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < PARTS / 64; ++i) m = fmaxf(m, part[blockIdx.x * PARTS + i * 64 + threadIdx.x]);
+    for (int k = 0; k < PARTS / 64; ++k) m = fmaxf(m, part[i * PARTS + k * 64 + threadIdx.x]);
     m = wave_max(m);
     if (threadIdx.x == 0) {
         int e = 0;
         if (m > 0.f) (void)frexpf(m, &e);  // m in [2^(e - 1), 2^e)
-        exps[blockIdx.x] = m > 0.f ? top + 1 - e : 0;
+        exps[i] = m > 0.f ? top + 1 - e : 0;
     }
 }
 
@@ -158,22 +163,23 @@ __global__ __launch_bounds__(NT) void across_kernel(const Source s, int slots, c
     }
 }
 
-void maxima(const Source &s0, float *part, hipStream_t st) {
+void maxima(const Source (&s)[2], float *part, hipStream_t st) {
     Timed tm("maxima", st);
     constexpr int64_t LONG = 8192;
-    Source s = s0;
-    if (s.ld == s.cols && !s.targets && !s.index && s.rows * s.cols % LONG == 0) {  // rows in one piece: of any length
-        s.rows = s.rows * s.cols / LONG;
-        s.ld = s.cols = LONG;
-    }
-    const dim3 grid(PARTS), block(1024);
-    if (s.dt == DT_F32) hipLaunchKernelGGL((maxima_kernel<DT_F32>), grid, block, 0, st, s, part);
-    else if (s.dt == DT_BF16) hipLaunchKernelGGL((maxima_kernel<DT_BF16>), grid, block, 0, st, s, part);
-    else hipLaunchKernelGGL((maxima_kernel<DT_F16>), grid, block, 0, st, s, part);
+    Pair p{{s[0], s[1]}};
+    for (Source &m : p.s)
+        if (m.ld == m.cols && !m.targets && !m.index && m.rows * m.cols % LONG == 0) {  // rows in one piece: of any length
+            m.rows = m.rows * m.cols / LONG;
+            m.ld = m.cols = LONG;
+        }
+    const dim3 grid(2 * PARTS), block(1024);
+    if (s[0].dt == DT_F32) hipLaunchKernelGGL((maxima_kernel<DT_F32>), grid, block, 0, st, p, part);
+    else if (s[0].dt == DT_BF16) hipLaunchKernelGGL((maxima_kernel<DT_BF16>), grid, block, 0, st, p, part);
+    else hipLaunchKernelGGL((maxima_kernel<DT_F16>), grid, block, 0, st, p, part);
 }
 
-void exponents(const float *part, int n, int top, int *exps, hipStream_t st) {
-    hipLaunchKernelGGL(exponents_kernel, dim3(n), dim3(64), 0, st, part, top, exps);
+void exponents(const float *part, const Tops &top, int *exps, hipStream_t st) {
+    hipLaunchKernelGGL(exponents_kernel, dim3(3), dim3(64), 0, st, part, top, exps);
 }
 
 #define GDN_TERMS_OF(KERNEL, F16, ...)                                                                                \
