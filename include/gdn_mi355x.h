@@ -389,7 +389,7 @@ int gdn_embedding_bwd(const int64_t *ids, const void *dy, void *dw, void *worksp
  * codes [N][ceil(K / 32) * 16], on 16 bytes: two elements to a byte, the even one low, each a sign and one of 0, 0.5, 1, 1.5, 2,
  * 3, 4, 6; scales [N][ceil(K / 32)]: biased exponents of a block's power of two, 255 for NaN.  Quantisation takes a block's
  * largest magnitude to [4, 8), rounds to the nearest (ties to the even code) and ends at 6; a block with an infinite or NaN
- * element has scale 255.  gdn_mxfp4_dequantize writes the values, contiguous (dtype, on 16 bytes).
+ * element has scale 255.  gdn_mxfp4_dequantize writes the values, contiguous (dtype).
  *
  * gdn_mxfp4_linear: y [M][N] = x w^T, gdn_mxfp4_linear_bwd: dx [M][K] = dy w (x, dy of dtype, rows x_stride or dy_stride
  * elements apart; y, dx contiguous, of dtype); the weight's values and every bit of x or dy enter 32-bit sums.  A forward call

@@ -23,85 +23,87 @@ using namespace mm;
 
 constexpr int NT = 256;
 constexpr int MOST = 64;                 // tokens that read the 4-bit weight itself
+constexpr int WAVES = 8;                 // along K, for these
 constexpr int64_t KEPT = 1 << 26;        // elements of the copy at a time
 typedef float f4 __attribute__((ext_vector_type(4)));
-typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+
+// i / d, in 32 bits where that does (a division in 64 bits costs more than the rest of a streaming kernel's work on 16 bytes).
+__device__ __forceinline__ int64_t divided(int64_t i, uint32_t d) { return i >> 32 ? i / d : (uint32_t)i / d; }
 
 // ------------------------------------------------------------------------------------------------ quantisation
 
 // Four lanes to a block, eight elements to a lane.
-template <bool WIDE>
+template <int DT>
 __global__ __launch_bounds__(NT) void quantize_kernel(const void *w, uint32_t *codes, uint8_t *scales, int64_t N, int64_t K,
-                                                      int64_t ld, int64_t blocks, int dt) {
-    const int64_t i = block_index() * NT + threadIdx.x, n = i / (blocks * 4), c = (i - n * blocks * 4) * 8;
+                                                      int64_t ld, int64_t blocks) {
+    const int64_t i = block_index() * NT + threadIdx.x, n = divided(i, (uint32_t)blocks * 4), c = (i - n * blocks * 4) * 8;
     if (n >= N) return;  // whole blocks
     float x[8];
-    if (WIDE && c + 8 <= K) {
-        ops::loadv<8>(w, n * ld + c, dt, x);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = c + j < K ? load_as_f32(w, n * ld + c + j, dt) : 0.f;
-    }
+    ops::load_first<8, DT>(w, n * ld + c, K - c, x);
     uint32_t top = 0;  // magnitudes are ordered as their bits, NaN above all
 #pragma unroll
     for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
     top = max(top, (uint32_t)__shfl_xor((int)top, 1));
     top = max(top, (uint32_t)__shfl_xor((int)top, 2));
-    int e = -127;
-    if (top > 0) {
-        (void)frexpf(__uint_as_float(top), &e);  // in [2^(e - 1), 2^e)
-        e = max(e - 3, -127);
-    }
+    // the largest magnitude's biased exponent less 2 (a subnormal one's is 0, and so is the scale's)
     const bool odd = top >= 0x7f800000u;
+    const uint32_t e = odd ? 255u : max(top >> 23, 2u) - 2u;
+    const float scale = __uint_as_float(e << 23);  // only its exponent counts
     uint32_t out = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float m = ldexpf(fabsf(x[j]), -e);
-        uint32_t q = (m > 0.25f) + (m >= 0.75f) + (m > 1.25f) + (m >= 1.75f) + (m > 2.5f) + (m >= 3.5f) + (m > 5.f);
-        q |= __float_as_uint(x[j]) >> 28 & 8u;
-        out |= q << (4 * j);
-    }
+    out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, x[0], x[1], scale, 0);
+    out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, x[2], x[3], scale, 1);
+    out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, x[4], x[5], scale, 2);
+    out = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(out, x[6], x[7], scale, 3);
     codes[i] = odd ? 0u : out;
-    if ((threadIdx.x & 3) == 0) scales[i >> 2] = odd ? 255 : (uint8_t)(e + 127);
+    if ((threadIdx.x & 3) == 0) scales[i >> 2] = (uint8_t)e;
 }
 
-__device__ __forceinline__ float scale_of(uint8_t s) { return s == 255 ? NAN : ldexpf(1.f, (int)s - 127); }
+typedef float f2 __attribute__((ext_vector_type(2)));
 
-__device__ __forceinline__ float value(uint32_t code, float scale) {
-    const uint32_t c = code & 7u;
-    // e2m1 above the subnormal 0.5 as fp32 bits
-    const float m = c < 2 ? 0.5f * (float)c : __uint_as_float(((c >> 1) + 126u) << 23 | (c & 1u) << 22);
-    return (code & 8u ? -m : m) * scale;
+// The scale as the conversions take it, and eight codes as bf16 numbers (four pairs).
+__device__ __forceinline__ float scale_of(uint32_t s) { return __uint_as_float(s << 23); }
+__device__ __forceinline__ u4 values_of(uint32_t c, float s) {
+    return u4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0)),
+              __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1)),
+              __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2)),
+              __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3))};
 }
 
-// Eight elements to a thread: rows of K elements (dt), or of bf16 numbers `kp` apart with zeros behind the last.
-template <bool OPERAND>
+// Eight elements to a thread: rows of K elements.
+template <int DT>
 __global__ __launch_bounds__(NT) void values_kernel(const uint32_t *codes, const uint8_t *scales, void *out, int64_t N, int64_t K,
-                                                    int64_t blocks, int64_t kp, int dt) {
-    const int64_t per = OPERAND ? kp / 8 : blocks * 4;
-    const int64_t i = block_index() * NT + threadIdx.x, n = i / per, u = i - n * per;
+                                                    int64_t blocks) {
+    const int64_t i = block_index() * NT + threadIdx.x, n = divided(i, (uint32_t)blocks * 4), u = i - n * blocks * 4;
     if (n >= N) return;
+    const uint32_t c = codes[i];
+    const float s = scale_of(scales[i >> 2]);
     float x[8];
-    if (u < blocks * 4) {
-        const uint32_t c = codes[n * blocks * 4 + u];
-        const float s = scale_of(scales[n * blocks + (u >> 2)]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = value(c >> (4 * j), s);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = 0.f;
+#define GDN_PAIR(j)                                                          \
+    {                                                                        \
+        const f2 v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, j);      \
+        x[2 * j] = v[0];                                                     \
+        x[2 * j + 1] = v[1];                                                 \
     }
-    if constexpr (OPERAND) {
+    GDN_PAIR(0) GDN_PAIR(1) GDN_PAIR(2) GDN_PAIR(3)
+#undef GDN_PAIR
+    ops::store_first<8, DT>(out, n * K + u * 8, K - u * 8, x);
+}
+
+// The same as an operand: bf16 rows `kp` elements apart, zeros behind the last (a NaN scale reaches no column that is not there).
+__global__ __launch_bounds__(NT) void operand_kernel(const uint32_t *codes, const uint8_t *scales, uint16_t *out, int64_t N,
+                                                     int64_t K, int64_t blocks, int64_t kp) {
+    const int64_t i = block_index() * NT + threadIdx.x, n = divided(i, (uint32_t)(kp / 8)), u = i - n * (kp / 8);
+    if (n >= N) return;
+    u4 v = u4{0, 0, 0, 0};
+    if (u * 8 < K) {
+        v = values_of(codes[n * blocks * 4 + u], scale_of(scales[n * blocks + (u >> 2)]));
+        if (u * 8 + 8 > K) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (u * 8 + j >= K) x[j] = 0.f;  // a NaN scale reaches no column that is not there
-        ops::storev<8>(out, n * kp + u * 8, DT_BF16, x);
-    } else if (K % 8 == 0) {
-        ops::storev<8>(out, n * K + u * 8, dt, x);
-    } else {
-        for (int j = 0; j < 8; ++j)
-            if (u * 8 + j < K) store_from_f32(out, n * K + u * 8 + j, x[j], dt);
+            for (int j = 0; j < 8; ++j)
+                if (u * 8 + j >= K) v[j / 2] &= j % 2 ? 0xffffu : 0xffff0000u;
+        }
     }
+    *reinterpret_cast<u4 *>(out + n * kp + u * 8) = v;
 }
 
 // The weight's rows [0, N) as bf16 numbers along N: out[k][n], rows np apart, zeros behind the last; 64 x 64 to a workgroup.
@@ -121,8 +123,9 @@ __global__ __launch_bounds__(NT) void across_kernel(const uint32_t *codes, const
             c = codes[n * blocks * 4 + u];
             s = scale_of(scales[n * blocks + (u >> 2)]);
         }
+        const u4 v = values_of(c, s);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) tile[nl][ul * 8 + j] = f32_to_bf16_cvt(value(c >> (4 * j), s));
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint32_t *>(&tile[nl][ul * 8 + 2 * j]) = v[j];
     }
     __syncthreads();
 #pragma unroll
@@ -166,9 +169,10 @@ struct StepArgs {
 // 16 rows of the weight to a workgroup, its WAVES waves taking groups of four blocks along K in turn.  Lane (r, g) holds block g
 // of row r, 32 elements in 16 bytes: four matrix instructions, of which each takes eight elements of every lane's block, the
 // order along K being the same for both operands.  x comes through the caches.
-template <int DT, int TILES, int WAVES, bool WIDE>
+template <int DT, int TILES, bool WIDE>
 __global__ __launch_bounds__(64 * WAVES) void step_kernel(const StepArgs a) {
     constexpr int TERMS = DT == DT_BF16 ? 1 : DT == DT_F16 ? 2 : 3;
+    constexpr int AHEAD = 2;  // groups of blocks whose codes are loaded together
     __shared__ f4 part[WAVES][TILES][64];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
     const int64_t n0 = (int64_t)blockIdx.x * 16, n = min(n0 + r, a.N - 1);
@@ -177,46 +181,41 @@ __global__ __launch_bounds__(64 * WAVES) void step_kernel(const StepArgs a) {
     f4 acc[TILES];
 #pragma unroll
     for (int t = 0; t < TILES; ++t) acc[t] = f4{0.f, 0.f, 0.f, 0.f};
-    for (int b0 = w * 4; b0 < a.blocks; b0 += WAVES * 4) {
-        const int b = b0 + g;
-        const bool any = b < a.blocks;
-        uint4 c = make_uint4(0, 0, 0, 0);
-        float s = 1.f;
-        if (any) {
-            c = codes[b];
-            s = scale_of(scales[b]);
+    for (int b0 = w * 4; b0 < a.blocks; b0 += AHEAD * WAVES * 4) {
+        uint4 c[AHEAD];
+        uint32_t e[AHEAD];
+#pragma unroll
+        for (int h = 0; h < AHEAD; ++h) {
+            const int b = b0 + h * WAVES * 4 + g;
+            c[h] = b < a.blocks ? codes[b] : make_uint4(0, 0, 0, 0);
+            e[h] = b < a.blocks ? scales[b] : 127;
         }
-        const uint32_t cw[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            uint32_t v[4];
+        for (int h = 0; h < AHEAD; ++h) {
+            const int b = b0 + h * WAVES * 4 + g;
+            const float s = scale_of(e[h]);
+            const uint32_t cw[4] = {c[h].x, c[h].y, c[h].z, c[h].w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float lo = value(cw[m] >> (8 * j), s), hi = value(cw[m] >> (8 * j + 4), s);
-                v[j] = __float_as_uint(lo) >> 16 | (__float_as_uint(hi) & 0xffff0000u);
-            }
-            const bf8 A = __builtin_bit_cast(bf8, (u4{v[0], v[1], v[2], v[3]}));
-            const int k = b * 32 + 8 * m;
+            for (int m = 0; m < 4; ++m) {
+                const bf8 A = __builtin_bit_cast(bf8, values_of(cw[m], s));
+                const int k = b * 32 + 8 * m;
 #pragma unroll
-            for (int t = 0; t < TILES; ++t) {
-                const int token = min(16 * t + r, a.M - 1);
-                float x[8];
-                u4 B[TERMS];
-                if (WIDE && DT == DT_BF16) {
-                    B[0] = u4{0, 0, 0, 0};
-                    if (any && k < a.K) B[0] = *reinterpret_cast<const u4 *>(static_cast<const uint16_t *>(a.x) + token * a.ld + k);
-                } else {
-                    if (WIDE && any && k < a.K) {
-                        ops::loadv<8>(a.x, token * a.ld + k, DT, x);
+                for (int t = 0; t < TILES; ++t) {
+                    const int64_t token = min(16 * t + r, a.M - 1);
+                    u4 B[TERMS];
+                    if constexpr (WIDE) {  // bf16 rows of whole vectors need no conversion
+                        typedef u4 any4 __attribute__((aligned(2)));
+                        B[0] = u4{0, 0, 0, 0};
+                        if (k < a.K) B[0] = *reinterpret_cast<const any4 *>(static_cast<const uint16_t *>(a.x) + token * a.ld + k);
                     } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) x[j] = any && k + j < a.K ? load_as_f32(a.x, token * a.ld + k + j, DT) : 0.f;
+                        float x[8];
+                        ops::load_first<8, DT>(a.x, token * a.ld + k, a.K - k, x);
+                        split<TERMS>(x, B);
                     }
-                    split<TERMS>(x, B);
-                }
 #pragma unroll
-                for (int q = 0; q < TERMS; ++q)
-                    acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, __builtin_bit_cast(bf8, B[q]), acc[t], 0, 0, 0);
+                    for (int q = 0; q < TERMS; ++q)
+                        acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(A, __builtin_bit_cast(bf8, B[q]), acc[t], 0, 0, 0);
+                }
             }
         }
     }
@@ -233,19 +232,12 @@ __global__ __launch_bounds__(64 * WAVES) void step_kernel(const StepArgs a) {
     }
 }
 
-template <int DT, int WAVES, bool WIDE>
+template <int DT, bool WIDE>
 static void launch_step(const StepArgs &a, hipStream_t st) {
     const dim3 grid((unsigned)((a.N + 15) / 16)), block(64 * WAVES);
-    if (a.M <= 16) hipLaunchKernelGGL((step_kernel<DT, 1, WAVES, WIDE>), grid, block, 0, st, a);
-    else if (a.M <= 32) hipLaunchKernelGGL((step_kernel<DT, 2, WAVES, WIDE>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((step_kernel<DT, 4, WAVES, WIDE>), grid, block, 0, st, a);
-}
-
-template <int DT>
-static void launch_step_of(const StepArgs &a, hipStream_t st) {
-    const bool wide = a.K % 8 == 0 && a.ld % 8 == 0 && aligned_to(a.x, 16);
-    if (wide) launch_step<DT, 8, true>(a, st);
-    else launch_step<DT, 8, false>(a, st);
+    if (a.M <= 16) hipLaunchKernelGGL((step_kernel<DT, 1, WIDE>), grid, block, 0, st, a);
+    else if (a.M <= 32) hipLaunchKernelGGL((step_kernel<DT, 2, WIDE>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((step_kernel<DT, 4, WIDE>), grid, block, 0, st, a);
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -347,10 +339,11 @@ extern "C" int gdn_mxfp4_quantize(const void *w, void *codes, void *scales, int6
         Timed tm("mxfp4_quantize", st);
         uint32_t *c = static_cast<uint32_t *>(codes);
         uint8_t *s = static_cast<uint8_t *>(scales);
-        if (w_stride % 8 == 0 && aligned_to(w, 16))
-            hipLaunchKernelGGL((quantize_kernel<true>), grid, dim3(NT), 0, st, w, c, s, N, K, w_stride, blocks, dtype);
-        else
-            hipLaunchKernelGGL((quantize_kernel<false>), grid, dim3(NT), 0, st, w, c, s, N, K, w_stride, blocks, dtype);
+#define GDN_QUANTIZE(DT) hipLaunchKernelGGL((quantize_kernel<DT>), grid, dim3(NT), 0, st, w, c, s, N, K, w_stride, blocks)
+        if (dtype == GDN_F32) GDN_QUANTIZE(DT_F32);
+        else if (dtype == GDN_BF16) GDN_QUANTIZE(DT_BF16);
+        else GDN_QUANTIZE(DT_F16);
+#undef GDN_QUANTIZE
     }
     return check_launch(st, "gdn_mxfp4_quantize");
 }
@@ -362,13 +355,17 @@ extern "C" int gdn_mxfp4_dequantize(const void *codes, const void *scales, void 
     if (N == 0) return GDN_OK;
     if (!out) return fail(GDN_ERR_INVALID, "null pointer");
     if (const int rc = check_weight(codes, scales)) return rc;
-    if (!aligned_to(out, 16)) return fail(GDN_ERR_INVALID, "the output must lie on 16 bytes");
     hipStream_t st = static_cast<hipStream_t>(stream);
     const int64_t blocks = blocks_of(K);
     {
         Timed tm("mxfp4_values", st);
-        hipLaunchKernelGGL((values_kernel<false>), grid_of((N * blocks * 4 + NT - 1) / NT), dim3(NT), 0, st,
-                           static_cast<const uint32_t *>(codes), static_cast<const uint8_t *>(scales), out, N, K, blocks, 0, dtype);
+#define GDN_VALUES(DT)                                                                                              \
+    hipLaunchKernelGGL((values_kernel<DT>), grid_of((N * blocks * 4 + NT - 1) / NT), dim3(NT), 0, st,         \
+                       static_cast<const uint32_t *>(codes), static_cast<const uint8_t *>(scales), out, N, K, blocks)
+        if (dtype == GDN_F32) GDN_VALUES(DT_F32);
+        else if (dtype == GDN_BF16) GDN_VALUES(DT_BF16);
+        else GDN_VALUES(DT_F16);
+#undef GDN_VALUES
     }
     return check_launch(st, "gdn_mxfp4_dequantize");
 }
@@ -404,9 +401,10 @@ extern "C" int gdn_mxfp4_linear(const void *x, const void *codes, const void *sc
         const StepArgs a{x, static_cast<const uint4 *>(codes), static_cast<const uint8_t *>(scales), y, x_stride, N, (int)M, (int)K,
                          (int)blocks, dtype};
         Timed tm("mxfp4_step", st);
-        if (dtype == GDN_BF16) launch_step_of<DT_BF16>(a, st);
-        else if (dtype == GDN_F16) launch_step_of<DT_F16>(a, st);
-        else launch_step_of<DT_F32>(a, st);
+        if (dtype == GDN_F32) launch_step<DT_F32, false>(a, st);
+        else if (dtype == GDN_F16) launch_step<DT_F16, false>(a, st);
+        else if (K % 8 == 0) launch_step<DT_BF16, true>(a, st);
+        else launch_step<DT_BF16, false>(a, st);
     } else {
         const Sizes s = sizes(M, K, N, dtype, false);
         const bool as_it_lies = direct(x, x_stride, K, dtype);
@@ -422,9 +420,10 @@ extern "C" int gdn_mxfp4_linear(const void *x, const void *codes, const void *sc
             const int64_t rows = N - n0 < s.piece ? N - n0 : s.piece;
             {
                 Timed tm("mxfp4_values", st);
-                hipLaunchKernelGGL((values_kernel<true>), grid_of((rows * (s.kp / 8) + NT - 1) / NT), dim3(NT), 0, st,
+                hipLaunchKernelGGL(operand_kernel, grid_of((rows * (s.kp / 8) + NT - 1) / NT), dim3(NT), 0, st,
                                    static_cast<const uint32_t *>(codes) + n0 * blocks * 4,
-                                   static_cast<const uint8_t *>(scales) + n0 * blocks, b.w, rows, K, blocks, s.kp, 0);
+                                   static_cast<const uint8_t *>(scales) + n0 * blocks, reinterpret_cast<uint16_t *>(b.w), rows, K, blocks,
+                                   s.kp);
             }
             g.a = Operand{b.w, s.kp * 2, rows, {0, 0, 0}};
             const Result r{static_cast<char *>(y) + n0 * elem, N, dtype, nullptr, nullptr, 0, {0, 0, 0}, b.acc, columns_of(rows), 0, nullptr};
