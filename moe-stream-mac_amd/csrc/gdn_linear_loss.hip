@@ -7,8 +7,8 @@
 //
 // Forward: one product whose tiles of logits end in registers, each as the maximum and the sum of exponentials of its words
 // per token; a second kernel joins them.  Backward: the words in pieces; of each piece the logits again (their normaliser is
-// known only after the last word), from them the differences p - [v = t] as fp16 numbers, then two more products.  What
-// is stored at any time is one piece of differences, at most 2^26 of them.
+// known only after the last word), from them the differences p - [v = t] as 16-bit numbers, then two more products, which read
+// them along the words for dx and across for dW.  What is stored at any time is one piece of differences, at most 2^26 of them.
 //
 // Words lie along registers and tokens along lanes, so that maxima and sums run within a lane.
 //
@@ -19,14 +19,15 @@
 //
 // Precision.  Differences lie in [-1, 1] and have 11 bits as fp16 numbers times 2^15 (those below 2^-29 fewer); bf16 would
 // leave 8, as many as the results have, and make bf16 gradients up to 1.4 times as far from the exact ones.  W and x are fp16
-// numbers times a power of two then (gdn_terms.hip), which holds bf16 numbers exactly.  The differences for dW carry the
-// token's cotangent relative to the largest; those for dx do not, since it can be applied to the sum.  With fp32 inputs every
-// operand is two fp16 terms (2^-22) and every product three; a difference's second term is stored times 2^11, so that small
-// probabilities keep their bits (2^-22 of them down to 2^-29, 2^-51 below; in one term 2^-11 and 2^-40).
+// numbers times a power of two then (gdn_terms.hip), which holds bf16 numbers exactly.  Of a token's cotangent the differences
+// carry a factor of 0.75 to 1.5 and its sum for dx, or its x for dW, the power of two that is left, so that it costs no rounding
+// of its own.  With fp32 inputs every operand is two fp16 terms (2^-22) and every product three; a difference's second term is
+// stored times 2^11, so that small probabilities keep their bits (2^-22 of them down to 2^-29, 2^-51 below; in one term 2^-11 and
+// 2^-40).
 //
 // Few tokens (below DOWN) read the weight so often that its scaled copy, which lies along the words, costs more than the products:
 // dx is then formed from the weight as it lies (gdn_product.h), with fp16 weights by the differences as they are, with bf16 weights
-// by two bf16 terms of them (2^-17), rows of the same operand.
+// by two bf16 terms of them (2^-17), rows of the same operand; dW by both terms and x.
 #include "gdn_common.h"
 #include "gdn_host.h"
 #include "gdn_product.h"
@@ -47,7 +48,7 @@ constexpr int64_t MOST_TOKENS = 1 << 20;  // three slots of 16 bits for each are
 constexpr int SHIFT = 15;          // differences are stored times 2^15
 constexpr int TOP = 14;            // largest magnitudes of scaled operands: [2^14, 2^15)
 
-enum : int { E_X = 0, E_W = 1, E_D = 2 };
+enum : int { E_X = 0, E_W = 1 };
 
 // ------------------------------------------------------------------------------------------------ tokens that count
 
@@ -58,36 +59,46 @@ struct Tokens {      // of COMPACT tokens and more
     int64_t *target; // [N] their targets
 };
 
-// One workgroup, a run of tokens to each thread.  Tokens that do not count have loss 0.
+// One workgroup; the order of the tokens is kept.  Tokens that do not count have loss 0.
 __global__ __launch_bounds__(1024) void tokens_kernel(const int64_t *targets, int64_t N, int64_t ignore, Tokens t, float *loss) {
-    __shared__ int sums[16];
+    constexpr int ROUNDS = 8, STEP = ROUNDS * 1024;  // tokens whose loads are under way together
+    __shared__ int sums[2][16];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t per = (N + 1023) / 1024, n0 = min(N, threadIdx.x * per), n1 = min(N, n0 + per);
-    int own = 0;
-    for (int64_t n = n0; n < n1; ++n) own += targets[n] != ignore;
-    int before = own;  // of the threads up to this one
+    int before = 0;  // tokens that count before this step's
+    for (int64_t s0 = 0; s0 < N; s0 += STEP) {
+        const int64_t n0 = s0 + w * (ROUNDS * 64) + lane;
+        int64_t v[ROUNDS];
+        int own = 0, total = 0;
 #pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        const int v = __shfl_up(before, o);
-        if (lane >= o) before += v;
-    }
-    if (lane == 63) sums[w] = before;
-    __syncthreads();
-    int c = before - own;
-    for (int i = 0; i < w; ++i) c += sums[i];
-    for (int64_t n = n0; n < n1; ++n) {
-        const int64_t v = targets[n];
-        const bool live = v != ignore;
-        t.place[n] = live ? c : -1;
-        if (live) {
-            t.index[c] = (int)n;
-            t.target[c] = v;
-            ++c;
-        } else if (loss) {
-            loss[n] = 0.f;
+        for (int i = 0; i < ROUNDS; ++i) v[i] = n0 + i * 64 < N ? targets[n0 + i * 64] : ignore;
+#pragma unroll
+        for (int i = 0; i < ROUNDS; ++i) own += __popcll(__ballot(v[i] != ignore));
+        int *sum = sums[s0 / STEP & 1];  // two: a wave may be a step ahead of another
+        if (lane == 0) sum[w] = own;
+        __syncthreads();
+        int c = before;
+        for (int i = 0; i < 16; ++i) {
+            if (i < w) c += sum[i];
+            total += sum[i];
         }
+#pragma unroll
+        for (int i = 0; i < ROUNDS; ++i) {
+            const int64_t n = n0 + i * 64;
+            const bool live = v[i] != ignore;
+            const uint64_t all = __ballot(live);
+            const int at = c + __popcll(all & ((1ull << lane) - 1));
+            if (n < N) t.place[n] = live ? at : -1;
+            if (live) {
+                t.index[at] = (int)n;
+                t.target[at] = v[i];
+            } else if (loss && n < N) {
+                loss[n] = 0.f;
+            }
+            c += __popcll(all);
+        }
+        before += total;
     }
-    if (threadIdx.x == 1023) *t.count = c;
+    if (threadIdx.x == 0) *t.count = before;
 }
 
 // ------------------------------------------------------------------------------------------------ forward
@@ -224,22 +235,34 @@ __global__ __launch_bounds__(1024) void total_kernel(const float *loss, const in
 
 // ------------------------------------------------------------------------------------------------ backward
 
-// d[n] = the token's cotangent: 0 where it does not count, NaN where its target is no word.  part = partial maxima of |d|.
+// The token's cotangent, 0 where it does not count and NaN where its target is no word, as power[n] times factor[n], a power of two
+// and what is left, of magnitude 0.75 to 1.5 (larger only within a factor of 1.5 of the largest fp32 number): differences times it
+// and 2^15 are below 2^16, and the smallest lose half a bit at most to the factor.  part = partial maxima of the powers.
 __global__ __launch_bounds__(NT) void cotangent_kernel(const int64_t *targets, const float *dloss, int64_t stride,
-                                                       const float *factor, int64_t N, int64_t V, int64_t ignore, float *d,
-                                                       float *part, const int *index, const int *count) {
+                                                       const float *mean, int64_t N, int64_t V, int64_t ignore, float *power,
+                                                       float *factor, float *part, const int *index, const int *count) {
     __shared__ float red[NT];
     float m = 0.f;
     if (count) N = *count;
     for (int64_t n = (int64_t)blockIdx.x * NT + threadIdx.x; n < N; n += (int64_t)PARTS * NT) {
         const int64_t t = targets[n];
         float x = dloss[(index ? index[n] : n) * stride];
-        if (factor) x *= factor[0];
+        if (mean) x *= mean[0];
         if (t < 0 || t >= V) x = NAN;
         if (t == ignore) x = 0.f;
-        d[n] = x;
-        const float a = fabsf(x);
-        m = fmaxf(m, a <= 3.4028234e38f ? a : 0.f);
+        float p = x, f = 1.f;  // 0, infinities and NaN
+        if (x != 0.f && fabsf(x) <= 3.4028234e38f) {
+            int e;
+            f = frexpf(x, &e);
+            if (fabsf(f) < 0.75f || e > 127) {
+                f *= 2.f;
+                --e;
+            }
+            p = ldexpf(1.f, e);
+            m = fmaxf(m, p);
+        }
+        power[n] = p;
+        factor[n] = f;
     }
     red[threadIdx.x] = m;
     __syncthreads();
@@ -253,10 +276,10 @@ __global__ __launch_bounds__(NT) void cotangent_kernel(const int64_t *targets, c
 struct DiffArgs {
     const int64_t *targets;
     const float2 *stat;
-    const float *d;
-    const int *exps;  // with fp32 inputs also the logits' scale
-    uint16_t *p, *pt; // [N][terms * kp], [words][terms * np]; either may be NULL
-    int64_t v0, kp, np;
+    const float *power, *factor;  // cotangents
+    const int *exps;  // with fp32 inputs: the logits' scale
+    uint16_t *p;      // [N][terms * kp], or [terms * N][kp]
+    int64_t v0, kp;
 };
 
 // x as it was rounded: the compiler may round a product or sum to 16 bits at once in one place and in two steps in another, and
@@ -271,10 +294,10 @@ __device__ __forceinline__ float left_of(float x) {
     return (x - __half2float(__float2half(x))) * (float)(1 << LOW);
 }
 
-enum : int { ONE16 = 1, TWO16 = 2, ROWS = 3 };  // differences for dx: one fp16 term, two (fp32 inputs), two bf16 terms as rows
+enum : int { ONE16 = 1, TWO16 = 2, ROWS = 3 };  // differences: one fp16 term, two (fp32 inputs), two bf16 terms as rows
 
-// The differences of a piece of words, 2^15 (p - [v = t]), and times d / (the power of two over the largest |d|) for dW.
-template <class S, bool F16, int KIND, bool DX, bool DW>
+// The differences of a piece of words, 2^15 factor (p - [v = t]); zeros for tokens that do not count.
+template <class S, bool F16, int KIND>
 __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, const DiffArgs a) {
     constexpr int TERMS = KIND == TWO16 ? 2 : 1;  // side by side
     __shared__ __attribute__((aligned(16))) char lds[S::LDS + S::STORE];
@@ -286,14 +309,13 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
         const int64_t m0 = (int64_t)tm * S::BM + wm * (S::BM / S::WM), n0 = (int64_t)tn * S::BN + wn * (S::BN / S::WN);
         const int words = (int)min((int64_t)(S::BM / S::WM), g.a.rows - m0);  // of this wave's; may be negative
         const int e = TERMS > 1 ? -(a.exps[E_X] + a.exps[E_W]) : 0;
-        float r[S::TN];
 #pragma unroll
         for (int j = 0; j < S::TN; ++j) {
             const int64_t n = n0 + 16 * j + (lane & 15);
-            const bool live = n < ext.rows_b;
-            const float2 st = live ? a.stat[n] : make_float2(0.f, 0.f);
-            r[j] = DW && live ? ldexpf(a.d[n], a.exps[E_D]) : 0.f;
-            const float inv = st.y * (float)(1 << SHIFT);
+            const bool in = n < ext.rows_b;
+            const float2 st = in ? a.stat[n] : make_float2(0.f, 0.f);
+            const bool live = in && a.power[n] != 0.f;
+            const float scale = live ? a.factor[n] * (float)(1 << SHIFT) : 0.f, inv = st.y * scale;
             const int64_t hot = live ? a.targets[n] - a.v0 - m0 - 4 * (lane >> 4) : -1;
 #pragma unroll
             for (int i = 0; i < S::TM; ++i)
@@ -303,77 +325,43 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
                     float z = acc[i][j][q];
                     if constexpr (TERMS > 1) z = ldexpf(z, e);
                     float x = __builtin_amdgcn_exp2f((z - st.x) * LOG2E) * inv;
-                    if (hot == m) x -= (float)(1 << SHIFT);
-                    if (words < S::BM / S::WM && m + 4 * (lane >> 4) >= words) x = 0.f;
+                    if (hot == m) x -= scale;
                     acc[i][j][q] = KIND != ONE16 ? as_rounded(x) : x;
                 }
-        }
-        if constexpr (DX) {
+            if (words < S::BM / S::WM || !__all(live)) {
+                const int left = live ? words - 4 * (lane >> 4) : 0;
 #pragma unroll
-            for (int j = 0; j < S::TN; j += 2) {
-                const int64_t n = n0 + 16 * j, rows = ext.rows_b - n;
-                if (rows <= 0) break;
+                for (int i = 0; i < S::TM; ++i)
 #pragma unroll
-                for (int i = 0; i < S::TM; i += 4) {
-                    const int64_t m = m0 + 16 * i;
-                    if (m >= a.kp) break;
-#pragma unroll 1
-                    for (int t = 0; t < (KIND == ONE16 ? 1 : 2); ++t) {
-#pragma unroll
-                        for (int ii = 0; ii < 4; ++ii)
-#pragma unroll
-                            for (int jj = 0; jj < 2; ++jj) {
-                                float y[4];
-                                constexpr int DT = KIND == ROWS ? DT_BF16 : DT_F16;
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) {
-                                    y[k] = acc[i + ii][j + jj][k];
-                                    if (t) y[k] = KIND == ROWS ? y[k] - bf16_to_f32(f32_to_bf16_cvt(y[k])) : left_of(y[k]);
-                                }
-                                put16(lane, store, ii, jj, ops::pack2_cvt(y[0], y[1], DT), ops::pack2_cvt(y[2], y[3], DT));
-                            }
-                        uint16_t *to = KIND == ROWS ? a.p + (t * g.b.rows + n) * a.kp : a.p + n * (TERMS * a.kp) + t * a.kp;
-                        store_rows(lane, store, reinterpret_cast<char *>(to + m), (uint32_t)(TERMS * a.kp * 2), rows, (a.kp - m) * 2,
-                                   2);
-                    }
-                }
+                    for (int q = 0; q < 4; ++q)
+                        if (16 * i + q >= left) acc[i][j][q] = 0.f;
             }
         }
-        if constexpr (DW) {
-            constexpr int W = S::TN < 4 ? 2 : 4;  // tiles of tokens side by side
 #pragma unroll
-            for (int j = 0; j < S::TN; j += W) {
-                const int64_t n = n0 + 16 * j;
-                if (n >= a.np) break;
+        for (int j = 0; j < S::TN; j += 2) {
+            const int64_t n = n0 + 16 * j, rows = ext.rows_b - n;
+            if (rows <= 0) break;
 #pragma unroll
-                for (int i = 0; i < S::TM; i += 2) {
-                    if (16 * i >= words) break;
+            for (int i = 0; i < S::TM; i += 4) {
+                const int64_t m = m0 + 16 * i;
+                if (m >= a.kp) break;
 #pragma unroll 1
-                    for (int t = 0; t < TERMS; ++t) {
+                for (int t = 0; t < (KIND == ONE16 ? 1 : 2); ++t) {
 #pragma unroll
-                        for (int ii = 0; ii < 2; ++ii)
+                    for (int ii = 0; ii < 4; ++ii)
 #pragma unroll
-                            for (int h = 0; h < W; ++h)
+                        for (int jj = 0; jj < 2; ++jj) {
+                            float y[4];
+                            constexpr int DT = KIND == ROWS ? DT_BF16 : DT_F16;
 #pragma unroll
-                                for (int q = 0; q < 4; q += 2) {
-                                    float y[2];
-#pragma unroll
-                                    for (int k = 0; k < 2; ++k) {
-                                        y[k] = r[j + h] == 0.f ? 0.f : acc[i + ii][j + h][q + k] * r[j + h];
-                                        if (TERMS > 1) y[k] = as_rounded(y[k]);
-                                        if (t) y[k] = left_of(y[k]);
-                                    }
-                                    // two words of a token become two tokens of a word, with the neighbouring lane
-                                    const uint32_t own = ops::pack2(y[0], y[1], DT_F16);
-                                    const uint32_t its = __builtin_amdgcn_update_dpp(0, (int)own, DPP_QUAD_1032, 0xF, 0xF, false);
-                                    const uint32_t v = lane & 1 ? (its >> 16) | (own & 0xffff0000u) : (own & 0xffffu) | (its << 16);
-                                    const int row = 16 * ii + 4 * (lane >> 4) + q + (lane & 1), col = 16 * h + (lane & 14);
-                                    *reinterpret_cast<uint32_t *>(store_chunk(store, row, col >> 3) + (col & 7) * 2) = v;
-                                }
-                        const int64_t left = (a.np - n) * 2;
-                        store_rows(lane, store, reinterpret_cast<char *>(a.pt + (m0 + 16 * i) * (TERMS * a.np) + t * a.np + n),
-                                   (uint32_t)(TERMS * a.np * 2), words - 16 * i, left < W * 32 ? left : W * 32, 2);
-                    }
+                            for (int k = 0; k < 4; ++k) {
+                                y[k] = acc[i + ii][j + jj][k];
+                                if (t) y[k] = KIND == ROWS ? y[k] - bf16_to_f32(f32_to_bf16_cvt(y[k])) : left_of(y[k]);
+                            }
+                            put16(lane, store, ii, jj, ops::pack2_cvt(y[0], y[1], DT), ops::pack2_cvt(y[2], y[3], DT));
+                        }
+                    uint16_t *to = KIND == ROWS ? a.p + (t * g.b.rows + n) * a.kp : a.p + n * (TERMS * a.kp) + t * a.kp;
+                    store_rows(lane, store, reinterpret_cast<char *>(to + m), (uint32_t)(TERMS * a.kp * 2), rows, (a.kp - m) * 2, 2);
                 }
             }
         }
@@ -382,19 +370,18 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
 
 // ------------------------------------------------------------------------------------------------ host
 
-// The segments of a product of operands with `terms` terms, kp elements each: all pairs but the least.  `across`: a has the
-// slots of terms_across and b's second term is stored times 2^LOW.
-static void segments(Args &g, int terms, int64_t kp, bool across) {
+// The segments of a product of operands with `slots` terms for a, kp elements each, and one or two terms for b, the second
+// `second` bytes on (0: one): all pairs of terms but the least.  Three slots are those of terms_across, of which the third meets
+// b's second term, stored times 2^LOW.
+static void segments(Args &g, int slots, int64_t kp, int64_t second) {
     g.kit = (int)(kp / BK);
-    g.nseg = terms == 1 ? 1 : 3;
-    for (int s = 0; s < 3; ++s) g.a.off[s] = g.b.off[s] = 0;
-    if (terms > 1) {
-        g.a.off[1] = kp * 2;
-        g.b.off[2] = kp * 2;
-        if (across) g.a.off[2] = 2 * kp * 2;
+    g.nseg = 1;
+    g.a.ld = slots * kp * 2;
+    if (slots > 1) g.a.off[g.nseg++] = kp * 2;
+    if (second) {
+        g.a.off[g.nseg] = slots == 3 ? 2 * kp * 2 : 0;
+        g.b.off[g.nseg++] = second;
     }
-    g.a.ld = (across ? across_slots(terms) : terms) * kp * 2;
-    g.b.ld = terms * kp * 2;
 }
 
 struct Sizes {
@@ -402,7 +389,9 @@ struct Sizes {
     int terms;
     bool compact;
     bool down;     // dx from the weight as it lies
-    int64_t prows; // rows of the differences for dx
+    bool rows;     // the differences are two bf16 terms, as rows
+    int64_t prows; // rows of the differences
+    int slots;     // terms of the operands that meet them: the weight for dx, x for dW
     int64_t parts, tokens;  // parts of the words with statistics of their own; tokens at a time in the forward pass
     Plan px, pw;
 };
@@ -411,7 +400,7 @@ static bool direct(const void *p, int64_t ld, int64_t H, int dt) {
     return dt != GDN_F32 && H % BK == 0 && ld % 8 == 0 && aligned_to(p, 16) && pitch_fits(ld * 2);
 }
 
-static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt, bool direct_w) {
+static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt, bool direct_w, bool dx) {
     Sizes s{};
     s.N = N; s.H = H; s.V = V;
     s.hp = padded(H);
@@ -419,7 +408,9 @@ static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt, bool direct_w) {
     s.terms = dt == GDN_F32 ? 2 : 1;
     s.compact = N >= COMPACT;
     s.down = N < DOWN && direct_w;
-    s.prows = s.down && dt == GDN_BF16 ? 2 * N : N;
+    s.rows = s.down && dx && dt == GDN_BF16;
+    s.prows = s.rows ? 2 * N : N;
+    s.slots = s.terms == 1 ? 1 : 3;
     int64_t most = KEPT / s.np / 256 * 256;
     if (most < 256) most = 256;
     s.pieces = (V + most - 1) / most;
@@ -429,10 +420,9 @@ static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt, bool direct_w) {
     s.tokens = KEPT / s.parts / 256 * 256;
     if (s.tokens < 256) s.tokens = 256;
     if (s.tokens > N) s.tokens = N;
-    const int64_t seg = s.terms == 1 ? 1 : 3;
     const int64_t words = s.piece < V ? s.piece : V;
-    s.px = plan(s.prows, H, seg * padded(words) / BK, s.down ? 32 : 16);
-    s.pw = plan(words, H, seg * s.np / BK, 8);
+    s.px = plan(s.prows, H, s.slots * padded(words) / BK, s.down ? 32 : 16);
+    s.pw = plan(words, H, (s.rows ? 2 : s.slots) * s.np / BK, 8, true);
     return s;
 }
 
@@ -448,8 +438,8 @@ struct Space {
 };
 
 struct Buffers {
-    uint16_t *x, *w, *wt, *xt, *p, *pt;
-    float *part, *zt, *d, *acc_x, *acc_w;
+    uint16_t *x, *w, *wt, *xt, *p;
+    float *part, *zt, *power, *factor, *most, *acc_x, *acc_w;
     float2 *stats;
     int *exps;
     Tokens tokens;
@@ -459,7 +449,8 @@ static Buffers place(Space &sp, const Sizes &s, bool dx, bool dw, bool bwd, bool
     Buffers b{};
     const int t = s.terms;
     const int64_t words = s.piece < s.V ? s.piece : s.V;
-    b.exps = sp.take<int>(4);
+    b.exps = sp.take<int>(2);
+    b.most = sp.take<float>(1);
     b.part = sp.take<float>(3 * PARTS);
     if (s.compact) {
         b.tokens.count = sp.take<int>(1);
@@ -474,15 +465,15 @@ static Buffers place(Space &sp, const Sizes &s, bool dx, bool dw, bool bwd, bool
         b.zt = sp.take<float>(s.tokens);
         return b;
     }
-    b.d = sp.take<float>(s.N);
+    b.power = sp.take<float>(s.N);
+    b.factor = sp.take<float>(s.N);
+    b.p = sp.take<uint16_t>(s.prows * t * padded(words));
     if (dx) {
-        if (!s.down) b.wt = sp.take<uint16_t>(s.H * across_slots(t) * padded(words));
-        b.p = sp.take<uint16_t>(s.prows * t * padded(words));
+        if (!s.down) b.wt = sp.take<uint16_t>(s.H * s.slots * padded(words));
         b.acc_x = sp.take<float>((int64_t)s.px.splits * s.prows * columns_of(s.H));
     }
     if (dw) {
-        b.xt = sp.take<uint16_t>(s.H * across_slots(t) * s.np);
-        b.pt = sp.take<uint16_t>(words * t * s.np);
+        b.xt = sp.take<uint16_t>(s.H * s.slots * s.np);
         if (s.pw.splits > 1) b.acc_w = sp.take<float>((int64_t)s.pw.splits * words * columns_of(s.H));
     }
     return b;
@@ -504,14 +495,6 @@ static void launch_stat(Args &g, const StatArgs &a, bool scaled, hipStream_t st)
     else hipLaunchKernelGGL((stat_kernel<S, F16, false>), grid, dim3(S::NT), 0, st, g, a);
 }
 
-template <class S, bool F16, int KIND>
-static void launch_diff(Args &g, const DiffArgs &a, hipStream_t st) {
-    const dim3 grid = tiles_of<S>(g, 1);
-    if (a.p && a.pt) hipLaunchKernelGGL((diff_kernel<S, F16, KIND, true, true>), grid, dim3(S::NT), 0, st, g, a);
-    else if (a.p) hipLaunchKernelGGL((diff_kernel<S, F16, KIND, true, false>), grid, dim3(S::NT), 0, st, g, a);
-    else if constexpr (KIND != ROWS) hipLaunchKernelGGL((diff_kernel<S, F16, KIND, false, true>), grid, dim3(S::NT), 0, st, g, a);
-}
-
 // 16-bit inputs as they are, fp32 inputs as two fp16 terms.
 template <class S>
 static void launch_stat_of(Args &g, const StatArgs &a, int dt, hipStream_t st) {
@@ -520,10 +503,11 @@ static void launch_stat_of(Args &g, const StatArgs &a, int dt, hipStream_t st) {
 }
 template <class S>
 static void launch_diff_of(Args &g, const DiffArgs &a, int dt, bool rows, hipStream_t st) {
-    if (dt == GDN_F32) launch_diff<S, true, TWO16>(g, a, st);
-    else if (dt == GDN_F16) launch_diff<S, true, ONE16>(g, a, st);
-    else if (rows) launch_diff<S, false, ROWS>(g, a, st);
-    else launch_diff<S, false, ONE16>(g, a, st);
+    const dim3 grid = tiles_of<S>(g, 1), block(S::NT);
+    if (dt == GDN_F32) hipLaunchKernelGGL((diff_kernel<S, true, TWO16>), grid, block, 0, st, g, a);
+    else if (dt == GDN_F16) hipLaunchKernelGGL((diff_kernel<S, true, ONE16>), grid, block, 0, st, g, a);
+    else if (rows) hipLaunchKernelGGL((diff_kernel<S, false, ROWS>), grid, block, 0, st, g, a);
+    else hipLaunchKernelGGL((diff_kernel<S, false, ONE16>), grid, block, 0, st, g, a);
 }
 
 #define GDN_BY_SHAPE(shape, call)              \
@@ -550,7 +534,7 @@ extern "C" size_t gdn_linear_loss_workspace_bytes(int64_t N, int64_t H, int64_t 
                                                   int want_dw) {
     if (N <= 0 || H <= 0 || V <= 0 || N > MOST_TOKENS || V > 1 << 24 || H > 1 << 17) return 0;
     const bool copy = !aligned || dtype == GDN_F32 || H % BK;
-    return need(sizes(N, H, V, dtype, !copy), want_dx, want_dw, want_dx || want_dw, copy, copy);
+    return need(sizes(N, H, V, dtype, !copy, want_dx), want_dx, want_dw, want_dx || want_dw, copy, copy);
 }
 
 extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *targets, float *loss, float *stat, float *total,
@@ -565,7 +549,7 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
     if (N > 0) {
         if (!x || !w || !targets || !loss || !workspace) return fail(GDN_ERR_INVALID, "null pointer");
         const bool dw = direct(w, w_stride, H, dtype);
-        const Sizes s = sizes(N, H, V, dtype, dw);
+        const Sizes s = sizes(N, H, V, dtype, dw, false);
         const bool dx = !s.compact && direct(x, x_stride, H, dtype);
         const size_t bytes = need(s, false, false, false, !dx, !dw);
         if (workspace_bytes < bytes)
@@ -582,7 +566,7 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
             hipLaunchKernelGGL(tokens_kernel, dim3(1), dim3(1024), 0, st, targets, N, ignore_index, tk, loss);
         if (dtype == GDN_F32) {
             maxima({sx, sw}, b.part, st);
-            exponents(b.part, Tops{{TOP, TOP, 0}}, b.exps, st);  // the third is not read
+            exponents(b.part, TOP, b.exps, b.most, st);  // the third is not read
             exps = b.exps;
         }
         if (!dx) terms(sx, s.terms, f16, exps, E_X, b.x, st);
@@ -590,12 +574,13 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
         const int64_t step = dw ? V : s.piece;
         for (int64_t n0 = 0; n0 < N; n0 += s.tokens) {
             const int64_t tokens = N - n0 < s.tokens ? N - n0 : s.tokens;
-            const int shape = plan(tokens, V, 1, 1).shape;
+            const int shape = plan(tokens, dw ? V : s.piece, s.slots * s.hp / BK, 1).shape;
             int parts = 0;
             for (int64_t v0 = 0; v0 < V; v0 += step) {
                 const int64_t words = V - v0 < step ? V - v0 : step;
                 Args g{};
-                segments(g, s.terms, s.hp, false);
+                segments(g, s.terms, s.hp, s.terms > 1 ? s.hp * 2 : 0);
+                g.b.ld = s.terms * s.hp * 2;
                 g.a.rows = words;
                 g.b.rows = tokens;
                 g.live = tk.count;
@@ -654,7 +639,7 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
     if (N == 0) return fail(GDN_ERR_INVALID, "no tokens: the gradients are zeros, which this call does not write");
     if (!x || !w || !targets || !stat || !dloss || !workspace) return fail(GDN_ERR_INVALID, "null pointer");
     const bool direct_w = direct(w, w_stride, H, dtype);
-    const Sizes s = sizes(N, H, V, dtype, direct_w);
+    const Sizes s = sizes(N, H, V, dtype, direct_w, dx);
     const bool direct_x = !s.compact && direct(x, x_stride, H, dtype);
     const size_t bytes = need(s, dx, dw, true, !direct_x, !direct_w);
     if (workspace_bytes < bytes)
@@ -669,23 +654,24 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
     const Source sw{w, dtype, V, H, w_stride, nullptr, 0, nullptr, nullptr};
     if (s.compact) hipLaunchKernelGGL(tokens_kernel, dim3(1), dim3(1024), 0, st, targets, N, ignore_index, tk, nullptr);
     hipLaunchKernelGGL(cotangent_kernel, dim3(PARTS), dim3(NT), 0, st, tt, dloss, dloss_stride, factor, N, V, ignore_index,
-                       b.d, b.part + E_D * PARTS, tk.index, tk.count);
+                       b.power, b.factor, b.part + 2 * PARTS, tk.index, tk.count);
     Source mx = sx, mw = sw;  // what is stored times a power of two
-    if (!dw && dtype != GDN_F32) mx.rows = 0;
+    if ((!dw || s.rows) && dtype != GDN_F32) mx.rows = 0;
     if ((!dx || s.down) && dtype != GDN_F32) mw.rows = 0;
     if (mx.rows + mw.rows > 0) maxima({mx, mw}, b.part, st);
-    if (mx.rows + mw.rows > 0) exponents(b.part, Tops{{TOP, TOP, -1}}, b.exps, st);  // |d| below 1
+    if (dw || mw.rows > 0) exponents(b.part, TOP, b.exps, b.most, st);
     const int *exps = dtype == GDN_F32 ? b.exps : nullptr;
     if (!direct_x) terms(sx, t, f16, exps, E_X, b.x, st);
-    if (dw) terms_across(sx, t, true, b.exps, E_X, b.xt, st);
-    const int shape = plan(dw ? s.np : N, s.piece, 1, 1).shape;  // tiles that cover the columns that dW's product reads
+    if (dw) terms_across(sx, s.slots, !s.rows, s.rows ? nullptr : b.exps, E_X, Factors{b.power, b.most}, b.xt, st);
+    const int shape = plan(N, s.piece, s.slots * s.hp / BK, 1).shape;
     for (int64_t v0 = 0; v0 < V; v0 += s.piece) {
         const int64_t words = V - v0 < s.piece ? V - v0 : s.piece, kp = padded(words);
         Source part = sw;
         part.p = static_cast<const char *>(w) + v0 * w_stride * elem;
         part.rows = words;
         Args g{};
-        segments(g, t, s.hp, false);
+        segments(g, t, s.hp, t > 1 ? s.hp * 2 : 0);
+        g.b.ld = t * s.hp * 2;
         g.a.rows = words;
         g.b.rows = N;
         g.live = tk.count;
@@ -701,48 +687,54 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
             g.b.p = static_cast<const char *>(x);
             g.b.ld = x_stride * 2;
         }
-        const DiffArgs a{tt, reinterpret_cast<const float2 *>(stat), b.d, b.exps, b.p, b.pt, v0, kp, s.np};
+        const DiffArgs a{tt, reinterpret_cast<const float2 *>(stat), b.power, b.factor, b.exps, b.p, v0, kp};
         {
             Timed tm("loss_diff", st);
-#define GDN_DIFF(S) launch_diff_of<S>(g, a, dtype, s.down && dx, st)
+#define GDN_DIFF(S) launch_diff_of<S>(g, a, dtype, s.rows, st)
             GDN_BY_SHAPE(shape, GDN_DIFF)
 #undef GDN_DIFF
         }
         if (dx) {
             Args h{};
             if (s.down) {
-                h.a = Operand{static_cast<const char *>(part.p), w_stride * 2, H, {0, 0, 0}};
-                h.b.ld = kp * 2;
+                h.a = Operand{static_cast<const char *>(part.p), w_stride * 2, H, {0, 0, 0}, H * 2};
                 h.kit = (int)(kp / BK);
                 h.nseg = 1;
+                h.across = DOWN_A;
                 h.down = words;
             } else {
-                terms_across(part, t, true, b.exps, E_W, b.wt, st);
-                segments(h, t, kp, true);
+                terms_across(part, s.slots, true, b.exps, E_W, Factors{nullptr, nullptr}, b.wt, st);
+                segments(h, s.slots, kp, t > 1 ? kp * 2 : 0);
                 h.a.p = reinterpret_cast<const char *>(b.wt);
                 h.a.rows = H;
             }
+            h.b.ld = t * kp * 2;
             h.b.p = reinterpret_cast<const char *>(b.p);
             h.b.rows = s.prows;
             h.live = tk.count;
             const Plan pl = s.px;  // parts without a block of the last piece add nothing
-            Result r{dx, H, dtype, b.d, b.exps, -SHIFT, {0, s.down ? 0 : -1, 0}, nullptr, columns_of(H), v0 > 0, tk.place};
+            Result r{dx, H, dtype, b.power, b.exps, -SHIFT, {0, s.down ? 0 : -1}, nullptr, columns_of(H), v0 > 0, nullptr, tk.place};
             if (s.down || s.compact || s.pieces > 1 || pl.splits > 1) r.acc = b.acc_x;
             multiply(h, !s.down || dtype == GDN_F16, pl, r, st);
             if (r.acc && v0 + words == V) finish(r, pl.splits * (int)(s.prows / N), N, H, st);  // terms are parts too
         }
         if (dw) {
             Args h{};
-            segments(h, t, s.np, true);
+            segments(h, s.slots, s.np, s.rows ? N * kp * 2 : t > 1 ? kp * 2 : 0);
             h.a.p = reinterpret_cast<const char *>(b.xt);
             h.a.rows = H;
-            h.b.p = reinterpret_cast<const char *>(b.pt);
+            h.b.p = reinterpret_cast<const char *>(b.p);
+            h.b.ld = t * kp * 2;
             h.b.rows = words;
+            h.b.width = kp * 2;
+            h.across = DOWN_B;
+            h.down = N;
             h.live = tk.count;
             h.live_k = 1;
-            Result r{static_cast<char *>(dw) + v0 * H * elem, H, dtype, nullptr, b.exps, -SHIFT, {-1, 0, -1}, nullptr, columns_of(H), 0, nullptr};
+            Result r{static_cast<char *>(dw) + v0 * H * elem, H, dtype, nullptr, b.exps, -SHIFT, {s.rows ? 0 : -1, 0}, nullptr,
+                     columns_of(H), 0, b.most, nullptr};
             if (s.pw.splits > 1) r.acc = b.acc_w;
-            multiply(h, true, s.pw, r, st);
+            multiply(h, !s.rows, s.pw, r, st);
             if (r.acc) finish(r, s.pw.splits, words, H, st);
         }
     }

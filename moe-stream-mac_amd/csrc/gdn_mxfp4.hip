@@ -425,8 +425,8 @@ extern "C" int gdn_mxfp4_linear(const void *x, const void *codes, const void *sc
                                    static_cast<const uint8_t *>(scales) + n0 * blocks, reinterpret_cast<uint16_t *>(b.w), rows, K, blocks,
                                    s.kp);
             }
-            g.a = Operand{b.w, s.kp * 2, rows, {0, 0, 0}};
-            const Result r{static_cast<char *>(y) + n0 * elem, N, dtype, nullptr, nullptr, 0, {0, 0, 0}, b.acc, columns_of(rows), 0, nullptr};
+            g.a = Operand{b.w, s.kp * 2, rows, {0, 0, 0}, 0};
+            const Result r{static_cast<char *>(y) + n0 * elem, N, dtype, nullptr, nullptr, 0, {0, 0}, b.acc, columns_of(rows), 0, nullptr, nullptr};
             multiply(g, false, s.plan, r, st);
             if (r.acc) finish(r, s.plan.splits, M, rows, st);
         }
@@ -463,8 +463,8 @@ extern "C" int gdn_mxfp4_linear_bwd(const void *dy, const void *codes, const voi
                                static_cast<const uint8_t *>(scales) + n0 * blocks, reinterpret_cast<uint16_t *>(b.w), rows, K,
                                blocks, np, tiles_k, tiles);
         }
-        g.a = Operand{b.w, np * 2, K, {0, 0, 0}};
-        const Result r{dx, K, dtype, nullptr, nullptr, 0, {0, 0, 0}, b.acc, columns_of(K), n0 > 0, nullptr};
+        g.a = Operand{b.w, np * 2, K, {0, 0, 0}, 0};
+        const Result r{dx, K, dtype, nullptr, nullptr, 0, {0, 0}, b.acc, columns_of(K), n0 > 0, nullptr, nullptr};
         multiply(g, false, s.plan, r, st);
         if (r.acc && n0 + rows == N) finish(r, s.plan.splits, M, K, st);
     }

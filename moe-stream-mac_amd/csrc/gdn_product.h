@@ -49,6 +49,7 @@ struct Operand {
     const char *p;
     int64_t ld, rows;
     int64_t off[3];
+    int64_t width;  // across the contraction: bytes of a row that may be read, a multiple of 16
 };
 struct Args {
     Operand a, b;
@@ -61,19 +62,21 @@ struct Args {
     const int *live;
     int64_t live0;
     int live_k;
-    int64_t down;  // not 0: A lies across the contraction, this many rows of a.rows columns; one segment, results in parts
+    int across;    // the operand that lies across the contraction: 0, DOWN_A or DOWN_B
+    int64_t down;  // its rows; its `rows` are columns then
 };
 struct Extent {
-    int64_t rows_b;
+    int64_t rows_b, down;
     int nt, kit;
 };
 template <class S>
 __device__ __forceinline__ Extent extent_of(const Args &g) {
-    Extent x{g.b.rows, g.nt, g.kit};
+    Extent x{g.b.rows, g.down, g.nt, g.kit};
     if (g.live) {
         const int64_t n = max((int64_t)0, (int64_t)*g.live - g.live0);
         if (g.live_k) {
             x.kit = (int)min((int64_t)g.kit, (n + BK - 1) / BK);
+            x.down = min(g.down, n);
         } else {
             x.rows_b = min(g.b.rows, n);
             x.nt = (int)((x.rows_b + S::BN - 1) / S::BN);
@@ -124,97 +127,110 @@ __device__ __forceinline__ void tile_of(int id, int mt, int nt, int &tm, int &tn
     tn = r / width;
 }
 
-// A may also lie across the contraction (DOWN): rows of m, one for each k, read as they are and turned by LDS reads that transpose
-// 4 x 16 numbers.  32 bytes, what such a read takes of a row, lie in place (pair ^ down_swizzle(row)) of the row's, so that the
-// 16 rows of one read fill all banks twice.  Rows behind the last (g.down of them) read as zeros.
+// An operand may also lie across the contraction (DOWN_A, DOWN_B): rows of m or n, one for each k, read as they are and turned by
+// LDS reads that transpose 4 x 16 numbers.  32 bytes, what such a read takes of a row, lie in place (pair ^ down_swizzle(row)) of
+// the row's, so that the 16 rows of one read fill all banks twice.  Rows behind the last (Extent::down of them) read as zeros;
+// columns behind the last are whatever follows them, and nothing of them is stored.  2048 x 8192 x 8192: 1.44 PFLOP/s with A so.
+enum : int { DOWN_A = 1, DOWN_B = 2 };
 __device__ __forceinline__ int down_swizzle(int row) { return (row & 3) | (row >> 3 & 1) << 2; }
 // The chunk of 16 bytes of a row that lies in place p.
 __device__ __forceinline__ int down_chunk(int p, int row) { return ((p >> 1) ^ down_swizzle(row)) << 1 | (p & 1); }
 
+// One operand's share of a workgroup's loads: ROWS rows of the tile (of m or n), or with DOWN their columns.
+template <class S, int ROWS, bool DOWN>
+struct Side {
+    static constexpr int LOADS = ROWS * 8 / S::NT;                      // of a thread for a block
+    static constexpr int LANES = ROWS / 8, ROUND = S::NT / (DOWN ? LANES : 8);  // DOWN: lanes to a row; rows to a load
+    const char *p;       // of the block to load next
+    int64_t rest;        // DOWN: bytes from p to the operand's end
+    uint32_t at, at_odd; // this thread's offset in a block, DOWN also of odd loads
+    uint32_t size, step; // bytes that loads may reach, none behind the last row; from one load's rows to the next one's
+
+    // The tile's row (or column) r0 on of `rows`, block kk of a term at `off`; `down` rows along the contraction.
+    __device__ __forceinline__ void start(const Operand &o, int64_t off, int64_t r0, int64_t rows, int kk, int64_t down) {
+        const uint32_t ld = (uint32_t)o.ld;
+        step = ROUND * ld;
+        if constexpr (DOWN) {
+            const int r = threadIdx.x / LANES, c = threadIdx.x % LANES;
+            at = r * ld + down_chunk(c, r) * 16;
+            at_odd = r * ld + down_chunk(c, r + ROUND) * 16;
+            const int64_t from = (int64_t)kk * BK * o.ld + r0 * 2;
+            p = o.p + off + from;
+            rest = (down - 1) * o.ld + o.width - from;
+        } else {
+            const int r = threadIdx.x >> 3, c = threadIdx.x & 7;
+            at = r * ld + ((c ^ (r >> 1 & 7)) << 4);
+            p = o.p + off + r0 * o.ld + (int64_t)kk * (BK * 2);
+            size = (uint32_t)(min((int64_t)ROWS, rows - r0) - 1) * ld + BK * 2;
+        }
+    }
+    __device__ __forceinline__ void next(const Operand &o) {
+        if constexpr (DOWN) {
+            p += BK * o.ld;
+            rest -= BK * o.ld;
+        } else {
+            p += BK * 2;
+        }
+    }
+    // From the end of a term of kit blocks to the start of another, `off` bytes on.
+    __device__ __forceinline__ void turn(const Operand &o, int64_t off, int kit) {
+        if constexpr (DOWN) {
+            p += off - (int64_t)kit * BK * o.ld;
+            rest += (int64_t)kit * BK * o.ld;
+        } else {
+            p += off - (int64_t)kit * (BK * 2);
+        }
+    }
+    // Load r of a block.
+    __device__ __forceinline__ void load(char *__restrict__ dst, int r, int w) const {
+#ifdef __HIP_DEVICE_COMPILE__  // the host's pass does not know buffer resources
+        constexpr int RAW = 0x00020000;
+        const uint32_t n = DOWN ? (uint32_t)min(max(rest, (int64_t)0), (int64_t)1 << 31) : size;
+        const auto res = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(p), 0, n, RAW);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(res, (lvoid *)(dst + r * (S::NT * 16) + w * 1024), 16,
+                                                 (DOWN && r % 2 ? at_odd : at) + r * step, 0, 0, 0);
+#endif
+    }
+};
+
 // A workgroup's walk over its tiles and their blocks: tiles blockIdx.x, blockIdx.x + gridDim.x, ..., each from block `first`
 // to `end`.  It runs two blocks ahead of the products, over the border between two tiles too, so that the next tile's first
 // loads are under way while results are written.
-template <class S, bool DOWN>
+template <class S, int DOWN>
 struct Loader {
-    static constexpr int ROW = S::BM * 2, LANES = S::BM / 8, ROUND = S::NT / LANES;  // DOWN: a row's bytes, its lanes, rows a load
-    const char *pa, *pb;  // of the block to load next
-    uint32_t va, vb, na, nb;  // this thread's offset in a tile, and the bytes that loads may reach: none behind the last row
-    uint32_t step_a, step_b;  // from one load's rows to the next one's
-    uint32_t va_odd;          // DOWN: va of odd loads
-    int64_t rest;             // DOWN: bytes from pa to the operand's end
+    Side<S, S::BM, (DOWN & DOWN_A) != 0> a;
+    Side<S, S::BN, (DOWN & DOWN_B) != 0> b;
     int left, seg_left, seg, tile, tiles, w;  // blocks left of the tile and of the segment
 
     __device__ __forceinline__ void start(const Args &g, const Extent &x, int first, int end) {  // of a tile
         int tm, tn;
         tile_of(tile, g.mt, x.nt, tm, tn);
-        const int lane = threadIdx.x & 63, r0 = (threadIdx.x >> 3);
-        const uint32_t chunk = ((lane & 7) ^ (r0 >> 1 & 7)) << 4;
-        const int mb = (int)min((int64_t)S::BN, x.rows_b - (int64_t)tn * S::BN);
-        if constexpr (DOWN) {
-            const int r = threadIdx.x / LANES, p = threadIdx.x % LANES;
-            va = (uint32_t)r * (uint32_t)g.a.ld + down_chunk(p, r) * 16;
-            va_odd = (uint32_t)r * (uint32_t)g.a.ld + down_chunk(p, r + ROUND) * 16;
-            step_a = (uint32_t)ROUND * (uint32_t)g.a.ld;
-        } else {
-            const int ma = (int)min((int64_t)S::BM, g.a.rows - (int64_t)tm * S::BM);
-            va = (uint32_t)r0 * (uint32_t)g.a.ld + chunk;
-            na = (uint32_t)(ma - 1) * (uint32_t)g.a.ld + BK * 2;
-            step_a = (uint32_t)(S::NT / 8) * (uint32_t)g.a.ld;
-        }
-        vb = (uint32_t)r0 * (uint32_t)g.b.ld + chunk;
-        nb = (uint32_t)(mb - 1) * (uint32_t)g.b.ld + BK * 2;
-        step_b = (uint32_t)(S::NT / 8) * (uint32_t)g.b.ld;
         left = end - first;
         seg = first / x.kit;
         const int kk = first - seg * x.kit;
         seg_left = x.kit - kk;
-        if constexpr (DOWN) {
-            const int64_t at = (int64_t)kk * BK * g.a.ld + (int64_t)tm * S::BM * 2;
-            pa = g.a.p + at;
-            rest = (g.down - 1) * g.a.ld + g.a.rows * 2 - at;
-        } else {
-            pa = g.a.p + (int64_t)tm * S::BM * g.a.ld + g.a.off[seg] + (int64_t)kk * (BK * 2);
-        }
-        pb = g.b.p + (int64_t)tn * S::BN * g.b.ld + g.b.off[seg] + (int64_t)kk * (BK * 2);
+        a.start(g.a, g.a.off[seg], (int64_t)tm * S::BM, g.a.rows, kk, x.down);
+        b.start(g.b, g.b.off[seg], (int64_t)tn * S::BN, x.rows_b, kk, x.down);
     }
-    // Loads [R0, R1) of a block's RA + RB.  Rows behind the last read as zeros.
+    // Loads [R0, R1) of a block's RA + RB.
     template <int R0, int R1>
     __device__ __forceinline__ void load(char *__restrict__ dst) const {
-#ifdef __HIP_DEVICE_COMPILE__  // the host's pass does not know buffer resources
-        constexpr int RAW = 0x00020000;
-        const uint32_t la = DOWN ? (uint32_t)min(max(rest, (int64_t)0), (int64_t)1 << 31) : na;
-        const auto a = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(pa), 0, la, RAW);
-        const auto b = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(pb), 0, nb, RAW);
 #pragma unroll
         for (int r = R0; r < R1; ++r) {
-            lvoid *to = (lvoid *)(dst + r * (S::NT * 16) + w * 1024);
-            if (r < S::RA)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(a, to, 16, (DOWN && r % 2 ? va_odd : va) + r * step_a, 0, 0, 0);
-            else
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(b, to, 16, vb + (r - S::RA) * step_b, 0, 0, 0);
+            if (r < S::RA) a.load(dst, r, w);
+            else b.load(dst + S::A_BYTES, r - S::RA, w);
         }
-#endif
     }
     // On to the next block; after the very last one it stays there, so that loads need no branch around them.
     __device__ __forceinline__ void next(const Args &g, const Extent &x, int first, int end) {
         if (left > 1) {
-            if constexpr (DOWN) {
-                pa += BK * g.a.ld;
-                rest -= BK * g.a.ld;
-            } else {
-                pa += BK * 2;
-            }
-            pb += BK * 2;
+            a.next(g.a);
+            b.next(g.b);
             --left;
             if (--seg_left == 0) {
                 seg_left = x.kit;
-                if constexpr (DOWN) {
-                    pa -= (int64_t)x.kit * BK * g.a.ld;
-                    rest += (int64_t)x.kit * BK * g.a.ld;
-                } else {
-                    pa += g.a.off[seg + 1] - g.a.off[seg] - (int64_t)x.kit * (BK * 2);
-                }
-                pb += g.b.off[seg + 1] - g.b.off[seg] - (int64_t)x.kit * (BK * 2);
+                a.turn(g.a, g.a.off[seg + 1] - g.a.off[seg], x.kit);
+                b.turn(g.b, g.b.off[seg + 1] - g.b.off[seg], x.kit);
                 ++seg;
             }
         } else if (tile + (int)gridDim.x < tiles) {
@@ -234,37 +250,56 @@ __device__ __forceinline__ void stage_barrier() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
+// Tile i of 16 rows of an operand, 8 numbers along the contraction to a lane: 16 bytes of a row of the operand (at[k] for step k);
+// or DOWN two reads of four rows each, at[0] the lane's place in a row of tile 0 and at[1] its swizzle, PITCH bytes a row.
+template <bool DOWN, int PITCH>
+__device__ __forceinline__ u4 fragment(const char *__restrict__ lds, const uint32_t (&at)[2], int k, int i) {
+    if constexpr (DOWN) {
+        typedef short s4 __attribute__((ext_vector_type(4)));
+        typedef short s8 __attribute__((ext_vector_type(8)));
+        typedef __attribute__((address_space(3))) s4 lds_s4;
+        const char *p = lds + at[0] + k * 32 * PITCH + ((uint32_t)(i * 32) ^ at[1]);
+        const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)p);
+        const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(p + 4 * PITCH));
+        return __builtin_bit_cast(u4, (s8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+        return *reinterpret_cast<const u4 *>(lds + at[k] + i * 16 * BK * 2);
+    }
+}
+
+// A lane's places for `fragment`, from the operand's LDS on, for a wave whose rows begin at tile `first` (a multiple of `tiles`, 2,
+// 4 or 8, that it has).
+template <bool DOWN, int PITCH>
+__device__ __forceinline__ void places(uint32_t (&at)[2], int lane, uint32_t base, int first) {
+    if constexpr (DOWN) {
+        const int row = 8 * (lane >> 4) + (lane >> 2 & 3);
+        at[0] = base + row * PITCH + (lane & 3) * 8 + (first & ~7) * 32;
+        at[1] = (uint32_t)(down_swizzle(row) ^ (first & 7)) * 32;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            at[k] = base + (first * 16 + (lane & 15)) * BK * 2 + (((k * 4 + (lane >> 4)) ^ (lane >> 1 & 7)) << 4);
+    }
+}
+
 // The fragments of a block: two steps of 32 along the contraction; A's rows in two halves.
-template <class S, bool DOWN>
+template <class S, int DOWN>
 struct Frags {
     static constexpr int H = S::TM / 2;
+    static constexpr bool DA = (DOWN & DOWN_A) != 0, DB = (DOWN & DOWN_B) != 0;
+    static constexpr int READ_A = DA ? 2 : 1, READ_B = DB ? 2 : 1;  // reads from LDS for a tile
     u4 lo[2][H], hi[2][H], b[2][S::TN];
-    // Tile i of A: 16 bytes of a row, or DOWN two reads of four rows each, at_a[0] the lane's place in a row of tile 0 and at_a[1]
-    // its swizzle.
-    __device__ __forceinline__ static u4 read_a(const char *__restrict__ lds, const uint32_t (&at_a)[2], int k, int i) {
-        if constexpr (DOWN) {
-            typedef short s4 __attribute__((ext_vector_type(4)));
-            typedef short s8 __attribute__((ext_vector_type(8)));
-            typedef __attribute__((address_space(3))) s4 lds_s4;
-            const char *at = lds + at_a[0] + k * 32 * S::BM * 2 + ((uint32_t)(i * 32) ^ at_a[1]);
-            const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)at);
-            const s4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(at + 4 * S::BM * 2));
-            return __builtin_bit_cast(u4, (s8)__builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-        } else {
-            return *reinterpret_cast<const u4 *>(lds + at_a[k] + i * 16 * BK * 2);
-        }
-    }
     __device__ __forceinline__ void read_lo(const char *__restrict__ lds, const uint32_t (&at_a)[2], int k) {
 #pragma unroll
-        for (int i = 0; i < H; ++i) lo[k][i] = read_a(lds, at_a, k, i);
+        for (int i = 0; i < H; ++i) lo[k][i] = fragment<DA, S::BM * 2>(lds, at_a, k, i);
     }
     __device__ __forceinline__ void read_hi(const char *__restrict__ lds, const uint32_t (&at_a)[2], int k) {
 #pragma unroll
-        for (int i = 0; i < H; ++i) hi[k][i] = read_a(lds, at_a, k, H + i);
+        for (int i = 0; i < H; ++i) hi[k][i] = fragment<DA, S::BM * 2>(lds, at_a, k, H + i);
     }
     __device__ __forceinline__ void read_b(const char *__restrict__ lds, const uint32_t (&at_b)[2], int k) {
 #pragma unroll
-        for (int j = 0; j < S::TN; ++j) b[k][j] = *reinterpret_cast<const u4 *>(lds + at_b[k] + j * 16 * BK * 2);
+        for (int j = 0; j < S::TN; ++j) b[k][j] = fragment<DB, S::BN * 2>(lds, at_b, k, j);
     }
     template <bool F16>
     __device__ __forceinline__ void mul_lo(acc_t (&acc)[S::TM][S::TN], int k) const {
@@ -284,10 +319,11 @@ struct Frags {
 
 // First half of a block: the products of A's lower rows, while the rest of the block's fragments are read, one between two
 // products, and the first product before them (its wait is for what the last half has read).
-template <class S, bool F16, bool DOWN>
+template <class S, bool F16, int DOWN>
 __device__ __forceinline__ void first_half(const char *__restrict__ rd, const uint32_t (&at_a)[2], const uint32_t (&at_b)[2],
                                            Frags<S, DOWN> &f, acc_t (&acc)[S::TM][S::TN]) {
-    constexpr int H = S::TM / 2, READS = S::TN + 2 * H * (DOWN ? 2 : 1), PRODUCTS = H * S::TN;
+    constexpr int H = S::TM / 2, PRODUCTS = H * S::TN;
+    constexpr int READS = S::TN * Frags<S, DOWN>::READ_B + 2 * H * Frags<S, DOWN>::READ_A;
     f.template mul_lo<F16>(acc, 0);
     f.read_b(rd, at_b, 1);
     f.read_hi(rd, at_a, 0);
@@ -307,11 +343,12 @@ __device__ __forceinline__ void first_half(const char *__restrict__ rd, const ui
 // Second half: the products of A's upper rows, while the block after the next is loaded into this one's LDS and the next
 // one's fragments are read in the place of those that no product needs any more.  A load takes the memory pipe 16 cycles for
 // each of the workgroup's waves, so loads stand between products: in one run they held the products up.
-template <class S, bool F16, bool DOWN>
+template <class S, bool F16, int DOWN>
 __device__ __forceinline__ void second_half(const char *__restrict__ rd, char *__restrict__ wr, const Loader<S, DOWN> &ld,
                                             const uint32_t (&at_a)[2], const uint32_t (&at_b)[2], Frags<S, DOWN> &f,
                                             acc_t (&acc)[S::TM][S::TN]) {
-    constexpr int R = S::RA + S::RB, P = S::TM / 2 * S::TN, READS = S::TM * (DOWN ? 2 : 1);
+    constexpr int R = S::RA + S::RB, P = S::TM / 2 * S::TN;
+    constexpr int READS = S::TM * Frags<S, DOWN>::READ_A, READS_B = S::TN * Frags<S, DOWN>::READ_B;
     ld.template load<0, R / 2>(wr);
     f.template mul_hi<F16>(acc, 0);
     f.read_lo(rd, at_a, 0);
@@ -328,7 +365,7 @@ __device__ __forceinline__ void second_half(const char *__restrict__ rd, char *_
     f.template mul_hi<F16>(acc, 1);
 #pragma unroll
     for (int i = 0; i < P / 2; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, (READS_B + P / 2 - 1) / (P / 2), 0);
         __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
         __builtin_amdgcn_sched_group_barrier(0x020, (R - R / 2 + P / 2 - 1) / (P / 2), 0);
     }
@@ -345,7 +382,7 @@ __device__ __forceinline__ void clear(acc_t (&acc)[S::TM][S::TN]) {
 
 // Forms the workgroup's tiles and hands each to epilogue(tm, tn, acc).
 // acc[i][j]: rows m = 16 i + 4 (lane / 16) + q of this wave's part for register q, column n = 16 j + lane % 16.
-template <class S, bool F16, bool DOWN = false, class E>
+template <class S, bool F16, int DOWN = 0, class E>
 __device__ __forceinline__ void products(const Args &g, const Extent &x, char *lds, E &&epilogue) {
     const int lane = threadIdx.x & 63, w = wave_index(), wm = w / S::WN, wn = w % S::WN;
     const int total = x.kit * g.nseg;
@@ -357,17 +394,8 @@ __device__ __forceinline__ void products(const Args &g, const Extent &x, char *l
     ld.w = w;
     if (ld.tile >= ld.tiles) return;
     uint32_t at_a[2], at_b[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const uint32_t c = ((k * 4 + (lane >> 4)) ^ (lane >> 1 & 7)) << 4;
-        at_a[k] = (wm * (S::BM / S::WM) + (lane & 15)) * BK * 2 + c;
-        at_b[k] = S::A_BYTES + (wn * (S::BN / S::WN) + (lane & 15)) * BK * 2 + c;
-    }
-    if constexpr (DOWN) {
-        const int row = 8 * (lane >> 4) + (lane >> 2 & 3), first_pair = wm * S::TM;  // of a multiple of 4, a power of two
-        at_a[0] = row * S::BM * 2 + (lane & 3) * 8 + (first_pair & ~7) * 32;
-        at_a[1] = (uint32_t)(down_swizzle(row) ^ (first_pair & 7)) * 32;
-    }
+    places<(DOWN & DOWN_A) != 0, S::BM * 2>(at_a, lane, 0, wm * S::TM);
+    places<(DOWN & DOWN_B) != 0, S::BN * 2>(at_b, lane, S::A_BYTES, wn * S::TN);
     char *cur = lds, *other = lds + S::STAGE;
     if (blocks > 0) {  // else empty sums
         ld.start(g, x, first, end);
@@ -475,10 +503,11 @@ struct Result {
     int dt;
     const float *row;
     const int *exps;
-    int base, sign[3];
+    int base, sign[2];
     float *acc;
     int64_t ldp;
     int add;
+    const float *by;   // y times by[0], where given
     const int *place;  // for finish(): the row of acc (and of `row`) that y's row n is, or -1 for zeros; NULL: row n
 };
 inline int64_t columns_of(int64_t cols) { return (cols + 3) / 4 * 4; }  // whole 16 bytes
@@ -487,8 +516,9 @@ enum : int { BIG = 0, MID = 1, FEW = 2, ONE = 3 };
 struct Plan {
     int shape, splits;
 };
-// The tile and the split of the contraction (at most max_splits) for rows x cols results of `blocks` BK-blocks.
-Plan plan(int64_t rows, int64_t cols, int64_t blocks, int max_splits);
+// The tile and the split of the contraction (at most max_splits) for rows x cols results of `blocks` BK-blocks.  large: not the
+// tiles for few rows (an operand across the contraction has wide rows in LDS).
+Plan plan(int64_t rows, int64_t cols, int64_t blocks, int max_splits, bool large = false);
 
 // Fills in the tiles of g and the grid of a launch.
 template <class S>
@@ -507,7 +537,7 @@ void finish(const Result &r, int splits, int64_t rows, int64_t cols, hipStream_t
 
 __device__ __forceinline__ int exponent_of(const Result &r) {
     int e = r.base;
-    if (r.exps) e += r.sign[0] * r.exps[0] + r.sign[1] * r.exps[1] + r.sign[2] * r.exps[2];
+    if (r.exps) e += r.sign[0] * r.exps[0] + r.sign[1] * r.exps[1];
     return e;
 }
 

@@ -64,8 +64,8 @@ __global__ __launch_bounds__(1024) void maxima_kernel(const Pair both, float *pa
     }
 }
 
-__global__ __launch_bounds__(64) void exponents_kernel(const float *part, const Tops tops, int *exps) {
-    const int i = blockIdx.x, top = i == 0 ? tops.top[0] : i == 1 ? tops.top[1] : tops.top[2];
+__global__ __launch_bounds__(64) void exponents_kernel(const float *part, int top, int *exps, float *most) {
+    const int i = blockIdx.x;
     float m = 0.f;
 #pragma unroll
     for (int k = 0; k < PARTS / 64; ++k) m = fmaxf(m, part[i * PARTS + k * 64 + threadIdx.x]);
@@ -73,7 +73,8 @@ __global__ __launch_bounds__(64) void exponents_kernel(const float *part, const 
     if (threadIdx.x == 0) {
         int e = 0;
         if (m > 0.f) (void)frexpf(m, &e);  // m in [2^(e - 1), 2^e)
-        exps[i] = m > 0.f ? top + 1 - e : 0;
+        if (i < 2) exps[i] = m > 0.f ? top + 1 - e : 0;
+        else most[0] = m;
     }
 }
 
@@ -124,8 +125,8 @@ __global__ __launch_bounds__(NT) void terms_kernel(const Source s, int nterms, c
 
 // 64 x 64 elements to a workgroup, turned over in LDS.
 template <bool F16, int DT>
-__global__ __launch_bounds__(NT) void across_kernel(const Source s, int slots, const int *exps, int which, uint16_t *dst,
-                                                    int64_t kp, int64_t tiles_c, int64_t tiles) {
+__global__ __launch_bounds__(NT) void across_kernel(const Source s, int slots, const int *exps, int which, const Factors f,
+                                                    uint16_t *dst, int64_t kp, int64_t tiles_c, int64_t tiles) {
     __shared__ float tile[64][65];
     const int64_t t0 = block_index();
     if (t0 >= tiles) return;
@@ -138,8 +139,13 @@ __global__ __launch_bounds__(NT) void across_kernel(const Source s, int slots, c
         float x[8];
         const int64_t at = r < s.rows ? row_of(s, r) : -1;
         ops::load_first<8, DT>(s.p, at * s.ld + c, at < 0 ? 0 : s.cols - c, x);
+        float by = 1.f;
+        if (f.row && at >= 0) {
+            const float most = f.by[0];
+            by = most > 0.f ? f.row[r] / most : f.row[r];
+        }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) tile[rl][cl + j] = ldexpf(x[j], e);
+        for (int j = 0; j < 8; ++j) tile[rl][cl + j] = at < 0 ? 0.f : ldexpf(x[j] * by, e);
     }
     __syncthreads();
 #pragma unroll
@@ -178,8 +184,8 @@ void maxima(const Source (&s)[2], float *part, hipStream_t st) {
     else hipLaunchKernelGGL((maxima_kernel<DT_F16>), grid, block, 0, st, p, part);
 }
 
-void exponents(const float *part, const Tops &top, int *exps, hipStream_t st) {
-    hipLaunchKernelGGL(exponents_kernel, dim3(3), dim3(64), 0, st, part, top, exps);
+void exponents(const float *part, int top, int *exps, float *most, hipStream_t st) {
+    hipLaunchKernelGGL(exponents_kernel, dim3(3), dim3(64), 0, st, part, top, exps, most);
 }
 
 #define GDN_TERMS_OF(KERNEL, F16, ...)                                                                                \
@@ -197,11 +203,11 @@ void terms(const Source &s, int nterms, bool f16, const int *exps, int which, vo
     GDN_TERMS(terms_kernel, s, nterms, exps, which, static_cast<uint16_t *>(dst), kp);
 }
 
-void terms_across(const Source &s, int nterms, bool f16, const int *exps, int which, void *dst, hipStream_t st) {
+void terms_across(const Source &s, int slots, bool f16, const int *exps, int which, const Factors &f, void *dst, hipStream_t st) {
     Timed tm("terms_across", st);
     const int64_t kp = padded(s.rows), tc = (s.cols + 63) / 64, tiles = kp / 64 * tc;
     const dim3 grid = grid_of(tiles);
-    GDN_TERMS(across_kernel, s, across_slots(nterms), exps, which, static_cast<uint16_t *>(dst), kp, tc, tiles);
+    GDN_TERMS(across_kernel, s, slots, exps, which, f, static_cast<uint16_t *>(dst), kp, tc, tiles);
 }
 #undef GDN_TERMS
 #undef GDN_TERMS_OF
