@@ -357,7 +357,7 @@ int gdn_clip_grad_norm(const void *const *x, void *const *y, const int64_t *nume
 /* Cross entropy of the logits z = x w^T, which are never kept.  x [N][H] and w [V][H] (dtype; row strides in elements, channels
  * contiguous), targets [N]:
  *   loss [N]      log sum_v e^{z_v} - z_target; 0 where targets == ignore_index; NaN where the target is outside [0, V)
- *   stat [N][2]   what gdn_linear_loss_bwd needs (may be NULL)
+ *   stat [N + 1][2]   what gdn_linear_loss_bwd needs (may be NULL)
  *   total [1]     reduction 1: the losses' sum; 2: their mean over the tokens that count (0 if none does)
  *   factor [1]    what takes the cotangent of that to a token's.  reduction 0: neither is written, both may be NULL
  * fp32 outputs.  What x holds at ignored tokens does not reach any other token, nor w's gradient.

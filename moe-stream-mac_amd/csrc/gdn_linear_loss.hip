@@ -389,6 +389,7 @@ struct Sizes {
     int terms;
     bool compact;
     bool down;     // dx from the weight as it lies
+    int wslots;    // terms of the weight's rows
     bool rows;     // the differences are two bf16 terms, as rows
     int64_t prows; // rows of the differences
     int slots;     // terms of the operands that meet them: the weight for dx, x for dW
@@ -411,6 +412,7 @@ static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt, bool direct_w, bool 
     s.rows = s.down && dx && dt == GDN_BF16;
     s.prows = s.rows ? 2 * N : N;
     s.slots = s.terms == 1 ? 1 : 3;
+    s.wslots = s.terms > 1 && dx ? s.slots : s.terms;
     int64_t most = KEPT / s.np / 256 * 256;
     if (most < 256) most = 256;
     s.pieces = (V + most - 1) / most;
@@ -459,7 +461,7 @@ static Buffers place(Space &sp, const Sizes &s, bool dx, bool dw, bool bwd, bool
         b.tokens.target = sp.take<int64_t>(s.N);
     }
     if (copy_x || s.compact) b.x = sp.take<uint16_t>(s.N * t * s.hp);
-    if (copy_w) b.w = sp.take<uint16_t>(words * t * s.hp);
+    if (copy_w) b.w = sp.take<uint16_t>(words * s.wslots * s.hp);
     if (!bwd) {
         b.stats = sp.take<float2>(s.parts * s.tokens);
         b.zt = sp.take<float>(s.tokens);
@@ -469,7 +471,7 @@ static Buffers place(Space &sp, const Sizes &s, bool dx, bool dw, bool bwd, bool
     b.factor = sp.take<float>(s.N);
     b.p = sp.take<uint16_t>(s.prows * t * padded(words));
     if (dx) {
-        if (!s.down) b.wt = sp.take<uint16_t>(s.H * s.slots * padded(words));
+        if (!s.down && t == 1) b.wt = sp.take<uint16_t>(s.H * s.slots * padded(words));
         b.acc_x = sp.take<float>((int64_t)s.px.splits * s.prows * columns_of(s.H));
     }
     if (dw) {
@@ -566,8 +568,9 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
             hipLaunchKernelGGL(tokens_kernel, dim3(1), dim3(1024), 0, st, targets, N, ignore_index, tk, loss);
         if (dtype == GDN_F32) {
             maxima({sx, sw}, b.part, st);
-            exponents(b.part, TOP, b.exps, b.most, st);  // the third is not read
-            exps = b.exps;
+            int *to = stat ? reinterpret_cast<int *>(stat + 2 * N) : b.exps;
+            exponents(b.part, TOP, to, b.most, st);  // b.most is not read
+            exps = to;
         }
         if (!dx) terms(sx, s.terms, f16, exps, E_X, b.x, st);
         // operands that are used as they lie need no pieces
@@ -655,14 +658,18 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
     if (s.compact) hipLaunchKernelGGL(tokens_kernel, dim3(1), dim3(1024), 0, st, targets, N, ignore_index, tk, nullptr);
     hipLaunchKernelGGL(cotangent_kernel, dim3(PARTS), dim3(NT), 0, st, tt, dloss, dloss_stride, factor, N, V, ignore_index,
                        b.power, b.factor, b.part + 2 * PARTS, tk.index, tk.count);
-    Source mx = sx, mw = sw;  // what is stored times a power of two
-    if ((!dw || s.rows) && dtype != GDN_F32) mx.rows = 0;
-    if ((!dx || s.down) && dtype != GDN_F32) mw.rows = 0;
-    if (mx.rows + mw.rows > 0) maxima({mx, mw}, b.part, st);
-    if (dw || mw.rows > 0) exponents(b.part, TOP, b.exps, b.most, st);
-    const int *exps = dtype == GDN_F32 ? b.exps : nullptr;
-    if (!direct_x) terms(sx, t, f16, exps, E_X, b.x, st);
-    if (dw) terms_across(sx, s.slots, !s.rows, s.rows ? nullptr : b.exps, E_X, Factors{b.power, b.most}, b.xt, st);
+    // what is stored times a power of two: of fp32 inputs the forward call has found it
+    const int *exps = t > 1 ? reinterpret_cast<const int *>(stat + 2 * N) : b.exps;
+    const bool scaled_x = t == 1 && dw && !s.rows, scaled_w = t == 1 && dx && !s.down;
+    if (scaled_x || scaled_w) {
+        Source mx = sx, mw = sw;
+        if (!scaled_x) mx.rows = 0;
+        if (!scaled_w) mw.rows = 0;
+        maxima({mx, mw}, b.part, st);
+    }
+    if (dw || scaled_w) exponents(b.part, TOP, scaled_x || scaled_w ? b.exps : nullptr, b.most, st);
+    if (!direct_x) terms(sx, t, f16, t > 1 ? exps : nullptr, E_X, b.x, st);
+    if (dw) terms_across(sx, s.slots, !s.rows, s.rows ? nullptr : exps, E_X, Factors{b.power, b.most}, b.xt, st);
     const int shape = plan(N, s.piece, s.slots * s.hp / BK, 1).shape;
     for (int64_t v0 = 0; v0 < V; v0 += s.piece) {
         const int64_t words = V - v0 < s.piece ? V - v0 : s.piece, kp = padded(words);
@@ -681,13 +688,14 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
             g.a.p = static_cast<const char *>(part.p);
             g.a.ld = w_stride * 2;
         } else {
-            terms(part, t, f16, exps, E_W, b.w, st);
+            g.a.ld = s.wslots * s.hp * 2;
+            terms(part, s.wslots, f16, t > 1 ? exps : nullptr, E_W, b.w, st);
         }
         if (direct_x) {
             g.b.p = static_cast<const char *>(x);
             g.b.ld = x_stride * 2;
         }
-        const DiffArgs a{tt, reinterpret_cast<const float2 *>(stat), b.power, b.factor, b.exps, b.p, v0, kp};
+        const DiffArgs a{tt, reinterpret_cast<const float2 *>(stat), b.power, b.factor, exps, b.p, v0, kp};
         {
             Timed tm("loss_diff", st);
 #define GDN_DIFF(S) launch_diff_of<S>(g, a, dtype, s.rows, st)
@@ -696,15 +704,20 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
         }
         if (dx) {
             Args h{};
-            if (s.down) {
-                h.a = Operand{static_cast<const char *>(part.p), w_stride * 2, H, {0, 0, 0}, H * 2};
+            if (s.down || t > 1) {
                 h.kit = (int)(kp / BK);
-                h.nseg = 1;
+                h.nseg = s.slots;
                 h.across = DOWN_A;
                 h.down = words;
+                if (s.down) {
+                    h.a = Operand{static_cast<const char *>(part.p), w_stride * 2, H, {0, 0, 0}, H * 2};
+                } else {
+                    h.a = Operand{reinterpret_cast<const char *>(b.w), g.a.ld, H, {0, s.hp * 2, s.hp * 4}, s.hp * 2};
+                    h.b.off[2] = kp * 2;
+                }
             } else {
-                terms_across(part, s.slots, true, b.exps, E_W, Factors{nullptr, nullptr}, b.wt, st);
-                segments(h, s.slots, kp, t > 1 ? kp * 2 : 0);
+                terms_across(part, 1, true, exps, E_W, Factors{nullptr, nullptr}, b.wt, st);
+                segments(h, 1, kp, 0);
                 h.a.p = reinterpret_cast<const char *>(b.wt);
                 h.a.rows = H;
             }
@@ -713,8 +726,8 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
             h.b.rows = s.prows;
             h.live = tk.count;
             const Plan pl = s.px;  // parts without a block of the last piece add nothing
-            Result r{dx, H, dtype, b.power, b.exps, -SHIFT, {0, s.down ? 0 : -1}, nullptr, columns_of(H), v0 > 0, nullptr, tk.place};
-            if (s.down || s.compact || s.pieces > 1 || pl.splits > 1) r.acc = b.acc_x;
+            Result r{dx, H, dtype, b.power, exps, -SHIFT, {0, s.down ? 0 : -1}, nullptr, columns_of(H), v0 > 0, nullptr, tk.place};
+            if (h.across || s.compact || s.pieces > 1 || pl.splits > 1) r.acc = b.acc_x;
             multiply(h, !s.down || dtype == GDN_F16, pl, r, st);
             if (r.acc && v0 + words == V) finish(r, pl.splits * (int)(s.prows / N), N, H, st);  // terms are parts too
         }
@@ -731,7 +744,7 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
             h.down = N;
             h.live = tk.count;
             h.live_k = 1;
-            Result r{static_cast<char *>(dw) + v0 * H * elem, H, dtype, nullptr, b.exps, -SHIFT, {s.rows ? 0 : -1, 0}, nullptr,
+            Result r{static_cast<char *>(dw) + v0 * H * elem, H, dtype, nullptr, exps, -SHIFT, {s.rows ? 0 : -1, 0}, nullptr,
                      columns_of(H), 0, b.most, nullptr};
             if (s.pw.splits > 1) r.acc = b.acc_w;
             multiply(h, !s.rows, s.pw, r, st);

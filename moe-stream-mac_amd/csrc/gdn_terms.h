@@ -31,16 +31,16 @@ inline int64_t padded(int64_t cols) { return (cols + 63) / 64 * 64; }
 void maxima(const Source (&s)[2], float *part, hipStream_t st);
 
 // exps[i] = the exponent e_i that takes the largest of part[i][PARTS] to [2^top, 2^(top + 1)), for i < 2, 0 for zeros; most[0] = the
-// largest of part[2][PARTS].
+// largest of part[2][PARTS].  exps NULL: only that.
 void exponents(const float *part, int top, int *exps, float *most, hipStream_t st);
 
-// dst[r][t * padded(cols) + c] = term t of 2^e s[r][c], e = exps[which] (0 without exps), zeros behind the last column: x is
-// the sum of its terms up to the last one's rounding.  f16 or bf16 terms.
-void terms(const Source &s, int nterms, bool f16, const int *exps, int which, void *dst, hipStream_t st);
-
-// The same transposed, times f's factors (where f.row is not NULL): dst[c][t * padded(rows) + r] for t < slots.  The third of three
-// slots holds the first term times 2^-LOW, the partner of a second term that is stored times 2^LOW.
+// dst[r][t * padded(cols) + c] = term t < slots of 2^e s[r][c], e = exps[which] (0 without exps), zeros behind the last column: x
+// is the sum of its terms up to the last one's rounding.  f16 or bf16 terms; the third of three fp16 slots holds the first term
+// times 2^-LOW, the partner of a second term that is stored times 2^LOW.
 constexpr int LOW = 11;
+void terms(const Source &s, int slots, bool f16, const int *exps, int which, void *dst, hipStream_t st);
+
+// The same transposed, times f's factors (where f.row is not NULL): dst[c][t * padded(rows) + r].
 void terms_across(const Source &s, int slots, bool f16, const int *exps, int which, const Factors &f, void *dst, hipStream_t st);
 
 }  // namespace mm

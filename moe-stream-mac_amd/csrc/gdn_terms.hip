@@ -66,6 +66,7 @@ __global__ __launch_bounds__(1024) void maxima_kernel(const Pair both, float *pa
 
 __global__ __launch_bounds__(64) void exponents_kernel(const float *part, int top, int *exps, float *most) {
     const int i = blockIdx.x;
+    if (i < 2 && !exps) return;
     float m = 0.f;
 #pragma unroll
     for (int k = 0; k < PARTS / 64; ++k) m = fmaxf(m, part[i * PARTS + k * 64 + threadIdx.x]);
@@ -103,23 +104,27 @@ __device__ __forceinline__ uint4 pack8(const uint16_t (&b)[8]) {
 
 // Eight elements of a row to a thread.
 template <bool F16, int DT>
-__global__ __launch_bounds__(NT) void terms_kernel(const Source s, int nterms, const int *exps, int which, uint16_t *dst,
+__global__ __launch_bounds__(NT) void terms_kernel(const Source s, int slots, const int *exps, int which, uint16_t *dst,
                                                    int64_t kp) {
     const int64_t i = block_index() * NT + threadIdx.x;
     const uint32_t per = (uint32_t)(kp / 8);
     const int64_t r = i >> 32 ? i / per : (uint32_t)i / per, c = (i - r * per) * 8;
     if (r >= s.rows) return;
     const int e = exps ? exps[which] : 0;
-    float x[8];
+    float x[8], whole[8];
     const int64_t at = row_of(s, r);
     ops::load_first<8, DT>(s.p, at * s.ld + c, at < 0 ? 0 : s.cols - c, x);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = ldexpf(x[j], e);
-    for (int t = 0; t < nterms; ++t) {
+    for (int j = 0; j < 8; ++j) x[j] = whole[j] = ldexpf(x[j], e);
+    for (int t = 0; t < slots; ++t) {
         uint16_t b[8];
+        if (F16 && t == 2) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = ldexpf(whole[j], -LOW);
+        }
 #pragma unroll
         for (int j = 0; j < 8; ++j) b[j] = next_term<F16>(x[j]);
-        *reinterpret_cast<uint4 *>(dst + r * (kp * nterms) + t * kp + c) = pack8(b);
+        *reinterpret_cast<uint4 *>(dst + r * (kp * slots) + t * kp + c) = pack8(b);
     }
 }
 
@@ -158,7 +163,7 @@ __global__ __launch_bounds__(NT) void across_kernel(const Source s, int slots, c
         uint16_t *to = dst + (c0 + cl) * (kp * slots) + r0 + rl;
         for (int t = 0; t < slots; ++t) {
             uint16_t b[8];
-            if (t == 2) {
+            if (F16 && t == 2) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[j] = ldexpf(tile[rl + j][cl], -LOW);
             }
@@ -196,11 +201,11 @@ void exponents(const float *part, int top, int *exps, float *most, hipStream_t s
     if (f16) { GDN_TERMS_OF(KERNEL, true, __VA_ARGS__); }   \
     else { GDN_TERMS_OF(KERNEL, false, __VA_ARGS__); }
 
-void terms(const Source &s, int nterms, bool f16, const int *exps, int which, void *dst, hipStream_t st) {
+void terms(const Source &s, int slots, bool f16, const int *exps, int which, void *dst, hipStream_t st) {
     Timed tm("terms", st);
     const int64_t kp = padded(s.cols);
     const dim3 grid = grid_of((s.rows * (kp / 8) + NT - 1) / NT);
-    GDN_TERMS(terms_kernel, s, nterms, exps, which, static_cast<uint16_t *>(dst), kp);
+    GDN_TERMS(terms_kernel, s, slots, exps, which, static_cast<uint16_t *>(dst), kp);
 }
 
 void terms_across(const Source &s, int slots, bool f16, const int *exps, int which, const Factors &f, void *dst, hipStream_t st) {

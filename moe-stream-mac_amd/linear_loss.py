@@ -38,7 +38,7 @@ def _forward(x, w, targets, ignore_index, reduction, need_grad):
     (N, H), V = x.shape, w.shape[0]
     lib, dtype = L.load(), L.DTYPE_CODE[x.dtype]
     loss = torch.empty((N,), dtype=torch.float32, device=dev)
-    stat = torch.empty((N, 2), dtype=torch.float32, device=dev) if need_grad else None
+    stat = torch.empty((N + 1, 2), dtype=torch.float32, device=dev) if need_grad else None
     total = torch.empty((), dtype=torch.float32, device=dev) if reduction else None
     factor = torch.empty((), dtype=torch.float32, device=dev) if reduction else None
     nws = lib.gdn_linear_loss_workspace_bytes(N, H, V, dtype, _aligned(x, w), 0, 0)
