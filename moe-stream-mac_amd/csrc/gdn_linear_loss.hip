@@ -45,6 +45,7 @@ constexpr int64_t COMPACT = 2048;
 constexpr int64_t DOWN = 512;
 constexpr int64_t KEPT = 1 << 26;  // differences of a piece; statistics of the parts of the words
 constexpr int64_t MOST_TOKENS = 1 << 20;  // three slots of 16 bits for each are a row pitch that a product takes
+constexpr int WIDE = 128;          // up to here an fp32 weight is read as it lies
 constexpr int SHIFT = 15;          // differences are stored times 2^15
 constexpr int TOP = 14;            // largest magnitudes of scaled operands: [2^14, 2^15)
 
@@ -112,6 +113,51 @@ struct StatArgs {
     int part0;
 };
 
+// The statistics of a wave's words, `rows` - m0 of 16 TM, for its 16 TN tokens from n0 on.  e: the logits' scale.
+template <int TM, int TN, bool SCALED>
+__device__ __forceinline__ void statistics(const StatArgs &a, int64_t rows, int64_t tokens, int64_t m0, int64_t n0, int64_t part,
+                                           int e, acc_t (&acc)[TM][TN]) {
+    const int lane = lane_here();
+    const int words = (int)min((int64_t)(16 * TM), rows - m0);
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+        const int64_t n = n0 + 16 * j + (lane & 15);
+        const bool live = n < tokens;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                if constexpr (SCALED) acc[i][j][q] = ldexpf(acc[i][j][q], e);
+                if (words < 16 * TM && 16 * i + 4 * (lane >> 4) + q >= words) acc[i][j][q] = -INFINITY;
+                mx = fmaxf(mx, acc[i][j][q]);
+            }
+        mx = fmaxf(mx, lane_xor16(mx));
+        mx = fmaxf(mx, lane_xor32(mx));
+        const float ref = mx == -INFINITY ? 0.f : mx;
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) s += __builtin_amdgcn_exp2f((acc[i][j][q] - ref) * LOG2E);
+        s += lane_xor16(s);
+        s += lane_xor32(s);
+        if (live && lane < 16) a.part[part * a.N + n] = make_float2(mx, s);
+        const int64_t t = live ? a.targets[n] - a.v0 - m0 : -1;
+        const bool here = t >= 0 && t < words && ((t >> 2 & 3) == (lane >> 4));
+        if (__any(here)) {
+            const int tl = here ? (int)t - 4 * (lane >> 4) : -1;
+            float z = 0.f;
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (tl == 16 * i + q) z = acc[i][j][q];
+            if (here) a.zt[n] = z;
+        }
+    }
+}
+
 // Waves leave the statistics of their own words.
 template <class S, bool F16, bool SCALED>
 __global__ __launch_bounds__(S::NT, S::WAVES_EU) void stat_kernel(const Args g, const StatArgs a) {
@@ -119,48 +165,118 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void stat_kernel(const Args g, 
     const int w = wave_index(), wm = w / S::WN, wn = w % S::WN;
     const Extent ext = extent_of<S>(g);
     products<S, F16>(g, ext, lds, [&](int tm, int tn, acc_t(&acc)[S::TM][S::TN]) {
-        const int lane = lane_here();
-        const int64_t m0 = (int64_t)tm * S::BM + wm * (S::BM / S::WM);  // of the operand's rows
-        const int words = (int)min((int64_t)(S::BM / S::WM), g.a.rows - m0);
+        const int64_t m0 = (int64_t)tm * S::BM + wm * (S::BM / S::WM), n0 = (int64_t)tn * S::BN + wn * (S::BN / S::WN);
         const int e = SCALED ? -(a.exps[E_X] + a.exps[E_W]) : 0;
+        statistics<S::TM, S::TN, SCALED>(a, g.a.rows, ext.rows_b, m0, n0, a.part0 + tm * S::WM + wm, e, acc);
+    });
+}
+
+// Few tokens and fp32 words, forward: read once, as they lie, and split in registers into three bf16 terms, which hold them exactly
+// and at any magnitude, so that they need no scale.  Six products of terms; those left out are below 2^-21 of the factors.  The
+// tokens' terms, 16 TN rows of three slots, go through LDS, two stages of 64 along the contraction; a wave's 32 words stay its own
+// and go to registers, a stage ahead.  64765 x 4096 weights (1.06 GB, 208 us at a copy's rate): 32 tokens 238 us, 118 tokens 489 us,
+// where the conversions and one wave to a SIMD hold it back; by way of two fp16 terms 878 and 920.
+template <int TN>
+struct Wide {
+    static constexpr int NT = 256, BM = 128, BN = 16 * TN, TM = 2, SLOT = BN * BK * 2, STAGE = 3 * SLOT;
+    static constexpr int WAVES_EU = TN > 4 ? 1 : 2;
+};
+struct WideArgs {
+    const float *w;
+    int64_t ld, rows;
+    Operand x;
+    int kit;
+};
+
+// The first terms of x, cut off, and in x what they leave: NaN of infinities and NaN.
+__device__ __forceinline__ uint4 cut(float (&x)[8]) {
+    uint32_t b[8];
 #pragma unroll
-        for (int j = 0; j < S::TN; ++j) {
-            const int64_t n = (int64_t)tn * S::BN + wn * (S::BN / S::WN) + 16 * j + (lane & 15);
-            const bool live = n < ext.rows_b;
-            float mx = -INFINITY;
+    for (int k = 0; k < 8; ++k) {
+        b[k] = __float_as_uint(x[k]);
+        x[k] -= __uint_as_float(b[k] & 0xffff0000u);
+    }
+    uint4 y;
+    y.x = b[0] >> 16 | (b[1] & 0xffff0000u);
+    y.y = b[2] >> 16 | (b[3] & 0xffff0000u);
+    y.z = b[4] >> 16 | (b[5] & 0xffff0000u);
+    y.w = b[6] >> 16 | (b[7] & 0xffff0000u);
+    return y;
+}
+
+template <int TN>
+__global__ __launch_bounds__(256, Wide<TN>::WAVES_EU) void wide_kernel(const WideArgs g, const StatArgs a) {
+    typedef Wide<TN> S;
+    __shared__ __attribute__((aligned(16))) char lds[2 * S::STAGE];
+    const int lane = threadIdx.x & 63, w = wave_index();
+    const int64_t m0 = (int64_t)blockIdx.x * S::BM + w * 32;
+    const float *row[S::TM];
+#pragma unroll
+    for (int i = 0; i < S::TM; ++i) row[i] = g.w + min(m0 + 16 * i + (lane & 15), g.rows - 1) * g.ld + 8 * (lane >> 4);
+    Side<S, S::BN, false> b[3];
+#pragma unroll
+    for (int t = 0; t < 3; ++t) b[t].start(g.x, g.x.off[t], 0, g.x.rows, 0, 0);
+    float4 now[2][S::TM][2], next[2][S::TM][2];
+    const auto load = [&](float4(&to)[2][S::TM][2], char *stage) {
+#pragma unroll
+        for (int t = 0; t < 3; ++t) {
+#pragma unroll
+            for (int r = 0; r < Side<S, S::BN, false>::LOADS; ++r) b[t].load(stage + t * S::SLOT, r, w);
+            b[t].next(g.x);
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int i = 0; i < S::TM; ++i)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    if constexpr (SCALED) acc[i][j][q] = ldexpf(acc[i][j][q], e);
-                    if (words < S::BM / S::WM && 16 * i + 4 * (lane >> 4) + q >= words) acc[i][j][q] = -INFINITY;
-                    mx = fmaxf(mx, acc[i][j][q]);
-                }
-            mx = fmaxf(mx, lane_xor16(mx));
-            mx = fmaxf(mx, lane_xor32(mx));
-            const float ref = mx == -INFINITY ? 0.f : mx;
-            float s = 0.f;
+                for (int h = 0; h < 2; ++h) to[s][i][h] = *reinterpret_cast<const float4 *>(row[i] + s * 32 + h * 4);
 #pragma unroll
-            for (int i = 0; i < S::TM; ++i)
+        for (int i = 0; i < S::TM; ++i) row[i] += BK;
+    };
+    uint32_t at[2];
+    places<false, 0>(at, lane, 0, 0);
+    acc_t acc[S::TM][TN];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) s += __builtin_amdgcn_exp2f((acc[i][j][q] - ref) * LOG2E);
-            s += lane_xor16(s);
-            s += lane_xor32(s);
-            if (live && lane < 16) a.part[(int64_t)(a.part0 + tm * S::WM + wm) * a.N + n] = make_float2(mx, s);
-            const int64_t t = live ? a.targets[n] - a.v0 - m0 : -1;
-            const bool here = t >= 0 && t < words && ((t >> 2 & 3) == (lane >> 4));
-            if (__any(here)) {
-                const int tl = here ? (int)t - 4 * (lane >> 4) : -1;
-                float z = 0.f;
+    for (int i = 0; i < S::TM; ++i)
 #pragma unroll
-                for (int i = 0; i < S::TM; ++i)
+        for (int j = 0; j < TN; ++j) acc[i][j] = acc_t{0.f, 0.f, 0.f, 0.f};
+    load(now, lds);
+    for (int k = 0; k < g.kit; ++k) {
+        const char *stage = lds + (k & 1) * S::STAGE;
+        stage_barrier();
+        if (k + 1 < g.kit) load(next, lds + (~k & 1) * S::STAGE);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        if (tl == 16 * i + q) z = acc[i][j][q];
-                if (here) a.zt[n] = z;
+        for (int s = 0; s < 2; ++s) {
+            u4 x[S::TM][3];
+#pragma unroll
+            for (int i = 0; i < S::TM; ++i) {
+                const float4 lo = now[s][i][0], hi = now[s][i][1];
+                float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                for (int t = 0; t < 3; ++t) x[i][t] = __builtin_bit_cast(u4, cut(v));
+            }
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                u4 y[3];
+#pragma unroll
+                for (int t = 0; t < 3; ++t) y[t] = fragment<false, 0>(stage + t * S::SLOT, at, s, j);
+#pragma unroll
+                for (int t = 2; t >= 0; --t)  // the smallest first
+#pragma unroll
+                    for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+                        for (int c = 0; c <= t; ++c) acc[i][j] = mfma<false>(x[i][c], y[t - c], acc[i][j]);
             }
         }
-    });
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) now[s][i][h] = next[s][i][h];
+    }
+    statistics<S::TM, TN, false>(a, g.rows, g.x.rows, m0, 0, blockIdx.x * 4 + w, 0, acc);
 }
 
 // Joins a token's parts: TOKENS tokens to a workgroup, NT / TOKENS threads to a token.
@@ -428,6 +544,11 @@ static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt, bool direct_w, bool 
     return s;
 }
 
+// Whether the weight is read as fp32 numbers: few tokens, rows of whole blocks, 16 bytes aligned.
+static bool wide(const void *p, int64_t ld, int64_t N, int64_t H, int dt) {
+    return dt == GDN_F32 && N <= WIDE && H % BK == 0 && ld % 4 == 0 && aligned_to(p, 16);
+}
+
 struct Space {
     char *base;
     size_t at = 0;
@@ -478,6 +599,16 @@ static Buffers place(Space &sp, const Sizes &s, bool dx, bool dw, bool bwd, bool
         b.xt = sp.take<uint16_t>(s.H * s.slots * s.np);
         if (s.pw.splits > 1) b.acc_w = sp.take<float>((int64_t)s.pw.splits * words * columns_of(s.H));
     }
+    return b;
+}
+
+static Buffers place_wide(Space &sp, const Sizes &s) {
+    Buffers b{};
+    b.most = sp.take<float>(1);
+    b.part = sp.take<float>(3 * PARTS);
+    b.x = sp.take<uint16_t>(s.N * 3 * s.hp);
+    b.stats = sp.take<float2>((s.V + 127) / 128 * 4 * s.N);
+    b.zt = sp.take<float>(s.N);
     return b;
 }
 
@@ -535,8 +666,13 @@ static size_t need(const Sizes &s, bool dx, bool dw, bool bwd, bool copy_x, bool
 extern "C" size_t gdn_linear_loss_workspace_bytes(int64_t N, int64_t H, int64_t V, int dtype, int aligned, int want_dx,
                                                   int want_dw) {
     if (N <= 0 || H <= 0 || V <= 0 || N > MOST_TOKENS || V > 1 << 24 || H > 1 << 17) return 0;
-    const bool copy = !aligned || dtype == GDN_F32 || H % BK;
-    return need(sizes(N, H, V, dtype, !copy, want_dx), want_dx, want_dw, want_dx || want_dw, copy, copy);
+    const bool copy = !aligned || dtype == GDN_F32 || H % BK, bwd = want_dx || want_dw;
+    const Sizes s = sizes(N, H, V, dtype, !copy, want_dx);
+    const size_t bytes = need(s, want_dx, want_dw, bwd, copy, copy);
+    if (bwd || !wide(nullptr, 0, N, H, dtype)) return bytes;
+    Space sp{nullptr};  // the forward call alone reads fp32 weights so, where they are aligned
+    place_wide(sp, s);
+    return bytes < sp.at ? sp.at : bytes;
 }
 
 extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *targets, float *loss, float *stat, float *total,
@@ -553,11 +689,13 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
         const bool dw = direct(w, w_stride, H, dtype);
         const Sizes s = sizes(N, H, V, dtype, dw, false);
         const bool dx = !s.compact && direct(x, x_stride, H, dtype);
-        const size_t bytes = need(s, false, false, false, !dx, !dw);
-        if (workspace_bytes < bytes)
-            return fail(GDN_ERR_WORKSPACE, "the workspace holds %zu bytes, %zu are needed", workspace_bytes, bytes);
-        Space sp{static_cast<char *>(workspace)};
-        const Buffers b = place(sp, s, false, false, false, !dx, !dw);
+        const bool few = wide(w, w_stride, N, H, dtype);
+        Space size{nullptr}, sp{static_cast<char *>(workspace)};
+        if (few) place_wide(size, s);
+        else place(size, s, false, false, false, !dx, !dw);
+        if (workspace_bytes < size.at)
+            return fail(GDN_ERR_WORKSPACE, "the workspace holds %zu bytes, %zu are needed", workspace_bytes, size.at);
+        const Buffers b = few ? place_wide(sp, s) : place(sp, s, false, false, false, !dx, !dw);
         const bool f16 = dtype != GDN_BF16;
         const int *exps = nullptr;
         const Tokens &tk = b.tokens;  // empty without
@@ -566,20 +704,32 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
         const Source sw{w, dtype, V, H, w_stride, nullptr, 0, nullptr, nullptr};
         if (s.compact)
             hipLaunchKernelGGL(tokens_kernel, dim3(1), dim3(1024), 0, st, targets, N, ignore_index, tk, loss);
-        if (dtype == GDN_F32) {
+        if (dtype == GDN_F32 && (stat || !few)) {
             maxima({sx, sw}, b.part, st);
             int *to = stat ? reinterpret_cast<int *>(stat + 2 * N) : b.exps;
             exponents(b.part, TOP, to, b.most, st);  // b.most is not read
             exps = to;
         }
-        if (!dx) terms(sx, s.terms, f16, exps, E_X, b.x, st);
+        if (few) terms(sx, 3, false, nullptr, E_X, b.x, st);
+        else if (!dx) terms(sx, s.terms, f16, exps, E_X, b.x, st);
         // operands that are used as they lie need no pieces
         const int64_t step = dw ? V : s.piece;
         for (int64_t n0 = 0; n0 < N; n0 += s.tokens) {
             const int64_t tokens = N - n0 < s.tokens ? N - n0 : s.tokens;
             const int shape = plan(tokens, dw ? V : s.piece, s.slots * s.hp / BK, 1).shape;
             int parts = 0;
-            for (int64_t v0 = 0; v0 < V; v0 += step) {
+            if (few) {  // all tokens
+                const Operand rows{reinterpret_cast<const char *>(b.x), 3 * s.hp * 2, N, {0, s.hp * 2, s.hp * 4}, 0};
+                const WideArgs g{static_cast<const float *>(w), w_stride, V, rows, (int)(s.hp / BK)};
+                const StatArgs a{tt, b.stats, b.zt, nullptr, N, V, 0, 0};
+                const dim3 grid((unsigned)((V + 127) / 128));
+                Timed tm("loss_stat", st);
+                if (N <= 32) hipLaunchKernelGGL((wide_kernel<2>), grid, dim3(256), 0, st, g, a);
+                else if (N <= 64) hipLaunchKernelGGL((wide_kernel<4>), grid, dim3(256), 0, st, g, a);
+                else hipLaunchKernelGGL((wide_kernel<8>), grid, dim3(256), 0, st, g, a);
+                parts = 4 * (int)grid.x;
+            }
+            for (int64_t v0 = 0; v0 < V && !few; v0 += step) {
                 const int64_t words = V - v0 < step ? V - v0 : step;
                 Args g{};
                 segments(g, s.terms, s.hp, s.terms > 1 ? s.hp * 2 : 0);

@@ -308,3 +308,40 @@ def test_second_gradients_are_refused(dev):
         leaf.mul_(2)
     with pytest.raises(RuntimeError, match="modified by an inplace"):
         loss.backward()
+
+
+@pytest.mark.parametrize("N,H,V", [(1, 64, 1), (1, 2048, 5000), (17, 192, 129), (33, 320, 3001), (64, 64, 128), (65, 1024, 777),
+                                   (128, 512, 4099), (129, 64, 300)])
+def test_few_fp32_scores(dev, N, H, V):
+    """Without gradients, few tokens, fp32 weights read as they lie (up to 128 tokens): three terms of each number are exact, and
+    the products left out, of a second and a third term, are below 2 * 2^-22 of the factors' product."""
+    from linear_loss import linear_cross_entropy
+    print("scores", N, H, V, flush=True)
+    x, w, t, _ = inputs(dev, N, H, V, torch.float32, 11)
+    if N > 2:
+        t[2] = -100
+        x[2] = math.nan  # of a token that does not count
+    want, tol = plain(x, w, t, torch.zeros(N, device=dev))
+    within(linear_cross_entropy(x, w, t, reduction="none"), want[0], tol[0], "loss")
+    rows = torch.full((V, H + 4), math.nan, device=dev)[:, :H].copy_(w)  # rows apart, still aligned
+    within(linear_cross_entropy(x, rows, t, reduction="none"), want[0], tol[0], "rows apart")
+    odd = torch.full((V * H + 1,), math.nan, device=dev)[1:].view(V, H).copy_(w)  # not aligned
+    within(linear_cross_entropy(x, odd, t, reduction="none"), want[0], tol[0], "not aligned")
+
+
+def test_few_fp32_scores_of_odd_values(dev):
+    """Magnitudes that no scale of fp16 terms would span, infinite words, NaN and targets that are no word."""
+    from linear_loss import linear_cross_entropy
+    N, H, V = 20, 128, 500
+    x, w, t, _ = inputs(dev, N, H, V, torch.float32, 12, ignored=False)
+    x[:, 0] *= 2.0 ** -60
+    w[:, 0] *= 2.0 ** 60
+    x[:, 1] *= 2.0 ** 50
+    w[:, 1] *= 2.0 ** -50
+    t[3], t[4] = V, -7
+    want, tol = plain(x, w, t, torch.zeros(N, device=dev))
+    within(linear_cross_entropy(x, w, t, reduction="none"), want[0], tol[0], "loss")
+    t[3] = t[4] = 0
+    for odd in (-math.inf, math.nan, math.inf):  # no number of terms adds up to an infinity: it counts as NaN
+        w[9, 5] = odd
+        assert bool(torch.isnan(linear_cross_entropy(x, w, t, reduction="none")).all())
