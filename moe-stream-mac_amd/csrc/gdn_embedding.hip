@@ -10,8 +10,9 @@
 // the sum of its lower bounds in all of them, looked up by bisection.  32768 tokens take two launches, a million three.
 //
 // Summing.  A word may have most of the tokens, so the sorted list is cut into chunks of 32.  A workgroup sums the
-// runs in its chunk: it writes the rows of words that begin and end there, and leaves what it has of the others.  A word's row
-// is then the sum of what its chunks left; of long batches, groups of 64 chunks of one word are summed first.
+// runs in its chunk: it writes the rows of words that begin and end there, and leaves what it has of the others, whose rows are
+// then the sums of what their chunks left; of long batches, groups of 64 chunks of one word are summed first.  Other workgroups
+// write the zeros of words without a token meanwhile.
 #include "gdn_common.h"
 #include "gdn_host.h"
 #include "gdn_vec.h"
@@ -26,6 +27,7 @@ constexpr int RUN_BITS = 10;
 constexpr int WAYS = 32;    // runs joined at a time
 constexpr int CHUNK = 32;   // tokens summed together
 constexpr int CT = 128;     // threads that do so
+constexpr int WORDS = 32;   // words whose zeros a workgroup writes
 constexpr int GROUP = 64;   // chunks of one word summed first
 constexpr int64_t LONG = 1 << 16;  // tokens from which on they are
 
@@ -128,7 +130,7 @@ struct SumArgs {
     double *group;  // [groups][H] of GROUP chunks that began with, and are within, one word; of long batches
     int *starts;    // [words + 1] the first place of each word's run
     int64_t N, words, ld;
-    int H, lanes;  // lanes: threads to a row, a power of two
+    int H;
     double scale;
 };
 
@@ -143,7 +145,9 @@ __device__ __forceinline__ void store_row(const SumArgs &s, int64_t v, int64_t c
     ops::store_first<V, DT>(s.dw, v * s.H + c, s.H - c, y);
 }
 
-// The first workgroups: sums of chunks, CT * V columns of one to each.  The others: the words' first places.
+// The first workgroups: sums of chunks, CT * V columns of one to each.  The others: the first places of WORDS words each, and the
+// zeros of those that no token has.  Their stores fill the memory's time while the sums wait for loads: 16384 tokens of 2048 bf16
+// channels, 32000 words (some 200 MB) 46 us, with the zeros in a pass of their own 35 and 38.
 template <int DT>
 __global__ __launch_bounds__(CT) void chunk_kernel(const SumArgs s, int64_t chunks, int parts) {
     constexpr int V = Width<DT>::V, U = 8;
@@ -199,17 +203,31 @@ __global__ __launch_bounds__(CT) void chunk_kernel(const SumArgs s, int64_t chun
         }
         return;
     }
-    const int64_t v = (g - chunks * parts) * CT + threadIdx.x;
-    if (v > s.words) return;
-    const uint64_t key = (uint64_t)v << 32;
-    int64_t lo = 0, len = s.N;
-    while (len > 0) {
-        const int64_t half = len >> 1;
-        const bool below = s.keys[lo + half] < key;
-        lo = below ? lo + half + 1 : lo;
-        len = below ? len - half - 1 : half;
+    __shared__ int64_t from[WORDS + 1];
+    const int64_t v0 = (g - chunks * parts) * WORDS;
+    if (v0 >= s.words) return;
+    const int words = (int)min((int64_t)WORDS, s.words - v0);
+    if ((int)threadIdx.x <= words) {
+        const uint64_t key = (uint64_t)(v0 + threadIdx.x) << 32;
+        int64_t lo = 0, len = s.N;
+        while (len > 0) {
+            const int64_t half = len >> 1;
+            const bool below = s.keys[lo + half] < key;
+            lo = below ? lo + half + 1 : lo;
+            len = below ? len - half - 1 : half;
+        }
+        from[threadIdx.x] = lo;
+        if ((int)threadIdx.x < words || v0 + words == s.words) s.starts[v0 + threadIdx.x] = (int)lo;
     }
-    s.starts[v] = (int)lo;
+    __syncthreads();
+    const uint32_t per = (uint32_t)((s.H + V - 1) / V);
+    double zero[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) zero[j] = 0.;
+    for (uint32_t i = threadIdx.x; i < per * words; i += CT) {
+        const uint32_t r = i / per;
+        if (from[r] == from[r + 1]) store_row<DT>(s, v0 + r, (int64_t)(i - r * per) * V, zero);
+    }
 }
 
 // x += `count` rows of sums, `step` numbers apart.
@@ -235,47 +253,42 @@ __global__ __launch_bounds__(NT) void group_kernel(const SumArgs s) {
     }
 }
 
+// The words whose runs go over the end of a chunk: each by the workgroups of the second chunk that has it, two columns to a thread.
 template <int DT>
-__global__ __launch_bounds__(NT) void words_kernel(const SumArgs s) {
-    constexpr int V = Width<DT>::V;
-    const int lane = threadIdx.x & (s.lanes - 1);
-    const int64_t v = block_index() * (NT / s.lanes) + threadIdx.x / s.lanes;
-    if (v >= s.words) return;
-    const int64_t a = s.starts[v], b = s.starts[v + 1];
-    const int64_t c0 = a / CHUNK, c1 = (b - 1) / CHUNK;
-    if (a < b && c0 == c1) return;  // written by its chunk
-    for (int64_t c = (int64_t)lane * V; c < s.H; c += s.lanes * V) {
-        double x[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) x[j] = 0.;
-        if (a < b) {
-            // what chunk c0 left of the run that goes on, then what chunks c0 + 1 to c1 did of the run that began before, whole
-            // groups of them at once
-            const int64_t step = 2 * s.H, g0 = (c0 + GROUP) / GROUP, g1 = s.group ? b / CHUNK / GROUP : 0;
-            const bool grouped = g0 < g1;
+__global__ __launch_bounds__(NT) void words_kernel(const SumArgs s, int parts) {
+    const int64_t i = block_index(), chunk = i / parts + 1;
+    if (chunk * CHUNK >= s.N) return;
+    const int64_t id = word(s.keys[chunk * CHUNK]);
+    if (id == s.words || word(s.keys[chunk * CHUNK - 1]) != id) return;
+    const int64_t a = s.starts[id], b = s.starts[id + 1], c0 = a / CHUNK, c1 = (b - 1) / CHUNK;
+    const int64_t c = ((i - (chunk - 1) * parts) * NT + threadIdx.x) * 2;
+    if (c0 != chunk - 1 || c >= s.H) return;
+    // what chunk c0 left of the run that goes on, then what chunks c0 + 1 to c1 did of the run that began before, whole groups of
+    // them at once
+    double x[2] = {0., 0.};
+    const int64_t step = 2 * s.H, g0 = (c0 + GROUP) / GROUP, g1 = s.group ? b / CHUNK / GROUP : 0;
+    const bool grouped = g0 < g1;
 #pragma unroll 1
-            for (int k = 0; k < 4; ++k) {
-                const double *p = s.part + c;
-                int64_t count, by = step;
-                if (k == 0) {
-                    p += c0 * step + s.H;
-                    count = 1;
-                } else if (k == 1) {
-                    p += (c0 + 1) * step;
-                    count = grouped ? g0 * GROUP - c0 - 1 : c1 - c0;
-                } else if (k == 2) {
-                    p = s.group + g0 * s.H + c;
-                    count = grouped ? g1 - g0 : 0;
-                    by = s.H;
-                } else {
-                    p += g1 * GROUP * step;
-                    count = grouped ? c1 + 1 - g1 * GROUP : 0;
-                }
-                add_sums<V>(p, count, by, s.H - c, x);
-            }
+    for (int k = 0; k < 4; ++k) {
+        const double *p = s.part + c;
+        int64_t count, by = step;
+        if (k == 0) {
+            p += c0 * step + s.H;
+            count = 1;
+        } else if (k == 1) {
+            p += (c0 + 1) * step;
+            count = grouped ? g0 * GROUP - c0 - 1 : c1 - c0;
+        } else if (k == 2) {
+            p = s.group + g0 * s.H + c;
+            count = grouped ? g1 - g0 : 0;
+            by = s.H;
+        } else {
+            p += g1 * GROUP * step;
+            count = grouped ? c1 + 1 - g1 * GROUP : 0;
         }
-        store_row<DT>(s, v, c, x);
+        add_sums<2>(p, count, by, s.H - c, x);
     }
+    for (int j = 0; j < 2 && c + j < s.H; ++j) store_from_f32(s.dw, id * s.H + c + j, (float)(x[j] * s.scale), DT);
 }
 
 static int check(int64_t N, int64_t V, int64_t H, int dt) {
@@ -357,17 +370,15 @@ extern "C" int gdn_embedding_bwd(const int64_t *ids, const void *dy, void *dw, v
     }
     s.keys = keys; s.dy = dy; s.dw = dw;
     s.N = N; s.words = V; s.ld = dy_stride; s.H = (int)H; s.scale = scale;
-    s.lanes = 1;
-    while (s.lanes < emb::NT && s.lanes * emb::width(dtype) < H) s.lanes *= 2;
     const int parts = (int)((H + emb::CT * emb::width(dtype) - 1) / (emb::CT * emb::width(dtype)));
-    const dim3 block(emb::NT), some = grid_of(chunks * parts + (V + emb::CT) / emb::CT);
-    const dim3 all = grid_of((V + emb::NT / s.lanes - 1) / (emb::NT / s.lanes));
+    const int pairs = (int)((H + 2 * emb::NT - 1) / (2 * emb::NT));
+    const dim3 block(emb::NT), some = grid_of(chunks * parts + (V + emb::WORDS - 1) / emb::WORDS);
     {
         Timed tm("embedding_sum", st);
 #define GDN_SUMS(DT)                                                                  \
     hipLaunchKernelGGL((emb::chunk_kernel<DT>), some, dim3(emb::CT), 0, st, s, chunks, parts); \
     if (groups) hipLaunchKernelGGL(emb::group_kernel, dim3((unsigned)groups), block, 0, st, s); \
-    hipLaunchKernelGGL((emb::words_kernel<DT>), all, block, 0, st, s)
+    if (chunks > 1) hipLaunchKernelGGL((emb::words_kernel<DT>), grid_of((chunks - 1) * pairs), block, 0, st, s, pairs)
         GDN_BY_TYPE(dtype, GDN_SUMS)
 #undef GDN_SUMS
     }
