@@ -437,13 +437,24 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
             for (int i = 0; i < S::TM; ++i)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const int m = 16 * i + q;
                     float z = acc[i][j][q];
                     if constexpr (TERMS > 1) z = ldexpf(z, e);
-                    float x = __builtin_amdgcn_exp2f((z - st.x) * LOG2E) * inv;
-                    if (hot == m) x -= scale;
-                    acc[i][j][q] = KIND != ONE16 ? as_rounded(x) : x;
+                    acc[i][j][q] = __builtin_amdgcn_exp2f((z - st.x) * LOG2E) * inv;
                 }
+            if (__any(hot >= 0 && hot < S::BM / S::WM)) {  // rare: a wave has 64 or 128 words
+                const int at = hot >= 0 && hot < S::BM / S::WM ? (int)hot : -1;
+#pragma unroll
+                for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        if (at == 16 * i + q) acc[i][j][q] -= scale;
+            }
+            if constexpr (KIND != ONE16) {
+#pragma unroll
+                for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) acc[i][j][q] = as_rounded(acc[i][j][q]);
+            }
             if (words < S::BM / S::WM || !__all(live)) {
                 const int left = live ? words - 4 * (lane >> 4) : 0;
 #pragma unroll
@@ -670,9 +681,9 @@ extern "C" size_t gdn_linear_loss_workspace_bytes(int64_t N, int64_t H, int64_t 
     const Sizes s = sizes(N, H, V, dtype, !copy, want_dx);
     const size_t bytes = need(s, want_dx, want_dw, bwd, copy, copy);
     if (bwd || !wide(nullptr, 0, N, H, dtype)) return bytes;
-    Space sp{nullptr};  // the forward call alone reads fp32 weights so, where they are aligned
+    Space sp{nullptr};  // what the forward call needs for an aligned weight; x alone may be what is not aligned
     place_wide(sp, s);
-    return bytes < sp.at ? sp.at : bytes;
+    return aligned || bytes < sp.at ? sp.at : bytes;
 }
 
 extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *targets, float *loss, float *stat, float *total,

@@ -1,9 +1,9 @@
 // The matrix product of the operators that are not bound by memory: C[n][m] = sum_k B[n][k] A[m][k] with 16-bit operands
-// that both lie along the contraction, 32-bit sums on the matrix cores, for gfx950.
+// that lie along the contraction, or one of them across it, 32-bit sums on the matrix cores, for gfx950.
 //
-// Operands in one order only: whoever has another order, type or an odd size lays its operand out in a pass of its own
-// (gdn_terms.h), which costs a percent or two of a large product and leaves one loop to make fast.  fp32 operands become
-// sums of 16-bit terms, side by side along the contraction; the product then walks pairs of terms ("segments").
+// Whoever has another type or an odd size lays its operand out in a pass of its own (gdn_terms.h), which costs a percent or two
+// of a large product and leaves one loop to make fast.  fp32 operands become sums of 16-bit terms, side by side along the
+// contraction; the product then walks pairs of terms ("segments").
 //
 // A workgroup forms a BM x BN tile, BK = 64 at a time: rows of 128 bytes go from memory to LDS without passing through
 // registers, two stages deep.  Chunk c of 16 bytes of row r lies in place c ^ (r / 2 & 7): sixteen rows of one chunk, which an
