@@ -365,8 +365,8 @@ int gdn_clip_grad_norm(const void *const *x, void *const *y, const int64_t *nume
  *
  * gdn_linear_loss_bwd: dx [N][H] and dw [V][H], contiguous (dtype; either may be NULL), from the cotangents dloss (fp32;
  * dloss_stride 1: one for each token, 0: one for all), times factor [0] (NULL for 1); dx is 0 at ignored tokens.
- * N <= 2^20, V <= 2^24, H <= 2^17.  The workspace of the forward pass: want_dx = want_dw = 0.  aligned: both operands lie on 16 bytes,
- * with rows a multiple of 16 bytes apart; without it there is room for copies of them. */
+ * N <= 2^20, V <= 2^24, H <= 2^17.  The workspace of the forward pass: want_dx = want_dw = 0.  aligned: both operands lie on
+ * 16 bytes, with rows a multiple of 16 bytes apart; without it there is room for copies of them. */
 size_t gdn_linear_loss_workspace_bytes(int64_t N, int64_t H, int64_t V, int dtype, int aligned, int want_dx, int want_dw);
 int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *targets, float *loss, float *stat, float *total,
                         float *factor, void *workspace, size_t workspace_bytes, int64_t N, int64_t H, int64_t V, int64_t x_stride,

@@ -6,8 +6,8 @@
 // every row of dW, zeros where no token points.  Without an order of arrival that could matter: no atomics.
 //
 // Sorting.  A token's key is its id above its place, so keys are unique and every key's place in the order is a count of
-// smaller keys.  Runs of 1024 keys are sorted by a workgroup each; then up to 32 runs at a time are joined by counting: a key's place is
-// the sum of its lower bounds in all of them, looked up by bisection.  32768 tokens take two launches, a million three.
+// smaller keys.  Runs of 1024 keys are sorted by a workgroup each; then up to 32 runs at a time are joined by counting: a key's
+// place is the sum of its lower bounds in all of them, looked up by bisection.  32768 tokens take two launches, a million three.
 //
 // Summing.  A word may have most of the tokens, so the sorted list is cut into chunks of 32.  A workgroup sums the
 // runs in its chunk: it writes the rows of words that begin and end there, and leaves what it has of the others, whose rows are
@@ -362,7 +362,8 @@ extern "C" int gdn_embedding_bwd(const int64_t *ids, const void *dy, void *dw, v
         hipLaunchKernelGGL(emb::run_kernel, grid_of((N + emb::RUN - 1) / emb::RUN), dim3(emb::RUN), 0, st, ids, keys, N, V,
                            padding_idx);
         for (int64_t run = emb::RUN; run < N; run *= emb::WAYS) {
-            hipLaunchKernelGGL(emb::join_kernel, grid_of((N * 8 + emb::NT - 1) / emb::NT), dim3(emb::NT), 0, st, keys, other, N, run);
+            hipLaunchKernelGGL(emb::join_kernel, grid_of((N * 8 + emb::NT - 1) / emb::NT), dim3(emb::NT), 0, st, keys, other, N,
+                               run);
             uint64_t *t = keys;
             keys = other;
             other = t;

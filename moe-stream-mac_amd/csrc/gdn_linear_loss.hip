@@ -488,7 +488,8 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
                             put16(lane, store, ii, jj, ops::pack2_cvt(y[0], y[1], DT), ops::pack2_cvt(y[2], y[3], DT));
                         }
                     uint16_t *to = KIND == ROWS ? a.p + (t * g.b.rows + n) * a.kp : a.p + n * (TERMS * a.kp) + t * a.kp;
-                    store_rows(lane, store, reinterpret_cast<char *>(to + m), (uint32_t)(TERMS * a.kp * 2), rows, (a.kp - m) * 2, 2);
+                    store_rows(lane, store, reinterpret_cast<char *>(to + m), (uint32_t)(TERMS * a.kp * 2), rows, (a.kp - m) * 2,
+                               2);
                 }
             }
         }
@@ -687,8 +688,9 @@ extern "C" size_t gdn_linear_loss_workspace_bytes(int64_t N, int64_t H, int64_t 
 }
 
 extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *targets, float *loss, float *stat, float *total,
-                                   float *factor, void *workspace, size_t workspace_bytes, int64_t N, int64_t H, int64_t V, int64_t x_stride,
-                                   int64_t w_stride, int64_t ignore_index, int reduction, int dtype, void *stream) {
+                                   float *factor, void *workspace, size_t workspace_bytes, int64_t N, int64_t H, int64_t V,
+                                   int64_t x_stride, int64_t w_stride, int64_t ignore_index, int reduction, int dtype,
+                                   void *stream) {
     clear_error();
     if (const int rc = check(N, H, V, x_stride, w_stride, dtype)) return rc;
     if (reduction < 0 || reduction > 2) return fail(GDN_ERR_INVALID, "unknown reduction");
@@ -887,7 +889,8 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
             h.b.rows = s.prows;
             h.live = tk.count;
             const Plan pl = s.px;  // parts without a block of the last piece add nothing
-            Result r{dx, H, dtype, b.power, exps, -SHIFT, {0, s.down ? 0 : -1}, nullptr, columns_of(H), v0 > 0, nullptr, tk.place};
+            Result r{dx, H, dtype, b.power, exps, -SHIFT, {0, s.down ? 0 : -1}, nullptr, columns_of(H), v0 > 0, nullptr,
+                     tk.place};
             if (h.across || s.compact || s.pieces > 1 || pl.splits > 1) r.acc = b.acc_x;
             multiply(h, !s.down || dtype == GDN_F16, pl, r, st);
             if (r.acc && v0 + words == V) finish(r, pl.splits * (int)(s.prows / N), N, H, st);  // terms are parts too

@@ -426,7 +426,8 @@ extern "C" int gdn_mxfp4_linear(const void *x, const void *codes, const void *sc
                                    s.kp);
             }
             g.a = Operand{b.w, s.kp * 2, rows, {0, 0, 0}, 0};
-            const Result r{static_cast<char *>(y) + n0 * elem, N, dtype, nullptr, nullptr, 0, {0, 0}, b.acc, columns_of(rows), 0, nullptr, nullptr};
+            const Result r{static_cast<char *>(y) + n0 * elem, N, dtype, nullptr, nullptr, 0, {0, 0}, b.acc, columns_of(rows), 0,
+                           nullptr, nullptr};
             multiply(g, false, s.plan, r, st);
             if (r.acc) finish(r, s.plan.splits, M, rows, st);
         }
@@ -456,7 +457,8 @@ extern "C" int gdn_mxfp4_linear_bwd(const void *dy, const void *codes, const voi
         const int64_t rows = N - n0 < s.piece ? N - n0 : s.piece, np = padded(rows), tiles_k = (K + 63) / 64;
         const int64_t tiles = np / 64 * tiles_k;
         Args g{};
-        operand(g, Source{static_cast<const char *>(dy) + n0 * elem, dtype, M, rows, dy_stride, nullptr, 0, nullptr, nullptr}, s, b.x, as_it_lies, st);
+        const Source part{static_cast<const char *>(dy) + n0 * elem, dtype, M, rows, dy_stride, nullptr, 0, nullptr, nullptr};
+        operand(g, part, s, b.x, as_it_lies, st);
         {
             Timed tm("mxfp4_across", st);
             hipLaunchKernelGGL(across_kernel, grid_of(tiles), dim3(NT), 0, st, static_cast<const uint32_t *>(codes) + n0 * blocks * 4,

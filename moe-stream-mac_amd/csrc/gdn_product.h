@@ -471,7 +471,8 @@ __device__ __forceinline__ void add_rows(int lane, char *st, const char *from, u
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
         const int r = t * 8 + (lane >> 3);
-        v[t] = r < rows && c * 16 < bytes ? *reinterpret_cast<const float4 *>(from + ((uint32_t)r * ld + (uint32_t)c * 16)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        v[t] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < rows && c * 16 < bytes) v[t] = *reinterpret_cast<const float4 *>(from + ((uint32_t)r * ld + (uint32_t)c * 16));
     }
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -487,7 +488,8 @@ __device__ __forceinline__ void put16(int lane, char *st, int ii, int jj, uint32
 }
 // The same of 2 x 2 tiles as fp32 numbers.
 __device__ __forceinline__ void put32(int lane, char *st, int ii, int jj, const float (&x)[4]) {
-    *reinterpret_cast<float4 *>(store_chunk(st, 16 * jj + (lane & 15), 4 * ii + (lane >> 4))) = make_float4(x[0], x[1], x[2], x[3]);
+    char *at = store_chunk(st, 16 * jj + (lane & 15), 4 * ii + (lane >> 4));
+    *reinterpret_cast<float4 *>(at) = make_float4(x[0], x[1], x[2], x[3]);
 }
 
 // Whether a product takes operands with this row pitch: offsets within a tile of 256 rows stay below 2^31.

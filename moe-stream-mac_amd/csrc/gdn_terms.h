@@ -30,8 +30,8 @@ inline int64_t padded(int64_t cols) { return (cols + 63) / 64 * 64; }
 // part[i][PARTS] = partial maxima of the finite magnitudes of s[i], i < 2, matrices of one type; without rows: zeros.
 void maxima(const Source (&s)[2], float *part, hipStream_t st);
 
-// exps[i] = the exponent e_i that takes the largest of part[i][PARTS] to [2^top, 2^(top + 1)), for i < 2, 0 for zeros; most[0] = the
-// largest of part[2][PARTS].  exps NULL: only that.
+// exps[i] = the exponent e_i that takes the largest of part[i][PARTS] to [2^top, 2^(top + 1)), for i < 2, 0 for zeros;
+// most[0] = the largest of part[2][PARTS].  exps NULL: only that.
 void exponents(const float *part, int top, int *exps, float *most, hipStream_t st);
 
 // dst[r][t * padded(cols) + c] = term t < slots of 2^e s[r][c], e = exps[which] (0 without exps), zeros behind the last column: x
