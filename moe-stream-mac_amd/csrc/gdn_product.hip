@@ -12,6 +12,7 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void product_kernel(const Args 
     const int w = wave_index(), wm = w / S::WN, wn = w % S::WN;
     char *st = lds + S::LDS + w * 4096;
     const Extent ext = extent_of<S>(g);
+    const int z = part_of(g).z;
     products<S, F16, DOWN>(g, ext, lds, [&](int tm, int tn, acc_t(&acc)[S::TM][S::TN]) {
         const int lane = lane_here();
         const int64_t m0 = (int64_t)tm * S::BM + wm * (S::BM / S::WM), n0 = (int64_t)tn * S::BN + wn * (S::BN / S::WN);
@@ -61,7 +62,7 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void product_kernel(const Args 
                         store_rows(lane, st, static_cast<char *>(r.y) + (n * r.ldy + m) * 4, (uint32_t)(r.ldy * 4), rows,
                                    (g.a.rows - m) * 4, 4);
                     } else {
-                        char *to = reinterpret_cast<char *>(r.acc + ((int64_t)blockIdx.z * g.b.rows + n) * r.ldp + m);
+                        char *to = reinterpret_cast<char *>(r.acc + ((int64_t)z * g.b.rows + n) * r.ldp + m);
                         if (r.add) add_rows(lane, st, to, (uint32_t)(r.ldp * 4), rows, (r.ldp - m) * 4);
                         store_rows(lane, st, to, (uint32_t)(r.ldp * 4), rows, (r.ldp - m) * 4, 4);
                     }
