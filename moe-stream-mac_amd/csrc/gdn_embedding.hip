@@ -12,7 +12,11 @@
 // Summing.  A word may have most of the tokens, so the sorted list is cut into chunks of 32.  A workgroup sums the
 // runs in its chunk: it writes the rows of words that begin and end there, and leaves what it has of the others, whose rows are
 // then the sums of what their chunks left; of long batches, groups of 64 chunks of one word are summed first.  Other workgroups
-// write the zeros of words without a token meanwhile.
+// write the zeros of words without a token meanwhile.  65536 tokens, two thirds of one word, 1024 bf16 channels: 202 us with the
+// groups, 283 without.
+//
+// Measured, 16384 tokens, 32000 x 2048 bf16: rows 26 us (5 TB/s with what the caches hold), the order 20, chunks and zeros 46, the
+// words over ends of chunks 7.
 #include "gdn_common.h"
 #include "gdn_host.h"
 #include "gdn_vec.h"

@@ -14,11 +14,13 @@
 //
 // Tokens that do not count (prompts, padding) are left out: from COMPACT tokens on, the others' hidden states are gathered into
 // the workspace, in their order, and every product forms the tiles of these alone.  How many there are only the device knows,
-// so launches are for all of them and workgroups without a token end at once.  Fewer tokens are taken as they lie: the
-// gathering, 20 us in all, would cost more than a few tokens less give.
+// so launches are for all of them and workgroups without a token end at once.  Fewer tokens are taken as they lie: 2048 of
+// 2048 channels, 32000 words and both gradients take 1034 us as they lie and 1051 gathered if all count, 1023 and 966 if a fifth does
+// not; 1024 take 614 and 636, 610 and 587.
 //
 // Precision.  Differences lie in [-1, 1] and have 11 bits as fp16 numbers times 2^15 (those below 2^-29 fewer); bf16 would
-// leave 8, as many as the results have, and make bf16 gradients up to 1.4 times as far from the exact ones.  W and x are fp16
+// leave 8, as many as the results have, and make bf16 gradients up to 1.4 times as far from the exact ones.  fp16 gradients, which
+// have 11 bits themselves, are so (2.9e-4 of the whole for 2.1e-4); a second term would double their products.  W and x are fp16
 // numbers times a power of two then (gdn_terms.hip), which holds bf16 numbers exactly.  Of a token's cotangent the differences
 // carry a factor of 0.75 to 1.5 and its sum for dx, or its x for dW, the power of two that is left, so that it costs no rounding
 // of its own.  With fp32 inputs every operand is two fp16 terms (2^-22) and every product three; a difference's second term is
@@ -27,7 +29,12 @@
 //
 // Few tokens (below DOWN) read the weight so often that its scaled copy, which lies along the words, costs more than the products:
 // dx is then formed from the weight as it lies (gdn_product.h), with fp16 weights by the differences as they are, with bf16 weights
-// by two bf16 terms of them (2^-17), rows of the same operand; dW by both terms and x.
+// by two bf16 terms of them (2^-17), rows of the same operand; dW by both terms and x.  2048 x 32000 bf16, forward and dx: 256
+// tokens 186 us so, 248 with a copy; 511 278 and 315; 1024 493 and 468.
+//
+// Measured, bf16, 8192 tokens of which a fifth does not count, 2048 x 32000, both gradients: 685 us for the statistics (1.25
+// PFLOP/s), then four pieces with 222 for the differences, 191 for dx and 167 for dW; the matrix units are busy 65, 46, 54 and 65 %
+// of the time.  Results and exponentials of a tile do not run beside another's products, which is what is lost most.
 #include "gdn_common.h"
 #include "gdn_host.h"
 #include "gdn_product.h"
@@ -174,8 +181,9 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void stat_kernel(const Args g, 
 // Few tokens and fp32 words, forward: read once, as they lie, and split in registers into three bf16 terms, which hold them exactly
 // and at any magnitude, so that they need no scale.  Six products of terms; those left out are below 2^-21 of the factors.  The
 // tokens' terms, 16 TN rows of three slots, go through LDS, two stages of 64 along the contraction; a wave's 32 words stay its own
-// and go to registers, a stage ahead.  64765 x 4096 weights (1.06 GB, 208 us at a copy's rate): 32 tokens 238 us, 118 tokens 489 us,
-// where the conversions and one wave to a SIMD hold it back; by way of two fp16 terms 878 and 920.
+// and go to registers, a stage ahead.  64765 x 4096 weights (1.06 GB, 208 us at a copy's rate): 32 tokens 229 us, 118 tokens 489 us,
+// where the conversions and one wave to a SIMD hold it back; by way of two fp16 terms 878 and 920.  128 tokens, 32000 x 2048: 124
+// and 267.
 template <int TN>
 struct Wide {
     static constexpr int NT = 256, BM = 128, BN = 16 * TN, TM = 2, SLOT = BN * BK * 2, STAGE = 3 * SLOT;

@@ -8,8 +8,11 @@
 // Every q 2^(s - 127) is a bf16 number, so products run on bf16 matrix instructions and lose nothing to the weight.  x keeps its
 // bits too: one bf16 term for bf16, two for fp16, three for fp32.
 //   y = x W^T:  up to 64 tokens read the 4-bit weight itself, which is what bounds them (step_kernel); more get a bf16 copy
-//   of the weight in the workspace first (gdn_product.h), 4.25 bits read and 16 written for 2 M products each.
+//   of the weight in the workspace first (gdn_product.h), 4.25 bits read and 16 written for 2 M products each.  8192 x 2048 bf16:
+//   16 tokens 16 us so and 33 with a copy, 32 20 and 32, 64 29 and 30.
 //   dx = dy W:  as the latter, with a copy that lies along N.
+// 8192 tokens through 2048 -> 8192 bf16, both ways: 418 us, of them 24 for the copies and 390 for the products.  One token: 5.4 us
+// of kernel for 8.9 MB, latency.
 #include "gdn_common.h"
 #include "gdn_host.h"
 #include "gdn_product.h"
