@@ -15,21 +15,21 @@
 // Tokens that do not count (prompts, padding) are left out: from COMPACT tokens on, the others' hidden states are gathered into
 // the workspace, in their order, and every product forms the tiles of these alone.  How many there are only the device knows,
 // so launches are for all of them and workgroups without a token end at once.  Fewer tokens are taken as they lie: 2048 of
-// 2048 channels, 32000 words and both gradients take 1034 us as they lie and 1051 gathered if all count, 1023 and 966 if a fifth does
-// not; 1024 take 614 and 636, 610 and 587.
+// 2048 channels, 32000 words and both gradients take 1034 us as they lie and 1051 gathered if all count, 1023 and 966 if a fifth
+// does not; 1024 take 614 and 636, 610 and 587.
 //
 // Precision.  Differences lie in [-1, 1] and have 11 bits as fp16 numbers times 2^15 (those below 2^-29 fewer); bf16 would
-// leave 8, as many as the results have, and make bf16 gradients up to 1.4 times as far from the exact ones.  fp16 gradients, which
-// have 11 bits themselves, are so (2.9e-4 of the whole for 2.1e-4); a second term would double their products.  W and x are fp16
-// numbers times a power of two then (gdn_terms.hip), which holds bf16 numbers exactly.  Of a token's cotangent the differences
-// carry a factor of 0.75 to 1.5 and its sum for dx, or its x for dW, the power of two that is left, so that it costs no rounding
-// of its own.  With fp32 inputs every operand is two fp16 terms (2^-22) and every product three; a difference's second term is
+// leave 8, as many as the results have, and make bf16 gradients up to 1.4 times as far from the exact ones.  With fp16 inputs,
+// whose results have 11 bits themselves, they are two terms, and the products that read them two (8192 x 2048 x 32000 4.5 ms, of
+// bf16 3.0): with one they were 1.4 times as far, 2.9e-4 of the whole.  W and x are fp16 numbers times a power of two then
+// (gdn_terms.hip), which holds bf16 numbers exactly.  Of a token's cotangent the differences carry a factor of 0.75 to 1.5 and
+// its sum for dx, or its x for dW, the power of two that is left, so that it costs no rounding of its own.  With fp32 inputs every operand is two fp16 terms (2^-22) and every product three; a difference's second term is
 // stored times 2^11, so that small probabilities keep their bits (2^-22 of them down to 2^-29, 2^-51 below; in one term 2^-11 and
 // 2^-40).
 //
 // Few tokens (below DOWN) read the weight so often that its scaled copy, which lies along the words, costs more than the products:
-// dx is then formed from the weight as it lies (gdn_product.h), with fp16 weights by the differences as they are, with bf16 weights
-// by two bf16 terms of them (2^-17), rows of the same operand; dW by both terms and x.  2048 x 32000 bf16, forward and dx: 256
+// dx is then formed from the weight as it lies (gdn_product.h), by two terms of the differences in its type (bf16: 2^-17), rows of
+// the same operand; dW by both terms and x.  2048 x 32000 bf16, forward and dx: 256
 // tokens 186 us so, 248 with a copy; 511 278 and 315; 1024 493 and 468.
 //
 // Measured, bf16, 8192 tokens of which a fifth does not count, 2048 x 32000, both gradients: 685 us for the statistics (1.25
@@ -402,8 +402,8 @@ struct DiffArgs {
     const float2 *stat;
     const float *power, *factor;  // cotangents
     const int *exps;  // with fp32 inputs: the logits' scale
-    uint16_t *p;      // [N][terms * kp], or [terms * N][kp]
-    int64_t v0, kp;
+    uint16_t *p;      // kp to a row and term: rows `row` apart, a second term `second` on
+    int64_t v0, kp, row, second;
 };
 
 // x as it was rounded: the compiler may round a product or sum to 16 bits at once in one place and in two steps in another, and
@@ -413,17 +413,19 @@ __device__ __forceinline__ float as_rounded(float x) {
     return x;
 }
 
-// What a term leaves of x, times 2^LOW: the next term.
+// What an fp16 term leaves of x, the next term, times 2^LOW where it is stored so.
+template <bool SCALED>
 __device__ __forceinline__ float left_of(float x) {
-    return (x - __half2float(__float2half(x))) * (float)(1 << LOW);
+    return (x - __half2float(__float2half(x))) * (SCALED ? (float)(1 << LOW) : 1.f);
 }
 
-enum : int { ONE16 = 1, TWO16 = 2, ROWS = 3 };  // differences: one fp16 term, two (fp32 inputs), two bf16 terms as rows
+enum : int { ONE16 = 1, TWO16 = 2, TWO = 3 };  // differences: one fp16 term, two (fp32 inputs), two of the inputs' type
 
 // The differences of a piece of words, 2^15 factor (p - [v = t]); zeros for tokens that do not count.
 template <class S, bool F16, int KIND>
 __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, const DiffArgs a) {
-    constexpr int TERMS = KIND == TWO16 ? 2 : 1;  // side by side
+    constexpr bool SCALED = KIND == TWO16;
+    constexpr int DT = KIND == TWO && !F16 ? DT_BF16 : DT_F16;
     __shared__ __attribute__((aligned(16))) char lds[S::LDS + S::STORE];
     const int w = wave_index(), wm = w / S::WN, wn = w % S::WN;
     char *store = lds + S::LDS + w * 4096;
@@ -432,7 +434,7 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
         const int lane = lane_here();
         const int64_t m0 = (int64_t)tm * S::BM + wm * (S::BM / S::WM), n0 = (int64_t)tn * S::BN + wn * (S::BN / S::WN);
         const int words = (int)min((int64_t)(S::BM / S::WM), g.a.rows - m0);  // of this wave's; may be negative
-        const int e = TERMS > 1 ? -(a.exps[E_X] + a.exps[E_W]) : 0;
+        const int e = SCALED ? -(a.exps[E_X] + a.exps[E_W]) : 0;
 #pragma unroll
         for (int j = 0; j < S::TN; ++j) {
             const int64_t n = n0 + 16 * j + (lane & 15);
@@ -446,7 +448,7 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     float z = acc[i][j][q];
-                    if constexpr (TERMS > 1) z = ldexpf(z, e);
+                    if constexpr (SCALED) z = ldexpf(z, e);
                     acc[i][j][q] = __builtin_amdgcn_exp2f((z - st.x) * LOG2E) * inv;
                 }
             if (__any(hot >= 0 && hot < S::BM / S::WM)) {  // rare: a wave has 64 or 128 words
@@ -487,17 +489,15 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
 #pragma unroll
                         for (int jj = 0; jj < 2; ++jj) {
                             float y[4];
-                            constexpr int DT = KIND == ROWS ? DT_BF16 : DT_F16;
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
                                 y[k] = acc[i + ii][j + jj][k];
-                                if (t) y[k] = KIND == ROWS ? y[k] - bf16_to_f32(f32_to_bf16_cvt(y[k])) : left_of(y[k]);
+                                if (t) y[k] = DT == DT_BF16 ? y[k] - bf16_to_f32(f32_to_bf16_cvt(y[k])) : left_of<SCALED>(y[k]);
                             }
                             put16(lane, store, ii, jj, ops::pack2_cvt(y[0], y[1], DT), ops::pack2_cvt(y[2], y[3], DT));
                         }
-                    uint16_t *to = KIND == ROWS ? a.p + (t * g.b.rows + n) * a.kp : a.p + n * (TERMS * a.kp) + t * a.kp;
-                    store_rows(lane, store, reinterpret_cast<char *>(to + m), (uint32_t)(TERMS * a.kp * 2), rows, (a.kp - m) * 2,
-                               2);
+                    uint16_t *to = a.p + n * a.row + t * a.second + m;
+                    store_rows(lane, store, reinterpret_cast<char *>(to), (uint32_t)(a.row * 2), rows, (a.kp - m) * 2, 2);
                 }
             }
         }
@@ -526,9 +526,12 @@ struct Sizes {
     bool compact;
     bool down;     // dx from the weight as it lies
     int wslots;    // terms of the weight's rows
-    bool rows;     // the differences are two bf16 terms, as rows
+    bool rows;     // the differences are two terms, as rows
+    bool bf;       // and bf16
     int64_t prows; // rows of the differences
+    int pterms;    // their terms side by side
     int slots;     // terms of the operands that meet them: the weight for dx, x for dW
+    int pairs;     // of terms, in the product for dW
     int64_t parts, tokens;  // parts of the words with statistics of their own; tokens at a time in the forward pass
     Plan px, pw;
 };
@@ -545,9 +548,12 @@ static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt, bool direct_w, bool 
     s.terms = dt == GDN_F32 ? 2 : 1;
     s.compact = N >= COMPACT;
     s.down = N < DOWN && direct_w;
-    s.rows = s.down && dx && dt == GDN_BF16;
+    s.rows = s.down && dx;
+    s.bf = s.rows && dt == GDN_BF16;
     s.prows = s.rows ? 2 * N : N;
+    s.pterms = s.rows || dt == GDN_BF16 ? 1 : 2;
     s.slots = s.terms == 1 ? 1 : 3;
+    s.pairs = s.terms > 1 ? 3 : s.rows ? 2 : s.pterms;
     s.wslots = s.terms > 1 && dx ? s.slots : s.terms;
     int64_t most = KEPT / s.np / 256 * 256;
     if (most < 256) most = 256;
@@ -559,8 +565,8 @@ static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt, bool direct_w, bool 
     if (s.tokens < 256) s.tokens = 256;
     if (s.tokens > N) s.tokens = N;
     const int64_t words = s.piece < V ? s.piece : V;
-    s.px = plan(s.prows, H, s.slots * padded(words) / BK, s.down ? 32 : 16);
-    s.pw = plan(words, H, (s.rows ? 2 : s.slots) * s.np / BK, 8, true);
+    s.px = plan(s.prows, H, (s.rows ? 1 : s.pairs) * padded(words) / BK, s.down ? 32 : 16);
+    s.pw = plan(words, H, s.pairs * s.np / BK, 8, true);
     return s;
 }
 
@@ -610,7 +616,7 @@ static Buffers place(Space &sp, const Sizes &s, bool dx, bool dw, bool bwd, bool
     }
     b.power = sp.take<float>(s.N);
     b.factor = sp.take<float>(s.N);
-    b.p = sp.take<uint16_t>(s.prows * t * padded(words));
+    b.p = sp.take<uint16_t>(s.prows * s.pterms * padded(words));
     if (dx) {
         if (!s.down && t == 1) b.wt = sp.take<uint16_t>(s.H * s.slots * padded(words));
         b.acc_x = sp.take<float>((int64_t)s.px.splits * s.prows * columns_of(s.H));
@@ -658,8 +664,8 @@ template <class S>
 static void launch_diff_of(Args &g, const DiffArgs &a, int dt, bool rows, hipStream_t st) {
     const dim3 grid = tiles_of<S>(g, 1), block(S::NT);
     if (dt == GDN_F32) hipLaunchKernelGGL((diff_kernel<S, true, TWO16>), grid, block, 0, st, g, a);
-    else if (dt == GDN_F16) hipLaunchKernelGGL((diff_kernel<S, true, ONE16>), grid, block, 0, st, g, a);
-    else if (rows) hipLaunchKernelGGL((diff_kernel<S, false, ROWS>), grid, block, 0, st, g, a);
+    else if (dt == GDN_F16) hipLaunchKernelGGL((diff_kernel<S, true, TWO>), grid, block, 0, st, g, a);
+    else if (rows) hipLaunchKernelGGL((diff_kernel<S, false, TWO>), grid, block, 0, st, g, a);
     else hipLaunchKernelGGL((diff_kernel<S, false, ONE16>), grid, block, 0, st, g, a);
 }
 
@@ -831,7 +837,7 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
                        b.power, b.factor, b.part + 2 * PARTS, tk.index, tk.count);
     // what is stored times a power of two: of fp32 inputs the forward call has found it
     const int *exps = t > 1 ? reinterpret_cast<const int *>(stat + 2 * N) : b.exps;
-    const bool scaled_x = t == 1 && dw && !s.rows, scaled_w = t == 1 && dx && !s.down;
+    const bool scaled_x = t == 1 && dw && !s.bf, scaled_w = t == 1 && dx && !s.down;
     if (scaled_x || scaled_w) {
         Source mx = sx, mw = sw;
         if (!scaled_x) mx.rows = 0;
@@ -840,7 +846,7 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
     }
     if (dw || scaled_w) exponents(b.part, TOP, scaled_x || scaled_w ? b.exps : nullptr, b.most, st);
     if (!direct_x) terms(sx, t, f16, t > 1 ? exps : nullptr, E_X, b.x, st);
-    if (dw) terms_across(sx, s.slots, !s.rows, s.rows ? nullptr : exps, E_X, Factors{b.power, b.most}, b.xt, st);
+    if (dw) terms_across(sx, s.slots, !s.bf, s.bf ? nullptr : exps, E_X, Factors{b.power, b.most}, b.xt, st);
     const int shape = plan(N, s.piece, s.slots * s.hp / BK, 1).shape;
     for (int64_t v0 = 0; v0 < V; v0 += s.piece) {
         const int64_t words = V - v0 < s.piece ? V - v0 : s.piece, kp = padded(words);
@@ -866,7 +872,8 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
             g.b.p = static_cast<const char *>(x);
             g.b.ld = x_stride * 2;
         }
-        const DiffArgs a{tt, reinterpret_cast<const float2 *>(stat), b.power, b.factor, exps, b.p, v0, kp};
+        const int64_t second = s.rows ? N * kp : kp;  // where there is one
+        const DiffArgs a{tt, reinterpret_cast<const float2 *>(stat), b.power, b.factor, exps, b.p, v0, kp, s.pterms * kp, second};
         {
             Timed tm("loss_diff", st);
 #define GDN_DIFF(S) launch_diff_of<S>(g, a, dtype, s.rows, st)
@@ -888,11 +895,11 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
                 }
             } else {
                 terms_across(part, 1, true, exps, E_W, Factors{nullptr, nullptr}, b.wt, st);
-                segments(h, 1, kp, 0);
+                segments(h, 1, kp, s.pterms > 1 ? kp * 2 : 0);
                 h.a.p = reinterpret_cast<const char *>(b.wt);
                 h.a.rows = H;
             }
-            h.b.ld = t * kp * 2;
+            h.b.ld = s.pterms * kp * 2;
             h.b.p = reinterpret_cast<const char *>(b.p);
             h.b.rows = s.prows;
             h.live = tk.count;
@@ -905,21 +912,21 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
         }
         if (dw) {
             Args h{};
-            segments(h, s.slots, s.np, s.rows ? N * kp * 2 : t > 1 ? kp * 2 : 0);
+            segments(h, s.slots, s.np, s.pairs > 1 ? second * 2 : 0);
             h.a.p = reinterpret_cast<const char *>(b.xt);
             h.a.rows = H;
             h.b.p = reinterpret_cast<const char *>(b.p);
-            h.b.ld = t * kp * 2;
+            h.b.ld = s.pterms * kp * 2;
             h.b.rows = words;
             h.b.width = kp * 2;
             h.across = DOWN_B;
             h.down = N;
             h.live = tk.count;
             h.live_k = 1;
-            Result r{static_cast<char *>(dw) + v0 * H * elem, H, dtype, nullptr, exps, -SHIFT, {s.rows ? 0 : -1, 0}, nullptr,
+            Result r{static_cast<char *>(dw) + v0 * H * elem, H, dtype, nullptr, exps, -SHIFT, {s.bf ? 0 : -1, 0}, nullptr,
                      columns_of(H), 0, b.most, nullptr};
             if (s.pw.splits > 1) r.acc = b.acc_w;
-            multiply(h, !s.rows, s.pw, r, st);
+            multiply(h, !s.bf, s.pw, r, st);
             if (r.acc) finish(r, s.pw.splits, words, H, st);
         }
     }
