@@ -23,9 +23,9 @@
 // whose results have 11 bits themselves, they are two terms, and the products that read them two (8192 x 2048 x 32000 4.5 ms, of
 // bf16 3.0): with one they were 1.4 times as far, 2.9e-4 of the whole.  W and x are fp16 numbers times a power of two then
 // (gdn_terms.hip), which holds bf16 numbers exactly.  Of a token's cotangent the differences carry a factor of 0.75 to 1.5 and
-// its sum for dx, or its x for dW, the power of two that is left, so that it costs no rounding of its own.  With fp32 inputs every operand is two fp16 terms (2^-22) and every product three; a difference's second term is
-// stored times 2^11, so that small probabilities keep their bits (2^-22 of them down to 2^-29, 2^-51 below; in one term 2^-11 and
-// 2^-40).
+// its sum for dx, or its x for dW, the power of two that is left, so that it costs no rounding of its own.  With fp32 inputs
+// every operand is two fp16 terms (2^-22) and every product three; a difference's second term is stored times 2^11, so that
+// small probabilities keep their bits (2^-22 of them down to 2^-29, 2^-51 below; in one term 2^-11 and 2^-40).
 //
 // Few tokens (below DOWN) read the weight so often that its scaled copy, which lies along the words, costs more than the products:
 // dx is then formed from the weight as it lies (gdn_product.h), by two terms of the differences in its type (bf16: 2^-17), rows of
