@@ -345,3 +345,22 @@ def test_few_fp32_scores_of_odd_values(dev):
     for odd in (-math.inf, math.nan, math.inf):  # no number of terms adds up to an infinity: it counts as NaN
         w[9, 5] = odd
         assert bool(torch.isnan(linear_cross_entropy(x, w, t, reduction="none")).all())
+
+
+@pytest.mark.parametrize("V,dtype", [(1_060_001, torch.bfloat16), (530_001, torch.float32)])
+def test_weights_beyond_32_bits(dev, V, dtype):
+    """A weight of more than 2^32 bytes, targets at both of its ends."""
+    from linear_loss import linear_cross_entropy
+    N, H = 8, 2048
+    print("large weight", V, dtype, flush=True)
+    x, w, t, d = inputs(dev, N, H, V, dtype, 13, ignored=False)
+    t[0], t[1], t[2] = V - 1, 0, -100
+    want, tol = plain(x, w, t, d)
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    loss = linear_cross_entropy(x, w, t, reduction="none")
+    dx, dw = torch.autograd.grad(loss, [x, w], d)
+    within(loss.detach(), want[0], tol[0], "loss")
+    within(dx, want[1], tol[1], "dx")
+    for rows in (slice(0, 2000), slice(V // 2, V // 2 + 2000), slice(V - 2000, V)):
+        within(dw[rows], want[2][rows], tol[2][rows], "dw")
