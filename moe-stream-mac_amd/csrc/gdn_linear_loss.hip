@@ -7,34 +7,36 @@
 //
 // Forward: one product whose tiles of logits end in registers, each as the maximum and the sum of exponentials of its words
 // per token; a second kernel joins them.  Backward: the words in pieces; of each piece the logits again (their normaliser is
-// known only after the last word), from them the differences p - [v = t] as 16-bit numbers, then two more products, which read
-// them along the words for dx and across for dW.  What is stored at any time is one piece of differences, at most 2^26 of them.
+// known only after the last word), from them the differences p - [v = t] as two 16-bit terms, then two more products, which read
+// them along the words for dx, with the weight's rows across, and across for dW.  What is stored at any time is one piece of
+// differences: 2^26 of them, or those of 256 words.
 //
 // Words lie along registers and tokens along lanes, so that maxima and sums run within a lane.
 //
 // Tokens that do not count (prompts, padding) are left out: from COMPACT tokens on, the others' hidden states are gathered into
 // the workspace, in their order, and every product forms the tiles of these alone.  How many there are only the device knows,
-// so launches are for all of them and workgroups without a token end at once.  Fewer tokens are taken as they lie: 2048 of
-// 2048 channels, 32000 words and both gradients take 1034 us as they lie and 1051 gathered if all count, 1023 and 966 if a fifth
-// does not; 1024 take 614 and 636, 610 and 587.
+// so launches are for all of them and workgroups without a token end at once.  Fewer tokens are taken as they lie: bf16, 2048
+// tokens of 2048 channels, 32000 words and both gradients take 1372 us as they lie and 1380 gathered if all count, 1345 and 1237 if a
+// fifth does not; 1024 take 804 and 811, 784 and 739; fp32, 2048 tokens 2968 and 2977, 2883 and 2716, 1024 1703 and 1707, 1663
+// and 1600.
 //
-// Precision.  Differences lie in [-1, 1] and have 11 bits as fp16 numbers times 2^15 (those below 2^-29 fewer); bf16 would
-// leave 8, as many as the results have, and make bf16 gradients up to 1.4 times as far from the exact ones.  With fp16 inputs,
-// whose results have 11 bits themselves, they are two terms, and the products that read them two (8192 x 2048 x 32000 4.5 ms, of
-// bf16 3.0): with one they were 1.4 times as far, 2.9e-4 of the whole.  W and x are fp16 numbers times a power of two then
-// (gdn_terms.hip), which holds bf16 numbers exactly.  Of a token's cotangent the differences carry a factor of 0.75 to 1.5 and
-// its sum for dx, or its x for dW, the power of two that is left, so that it costs no rounding of its own.  With fp32 inputs
-// every operand is two fp16 terms (2^-22) and every product three; a difference's second term is stored times 2^11, so that
-// small probabilities keep their bits (2^-22 of them down to 2^-29, 2^-51 below; in one term 2^-11 and 2^-40).
+// Precision.  bf16 differences are two bf16 terms, each off by half a step of what it rounds: 2^-16 of a difference of any size,
+// so that gradients lose nothing but their own rounding; x and W are their own operands.  (In one fp16 term, 11 bits that end at
+// 2^-40, training took 2960 us instead of 4280, gradients were 1.2e-3 of the whole away from those of 32-bit sums instead of 1.5e-4,
+// and the rows of dW of words that no token expects were coarse or zero.)  fp16: two fp16 terms of a difference times 2^15, 2^-22 of it or
+// 2^-40; what that leaves out is below fp16 results, which end at 2^-25, unless cotangents times x pass 2^15.  x is an fp16 number
+// times a power of two there for dW (gdn_terms.hip).  Of a token's cotangent the differences carry a factor of 0.75 to 1.5 and its sum
+// for dx, or its x for dW, the power of two that is left, so that it costs no rounding of its own.  With fp32 inputs every operand is
+// two fp16 terms (2^-22) and every product three; a difference's second term is stored times 2^11, so that small probabilities
+// keep their bits (2^-22 of them down to 2^-29, 2^-51 below).
 //
-// Few tokens (below DOWN) read the weight so often that its scaled copy, which lies along the words, costs more than the products:
-// dx is then formed from the weight as it lies (gdn_product.h), by two terms of the differences in its type (bf16: 2^-17), rows of
-// the same operand; dW by both terms and x.  2048 x 32000 bf16, forward and dx: 256
-// tokens 186 us so, 248 with a copy; 511 278 and 315; 1024 493 and 468.
+// Of few tokens (below ROWS) the differences' terms are rows of one operand for dx, so that the weight, which lies along the
+// channels, is read once.  2048 x 32000 bf16, forward and dx: 64 tokens 117 us so, 123 with terms side by side; 256 187 and 187; 511 272
+// and 276; 1024 497 and 498; 1500 771 and 711.
 //
-// Measured, bf16, 8192 tokens of which a fifth does not count, 2048 x 32000, both gradients: 685 us for the statistics (1.25
-// PFLOP/s), then four pieces with 222 for the differences, 191 for dx and 167 for dW; the matrix units are busy 65, 46, 54 and 65 %
-// of the time.  Results and exponentials of a tile do not run beside another's products, which is what is lost most.
+// Measured, bf16, 8192 tokens of which a fifth does not count, 2048 x 32000, both gradients: 686 us for the statistics (1.25
+// PFLOP/s), then four pieces with 247 for the differences, 381 for dx and 323 for dW (1.15 and 1.36 PFLOP/s over both terms).
+// Results and exponentials of a tile do not run beside another's products, which is what is lost most.
 #include "gdn_common.h"
 #include "gdn_host.h"
 #include "gdn_product.h"
@@ -49,11 +51,11 @@ using namespace mm;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int NT = 256;
 constexpr int64_t COMPACT = 2048;
-constexpr int64_t DOWN = 512;
-constexpr int64_t KEPT = 1 << 26;  // differences of a piece; statistics of the parts of the words
+constexpr int64_t ROWS = 512;
+constexpr int64_t KEPT = 1 << 26;  // differences of a piece, if that is 256 words or more; statistics of the parts of the words
 constexpr int64_t MOST_TOKENS = 1 << 20;  // three slots of 16 bits for each are a row pitch that a product takes
 constexpr int WIDE = 128;          // up to here an fp32 weight is read as it lies
-constexpr int SHIFT = 15;          // differences are stored times 2^15
+constexpr int SHIFT = 15;          // fp16 differences are stored times 2^15
 constexpr int TOP = 14;            // largest magnitudes of scaled operands: [2^14, 2^15)
 
 enum : int { E_X = 0, E_W = 1 };
@@ -419,13 +421,11 @@ __device__ __forceinline__ float left_of(float x) {
     return (x - __half2float(__float2half(x))) * (SCALED ? (float)(1 << LOW) : 1.f);
 }
 
-enum : int { ONE16 = 1, TWO16 = 2, TWO = 3 };  // differences: one fp16 term, two (fp32 inputs), two of the inputs' type
-
-// The differences of a piece of words, 2^15 factor (p - [v = t]); zeros for tokens that do not count.
-template <class S, bool F16, int KIND>
+// The differences of a piece of words, factor (p - [v = t]), fp16 ones times 2^SHIFT, in two terms; zeros for tokens that do not
+// count.  SCALED: of fp32 inputs, whose logits have a scale and whose second terms are stored times 2^LOW.
+template <class S, bool F16, bool SCALED>
 __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, const DiffArgs a) {
-    constexpr bool SCALED = KIND == TWO16;
-    constexpr int DT = KIND == TWO && !F16 ? DT_BF16 : DT_F16;
+    constexpr int DT = F16 ? DT_F16 : DT_BF16;
     __shared__ __attribute__((aligned(16))) char lds[S::LDS + S::STORE];
     const int w = wave_index(), wm = w / S::WN, wn = w % S::WN;
     char *store = lds + S::LDS + w * 4096;
@@ -441,7 +441,7 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
             const bool in = n < ext.rows_b;
             const float2 st = in ? a.stat[n] : make_float2(0.f, 0.f);
             const bool live = in && a.power[n] != 0.f;
-            const float scale = live ? a.factor[n] * (float)(1 << SHIFT) : 0.f, inv = st.y * scale;
+            const float scale = live ? a.factor[n] * (F16 ? (float)(1 << SHIFT) : 1.f) : 0.f, inv = st.y * scale;
             const int64_t hot = live ? a.targets[n] - a.v0 - m0 - 4 * (lane >> 4) : -1;
 #pragma unroll
             for (int i = 0; i < S::TM; ++i)
@@ -459,12 +459,10 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
                     for (int q = 0; q < 4; ++q)
                         if (at == 16 * i + q) acc[i][j][q] -= scale;
             }
-            if constexpr (KIND != ONE16) {
 #pragma unroll
-                for (int i = 0; i < S::TM; ++i)
+            for (int i = 0; i < S::TM; ++i)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) acc[i][j][q] = as_rounded(acc[i][j][q]);
-            }
+                for (int q = 0; q < 4; ++q) acc[i][j][q] = as_rounded(acc[i][j][q]);
             if (words < S::BM / S::WM || !__all(live)) {
                 const int left = live ? words - 4 * (lane >> 4) : 0;
 #pragma unroll
@@ -483,7 +481,7 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
                 const int64_t m = m0 + 16 * i;
                 if (m >= a.kp) break;
 #pragma unroll 1
-                for (int t = 0; t < (KIND == ONE16 ? 1 : 2); ++t) {
+                for (int t = 0; t < 2; ++t) {
 #pragma unroll
                     for (int ii = 0; ii < 4; ++ii)
 #pragma unroll
@@ -524,14 +522,12 @@ struct Sizes {
     int64_t N, H, V, hp, np, piece, pieces;  // hp, np: H and N in whole blocks; piece: words at a time
     int terms;
     bool compact;
-    bool down;     // dx from the weight as it lies
     int wslots;    // terms of the weight's rows
-    bool rows;     // the differences are two terms, as rows
-    bool bf;       // and bf16
+    bool rows;     // the differences' two terms are rows of one operand, else side by side
     int64_t prows; // rows of the differences
     int pterms;    // their terms side by side
     int slots;     // terms of the operands that meet them: the weight for dx, x for dW
-    int pairs;     // of terms, in the product for dW
+    int pairs;     // of terms, in these products
     int64_t parts, tokens;  // parts of the words with statistics of their own; tokens at a time in the forward pass
     Plan px, pw;
 };
@@ -547,13 +543,11 @@ static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt, bool direct_w, bool 
     s.np = padded(N);
     s.terms = dt == GDN_F32 ? 2 : 1;
     s.compact = N >= COMPACT;
-    s.down = N < DOWN && direct_w;
-    s.rows = s.down && dx;
-    s.bf = s.rows && dt == GDN_BF16;
+    s.rows = N < ROWS && direct_w && dx;
     s.prows = s.rows ? 2 * N : N;
-    s.pterms = s.rows || dt == GDN_BF16 ? 1 : 2;
+    s.pterms = s.rows ? 1 : 2;
     s.slots = s.terms == 1 ? 1 : 3;
-    s.pairs = s.terms > 1 ? 3 : s.rows ? 2 : s.pterms;
+    s.pairs = s.terms > 1 ? 3 : 2;
     s.wslots = s.terms > 1 && dx ? s.slots : s.terms;
     int64_t most = KEPT / s.np / 256 * 256;
     if (most < 256) most = 256;
@@ -565,7 +559,7 @@ static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt, bool direct_w, bool 
     if (s.tokens < 256) s.tokens = 256;
     if (s.tokens > N) s.tokens = N;
     const int64_t words = s.piece < V ? s.piece : V;
-    s.px = plan(s.prows, H, (s.rows ? 1 : s.pairs) * padded(words) / BK, s.down ? 32 : 16);
+    s.px = plan(s.prows, H, (s.rows ? 1 : s.pairs) * padded(words) / BK, s.rows ? 32 : 16);
     s.pw = plan(words, H, s.pairs * s.np / BK, 8, true);
     return s;
 }
@@ -587,7 +581,7 @@ struct Space {
 };
 
 struct Buffers {
-    uint16_t *x, *w, *wt, *xt, *p;
+    uint16_t *x, *w, *xt, *p;
     float *part, *zt, *power, *factor, *most, *acc_x, *acc_w;
     float2 *stats;
     int *exps;
@@ -617,10 +611,7 @@ static Buffers place(Space &sp, const Sizes &s, bool dx, bool dw, bool bwd, bool
     b.power = sp.take<float>(s.N);
     b.factor = sp.take<float>(s.N);
     b.p = sp.take<uint16_t>(s.prows * s.pterms * padded(words));
-    if (dx) {
-        if (!s.down && t == 1) b.wt = sp.take<uint16_t>(s.H * s.slots * padded(words));
-        b.acc_x = sp.take<float>((int64_t)s.px.splits * s.prows * columns_of(s.H));
-    }
+    if (dx) b.acc_x = sp.take<float>((int64_t)s.px.splits * s.prows * columns_of(s.H));
     if (dw) {
         b.xt = sp.take<uint16_t>(s.H * s.slots * s.np);
         if (s.pw.splits > 1) b.acc_w = sp.take<float>((int64_t)s.pw.splits * words * columns_of(s.H));
@@ -661,12 +652,11 @@ static void launch_stat_of(Args &g, const StatArgs &a, int dt, hipStream_t st) {
     else launch_stat<S, true>(g, a, dt == GDN_F32, st);
 }
 template <class S>
-static void launch_diff_of(Args &g, const DiffArgs &a, int dt, bool rows, hipStream_t st) {
+static void launch_diff_of(Args &g, const DiffArgs &a, int dt, hipStream_t st) {
     const dim3 grid = tiles_of<S>(g, 1), block(S::NT);
-    if (dt == GDN_F32) hipLaunchKernelGGL((diff_kernel<S, true, TWO16>), grid, block, 0, st, g, a);
-    else if (dt == GDN_F16) hipLaunchKernelGGL((diff_kernel<S, true, TWO>), grid, block, 0, st, g, a);
-    else if (rows) hipLaunchKernelGGL((diff_kernel<S, false, TWO>), grid, block, 0, st, g, a);
-    else hipLaunchKernelGGL((diff_kernel<S, false, ONE16>), grid, block, 0, st, g, a);
+    if (dt == GDN_F32) hipLaunchKernelGGL((diff_kernel<S, true, true>), grid, block, 0, st, g, a);
+    else if (dt == GDN_F16) hipLaunchKernelGGL((diff_kernel<S, true, false>), grid, block, 0, st, g, a);
+    else hipLaunchKernelGGL((diff_kernel<S, false, false>), grid, block, 0, st, g, a);
 }
 
 #define GDN_BY_SHAPE(shape, call)              \
@@ -826,8 +816,8 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
         return fail(GDN_ERR_WORKSPACE, "the workspace holds %zu bytes, %zu are needed", workspace_bytes, bytes);
     Space sp{static_cast<char *>(workspace)};
     const Buffers b = place(sp, s, dx, dw, true, !direct_x, !direct_w);
-    const bool f16 = dtype != GDN_BF16;
-    const int elem = dtype == GDN_F32 ? 4 : 2, t = s.terms;
+    const bool f16 = dtype != GDN_BF16;  // terms
+    const int elem = dtype == GDN_F32 ? 4 : 2, t = s.terms, shift = f16 ? -SHIFT : 0;
     const Tokens &tk = b.tokens;  // empty without
     const int64_t *tt = s.compact ? tk.target : targets;
     const Source sx{x, dtype, N, H, x_stride, s.compact ? nullptr : targets, ignore_index, tk.index, tk.count};
@@ -835,18 +825,17 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
     if (s.compact) hipLaunchKernelGGL(tokens_kernel, dim3(1), dim3(1024), 0, st, targets, N, ignore_index, tk, nullptr);
     hipLaunchKernelGGL(cotangent_kernel, dim3(PARTS), dim3(NT), 0, st, tt, dloss, dloss_stride, factor, N, V, ignore_index,
                        b.power, b.factor, b.part + 2 * PARTS, tk.index, tk.count);
-    // what is stored times a power of two: of fp32 inputs the forward call has found it
+    // what is stored times a power of two: fp32 inputs, for which the forward call has found it, and x across in fp16
     const int *exps = t > 1 ? reinterpret_cast<const int *>(stat + 2 * N) : b.exps;
-    const bool scaled_x = t == 1 && dw && !s.bf, scaled_w = t == 1 && dx && !s.down;
-    if (scaled_x || scaled_w) {
-        Source mx = sx, mw = sw;
-        if (!scaled_x) mx.rows = 0;
-        if (!scaled_w) mw.rows = 0;
-        maxima({mx, mw}, b.part, st);
+    const bool scaled_x = dtype == GDN_F16 && dw;
+    if (scaled_x) {
+        Source none = sw;
+        none.rows = 0;
+        maxima({sx, none}, b.part, st);
     }
-    if (dw || scaled_w) exponents(b.part, TOP, scaled_x || scaled_w ? b.exps : nullptr, b.most, st);
+    if (dw) exponents(b.part, TOP, scaled_x ? b.exps : nullptr, b.most, st);
     if (!direct_x) terms(sx, t, f16, t > 1 ? exps : nullptr, E_X, b.x, st);
-    if (dw) terms_across(sx, s.slots, !s.bf, s.bf ? nullptr : exps, E_X, Factors{b.power, b.most}, b.xt, st);
+    if (dw) terms_across(sx, s.slots, f16 ? exps : nullptr, E_X, Factors{b.power, b.most}, b.xt, st);
     const int shape = plan(N, s.piece, s.slots * s.hp / BK, 1).shape;
     for (int64_t v0 = 0; v0 < V; v0 += s.piece) {
         const int64_t words = V - v0 < s.piece ? V - v0 : s.piece, kp = padded(words);
@@ -872,47 +861,37 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
             g.b.p = static_cast<const char *>(x);
             g.b.ld = x_stride * 2;
         }
-        const int64_t second = s.rows ? N * kp : kp;  // where there is one
+        const int64_t second = s.rows ? N * kp : kp;
         const DiffArgs a{tt, reinterpret_cast<const float2 *>(stat), b.power, b.factor, exps, b.p, v0, kp, s.pterms * kp, second};
         {
             Timed tm("loss_diff", st);
-#define GDN_DIFF(S) launch_diff_of<S>(g, a, dtype, s.rows, st)
+#define GDN_DIFF(S) launch_diff_of<S>(g, a, dtype, st)
             GDN_BY_SHAPE(shape, GDN_DIFF)
 #undef GDN_DIFF
         }
         if (dx) {
             Args h{};
-            if (s.down || t > 1) {
-                h.kit = (int)(kp / BK);
-                h.nseg = s.slots;
-                h.across = DOWN_A;
-                h.down = words;
-                if (s.down) {
-                    h.a = Operand{static_cast<const char *>(part.p), w_stride * 2, H, {0, 0, 0}, H * 2};
-                } else {
-                    h.a = Operand{reinterpret_cast<const char *>(b.w), g.a.ld, H, {0, s.hp * 2, s.hp * 4}, s.hp * 2};
-                    h.b.off[2] = kp * 2;
-                }
-            } else {
-                terms_across(part, 1, true, exps, E_W, Factors{nullptr, nullptr}, b.wt, st);
-                segments(h, 1, kp, s.pterms > 1 ? kp * 2 : 0);
-                h.a.p = reinterpret_cast<const char *>(b.wt);
-                h.a.rows = H;
-            }
+            segments(h, s.slots, s.hp, s.rows ? 0 : kp * 2);
+            h.kit = (int)(kp / BK);
+            h.across = DOWN_A;
+            h.down = words;
+            h.a.p = g.a.p;
+            h.a.ld = g.a.ld;
+            h.a.rows = H;
+            h.a.width = (direct_w ? H : s.hp) * 2;
             h.b.ld = s.pterms * kp * 2;
             h.b.p = reinterpret_cast<const char *>(b.p);
             h.b.rows = s.prows;
             h.live = tk.count;
-            const Plan pl = s.px;  // parts without a block of the last piece add nothing
-            Result r{dx, H, dtype, b.power, exps, -SHIFT, {0, s.down ? 0 : -1}, nullptr, columns_of(H), v0 > 0, nullptr,
-                     tk.place};
-            if (h.across || s.compact || s.pieces > 1 || pl.splits > 1) r.acc = b.acc_x;
-            multiply(h, !s.down || dtype == GDN_F16, pl, r, st);
-            if (r.acc && v0 + words == V) finish(r, pl.splits * (int)(s.prows / N), N, H, st);  // terms are parts too
+            // parts without a block of the last piece add nothing
+            const Result r{dx, H, dtype, b.power, exps, shift, {0, t > 1 ? -1 : 0}, b.acc_x, columns_of(H), v0 > 0, nullptr,
+                           tk.place};
+            multiply(h, f16, s.px, r, st);
+            if (v0 + words == V) finish(r, s.px.splits * (int)(s.prows / N), N, H, st);  // terms as rows are parts too
         }
         if (dw) {
             Args h{};
-            segments(h, s.slots, s.np, s.pairs > 1 ? second * 2 : 0);
+            segments(h, s.slots, s.np, second * 2);
             h.a.p = reinterpret_cast<const char *>(b.xt);
             h.a.rows = H;
             h.b.p = reinterpret_cast<const char *>(b.p);
@@ -923,10 +902,10 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
             h.down = N;
             h.live = tk.count;
             h.live_k = 1;
-            Result r{static_cast<char *>(dw) + v0 * H * elem, H, dtype, nullptr, exps, -SHIFT, {s.bf ? 0 : -1, 0}, nullptr,
+            Result r{static_cast<char *>(dw) + v0 * H * elem, H, dtype, nullptr, exps, shift, {f16 ? -1 : 0, 0}, nullptr,
                      columns_of(H), 0, b.most, nullptr};
             if (s.pw.splits > 1) r.acc = b.acc_w;
-            multiply(h, !s.bf, s.pw, r, st);
+            multiply(h, f16, s.pw, r, st);
             if (r.acc) finish(r, s.pw.splits, words, H, st);
         }
     }

@@ -107,7 +107,7 @@ static void launch(Args &g, int splits, const Result &r, hipStream_t st) {
     const dim3 grid = tiles_of<S>(g, splits);
     if (r.acc) hipLaunchKernelGGL((product_kernel<S, F16, PARTS, DOWN>), grid, dim3(S::NT), 0, st, g, r);
     else if constexpr (DOWN != DOWN_A) {  // always in parts
-        if constexpr (F16 == (DOWN == DOWN_B)) {  // the others' callers have 16-bit results
+        if constexpr (F16 == (DOWN == DOWN_B)) {  // the other's callers have 16-bit results
             if (r.dt == DT_F32) {
                 hipLaunchKernelGGL((product_kernel<S, F16, OUT32, DOWN>), grid, dim3(S::NT), 0, st, g, r);
                 return;
@@ -130,8 +130,7 @@ static void launch(Args &g, bool f16, int splits, const Result &r, hipStream_t s
             return;
         }
     }
-    if (f16) launch<S, true, 0>(g, splits, r, st);
-    else launch<S, false, 0>(g, splits, r, st);
+    launch<S, false, 0>(g, splits, r, st);  // fp16 terms along the contraction only meet epilogues of their own
 }
 
 void multiply(Args g, bool f16, const Plan &p, const Result &r, hipStream_t st) {

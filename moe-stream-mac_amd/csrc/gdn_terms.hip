@@ -2,8 +2,7 @@
 //
 // A number of more bits than a 16-bit type holds is a sum of terms, each the rounding of what the earlier ones leave:
 // fp32 = 2 fp16 terms up to 2^-22 of it, or 3 bf16 terms.  fp16 has 5 bits of exponent, so a whole matrix is first
-// multiplied by the power of two that takes its largest magnitude to 2^14: a bf16 number (8 bits) is then exact down to
-// 2^-32 of the largest, and what is smaller is off by 2^-40 of it at most.
+// multiplied by the power of two that takes its largest magnitude to 2^14: a number is then off by 2^-39 of the largest at most.
 #include "gdn_common.h"
 #include "gdn_terms.h"
 #include "gdn_vec.h"
@@ -193,29 +192,32 @@ void exponents(const float *part, int top, int *exps, float *most, hipStream_t s
     hipLaunchKernelGGL(exponents_kernel, dim3(3), dim3(64), 0, st, part, top, exps, most);
 }
 
-#define GDN_TERMS_OF(KERNEL, F16, ...)                                                                                \
-    if (s.dt == DT_F32) hipLaunchKernelGGL((KERNEL<F16, DT_F32>), grid, dim3(NT), 0, st, __VA_ARGS__);                 \
-    else if (s.dt == DT_BF16) hipLaunchKernelGGL((KERNEL<F16, DT_BF16>), grid, dim3(NT), 0, st, __VA_ARGS__);          \
-    else hipLaunchKernelGGL((KERNEL<F16, DT_F16>), grid, dim3(NT), 0, st, __VA_ARGS__)
-#define GDN_TERMS(KERNEL, ...)                             \
-    if (f16) { GDN_TERMS_OF(KERNEL, true, __VA_ARGS__); }   \
-    else { GDN_TERMS_OF(KERNEL, false, __VA_ARGS__); }
+#define GDN_TERMS(KERNEL, F16, DT, ...) hipLaunchKernelGGL((KERNEL<F16, DT>), grid, dim3(NT), 0, st, __VA_ARGS__)
 
 void terms(const Source &s, int slots, bool f16, const int *exps, int which, void *dst, hipStream_t st) {
     Timed tm("terms", st);
     const int64_t kp = padded(s.cols);
     const dim3 grid = grid_of((s.rows * (kp / 8) + NT - 1) / NT);
-    GDN_TERMS(terms_kernel, s, slots, exps, which, static_cast<uint16_t *>(dst), kp);
+#define GDN_STRAIGHT(F16, DT) GDN_TERMS(terms_kernel, F16, DT, s, slots, exps, which, static_cast<uint16_t *>(dst), kp)
+    if (s.dt == DT_BF16) GDN_STRAIGHT(false, DT_BF16);  // never in fp16
+    else if (s.dt == DT_F16 && f16) GDN_STRAIGHT(true, DT_F16);
+    else if (s.dt == DT_F16) GDN_STRAIGHT(false, DT_F16);
+    else if (f16) GDN_STRAIGHT(true, DT_F32);
+    else GDN_STRAIGHT(false, DT_F32);
+#undef GDN_STRAIGHT
 }
 
-void terms_across(const Source &s, int slots, bool f16, const int *exps, int which, const Factors &f, void *dst, hipStream_t st) {
+void terms_across(const Source &s, int slots, const int *exps, int which, const Factors &f, void *dst, hipStream_t st) {
     Timed tm("terms_across", st);
     const int64_t kp = padded(s.rows), tc = (s.cols + 63) / 64, tiles = kp / 64 * tc;
     const dim3 grid = grid_of(tiles);
-    GDN_TERMS(across_kernel, s, slots, exps, which, f, static_cast<uint16_t *>(dst), kp, tc, tiles);
+#define GDN_ACROSS(F16, DT) GDN_TERMS(across_kernel, F16, DT, s, slots, exps, which, f, static_cast<uint16_t *>(dst), kp, tc, tiles)
+    if (s.dt == DT_BF16) GDN_ACROSS(false, DT_BF16);
+    else if (s.dt == DT_F16) GDN_ACROSS(true, DT_F16);
+    else GDN_ACROSS(true, DT_F32);
+#undef GDN_ACROSS
 }
 #undef GDN_TERMS
-#undef GDN_TERMS_OF
 
 }  // namespace mm
 }  // namespace gdn

@@ -92,9 +92,9 @@ def linear_cross_entropy(x: Array, weight: Array, targets: Array, *, ignore_inde
     ``weight``; a frozen weight costs no gradient of its own.  ``x`` and ``weight`` may be views with contiguous channels.
 
     Tokens that do not count cost no time where there are many (2048 and more in all).  Memory beside the gradients: 8 bytes for
-    each token and 64 words and a copy of ``x`` forward; backward up to 2^26 probabilities in 16 bits (twice, but for bfloat16
-    inputs), the piece of the weight that they belong to, and two copies of ``x`` with its gradient's sums.  float32 operands become sums of
-    16-bit terms, which hold no infinities: those may count as NaN."""
+    each token and 64 words and a copy of ``x`` forward; backward up to 2^26 probabilities, 32 bits each, the piece of the weight
+    that they belong to, and two copies of ``x`` with its gradient's sums.  float32 operands become sums of 16-bit terms, which hold
+    no infinities: those may count as NaN."""
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"x must be [..., H] and weight [V, H]; got {tuple(x.shape)} and {tuple(weight.shape)}")
     if tuple(targets.shape) != tuple(x.shape[:-1]):
