@@ -5,34 +5,36 @@
 //   dx_i = d_i sum_v (p_iv - [v = t_i]) W_v,    dW_v = sum_i d_i (p_iv - [v = t_i]) x_i
 // for the cotangents d_i of the losses.
 //
-// Forward: one product whose tiles of logits end in registers, each as the maximum and the sum of exponentials of its words
-// per token; a second kernel joins them.  Backward: the words in pieces; of each piece the logits again (their normaliser is
-// known only after the last word), from them the differences p - [v = t] as two 16-bit terms, then two more products, which read
-// them along the words for dx, with the weight's rows across, and across for dW.  What is stored at any time is one piece of
+// Forward: one product whose tiles of logits end in registers, each as the maximum and the sum of exponentials of its words per
+// token; a second kernel joins them.  Backward: the words in pieces; of each piece the logits again (their normaliser is known
+// only after the last word), from them the differences p - [v = t] as 16-bit terms, then two more products, which read them
+// along the words for dx, with the weight's rows across, and across for dW.  What is stored at any time is one piece of
 // differences: 2^26 of them, or those of 256 words.
 //
 // Words lie along registers and tokens along lanes, so that maxima and sums run within a lane.
 //
 // Tokens that do not count (prompts, padding) are left out: from COMPACT tokens on, the others' hidden states are gathered into
-// the workspace, in their order, and every product forms the tiles of these alone.  How many there are only the device knows,
-// so launches are for all of them and workgroups without a token end at once.  Fewer tokens are taken as they lie: bf16, 2048
-// tokens of 2048 channels, 32000 words and both gradients take 1372 us as they lie and 1380 gathered if all count, 1345 and 1237 if a
-// fifth does not; 1024 take 804 and 811, 784 and 739; fp32, 2048 tokens 2968 and 2977, 2883 and 2716, 1024 1703 and 1707, 1663
-// and 1600.
+// the workspace, in their order, and every product forms the tiles of these alone.  How many there are only the device knows, so
+// launches are for all of them and workgroups without a token end at once.  Fewer tokens are taken as they lie: bf16, 2048
+// tokens of 2048 channels, 32000 words and both gradients take 1372 us as they lie and 1380 gathered if all count, 1345 and 1237
+// if a fifth does not; 1024 take 804 and 811, 784 and 739; fp32, 2048 tokens 2968 and 2977, 2883 and 2716, 1024 1703 and 1707,
+// 1663 and 1600.
 //
 // Precision.  bf16 differences are two bf16 terms, each off by half a step of what it rounds: 2^-16 of a difference of any size,
 // so that gradients lose nothing but their own rounding; x and W are their own operands.  (In one fp16 term, 11 bits that end at
-// 2^-40, training took 2960 us instead of 4280, gradients were 1.2e-3 of the whole away from those of 32-bit sums instead of 1.5e-4,
-// and the rows of dW of words that no token expects were coarse or zero.)  fp16: two fp16 terms of a difference times 2^15, 2^-22 of it or
-// 2^-40; what that leaves out is below fp16 results, which end at 2^-25, unless cotangents times x pass 2^15.  x is an fp16 number
-// times a power of two there for dW (gdn_terms.hip).  Of a token's cotangent the differences carry a factor of 0.75 to 1.5 and its sum
-// for dx, or its x for dW, the power of two that is left, so that it costs no rounding of its own.  With fp32 inputs every operand is
-// two fp16 terms (2^-22) and every product three; a difference's second term is stored times 2^11, so that small probabilities
-// keep their bits (2^-22 of them down to 2^-29, 2^-51 below).
+// 2^-40, training took 2960 us instead of 4280, gradients were 1.2e-3 of the whole away from those of 32-bit sums instead of
+// 1.5e-4, and the rows of dW of words that no token expects were coarse or zero.)  fp16: two fp16 terms of a difference times
+// 2^15, 2^-22 of it or 2^-40; what that leaves out is below fp16 results, which end at 2^-25, unless cotangents times x pass
+// 2^15.  x is an fp16 number times a power of two there for dW (gdn_terms.hip).  Of a token's cotangent the differences carry a
+// factor of 0.75 to 1.5 and its sum for dx, or its x for dW, the power of two that is left, so that it costs no rounding of its
+// own.  fp32 operands are two fp16 terms under one power of two (2^-22 of a number, or 2^-39 of its matrix's largest) and every
+// product three pairs of them; a difference's second term is stored times 2^11, so that small probabilities keep their bits
+// (2^-22 of them down to 2^-29, 2^-51 below).  Up to WIDE fp32 tokens, forward and backward: three bf16 terms, which hold a
+// number of any magnitude as it is, and six pairs; those left out are below 2^-21 of the factors.
 //
 // Of few tokens (below ROWS) the differences' terms are rows of one operand for dx, so that the weight, which lies along the
-// channels, is read once.  2048 x 32000 bf16, forward and dx: 64 tokens 117 us so, 123 with terms side by side; 256 187 and 187; 511 272
-// and 276; 1024 497 and 498; 1500 771 and 711.
+// channels, is read once.  2048 x 32000 bf16, forward and dx: 64 tokens 117 us so, 123 with terms side by side; 256 187 and 187;
+// 511 272 and 276; 1024 497 and 498; 1500 771 and 711.
 //
 // Measured, bf16, 8192 tokens of which a fifth does not count, 2048 x 32000, both gradients: 686 us for the statistics (1.25
 // PFLOP/s), then four pieces with 247 for the differences, 381 for dx and 323 for dW (1.15 and 1.36 PFLOP/s over both terms).
@@ -54,7 +56,7 @@ constexpr int64_t COMPACT = 2048;
 constexpr int64_t ROWS = 512;
 constexpr int64_t KEPT = 1 << 26;  // differences of a piece, if that is 256 words or more; statistics of the parts of the words
 constexpr int64_t MOST_TOKENS = 1 << 20;  // three slots of 16 bits for each are a row pitch that a product takes
-constexpr int WIDE = 128;          // up to here an fp32 weight is read as it lies
+constexpr int WIDE = 128;          // up to here fp32 numbers are three bf16 terms, and a forward call reads the words as they lie
 constexpr int SHIFT = 15;          // fp16 differences are stored times 2^15
 constexpr int TOP = 14;            // largest magnitudes of scaled operands: [2^14, 2^15)
 
@@ -403,8 +405,8 @@ struct DiffArgs {
     const int64_t *targets;
     const float2 *stat;
     const float *power, *factor;  // cotangents
-    const int *exps;  // with fp32 inputs: the logits' scale
-    uint16_t *p;      // kp to a row and term: rows `row` apart, a second term `second` on
+    const int *exps;  // SCALED: the logits' scale
+    uint16_t *p;      // kp to a row and term: rows `row` apart, a next term `second` on
     int64_t v0, kp, row, second;
 };
 
@@ -415,15 +417,16 @@ __device__ __forceinline__ float as_rounded(float x) {
     return x;
 }
 
-// What an fp16 term leaves of x, the next term, times 2^LOW where it is stored so.
-template <bool SCALED>
+// What a term leaves of x: the next term, times 2^LOW where it is stored so.
+template <bool F16, bool SCALED>
 __device__ __forceinline__ float left_of(float x) {
-    return (x - __half2float(__float2half(x))) * (SCALED ? (float)(1 << LOW) : 1.f);
+    if constexpr (F16) return (x - __half2float(__float2half(x))) * (SCALED ? (float)(1 << LOW) : 1.f);
+    return x - bf16_to_f32(f32_to_bf16_cvt(x));
 }
 
-// The differences of a piece of words, factor (p - [v = t]), fp16 ones times 2^SHIFT, in two terms; zeros for tokens that do not
-// count.  SCALED: of fp32 inputs, whose logits have a scale and whose second terms are stored times 2^LOW.
-template <class S, bool F16, bool SCALED>
+// The differences of a piece of words, factor (p - [v = t]), fp16 ones times 2^SHIFT, in TERMS terms; zeros for tokens that do not
+// count.  SCALED: the logits have a scale, and second terms are stored times 2^LOW.
+template <class S, bool F16, bool SCALED, int TERMS>
 __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, const DiffArgs a) {
     constexpr int DT = F16 ? DT_F16 : DT_BF16;
     __shared__ __attribute__((aligned(16))) char lds[S::LDS + S::STORE];
@@ -481,7 +484,7 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
                 const int64_t m = m0 + 16 * i;
                 if (m >= a.kp) break;
 #pragma unroll 1
-                for (int t = 0; t < 2; ++t) {
+                for (int t = 0; t < TERMS; ++t) {
 #pragma unroll
                     for (int ii = 0; ii < 4; ++ii)
 #pragma unroll
@@ -490,7 +493,8 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
 #pragma unroll
                             for (int k = 0; k < 4; ++k) {
                                 y[k] = acc[i + ii][j + jj][k];
-                                if (t) y[k] = DT == DT_BF16 ? y[k] - bf16_to_f32(f32_to_bf16_cvt(y[k])) : left_of<SCALED>(y[k]);
+                                if (t > 0) y[k] = left_of<F16, SCALED>(y[k]);
+                                if (TERMS > 2 && t > 1) y[k] = left_of<F16, SCALED>(y[k]);
                             }
                             put16(lane, store, ii, jj, ops::pack2_cvt(y[0], y[1], DT), ops::pack2_cvt(y[2], y[3], DT));
                         }
@@ -504,33 +508,42 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
 
 // ------------------------------------------------------------------------------------------------ host
 
-// The segments of a product of operands with `slots` terms for a, kp elements each, and one or two terms for b, the second
-// `second` bytes on (0: one): all pairs of terms but the least.  Three slots are those of terms_across, of which the third meets
-// b's second term, stored times 2^LOW.
-static void segments(Args &g, int slots, int64_t kp, int64_t second) {
-    g.kit = (int)(kp / BK);
-    g.nseg = 1;
-    g.a.ld = slots * kp * 2;
-    if (slots > 1) g.a.off[g.nseg++] = kp * 2;
-    if (second) {
-        g.a.off[g.nseg] = slots == 3 ? 2 * kp * 2 : 0;
-        g.b.off[g.nseg++] = second;
-    }
-}
-
 struct Sizes {
     int64_t N, H, V, hp, np, piece, pieces;  // hp, np: H and N in whole blocks; piece: words at a time
-    int terms;
+    bool f16, scaled;  // terms are fp16; and of operands times a power of two
+    int terms;         // of an operand
     bool compact;
     int wslots;    // terms of the weight's rows
     bool rows;     // the differences' two terms are rows of one operand, else side by side
     int64_t prows; // rows of the differences
     int pterms;    // their terms side by side
-    int slots;     // terms of the operands that meet them: the weight for dx, x for dW
+    int slots;     // terms of the operands that meet them, as they are laid out: the weight for dx, x for dW
     int pairs;     // of terms, in these products
     int64_t parts, tokens;  // parts of the words with statistics of their own; tokens at a time in the forward pass
     Plan px, pw;
 };
+
+// The segments of a product over kp elements: a's terms `first` elements apart, b's `second`.
+//   one term of a, two of b:  both pairs
+//   two terms (fp16):         all pairs but that of the second ones.  a has three slots in the backward pass, as terms() makes them;
+//                             the third meets b's second term, stored times 2^LOW
+//   three terms (bf16):       all pairs but those below 2^-16 of the first, the smallest first
+static void segments(Args &g, const Sizes &s, bool back, int64_t kp, int64_t first, int64_t second) {
+    const auto pair = [&](int i, int j) {
+        g.a.off[g.nseg] = i * first * 2;
+        g.b.off[g.nseg++] = j * second * 2;
+    };
+    g.kit = (int)(kp / BK);
+    g.nseg = 0;
+    if (s.terms == 3)
+        for (int i = 2; i >= 0; --i)
+            for (int k = i; k >= 0; --k) pair(k, i - k);
+    else {
+        pair(0, 0);
+        if (s.terms == 2) pair(1, 0);
+        if (s.terms == 2 || back) pair(back && s.terms == 2 ? 2 : 0, 1);
+    }
+}
 
 static bool direct(const void *p, int64_t ld, int64_t H, int dt) {
     return dt != GDN_F32 && H % BK == 0 && ld % 8 == 0 && aligned_to(p, 16) && pitch_fits(ld * 2);
@@ -541,13 +554,16 @@ static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt, bool direct_w, bool 
     s.N = N; s.H = H; s.V = V;
     s.hp = padded(H);
     s.np = padded(N);
-    s.terms = dt == GDN_F32 ? 2 : 1;
+    const bool any = dt == GDN_F32 && N <= WIDE;  // three bf16 terms hold numbers of any magnitude
+    s.terms = any ? 3 : dt == GDN_F32 ? 2 : 1;
+    s.scaled = s.terms == 2;
+    s.f16 = s.scaled || dt == GDN_F16;
     s.compact = N >= COMPACT;
-    s.rows = N < ROWS && direct_w && dx;
+    s.rows = N < ROWS && direct_w && dx;  // 16-bit weights only
     s.prows = s.rows ? 2 * N : N;
-    s.pterms = s.rows ? 1 : 2;
+    s.pterms = s.rows ? 1 : any ? 3 : 2;
     s.slots = s.terms == 1 ? 1 : 3;
-    s.pairs = s.terms > 1 ? 3 : 2;
+    s.pairs = any ? 6 : s.scaled ? 3 : 2;
     s.wslots = s.terms > 1 && dx ? s.slots : s.terms;
     int64_t most = KEPT / s.np / 256 * 256;
     if (most < 256) most = 256;
@@ -621,8 +637,6 @@ static Buffers place(Space &sp, const Sizes &s, bool dx, bool dw, bool bwd, bool
 
 static Buffers place_wide(Space &sp, const Sizes &s) {
     Buffers b{};
-    b.most = sp.take<float>(1);
-    b.part = sp.take<float>(3 * PARTS);
     b.x = sp.take<uint16_t>(s.N * 3 * s.hp);
     b.stats = sp.take<float2>((s.V + 127) / 128 * 4 * s.N);
     b.zt = sp.take<float>(s.N);
@@ -638,25 +652,20 @@ static int check(int64_t N, int64_t H, int64_t V, int64_t x_ld, int64_t w_ld, in
     return GDN_OK;
 }
 
-template <class S, bool F16>
-static void launch_stat(Args &g, const StatArgs &a, bool scaled, hipStream_t st) {
-    const dim3 grid = tiles_of<S>(g, 1);
-    if (scaled) hipLaunchKernelGGL((stat_kernel<S, F16, true>), grid, dim3(S::NT), 0, st, g, a);
-    else hipLaunchKernelGGL((stat_kernel<S, F16, false>), grid, dim3(S::NT), 0, st, g, a);
-}
-
-// 16-bit inputs as they are, fp32 inputs as two fp16 terms.
 template <class S>
-static void launch_stat_of(Args &g, const StatArgs &a, int dt, hipStream_t st) {
-    if (dt == GDN_BF16) launch_stat<S, false>(g, a, false, st);
-    else launch_stat<S, true>(g, a, dt == GDN_F32, st);
-}
-template <class S>
-static void launch_diff_of(Args &g, const DiffArgs &a, int dt, hipStream_t st) {
+static void launch_stat(Args &g, const StatArgs &a, const Sizes &s, hipStream_t st) {
     const dim3 grid = tiles_of<S>(g, 1), block(S::NT);
-    if (dt == GDN_F32) hipLaunchKernelGGL((diff_kernel<S, true, true>), grid, block, 0, st, g, a);
-    else if (dt == GDN_F16) hipLaunchKernelGGL((diff_kernel<S, true, false>), grid, block, 0, st, g, a);
-    else hipLaunchKernelGGL((diff_kernel<S, false, false>), grid, block, 0, st, g, a);
+    if (s.scaled) hipLaunchKernelGGL((stat_kernel<S, true, true>), grid, block, 0, st, g, a);
+    else if (s.f16) hipLaunchKernelGGL((stat_kernel<S, true, false>), grid, block, 0, st, g, a);
+    else hipLaunchKernelGGL((stat_kernel<S, false, false>), grid, block, 0, st, g, a);
+}
+template <class S>
+static void launch_diff(Args &g, const DiffArgs &a, const Sizes &s, hipStream_t st) {
+    const dim3 grid = tiles_of<S>(g, 1), block(S::NT);
+    if (s.scaled) hipLaunchKernelGGL((diff_kernel<S, true, true, 2>), grid, block, 0, st, g, a);
+    else if (s.f16) hipLaunchKernelGGL((diff_kernel<S, true, false, 2>), grid, block, 0, st, g, a);
+    else if (s.terms == 1) hipLaunchKernelGGL((diff_kernel<S, false, false, 2>), grid, block, 0, st, g, a);
+    else hipLaunchKernelGGL((diff_kernel<S, false, false, 3>), grid, block, 0, st, g, a);
 }
 
 #define GDN_BY_SHAPE(shape, call)              \
@@ -713,7 +722,6 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
         if (workspace_bytes < size.at)
             return fail(GDN_ERR_WORKSPACE, "the workspace holds %zu bytes, %zu are needed", workspace_bytes, size.at);
         const Buffers b = few ? place_wide(sp, s) : place(sp, s, false, false, false, !dx, !dw);
-        const bool f16 = dtype != GDN_BF16;
         const int *exps = nullptr;
         const Tokens &tk = b.tokens;  // empty without
         const int64_t *tt = s.compact ? tk.target : targets;
@@ -721,14 +729,14 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
         const Source sw{w, dtype, V, H, w_stride, nullptr, 0, nullptr, nullptr};
         if (s.compact)
             hipLaunchKernelGGL(tokens_kernel, dim3(1), dim3(1024), 0, st, targets, N, ignore_index, tk, loss);
-        if (dtype == GDN_F32 && (stat || !few)) {
+        if (s.scaled) {
             maxima({sx, sw}, b.part, st);
             int *to = stat ? reinterpret_cast<int *>(stat + 2 * N) : b.exps;
             exponents(b.part, TOP, to, b.most, st);  // b.most is not read
             exps = to;
         }
         if (few) terms(sx, 3, false, nullptr, E_X, b.x, st);
-        else if (!dx) terms(sx, s.terms, f16, exps, E_X, b.x, st);
+        else if (!dx) terms(sx, s.terms, s.f16, exps, E_X, b.x, st);
         // operands that are used as they lie need no pieces
         const int64_t step = dw ? V : s.piece;
         for (int64_t n0 = 0; n0 < N; n0 += s.tokens) {
@@ -749,8 +757,8 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
             for (int64_t v0 = 0; v0 < V && !few; v0 += step) {
                 const int64_t words = V - v0 < step ? V - v0 : step;
                 Args g{};
-                segments(g, s.terms, s.hp, s.terms > 1 ? s.hp * 2 : 0);
-                g.b.ld = s.terms * s.hp * 2;
+                segments(g, s, false, s.hp, s.hp, s.hp);
+                g.a.ld = g.b.ld = s.terms * s.hp * 2;
                 g.a.rows = words;
                 g.b.rows = tokens;
                 g.live = tk.count;
@@ -764,7 +772,7 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
                     Source part = sw;
                     part.p = static_cast<const char *>(w) + v0 * w_stride * (dtype == GDN_F32 ? 4 : 2);
                     part.rows = words;
-                    terms(part, s.terms, f16, exps, E_W, b.w, st);
+                    terms(part, s.terms, s.f16, exps, E_W, b.w, st);
                 }
                 if (dx) {
                     g.b.p = static_cast<const char *>(x) + n0 * x_stride * 2;
@@ -773,7 +781,7 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
                 const StatArgs a{tt + n0, b.stats, b.zt, exps, tokens, V, v0, parts};
                 Timed tm("loss_stat", st);
 #define GDN_STAT(S)                                \
-    launch_stat_of<S>(g, a, dtype, st);            \
+    launch_stat<S>(g, a, s, st);                   \
     parts += g.mt * S::WM
                 GDN_BY_SHAPE(shape, GDN_STAT)
 #undef GDN_STAT
@@ -816,8 +824,7 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
         return fail(GDN_ERR_WORKSPACE, "the workspace holds %zu bytes, %zu are needed", workspace_bytes, bytes);
     Space sp{static_cast<char *>(workspace)};
     const Buffers b = place(sp, s, dx, dw, true, !direct_x, !direct_w);
-    const bool f16 = dtype != GDN_BF16;  // terms
-    const int elem = dtype == GDN_F32 ? 4 : 2, t = s.terms, shift = f16 ? -SHIFT : 0;
+    const int elem = dtype == GDN_F32 ? 4 : 2, t = s.terms, shift = s.f16 ? -SHIFT : 0;
     const Tokens &tk = b.tokens;  // empty without
     const int64_t *tt = s.compact ? tk.target : targets;
     const Source sx{x, dtype, N, H, x_stride, s.compact ? nullptr : targets, ignore_index, tk.index, tk.count};
@@ -825,8 +832,8 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
     if (s.compact) hipLaunchKernelGGL(tokens_kernel, dim3(1), dim3(1024), 0, st, targets, N, ignore_index, tk, nullptr);
     hipLaunchKernelGGL(cotangent_kernel, dim3(PARTS), dim3(NT), 0, st, tt, dloss, dloss_stride, factor, N, V, ignore_index,
                        b.power, b.factor, b.part + 2 * PARTS, tk.index, tk.count);
-    // what is stored times a power of two: fp32 inputs, for which the forward call has found it, and x across in fp16
-    const int *exps = t > 1 ? reinterpret_cast<const int *>(stat + 2 * N) : b.exps;
+    // what is stored times a power of two: both operands, for which the forward call has found it, or x across in fp16
+    const int *exps = s.scaled ? reinterpret_cast<const int *>(stat + 2 * N) : b.exps;
     const bool scaled_x = dtype == GDN_F16 && dw;
     if (scaled_x) {
         Source none = sw;
@@ -834,8 +841,8 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
         maxima({sx, none}, b.part, st);
     }
     if (dw) exponents(b.part, TOP, scaled_x ? b.exps : nullptr, b.most, st);
-    if (!direct_x) terms(sx, t, f16, t > 1 ? exps : nullptr, E_X, b.x, st);
-    if (dw) terms_across(sx, s.slots, f16 ? exps : nullptr, E_X, Factors{b.power, b.most}, b.xt, st);
+    if (!direct_x) terms(sx, t, s.f16, s.scaled ? exps : nullptr, E_X, b.x, st);
+    if (dw) terms_across(sx, s.slots, s.f16, s.f16 ? exps : nullptr, E_X, Factors{b.power, b.most}, b.xt, st);
     const int shape = plan(N, s.piece, s.slots * s.hp / BK, 1).shape;
     for (int64_t v0 = 0; v0 < V; v0 += s.piece) {
         const int64_t words = V - v0 < s.piece ? V - v0 : s.piece, kp = padded(words);
@@ -843,7 +850,7 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
         part.p = static_cast<const char *>(w) + v0 * w_stride * elem;
         part.rows = words;
         Args g{};
-        segments(g, t, s.hp, t > 1 ? s.hp * 2 : 0);
+        segments(g, s, false, s.hp, s.hp, s.hp);
         g.b.ld = t * s.hp * 2;
         g.a.rows = words;
         g.b.rows = N;
@@ -855,7 +862,7 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
             g.a.ld = w_stride * 2;
         } else {
             g.a.ld = s.wslots * s.hp * 2;
-            terms(part, s.wslots, f16, t > 1 ? exps : nullptr, E_W, b.w, st);
+            terms(part, s.wslots, s.f16, s.scaled ? exps : nullptr, E_W, b.w, st);
         }
         if (direct_x) {
             g.b.p = static_cast<const char *>(x);
@@ -865,14 +872,13 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
         const DiffArgs a{tt, reinterpret_cast<const float2 *>(stat), b.power, b.factor, exps, b.p, v0, kp, s.pterms * kp, second};
         {
             Timed tm("loss_diff", st);
-#define GDN_DIFF(S) launch_diff_of<S>(g, a, dtype, st)
+#define GDN_DIFF(S) launch_diff<S>(g, a, s, st)
             GDN_BY_SHAPE(shape, GDN_DIFF)
 #undef GDN_DIFF
         }
         if (dx) {
             Args h{};
-            segments(h, s.slots, s.hp, s.rows ? 0 : kp * 2);
-            h.kit = (int)(kp / BK);
+            segments(h, s, !s.rows, kp, s.hp, kp);
             h.across = DOWN_A;
             h.down = words;
             h.a.p = g.a.p;
@@ -884,15 +890,16 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
             h.b.rows = s.prows;
             h.live = tk.count;
             // parts without a block of the last piece add nothing
-            const Result r{dx, H, dtype, b.power, exps, shift, {0, t > 1 ? -1 : 0}, b.acc_x, columns_of(H), v0 > 0, nullptr,
+            const Result r{dx, H, dtype, b.power, exps, shift, {0, s.scaled ? -1 : 0}, b.acc_x, columns_of(H), v0 > 0, nullptr,
                            tk.place};
-            multiply(h, f16, s.px, r, st);
+            multiply(h, s.f16, s.px, r, st);
             if (v0 + words == V) finish(r, s.px.splits * (int)(s.prows / N), N, H, st);  // terms as rows are parts too
         }
         if (dw) {
             Args h{};
-            segments(h, s.slots, s.np, second * 2);
+            segments(h, s, true, s.np, s.np, second);
             h.a.p = reinterpret_cast<const char *>(b.xt);
+            h.a.ld = s.slots * s.np * 2;
             h.a.rows = H;
             h.b.p = reinterpret_cast<const char *>(b.p);
             h.b.ld = s.pterms * kp * 2;
@@ -902,10 +909,10 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
             h.down = N;
             h.live = tk.count;
             h.live_k = 1;
-            Result r{static_cast<char *>(dw) + v0 * H * elem, H, dtype, nullptr, exps, shift, {f16 ? -1 : 0, 0}, nullptr,
+            Result r{static_cast<char *>(dw) + v0 * H * elem, H, dtype, nullptr, exps, shift, {s.f16 ? -1 : 0, 0}, nullptr,
                      columns_of(H), 0, b.most, nullptr};
             if (s.pw.splits > 1) r.acc = b.acc_w;
-            multiply(h, f16, s.pw, r, st);
+            multiply(h, s.f16, s.pw, r, st);
             if (r.acc) finish(r, s.pw.splits, words, H, st);
         }
     }

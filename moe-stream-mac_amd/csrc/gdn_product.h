@@ -44,17 +44,18 @@ __device__ __forceinline__ acc_t mfma(u4 a, u4 b, acc_t c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
 }
 
+constexpr int PAIRS = 6;  // of terms, at most
 // A matrix of `rows` rows, `ld` bytes apart, of `off[s]` bytes to the term that segment s takes.
 struct Operand {
     const char *p;
     int64_t ld, rows;
-    int64_t off[3];
+    int64_t off[PAIRS];
     int64_t width;  // across the contraction: bytes of a row that may be read, a multiple of 16
 };
 struct Args {
     Operand a, b;
     int kit;     // BK-blocks of a term
-    int nseg;    // 1 to 3
+    int nseg;    // 1 to PAIRS
     int splits;  // the nseg * kit blocks in this many parts (grid.z)
     int mt, nt;  // tiles
     // Sizes that only the device knows: `live` tokens count, of which these are those from live0 on.  They are b's rows, or with

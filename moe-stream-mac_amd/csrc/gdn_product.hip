@@ -107,13 +107,8 @@ static void launch(Args &g, int splits, const Result &r, hipStream_t st) {
     const dim3 grid = tiles_of<S>(g, splits);
     if (r.acc) hipLaunchKernelGGL((product_kernel<S, F16, PARTS, DOWN>), grid, dim3(S::NT), 0, st, g, r);
     else if constexpr (DOWN != DOWN_A) {  // always in parts
-        if constexpr (F16 == (DOWN == DOWN_B)) {  // the other's callers have 16-bit results
-            if (r.dt == DT_F32) {
-                hipLaunchKernelGGL((product_kernel<S, F16, OUT32, DOWN>), grid, dim3(S::NT), 0, st, g, r);
-                return;
-            }
-        }
-        hipLaunchKernelGGL((product_kernel<S, F16, OUT16, DOWN>), grid, dim3(S::NT), 0, st, g, r);
+        if (r.dt == DT_F32) hipLaunchKernelGGL((product_kernel<S, F16, OUT32, DOWN>), grid, dim3(S::NT), 0, st, g, r);
+        else hipLaunchKernelGGL((product_kernel<S, F16, OUT16, DOWN>), grid, dim3(S::NT), 0, st, g, r);
     }
 }
 template <class S>

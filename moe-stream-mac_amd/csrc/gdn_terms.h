@@ -40,9 +40,8 @@ void exponents(const float *part, int top, int *exps, float *most, hipStream_t s
 constexpr int LOW = 11;
 void terms(const Source &s, int slots, bool f16, const int *exps, int which, void *dst, hipStream_t st);
 
-// The same transposed, times f's factors (where f.row is not NULL), bf16 terms of bf16 numbers and else fp16:
-// dst[c][t * padded(rows) + r].
-void terms_across(const Source &s, int slots, const int *exps, int which, const Factors &f, void *dst, hipStream_t st);
+// The same transposed, times f's factors (where f.row is not NULL): dst[c][t * padded(rows) + r].
+void terms_across(const Source &s, int slots, bool f16, const int *exps, int which, const Factors &f, void *dst, hipStream_t st);
 
 }  // namespace mm
 }  // namespace gdn

@@ -207,14 +207,15 @@ void terms(const Source &s, int slots, bool f16, const int *exps, int which, voi
 #undef GDN_STRAIGHT
 }
 
-void terms_across(const Source &s, int slots, const int *exps, int which, const Factors &f, void *dst, hipStream_t st) {
+void terms_across(const Source &s, int slots, bool f16, const int *exps, int which, const Factors &f, void *dst, hipStream_t st) {
     Timed tm("terms_across", st);
     const int64_t kp = padded(s.rows), tc = (s.cols + 63) / 64, tiles = kp / 64 * tc;
     const dim3 grid = grid_of(tiles);
 #define GDN_ACROSS(F16, DT) GDN_TERMS(across_kernel, F16, DT, s, slots, exps, which, f, static_cast<uint16_t *>(dst), kp, tc, tiles)
     if (s.dt == DT_BF16) GDN_ACROSS(false, DT_BF16);
     else if (s.dt == DT_F16) GDN_ACROSS(true, DT_F16);
-    else GDN_ACROSS(true, DT_F32);
+    else if (f16) GDN_ACROSS(true, DT_F32);
+    else GDN_ACROSS(false, DT_F32);
 #undef GDN_ACROSS
 }
 #undef GDN_TERMS

@@ -81,3 +81,42 @@ def test_bits_of_small_probabilities(dev, N, H, V, apart):
         dw = gradients(x, w, t, d, wanted)[-1]
         within(dw[rows], want[1][rows], tol[1][rows], "dw")
         assert bool(dw[rows].any(1).all())
+
+
+@pytest.mark.parametrize("N,H,V", [(1, 64, 7), (20, 128, 500), (33, 70, 129), (64, 192, 1000), (128, 64, 3001)])
+def test_few_fp32_tokens_of_any_magnitude(dev, N, H, V):
+    """Channels whose factors lie up to 2^120 apart, of up to 128 tokens with fp32 words: loss and gradients of one channel do not
+    suffer from another's magnitude.  Three terms hold every number; the products that are left out, of a second and a third term,
+    are below 2 * 2^-22 of the factors' product (3 here)."""
+    from linear_loss import linear_cross_entropy
+    print("magnitudes", N, H, V, flush=True)
+    g = torch.Generator(device=dev)
+    g.manual_seed(N + V)
+    x = torch.randn(N, H, device=dev, generator=g)
+    w = 3 * H ** -0.5 * torch.randn(V, H, device=dev, generator=g)
+    for c, e in ((0, 60), (1, -50), (2, 20), (H - 1, -33)):
+        x[:, c] *= 2.0 ** -e
+        w[:, c] *= 2.0 ** e
+    t = torch.randint(0, V, (N,), device=dev, generator=g)
+    if N > 2:
+        t[1] = -100
+    d = torch.randn(N, device=dev, generator=g)
+    X, W, D = x.double(), w.double(), torch.where(t != -100, d.double(), 0.0)
+    z = X @ W.t()
+    lse = torch.logsumexp(z, 1, keepdim=True)
+    p = (z - lse).exp()
+    at = (torch.arange(N, device=dev), t.clamp_min(0))
+    loss = torch.where(t != -100, lse[:, 0] - z[at], 0.0)
+    part = 20 * U + 3 * 2.0 ** -22  # of a product of two sums of terms, and of sums of them
+    zerr = part * (X.abs() @ W.abs().t()).amax(1, keepdim=True)
+    diff = p.clone()
+    diff[at] -= 1
+    err = D.abs()[:, None] * (diff.abs() * part + p * (2 * zerr + 40 * U + 2 * U * z.abs().amax(1, keepdim=True)))
+    diff = D[:, None] * diff
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    got = linear_cross_entropy(x, w, t, reduction="none")
+    dx, dw = torch.autograd.grad(got, [x, w], d)
+    within(got.detach(), loss, 2 * zerr[:, 0] + U * (16 + 4 * loss.abs() + 4 * z.abs().amax(1)), "loss")
+    within(dx, diff @ W, err @ W.abs(), "dx")
+    within(dw, diff.t().contiguous() @ X, err.t().contiguous() @ X.abs(), "dw")
