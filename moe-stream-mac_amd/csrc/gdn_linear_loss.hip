@@ -27,10 +27,11 @@
 // 2^15, 2^-22 of it or 2^-40; what that leaves out is below fp16 results, which end at 2^-25, unless cotangents times x pass
 // 2^15.  x is an fp16 number times a power of two there for dW (gdn_terms.hip).  Of a token's cotangent the differences carry a
 // factor of 0.75 to 1.5 and its sum for dx, or its x for dW, the power of two that is left, so that it costs no rounding of its
-// own.  fp32 operands are two fp16 terms under one power of two (2^-22 of a number, or 2^-39 of its matrix's largest) and every
-// product three pairs of them; a difference's second term is stored times 2^11, so that small probabilities keep their bits
-// (2^-22 of them down to 2^-29, 2^-51 below).  Up to WIDE fp32 tokens, forward and backward: three bf16 terms, which hold a
-// number of any magnitude as it is, and six pairs; those left out are below 2^-21 of the factors.
+// own.  fp32 operands are two fp16 terms under a power of two (2^-22 of a number, or 2^-39 of the largest under it), and every
+// product three pairs of them; for the logits each token has a power of its own, so that no token costs another its bits; a
+// difference's second term is stored times 2^11, so that small probabilities keep their bits (2^-22 of them down to 2^-29, 2^-51
+// below).  Up to WIDE fp32 tokens, forward and backward: three bf16 terms, which hold a number of any magnitude as it is, and
+// six pairs; those left out are below 2^-21 of the factors.
 //
 // Of few tokens (below ROWS) the differences' terms are rows of one operand for dx, so that the weight, which lies along the
 // channels, is read once.  2048 x 32000 bf16, forward and dx: 64 tokens 117 us so, 123 with terms side by side; 256 187 and 187;
@@ -119,21 +120,22 @@ struct StatArgs {
     const int64_t *targets;
     float2 *part;  // [parts][N]: maximum and sum of a part of the words
     float *zt;     // [N] the target's logit
-    const int *exps;
+    const int *exps, *each;  // SCALED: the words' exponent is exps[E_W], a token's each[n]
     int64_t N, V, v0;  // word of the operand's first row
     int part0;
 };
 
-// The statistics of a wave's words, `rows` - m0 of 16 TM, for its 16 TN tokens from n0 on.  e: the logits' scale.
+// The statistics of a wave's words, `rows` - m0 of 16 TM, for its 16 TN tokens from n0 on.
 template <int TM, int TN, bool SCALED>
 __device__ __forceinline__ void statistics(const StatArgs &a, int64_t rows, int64_t tokens, int64_t m0, int64_t n0, int64_t part,
-                                           int e, acc_t (&acc)[TM][TN]) {
+                                           acc_t (&acc)[TM][TN]) {
     const int lane = lane_here();
     const int words = (int)min((int64_t)(16 * TM), rows - m0);
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
         const int64_t n = n0 + 16 * j + (lane & 15);
         const bool live = n < tokens;
+        const int e = SCALED && live ? -(a.exps[E_W] + a.each[n]) : 0;
         float mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < TM; ++i)
@@ -177,8 +179,7 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void stat_kernel(const Args g, 
     const Extent ext = extent_of<S>(g);
     products<S, F16>(g, ext, lds, [&](int tm, int tn, acc_t(&acc)[S::TM][S::TN]) {
         const int64_t m0 = (int64_t)tm * S::BM + wm * (S::BM / S::WM), n0 = (int64_t)tn * S::BN + wn * (S::BN / S::WN);
-        const int e = SCALED ? -(a.exps[E_X] + a.exps[E_W]) : 0;
-        statistics<S::TM, S::TN, SCALED>(a, g.a.rows, ext.rows_b, m0, n0, a.part0 + tm * S::WM + wm, e, acc);
+        statistics<S::TM, S::TN, SCALED>(a, g.a.rows, ext.rows_b, m0, n0, a.part0 + tm * S::WM + wm, acc);
     });
 }
 
@@ -288,7 +289,7 @@ __global__ __launch_bounds__(256, Wide<TN>::WAVES_EU) void wide_kernel(const Wid
 #pragma unroll
                 for (int h = 0; h < 2; ++h) now[s][i][h] = next[s][i][h];
     }
-    statistics<S::TM, TN, false>(a, g.rows, g.x.rows, m0, 0, blockIdx.x * 4 + w, 0, acc);
+    statistics<S::TM, TN, false>(a, g.rows, g.x.rows, m0, 0, blockIdx.x * 4 + w, acc);
 }
 
 // Joins a token's parts: TOKENS tokens to a workgroup, NT / TOKENS threads to a token.
@@ -405,7 +406,7 @@ struct DiffArgs {
     const int64_t *targets;
     const float2 *stat;
     const float *power, *factor;  // cotangents
-    const int *exps;  // SCALED: the logits' scale
+    const int *exps, *each;  // SCALED: the logits' scale
     uint16_t *p;      // kp to a row and term: rows `row` apart, a next term `second` on
     int64_t v0, kp, row, second;
 };
@@ -437,11 +438,11 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void diff_kernel(const Args g, 
         const int lane = lane_here();
         const int64_t m0 = (int64_t)tm * S::BM + wm * (S::BM / S::WM), n0 = (int64_t)tn * S::BN + wn * (S::BN / S::WN);
         const int words = (int)min((int64_t)(S::BM / S::WM), g.a.rows - m0);  // of this wave's; may be negative
-        const int e = SCALED ? -(a.exps[E_X] + a.exps[E_W]) : 0;
 #pragma unroll
         for (int j = 0; j < S::TN; ++j) {
             const int64_t n = n0 + 16 * j + (lane & 15);
             const bool in = n < ext.rows_b;
+            const int e = SCALED && in ? -(a.exps[E_W] + a.each[n]) : 0;
             const float2 st = in ? a.stat[n] : make_float2(0.f, 0.f);
             const bool live = in && a.power[n] != 0.f;
             const float scale = live ? a.factor[n] * (F16 ? (float)(1 << SHIFT) : 1.f) : 0.f, inv = st.y * scale;
@@ -525,8 +526,8 @@ struct Sizes {
 
 // The segments of a product over kp elements: a's terms `first` elements apart, b's `second`.
 //   one term of a, two of b:  both pairs
-//   two terms (fp16):         all pairs but that of the second ones.  a has three slots in the backward pass, as terms() makes them;
-//                             the third meets b's second term, stored times 2^LOW
+//   two terms (fp16):         all pairs but that of the second ones.  a has three slots in the backward pass, as terms() makes
+//                             them; the third meets b's second term, stored times 2^LOW
 //   three terms (bf16):       all pairs but those below 2^-16 of the first, the smallest first
 static void segments(Args &g, const Sizes &s, bool back, int64_t kp, int64_t first, int64_t second) {
     const auto pair = [&](int i, int j) {
@@ -600,7 +601,7 @@ struct Buffers {
     uint16_t *x, *w, *xt, *p;
     float *part, *zt, *power, *factor, *most, *acc_x, *acc_w;
     float2 *stats;
-    int *exps;
+    int *exps, *each;
     Tokens tokens;
 };
 
@@ -617,6 +618,7 @@ static Buffers place(Space &sp, const Sizes &s, bool dx, bool dw, bool bwd, bool
         b.tokens.place = sp.take<int>(s.N);
         b.tokens.target = sp.take<int64_t>(s.N);
     }
+    if (s.scaled) b.each = sp.take<int>(s.N);
     if (copy_x || s.compact) b.x = sp.take<uint16_t>(s.N * t * s.hp);
     if (copy_w) b.w = sp.take<uint16_t>(words * s.wslots * s.hp);
     if (!bwd) {
@@ -734,9 +736,10 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
             int *to = stat ? reinterpret_cast<int *>(stat + 2 * N) : b.exps;
             exponents(b.part, TOP, to, b.most, st);  // b.most is not read
             exps = to;
+            row_exponents(sx, TOP, b.each, st);
         }
         if (few) terms(sx, 3, false, nullptr, E_X, b.x, st);
-        else if (!dx) terms(sx, s.terms, s.f16, exps, E_X, b.x, st);
+        else if (!dx) terms(sx, s.terms, s.f16, b.each, EACH_ROW, b.x, st);
         // operands that are used as they lie need no pieces
         const int64_t step = dw ? V : s.piece;
         for (int64_t n0 = 0; n0 < N; n0 += s.tokens) {
@@ -746,7 +749,7 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
             if (few) {  // all tokens
                 const Operand rows{reinterpret_cast<const char *>(b.x), 3 * s.hp * 2, N, {0, s.hp * 2, s.hp * 4}, 0};
                 const WideArgs g{static_cast<const float *>(w), w_stride, V, rows, (int)(s.hp / BK)};
-                const StatArgs a{tt, b.stats, b.zt, nullptr, N, V, 0, 0};
+                const StatArgs a{tt, b.stats, b.zt, nullptr, nullptr, N, V, 0, 0};
                 const dim3 grid((unsigned)((V + 127) / 128));
                 Timed tm("loss_stat", st);
                 if (N <= 32) hipLaunchKernelGGL((wide_kernel<2>), grid, dim3(256), 0, st, g, a);
@@ -778,7 +781,7 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
                     g.b.p = static_cast<const char *>(x) + n0 * x_stride * 2;
                     g.b.ld = x_stride * 2;
                 }
-                const StatArgs a{tt + n0, b.stats, b.zt, exps, tokens, V, v0, parts};
+                const StatArgs a{tt + n0, b.stats, b.zt, exps, s.scaled ? b.each + n0 : nullptr, tokens, V, v0, parts};
                 Timed tm("loss_stat", st);
 #define GDN_STAT(S)                                \
     launch_stat<S>(g, a, s, st);                   \
@@ -841,7 +844,8 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
         maxima({sx, none}, b.part, st);
     }
     if (dw) exponents(b.part, TOP, scaled_x ? b.exps : nullptr, b.most, st);
-    if (!direct_x) terms(sx, t, s.f16, s.scaled ? exps : nullptr, E_X, b.x, st);
+    if (s.scaled) row_exponents(sx, TOP, b.each, st);
+    if (!direct_x) terms(sx, t, s.f16, b.each, EACH_ROW, b.x, st);
     if (dw) terms_across(sx, s.slots, s.f16, s.f16 ? exps : nullptr, E_X, Factors{b.power, b.most}, b.xt, st);
     const int shape = plan(N, s.piece, s.slots * s.hp / BK, 1).shape;
     for (int64_t v0 = 0; v0 < V; v0 += s.piece) {
@@ -869,7 +873,8 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
             g.b.ld = x_stride * 2;
         }
         const int64_t second = s.rows ? N * kp : kp;
-        const DiffArgs a{tt, reinterpret_cast<const float2 *>(stat), b.power, b.factor, exps, b.p, v0, kp, s.pterms * kp, second};
+        const DiffArgs a{tt, reinterpret_cast<const float2 *>(stat), b.power, b.factor, exps, b.each, b.p, v0, kp, s.pterms * kp,
+                         second};
         {
             Timed tm("loss_diff", st);
 #define GDN_DIFF(S) launch_diff<S>(g, a, s, st)

@@ -34,10 +34,13 @@ void maxima(const Source (&s)[2], float *part, hipStream_t st);
 // most[0] = the largest of part[2][PARTS].  exps NULL: only that.
 void exponents(const float *part, int top, int *exps, float *most, hipStream_t st);
 
-// dst[r][t * padded(cols) + c] = term t < slots of 2^e s[r][c], e = exps[which] (0 without exps), zeros behind the last column: x
-// is the sum of its terms up to the last one's rounding.  f16 or bf16 terms; the third of three fp16 slots holds the first term
-// times 2^-LOW, the partner of a second term that is stored times 2^LOW.
-constexpr int LOW = 11;
+// exps[r] = the same for the finite magnitudes of row r alone.
+void row_exponents(const Source &s, int top, int *exps, hipStream_t st);
+
+// dst[r][t * padded(cols) + c] = term t < slots of 2^e s[r][c], e = exps[which], or exps[r] with which = EACH_ROW (0 without exps),
+// zeros behind the last column: x is the sum of its terms up to the last one's rounding.  f16 or bf16 terms; the third of three
+// fp16 slots holds the first term times 2^-LOW, the partner of a second term that is stored times 2^LOW.
+constexpr int LOW = 11, EACH_ROW = -1;
 void terms(const Source &s, int slots, bool f16, const int *exps, int which, void *dst, hipStream_t st);
 
 // The same transposed, times f's factors (where f.row is not NULL): dst[c][t * padded(rows) + r].

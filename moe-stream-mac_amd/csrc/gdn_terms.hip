@@ -63,6 +63,13 @@ __global__ __launch_bounds__(1024) void maxima_kernel(const Pair both, float *pa
     }
 }
 
+// The exponent that takes m to [2^top, 2^(top + 1)), 0 for 0.
+__device__ __forceinline__ int exponent_to(float m, int top) {
+    int e = 0;
+    if (m > 0.f) (void)frexpf(m, &e);  // m in [2^(e - 1), 2^e)
+    return m > 0.f ? top + 1 - e : 0;
+}
+
 __global__ __launch_bounds__(64) void exponents_kernel(const float *part, int top, int *exps, float *most) {
     const int i = blockIdx.x;
     if (i < 2 && !exps) return;
@@ -71,11 +78,27 @@ __global__ __launch_bounds__(64) void exponents_kernel(const float *part, int to
     for (int k = 0; k < PARTS / 64; ++k) m = fmaxf(m, part[i * PARTS + k * 64 + threadIdx.x]);
     m = wave_max(m);
     if (threadIdx.x == 0) {
-        int e = 0;
-        if (m > 0.f) (void)frexpf(m, &e);  // m in [2^(e - 1), 2^e)
-        if (i < 2) exps[i] = m > 0.f ? top + 1 - e : 0;
+        if (i < 2) exps[i] = exponent_to(m, top);
         else most[0] = m;
     }
+}
+
+// A wave to a row of fp32 numbers.
+__global__ __launch_bounds__(NT) void row_exponents_kernel(const Source s, int top, int *exps) {
+    const int lane = threadIdx.x & 63;
+    const int64_t r = block_index() * (NT / 64) + (threadIdx.x >> 6);
+    if (r >= s.rows) return;
+    const int64_t at = row_of(s, r);
+    float m = 0.f;
+    if (at >= 0)
+        for (int64_t c = lane * 8; c < s.cols; c += 512) {
+            float x[8];
+            ops::load_first<8, DT_F32>(s.p, at * s.ld + c, s.cols - c, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = fmaxf(m, magnitude(x[j]));
+        }
+    m = wave_max(m);
+    if (lane == 0) exps[r] = exponent_to(m, top);
 }
 
 // The next term of y, which keeps the rest: rounded (fp16) or cut off (bf16: three take the 24 bits of an fp32 number as they
@@ -109,7 +132,7 @@ __global__ __launch_bounds__(NT) void terms_kernel(const Source s, int slots, co
     const uint32_t per = (uint32_t)(kp / 8);
     const int64_t r = i >> 32 ? i / per : (uint32_t)i / per, c = (i - r * per) * 8;
     if (r >= s.rows) return;
-    const int e = exps ? exps[which] : 0;
+    const int e = !exps ? 0 : exps[which == EACH_ROW ? r : which];
     float x[8], whole[8];
     const int64_t at = row_of(s, r);
     ops::load_first<8, DT>(s.p, at * s.ld + c, at < 0 ? 0 : s.cols - c, x);
@@ -190,6 +213,11 @@ void maxima(const Source (&s)[2], float *part, hipStream_t st) {
 
 void exponents(const float *part, int top, int *exps, float *most, hipStream_t st) {
     hipLaunchKernelGGL(exponents_kernel, dim3(3), dim3(64), 0, st, part, top, exps, most);
+}
+
+void row_exponents(const Source &s, int top, int *exps, hipStream_t st) {
+    Timed tm("row_exponents", st);
+    hipLaunchKernelGGL(row_exponents_kernel, grid_of((s.rows + NT / 64 - 1) / (NT / 64)), dim3(NT), 0, st, s, top, exps);
 }
 
 #define GDN_TERMS(KERNEL, F16, DT, ...) hipLaunchKernelGGL((KERNEL<F16, DT>), grid, dim3(NT), 0, st, __VA_ARGS__)

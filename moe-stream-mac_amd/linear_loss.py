@@ -93,8 +93,12 @@ def linear_cross_entropy(x: Array, weight: Array, targets: Array, *, ignore_inde
 
     Tokens that do not count cost no time where there are many (2048 and more in all).  Memory beside the gradients: 8 bytes for
     each token and 64 words and a copy of ``x`` forward; backward up to 2^26 probabilities, 32 bits each, the piece of the weight
-    that they belong to, and two copies of ``x`` with its gradient's sums.  float32 operands become sums of 16-bit terms, which hold
-    no infinities: those may count as NaN."""
+    that they belong to, and two copies of ``x`` with its gradient's sums.
+
+    bfloat16 and float16 inputs enter with all their bits, and gradients are as good as 32-bit sums rounded once.  float32
+    inputs are sums of 16-bit terms, which hold no infinities: those may count as NaN.  Up to 128 tokens the terms are exact.
+    More have 2^-22 of a number, or 2^-39 of the largest of its token (``x``, in the loss and its own gradient), of ``weight``,
+    or of ``x`` (in ``weight``'s gradient), whichever is more."""
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"x must be [..., H] and weight [V, H]; got {tuple(x.shape)} and {tuple(weight.shape)}")
     if tuple(targets.shape) != tuple(x.shape[:-1]):

@@ -120,3 +120,22 @@ def test_few_fp32_tokens_of_any_magnitude(dev, N, H, V):
     within(got.detach(), loss, 2 * zerr[:, 0] + U * (16 + 4 * loss.abs() + 4 * z.abs().amax(1)), "loss")
     within(dx, diff @ W, err @ W.abs(), "dx")
     within(dw, diff.t().contiguous() @ X, err.t().contiguous() @ X.abs(), "dw")
+
+
+@pytest.mark.parametrize("N,H,V", [(129, 64, 300), (200, 70, 1501), (2111, 192, 777)])
+def test_fp32_tokens_leave_others_alone(dev, N, H, V):
+    """A huge token and a tiny one among others: each token's loss and dx are as good as its own numbers allow."""
+    from linear_loss import linear_cross_entropy
+    from test_gpu_linear_loss import inputs, plain
+    print("huge token", N, H, V, flush=True)
+    x, w, t, d = inputs(dev, N, H, V, torch.float32, N)
+    t[5] = t[9] = 3
+    x[5] *= 2.0 ** 40
+    x[9] *= 2.0 ** -50
+    x.requires_grad_(True)
+    want, tol = plain(x, w, t, d)
+    loss = linear_cross_entropy(x, w, t, reduction="none")
+    dx, = torch.autograd.grad(loss, [x], d)
+    within(loss.detach(), want[0], tol[0], "loss")
+    within(dx, want[1], tol[1], "dx")
+    within(linear_cross_entropy(x.detach(), w, t, reduction="none"), want[0], tol[0], "loss alone")
