@@ -62,6 +62,7 @@ def embedding(ids: Array, weight: Array, *, scale: float = 1.0, padding_idx: Opt
         raise ValueError(f"ids must be int64 or int32; got {ids.dtype}")
     if padding_idx is not None and not 0 <= padding_idx < weight.shape[0]:
         raise ValueError(f"padding_idx must be in [0, {weight.shape[0]}); got {padding_idx}")
+    L.refuse_tangents("embedding", weight)
     if weight.device.type != "cuda":
         raise RuntimeError("embedding runs on a ROCm GPU only; got tensors on " + str(weight.device))
     if ids.device != weight.device:

@@ -14,6 +14,7 @@ import re
 from pathlib import Path
 
 import torch  # noqa: F401  (must precede loading the HIP library)
+import torch.autograd.forward_ad as fwAD
 
 LIB_PATH = Path(__file__).resolve().parent / "libgdn_mi355x.so"
 HEADER = Path(__file__).resolve().parent.parent / "include" / "gdn_mi355x.h"
@@ -137,6 +138,12 @@ def written(tensors) -> None:
     torch.autograd.graph.increment_version(tensors)
 
 
+def refuse_tangents(what: str, *tensors) -> None:
+    """Raises where a tensor carries a forward-mode tangent: a kernel sees the primal alone, and its result would be a constant."""
+    if fwAD._current_level >= 0 and any(t is not None and fwAD.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative")
+
+
 class _Once(torch.autograd.Function):
     @staticmethod
     def forward(ctx, n, *inputs_and_grads):
@@ -149,7 +156,8 @@ class _Once(torch.autograd.Function):
 
 def once(inputs, *grads):
     """A backward pass's results: with create_graph, ones that raise when they are differentiated in what they depend on,
-    its ``inputs``, instead of constants."""
+    its ``inputs``, instead of constants.  Forward-mode tangents of the inputs are refused."""
+    refuse_tangents("a gradient of this operator", *inputs)
     return _Once.apply(len(inputs), *inputs, *grads) if torch.is_grad_enabled() else grads
 
 

@@ -111,6 +111,7 @@ def linear_cross_entropy(x: Array, weight: Array, targets: Array, *, ignore_inde
         raise ValueError("weight must not be empty")
     if reduction not in REDUCTIONS:
         raise ValueError(f"reduction must be one of {', '.join(REDUCTIONS)}; got {reduction!r}")
+    L.refuse_tangents("linear_cross_entropy", x, weight)
     if x.device.type != "cuda":
         raise RuntimeError("linear_cross_entropy runs on a ROCm GPU only; got tensors on " + str(x.device))
     if weight.device != x.device or targets.device != x.device:

@@ -123,6 +123,7 @@ def linear(x: Array, q: Weight) -> Array:
         raise ValueError(f"x must be [..., {q.columns}]; got {tuple(x.shape)}")
     if x.dtype not in L.DTYPE_CODE:
         raise ValueError(f"unsupported dtype {x.dtype}; use float32, bfloat16 or float16")
+    L.refuse_tangents("linear", x)
     _on_gpu(x, "linear")
     if q.codes.device != x.device:
         raise ValueError("all inputs must be on the same device")

@@ -1,0 +1,44 @@
+"""Forward-mode tangents are refused where a kernel would leave them out (no kernel launches)."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+import gdn_lib as L
+
+
+def calls(x, w):
+    """Calls of the operators with x [6, 64] and w [9, 64], and the tensors through which a tangent may come."""
+    import mxfp4
+    from embedding import embedding
+    from linear_loss import linear_cross_entropy
+    t = torch.zeros(6, dtype=torch.int64)
+    q = mxfp4.Weight(torch.zeros(9, 32, dtype=torch.uint8), torch.zeros(9, 2, dtype=torch.uint8), 64)
+    return {"linear_cross_entropy": lambda: linear_cross_entropy(x, w, t), "embedding": lambda: embedding(t, w),
+            "linear": lambda: mxfp4.linear(x, q)}
+
+
+@pytest.mark.parametrize("which", ["x", "w"])
+def test_operators_at_both_ends(which):
+    x, w = torch.randn(6, 64), torch.randn(9, 64)
+    with fwAD.dual_level():
+        dual = {"x": x, "w": w}
+        dual[which] = fwAD.make_dual(dual[which], torch.ones_like(dual[which]))
+        for name, call in calls(dual["x"], dual["w"]).items():
+            takes = {"x": name != "embedding", "w": name != "linear"}[which]
+            with pytest.raises(RuntimeError, match=f"{name} has no forward-mode" if takes else "ROCm GPU only"):
+                call()
+        for call in calls(x, w).values():  # an open level alone changes nothing
+            with pytest.raises(RuntimeError, match="ROCm GPU only"):
+                call()
+    with pytest.raises(RuntimeError, match="linear_cross_entropy has no forward-mode"):
+        torch.func.jvp(lambda a: calls(a, w)["linear_cross_entropy"](), (x,), (x,))
+
+
+def test_backward_passes():
+    """A cotangent with a tangent of its own would lose it in every backward pass."""
+    g = torch.randn(3)
+    with fwAD.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            L.once((g, fwAD.make_dual(g, g)), g)
+        assert L.once((g, None), g)[0] is g or torch.equal(L.once((g, None), g)[0], g)
