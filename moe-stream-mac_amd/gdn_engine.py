@@ -190,6 +190,7 @@ def recurrence(q, k, v, g, beta, state, mask=None, chunk: int = 64, log_gate: bo
     if chunk <= 0:
         raise ValueError("chunk must be a positive integer")
     check_shapes(q, k, v, g, beta, state, mask)
+    L.refuse_tangents("the GDN recurrence", q, k, v, g, beta, state)
     _require_device(q, k, v, g, beta, state)
     out_dtype = output_dtype
     if out_dtype is None:
@@ -225,6 +226,7 @@ def decode_step(q, k, v, g, beta, state_in, state_out, log_gate: bool = False,
     """One token of B sequences: q, k [B, Hk, Dk], v [B, Hv, Dv], g [B, Hv] (or [B, Hv, Dk]), beta [B, Hv];
     reads state_in [B, Hv, Dv, Dk] fp32 (None = zeros) and writes state_out (which may be state_in: in place).
     Returns y [B, Hv, Dv].  Forward only (engine/include/gdn.h:27-38)."""
+    L.refuse_tangents("a step of the GDN recurrence", q, k, v, g, beta, state_in)
     dev = _require_device(q, k, v, g, beta, state_out)
     B, Hk, Dk = q.shape
     Hv, Dv = v.shape[1], v.shape[2]

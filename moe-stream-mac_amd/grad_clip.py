@@ -40,6 +40,7 @@ def _check(tensors, norm_type) -> None:
         raise ValueError(f"unsupported tensor ({t.dtype}, {t.layout}); use dense float32, bfloat16 or float16")
     if len(set(map(_index, tensors))) > 1:
         raise ValueError("all tensors must be on the same device")
+    L.refuse_tangents("grad_clip", *tensors)
     if tensors[0].device.type != "cuda":
         raise RuntimeError("grad_clip runs on a ROCm GPU only; got tensors on " + str(tensors[0].device))
 

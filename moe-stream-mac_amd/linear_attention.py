@@ -37,6 +37,7 @@ def _check(q: Array, k: Array, v: Array, g: Array, state: Optional[Array], lead:
         raise ValueError(f"unsupported dtype {g.dtype} of g; use float32, bfloat16 or float16")
     if state is not None and tuple(state.shape) != (B, Hv, Dv, Dk):
         raise ValueError(f"state must be [B, Hv, Dv, Dk] = {(B, Hv, Dv, Dk)}; got {tuple(state.shape)}")
+    L.refuse_tangents("linear attention", q, k, v, g, state)
     if q.device.type != "cuda":
         raise RuntimeError("linear attention runs on a ROCm GPU only; got tensors on " + str(q.device))
     if any(t is not None and t.device != q.device for t in (k, v, g, state)):

@@ -98,6 +98,7 @@ def rotary(q: Array, k: Array, positions: Array, inv_freq: Array, *, interleaved
         raise ValueError(f"positions must be int64 or int32; got {positions.dtype}")
     if inv_freq.dim() != 1 or not 0 < 2 * inv_freq.numel() <= D:
         raise ValueError(f"inv_freq must hold between 1 and D / 2 = {D // 2} frequencies; got {tuple(inv_freq.shape)}")
+    L.refuse_tangents("rotary", q, k)
     if q.device.type != "cuda":
         raise RuntimeError("rotary runs on a ROCm GPU only; got tensors on " + str(q.device))
     if any(t.device != q.device for t in (k, positions, inv_freq)):

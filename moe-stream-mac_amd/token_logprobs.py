@@ -111,6 +111,7 @@ def token_logprobs(logits: Array, targets: Array, *, entropy: bool = False, top:
         raise ValueError(f"targets must be int64 or int32; got {targets.dtype}")
     if logits.shape[-1] == 0 or not 0 <= top <= logits.shape[-1]:
         raise ValueError(f"top must be between 0 and V = {logits.shape[-1]}, V positive; got {top}")
+    L.refuse_tangents("token_logprobs", logits)
     if logits.device.type != "cuda":
         raise RuntimeError("token_logprobs runs on a ROCm GPU only; got tensors on " + str(logits.device))
     if targets.device != logits.device:

@@ -42,3 +42,29 @@ def test_backward_passes():
         with pytest.raises(RuntimeError, match="forward-mode"):
             L.once((g, fwAD.make_dual(g, g)), g)
         assert L.once((g, None), g)[0] is g or torch.equal(L.once((g, None), g)[0], g)
+
+
+def test_operators_between():
+    """The operators inside a model, each of its differentiable inputs in turn."""
+    import grad_clip
+    from gdn_engine import decode_step, recurrence
+    from linear_attention import linear_attention, linear_attention_step
+    from rotary import rotary, rotary_frequencies
+    from token_logprobs import token_logprobs
+    n = torch.randn
+    inv, t, at = rotary_frequencies(4)[0], torch.zeros(2, 3, dtype=torch.int64), torch.arange(3)
+    qkvg = [n(2, 3, 2, 8), n(2, 3, 2, 8), n(2, 3, 2, 8), -torch.rand(2, 3, 2), n(2, 2, 8, 8)]
+    beta = torch.rand(2, 3, 2)
+    for call, inputs in ((lambda q, k: rotary(q, k, at, inv), qkvg[:2]), (lambda z: token_logprobs(z, t), [n(2, 3, 9)]),
+                         (lambda g: grad_clip.grad_norm([g]), [n(5)]), (lambda g: grad_clip.clip_grad_norm([g], 1.0), [n(5)]),
+                         (linear_attention, qkvg),
+                         (lambda q, k, v, g, s: recurrence(q, k, v, g, beta, s), qkvg),
+                         (linear_attention_step, [*[a[:, 0] for a in qkvg[:4]], qkvg[4]]),
+                         (lambda q, k, v, g, s: decode_step(q, k, v, g, beta[:, 0], s, s.detach().clone()),
+                          [*[a[:, 0] for a in qkvg[:4]], qkvg[4]])):
+        with pytest.raises(RuntimeError, match="ROCm GPU only"):
+            call(*inputs)
+        with fwAD.dual_level():
+            for i in range(len(inputs)):
+                with pytest.raises(RuntimeError, match="no forward-mode"):
+                    call(*[fwAD.make_dual(a, torch.ones_like(a)) if i == j else a for j, a in enumerate(inputs)])
