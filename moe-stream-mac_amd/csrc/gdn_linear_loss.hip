@@ -33,9 +33,9 @@
 // below).  Up to WIDE fp32 tokens, forward and backward: three bf16 terms, which hold a number of any magnitude as it is, and
 // six pairs; those left out are below 2^-21 of the factors.
 //
-// Of few tokens (below ROWS) the differences' terms are rows of one operand for dx, so that the weight, which lies along the
-// channels, is read once.  2048 x 32000 bf16, forward and dx: 64 tokens 117 us so, 123 with terms side by side; 256 187 and 187;
-// 511 272 and 276; 1024 497 and 498; 1500 771 and 711.
+// Of few tokens (up to ROWS, 16-bit inputs) the differences' terms are rows of one operand for dx, so that the weight, which
+// lies along the channels, is read once.  2048 x 32000 bf16, forward and dx: 8 tokens 109 us so, 118 with terms side by side; 64
+// 115 and 123; 100 145 and 158; 256 180 and 174; 511 273 and 267.
 //
 // Measured, bf16, 8192 tokens of which a fifth does not count, 2048 x 32000, both gradients: 686 us for the statistics (1.25
 // PFLOP/s), then four pieces with 247 for the differences, 381 for dx and 323 for dW (1.15 and 1.36 PFLOP/s over both terms).
@@ -54,7 +54,7 @@ using namespace mm;
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int NT = 256;
 constexpr int64_t COMPACT = 2048;
-constexpr int64_t ROWS = 512;
+constexpr int64_t ROWS = 128;
 constexpr int64_t KEPT = 1 << 26;  // differences of a piece, if that is 256 words or more; statistics of the parts of the words
 constexpr int64_t MOST_TOKENS = 1 << 20;  // three slots of 16 bits for each are a row pitch that a product takes
 constexpr int WIDE = 128;          // up to here fp32 numbers are three bf16 terms, and a forward call reads the words as they lie
@@ -550,7 +550,8 @@ static bool direct(const void *p, int64_t ld, int64_t H, int dt) {
     return dt != GDN_F32 && H % BK == 0 && ld % 8 == 0 && aligned_to(p, 16) && pitch_fits(ld * 2);
 }
 
-static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt, bool direct_w, bool dx) {
+// The same however the operands lie: what they ask for is room for copies, no more.
+static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt, bool dx) {
     Sizes s{};
     s.N = N; s.H = H; s.V = V;
     s.hp = padded(H);
@@ -560,7 +561,7 @@ static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt, bool direct_w, bool 
     s.scaled = s.terms == 2;
     s.f16 = s.scaled || dt == GDN_F16;
     s.compact = N >= COMPACT;
-    s.rows = N < ROWS && direct_w && dx;  // 16-bit weights only
+    s.rows = N <= ROWS && dx && s.terms == 1;
     s.prows = s.rows ? 2 * N : N;
     s.pterms = s.rows ? 1 : any ? 3 : 2;
     s.slots = s.terms == 1 ? 1 : 3;
@@ -576,7 +577,7 @@ static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt, bool direct_w, bool 
     if (s.tokens < 256) s.tokens = 256;
     if (s.tokens > N) s.tokens = N;
     const int64_t words = s.piece < V ? s.piece : V;
-    s.px = plan(s.prows, H, (s.rows ? 1 : s.pairs) * padded(words) / BK, s.rows ? 32 : 16);
+    s.px = plan(s.prows, H, (s.rows ? 1 : s.pairs) * padded(words) / BK, 32);
     s.pw = plan(words, H, s.pairs * s.np / BK, 8, true);
     return s;
 }
@@ -694,7 +695,7 @@ extern "C" size_t gdn_linear_loss_workspace_bytes(int64_t N, int64_t H, int64_t 
                                                   int want_dw) {
     if (N <= 0 || H <= 0 || V <= 0 || N > MOST_TOKENS || V > 1 << 24 || H > 1 << 17) return 0;
     const bool copy = !aligned || dtype == GDN_F32 || H % BK, bwd = want_dx || want_dw;
-    const Sizes s = sizes(N, H, V, dtype, !copy, want_dx);
+    const Sizes s = sizes(N, H, V, dtype, want_dx);
     const size_t bytes = need(s, want_dx, want_dw, bwd, copy, copy);
     if (bwd || !wide(nullptr, 0, N, H, dtype)) return bytes;
     Space sp{nullptr};  // what the forward call needs for an aligned weight; x alone may be what is not aligned
@@ -715,7 +716,7 @@ extern "C" int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *
     if (N > 0) {
         if (!x || !w || !targets || !loss || !workspace) return fail(GDN_ERR_INVALID, "null pointer");
         const bool dw = direct(w, w_stride, H, dtype);
-        const Sizes s = sizes(N, H, V, dtype, dw, false);
+        const Sizes s = sizes(N, H, V, dtype, false);
         const bool dx = !s.compact && direct(x, x_stride, H, dtype);
         const bool few = wide(w, w_stride, N, H, dtype);
         Space size{nullptr}, sp{static_cast<char *>(workspace)};
@@ -820,7 +821,7 @@ extern "C" int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *
     if (N == 0) return fail(GDN_ERR_INVALID, "no tokens: the gradients are zeros, which this call does not write");
     if (!x || !w || !targets || !stat || !dloss || !workspace) return fail(GDN_ERR_INVALID, "null pointer");
     const bool direct_w = direct(w, w_stride, H, dtype);
-    const Sizes s = sizes(N, H, V, dtype, direct_w, dx);
+    const Sizes s = sizes(N, H, V, dtype, dx);
     const bool direct_x = !s.compact && direct(x, x_stride, H, dtype);
     const size_t bytes = need(s, dx, dw, true, !direct_x, !direct_w);
     if (workspace_bytes < bytes)

@@ -133,6 +133,16 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def row_stride(t) -> int:
+    """Elements from row to row of a matrix with contiguous channels."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def rows_lie_well(*rows) -> bool:
+    """Whether matrix products may read these matrices as they lie, which the workspace queries call aligned."""
+    return all(t.data_ptr() % 16 == 0 and row_stride(t) * t.element_size() % 16 == 0 for t in rows)
+
+
 def written(tensors) -> None:
     """Tensors that a kernel changed in place: autograd refuses to go back through what had saved their old values."""
     torch.autograd.graph.increment_version(tensors)

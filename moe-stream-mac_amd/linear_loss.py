@@ -24,14 +24,6 @@ def _rows(t: Array) -> Array:
     return t
 
 
-def _aligned(*rows: Array) -> bool:
-    return all(t.data_ptr() % 16 == 0 and _stride(t) * t.element_size() % 16 == 0 for t in rows)
-
-
-def _stride(t: Array) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
 def _forward(x, w, targets, ignore_index, reduction, need_grad):
     """(losses [N], their total and its factor, the tokens' statistics; None where not asked for)"""
     dev = x.device
@@ -41,11 +33,11 @@ def _forward(x, w, targets, ignore_index, reduction, need_grad):
     stat = torch.empty((N + 1, 2), dtype=torch.float32, device=dev) if need_grad else None
     total = torch.empty((), dtype=torch.float32, device=dev) if reduction else None
     factor = torch.empty((), dtype=torch.float32, device=dev) if reduction else None
-    nws = lib.gdn_linear_loss_workspace_bytes(N, H, V, dtype, _aligned(x, w), 0, 0)
+    nws = lib.gdn_linear_loss_workspace_bytes(N, H, V, dtype, L.rows_lie_well(x, w), 0, 0)
     ws = torch.empty((nws,), dtype=torch.uint8, device=dev)
     with L.on_device(dev):
         L.check(lib.gdn_linear_loss_fwd(x.data_ptr(), w.data_ptr(), targets.data_ptr(), loss.data_ptr(), L.ptr(stat),
-                                        L.ptr(total), L.ptr(factor), ws.data_ptr(), nws, N, H, V, _stride(x), _stride(w),
+                                        L.ptr(total), L.ptr(factor), ws.data_ptr(), nws, N, H, V, L.row_stride(x), L.row_stride(w),
                                         ignore_index, reduction, dtype, L.stream_handle(dev)))
     return loss, total, factor, stat
 
@@ -72,12 +64,12 @@ class _LinearLoss(torch.autograd.Function):
         dx = torch.empty((N, H), dtype=x.dtype, device=dev) if need_x else None
         dw = torch.empty((V, H), dtype=w.dtype, device=dev) if need_w else None
         lib, dtype = L.load(), L.DTYPE_CODE[x.dtype]
-        nws = lib.gdn_linear_loss_workspace_bytes(N, H, V, dtype, _aligned(x, w), need_x, need_w)
+        nws = lib.gdn_linear_loss_workspace_bytes(N, H, V, dtype, L.rows_lie_well(x, w), need_x, need_w)
         ws = torch.empty((nws,), dtype=torch.uint8, device=dev)
         with L.on_device(dev):
             L.check(lib.gdn_linear_loss_bwd(x.data_ptr(), w.data_ptr(), targets.data_ptr(), stat.data_ptr(), dloss.data_ptr(),
                                             0 if reduction else 1, L.ptr(factor), L.ptr(dx), L.ptr(dw),
-                                            ws.data_ptr(), nws, N, H, V, _stride(x), _stride(w), ignore_index,
+                                            ws.data_ptr(), nws, N, H, V, L.row_stride(x), L.row_stride(w), ignore_index,
                                             dtype, L.stream_handle(dev)))
         return (*L.once((x, w, dloss), dx, dw), None, None, None)
 
