@@ -367,7 +367,7 @@ int gdn_clip_grad_norm(const void *const *x, void *const *y, const int64_t *nume
  * gdn_linear_loss_bwd: dx [N][H] and dw [V][H], contiguous (dtype; either may be NULL), from the cotangents dloss (fp32;
  * dloss_stride 1: one for each token, 0: one for all), times factor [0] (NULL for 1); dx is 0 at ignored tokens.
  * N <= 2^20, V <= 2^24, H <= 2^17.  The workspace of the forward pass: want_dx = want_dw = 0.  aligned: both operands lie on
- * 16 bytes, with rows a multiple of 16 bytes apart; without it there is room for copies of them. */
+ * 16 bytes, with rows a multiple of 16 bytes and at most 8 MiB apart; without it there is room for copies of them. */
 size_t gdn_linear_loss_workspace_bytes(int64_t N, int64_t H, int64_t V, int dtype, int aligned, int want_dx, int want_dw);
 int gdn_linear_loss_fwd(const void *x, const void *w, const int64_t *targets, float *loss, float *stat, float *total,
                         float *factor, void *workspace, size_t workspace_bytes, int64_t N, int64_t H, int64_t V, int64_t x_stride,
@@ -395,7 +395,8 @@ int gdn_embedding_bwd(const int64_t *ids, const void *dy, void *dw, void *worksp
  *
  * gdn_mxfp4_linear: y [M][N] = x w^T, gdn_mxfp4_linear_bwd: dx [M][K] = dy w (x, dy of dtype, rows x_stride or dy_stride
  * elements apart; y, dx contiguous, of dtype); the weight's values and every bit of x or dy enter 32-bit sums.  A forward call
- * of at most 64 tokens needs no workspace.  aligned: x or dy lies on 16 bytes, with rows a multiple of 16 bytes apart.
+ * of at most 64 tokens needs no workspace.  aligned: x or dy lies on 16 bytes, with rows a multiple of 16 bytes and
+ * at most 8 MiB apart.
  * M, N <= 2^24, K <= 2^18. */
 int gdn_mxfp4_quantize(const void *w, void *codes, void *scales, int64_t N, int64_t K, int64_t w_stride, int dtype,
                        void *stream);

@@ -133,6 +133,9 @@ def ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+MOST_PITCH = 1 << 23  # bytes between the rows of an operand that a matrix product reads as it lies
+
+
 def row_stride(t) -> int:
     """Elements from row to row of a matrix with contiguous channels."""
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
@@ -140,7 +143,8 @@ def row_stride(t) -> int:
 
 def rows_lie_well(*rows) -> bool:
     """Whether matrix products may read these matrices as they lie, which the workspace queries call aligned."""
-    return all(t.data_ptr() % 16 == 0 and row_stride(t) * t.element_size() % 16 == 0 for t in rows)
+    return all(t.data_ptr() % 16 == 0 and row_stride(t) * t.element_size() % 16 == 0
+               and row_stride(t) * t.element_size() <= MOST_PITCH for t in rows)
 
 
 def written(tensors) -> None:

@@ -90,13 +90,11 @@ def _product(name: str, x: Array, q: Weight, backward: bool) -> Array:
         x = x.contiguous()
     y = torch.empty((M, K if backward else N), dtype=x.dtype, device=dev)
     lib, dtype = L.load(), L.DTYPE_CODE[x.dtype]
-    ld = x.stride(0) if M > 1 else x.shape[1]
-    aligned = x.data_ptr() % 16 == 0 and ld * x.element_size() % 16 == 0
-    nws = lib.gdn_mxfp4_linear_workspace_bytes(M, K, N, dtype, aligned, backward)
+    nws = lib.gdn_mxfp4_linear_workspace_bytes(M, K, N, dtype, L.rows_lie_well(x), backward)
     ws = torch.empty((nws,), dtype=torch.uint8, device=dev) if nws else None
     with L.on_device(dev):
-        L.check(getattr(lib, name)(x.data_ptr(), q.codes.data_ptr(), q.scales.data_ptr(), y.data_ptr(), L.ptr(ws), nws, M, K, N, ld,
-                                   dtype, L.stream_handle(dev)))
+        L.check(getattr(lib, name)(x.data_ptr(), q.codes.data_ptr(), q.scales.data_ptr(), y.data_ptr(), L.ptr(ws), nws, M, K, N,
+                                   L.row_stride(x), dtype, L.stream_handle(dev)))
     return y
 
 

@@ -40,3 +40,27 @@ def test_loss(dev, N, H, V, dtype):
             assert all(torch.equal(g, f) for g, f in zip(got[1:], first[1:])) or dtype == torch.float32, (a, b)
             only = linear_cross_entropy(lying(x, a).requires_grad_(True), lying(w, b), t, reduction="none")
             assert torch.equal(only.detach(), got[0])
+
+
+def test_last_tokens_of_long_sequences(dev):
+    """hidden[:, -1]: rows more than 8 MiB apart, with gradients, through a head and a 4-bit weight; and a head of such rows."""
+    import mxfp4
+    from linear_loss import linear_cross_entropy
+    B, T, H, V = 70, 4097, 1024, 300
+    hidden = torch.zeros(B, T, H, dtype=torch.bfloat16, device=dev)
+    x, w, t, d = inputs(dev, B, H, V, torch.bfloat16, 3)
+    hidden[:, -1] = x
+    far = hidden[:, -1].detach().requires_grad_(True)
+    assert far.stride(0) * 2 > 1 << 23
+    near, w = x.requires_grad_(True), w.requires_grad_(True)
+    got, want = (linear_cross_entropy(a, w, t, reduction="none") for a in (far, near))
+    assert torch.equal(got, want)
+    for a, b in zip(torch.autograd.grad(got, [far, w], d), torch.autograd.grad(want, [near, w], d)):
+        assert torch.equal(a, b)
+    q = mxfp4.quantize(w)
+    got, want = mxfp4.linear(far, q), mxfp4.linear(near, q)
+    assert torch.equal(got, want)
+    dy = torch.empty_strided((B, V), (5 << 20, 1), dtype=torch.bfloat16, device=dev).copy_(want)  # cotangents as far apart
+    assert torch.equal(torch.autograd.grad(got, far, dy)[0], torch.autograd.grad(want, near, dy.contiguous())[0])
+    head = torch.empty_strided((V, H), (5 << 20, 1), dtype=torch.bfloat16, device=dev).copy_(w)
+    assert torch.equal(linear_cross_entropy(near, head, t), linear_cross_entropy(near, w, t))

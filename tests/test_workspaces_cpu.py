@@ -1,12 +1,13 @@
 """The workspace that the queries grant is what the calls ask for, whatever the operands' layout (no kernel launches)."""
 
-import ctypes
 import re
 
 import pytest
 import torch
 
 import gdn_lib as L
+
+FAR = 4096 * 2048  # elements: the last hidden states of sequences of 4096 tokens of 2048 channels
 
 
 def rows(n, cols, dtype, stride):
@@ -21,8 +22,8 @@ def needed(call):
 
 
 def layouts(H):
-    """(row stride in elements, the address's offset in bytes): as they should be, off 16 bytes, and odd."""
-    return ((H, 0), (H + 8, 0), (H, 2), (H + 1, 0))
+    """(row stride in elements, the address's offset in bytes): as they should be, off 16 bytes, odd, and far apart."""
+    return ((H, 0), (H + 8, 0), (H, 2), (H + 1, 0), (FAR, 0), (FAR + 4, 0))
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
