@@ -308,7 +308,10 @@ class Model(nn.Module):
         return self.lm_head(self.model(tokens, mask, cache))
 
     def loss(self, tokens: Array, targets: Array, mask: Optional[Array] = None, ignore_index: int = -100) -> Array:
-        """Mean cross entropy of ``targets`` (those that are not ``ignore_index``) without the logits."""
+        """Mean cross entropy of ``targets`` (those that are not ``ignore_index``) without the logits.  The head must be a plain
+        bias-free Linear: adapters on it, hooks and the like have a part in the logits only."""
+        if not _plain_linear(self.lm_head):
+            raise ValueError("the loss without logits takes a plain bias-free Linear head without hooks; got " + str(self.lm_head))
         return linear_cross_entropy(self.model(tokens, mask), self.lm_head.weight, targets, ignore_index=ignore_index)
 
 
@@ -393,6 +396,11 @@ def lora_group(x: Array, mods) -> tuple:
     for m in mods:
         wab += [m.base.weight.to(x.dtype), m.lora_a.to(x.dtype), m.lora_b.to(x.dtype)]
     return _LoRAGroupFn.apply(x, tuple(float(m.scale) for m in mods), *wab)
+
+
+def _plain_linear(m: nn.Module) -> bool:
+    """Whether m is x W^T and nothing else: a bias-free Linear itself that nothing has hooked."""
+    return type(m) is nn.Linear and m.bias is None and not (m._forward_hooks or m._forward_pre_hooks or "forward" in m.__dict__)
 
 
 class LoRALinear(nn.Module):

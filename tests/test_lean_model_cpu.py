@@ -1,0 +1,41 @@
+"""What the loss without logits, the sorted embedding and 4-bit layers do to a model that is not plain: kept or refused, never
+dropped (no kernel launches)."""
+
+import pytest
+import torch
+import torch.nn as nn
+
+import qwen3_5 as Q
+
+
+def model():
+    torch.manual_seed(0)
+    return Q.Model(Q.ModelArgs(hidden_size=32, intermediate_size=64, num_hidden_layers=2, num_attention_heads=2, vocab_size=50,
+                               linear_num_key_heads=1, linear_num_value_heads=2, linear_key_head_dim=64,
+                               linear_value_head_dim=64, full_attention_interval=2))
+
+
+def biased(m):
+    m.lm_head = nn.Linear(32, 50)
+
+
+def adapted(m):
+    m.lm_head = Q.LoRALinear(m.lm_head, 2, 2.0)
+
+
+def hooked(m):
+    m.lm_head.register_forward_hook(lambda mod, args, out: 2 * out)
+
+
+def normed(m):
+    m.lm_head = nn.utils.parametrizations.weight_norm(m.lm_head)
+
+
+@pytest.mark.parametrize("change", [biased, adapted, hooked, normed])
+def test_loss_takes_plain_heads_only(change):
+    """Adapters, a bias, hooks and parametrisations of the head have a part in the logits, which the loss would leave out."""
+    m = model()
+    change(m)
+    ids = torch.zeros(1, 4, dtype=torch.int64)
+    with pytest.raises(ValueError, match="bias-free Linear head"):
+        m.loss(ids, ids)
