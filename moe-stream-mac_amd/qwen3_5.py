@@ -462,8 +462,14 @@ def quantize_frozen(model: Model) -> int:
 
 
 def sorted_embedding(model: Model) -> None:
-    """The model's embedding as ``embedding.Embedding``, with the same parameter."""
+    """The model's embedding, a plain ``nn.Embedding``, as ``embedding.Embedding`` with the same parameter.  Options that this
+    does not have, and hooks, are refused; an ``embedding.Embedding`` stays."""
     old = model.model.embed_tokens
-    new = Embedding(old.num_embeddings, old.embedding_dim, old.padding_idx, device="meta")
+    if isinstance(old, Embedding):
+        return
+    if type(old) is not nn.Embedding or old._forward_hooks or old._forward_pre_hooks or "forward" in old.__dict__:
+        raise ValueError("the embedding must be a plain nn.Embedding without hooks; got " + str(old))
+    new = Embedding(old.num_embeddings, old.embedding_dim, old.padding_idx, max_norm=old.max_norm,
+                    scale_grad_by_freq=old.scale_grad_by_freq, sparse=old.sparse, device="meta")
     new.weight = old.weight
     model.model.embed_tokens = new

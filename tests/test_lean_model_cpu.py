@@ -6,6 +6,7 @@ import torch
 import torch.nn as nn
 
 import qwen3_5 as Q
+from embedding import Embedding
 
 
 def model():
@@ -39,3 +40,24 @@ def test_loss_takes_plain_heads_only(change):
     ids = torch.zeros(1, 4, dtype=torch.int64)
     with pytest.raises(ValueError, match="bias-free Linear head"):
         m.loss(ids, ids)
+
+
+def test_sorted_embedding_drops_nothing():
+    for kw in (dict(max_norm=1.0), dict(sparse=True), dict(scale_grad_by_freq=True)):
+        m = model()
+        m.model.embed_tokens = nn.Embedding(50, 32, **kw)
+        with pytest.raises(ValueError, match="not supported"):
+            Q.sorted_embedding(m)
+    m = model()
+    m.model.embed_tokens.register_forward_hook(lambda mod, args, out: 2 * out)
+    with pytest.raises(ValueError, match="hooks"):
+        Q.sorted_embedding(m)
+    m = model()
+    m.model.embed_tokens = scaled = Embedding(50, 32, scale=3.0)
+    Q.sorted_embedding(m)
+    assert m.model.embed_tokens is scaled
+    m = model()
+    old = m.model.embed_tokens = nn.Embedding(50, 32, padding_idx=-1)
+    Q.sorted_embedding(m)
+    new = m.model.embed_tokens
+    assert type(new) is Embedding and new.weight is old.weight and new.padding_idx == 49
