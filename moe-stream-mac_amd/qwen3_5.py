@@ -438,7 +438,12 @@ def freeze(module: nn.Module) -> None:
 
 def linear_to_lora_layers(model: Model, num_layers: int, rank: int = 2, scale: float = 2.0) -> None:
     """Freeze the model and put LoRA adapters on every Linear of the last ``num_layers`` decoder layers
-    (the convention of mlx_lm.tuner.utils.linear_to_lora_layers used by the reference tests)."""
+    (the convention of mlx_lm.tuner.utils.linear_to_lora_layers used by the reference tests).  Adapters come before
+    ``quantize_frozen``: layers in 4 bits without any are refused."""
+    for layer in list(model.layers)[-num_layers:]:
+        under = {id(m.base) for m in layer.modules() if isinstance(m, LoRALinear)}
+        if any(isinstance(m, mxfp4.MXFP4Linear) and id(m) not in under for m in layer.modules()):
+            raise ValueError("the model's layers are in 4 bits already; put the adapters on first")
     freeze(model)
     for layer in list(model.layers)[-num_layers:]:
         for name, mod in list(layer.named_modules()):
@@ -449,13 +454,13 @@ def linear_to_lora_layers(model: Model, num_layers: int, rank: int = 2, scale: f
 
 def quantize_frozen(model: Model) -> int:
     """The frozen bias-free Linear layers of the decoder layers, under adapters or not, in 4 bits (``mxfp4.MXFP4Linear``): where
-    the reference trains adapters on a 4-bit base.  Returns how many there were.  Layers must be on the GPU; those that train
-    keep their weights."""
+    the reference trains adapters on a 4-bit base.  Returns how many there were.  Layers must be on the GPU; those that train,
+    and those that something has hooked, keep their weights."""
     count = 0
     for layer in model.layers:
         for mod in list(layer.modules()):
             for name, child in list(mod.named_children()):
-                if type(child) is nn.Linear and child.bias is None and not child.weight.requires_grad:
+                if _plain_linear(child) and not child.weight.requires_grad:
                     setattr(mod, name, mxfp4.MXFP4Linear.of(child))
                     count += 1
     return count

@@ -5,6 +5,7 @@ import pytest
 import torch
 import torch.nn as nn
 
+import mxfp4
 import qwen3_5 as Q
 from embedding import Embedding
 
@@ -61,3 +62,18 @@ def test_sorted_embedding_drops_nothing():
     Q.sorted_embedding(m)
     new = m.model.embed_tokens
     assert type(new) is Embedding and new.weight is old.weight and new.padding_idx == 49
+
+
+def test_four_bits_keep_hooked_layers(monkeypatch):
+    q = mxfp4.Weight(torch.zeros(1, 16, dtype=torch.uint8), torch.zeros(1, 1, dtype=torch.uint8), 32)
+    monkeypatch.setattr(mxfp4, "quantize", lambda w: q)
+    m = model()
+    Q.linear_to_lora_layers(m, 1)
+    hooked = m.layers[0].gate_up
+    hooked.register_forward_hook(lambda mod, args, out: 2 * out)
+    count = Q.quantize_frozen(m)
+    assert count > 5 and m.layers[0].gate_up is hooked and isinstance(m.layers[0].down, mxfp4.MXFP4Linear)
+    assert isinstance(m.layers[1].down.base, mxfp4.MXFP4Linear)
+    Q.linear_to_lora_layers(m, 1)  # layers in 4 bits that have their adapters stay
+    with pytest.raises(ValueError, match="adapters on first"):
+        Q.linear_to_lora_layers(m, 2)
