@@ -89,4 +89,4 @@ class Embedding(torch.nn.Embedding):
         if self.weight.device.type == "cuda":
             return embedding(ids, self.weight, scale=self.scale, padding_idx=self.padding_idx)
         y = super().forward(ids)
-        return y if self.scale == 1.0 else (y.float() * self.scale).to(y.dtype)
+        return y if self.scale == 1.0 else (y.double() * self.scale).to(y.dtype)

@@ -77,3 +77,12 @@ def test_four_bits_keep_hooked_layers(monkeypatch):
     Q.linear_to_lora_layers(m, 1)  # layers in 4 bits that have their adapters stay
     with pytest.raises(ValueError, match="adapters on first"):
         Q.linear_to_lora_layers(m, 2)
+
+
+def test_scaled_rows_on_the_cpu_keep_their_bits():
+    """The factor meets the rows in 64 bits, as on the GPU."""
+    e = Embedding(7, 5, scale=3 ** 0.5, dtype=torch.float64)
+    ids = torch.arange(7)
+    assert torch.equal(e(ids), e.weight * 3 ** 0.5)
+    f = Embedding(7, 5, scale=3 ** 0.5)
+    assert torch.equal(f(ids), (f.weight.double() * 3 ** 0.5).float())
