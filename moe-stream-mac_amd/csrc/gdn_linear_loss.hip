@@ -55,6 +55,9 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int NT = 256;
 constexpr int64_t COMPACT = 2048;
 constexpr int64_t ROWS = 128;
+// dx of fewer tokens is formed in up to 32 parts of the words, of others in 16: bf16 with dx, 32000 words of 256 channels, 64
+// tokens 65 us and 75, 256 85 and 98, 511 104 and 114; fp32, 513 tokens, 50001 words of 1001 channels, both gradients, 1224 and 1075.
+constexpr int64_t FEW_TOKENS = 512;
 constexpr int64_t KEPT = 1 << 26;  // differences of a piece, if that is 256 words or more; statistics of the parts of the words
 constexpr int64_t MOST_TOKENS = 1 << 20;  // three slots of 16 bits for each are a row pitch that a product takes
 constexpr int WIDE = 128;          // up to here fp32 numbers are three bf16 terms, and a forward call reads the words as they lie
@@ -185,10 +188,10 @@ __global__ __launch_bounds__(S::NT, S::WAVES_EU) void stat_kernel(const Args g, 
 
 // Few tokens and fp32 words, forward: read once, as they lie, and split in registers into three bf16 terms, which hold them exactly
 // and at any magnitude, so that they need no scale.  Six products of terms; those left out are below 2^-21 of the factors.  The
-// tokens' terms, 16 TN rows of three slots, go through LDS, two stages of 64 along the contraction; a wave's 32 words stay its own
-// and go to registers, a stage ahead.  64765 x 4096 weights (1.06 GB, 208 us at a copy's rate): 32 tokens 229 us, 118 tokens 489 us,
-// where the conversions and one wave to a SIMD hold it back; by way of two fp16 terms 878 and 920.  128 tokens, 32000 x 2048: 124
-// and 267.
+// tokens' terms, 16 TN rows of three slots, go through LDS, two stages of 64 along the contraction; a wave's 32 words stay its
+// own and go to registers, a stage ahead.  64765 x 4096 weights (1.06 GB, 208 us at a copy's rate): 32 tokens 229 to 255 us, 118
+// tokens 444 to 489, where the conversions and one wave to a SIMD hold it back; through a copy of the words in terms, as weights
+// off 16 bytes take it, 1109 and 1199.  128 tokens, 32000 x 2048: 123 and 363; 129 tokens, by two fp16 terms, 277.
 template <int TN>
 struct Wide {
     static constexpr int NT = 256, BM = 128, BN = 16 * TN, TM = 2, SLOT = BN * BK * 2, STAGE = 3 * SLOT;
@@ -577,7 +580,7 @@ static Sizes sizes(int64_t N, int64_t H, int64_t V, int dt, bool dx) {
     if (s.tokens < 256) s.tokens = 256;
     if (s.tokens > N) s.tokens = N;
     const int64_t words = s.piece < V ? s.piece : V;
-    s.px = plan(s.prows, H, (s.rows ? 1 : s.pairs) * padded(words) / BK, 32);
+    s.px = plan(s.prows, H, (s.rows ? 1 : s.pairs) * padded(words) / BK, N < FEW_TOKENS ? 32 : 16);
     s.pw = plan(words, H, s.pairs * s.np / BK, 8, true);
     return s;
 }
