@@ -64,3 +64,19 @@ def test_last_tokens_of_long_sequences(dev):
     assert torch.equal(torch.autograd.grad(got, far, dy)[0], torch.autograd.grad(want, near, dy.contiguous())[0])
     head = torch.empty_strided((V, H), (5 << 20, 1), dtype=torch.bfloat16, device=dev).copy_(w)
     assert torch.equal(linear_cross_entropy(near, head, t), linear_cross_entropy(near, w, t))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(2, 3, 5, 64), (2, 1, 15, 128), (3, 4, 45, 96)])
+def test_linear_of_more_dimensions(dev, shape, dtype):
+    """An input of four dimensions, dense or a view, has the bits of its rows, up to 64 of them and more."""
+    import mxfp4
+    g = torch.Generator(device=dev)
+    g.manual_seed(shape[2])
+    q = mxfp4.quantize(torch.randn(77, shape[-1], device=dev, generator=g))
+    x = torch.randn(shape, device=dev, generator=g).to(dtype)
+    rows = mxfp4.linear(x.reshape(-1, shape[-1]), q)
+    assert torch.equal(mxfp4.linear(x, q).reshape(rows.shape), rows)
+    assert torch.equal(mxfp4.linear(x.transpose(0, 2).contiguous().transpose(0, 2), q).reshape(rows.shape), rows)
+    assert torch.equal(mxfp4.linear(lying(x.reshape(-1, shape[-1]), "off"), q), rows)
+    assert torch.equal(mxfp4.linear(lying(x.reshape(-1, shape[-1]), "odd"), q), rows)
