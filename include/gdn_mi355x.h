@@ -379,8 +379,9 @@ int gdn_linear_loss_bwd(const void *x, const void *w, const int64_t *targets, co
 
 /* Rows of a table: y [N][H] = scale * w[ids[n]] (dtype; w_stride elements from row to row, channels contiguous); rows of NaN
  * where an id lies outside [0, V).  Backward: dw [V][H] (contiguous, every row written) = scale times the sum of dy [N][H]
- * (dtype, dy_stride elements from row to row) over the tokens of each word, in their order, in 64 bits; without the tokens
- * equal to padding_idx (-1 for none) and those outside the table.  N <= 2^26, V < 2^22, H <= 2^20. */
+ * (dtype, dy_stride elements from row to row) over the tokens of each word, 32 at a time in their order, in 64 bits, rounded
+ * to 32 bits and dtype; without the tokens equal to padding_idx (-1 for none) and those outside the table.  N <= 2^26, V < 2^22,
+ * H <= 2^20. */
 int gdn_embedding_fwd(const int64_t *ids, const void *w, void *y, int64_t N, int64_t V, int64_t H, int64_t w_stride,
                       double scale, int dtype, void *stream);
 size_t gdn_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t H);

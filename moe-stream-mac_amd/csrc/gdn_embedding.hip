@@ -1,6 +1,6 @@
 // Rows of an embedding table, scaled, and the table's gradient by sorted tokens, for gfx950.
 //
-//   y_n = a W[id_n],     dW[v] = a sum_{n: id_n = v} dy_n   (64-bit sums in the order of n, rounded once)
+//   y_n = a W[id_n],     dW[v] = a sum_{n: id_n = v} dy_n   (64-bit sums, rounded to 32 bits and their type)
 //
 // Both stream: the forward reads and writes a row for each token; the backward reads a row of dy for each token and writes
 // every row of dW, zeros where no token points.  Without an order of arrival that could matter: no atomics.

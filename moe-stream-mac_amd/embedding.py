@@ -51,9 +51,10 @@ class _Embedding(torch.autograd.Function):
 def embedding(ids: Array, weight: Array, *, scale: float = 1.0, padding_idx: Optional[int] = None) -> Array:
     """``scale * weight[ids]`` for ``ids`` [...] (int64 or int32) and ``weight`` [V, H]: [..., H] of the weight's type.
 
-    Differentiable in ``weight``: its gradient is summed in 64 bits in the order of the tokens and rounded once, the same bits
-    every time.  Tokens equal to ``padding_idx`` have no gradient.  An id outside [0, V) gives a row of NaN, without a
-    gradient.  ``weight`` may be a view with contiguous rows."""
+    Differentiable in ``weight``: its gradient is summed in 64 bits, 32 tokens of a word at a time in their order, and rounded
+    to 32 bits and its type, the same bits every time.  The backward pass takes half a byte of workspace for each element of the
+    output and 16 bytes for each token.  Tokens equal to ``padding_idx`` have no gradient.  An id outside [0, V) gives a row of
+    NaN, without a gradient.  ``weight`` may be a view with contiguous rows."""
     if weight.dim() != 2 or weight.numel() == 0:
         raise ValueError(f"weight must be [V, H] and not empty; got {tuple(weight.shape)}")
     if weight.dtype not in L.DTYPE_CODE:

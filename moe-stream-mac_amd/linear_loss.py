@@ -83,9 +83,14 @@ def linear_cross_entropy(x: Array, weight: Array, targets: Array, *, ignore_inde
     there; a target outside [0, V) makes the token's loss NaN, and the gradients that it enters.  Differentiable in ``x`` and
     ``weight``; a frozen weight costs no gradient of its own.  ``x`` and ``weight`` may be views with contiguous channels.
 
-    Tokens that do not count cost no time where there are many (2048 and more in all).  Memory beside the gradients: 8 bytes for
-    each token and 64 words and a copy of ``x`` forward; backward up to 2^26 probabilities, 32 bits each, the piece of the weight
-    that they belong to, and two copies of ``x`` with its gradient's sums.
+    Tokens that do not count cost no time where there are many (2048 and more in all).  At most 2^20 tokens.
+
+    Memory beside the gradients.  Words come in pieces of 2^26 probabilities over all tokens, or of 256 words if that is more.
+    Forward: 8 bytes for each token and 64 words, up to 512 MB, and copies of what the matrix products cannot read as it lies:
+    ``x`` from 2048 tokens on, and of float32, odd sizes and rows off 16 bytes or more than 8 MiB apart ``x`` and a piece of
+    ``weight``, 2 bytes an element (float32 4, or 6 up to 128 tokens).  Backward: these copies (float32 6 bytes), a piece's
+    probabilities at 4 bytes each (up to 128 float32 tokens 6); for ``x``'s gradient float32 sums of its size, of few tokens
+    in up to 32 parts; for ``weight``'s another copy of ``x`` and, of few words, float32 sums of a piece in up to 8 parts.
 
     bfloat16 and float16 inputs enter with all their bits, and gradients are as good as 32-bit sums rounded once.  float32
     inputs are sums of 16-bit terms, which hold no infinities: those may count as NaN.  Up to 128 tokens the terms are exact.
