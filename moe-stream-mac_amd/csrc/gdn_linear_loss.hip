@@ -37,9 +37,10 @@
 // lies along the channels, is read once.  2048 x 32000 bf16, forward and dx: 8 tokens 109 us so, 118 with terms side by side; 64
 // 115 and 123; 100 145 and 158; 256 180 and 174; 511 273 and 267.
 //
-// Measured, bf16, 8192 tokens of which a fifth does not count, 2048 x 32000, both gradients: 686 us for the statistics (1.25
-// PFLOP/s), then four pieces with 247 for the differences, 381 for dx and 323 for dW (1.15 and 1.36 PFLOP/s over both terms).
-// Results and exponentials of a tile do not run beside another's products, which is what is lost most.
+// Measured, bf16, 8192 tokens of which a fifth does not count, 2048 x 32000, both gradients: 634 us for the statistics (1.35
+// PFLOP/s), then four pieces with 241 for the differences, 349 for dx and 300 for dW (1.26 and 1.47 PFLOP/s over both terms); on
+// another card 686, 247, 381 and 323.  The matrix units are busy 66, 42, 55 and 70 % of the time.  Results and exponentials of a
+// tile do not run beside another's products, which is what is lost most.
 #include "gdn_common.h"
 #include "gdn_host.h"
 #include "gdn_product.h"
