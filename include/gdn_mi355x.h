@@ -362,7 +362,8 @@ int gdn_clip_grad_norm(const void *const *x, void *const *y, const int64_t *nume
  *   factor [1]    what takes the cotangent of that to a token's.  reduction 0: neither is written, both may be NULL
  * fp32 outputs.  What x holds at ignored tokens does not reach any other token, nor w's gradient.  fp32 inputs are sums of 16-bit
  * terms: infinities among them may count as NaN.  Up to 128 tokens the terms are exact; with more they leave out 2^-22 of a number,
- * or 2^-39 of the largest of its token (x, in the loss and dx), of w, or of x (in dw), whichever is more.
+ * or 2^-39 of the largest of its token (x, in the loss and dx), of w, or of x (in dw), whichever is more, and of a probability
+ * 2^-22 or 2^-51 (fp16: 2^-22 or 2^-40; bf16: 2^-16).
  *
  * gdn_linear_loss_bwd: dx [N][H] and dw [V][H], contiguous (dtype; either may be NULL), from the cotangents dloss (fp32;
  * dloss_stride 1: one for each token, 0: one for all), times factor [0] (NULL for 1); dx is 0 at ignored tokens.

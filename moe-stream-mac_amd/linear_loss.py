@@ -92,10 +92,11 @@ def linear_cross_entropy(x: Array, weight: Array, targets: Array, *, ignore_inde
     probabilities at 4 bytes each (up to 128 float32 tokens 6); for ``x``'s gradient float32 sums of its size, of few tokens
     in up to 32 parts; for ``weight``'s another copy of ``x`` and, of few words, float32 sums of a piece in up to 8 parts.
 
-    bfloat16 and float16 inputs enter with all their bits, and gradients are as good as 32-bit sums rounded once.  float32
+    bfloat16 and float16 inputs enter with all their bits, and gradients are as good as 32-bit sums rounded once (float16, whose
+    gradients end at 2^-25, as long as cotangents times ``x`` stay below 2^15: probabilities are kept to 2^-40).  float32
     inputs are sums of 16-bit terms, which hold no infinities: those may count as NaN.  Up to 128 tokens the terms are exact.
-    More have 2^-22 of a number, or 2^-39 of the largest of its token (``x``, in the loss and its own gradient), of ``weight``,
-    or of ``x`` (in ``weight``'s gradient), whichever is more."""
+    With more they leave out 2^-22 of a number, or 2^-39 of the largest of its token (``x``, in the loss and its own gradient), of
+    ``weight``, or of ``x`` (in ``weight``'s gradient), whichever is more, and gradients 2^-22 of a probability or 2^-51."""
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"x must be [..., H] and weight [V, H]; got {tuple(x.shape)} and {tuple(weight.shape)}")
     if tuple(targets.shape) != tuple(x.shape[:-1]):
