@@ -666,13 +666,20 @@ static void launch_stat(Args &g, const StatArgs &a, const Sizes &s, hipStream_t 
     else if (s.f16) hipLaunchKernelGGL((stat_kernel<S, true, false>), grid, block, 0, st, g, a);
     else hipLaunchKernelGGL((stat_kernel<S, false, false>), grid, block, 0, st, g, a);
 }
+// Scaled operands come with more than 128 tokens, three terms with no more: plan() never gives those the narrow tiles, nor these the
+// large one (128 tokens need no fewer rounds of it).
 template <class S>
 static void launch_diff(Args &g, const DiffArgs &a, const Sizes &s, hipStream_t st) {
     const dim3 grid = tiles_of<S>(g, 1), block(S::NT);
-    if (s.scaled) hipLaunchKernelGGL((diff_kernel<S, true, true, 2>), grid, block, 0, st, g, a);
-    else if (s.f16) hipLaunchKernelGGL((diff_kernel<S, true, false, 2>), grid, block, 0, st, g, a);
-    else if (s.terms == 1) hipLaunchKernelGGL((diff_kernel<S, false, false, 2>), grid, block, 0, st, g, a);
-    else hipLaunchKernelGGL((diff_kernel<S, false, false, 3>), grid, block, 0, st, g, a);
+    if constexpr (S::BN >= 128) {
+        if (s.scaled) hipLaunchKernelGGL((diff_kernel<S, true, true, 2>), grid, block, 0, st, g, a);
+    }
+    if constexpr (S::BN <= 128) {
+        if (s.terms == 3) hipLaunchKernelGGL((diff_kernel<S, false, false, 3>), grid, block, 0, st, g, a);
+    }
+    if (s.terms > 1) return;
+    if (s.f16) hipLaunchKernelGGL((diff_kernel<S, true, false, 2>), grid, block, 0, st, g, a);
+    else hipLaunchKernelGGL((diff_kernel<S, false, false, 2>), grid, block, 0, st, g, a);
 }
 
 #define GDN_BY_SHAPE(shape, call)              \
